@@ -254,7 +254,7 @@ def _run_shared(s):
     case = s["case"]
     if own:
         from nnis_b200.csrc import ops
-        ops.attention_shared(s["q"], s["q"].shape[1], s["k"], s["v"], s["pos"], s["seq"], s["table"], s["plan"], s["out"],
+        ops.attention_shared(s["q"], s["q"].shape[1], s["k"], s["v"], s["pos"], s["table"], s["plan"], s["out"],
                              case["heads"], case["kv_heads"], case["dim"], s["scale"], s["workspace"])
         return s["out"]
     heads, kv, d, tokens = case["heads"], case["kv_heads"], case["dim"], case["tokens"]
