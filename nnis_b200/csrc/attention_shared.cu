@@ -1,0 +1,245 @@
+// Attention of token rows that share pages of the cache, any even head size up to 256, float32 or bfloat16, on the CUDA
+// cores; and the merge that all forms end with.  See attention_shared.cuh for units and records.
+//
+// A CTA owns a unit and a kv head: a tile of 16 or 64 entries (token row, query head) over the unit's pages.  A page of K
+// comes into shared memory as float32, scores of tile x 64 keys are sums in registers (a thread: 1 or 4 entries x 4 keys),
+// the softmax's running maximum and sum are a half-warp's shuffles, the weights go to shared memory and the outputs, a
+// thread's 1 or 4 entries x d / 16 values, are added up in registers while the page's V replaces its K.
+#include "attention_shared.cuh"
+
+namespace nnis {
+
+constexpr int kAnyThreads = 256;
+
+__device__ __forceinline__ int row_stride_any(int d) { return ((d + 3) & ~3) + 4; }
+
+// ROWS: entries a thread (tile = 16 ROWS); NJ: runs of 16 output values
+template <typename T, int ROWS, int NJ>
+__global__ void __launch_bounds__(kAnyThreads)
+attn_shared_any_kernel(const SharedArgs a) {
+    constexpr int kTile = 16 * ROWS;
+    extern __shared__ __align__(16) float smem_any[];
+    const int d = a.d, ds = row_stride_any(d);
+    float* q_s = smem_any;                      // [tile, ds], scaled
+    float* kv_s = q_s + kTile * ds;             // [64, ds]: a page's K, then its V
+    float* p_s = kv_s + kSharedPage * ds;       // [tile, 68]
+    const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+    const SharedUnit u = a.units[blockIdx.x];
+    pdl_wait();  // (the queries, and this step's keys and values, come from the kernel before)
+    pdl_launch_dependents();
+    if (u.entries <= 0) return;  // (before any barrier: the whole CTA)
+    const int hk = blockIdx.y, G = a.nq / a.nkv;
+    const int* members = a.members + u.members;
+    const int pos = u.ends ? a.token_pos[members[u.entry / G]] : 0x7fffffff;
+    const int n_pages = u.ends ? min(u.page_end, pos < 0 ? 0 : pos / kSharedPage + 1) : u.page_end;
+    const int* table = a.page_table + (size_t)u.seq * a.table_cols;
+    const T* q = static_cast<const T*>(a.q);
+
+    for (int i = tid; i < kTile * ds; i += kAnyThreads) {
+        const int e = i / ds, c = i % ds;
+        float x = 0.f;
+        if (e < u.entries && c < d) {
+            const int at = u.entry + e;
+            x = to_float(q[(size_t)members[at / G] * a.q_stride + (size_t)(hk * G + at % G) * d + c]) * (a.scale * 1.4426950408889634f);
+        }
+        q_s[i] = x;
+    }
+    float o[ROWS][NJ], m_run[ROWS], l_run[ROWS];
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+        m_run[r] = -INFINITY;
+        l_run[r] = 0.f;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) o[r][j] = 0.f;
+    }
+    auto load = [&](const void* cache, int page, int keys) {  // rows from `keys` on are zero: what lies there may be anything
+        const T* src = static_cast<const T*>(cache) + ((size_t)page * a.nkv + hk) * kSharedPage * d;
+        const int half = d / 2, hs = ds / 2;
+        for (int i = tid; i < kSharedPage * hs; i += kAnyThreads) {
+            const int row = i / hs, c = i % hs;
+            float2 x = make_float2(0.f, 0.f);
+            if (row < keys && c < half) x = load2(src + (size_t)row * d + 2 * c);
+            *reinterpret_cast<float2*>(kv_s + (size_t)row * ds + 2 * c) = x;
+        }
+    };
+    for (int it = u.page_begin; it < n_pages; ++it) {
+        const int page = table[it];
+        if (page < 0 || page >= a.pages) continue;  // (the table's gaps hold no keys)
+        const int keys = min(kSharedPage, u.ends ? pos + 1 - it * kSharedPage : kSharedPage);
+        __syncthreads();
+        load(a.k_cache, page, keys);
+        __syncthreads();
+        float s[ROWS][4];
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[r][i] = 0.f;
+        for (int c = 0; c < d; c += 4) {
+            float4 kk[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) kk[i] = *reinterpret_cast<const float4*>(kv_s + (size_t)(tx + 16 * i) * ds + c);
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) {
+                const float4 qq = *reinterpret_cast<const float4*>(q_s + (size_t)(ty * ROWS + r) * ds + c);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    s[r][i] = fmaf(qq.x, kk[i].x, s[r][i]);
+                    s[r][i] = fmaf(qq.y, kk[i].y, s[r][i]);
+                    s[r][i] = fmaf(qq.z, kk[i].z, s[r][i]);
+                    s[r][i] = fmaf(qq.w, kk[i].w, s[r][i]);
+                }
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+            float mx = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (tx + 16 * i >= keys) s[r][i] = -INFINITY;
+                mx = fmaxf(mx, s[r][i]);
+            }
+#pragma unroll
+            for (int w = 8; w > 0; w >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
+            const float m_new = fmaxf(m_run[r], mx), base = m_new == -INFINITY ? 0.f : m_new;
+            const float alpha = exp2f(m_run[r] - base);
+            m_run[r] = m_new;
+            float sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float p = exp2f(s[r][i] - base);
+                sum += p;
+                p_s[(ty * ROWS + r) * 68 + tx + 16 * i] = p;
+            }
+            l_run[r] = l_run[r] * alpha + half_warp_sum(sum);
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) o[r][j] *= alpha;
+        }
+        __syncthreads();
+        load(a.v_cache, page, keys);
+        __syncthreads();
+#pragma unroll 4
+        for (int t = 0; t < kSharedPage; ++t) {
+            float p[ROWS];
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) p[r] = p_s[(ty * ROWS + r) * 68 + t];
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                const float v = kv_s[(size_t)t * ds + min(tx + 16 * j, ds - 1)];
+#pragma unroll
+                for (int r = 0; r < ROWS; ++r) o[r][j] = fmaf(p[r], v, o[r][j]);
+            }
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+        const int e = ty * ROWS + r;
+        if (e >= u.entries) continue;
+        const int at = u.entry + e, row = members[at / G];
+        float* rec = a.partial + ((size_t)(a.record[row] + u.slot) * a.nq + hk * G + at % G) * (size_t)(d + 2);
+        if (tx == 0) {
+            rec[0] = m_run[r];
+            rec[1] = l_run[r];
+        }
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+            if (tx + 16 * j < d) rec[2 + tx + 16 * j] = o[r][j];
+    }
+}
+
+// A warp per (token row, head): lane s holds the weights of records s, s + 32, ...; every lane sums its values over the
+// records in their order.  A row without records (a padding row), or none of whose records holds a key, is zero.
+template <typename T>
+__global__ void __launch_bounds__(128)
+attn_shared_merge_kernel(const float* __restrict__ partial, const int* __restrict__ record, T* __restrict__ out, int n_tokens,
+                         int nq, int d) {
+    pdl_wait();
+    pdl_launch_dependents();
+    const int lane = threadIdx.x & 31;
+    const size_t at = (size_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+    if (at >= (size_t)n_tokens * nq) return;
+    const int row = (int)(at / nq), head = (int)(at % nq);
+    const int first = record[row], count = record[row + 1] - first;
+    const float* rec = partial + ((size_t)first * nq + head) * (size_t)(d + 2);
+    const size_t step = (size_t)nq * (d + 2);
+    float m = -INFINITY;
+    for (int s = lane; s < count; s += 32)
+        if (rec[s * step + 1] != 0.f) m = fmaxf(m, rec[s * step]);
+    m = warp_max(m);
+    float acc[8] = {}, l = 0.f;
+    for (int s0 = 0; s0 < count; s0 += 32) {
+        float w = 0.f;
+        if (s0 + lane < count) {
+            const float held = rec[(s0 + lane) * step + 1];
+            w = held != 0.f ? exp2f(rec[(s0 + lane) * step] - m) : 0.f;
+            l += held * w;
+        }
+        const int here = min(32, count - s0);
+        for (int s = 0; s < here; ++s) {
+            const float f = __shfl_sync(0xffffffffu, w, s);
+            if (f == 0.f) continue;  // (a record that holds nothing is never added)
+            const float* r = rec + (s0 + s) * step + 2;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (lane + 32 * j < d) acc[j] = fmaf(f, r[lane + 32 * j], acc[j]);
+        }
+    }
+    l = warp_sum(l);
+    const float inv = l != 0.f ? 1.0f / l : 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+        if (lane + 32 * j < d) out[at * d + lane + 32 * j] = from_float<T>(acc[j] * inv);
+}
+
+template <typename T, int ROWS, int NJ>
+static cudaError_t launch_any(const SharedArgs& a, int n_units, cudaStream_t stream) {
+    const int ds = ((a.d + 3) & ~3) + 4, tile = 16 * ROWS;
+    const size_t smem = ((size_t)(tile + kSharedPage) * ds + (size_t)tile * 68) * sizeof(float);
+    auto kernel = attn_shared_any_kernel<T, ROWS, NJ>;
+    if (smem > 48 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e != cudaSuccess) return e;
+    }
+    return launch_dependent(kernel, dim3(n_units, a.nkv), kAnyThreads, smem, stream, a);
+}
+
+template <typename T, int ROWS>
+static cudaError_t launch_any_size(const SharedArgs& a, int n_units, cudaStream_t stream) {
+    return a.d <= 64 ? launch_any<T, ROWS, 4>(a, n_units, stream) : a.d <= 128 ? launch_any<T, ROWS, 8>(a, n_units, stream)
+                                                                  : launch_any<T, ROWS, 16>(a, n_units, stream);
+}
+
+cudaError_t shared_units_any(const SharedArgs& a, int n_units, int tile, bool f32, cudaStream_t stream) {
+    if (f32) return tile == 16 ? launch_any_size<float, 1>(a, n_units, stream) : launch_any_size<float, 4>(a, n_units, stream);
+    return tile == 16 ? launch_any_size<bf16, 1>(a, n_units, stream) : launch_any_size<bf16, 4>(a, n_units, stream);
+}
+
+}  // namespace nnis
+
+// units: n_small units of at most 16 entries, then n_large of at most 64.  The plan (units, members, record) is the host's,
+// made of tables that the call's page table agrees with; page ids outside the store hold no keys.
+NNIS_API int nnis_attention_shared(const void* q, int q_stride, const void* k_cache, const void* v_cache, const int* token_pos,
+                                   const int* page_table, int table_cols, const int* units, int n_small, int n_large,
+                                   const int* members, const int* record, float* partial, void* out, int n_tokens, int nq, int nkv,
+                                   int d, int pages, int page_size, float scale, int dtype, cudaStream_t stream) {
+    using namespace nnis;
+    if (n_tokens <= 0 || nq <= 0 || nkv <= 0 || nq % nkv || table_cols <= 0 || n_small < 0 || n_large < 0 || pages <= 0 || !record || !partial ||
+        (n_small + n_large > 0 && (!units || !members)))
+        return NNIS_ERR_ARGUMENT;
+    if (page_size != kSharedPage || d < 2 || d > 256 || d % 2 || nkv > 65535) return NNIS_ERR_UNSUPPORTED;
+    if ((uintptr_t)units % 16 || (uintptr_t)partial % 8) return NNIS_ERR_ALIGNMENT;
+    if (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache) % (dtype == NNIS_DTYPE_F32 ? 8 : 4)) return NNIS_ERR_ALIGNMENT;
+    SharedArgs a = {q, k_cache, v_cache, token_pos, page_table, reinterpret_cast<const SharedUnit*>(units), members, record, partial,
+                    q_stride, table_cols, pages, nq, nkv, d, scale};
+    const bool f32 = dtype == NNIS_DTYPE_F32;
+    for (int large = 0; large < 2; ++large) {
+        const int n = large ? n_large : n_small;
+        if (!n) continue;
+        if (large) a.units += n_small;
+        const cudaError_t e = shared_units_any(a, n, large ? 64 : 16, f32, stream);
+        if (e != cudaSuccess) return (int)e;
+    }
+    const unsigned ctas = (unsigned)(((size_t)n_tokens * nq + 3) / 4);
+    const cudaError_t e = f32 ? launch_dependent(attn_shared_merge_kernel<float>, ctas, 128, 0, stream, partial, record, (float*)out, n_tokens, nq, d)
+                              : launch_dependent(attn_shared_merge_kernel<bf16>, ctas, 128, 0, stream, partial, record, (bf16*)out, n_tokens, nq, d);
+    return e == cudaSuccess ? NNIS_OK : (int)e;
+}

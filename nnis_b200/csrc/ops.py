@@ -141,6 +141,42 @@ class Pieces:
         self._run((ctypes.c_void_p * max(len(kept), 1))(*(t.data_ptr() for t in kept)), self.ptrs)
 
 
+def copy_pages(k: torch.Tensor, v: Optional[torch.Tensor], moves) -> None:
+    """Pages copied inside the store for all layers at once: for every (source page, target page, rows) of ``moves`` the
+    first ``rows`` positions of the target become the source's.  k: [layers, pages, kv_heads, page_size, dim], v the same with
+    its own dim, or None.  A page that is a target is the target of one move and the source of none."""
+    _cuda(k, v)
+    _need(k.dim() == 5 and k.numel() > 0, "copy_pages: k [layers, pages, kv_heads, page_size, dim]")
+    layers, pages, heads, page_size, dim = k.shape
+    size = k.element_size()
+    _need(v is None or (v.dim() == 5 and v.shape[:4] == k.shape[:4] and v.device == k.device and v.numel() > 0),
+          "copy_pages: v [layers, pages, kv_heads, page_size, value dim] beside k")
+    v_row = 0 if v is None else v.shape[4] * v.element_size()
+    _need(dim * size % 4 == 0 and v_row % 4 == 0, "copy_pages: rows of a multiple of four bytes")
+    _need(layers <= 65535, "copy_pages: at most 65,535 layers")
+    _need(heads * page_size * max(dim * size, v_row) < 2 ** 32, "copy_pages: pages below 4 GB")
+    flat = []
+    sources, targets = set(), set()
+    for src, dst, rows in moves:
+        _need(0 <= src < pages and 0 <= dst < pages, f"copy_pages: page {src} or {dst} is outside the store's {pages}")
+        _need(0 <= rows <= page_size, f"copy_pages: {rows} rows of a page of {page_size}")
+        _need(dst not in targets, f"copy_pages: page {dst} is the target of two moves")
+        targets.add(dst)
+        sources.add(src)
+        if rows:
+            flat += (src, dst, rows)
+    _need(sources.isdisjoint(targets), "copy_pages: a page is a source and a target")
+    if not flat:
+        return
+    if torch.cuda.current_device() != k.device.index:
+        with torch.cuda.device(k.device):
+            return copy_pages(k, v, moves)
+    count = len(flat) // 3
+    _check(_lib().nnis_copy_pages(_ptr(k), _ptr(v), layers, pages, heads, page_size, dim * size, v_row,
+                                  (ctypes.c_int * len(flat))(*flat), count, sm_count(k.device), _stream()), "copy_pages",
+           -(-count // 1024))
+
+
 def list_to_ints(values: list, limit: int):
     """A list of whole numbers from 0 to below ``limit`` as an int32 array; None where it holds anything else (the
     caller then looks at it number by number)."""
@@ -317,6 +353,42 @@ def sample_temperature(logits: torch.Tensor, temperature: torch.Tensor, rng_stat
     _need(rng_state.dtype == torch.int64 and rng_state.numel() >= n, "rng_state: int64 [n]")
     _check(_lib().nnis_sample_temperature(_ptr(logits), _ptr(temperature), _ptr(rng_state),
                                           _ptr(out), n, vocab, _stream()), "sample_temperature")
+
+
+def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, first_row: torch.Tensor, temperatures: torch.Tensor,
+                  accept_draws: torch.Tensor, pick_draws: torch.Tensor, accepted: torch.Tensor, picked: torch.Tensor,
+                  draft_logits: Optional[torch.Tensor], workspace) -> None:
+    """See ``sampling.device.verify_drafts``."""
+    _cuda(logits, drafts, first_row, temperatures, accept_draws, pick_draws, accepted, picked, draft_logits)
+    _need(logits.dim() == 2 and logits.dtype == torch.float32 and logits.numel() > 0, "verify: logits float32 [rows, vocab]")
+    rows, vocab = logits.shape
+    b = first_row.numel() - 1
+    _need(1 <= b <= rows, f"verify: first_row holds one number more than there are sequences; got {b + 1} for {rows} rows")
+    _need(rows <= 32767 and vocab <= 1 << 30, "verify: at most 32,767 rows")
+    drafted = rows - b
+    for t, name in ((drafts, "drafts"), (first_row, "first_row"), (accepted, "accepted"), (picked, "picked")):
+        _need(t.dtype == torch.int32, f"verify: {name} int32")
+    _need(drafts.numel() == drafted, f"verify: {drafted} drafts ({rows} rows of {b} sequences); got {drafts.numel()}")
+    _need(accept_draws.dtype == torch.float64 and accept_draws.numel() == drafted, "verify: accept_draws float64, one a draft")
+    _need(pick_draws.dtype == torch.float64 and pick_draws.numel() == b, "verify: pick_draws float64, one a sequence")
+    _need(temperatures.dtype == torch.float32 and temperatures.numel() == b, "verify: temperatures float32, one a sequence")
+    _need(accepted.numel() == b and picked.numel() == b, "verify: accepted and picked, one a sequence")
+    for t in (drafts, first_row, temperatures, accept_draws, pick_draws, accepted, picked, draft_logits):
+        _need(t is None or t.device == logits.device, "verify: tensors of one device")
+    if draft_logits is not None:
+        _need(draft_logits.dtype == torch.float32 and tuple(draft_logits.shape) == (drafted, vocab),
+              f"verify: draft_logits float32 [{drafted}, {vocab}]")
+        if not drafted:
+            draft_logits = None
+    if torch.cuda.current_device() != logits.device.index:
+        with torch.cuda.device(logits.device):
+            return verify_drafts(logits, drafts, first_row, temperatures, accept_draws, pick_draws, accepted, picked,
+                                 draft_logits, workspace)
+    need = int(_lib().nnis_verify_scratch(rows, drafted, vocab))
+    scratch = workspace.get("verify_sums", (need // 4,), torch.float32)
+    _check(_lib().nnis_verify_drafts(_ptr(logits), _ptr(draft_logits), _ptr(drafts), _ptr(first_row), _ptr(temperatures),
+                                     _ptr(accept_draws), _ptr(pick_draws), _ptr(scratch), b, rows, vocab, _ptr(accepted),
+                                     _ptr(picked), _stream()), "verify_drafts", 2)
 
 
 EPI_STORE, EPI_STORE_F32, EPI_ADD_F32, EPI_GATED, EPI_QKV, EPI_ARGMAX = 0, 1, 2, 3, 4, 5
@@ -2712,3 +2784,83 @@ def memory_finish(o_raw: torch.Tensor, a: torch.Tensor, gate_off: int, weight: t
     _check(_lib().nnis_memory_finish(_ptr(o_raw), _ptr(a), a.shape[1], gate_off, _ptr(weight), _ptr(token_pos),
                                      _ptr(out), n, heads, vdim, ctypes.c_float(eps), code_of(out.dtype), _stream()),
            "memory_finish")
+
+
+# ---------------------------------------------------------------------------
+# attention of token rows whose sequences share pages
+
+
+class SharedPlan:
+    """What ``attention_shared`` works through for a batch whose sequences share pages (see ``shared_plan``): good as long as
+    its rows stay at the positions that it was made for and their page lists do not change."""
+
+    def __init__(self, rows, heads, kv_heads, head_dim, dtype, units, n_small, n_large, members, record, seqs, cols):
+        self.rows, self.heads, self.kv_heads, self.head_dim, self.dtype = rows, heads, kv_heads, head_dim, dtype
+        self.units, self.n_small, self.n_large, self.members, self.record = units, n_small, n_large, members, record
+        self.records, self.seqs, self.cols = 0, seqs, cols
+
+
+def attention_shared_takes(head_dim: int, page_size: int) -> bool:
+    return page_size == 64 and head_dim % 2 == 0 and 2 <= head_dim <= 256
+
+
+def attention_shared_plan(tables, seqs, positions, heads: int, kv_heads: int, head_dim: int, dtype: torch.dtype,
+                          device) -> SharedPlan:
+    """The plan of a batch: ``tables`` the page list of every sequence, ``seqs`` and ``positions`` the sequence and the
+    position (-1: a padding row) of every token row."""
+    import numpy as np
+    from .shared_plan import PAGE as page, shared_nodes, shared_units
+    n = len(seqs)
+    _need(n > 0 and len(positions) == n, "shared attention: a sequence and a position per token row")
+    _need(kv_heads > 0 and heads % kv_heads == 0, "attention: heads is not a multiple of kv_heads")
+    _need(attention_shared_takes(head_dim, page), f"attention: head_dim {head_dim} is not an even size in 2..256")
+    code_of(dtype)
+    for s, p in zip(seqs, positions):
+        _need(0 <= s < len(tables), f"shared attention: sequence {s} of {len(tables)}")
+        _need(p < len(tables[s]) * page, f"shared attention: position {p} is beyond its sequence's {len(tables[s])} pages")
+    nodes, tails = shared_nodes(tables, seqs, positions)
+    group = heads // kv_heads
+    device = torch.device(device)
+    sms = sm_count(device)
+    small, large, members, record = shared_units(nodes, tails, seqs, group, kv_heads, 64, 4 * sms, 2, 2.0)
+    ints = np.concatenate([small.reshape(-1), large.reshape(-1), members, record]).astype(np.int32)
+    held = torch.from_numpy(ints).to(device)
+    o = small.size + large.size
+    plan = SharedPlan(n, heads, kv_heads, head_dim, dtype, held[:o], len(small), len(large), held[o:o + members.size],
+                      held[o + members.size:], 1 + max(seqs), max([p // page + 1 for p in positions] + [1]))
+    plan.records = int(record[-1])
+    return plan
+
+
+def attention_shared(q: torch.Tensor, q_stride: int, k_cache: torch.Tensor, v_cache: torch.Tensor, token_pos: torch.Tensor,
+                     page_table: torch.Tensor, plan: SharedPlan, out: torch.Tensor, heads: int, kv_heads: int, head_dim: int,
+                     scale: float, workspace) -> None:
+    """Causal attention of packed query tokens over the paged cache, pages that several rows share read once for all of them.
+    ``plan``: ``attention_shared_plan`` of the same rows, positions and page lists."""
+    _cuda(k_cache, v_cache, token_pos, page_table, out)
+    _need(q.is_cuda, "q: CUDA tensor")
+    n = out.shape[0]
+    pages, nkv, page_size, d = k_cache.shape
+    _need(nkv == kv_heads and d == head_dim and v_cache.shape == k_cache.shape, "cache shape differs from the heads given")
+    _need((plan.rows, plan.heads, plan.kv_heads, plan.head_dim, plan.dtype) == (n, heads, kv_heads, head_dim, k_cache.dtype),
+          "shared attention: the plan was made for other rows, heads or another dtype")
+    _need(attention_shared_takes(d, page_size), f"attention_shared: head_dim {d} / page {page_size} is not taken")
+    _need(out.dim() == 2 and out.shape[1] == heads * d and out.dtype == k_cache.dtype == v_cache.dtype == q.dtype,
+          "attention: out [n, heads * d] in the cache dtype")
+    _need(q_stride >= heads * d and q.dim() == 2 and q.shape[0] >= n and q.stride() == (q_stride, 1),
+          "attention: q [n, heads * d] in rows of q_stride")
+    _need(token_pos.dtype == torch.int32 and page_table.dtype == torch.int32 and token_pos.numel() >= n, "positions, tables: int32")
+    _need(page_table.dim() == 2 and page_table.shape[0] >= plan.seqs and page_table.shape[1] >= plan.cols,
+          "shared attention: the page table is smaller than the plan's")
+    for t in (q, v_cache, token_pos, page_table, out, plan.units):
+        _need(t.device == k_cache.device, "shared attention: tensors of one device")
+    if torch.cuda.current_device() != k_cache.device.index:
+        with torch.cuda.device(k_cache.device):
+            return attention_shared(q, q_stride, k_cache, v_cache, token_pos, page_table, plan, out, heads, kv_heads, head_dim,
+                                    scale, workspace)
+    partial = workspace.get("attn_shared_records", (max(1, plan.records) * heads * (d + 2),), torch.float32)
+    _check(_lib().nnis_attention_shared(
+        _ptr(q), q_stride, _ptr(k_cache), _ptr(v_cache), _ptr(token_pos), _ptr(page_table), page_table.shape[1],
+        _ptr(plan.units), plan.n_small, plan.n_large, _ptr(plan.members), _ptr(plan.record), _ptr(partial), _ptr(out), n, heads,
+        kv_heads, d, pages, page_size, ctypes.c_float(scale), code_of(k_cache.dtype), _stream()), "attention_shared",
+        1 + (plan.n_small > 0) + (plan.n_large > 0))

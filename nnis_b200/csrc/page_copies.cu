@@ -1,0 +1,99 @@
+// Copies of pages inside the store of keys and values, all layers and moves in one launch:
+//     k[layer, dst, head, :rows] = k[layer, src, head, :rows], v the same,
+// what a forked sequence needs before it writes into the page that it shares (its first rows), and what pages that
+// move to other places need (all rows).  Rows of a head are one run of memory, whole pages one run over all heads.
+// The moves are kernel parameters, so nothing is copied up from the host first.
+#include "async_copy.cuh"
+#include "common.cuh"
+
+namespace nnis {
+
+constexpr int kMoves = 1024;  // of a launch: 12 KB of parameters
+
+struct PageMoves {
+    int src[kMoves], dst[kMoves], rows[kMoves];
+};
+
+// A CTA: some words of one run.  blockIdx: x = move and which of k and v, y = layer, z = a share of the run(s).
+template <typename W>
+__global__ void __launch_bounds__(256)
+copy_pages_kernel(const __grid_constant__ PageMoves moves, void* k, void* v, int pages, int kv_heads, int page_size, int k_row,
+                  int v_row) {
+    const int move = v ? blockIdx.x >> 1 : blockIdx.x;
+    const bool values = v && (blockIdx.x & 1);
+    const int row = values ? v_row : k_row;  // words of a row
+    const int src = moves.src[move], dst = moves.dst[move], rows = moves.rows[move];
+    const long long head_words = (long long)page_size * row;
+    const bool whole = rows == page_size;
+    const int runs = whole ? 1 : kv_heads;
+    const unsigned words = whole ? (unsigned)(kv_heads * head_words) : (unsigned)(rows * row);  // of a run
+    W* base = reinterpret_cast<W*>(values ? v : k) + (long long)blockIdx.y * pages * kv_heads * head_words;
+    const W* from = base + (long long)src * kv_heads * head_words;
+    W* to = base + (long long)dst * kv_heads * head_words;
+    const unsigned total = words * runs, step = gridDim.z * 256u;
+    constexpr int kAhead = 4;  // words a thread has on their way
+    for (unsigned at = blockIdx.z * 256u + threadIdx.x; at < total; at += kAhead * step) {
+        W word[kAhead];
+        long long place[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const unsigned w = at + i * step;
+            const unsigned run = runs == 1 ? 0 : w / words;
+            place[i] = (long long)run * head_words + (w - run * words);
+            if (w < total) word[i] = from[place[i]];
+        }
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i)
+            if (at + i * step < total) to[place[i]] = word[i];
+    }
+}
+
+}  // namespace nnis
+
+// k and v (or null): [layers, pages, kv_heads, page_size, row] with rows of `k_row` and `v_row` bytes, multiples of 4.
+// moves: `count` triples (src, dst, rows) on the host, checked by the caller: no page is the target of two moves or
+// the target of one and the source of another, ids below `pages`, rows 1 to page_size.
+NNIS_API int nnis_copy_pages(void* k, void* v, int layers, int pages, int kv_heads, int page_size, int k_row, int v_row,
+                             const int* moves, int count, int sms, cudaStream_t stream) {
+    using namespace nnis;
+    if (!k || !moves || count < 0 || layers <= 0 || pages <= 0 || kv_heads <= 0 || page_size <= 0 || k_row <= 0 || k_row % 4 ||
+        (v && (v_row <= 0 || v_row % 4)))
+        return NNIS_ERR_ARGUMENT;
+    const long long page_bytes = (long long)kv_heads * page_size * (k_row > v_row ? k_row : v_row);
+    if (layers > 65535 || page_bytes / 4 >= (1LL << 31)) return NNIS_ERR_UNSUPPORTED;
+    for (int i = 0; i < count; ++i)
+        if (moves[3 * i] < 0 || moves[3 * i] >= pages || moves[3 * i + 1] < 0 || moves[3 * i + 1] >= pages ||
+            moves[3 * i + 2] <= 0 || moves[3 * i + 2] > page_size)
+            return NNIS_ERR_ARGUMENT;
+    if (((uintptr_t)k | (uintptr_t)v) % 4) return NNIS_ERR_ALIGNMENT;
+    const bool wide = ((uintptr_t)k | (uintptr_t)v | (uintptr_t)k_row | (uintptr_t)(v ? v_row : 0)) % 16 == 0;
+    const int unit = wide ? 16 : 4;
+    const int tensors = v ? 2 : 1;
+    static PageMoves none = {};
+    for (int first = 0; first < count; first += kMoves) {
+        PageMoves p = none;
+        const int n = count - first < kMoves ? count - first : kMoves;
+        int most = 1;
+        for (int i = 0; i < n; ++i) {
+            p.src[i] = moves[3 * (first + i)];
+            p.dst[i] = moves[3 * (first + i) + 1];
+            p.rows[i] = moves[3 * (first + i) + 2];
+            most = p.rows[i] > most ? p.rows[i] : most;
+        }
+        const long long words = (long long)kv_heads * most * (k_row > v_row ? k_row : v_row) / unit;
+        const long long ctas = (long long)n * tensors * layers;
+        long long share = (words + 1023) / 1024;                          // four words a thread
+        const long long fill = (16LL * sms + ctas - 1) / ctas;            // ... unless there are CTAs enough
+        if (share > fill) share = fill;
+        if (share < 1) share = 1;
+        if (share > 65535) share = 65535;
+        const dim3 grid((unsigned)(n * tensors), (unsigned)layers, (unsigned)share);
+        if (wide)
+            copy_pages_kernel<uint4><<<grid, 256, 0, stream>>>(p, k, v, pages, kv_heads, page_size, k_row / 16, v_row / 16);
+        else
+            copy_pages_kernel<uint32_t><<<grid, 256, 0, stream>>>(p, k, v, pages, kv_heads, page_size, k_row / 4, v_row / 4);
+        const cudaError_t e = cudaGetLastError();
+        if (e != cudaSuccess) return (int)e;
+    }
+    return NNIS_OK;
+}

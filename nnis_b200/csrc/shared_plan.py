@@ -1,0 +1,118 @@
+"""Which pages of a batch are read once for several token rows, as work for the kernels of
+``ops.attention_shared``.
+
+Pure host code.  The rows' page lists form a tree: rows whose lists begin alike share a node,
+with the pages that all of them see whole (so that nothing in them is hidden from any row); below
+it they part, and what a row has alone, its partly filled last page among it, is its tail.  Every
+node's queries, (row, head of a kv head's group), are cut into tiles, its pages into chunks, so
+that the CTAs fill the device; see ``attention_shared.cuh`` for a unit's eight numbers.
+"""
+from __future__ import annotations
+
+from typing import List, Sequence, Tuple
+
+import numpy as np
+
+PAGE = 64
+
+
+def _alike(a: Sequence[int], b: Sequence[int], low: int, high: int) -> int:
+    """The first index in ``low .. high`` at which the lists differ (``high`` if at none)."""
+    if a is b or a[low:high] == b[low:high]:
+        return high
+    good, bad = low, high  # alike below ``good``, not alike below ``bad``
+    while bad - good > 1:
+        mid = (good + bad) // 2
+        if a[good:mid] == b[good:mid]:
+            good = mid
+        else:
+            bad = mid
+    return good
+
+
+def shared_nodes(tables: Sequence[Sequence[int]], seqs: Sequence[int], positions: Sequence[int],
+                 horizon: int = 0) -> Tuple[List[tuple], List[tuple]]:
+    """(nodes, tails): nodes (rows, first page, end page) that several rows share, parents before children;
+    tails (row, first page, end page).  ``horizon`` > 0: tails go on to that page (rows that will grow)."""
+    nodes: List[tuple] = []
+    tails: List[tuple] = []
+
+    def tail(row: int, depth: int) -> None:
+        end = max(horizon, positions[row] // PAGE + 1)
+        if end > depth:
+            tails.append((row, depth, end))
+
+    work = [([r for r in range(len(seqs)) if positions[r] >= 0], 0)]
+    while work:
+        rows, depth = work.pop()
+        if not rows:
+            continue
+        if len(rows) == 1:
+            tail(rows[0], depth)
+            continue
+        whole = [(positions[r] + 1) // PAGE for r in rows]
+        first, end = tables[seqs[rows[0]]], min(whole)
+        if end > depth:
+            for r in rows[1:]:
+                end = _alike(first, tables[seqs[r]], depth, end)
+                if end == depth:
+                    break
+        if end > depth:
+            nodes.append((rows, depth, end))
+        classes = {}
+        for r, n in zip(rows, whole):
+            if n > end:
+                classes.setdefault(tables[seqs[r]][end], []).append(r)
+            else:
+                tail(r, end)
+        if end == depth and len(classes) == 1 and len(next(iter(classes.values()))) == len(rows):
+            raise ValueError("page lists that neither share a page nor part")  # (cannot be)
+        work.extend((c, end) for c in classes.values())
+    return nodes, tails
+
+
+def shared_units(nodes: Sequence[tuple], tails: Sequence[tuple], seqs: Sequence[int], group: int, kv_heads: int,
+                 tile: int, ctas: int, least: int, weight: float):
+    """(small units [*, 8], large units [*, 8], members, record offsets [rows + 1]).
+
+    ``tile``: entries of a large unit (small ones hold 16); ``ctas``: how many CTAs fill the device;
+    ``least``: fewest pages of a chunk; ``weight``: what a page costs a large unit beside a small one."""
+    pieces = []  # (rows, first, end, ends)
+    for rows, a, b in nodes:
+        pieces.append((rows, a, b, 0))
+    for row, a, b in tails:
+        pieces.append(([row], a, b, 1))
+    costs = []
+    for rows, a, b, _ in pieces:
+        entries = len(rows) * group
+        tiles = 1 if entries <= 16 else -(-entries // tile)
+        costs.append((tiles, 1.0 if entries <= 16 else weight))
+    total = sum(t * w * (p[2] - p[1]) for (t, w), p in zip(costs, pieces)) * kv_heads
+    goal = max(total / max(1, ctas), 1.0)  # cost of a CTA
+    small: List[tuple] = []
+    large: List[tuple] = []
+    members: List[int] = []
+    slots = [0] * len(seqs)
+    for (rows, a, b, ends), (tiles, w) in zip(pieces, costs):
+        entries = len(rows) * group
+        per = max(least, int(goal / w + 0.5), 1)
+        chunks = max(1, -(-(b - a) // per))
+        per = -(-(b - a) // chunks)
+        at = len(members)
+        members.extend(rows)
+        size = entries if entries <= 16 else tile
+        into = small if entries <= 16 else large
+        slot = slots[rows[0]]
+        for c in range(-(-(b - a) // per)):
+            for e in range(0, entries, size):
+                into.append((at, e, min(size, entries - e), a + c * per, min(b, a + (c + 1) * per), slot, seqs[rows[0]], ends))
+            slot += 1
+        for r in rows:
+            slots[r] = slot
+    # the units that take longest first: the last to start are short
+    for units in (small, large):
+        units.sort(key=lambda u: u[3] - u[4])
+    record = np.zeros(len(seqs) + 1, dtype=np.int32)
+    np.cumsum(slots, out=record[1:])
+    as_units = lambda units: np.asarray(units, dtype=np.int32).reshape(-1, 8)
+    return as_units(small), as_units(large), np.asarray(members, dtype=np.int32), record

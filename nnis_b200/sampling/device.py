@@ -3,6 +3,8 @@ temperature sampling whose generator state lives beside the batch on the GPU.
 The kernels are in ``csrc/sampling.cu``."""
 from __future__ import annotations
 
+from typing import Optional
+
 import torch
 
 from ..csrc import ops
@@ -24,3 +26,22 @@ def temperature(logits: torch.Tensor, temperatures: torch.Tensor, rng_state: tor
                 out: torch.Tensor) -> torch.Tensor:
     ops.sample_temperature(logits, temperatures, rng_state, out)
     return out
+
+
+def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, first_row: torch.Tensor, temperatures: torch.Tensor,
+                  accept_draws: torch.Tensor, pick_draws: torch.Tensor, accepted: torch.Tensor, picked: torch.Tensor,
+                  draft_logits: Optional[torch.Tensor], workspace) -> None:
+    """Which drafted tokens the target keeps, and the token after them, from given random numbers.
+
+    Sequence b has k drafts and k + 1 packed rows of ``logits`` (float32 [rows, vocab]; row i follows i drafts),
+    from ``first_row[b]`` on (int32, one number more than sequences, the last one the number of rows).  ``drafts`` (int32),
+    ``accept_draws`` (float64 in [0, 1)) and ``draft_logits`` (float32 [drafts, vocab], what the drafts were drawn from
+    at the same temperature; None: nobody drew them) are packed the same way without the sequences' last rows.
+    With p and q the softmax of the rows over the temperature, a draft is kept iff draw * q(draft) < p(draft)
+    (q = 1 without draft logits).  ``accepted[b]`` (int32): the drafts before the first that is not kept; ``picked[b]``
+    (int32): the token after them, drawn with ``pick_draws[b]`` (float64) in id order from max(p - q, 0) where a draft was
+    not kept and from p where all were.  Temperature 0 (or less): a draft is kept iff it is the argmax, which is also the pick.
+    An id outside the vocabulary is never kept.  A row without probability (all logits -inf, a NaN or +inf among
+    them) ends its sequence there: picked is -1.  Offsets that no packed rows have give 0 and -1."""
+    ops.verify_drafts(logits, drafts, first_row, temperatures, accept_draws, pick_draws, accepted, picked, draft_logits,
+                      workspace)
