@@ -135,59 +135,74 @@ attn_shared_any_kernel(const SharedArgs a) {
         const int e = ty * ROWS + r;
         if (e >= u.entries) continue;
         const int at = u.entry + e, row = members[at / G];
-        float* rec = a.partial + ((size_t)(a.record[row] + u.slot) * a.nq + hk * G + at % G) * (size_t)(d + 2);
-        if (tx == 0) {
-            rec[0] = m_run[r];
-            rec[1] = l_run[r];
-        }
+        const size_t rec = (size_t)(a.record[row] + u.slot) * a.nq + hk * G + at % G;
+        if (tx == 0) reinterpret_cast<float2*>(a.sums)[rec] = make_float2(m_run[r], l_run[r]);
 #pragma unroll
         for (int j = 0; j < NJ; ++j)
-            if (tx + 16 * j < d) rec[2 + tx + 16 * j] = o[r][j];
+            if (tx + 16 * j < d) a.partial[rec * d + tx + 16 * j] = o[r][j];
     }
 }
 
-// A warp per (token row, head): lane s holds the weights of records s, s + 32, ...; every lane sums its values over the
-// records in their order.  A row without records (a padding row), or none of whose records holds a key, is zero.
+// A warp per (token row, head): lane s holds the weights of records s, s + 32, ...; every lane sums its pairs of values over the
+// records in their order, eight records asked for at a time.  A row without records (a padding row), or none of whose
+// records holds a key, is zero.
 template <typename T>
 __global__ void __launch_bounds__(128)
-attn_shared_merge_kernel(const float* __restrict__ partial, const int* __restrict__ record, T* __restrict__ out, int n_tokens,
-                         int nq, int d) {
-    pdl_wait();
-    pdl_launch_dependents();
+attn_shared_merge_kernel(const float* __restrict__ partial, const float2* __restrict__ sums, const int* __restrict__ record,
+                         T* __restrict__ out, int n_tokens, int nq, int d) {
     const int lane = threadIdx.x & 31;
     const size_t at = (size_t)blockIdx.x * 4 + (threadIdx.x >> 5);
     if (at >= (size_t)n_tokens * nq) return;
     const int row = (int)(at / nq), head = (int)(at % nq);
     const int first = record[row], count = record[row + 1] - first;
-    const float* rec = partial + ((size_t)first * nq + head) * (size_t)(d + 2);
-    const size_t step = (size_t)nq * (d + 2);
+    pdl_wait();
+    pdl_launch_dependents();
+    const size_t rec = (size_t)first * nq + head;
     float m = -INFINITY;
-    for (int s = lane; s < count; s += 32)
-        if (rec[s * step + 1] != 0.f) m = fmaxf(m, rec[s * step]);
+    for (int s = lane; s < count; s += 32) {
+        const float2 x = sums[rec + (size_t)s * nq];
+        if (x.y != 0.f) m = fmaxf(m, x.x);
+    }
     m = warp_max(m);
-    float acc[8] = {}, l = 0.f;
+    float2 acc[4] = {};
+    float l = 0.f;
+    constexpr int kAhead = 8;
     for (int s0 = 0; s0 < count; s0 += 32) {
         float w = 0.f;
         if (s0 + lane < count) {
-            const float held = rec[(s0 + lane) * step + 1];
-            w = held != 0.f ? exp2f(rec[(s0 + lane) * step] - m) : 0.f;
-            l += held * w;
+            const float2 x = sums[rec + (size_t)(s0 + lane) * nq];
+            w = x.y != 0.f ? exp2f(x.x - m) : 0.f;
+            l += x.y * w;
         }
         const int here = min(32, count - s0);
-        for (int s = 0; s < here; ++s) {
-            const float f = __shfl_sync(0xffffffffu, w, s);
-            if (f == 0.f) continue;  // (a record that holds nothing is never added)
-            const float* r = rec + (s0 + s) * step + 2;
+        for (int s = 0; s < here; s += kAhead) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (lane + 32 * j < d) acc[j] = fmaf(f, r[lane + 32 * j], acc[j]);
+            for (int j = 0; j < 4; ++j) {
+                if (j * 64 >= d) break;
+                const int i = 2 * (lane + 32 * j);
+                float2 v[kAhead];
+#pragma unroll
+                for (int k = 0; k < kAhead; ++k)
+                    v[k] = s + k < here && i < d ? *reinterpret_cast<const float2*>(partial + (rec + (size_t)(s0 + s + k) * nq) * d + i)
+                                                 : make_float2(0.f, 0.f);
+#pragma unroll
+                for (int k = 0; k < kAhead; ++k) {
+                    const float f = __shfl_sync(0xffffffffu, w, (s + k) & 31);
+                    if (s + k < here && f != 0.f) {  // (a record that holds nothing is never added)
+                        acc[j].x = fmaf(f, v[k].x, acc[j].x);
+                        acc[j].y = fmaf(f, v[k].y, acc[j].y);
+                    }
+                }
+            }
         }
     }
     l = warp_sum(l);
     const float inv = l != 0.f ? 1.0f / l : 0.f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-        if (lane + 32 * j < d) out[at * d + lane + 32 * j] = from_float<T>(acc[j] * inv);
+    for (int j = 0; j < 4; ++j) {
+        const int i = 2 * (lane + 32 * j);
+        if (i < d) store2(out + at * d + i, acc[j].x * inv, acc[j].y * inv);
+    }
 }
 
 template <typename T, int ROWS, int NJ>
@@ -215,31 +230,44 @@ cudaError_t shared_units_any(const SharedArgs& a, int n_units, int tile, bool f3
 
 }  // namespace nnis
 
-// units: n_small units of at most 16 entries, then n_large of at most 64.  The plan (units, members, record) is the host's,
-// made of tables that the call's page table agrees with; page ids outside the store hold no keys.
+// units: n[0] units of the first kind, n[1] of the second, n[2] of the third.  `form` 0 (any even head size, float32 or
+// bfloat16): at most 16, at most 64 entries, none; `form` 1 (bfloat16, heads of 64 and 128): none, at most 32, at most 128, the last
+// of which cover only positions that all their rows see.  The plan (units, members, record) is the host's, made of
+// page lists that the call's page table agrees with; page ids outside the store hold no keys.  partial: records x nq x d floats,
+// sums: records x nq x 2.
 NNIS_API int nnis_attention_shared(const void* q, int q_stride, const void* k_cache, const void* v_cache, const int* token_pos,
-                                   const int* page_table, int table_cols, const int* units, int n_small, int n_large,
-                                   const int* members, const int* record, float* partial, void* out, int n_tokens, int nq, int nkv,
-                                   int d, int pages, int page_size, float scale, int dtype, cudaStream_t stream) {
+                                   const int* page_table, int table_cols, const int* units, int n0, int n1, int n2,
+                                   const int* members, const int* record, float* partial, float* sums, void* out, int n_tokens,
+                                   int nq, int nkv, int d, int pages, int page_size, float scale, int dtype, int form, int* status,
+                                   cudaStream_t stream) {
     using namespace nnis;
-    if (n_tokens <= 0 || nq <= 0 || nkv <= 0 || nq % nkv || table_cols <= 0 || n_small < 0 || n_large < 0 || pages <= 0 || !record || !partial ||
-        (n_small + n_large > 0 && (!units || !members)))
+    if (n_tokens <= 0 || nq <= 0 || nkv <= 0 || nq % nkv || table_cols <= 0 || n0 < 0 || n1 < 0 || n2 < 0 || pages <= 0 || !record ||
+        !partial || !sums || !(scale > 0.f) || (n0 + n1 + n2 > 0 && (!units || !members)))
         return NNIS_ERR_ARGUMENT;
     if (page_size != kSharedPage || d < 2 || d > 256 || d % 2 || nkv > 65535) return NNIS_ERR_UNSUPPORTED;
-    if ((uintptr_t)units % 16 || (uintptr_t)partial % 8) return NNIS_ERR_ALIGNMENT;
-    if (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache) % (dtype == NNIS_DTYPE_F32 ? 8 : 4)) return NNIS_ERR_ALIGNMENT;
-    SharedArgs a = {q, k_cache, v_cache, token_pos, page_table, reinterpret_cast<const SharedUnit*>(units), members, record, partial,
-                    q_stride, table_cols, pages, nq, nkv, d, scale};
     const bool f32 = dtype == NNIS_DTYPE_F32;
-    for (int large = 0; large < 2; ++large) {
-        const int n = large ? n_large : n_small;
+    if (form == 1 && (f32 || (d != 64 && d != 128) || n0)) return NNIS_ERR_UNSUPPORTED;
+    if (form != 1 && n2) return NNIS_ERR_UNSUPPORTED;
+    if ((uintptr_t)units % 16 || (uintptr_t)partial % 16 || (uintptr_t)sums % 8) return NNIS_ERR_ALIGNMENT;
+    const uintptr_t all = (uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache;
+    if (all % (form == 1 ? 16 : f32 ? 8 : 4) || (uintptr_t)out % (f32 ? 8 : 4) || (form == 1 && q_stride % 8)) return NNIS_ERR_ALIGNMENT;
+    SharedArgs a = {q,       k_cache, v_cache, token_pos, page_table, reinterpret_cast<const SharedUnit*>(units), members, record,
+                    partial, sums,    q_stride, table_cols, pages,    nq, nkv, d, scale};
+    // (the large units first: the small ones end what is left of the device)
+    const SharedUnit* first = a.units;
+    for (int kind = 2; kind >= 0; --kind) {
+        const int n = kind == 2 ? n2 : kind == 1 ? n1 : n0;
         if (!n) continue;
-        if (large) a.units += n_small;
-        const cudaError_t e = shared_units_any(a, n, large ? 64 : 16, f32, stream);
+        a.units = first + (kind == 2 ? n0 + n1 : kind == 1 ? n0 : 0);
+        const cudaError_t e = form != 1   ? shared_units_any(a, n, kind == 1 ? 64 : 16, f32, stream)
+                              : kind == 2 ? shared_units_tc(a, n, status, stream)
+                                          : shared_units_mma(a, n, stream);
         if (e != cudaSuccess) return (int)e;
     }
     const unsigned ctas = (unsigned)(((size_t)n_tokens * nq + 3) / 4);
-    const cudaError_t e = f32 ? launch_dependent(attn_shared_merge_kernel<float>, ctas, 128, 0, stream, partial, record, (float*)out, n_tokens, nq, d)
-                              : launch_dependent(attn_shared_merge_kernel<bf16>, ctas, 128, 0, stream, partial, record, (bf16*)out, n_tokens, nq, d);
+    const float2* held = reinterpret_cast<const float2*>(sums);
+    const cudaError_t e =
+        f32 ? launch_dependent(attn_shared_merge_kernel<float>, ctas, 128, 0, stream, partial, held, record, (float*)out, n_tokens, nq, d)
+            : launch_dependent(attn_shared_merge_kernel<bf16>, ctas, 128, 0, stream, partial, held, record, (bf16*)out, n_tokens, nq, d);
     return e == cudaSuccess ? NNIS_OK : (int)e;
 }

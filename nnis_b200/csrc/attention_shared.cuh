@@ -3,8 +3,8 @@
 //
 // Token rows whose sequences begin with the same pages see those pages alike, so their queries are stacked: an *entry* is a
 // (token row, query head of a kv head's group), and a *unit* is up to a tile of entries of one list of token rows over a
-// range of pages that all of them see.  Per (token row, head, unit) a record [maximum, sum, d unnormalised outputs], the
-// maximum in log2 units, goes to scratch; the merge kernel adds a row's records up.  Units of a single token row end at the
+// range of pages that all of them see.  Per (token row, head, unit) a record, d unnormalised outputs, their maximum (log2
+// units) and sum, goes to scratch; the merge kernel adds a row's records up.  Units of a single token row end at the
 // row's position, all others cover only positions that every one of their rows sees.
 #pragma once
 
@@ -36,13 +36,15 @@ struct SharedArgs {
     const SharedUnit* units;
     const int* members;
     const int* record;   // [tokens + 1]: the first record of every token row
-    float* partial;      // [records, nq, d + 2]
+    float* partial;      // [records, nq, d]: outputs
+    float* sums;         // [records, nq, 2]: maximum and sum
     int q_stride, table_cols, pages, nq, nkv, d;
     float scale;
 };
 
 // One launch of the named form over `n_units` units; each is defined in its own file.
 cudaError_t shared_units_any(const SharedArgs& a, int n_units, int tile, bool f32, cudaStream_t stream);
-cudaError_t shared_units_mma(const SharedArgs& a, int n_units, int tile, cudaStream_t stream);
+cudaError_t shared_units_mma(const SharedArgs& a, int n_units, cudaStream_t stream);
+cudaError_t shared_units_tc(const SharedArgs& a, int n_units, int* status, cudaStream_t stream);
 
 }  // namespace nnis

@@ -2794,10 +2794,11 @@ class SharedPlan:
     """What ``attention_shared`` works through for a batch whose sequences share pages (see ``shared_plan``): good as long as
     its rows stay at the positions that it was made for and their page lists do not change."""
 
-    def __init__(self, rows, heads, kv_heads, head_dim, dtype, units, n_small, n_large, members, record, seqs, cols):
+    def __init__(self, rows, heads, kv_heads, head_dim, dtype, counts, ints, records, seqs, cols, form):
         self.rows, self.heads, self.kv_heads, self.head_dim, self.dtype = rows, heads, kv_heads, head_dim, dtype
-        self.units, self.n_small, self.n_large, self.members, self.record = units, n_small, n_large, members, record
-        self.records, self.seqs, self.cols = 0, seqs, cols
+        self.counts, self.ints, self.records, self.seqs, self.cols, self.form = counts, ints, records, seqs, cols, form
+        units, members = 8 * sum(counts), ints.numel() - 8 * sum(counts) - rows - 1
+        self.units, self.members, self.record = ints.data_ptr(), ints.data_ptr() + 4 * units, ints.data_ptr() + 4 * (units + members)
 
 
 def attention_shared_takes(head_dim: int, page_size: int) -> bool:
@@ -2819,17 +2820,14 @@ def attention_shared_plan(tables, seqs, positions, heads: int, kv_heads: int, he
         _need(0 <= s < len(tables), f"shared attention: sequence {s} of {len(tables)}")
         _need(p < len(tables[s]) * page, f"shared attention: position {p} is beyond its sequence's {len(tables[s])} pages")
     nodes, tails = shared_nodes(tables, seqs, positions)
-    group = heads // kv_heads
     device = torch.device(device)
+    tensor = dtype == torch.bfloat16 and head_dim in (64, 128)  # (the forms on the tensor cores)
     sms = sm_count(device)
-    small, large, members, record = shared_units(nodes, tails, seqs, group, kv_heads, 64, 4 * sms, 2, 2.0)
-    ints = np.concatenate([small.reshape(-1), large.reshape(-1), members, record]).astype(np.int32)
-    held = torch.from_numpy(ints).to(device)
-    o = small.size + large.size
-    plan = SharedPlan(n, heads, kv_heads, head_dim, dtype, held[:o], len(small), len(large), held[o:o + members.size],
-                      held[o + members.size:], 1 + max(seqs), max([p // page + 1 for p in positions] + [1]))
-    plan.records = int(record[-1])
-    return plan
+    kinds, members, record = shared_units(nodes, tails, seqs, heads // kv_heads, kv_heads, *(
+        ((0, 32, 128), (0.0, 1.0, 1.0), 1, 2 * sms, 2) if tensor else ((16, 64, 0), (1.0, 2.0, 0.0), 1, 4 * sms, 2)))
+    ints = np.concatenate([k.reshape(-1) for k in kinds] + [members, record]).astype(np.int32)
+    return SharedPlan(n, heads, kv_heads, head_dim, dtype, [len(k) for k in kinds], torch.from_numpy(ints).to(device),
+                      int(record[-1]), 1 + max(seqs), max([p // page + 1 for p in positions] + [1]), int(tensor))
 
 
 def attention_shared(q: torch.Tensor, q_stride: int, k_cache: torch.Tensor, v_cache: torch.Tensor, token_pos: torch.Tensor,
@@ -2852,15 +2850,20 @@ def attention_shared(q: torch.Tensor, q_stride: int, k_cache: torch.Tensor, v_ca
     _need(token_pos.dtype == torch.int32 and page_table.dtype == torch.int32 and token_pos.numel() >= n, "positions, tables: int32")
     _need(page_table.dim() == 2 and page_table.shape[0] >= plan.seqs and page_table.shape[1] >= plan.cols,
           "shared attention: the page table is smaller than the plan's")
-    for t in (q, v_cache, token_pos, page_table, out, plan.units):
+    _need(scale > 0, "shared attention: a positive scale")
+    for t in (q, v_cache, token_pos, page_table, out, plan.ints):
         _need(t.device == k_cache.device, "shared attention: tensors of one device")
     if torch.cuda.current_device() != k_cache.device.index:
         with torch.cuda.device(k_cache.device):
             return attention_shared(q, q_stride, k_cache, v_cache, token_pos, page_table, plan, out, heads, kv_heads, head_dim,
                                     scale, workspace)
-    partial = workspace.get("attn_shared_records", (max(1, plan.records) * heads * (d + 2),), torch.float32)
+    held = max(1, plan.records) * heads
+    partial = workspace.get("attn_shared_records", (held, d + 2), torch.float32)
+    n0, n1, n2 = plan.counts
+    at = partial.data_ptr()
     _check(_lib().nnis_attention_shared(
         _ptr(q), q_stride, _ptr(k_cache), _ptr(v_cache), _ptr(token_pos), _ptr(page_table), page_table.shape[1],
-        _ptr(plan.units), plan.n_small, plan.n_large, _ptr(plan.members), _ptr(plan.record), _ptr(partial), _ptr(out), n, heads,
-        kv_heads, d, pages, page_size, ctypes.c_float(scale), code_of(k_cache.dtype), _stream()), "attention_shared",
-        1 + (plan.n_small > 0) + (plan.n_large > 0))
+        ctypes.c_void_p(plan.units), n0, n1, n2, ctypes.c_void_p(plan.members), ctypes.c_void_p(plan.record),
+        ctypes.c_void_p(at), ctypes.c_void_p(at + 4 * held * d), _ptr(out), n, heads, kv_heads, d, pages, page_size,
+        ctypes.c_float(scale), code_of(k_cache.dtype), plan.form, _ptr(status_word(k_cache.device)), _stream()),
+        "attention_shared", 1 + (n0 > 0) + (n1 > 0) + (n2 > 0))

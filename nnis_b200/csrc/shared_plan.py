@@ -72,47 +72,38 @@ def shared_nodes(tables: Sequence[Sequence[int]], seqs: Sequence[int], positions
 
 
 def shared_units(nodes: Sequence[tuple], tails: Sequence[tuple], seqs: Sequence[int], group: int, kv_heads: int,
-                 tile: int, ctas: int, least: int, weight: float):
-    """(small units [*, 8], large units [*, 8], members, record offsets [rows + 1]).
+                 tiles: Sequence[int], costs: Sequence[float], ending: int, ctas: int, least: int):
+    """(units of every kind [*, 8], members, record offsets [rows + 1]).
 
-    ``tile``: entries of a large unit (small ones hold 16); ``ctas``: how many CTAs fill the device;
-    ``least``: fewest pages of a chunk; ``weight``: what a page costs a large unit beside a small one."""
-    pieces = []  # (rows, first, end, ends)
-    for rows, a, b in nodes:
-        pieces.append((rows, a, b, 0))
-    for row, a, b in tails:
-        pieces.append(([row], a, b, 1))
-    costs = []
-    for rows, a, b, _ in pieces:
+    ``tiles``: most entries of a unit of each kind, ascending (0: the kernel has no such kind); ``costs``: what a page costs a
+    unit of the kind, beside one another; ``ending``: the last kind that takes units whose rows end inside them; ``ctas``:
+    how many units fill the device; ``least``: fewest pages of a chunk."""
+    pieces = []  # (rows, first, end, ends, kind)
+    total = 0.0
+    for rows, a, b, ends in [(*n, 0) for n in nodes] + [([r], a, b, 1) for r, a, b in tails]:
         entries = len(rows) * group
-        tiles = 1 if entries <= 16 else -(-entries // tile)
-        costs.append((tiles, 1.0 if entries <= 16 else weight))
-    total = sum(t * w * (p[2] - p[1]) for (t, w), p in zip(costs, pieces)) * kv_heads
-    goal = max(total / max(1, ctas), 1.0)  # cost of a CTA
-    small: List[tuple] = []
-    large: List[tuple] = []
+        kinds = [i for i, t in enumerate(tiles) if t and (not ends or i <= ending)]
+        kind = next((i for i in kinds if entries <= tiles[i]), kinds[-1])
+        pieces.append((rows, a, b, ends, kind))
+        total += -(-entries // tiles[kind]) * costs[kind] * (b - a)
+    goal = max(total * kv_heads / max(1, ctas), 1.0)  # cost of a unit
+    units: List[List[tuple]] = [[] for _ in tiles]
     members: List[int] = []
     slots = [0] * len(seqs)
-    for (rows, a, b, ends), (tiles, w) in zip(pieces, costs):
-        entries = len(rows) * group
-        per = max(least, int(goal / w + 0.5), 1)
-        chunks = max(1, -(-(b - a) // per))
+    for rows, a, b, ends, kind in pieces:
+        entries, tile = len(rows) * group, tiles[kind]
+        chunks = max(1, -(-(b - a) // max(least, int(goal / costs[kind] + 0.5))))
         per = -(-(b - a) // chunks)
-        at = len(members)
+        at, slot = len(members), slots[rows[0]]
         members.extend(rows)
-        size = entries if entries <= 16 else tile
-        into = small if entries <= 16 else large
-        slot = slots[rows[0]]
-        for c in range(-(-(b - a) // per)):
-            for e in range(0, entries, size):
-                into.append((at, e, min(size, entries - e), a + c * per, min(b, a + (c + 1) * per), slot, seqs[rows[0]], ends))
+        for c in range(a, b, per):
+            for e in range(0, entries, tile):
+                units[kind].append((at, e, min(tile, entries - e), c, min(b, c + per), slot, seqs[rows[0]], ends))
             slot += 1
         for r in rows:
             slots[r] = slot
-    # the units that take longest first: the last to start are short
-    for units in (small, large):
-        units.sort(key=lambda u: u[3] - u[4])
+    for kind in units:  # the units that take longest first: the last to start are short
+        kind.sort(key=lambda u: u[3] - u[4])
     record = np.zeros(len(seqs) + 1, dtype=np.int32)
     np.cumsum(slots, out=record[1:])
-    as_units = lambda units: np.asarray(units, dtype=np.int32).reshape(-1, 8)
-    return as_units(small), as_units(large), np.asarray(members, dtype=np.int32), record
+    return ([np.asarray(kind, dtype=np.int32).reshape(-1, 8) for kind in units], np.asarray(members, dtype=np.int32), record)
