@@ -7,6 +7,7 @@ here computes; without the compiled library nothing works, on purpose.
 """
 from __future__ import annotations
 
+import array
 import ctypes
 import functools
 import math
@@ -58,6 +59,28 @@ def _stream() -> ctypes.c_void_p:
     if _raw_stream is not None:
         return ctypes.c_void_p(_raw_stream(torch.cuda.current_device()))
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+_P, _I, _L, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
+_entries = {}
+
+
+def _entry(name: str, *types):
+    """An entry point that takes plain numbers for its arguments (made once: a call with thirty arguments wrapped one by one,
+    and the library asked for, costs the host 8 us, this one 3)."""
+    fn = _entries.get(name)
+    if fn is None:
+        fn = getattr(_lib(), name)
+        fn.argtypes = types
+        _entries[name] = fn
+    return fn
+
+
+def _stream_here() -> int:
+    """The current stream of the current device as a number."""
+    if _raw_stream is not None:
+        return _raw_stream(torch.cuda.current_device())
+    return torch.cuda.current_stream().cuda_stream
 
 
 def _ptr(t: Optional[torch.Tensor]) -> ctypes.c_void_p:
@@ -141,21 +164,8 @@ class Pieces:
         self._run((ctypes.c_void_p * max(len(kept), 1))(*(t.data_ptr() for t in kept)), self.ptrs)
 
 
-def copy_pages(k: torch.Tensor, v: Optional[torch.Tensor], moves) -> None:
-    """Pages copied inside the store for all layers at once: for every (source page, target page, rows) of ``moves`` the
-    first ``rows`` positions of the target become the source's.  k: [layers, pages, kv_heads, page_size, dim], v the same with
-    its own dim, or None.  A page that is a target is the target of one move and the source of none."""
-    _cuda(k, v)
-    _need(k.dim() == 5 and k.numel() > 0, "copy_pages: k [layers, pages, kv_heads, page_size, dim]")
-    layers, pages, heads, page_size, dim = k.shape
-    size = k.element_size()
-    _need(v is None or (v.dim() == 5 and v.shape[:4] == k.shape[:4] and v.device == k.device and v.numel() > 0),
-          "copy_pages: v [layers, pages, kv_heads, page_size, value dim] beside k")
-    v_row = 0 if v is None else v.shape[4] * v.element_size()
-    _need(dim * size % 4 == 0 and v_row % 4 == 0, "copy_pages: rows of a multiple of four bytes")
-    _need(layers <= 65535, "copy_pages: at most 65,535 layers")
-    _need(heads * page_size * max(dim * size, v_row) < 2 ** 32, "copy_pages: pages below 4 GB")
-    flat = []
+def _moves_refused(moves, pages: int, page_size: int) -> None:
+    """Says what is wrong with moves that the library has not taken."""
     sources, targets = set(), set()
     for src, dst, rows in moves:
         _need(0 <= src < pages and 0 <= dst < pages, f"copy_pages: page {src} or {dst} is outside the store's {pages}")
@@ -163,18 +173,40 @@ def copy_pages(k: torch.Tensor, v: Optional[torch.Tensor], moves) -> None:
         _need(dst not in targets, f"copy_pages: page {dst} is the target of two moves")
         targets.add(dst)
         sources.add(src)
-        if rows:
-            flat += (src, dst, rows)
     _need(sources.isdisjoint(targets), "copy_pages: a page is a source and a target")
-    if not flat:
+
+
+def copy_pages(k: torch.Tensor, v: Optional[torch.Tensor], moves) -> None:
+    """Pages copied inside the store for all layers at once: for every (source page, target page, rows) of ``moves`` the
+    first ``rows`` positions of the target become the source's.  k: [layers, pages, kv_heads, page_size, dim], v the same with
+    its own dim, or None.  A page that is a target is the target of one move and the source of none."""
+    _cuda(k, v)
+    _need(k.dim() == 5 and k.numel() > 0, "copy_pages: k [layers, pages, kv_heads, page_size, dim]")
+    layers, pages, heads, page_size, dim = k.shape
+    k_row, v_row = dim * k.element_size(), 0
+    if v is not None:
+        _need(v.dim() == 5 and v.shape[:4] == k.shape[:4] and v.device == k.device and v.numel() > 0,
+              "copy_pages: v [layers, pages, kv_heads, page_size, value dim] beside k")
+        v_row = v.shape[4] * v.element_size()
+    _need(k_row % 4 == 0 and v_row % 4 == 0, "copy_pages: rows of a multiple of four bytes")
+    _need(layers <= 65535 and heads * page_size * max(k_row, v_row) < 2 ** 32, "copy_pages: at most 65,535 layers, pages below 4 GB")
+    if not moves:
         return
-    if torch.cuda.current_device() != k.device.index:
-        with torch.cuda.device(k.device):
+    device = k.device.index
+    if torch.cuda.current_device() != device:
+        with torch.cuda.device(device):
             return copy_pages(k, v, moves)
-    count = len(flat) // 3
-    _check(_lib().nnis_copy_pages(_ptr(k), _ptr(v), layers, pages, heads, page_size, dim * size, v_row,
-                                  (ctypes.c_int * len(flat))(*flat), count, sm_count(k.device), _stream()), "copy_pages",
-           -(-count // 1024))
+    try:  # (a list of 63 moves read number by number in Python takes 40 us, as three rows 7)
+        src, dst, rows = zip(*moves, strict=True)
+        ints = array.array("i", src + dst + rows)
+    except (TypeError, ValueError, OverflowError) as error:
+        raise KernelError(f"copy_pages: moves are (source page, target page, rows), whole numbers: {error}") from None
+    code = _entry("nnis_copy_pages", _P, _P, _I, _I, _I, _I, _I, _I, _P, _I, _I, _P)(
+        k.data_ptr(), None if v is None else v.data_ptr(), layers, pages, heads, page_size, k_row, v_row, ints.buffer_info()[0],
+        len(src), sm_count(k.device), _stream_here())
+    if code == -1:
+        _moves_refused(moves, pages, page_size)
+    _check(code, "copy_pages", -(-len(src) // 1024))
 
 
 def list_to_ints(values: list, limit: int):
@@ -355,10 +387,8 @@ def sample_temperature(logits: torch.Tensor, temperature: torch.Tensor, rng_stat
                                           _ptr(out), n, vocab, _stream()), "sample_temperature")
 
 
-def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, first_row: torch.Tensor, temperatures: torch.Tensor,
-                  accept_draws: torch.Tensor, pick_draws: torch.Tensor, accepted: torch.Tensor, picked: torch.Tensor,
-                  draft_logits: Optional[torch.Tensor], workspace) -> None:
-    """See ``sampling.device.verify_drafts``."""
+def _verify_refused(logits, drafts, first_row, temperatures, accept_draws, pick_draws, accepted, picked, draft_logits) -> None:
+    """Says what is wrong with a call that ``verify_drafts`` does not take."""
     _cuda(logits, drafts, first_row, temperatures, accept_draws, pick_draws, accepted, picked, draft_logits)
     _need(logits.dim() == 2 and logits.dtype == torch.float32 and logits.numel() > 0, "verify: logits float32 [rows, vocab]")
     rows, vocab = logits.shape
@@ -375,20 +405,37 @@ def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, first_row: torch.T
     _need(accepted.numel() == b and picked.numel() == b, "verify: accepted and picked, one a sequence")
     for t in (drafts, first_row, temperatures, accept_draws, pick_draws, accepted, picked, draft_logits):
         _need(t is None or t.device == logits.device, "verify: tensors of one device")
+    _need(draft_logits is None or (draft_logits.dtype == torch.float32 and tuple(draft_logits.shape) == (drafted, vocab)),
+          f"verify: draft_logits float32 [{drafted}, {vocab}]")
+
+
+def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, first_row: torch.Tensor, temperatures: torch.Tensor,
+                  accept_draws: torch.Tensor, pick_draws: torch.Tensor, accepted: torch.Tensor, picked: torch.Tensor,
+                  draft_logits: Optional[torch.Tensor], workspace) -> None:
+    """See ``sampling.device.verify_drafts``."""
+    b, device, i32, f32, f64 = first_row.numel() - 1, logits.device, torch.int32, torch.float32, torch.float64
+    rows, vocab = logits.shape if logits.dim() == 2 else (0, 0)
+    drafted = rows - b
+    good = 1 <= b <= rows <= 32767 and 0 < vocab <= 1 << 30
+    for t, dtype, count in ((logits, f32, rows * vocab), (drafts, i32, drafted), (first_row, i32, b + 1), (temperatures, f32, b),
+                            (accept_draws, f64, drafted), (pick_draws, f64, b), (accepted, i32, b), (picked, i32, b)):
+        good = good and t.dtype == dtype and t.numel() == count and t.device == device and t.is_contiguous()
     if draft_logits is not None:
-        _need(draft_logits.dtype == torch.float32 and tuple(draft_logits.shape) == (drafted, vocab),
-              f"verify: draft_logits float32 [{drafted}, {vocab}]")
-        if not drafted:
-            draft_logits = None
-    if torch.cuda.current_device() != logits.device.index:
-        with torch.cuda.device(logits.device):
+        good = good and draft_logits.dtype == f32 and draft_logits.shape == (drafted, vocab) and draft_logits.device == device \
+            and draft_logits.is_contiguous()
+    if not good or device.type != "cuda":
+        _verify_refused(logits, drafts, first_row, temperatures, accept_draws, pick_draws, accepted, picked, draft_logits)
+        raise KernelError("verify: arguments that are not taken")
+    if torch.cuda.current_device() != device.index:
+        with torch.cuda.device(device):
             return verify_drafts(logits, drafts, first_row, temperatures, accept_draws, pick_draws, accepted, picked,
                                  draft_logits, workspace)
-    need = int(_lib().nnis_verify_scratch(rows, drafted, vocab))
-    scratch = workspace.get("verify_sums", (need // 4,), torch.float32)
-    _check(_lib().nnis_verify_drafts(_ptr(logits), _ptr(draft_logits), _ptr(drafts), _ptr(first_row), _ptr(temperatures),
-                                     _ptr(accept_draws), _ptr(pick_draws), _ptr(scratch), b, rows, vocab, _ptr(accepted),
-                                     _ptr(picked), _stream()), "verify_drafts", 2)
+    need = _entry("nnis_verify_scratch", _I, _I, _I)(rows, drafted, vocab)
+    scratch = workspace.get("verify_sums", (need // 4,), f32)
+    _check(_entry("nnis_verify_drafts", _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _P, _P, _P)(
+        logits.data_ptr(), draft_logits.data_ptr() if draft_logits is not None and drafted else None, drafts.data_ptr(),
+        first_row.data_ptr(), temperatures.data_ptr(), accept_draws.data_ptr(), pick_draws.data_ptr(), scratch.data_ptr(), b, rows,
+        vocab, accepted.data_ptr(), picked.data_ptr(), _stream_here()), "verify_drafts", 2)
 
 
 EPI_STORE, EPI_STORE_F32, EPI_ADD_F32, EPI_GATED, EPI_QKV, EPI_ARGMAX = 0, 1, 2, 3, 4, 5
@@ -2799,6 +2846,7 @@ class SharedPlan:
         self.counts, self.ints, self.records, self.seqs, self.cols, self.form = counts, ints, records, seqs, cols, form
         units, members = 8 * sum(counts), ints.numel() - 8 * sum(counts) - rows - 1
         self.units, self.members, self.record = ints.data_ptr(), ints.data_ptr() + 4 * units, ints.data_ptr() + 4 * (units + members)
+        self.device, self.status, self.launches = ints.device, status_word(ints.device).data_ptr(), 1 + sum(c > 0 for c in counts)
 
 
 def attention_shared_takes(head_dim: int, page_size: int) -> bool:
@@ -2835,35 +2883,33 @@ def attention_shared(q: torch.Tensor, q_stride: int, k_cache: torch.Tensor, v_ca
                      scale: float, workspace) -> None:
     """Causal attention of packed query tokens over the paged cache, pages that several rows share read once for all of them.
     ``plan``: ``attention_shared_plan`` of the same rows, positions and page lists."""
-    _cuda(k_cache, v_cache, token_pos, page_table, out)
-    _need(q.is_cuda, "q: CUDA tensor")
-    n = out.shape[0]
-    pages, nkv, page_size, d = k_cache.shape
-    _need(nkv == kv_heads and d == head_dim and v_cache.shape == k_cache.shape, "cache shape differs from the heads given")
-    _need((plan.rows, plan.heads, plan.kv_heads, plan.head_dim, plan.dtype) == (n, heads, kv_heads, head_dim, k_cache.dtype),
-          "shared attention: the plan was made for other rows, heads or another dtype")
-    _need(attention_shared_takes(d, page_size), f"attention_shared: head_dim {d} / page {page_size} is not taken")
-    _need(out.dim() == 2 and out.shape[1] == heads * d and out.dtype == k_cache.dtype == v_cache.dtype == q.dtype,
-          "attention: out [n, heads * d] in the cache dtype")
-    _need(q_stride >= heads * d and q.dim() == 2 and q.shape[0] >= n and q.stride() == (q_stride, 1),
-          "attention: q [n, heads * d] in rows of q_stride")
-    _need(token_pos.dtype == torch.int32 and page_table.dtype == torch.int32 and token_pos.numel() >= n, "positions, tables: int32")
-    _need(page_table.dim() == 2 and page_table.shape[0] >= plan.seqs and page_table.shape[1] >= plan.cols,
-          "shared attention: the page table is smaller than the plan's")
-    _need(scale > 0, "shared attention: a positive scale")
-    for t in (q, v_cache, token_pos, page_table, out, plan.ints):
-        _need(t.device == k_cache.device, "shared attention: tensors of one device")
-    if torch.cuda.current_device() != k_cache.device.index:
-        with torch.cuda.device(k_cache.device):
+    n, d, dtype, device = plan.rows, plan.head_dim, plan.dtype, plan.device
+    shape = k_cache.shape
+    if not (heads == plan.heads and kv_heads == plan.kv_heads and head_dim == d and len(shape) == 4 and shape[1] == kv_heads
+            and shape[2] == 64 and shape[3] == d and v_cache.shape == shape and out.shape == (n, heads * d)
+            and q.dim() == 2 and q.shape[0] >= n and q.stride() == (q_stride, 1) and q_stride >= heads * d
+            and token_pos.numel() >= n and page_table.dim() == 2 and page_table.shape[0] >= plan.seqs
+            and page_table.shape[1] >= plan.cols and q.dtype == k_cache.dtype == v_cache.dtype == out.dtype == dtype
+            and token_pos.dtype == page_table.dtype == torch.int32 and scale > 0
+            and q.device == k_cache.device == v_cache.device == token_pos.device == page_table.device == out.device == device
+            and k_cache.is_contiguous() and v_cache.is_contiguous() and out.is_contiguous() and token_pos.is_contiguous()
+            and page_table.is_contiguous() and shape[0] * kv_heads < 1 << 25):
+        raise KernelError(
+            f"attention_shared: the plan is of {n} rows, {plan.heads} heads over {plan.kv_heads} of {d}, {dtype}, {plan.seqs} sequences of "
+            f"{plan.cols} pages on {device}; wanted are q [rows, heads * d] in rows of q_stride, k and v [pages < 2^25 / kv_heads, "
+            f"kv_heads, 64, d], token_pos int32 [rows], page_table int32, out [rows, heads * d], contiguous, and a positive scale; got "
+            f"q {tuple(q.shape)} of {q.dtype}, cache {tuple(shape)} of {k_cache.dtype}, out {tuple(out.shape)}, page_table "
+            f"{tuple(page_table.shape)}, scale {scale}")
+    if torch.cuda.current_device() != device.index:
+        with torch.cuda.device(device):
             return attention_shared(q, q_stride, k_cache, v_cache, token_pos, page_table, plan, out, heads, kv_heads, head_dim,
                                     scale, workspace)
     held = max(1, plan.records) * heads
-    partial = workspace.get("attn_shared_records", (held, d + 2), torch.float32)
+    at = workspace.get("attn_shared_records", (held, d + 2), torch.float32).data_ptr()
     n0, n1, n2 = plan.counts
-    at = partial.data_ptr()
-    _check(_lib().nnis_attention_shared(
-        _ptr(q), q_stride, _ptr(k_cache), _ptr(v_cache), _ptr(token_pos), _ptr(page_table), page_table.shape[1],
-        ctypes.c_void_p(plan.units), n0, n1, n2, ctypes.c_void_p(plan.members), ctypes.c_void_p(plan.record),
-        ctypes.c_void_p(at), ctypes.c_void_p(at + 4 * held * d), _ptr(out), n, heads, kv_heads, d, pages, page_size,
-        ctypes.c_float(scale), code_of(k_cache.dtype), plan.form, _ptr(status_word(k_cache.device)), _stream()),
-        "attention_shared", 1 + (n0 > 0) + (n1 > 0) + (n2 > 0))
+    _check(_entry("nnis_attention_shared", _P, _I, _P, _P, _P, _P, _I, _P, _I, _I, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I,
+                  _F, _I, _I, _P, _P)(
+        q.data_ptr(), q_stride, k_cache.data_ptr(), v_cache.data_ptr(), token_pos.data_ptr(), page_table.data_ptr(),
+        page_table.shape[1], plan.units, n0, n1, n2, plan.members, plan.record, at, at + 4 * held * d, out.data_ptr(), n, heads,
+        kv_heads, d, shape[0], 64, scale, F32 if dtype == torch.float32 else BF16, plan.form, plan.status, _stream_here()),
+        "attention_shared", plan.launches)

@@ -3,6 +3,8 @@
 // what a forked sequence needs before it writes into the page that it shares (its first rows), and what pages that
 // move to other places need (all rows).  Rows of a head are one run of memory, whole pages one run over all heads.
 // The moves are kernel parameters, so nothing is copied up from the host first.
+#include <stdlib.h>
+
 #include "async_copy.cuh"
 #include "common.cuh"
 
@@ -51,8 +53,8 @@ copy_pages_kernel(const __grid_constant__ PageMoves moves, void* k, void* v, int
 }  // namespace nnis
 
 // k and v (or null): [layers, pages, kv_heads, page_size, row] with rows of `k_row` and `v_row` bytes, multiples of 4.
-// moves: `count` triples (src, dst, rows) on the host, checked by the caller: no page is the target of two moves or
-// the target of one and the source of another, ids below `pages`, rows 1 to page_size.
+// moves, on the host: `count` sources, then targets, then numbers of rows (0 to page_size).  NNIS_ERR_ARGUMENT, with nothing
+// copied, where a page is outside the store, the target of two moves, or a target and a source.
 NNIS_API int nnis_copy_pages(void* k, void* v, int layers, int pages, int kv_heads, int page_size, int k_row, int v_row,
                              const int* moves, int count, int sms, cudaStream_t stream) {
     using namespace nnis;
@@ -61,11 +63,21 @@ NNIS_API int nnis_copy_pages(void* k, void* v, int layers, int pages, int kv_hea
         return NNIS_ERR_ARGUMENT;
     const long long page_bytes = (long long)kv_heads * page_size * (k_row > v_row ? k_row : v_row);
     if (layers > 65535 || page_bytes / 4 >= (1LL << 31)) return NNIS_ERR_UNSUPPORTED;
-    for (int i = 0; i < count; ++i)
-        if (moves[3 * i] < 0 || moves[3 * i] >= pages || moves[3 * i + 1] < 0 || moves[3 * i + 1] >= pages ||
-            moves[3 * i + 2] <= 0 || moves[3 * i + 2] > page_size)
-            return NNIS_ERR_ARGUMENT;
     if (((uintptr_t)k | (uintptr_t)v) % 4) return NNIS_ERR_ALIGNMENT;
+    const int *src = moves, *dst = moves + count, *rows = moves + 2 * count;
+    unsigned char* seen = static_cast<unsigned char*>(calloc((size_t)pages, 1));  // 1: a source, 2: a target
+    if (!seen) return (int)cudaErrorMemoryAllocation;
+    bool good = true;
+    for (int i = 0; i < count && good; ++i) {
+        good = src[i] >= 0 && src[i] < pages && dst[i] >= 0 && dst[i] < pages && rows[i] >= 0 && rows[i] <= page_size;
+        if (good) seen[src[i]] |= 1;
+    }
+    for (int i = 0; i < count && good; ++i) {
+        good = !seen[dst[i]];
+        seen[dst[i]] |= 2;
+    }
+    free(seen);
+    if (!good) return NNIS_ERR_ARGUMENT;
     const bool wide = ((uintptr_t)k | (uintptr_t)v | (uintptr_t)k_row | (uintptr_t)(v ? v_row : 0)) % 16 == 0;
     const int unit = wide ? 16 : 4;
     const int tensors = v ? 2 : 1;
@@ -75,9 +87,9 @@ NNIS_API int nnis_copy_pages(void* k, void* v, int layers, int pages, int kv_hea
         const int n = count - first < kMoves ? count - first : kMoves;
         int most = 1;
         for (int i = 0; i < n; ++i) {
-            p.src[i] = moves[3 * (first + i)];
-            p.dst[i] = moves[3 * (first + i) + 1];
-            p.rows[i] = moves[3 * (first + i) + 2];
+            p.src[i] = src[first + i];
+            p.dst[i] = dst[first + i];
+            p.rows[i] = rows[first + i];
             most = p.rows[i] > most ? p.rows[i] : most;
         }
         const long long words = (long long)kv_heads * most * (k_row > v_row ? k_row : v_row) / unit;

@@ -30,12 +30,10 @@ constexpr int kVerifyShare = 8192;   // logits of a row that a CTA of the first 
 constexpr int kVerifyParts = 32;     // most CTAs a row
 constexpr int kPickThreads = 512;
 constexpr int kPickCtas = 8;         // of a cluster
-constexpr float kBad = 1.f;
 
 struct RowSum {
-    float max, sum;  // maximum logit, sum of exp((x - max) / T)
+    float max, sum;  // maximum logit, sum of exp((x - max) / T): no number where a logit is none, or +infinity
     int best;        // id of the maximum, the lower among equals
-    float bad;       // kBad: a logit is no number or +infinity
 };
 
 // log2(e) / T, within bounds that keep 0 and -infinity times it what they are (where that is another number the sums in 64
@@ -44,14 +42,20 @@ __device__ __forceinline__ float scale_of(float temperature) {
     return temperature > 0.f ? fmaxf(fminf(1.4426950408889634f / temperature, 1e30f), 1e-30f) : 1.f;
 }
 
+// 2^x; denormal results are zero
+__device__ __forceinline__ float weight32(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 // (m, s, best) of two sets of ids
 __device__ __forceinline__ RowSum joined(const RowSum& a, const RowSum& b, float c) {
     RowSum r;
     r.max = fmaxf(a.max, b.max);
-    r.bad = fmaxf(a.bad, b.bad);
     r.best = a.max > b.max || (a.max == b.max && a.best < b.best) ? a.best : b.best;
     const float base = r.max == -INFINITY ? 0.f : r.max;
-    r.sum = a.sum * exp2f((a.max - base) * c) + b.sum * exp2f((b.max - base) * c);
+    r.sum = a.sum * weight32((a.max - base) * c) + b.sum * weight32((b.max - base) * c);
     return r;
 }
 
@@ -75,27 +79,56 @@ verify_rows_kernel(const float* __restrict__ logits, const float* __restrict__ d
     const float c = scale_of(t);
     const float* row = of_draft ? draft_logits + (size_t)(r - rows) * vocab : logits + (size_t)r * vocab;
     const int begin = min(vocab, (int)blockIdx.x * per), end = min(vocab, begin + per);
-    RowSum mine = {-INFINITY, 0.f, 0x7fffffff, 0.f};
-    constexpr int kAhead = 8;
-    for (int at = begin + threadIdx.x; at < end; at += kAhead * kVerifyThreads) {
-        float x[kAhead];
+    // (32 bits: the maximum is taken off first, exactly, so that a large one costs no digits)
+    RowSum mine = {-INFINITY, 0.f, 0x7fffffff};
+    constexpr int kAhead = 4;  // quads a thread has on their way
+    auto take = [&](const float (&x)[4 * kAhead], int at, int step) {  // x[i] has the id at + step * (i / 4) + i % 4
+        float m = x[0];
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) x[i] = at + i * kVerifyThreads < end ? row[at + i * kVerifyThreads] : -INFINITY;
-        float m = mine.max;
+        for (int i = 1; i < 4 * kAhead; ++i) m = fmaxf(m, x[i]);
+        if (m > mine.max) {
+            mine.sum *= weight32((mine.max - m) * c);
+            mine.max = m;
+#pragma unroll
+            for (int i = 4 * kAhead - 1; i >= 0; --i)
+                if (x[i] == m) mine.best = at + step * (i / 4) + i % 4;
+        }
+        const float base = mine.max == -INFINITY ? 0.f : mine.max;
+        float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < 4 * kAhead; ++i) s[i & 3] += weight32((x[i] - base) * c);  // (a NaN or +infinity makes the sum one)
+        mine.sum += (s[0] + s[1]) + (s[2] + s[3]);
+    };
+    // quads from the row's first 16-byte boundary on; thread 0 takes what lies before it and what is left behind them
+    const int head = min(end - begin, (int)((4 - (((uintptr_t)(row + begin) >> 2) & 3)) & 3)), quads = (end - begin - head) / 4;
+    const float4* row4 = reinterpret_cast<const float4*>(row + begin + head);
+    for (int at = threadIdx.x; at < quads; at += kAhead * kVerifyThreads) {
+        float x[4 * kAhead];
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
-            if (!(x[i] < INFINITY)) mine.bad = kBad;
-            if (x[i] > m) {
-                m = x[i];
-                mine.best = at + i * kVerifyThreads;
-            }
+            const int w = at + i * kVerifyThreads;
+            const float4 v = w < quads ? __ldcs(row4 + w) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+            x[4 * i] = v.x;
+            x[4 * i + 1] = v.y;
+            x[4 * i + 2] = v.z;
+            x[4 * i + 3] = v.w;
         }
-        const float base = m == -INFINITY ? 0.f : m;
-        float s = mine.sum * exp2f((mine.max - base) * c);
+        take(x, begin + head + 4 * at, 4 * kVerifyThreads);
+    }
+    if (threadIdx.x == 0) {
+        float x[4 * kAhead];
+        const int tail = begin + head + 4 * quads;
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) s += x[i] == -INFINITY ? 0.f : exp2f((x[i] - base) * c);
-        mine.max = m;
-        mine.sum = s;
+        for (int i = 0; i < 4 * kAhead; ++i) x[i] = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+            if (i < head) x[i] = row[begin + i];
+            if (tail + i < end) x[4 + i] = row[tail + i];
+        }
+        RowSum kept = mine;
+        mine = {-INFINITY, 0.f, 0x7fffffff};
+        take(x, begin, tail - begin);
+        mine = joined(kept, mine, c);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
@@ -103,7 +136,6 @@ verify_rows_kernel(const float* __restrict__ logits, const float* __restrict__ d
         other.max = __shfl_xor_sync(0xffffffffu, mine.max, o);
         other.sum = __shfl_xor_sync(0xffffffffu, mine.sum, o);
         other.best = __shfl_xor_sync(0xffffffffu, mine.best, o);
-        other.bad = __shfl_xor_sync(0xffffffffu, mine.bad, o);
         mine = joined(mine, other, c);
     }
     if ((threadIdx.x & 31) == 0) warp_sum_s[threadIdx.x >> 5] = mine;
@@ -117,7 +149,7 @@ verify_rows_kernel(const float* __restrict__ logits, const float* __restrict__ d
 // A row's parts joined by a warp (at most 32 of them); every lane gets the result.
 __device__ __forceinline__ RowSum row_sum(const RowSum* __restrict__ parts, size_t row, int n_parts, float c) {
     const int lane = threadIdx.x & 31;
-    RowSum mine = {-INFINITY, 0.f, 0x7fffffff, 0.f};
+    RowSum mine = {-INFINITY, 0.f, 0x7fffffff};
     if (lane < n_parts) mine = parts[row * n_parts + lane];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
@@ -125,7 +157,6 @@ __device__ __forceinline__ RowSum row_sum(const RowSum* __restrict__ parts, size
         other.max = __shfl_xor_sync(0xffffffffu, mine.max, o);
         other.sum = __shfl_xor_sync(0xffffffffu, mine.sum, o);
         other.best = __shfl_xor_sync(0xffffffffu, mine.best, o);
-        other.bad = __shfl_xor_sync(0xffffffffu, mine.bad, o);
         mine = joined(mine, other, c);
     }
     return mine;
@@ -137,15 +168,27 @@ __device__ __forceinline__ double warp_sum64(double v) {
     return v;
 }
 
-__device__ __forceinline__ double weight64(float x, float max, double inv_t) {
-    return x == -INFINITY ? 0.0 : exp(((double)x - (double)max) * inv_t);
+// exp((x - max) / T) in 64 bits for x <= max: 2^(k / 64) from a table times the series of exp(r), |r| <= ln 2 / 128, to r^5 (what is
+// left out is 3e-17), after P. T. P. Tang's table-driven method (ACM TOMS 15, 1989).  Ten operations where
+// the library's exp, good to the last place, takes twice that: the sums of a row are bound by them.
+__device__ __forceinline__ double weight64(const double* table, float x, float max, double inv_t) {
+    const double t = ((double)x - (double)max) * inv_t;
+    if (!(t > -700.0) || x == -INFINITY) return t <= -700.0 || x == -INFINITY ? 0.0 : t;  // (too small to count; no number stays none)
+    constexpr double kRound = 6755399441055744.0;     // 1.5 * 2^52: adding it rounds to a whole number, in the low word
+    double k = fma(t, 92.33248261689366, kRound);     // 64 / ln 2
+    const int n = __double2loint(k);
+    k -= kRound;
+    const double r = fma(k, -3.623510646634843e-19, fma(k, -0.010830424696249145, t));  // ln 2 / 64 in two parts
+    const double p = fma(fma(fma(fma(r, 1.0 / 120.0, 1.0 / 24.0), r, 1.0 / 6.0), r, 0.5), r * r, r);
+    const double e = table[n & 63], w = fma(e, p, e);
+    return __hiloint2double(__double2hiint(w) + (n >> 6) * (1 << 20), __double2loint(w));
 }
 
 struct PickShared {
+    double table[64];    // 2^(j / 64)
     double warp[2][kPickThreads / 32];
     double cta[2];       // this CTA's sums, read by the others of its cluster
-    double mass;         // ... of what is drawn from
-    int picked;
+    int picked, stop;
 };
 
 // Sum over the whole cluster of up to two values a thread, every thread gets both.
@@ -176,7 +219,7 @@ __device__ __forceinline__ void cluster_sum(cg::cluster_group cluster, PickShare
     cluster.sync();
 }
 
-__global__ void __launch_bounds__(kPickThreads) __cluster_dims__(kPickCtas, 1, 1)
+__global__ void __launch_bounds__(kPickThreads, 1) __cluster_dims__(kPickCtas, 1, 1)
 verify_pick_kernel(const float* __restrict__ logits, const float* __restrict__ draft_logits, const int* __restrict__ drafts,
                    const int* __restrict__ first_row, const float* __restrict__ temperature, const double* __restrict__ accept_draws,
                    const double* __restrict__ pick_draws, const RowSum* __restrict__ parts, int n_parts, int rows, int vocab,
@@ -185,6 +228,9 @@ verify_pick_kernel(const float* __restrict__ logits, const float* __restrict__ d
     cg::cluster_group cluster = cg::this_cluster();
     const int b = blockIdx.y, rank = (int)cluster.block_rank();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    constexpr int kWarps = kPickThreads / 32;
+    if (tid < 64) s.table[tid] = exp2((double)tid * (1.0 / 64.0));
+    if (tid == 0) s.stop = 0x7fffffff;
     pdl_wait();
     pdl_launch_dependents();
     const int row0 = first_row[b], draft0 = row0 - b, count = first_row[b + 1] - row0 - 1;
@@ -195,137 +241,192 @@ verify_pick_kernel(const float* __restrict__ logits, const float* __restrict__ d
         }
         return;
     }
+    __syncthreads();
     const float t = temperature[b];
     const bool greedy = !(t > 0.f);
     const float c = scale_of(t);
     const double inv_t = greedy ? 1.0 : 1.0 / (double)t;
-    // this thread's ids: a range of the row per CTA, a range of that per warp
-    constexpr int kWarps = kPickThreads / 32;
+
+    // The drafts, a warp each: where the first one lies that is not kept for sure, and why (every CTA of the cluster for
+    // itself, all alike).
+    enum { kKept, kRefused, kNothing, kNear };
+    auto decide = [&](int i) -> int {
+        const RowSum zs = row_sum(parts, (size_t)(row0 + i), n_parts, c);
+        if (!(zs.sum >= 0.f) || zs.max == -INFINITY || zs.max == INFINITY) return kNothing;
+        if (i >= count) return kRefused;
+        const int d = drafts[draft0 + i];
+        if (greedy) return d == zs.best ? kKept : kRefused;
+        const bool known = d >= 0 && d < vocab;
+        double eq = 1.0, sum_q = 1.0;
+        if (draft_logits) {
+            const RowSum ys = row_sum(parts, (size_t)(rows + draft0 + i), n_parts, c);
+            if (!(ys.sum >= 0.f) || ys.max == -INFINITY || ys.max == INFINITY) return kNothing;
+            if (known) eq = weight64(s.table, draft_logits[(size_t)(draft0 + i) * vocab + d], ys.max, inv_t);
+            sum_q = (double)ys.sum;
+        }
+        if (!known) return kRefused;
+        const double left = accept_draws[draft0 + i] * eq * (double)zs.sum;
+        const double right = weight64(s.table, logits[(size_t)(row0 + i) * vocab + d], zs.max, inv_t) * sum_q;
+        if (fabs(left - right) <= 1e-4 * right || t < 1e-29f) return kNear;
+        return left < right ? kKept : kRefused;
+    };
+    // The ids of a warp lie together, lane by lane; a lane's weights of a row stay in registers where one block holds them.
+    constexpr int kHeld = 16;
     const int per_warp = (((vocab + kPickCtas * kWarps - 1) / (kPickCtas * kWarps)) + 31) & ~31;
     const int begin = min(vocab, (rank * kWarps + warp) * per_warp), end = min(vocab, begin + per_warp);
-
-    // the sums of a row of z and of its row of y, in 64 bits
-    auto exact_sums = [&](const float* z, float z_max, const float* y, float y_max, double& sp, double& sq) {
+    const int blocks = (per_warp + 32 * kHeld - 1) / (32 * kHeld);  // (one up to 65,536 ids)
+    double ez[kHeld], ey[kHeld];
+    const float *z = nullptr, *y = nullptr;
+    float z_max = 0.f, y_max = 0.f;
+    auto weights = [&](int block) {
+        float xz[kHeld], xy[kHeld];
+        const int first = begin + block * 32 * kHeld + lane;
+#pragma unroll
+        for (int k = 0; k < kHeld; ++k) {
+            const int i = first + 32 * k;
+            xz[k] = i < end ? z[i] : -INFINITY;
+            xy[k] = y && i < end ? y[i] : -INFINITY;
+        }
+#pragma unroll
+        for (int k = 0; k < kHeld; ++k) {
+            if (32 * k >= per_warp) {  // (nobody's)
+                ez[k] = ey[k] = 0.0;
+                continue;
+            }
+            ez[k] = weight64(s.table, xz[k], z_max, inv_t);
+            ey[k] = y ? weight64(s.table, xy[k], y_max, inv_t) : 0.0;
+        }
+    };
+    auto exact_sums = [&](int i, double& sp, double& sq) {  // of row i, in 64 bits
+        z = logits + (size_t)(row0 + i) * vocab;
+        z_max = row_sum(parts, (size_t)(row0 + i), n_parts, c).max;
+        y = draft_logits && i < count ? draft_logits + (size_t)(draft0 + i) * vocab : nullptr;
+        if (y) y_max = row_sum(parts, (size_t)(rows + draft0 + i), n_parts, c).max;
         sp = sq = 0.0;
-        for (int i = begin + lane; i < end; i += 32) {
-            sp += weight64(z[i], z_max, inv_t);
-            if (y) sq += weight64(y[i], y_max, inv_t);
+        for (int block = 0; block < blocks; ++block) {
+            weights(block);
+#pragma unroll
+            for (int k = 0; k < kHeld; ++k) {
+                sp += ez[k];
+                sq += ey[k];
+            }
         }
         cluster_sum(cluster, s, sp, sq);
+        if (!y) sq = 1.0;
     };
 
-    int a = 0;
-    bool none = false;
-    RowSum zs = {}, ys = {};
-    const float *z = nullptr, *y = nullptr;
-    int d = -1;
-    bool all = false;
-    for (;; ++a) {  // (every warp of the cluster decides for itself, all alike)
-        zs = row_sum(parts, (size_t)(row0 + a), n_parts, c);
-        z = logits + (size_t)(row0 + a) * vocab;
-        all = a >= count;
-        none = zs.bad != 0.f || zs.max == -INFINITY;
-        if (all || none) break;
-        d = drafts[draft0 + a];
-        if (greedy) {
-            if (d != zs.best) break;
-            continue;
-        }
-        if (draft_logits) {
-            ys = row_sum(parts, (size_t)(rows + draft0 + a), n_parts, c);
-            y = draft_logits + (size_t)(draft0 + a) * vocab;
-            none = ys.bad != 0.f || ys.max == -INFINITY;
-            if (none) break;
-        }
-        if (d < 0 || d >= vocab) break;
-        const double u = accept_draws[draft0 + a];
-        const double ep = weight64(z[d], zs.max, inv_t), eq = y ? weight64(y[d], ys.max, inv_t) : 1.0;
-        double left = u * eq * (double)zs.sum, right = ep * (y ? (double)ys.sum : 1.0);
-        if (fabs(left - right) <= 1e-4 * right || t < 1e-29f) {
-            double sp, sq;
-            exact_sums(z, zs.max, y, ys.max, sp, sq);
-            left = u * eq * sp;
-            right = ep * (y ? sq : 1.0);
-        }
-        if (!(left < right)) break;
-    }
-    int pick = -1;
-    if (!none && greedy) {
-        pick = zs.best;
-    } else if (!none) {
-        // the distribution to draw from: p, or what of it the draft's distribution leaves
-        double sp, sq;
-        if (all) y = nullptr;
-        exact_sums(z, zs.max, y, ys.max, sp, sq);
-        const double ip = 1.0 / sp, iq = y ? 1.0 / sq : 0.0;
-        auto mass_of = [&](int i, bool plain) -> double {
-            const double p = __dmul_rn(weight64(z[i], zs.max, inv_t), ip);  // (rounded like q: equal ones leave nothing)
-            if (plain) return p;
-            if (y) return fmax(p - __dmul_rn(weight64(y[i], ys.max, inv_t), iq), 0.0);
-            return i == d ? 0.0 : p;
-        };
-        bool plain = all;
-        double mine, total, unused;
-        for (;;) {
-            mine = 0.0;
-            for (int i = begin + lane; i < end; i += 32) mine += mass_of(i, plain);
-            total = mine;
-            unused = 0.0;
-            cluster_sum(cluster, s, total, unused);
-            if (plain || total > 0.0) break;
-            plain = true;  // nothing is left: p and q are one
-        }
-        // (s.warp[0]: this CTA's warps' sums; s.cta[0] of every CTA: theirs)
-        const double target = pick_draws[b] * total;
-        double before = 0.0, held = 0.0;
-        int last = 0;  // the last CTA with any weight
-        for (int i = 0; i < kPickCtas; ++i) {
-            const double other = cluster.map_shared_rank(&s, i)->cta[0];
-            if (i < rank) before += other;
-            if (i == rank) held = other;
-            if (other > 0.0) last = i;
-        }
-        if (tid == 0) s.picked = -1;
-        __syncthreads();
-        // a draw at the very end of the sums belongs to the last id with any weight
-        const bool here = (target >= before && target < before + held) || (rank == last && target >= before + held);
-        if (here) {
-            double ahead = before;
-            int last_warp = 0;
-            for (int w = 0; w < kWarps; ++w) {
-                if (w < warp) ahead += s.warp[0][w];
-                if (s.warp[0][w] > 0.0) last_warp = w;
+    double sp = 0.0, sq = 0.0;
+    int a = 0, why = kNear;
+    bool summed = false;
+    for (int from = 0;;) {
+        for (int i = from + warp; i <= count; i += kWarps) {
+            const int how = decide(i);
+            if (how != kKept) {
+                if (lane == 0) atomicMin(&s.stop, i * 4 + how);
+                break;
             }
-            const double own = s.warp[0][warp];
-            if (own > 0.0 && ((target >= ahead && target < ahead + own) || (warp == last_warp && target >= ahead + own))) {
-                int found = -1, last_id = -1;
-                for (int i0 = begin; i0 < end && found < 0; i0 += 32) {
-                    const double m = i0 + lane < end ? mass_of(i0 + lane, plain) : 0.0;
-                    double run = m;
+        }
+        __syncthreads();
+        a = s.stop >> 2;
+        why = s.stop & 3;
+        __syncthreads();
+        if (tid == 0) s.stop = 0x7fffffff;
+        if (why != kNear) break;
+        exact_sums(a, sp, sq);  // (all CTAs of the cluster come here together)
+        const int d = drafts[draft0 + a];
+        const double eq = y ? weight64(s.table, y[d], y_max, inv_t) : 1.0;
+        if (!(accept_draws[draft0 + a] * eq * sp < weight64(s.table, z[d], z_max, inv_t) * sq)) {
+            summed = true;
+            break;
+        }
+        from = a + 1;
+    }
+    if (why == kNothing || greedy) {
+        if (rank == 0 && tid < 32) {
+            const int best = row_sum(parts, (size_t)(row0 + a), n_parts, c).best;
+            if (tid == 0) {
+                accepted[b] = a;
+                picked[b] = why == kNothing ? -1 : best;
+            }
+        }
+        return;
+    }
+    // The distribution to draw from: p, or what of it the draft's distribution leaves.
+    const bool all = a >= count;
+    const int d = all ? -1 : drafts[draft0 + a];
+    if (!summed) exact_sums(a, sp, sq);
+    const double ip = 1.0 / sp, iq = 1.0 / sq;
+    bool plain = all;
+    auto masses = [&](int block) {  // into ez
+        const int first = begin + block * 32 * kHeld + lane;
+#pragma unroll
+        for (int k = 0; k < kHeld; ++k) {
+            const double p = __dmul_rn(ez[k], ip);  // (rounded like q: equal ones leave nothing)
+            ez[k] = plain ? p : y ? fmax(p - __dmul_rn(ey[k], iq), 0.0) : first + 32 * k == d ? 0.0 : p;
+        }
+    };
+    double total, unused;
+    for (;;) {
+        total = unused = 0.0;
+        for (int block = 0; block < blocks; ++block) {
+            if (blocks > 1) weights(block);
+            masses(block);
+#pragma unroll
+            for (int k = 0; k < kHeld; ++k) total += ez[k];
+        }
+        cluster_sum(cluster, s, total, unused);
+        if (plain || total > 0.0) break;
+        plain = true;  // nothing is left: p and q are one
+        if (blocks == 1) weights(0);
+    }
+    // (s.warp[0]: this CTA's warps' sums; s.cta[0] of every CTA: theirs)
+    const double target = pick_draws[b] * total;
+    double before = 0.0, held = 0.0;
+    int last = 0;  // the last CTA with any weight
+    for (int i = 0; i < kPickCtas; ++i) {
+        const double other = cluster.map_shared_rank(&s, i)->cta[0];
+        if (i < rank) before += other;
+        if (i == rank) held = other;
+        if (other > 0.0) last = i;
+    }
+    // a draw at the very end of the sums belongs to the last id with any weight
+    if ((target >= before && target < before + held) || (rank == last && target >= before + held)) {
+        double ahead = before;
+        int last_warp = 0;
+        for (int w = 0; w < kWarps; ++w) {
+            if (w < warp) ahead += s.warp[0][w];
+            if (s.warp[0][w] > 0.0) last_warp = w;
+        }
+        const double own = s.warp[0][warp];
+        if (own > 0.0 && ((target >= ahead && target < ahead + own) || (warp == last_warp && target >= ahead + own))) {
+            int found = -1, last_id = -1;
+            for (int block = 0; block < blocks && found < 0; ++block) {
+                if (blocks > 1) {
+                    weights(block);
+                    masses(block);
+                }
+#pragma unroll
+                for (int k = 0; k < kHeld; ++k) {
+                    if (found >= 0) break;
+                    double run = ez[k];
 #pragma unroll
                     for (int o = 1; o < 32; o <<= 1) {
                         const double up = __shfl_up_sync(0xffffffffu, run, o);
                         if (lane >= o) run += up;
                     }
-                    const unsigned over = __ballot_sync(0xffffffffu, m > 0.0 && ahead + run > target);
-                    const unsigned some = __ballot_sync(0xffffffffu, m > 0.0);
-                    if (over) found = i0 + __ffs(over) - 1;
-                    if (some) last_id = i0 + 31 - __clz(some);
+                    const unsigned over = __ballot_sync(0xffffffffu, ez[k] > 0.0 && ahead + run > target);
+                    const unsigned some = __ballot_sync(0xffffffffu, ez[k] > 0.0);
+                    const int first = begin + (block * kHeld + k) * 32;
+                    if (over) found = first + __ffs(over) - 1;
+                    if (some) last_id = first + 31 - __clz(some);
                     ahead += __shfl_sync(0xffffffffu, run, 31);
                 }
-                if (lane == 0) atomicMax(&s.picked, found >= 0 ? found : last_id);
             }
+            if (lane == 0) picked[b] = found >= 0 ? found : last_id;
         }
-        __syncthreads();
-        if (here && tid == 0) picked[b] = s.picked;
-        cluster.sync();  // nobody leaves while its sums may be read
-        if (rank == 0 && tid == 0) accepted[b] = a;
-        return;
     }
-    if (rank == 0 && tid == 0) {
-        accepted[b] = a;
-        picked[b] = pick;
-    }
+    if (rank == 0 && tid == 0) accepted[b] = a;
+    cluster.sync();  // nobody leaves while its sums may be read
 }
 
 static int verify_parts(int vocab) {

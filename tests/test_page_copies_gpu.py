@@ -79,7 +79,8 @@ def test_copies_run_on_the_current_stream_and_into_graphs():
 def test_moves_that_are_refused():
     o = ops()
     k = torch.zeros((1, 4, 1, 64, 2), device=DEV)
-    for moves in ([(0, 4, 1)], [(-1, 0, 1)], [(0, 1, 65)], [(0, 1, -1)], [(0, 1, 2), (2, 1, 3)], [(0, 1, 2), (1, 2, 2)], [(1, 1, 1)]):
+    for moves in ([(0, 4, 1)], [(-1, 0, 1)], [(0, 1, 65)], [(0, 1, -1)], [(0, 1, 2), (2, 1, 3)], [(0, 1, 2), (1, 2, 2)], [(1, 1, 1)],
+                  [(0, 1)], [(0, 1, 1), (2, 3)], [(0, 1, 2.5)], [(0, 1, 2 ** 40)]):
         with pytest.raises(o.KernelError):
             o.copy_pages(k, None, moves)
     with pytest.raises(o.KernelError):
