@@ -25,9 +25,7 @@ attn_shared_any_kernel(const SharedArgs a) {
     float* p_s = kv_s + kSharedPage * ds;       // [tile, 68]
     const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
     const SharedUnit u = a.units[blockIdx.x];
-    pdl_wait();  // (the queries, and this step's keys and values, come from the kernel before)
-    pdl_launch_dependents();
-    if (u.entries <= 0) return;  // (before any barrier: the whole CTA)
+    units_begin(a);
     const int hk = blockIdx.y, G = a.nq / a.nkv;
     const int* members = a.members + u.members;
     const int pos = u.ends ? a.token_pos[members[u.entry / G]] : 0x7fffffff;
@@ -141,68 +139,22 @@ attn_shared_any_kernel(const SharedArgs a) {
         for (int j = 0; j < NJ; ++j)
             if (tx + 16 * j < d) a.partial[rec * d + tx + 16 * j] = o[r][j];
     }
+    if (a.tickets) merge_finished<T, kAnyThreads>(a, u, hk, G, reinterpret_cast<int*>(p_s));
+    units_end(a);
 }
 
-// A warp per (token row, head): lane s holds the weights of records s, s + 32, ...; every lane sums its pairs of values over the
-// records in their order, eight records asked for at a time.  A row without records (a padding row), or none of whose
-// records holds a key, is zero.
+// A warp per (token row, head).
 template <typename T>
 __global__ void __launch_bounds__(128)
 attn_shared_merge_kernel(const float* __restrict__ partial, const float2* __restrict__ sums, const int* __restrict__ record,
                          T* __restrict__ out, int n_tokens, int nq, int d) {
-    const int lane = threadIdx.x & 31;
     const size_t at = (size_t)blockIdx.x * 4 + (threadIdx.x >> 5);
     if (at >= (size_t)n_tokens * nq) return;
-    const int row = (int)(at / nq), head = (int)(at % nq);
-    const int first = record[row], count = record[row + 1] - first;
+    const int row = (int)(at / nq), first = record[row];
+    const int count = record[row + 1] - first;
     pdl_wait();
     pdl_launch_dependents();
-    const size_t rec = (size_t)first * nq + head;
-    float m = -INFINITY;
-    for (int s = lane; s < count; s += 32) {
-        const float2 x = sums[rec + (size_t)s * nq];
-        if (x.y != 0.f) m = fmaxf(m, x.x);
-    }
-    m = warp_max(m);
-    float2 acc[4] = {};
-    float l = 0.f;
-    constexpr int kAhead = 8;
-    for (int s0 = 0; s0 < count; s0 += 32) {
-        float w = 0.f;
-        if (s0 + lane < count) {
-            const float2 x = sums[rec + (size_t)(s0 + lane) * nq];
-            w = x.y != 0.f ? exp2f(x.x - m) : 0.f;
-            l += x.y * w;
-        }
-        const int here = min(32, count - s0);
-        for (int s = 0; s < here; s += kAhead) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if (j * 64 >= d) break;
-                const int i = 2 * (lane + 32 * j);
-                float2 v[kAhead];
-#pragma unroll
-                for (int k = 0; k < kAhead; ++k)
-                    v[k] = s + k < here && i < d ? *reinterpret_cast<const float2*>(partial + (rec + (size_t)(s0 + s + k) * nq) * d + i)
-                                                 : make_float2(0.f, 0.f);
-#pragma unroll
-                for (int k = 0; k < kAhead; ++k) {
-                    const float f = __shfl_sync(0xffffffffu, w, (s + k) & 31);
-                    if (s + k < here && f != 0.f) {  // (a record that holds nothing is never added)
-                        acc[j].x = fmaf(f, v[k].x, acc[j].x);
-                        acc[j].y = fmaf(f, v[k].y, acc[j].y);
-                    }
-                }
-            }
-        }
-    }
-    l = warp_sum(l);
-    const float inv = l != 0.f ? 1.0f / l : 0.f;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const int i = 2 * (lane + 32 * j);
-        if (i < d) store2(out + at * d + i, acc[j].x * inv, acc[j].y * inv);
-    }
+    merge_row<T, 8>(partial, sums, first, count, row, (int)(at % nq), nq, d, out);
 }
 
 template <typename T, int ROWS, int NJ>
@@ -234,10 +186,11 @@ cudaError_t shared_units_any(const SharedArgs& a, int n_units, int tile, bool f3
 // bfloat16): at most 16, at most 64 entries, none; `form` 1 (bfloat16, heads of 64 and 128): none, at most 32, at most 128, the last
 // of which cover only positions that all their rows see.  The plan (units, members, record) is the host's, made of
 // page lists that the call's page table agrees with; page ids outside the store hold no keys.  partial: records x nq x d floats,
-// sums: records x nq x 2.
+// sums: records x nq x 2.  tickets (n_tokens x nq counters, zero, left zero): every row is merged by the CTA that completes it, and no
+// merge is launched (where there is no unit of the third kind); every row then has a record.
 NNIS_API int nnis_attention_shared(const void* q, int q_stride, const void* k_cache, const void* v_cache, const int* token_pos,
                                    const int* page_table, int table_cols, const int* units, int n0, int n1, int n2,
-                                   const int* members, const int* record, float* partial, float* sums, void* out, int n_tokens,
+                                   const int* members, const int* record, float* partial, float* sums, unsigned* tickets, void* out, int n_tokens,
                                    int nq, int nkv, int d, int pages, int page_size, float scale, int dtype, int form, int* status,
                                    cudaStream_t stream) {
     using namespace nnis;
@@ -247,12 +200,12 @@ NNIS_API int nnis_attention_shared(const void* q, int q_stride, const void* k_ca
     if (page_size != kSharedPage || d < 2 || d > 256 || d % 2 || nkv > 65535) return NNIS_ERR_UNSUPPORTED;
     const bool f32 = dtype == NNIS_DTYPE_F32;
     if (form == 1 && (f32 || (d != 64 && d != 128) || n0)) return NNIS_ERR_UNSUPPORTED;
-    if (form != 1 && n2) return NNIS_ERR_UNSUPPORTED;
+    if (n2 && (form != 1 || tickets)) return NNIS_ERR_UNSUPPORTED;
     if ((uintptr_t)units % 16 || (uintptr_t)partial % 16 || (uintptr_t)sums % 8) return NNIS_ERR_ALIGNMENT;
     const uintptr_t all = (uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache;
     if (all % (form == 1 ? 16 : f32 ? 8 : 4) || (uintptr_t)out % (f32 ? 8 : 4) || (form == 1 && q_stride % 8)) return NNIS_ERR_ALIGNMENT;
     SharedArgs a = {q,       k_cache, v_cache, token_pos, page_table, reinterpret_cast<const SharedUnit*>(units), members, record,
-                    partial, sums,    q_stride, table_cols, pages,    nq, nkv, d, scale};
+                    partial, sums,    tickets, out,       q_stride,   table_cols, pages,   nq,     nkv, d, scale, 0};
     // (the large units first: the small ones end what is left of the device)
     const SharedUnit* first = a.units;
     for (int kind = 2; kind >= 0; --kind) {
@@ -263,7 +216,9 @@ NNIS_API int nnis_attention_shared(const void* q, int q_stride, const void* k_ca
                               : kind == 2 ? shared_units_tc(a, n, status, stream)
                                           : shared_units_mma(a, n, stream);
         if (e != cudaSuccess) return (int)e;
+        a.beside = 1;
     }
+    if (tickets) return NNIS_OK;
     const unsigned ctas = (unsigned)(((size_t)n_tokens * nq + 3) / 4);
     const float2* held = reinterpret_cast<const float2*>(sums);
     const cudaError_t e =

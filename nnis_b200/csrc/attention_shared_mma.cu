@@ -33,9 +33,7 @@ attn_shared_mma_kernel(const SharedArgs a) {
     const SharedUnit u = a.units[blockIdx.x];
     const int hk = blockIdx.y, G = a.nq / a.nkv;
     const int* members = a.members + u.members;
-    pdl_wait();  // (the queries, and this step's keys and values, come from the kernel before)
-    pdl_launch_dependents();
-    if (u.entries <= 0) return;
+    units_begin(a);
     const bool two = u.entries > 16;  // the second tile of 16 entries holds any
     const int pos = u.ends ? a.token_pos[members[u.entry / G]] : 0x7fffffff;
     const int n_pages = (u.ends ? min(u.page_end, pos < 0 ? 0 : pos / kSharedPage + 1) : u.page_end) - u.page_begin;
@@ -213,6 +211,8 @@ attn_shared_mma_kernel(const SharedArgs a) {
             *reinterpret_cast<float4*>(a.partial + rec * D + c * 4) = x;
         }
     }
+    if (a.tickets) merge_finished<bf16, kSmThreads>(a, u, hk, G, reinterpret_cast<int*>(q_s));
+    units_end(a);
 }
 
 template <int D>

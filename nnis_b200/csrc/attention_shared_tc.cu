@@ -104,8 +104,7 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     const SharedUnit u = a.units[blockIdx.x];
     const int hk = blockIdx.y, G = a.nq / a.nkv;
     const int n_pages = u.entries > 0 ? u.page_end - u.page_begin : 0;
-    pdl_wait();  // (queries, keys and values come from the kernel before; the set-up above ran under it)
-    pdl_launch_dependents();
+    units_begin(a);  // (queries, keys and values come from the kernel before; the set-up above ran under it)
 
     if (n_pages <= 0) {
     } else if (warp == 0) {

@@ -431,7 +431,7 @@ def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, first_row: torch.T
             return verify_drafts(logits, drafts, first_row, temperatures, accept_draws, pick_draws, accepted, picked,
                                  draft_logits, workspace)
     need = _entry("nnis_verify_scratch", _I, _I, _I)(rows, drafted, vocab)
-    scratch = workspace.get("verify_sums", (need // 4,), f32)
+    scratch = workspace.room("verify_sums", need // 4, f32)
     _check(_entry("nnis_verify_drafts", _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _P, _P, _P)(
         logits.data_ptr(), draft_logits.data_ptr() if draft_logits is not None and drafted else None, drafts.data_ptr(),
         first_row.data_ptr(), temperatures.data_ptr(), accept_draws.data_ptr(), pick_draws.data_ptr(), scratch.data_ptr(), b, rows,
@@ -2846,7 +2846,10 @@ class SharedPlan:
         self.counts, self.ints, self.records, self.seqs, self.cols, self.form = counts, ints, records, seqs, cols, form
         units, members = 8 * sum(counts), ints.numel() - 8 * sum(counts) - rows - 1
         self.units, self.members, self.record = ints.data_ptr(), ints.data_ptr() + 4 * units, ints.data_ptr() + 4 * (units + members)
-        self.device, self.status, self.launches = ints.device, status_word(ints.device).data_ptr(), 1 + sum(c > 0 for c in counts)
+        # rows merged by the CTA that completes them save a launch, where a CTA has few of them to merge
+        self.merged_inside = counts[2] == 0 and sum(counts) * kv_heads <= 148 and records <= 4 * rows
+        self.device, self.status = ints.device, status_word(ints.device).data_ptr()
+        self.launches = (not self.merged_inside) + sum(c > 0 for c in counts)
 
 
 def attention_shared_takes(head_dim: int, page_size: int) -> bool:
@@ -2871,8 +2874,9 @@ def attention_shared_plan(tables, seqs, positions, heads: int, kv_heads: int, he
     device = torch.device(device)
     tensor = dtype == torch.bfloat16 and head_dim in (64, 128)  # (the forms on the tensor cores)
     sms = sm_count(device)
-    kinds, members, record = shared_units(nodes, tails, seqs, heads // kv_heads, kv_heads, *(
-        ((0, 32, 128), (0.0, 1.0, 1.0), 1, 2 * sms, 2) if tensor else ((16, 64, 0), (1.0, 2.0, 0.0), 1, 4 * sms, 2)))
+    kinds, members, record = shared_units(nodes, tails, seqs, heads // kv_heads, kv_heads, (
+        ((0, 0, 0, 0), (32, 6 * sms, 2, 16), (128, 2 * sms, 2, 1 << 20)) if tensor else
+        ((16, 4 * sms, 2, 16), (64, 4 * sms, 2, 16), (0, 0, 0, 0))), 1)
     ints = np.concatenate([k.reshape(-1) for k in kinds] + [members, record]).astype(np.int32)
     return SharedPlan(n, heads, kv_heads, head_dim, dtype, [len(k) for k in kinds], torch.from_numpy(ints).to(device),
                       int(record[-1]), 1 + max(seqs), max([p // page + 1 for p in positions] + [1]), int(tensor))
@@ -2905,11 +2909,12 @@ def attention_shared(q: torch.Tensor, q_stride: int, k_cache: torch.Tensor, v_ca
             return attention_shared(q, q_stride, k_cache, v_cache, token_pos, page_table, plan, out, heads, kv_heads, head_dim,
                                     scale, workspace)
     held = max(1, plan.records) * heads
-    at = workspace.get("attn_shared_records", (held, d + 2), torch.float32).data_ptr()
+    at = workspace.room("attn_shared_records", held * (d + 2), torch.float32).data_ptr()
+    tickets = workspace.zeros_room("attn_shared_tickets", n * heads, torch.int32).data_ptr() if plan.merged_inside else None
     n0, n1, n2 = plan.counts
-    _check(_entry("nnis_attention_shared", _P, _I, _P, _P, _P, _P, _I, _P, _I, _I, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I,
-                  _F, _I, _I, _P, _P)(
+    _check(_entry("nnis_attention_shared", _P, _I, _P, _P, _P, _P, _I, _P, _I, _I, _I, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I,
+                  _I, _F, _I, _I, _P, _P)(
         q.data_ptr(), q_stride, k_cache.data_ptr(), v_cache.data_ptr(), token_pos.data_ptr(), page_table.data_ptr(),
-        page_table.shape[1], plan.units, n0, n1, n2, plan.members, plan.record, at, at + 4 * held * d, out.data_ptr(), n, heads,
-        kv_heads, d, shape[0], 64, scale, F32 if dtype == torch.float32 else BF16, plan.form, plan.status, _stream_here()),
+        page_table.shape[1], plan.units, n0, n1, n2, plan.members, plan.record, at, at + 4 * held * d, tickets, out.data_ptr(), n,
+        heads, kv_heads, d, shape[0], 64, scale, F32 if dtype == torch.float32 else BF16, plan.form, plan.status, _stream_here()),
         "attention_shared", plan.launches)

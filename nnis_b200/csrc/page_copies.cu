@@ -10,16 +10,17 @@
 
 namespace nnis {
 
-constexpr int kMoves = 1024;  // of a launch: 12 KB of parameters
+constexpr int kMoves = 1024, kFewMoves = 32;  // of a launch: 12 KB of parameters, 384 bytes (2 us of the host less)
 
+template <int N>
 struct PageMoves {
-    int src[kMoves], dst[kMoves], rows[kMoves];
+    int src[N], dst[N], rows[N];
 };
 
 // A CTA: some words of one run.  blockIdx: x = move and which of k and v, y = layer, z = a share of the run(s).
-template <typename W>
+template <typename W, int N>
 __global__ void __launch_bounds__(256)
-copy_pages_kernel(const __grid_constant__ PageMoves moves, void* k, void* v, int pages, int kv_heads, int page_size, int k_row,
+copy_pages_kernel(const __grid_constant__ PageMoves<N> moves, void* k, void* v, int pages, int kv_heads, int page_size, int k_row,
                   int v_row) {
     const int move = v ? blockIdx.x >> 1 : blockIdx.x;
     const bool values = v && (blockIdx.x & 1);
@@ -50,6 +51,33 @@ copy_pages_kernel(const __grid_constant__ PageMoves moves, void* k, void* v, int
     }
 }
 
+// One launch of at most N moves.
+template <int N>
+static cudaError_t launch_moves(void* k, void* v, int layers, int pages, int kv_heads, int page_size, int k_row, int v_row,
+                                const int* src, const int* dst, const int* rows, int n, int sms, cudaStream_t stream) {
+    PageMoves<N> p;
+    int most = 1;
+    for (int i = 0; i < n; ++i) {
+        p.src[i] = src[i];
+        p.dst[i] = dst[i];
+        p.rows[i] = rows[i];
+        most = rows[i] > most ? rows[i] : most;
+    }
+    const bool wide = ((uintptr_t)k | (uintptr_t)v | (uintptr_t)k_row | (uintptr_t)(v ? v_row : 0)) % 16 == 0;
+    const int unit = wide ? 16 : 4, tensors = v ? 2 : 1;
+    const long long words = (long long)kv_heads * most * (k_row > v_row ? k_row : v_row) / unit;
+    const long long ctas = (long long)n * tensors * layers;
+    long long share = (words + 1023) / 1024;                // four words a thread
+    const long long fill = (16LL * sms + ctas - 1) / ctas;  // ... unless there are CTAs enough
+    if (share > fill) share = fill;
+    if (share < 1) share = 1;
+    if (share > 65535) share = 65535;
+    const dim3 grid((unsigned)(n * tensors), (unsigned)layers, (unsigned)share);
+    if (wide) copy_pages_kernel<uint4, N><<<grid, 256, 0, stream>>>(p, k, v, pages, kv_heads, page_size, k_row / 16, v_row / 16);
+    else copy_pages_kernel<uint32_t, N><<<grid, 256, 0, stream>>>(p, k, v, pages, kv_heads, page_size, k_row / 4, v_row / 4);
+    return cudaGetLastError();
+}
+
 }  // namespace nnis
 
 // k and v (or null): [layers, pages, kv_heads, page_size, row] with rows of `k_row` and `v_row` bytes, multiples of 4.
@@ -78,33 +106,11 @@ NNIS_API int nnis_copy_pages(void* k, void* v, int layers, int pages, int kv_hea
     }
     free(seen);
     if (!good) return NNIS_ERR_ARGUMENT;
-    const bool wide = ((uintptr_t)k | (uintptr_t)v | (uintptr_t)k_row | (uintptr_t)(v ? v_row : 0)) % 16 == 0;
-    const int unit = wide ? 16 : 4;
-    const int tensors = v ? 2 : 1;
-    static PageMoves none = {};
     for (int first = 0; first < count; first += kMoves) {
-        PageMoves p = none;
         const int n = count - first < kMoves ? count - first : kMoves;
-        int most = 1;
-        for (int i = 0; i < n; ++i) {
-            p.src[i] = src[first + i];
-            p.dst[i] = dst[first + i];
-            p.rows[i] = rows[first + i];
-            most = p.rows[i] > most ? p.rows[i] : most;
-        }
-        const long long words = (long long)kv_heads * most * (k_row > v_row ? k_row : v_row) / unit;
-        const long long ctas = (long long)n * tensors * layers;
-        long long share = (words + 1023) / 1024;                          // four words a thread
-        const long long fill = (16LL * sms + ctas - 1) / ctas;            // ... unless there are CTAs enough
-        if (share > fill) share = fill;
-        if (share < 1) share = 1;
-        if (share > 65535) share = 65535;
-        const dim3 grid((unsigned)(n * tensors), (unsigned)layers, (unsigned)share);
-        if (wide)
-            copy_pages_kernel<uint4><<<grid, 256, 0, stream>>>(p, k, v, pages, kv_heads, page_size, k_row / 16, v_row / 16);
-        else
-            copy_pages_kernel<uint32_t><<<grid, 256, 0, stream>>>(p, k, v, pages, kv_heads, page_size, k_row / 4, v_row / 4);
-        const cudaError_t e = cudaGetLastError();
+        auto launch = n <= kFewMoves ? launch_moves<kFewMoves> : launch_moves<kMoves>;
+        const cudaError_t e = launch(k, v, layers, pages, kv_heads, page_size, k_row, v_row, src + first, dst + first, rows + first, n,
+                                     sms, stream);
         if (e != cudaSuccess) return (int)e;
     }
     return NNIS_OK;

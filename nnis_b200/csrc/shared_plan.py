@@ -42,6 +42,8 @@ def shared_nodes(tables: Sequence[Sequence[int]], seqs: Sequence[int], positions
         if end > depth:
             tails.append((row, depth, end))
 
+    # (a padding row has a tail of no pages: the unit that writes its zeros)
+    tails += [(r, 0, 0) for r in range(len(seqs)) if positions[r] < 0]
     work = [([r for r in range(len(seqs)) if positions[r] >= 0], 0)]
     while work:
         rows, depth = work.pop()
@@ -72,31 +74,32 @@ def shared_nodes(tables: Sequence[Sequence[int]], seqs: Sequence[int], positions
 
 
 def shared_units(nodes: Sequence[tuple], tails: Sequence[tuple], seqs: Sequence[int], group: int, kv_heads: int,
-                 tiles: Sequence[int], costs: Sequence[float], ending: int, ctas: int, least: int):
+                 kinds: Sequence[tuple], ending: int):
     """(units of every kind [*, 8], members, record offsets [rows + 1]).
 
-    ``tiles``: most entries of a unit of each kind, ascending (0: the kernel has no such kind); ``costs``: what a page costs a
-    unit of the kind, beside one another; ``ending``: the last kind that takes units whose rows end inside them; ``ctas``:
-    how many units fill the device; ``least``: fewest pages of a chunk."""
+    ``kinds``: (most entries of a unit, CTAs of the kind that the device should be given, fewest and most pages of a chunk),
+    entries ascending, 0 where the kernel has no such kind; ``ending``: the last kind that takes units whose rows end inside
+    them."""
     pieces = []  # (rows, first, end, ends, kind)
-    total = 0.0
+    total = [0] * len(kinds)
     for rows, a, b, ends in [(*n, 0) for n in nodes] + [([r], a, b, 1) for r, a, b in tails]:
         entries = len(rows) * group
-        kinds = [i for i, t in enumerate(tiles) if t and (not ends or i <= ending)]
-        kind = next((i for i in kinds if entries <= tiles[i]), kinds[-1])
+        may = [i for i, k in enumerate(kinds) if k[0] and (not ends or i <= ending)]
+        kind = next((i for i in may if entries <= kinds[i][0]), may[-1])
         pieces.append((rows, a, b, ends, kind))
-        total += -(-entries // tiles[kind]) * costs[kind] * (b - a)
-    goal = max(total * kv_heads / max(1, ctas), 1.0)  # cost of a unit
-    units: List[List[tuple]] = [[] for _ in tiles]
+        total[kind] += -(-entries // kinds[kind][0]) * (b - a) * kv_heads
+    # pages of a chunk: as many as leave every CTA of the kind the same share
+    share = [min(k[3], max(k[2], -(-t // max(1, k[1])))) if k[0] else 1 for k, t in zip(kinds, total)]
+    units: List[List[tuple]] = [[] for _ in kinds]
     members: List[int] = []
     slots = [0] * len(seqs)
     for rows, a, b, ends, kind in pieces:
-        entries, tile = len(rows) * group, tiles[kind]
-        chunks = max(1, -(-(b - a) // max(least, int(goal / costs[kind] + 0.5))))
-        per = -(-(b - a) // chunks)
+        entries, tile = len(rows) * group, kinds[kind][0]
+        chunks = max(1, -(-(b - a) // share[kind]))
+        per = max(1, -(-(b - a) // chunks))
         at, slot = len(members), slots[rows[0]]
         members.extend(rows)
-        for c in range(a, b, per):
+        for c in range(a, b, per) if b > a else (a,):
             for e in range(0, entries, tile):
                 units[kind].append((at, e, min(tile, entries - e), c, min(b, c + per), slot, seqs[rows[0]], ends))
             slot += 1

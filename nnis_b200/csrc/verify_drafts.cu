@@ -31,7 +31,7 @@ constexpr int kVerifyParts = 32;     // most CTAs a row
 constexpr int kPickThreads = 512;
 constexpr int kPickCtas = 8;         // of a cluster
 
-struct RowSum {
+struct __align__(16) RowSum {
     float max, sum;  // maximum logit, sum of exp((x - max) / T): no number where a logit is none, or +infinity
     int best;        // id of the maximum, the lower among equals
 };
@@ -150,9 +150,9 @@ verify_rows_kernel(const float* __restrict__ logits, const float* __restrict__ d
 __device__ __forceinline__ RowSum row_sum(const RowSum* __restrict__ parts, size_t row, int n_parts, float c) {
     const int lane = threadIdx.x & 31;
     RowSum mine = {-INFINITY, 0.f, 0x7fffffff};
-    if (lane < n_parts) mine = parts[row * n_parts + lane];
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
+    const int part = n_parts <= 8 ? lane & 7 : lane;  // (few parts: each eighth of the warp joins them all)
+    if (part < n_parts) mine = parts[row * n_parts + part];
+    for (int o = n_parts <= 8 ? 4 : 16; o > 0; o >>= 1) {
         RowSum other;
         other.max = __shfl_xor_sync(0xffffffffu, mine.max, o);
         other.sum = __shfl_xor_sync(0xffffffffu, mine.sum, o);
@@ -184,56 +184,62 @@ __device__ __forceinline__ double weight64(const double* table, float x, float m
     return __hiloint2double(__double2hiint(w) + (n >> 6) * (1 << 20), __double2loint(w));
 }
 
+constexpr int kPickWarps = kPickThreads / 32;
+
 struct PickShared {
-    double table[64];    // 2^(j / 64)
-    double warp[2][kPickThreads / 32];
-    double cta[2];       // this CTA's sums, read by the others of its cluster
-    int picked, stop;
+    double table[64];                // 2^(j / 64)
+    double warp[2][kPickWarps];
+    double cta[2][2][kPickCtas];     // every CTA's sums, written by them: [turn][which][rank]
+    float row_max[2][kPickWarps];    // of the row at which a warp stopped
+    int stop;
 };
 
-// Sum over the whole cluster of up to two values a thread, every thread gets both.
-__device__ __forceinline__ void cluster_sum(cg::cluster_group cluster, PickShared& s, double& a, double& b) {
+// Sum over the whole cluster of up to two values a thread, every thread gets both.  Each CTA tells all others its sums, in
+// one of two places by turns: a place is written again only when everybody has met once more.
+__device__ __forceinline__ void cluster_sum(cg::cluster_group cluster, PickShared& s, int turn, double& a, double& b) {
+    const int lane = threadIdx.x & 31;
     a = warp_sum64(a);
     b = warp_sum64(b);
-    if ((threadIdx.x & 31) == 0) {
+    if (lane == 0) {
         s.warp[0][threadIdx.x >> 5] = a;
         s.warp[1][threadIdx.x >> 5] = b;
     }
     __syncthreads();
-    if (threadIdx.x == 0) {
-        double x = 0.0, y = 0.0;
-        for (int w = 0; w < kPickThreads / 32; ++w) {
-            x += s.warp[0][w];
-            y += s.warp[1][w];
+    const int ctas = (int)cluster.num_blocks();
+    if (threadIdx.x < 32) {
+        a = warp_sum64(lane < kPickWarps ? s.warp[0][lane] : 0.0);
+        b = warp_sum64(lane < kPickWarps ? s.warp[1][lane] : 0.0);
+        if (lane < 2 * ctas) {
+            PickShared* other = cluster.map_shared_rank(&s, lane >> 1);
+            other->cta[turn][lane & 1][cluster.block_rank()] = lane & 1 ? b : a;
         }
-        s.cta[0] = x;
-        s.cta[1] = y;
     }
     cluster.sync();
     a = b = 0.0;
-    for (unsigned i = 0; i < cluster.num_blocks(); ++i) {
-        const PickShared* other = cluster.map_shared_rank(&s, i);
-        a += other->cta[0];
-        b += other->cta[1];
+    for (int i = 0; i < ctas; ++i) {
+        a += s.cta[turn][0][i];
+        b += s.cta[turn][1][i];
     }
-    cluster.sync();
 }
 
-__global__ void __launch_bounds__(kPickThreads, 1) __cluster_dims__(kPickCtas, 1, 1)
+__global__ void __launch_bounds__(kPickThreads, 2)
 verify_pick_kernel(const float* __restrict__ logits, const float* __restrict__ draft_logits, const int* __restrict__ drafts,
                    const int* __restrict__ first_row, const float* __restrict__ temperature, const double* __restrict__ accept_draws,
                    const double* __restrict__ pick_draws, const RowSum* __restrict__ parts, int n_parts, int rows, int vocab,
                    int* __restrict__ accepted, int* __restrict__ picked) {
     __shared__ PickShared s;
     cg::cluster_group cluster = cg::this_cluster();
-    const int b = blockIdx.y, rank = (int)cluster.block_rank();
+    const int b = blockIdx.y, rank = (int)cluster.block_rank(), ctas = (int)cluster.num_blocks();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    constexpr int kWarps = kPickThreads / 32;
     if (tid < 64) s.table[tid] = exp2((double)tid * (1.0 / 64.0));
     if (tid == 0) s.stop = 0x7fffffff;
+    const int row0 = first_row[b], draft0 = row0 - b, count = first_row[b + 1] - row0 - 1;
+    const float t = temperature[b];
+    const bool greedy = !(t > 0.f);
+    const float c = scale_of(t);
+    const double inv_t = greedy ? 1.0 : 1.0 / (double)t;
     pdl_wait();
     pdl_launch_dependents();
-    const int row0 = first_row[b], draft0 = row0 - b, count = first_row[b + 1] - row0 - 1;
     if (row0 < b || count < 0 || row0 + count >= rows) {  // (offsets that no packed rows have: the whole cluster leaves)
         if (rank == 0 && tid == 0) {
             accepted[b] = 0;
@@ -241,85 +247,81 @@ verify_pick_kernel(const float* __restrict__ logits, const float* __restrict__ d
         }
         return;
     }
-    __syncthreads();
-    const float t = temperature[b];
-    const bool greedy = !(t > 0.f);
-    const float c = scale_of(t);
-    const double inv_t = greedy ? 1.0 : 1.0 / (double)t;
+    cluster.sync();  // (all of the cluster run: their shared memory may be written)
 
     // The drafts, a warp each: where the first one lies that is not kept for sure, and why (every CTA of the cluster for
     // itself, all alike).
     enum { kKept, kRefused, kNothing, kNear };
     auto decide = [&](int i) -> int {
-        const RowSum zs = row_sum(parts, (size_t)(row0 + i), n_parts, c);
-        if (!(zs.sum >= 0.f) || zs.max == -INFINITY || zs.max == INFINITY) return kNothing;
-        if (i >= count) return kRefused;
-        const int d = drafts[draft0 + i];
-        if (greedy) return d == zs.best ? kKept : kRefused;
+        const bool drafted = i < count, other = drafted && draft_logits && !greedy;
+        const int d = drafted ? drafts[draft0 + i] : -1;
+        const double u = drafted ? accept_draws[draft0 + i] : 0.0;
         const bool known = d >= 0 && d < vocab;
-        double eq = 1.0, sum_q = 1.0;
-        if (draft_logits) {
-            const RowSum ys = row_sum(parts, (size_t)(rows + draft0 + i), n_parts, c);
-            if (!(ys.sum >= 0.f) || ys.max == -INFINITY || ys.max == INFINITY) return kNothing;
-            if (known) eq = weight64(s.table, draft_logits[(size_t)(draft0 + i) * vocab + d], ys.max, inv_t);
-            sum_q = (double)ys.sum;
+        const float zd = known ? logits[(size_t)(row0 + i) * vocab + d] : 0.f;
+        const float yd = known && other ? draft_logits[(size_t)(draft0 + i) * vocab + d] : 0.f;
+        const RowSum zs = row_sum(parts, (size_t)(row0 + i), n_parts, c);
+        RowSum ys = {0.f, 1.f, 0};
+        if (other) ys = row_sum(parts, (size_t)(rows + draft0 + i), n_parts, c);
+        if (lane == 0) {
+            s.row_max[0][warp] = zs.max;
+            s.row_max[1][warp] = ys.max;
         }
+        if (!(zs.sum >= 0.f) || zs.max == -INFINITY || zs.max == INFINITY) return kNothing;
+        if (!drafted) return kRefused;
+        if (greedy) return d == zs.best ? kKept : kRefused;
+        if (!(ys.sum >= 0.f) || ys.max == -INFINITY || ys.max == INFINITY) return kNothing;
         if (!known) return kRefused;
-        const double left = accept_draws[draft0 + i] * eq * (double)zs.sum;
-        const double right = weight64(s.table, logits[(size_t)(row0 + i) * vocab + d], zs.max, inv_t) * sum_q;
+        const double eq = other ? weight64(s.table, yd, ys.max, inv_t) : 1.0;
+        const double left = u * eq * (double)zs.sum, right = weight64(s.table, zd, zs.max, inv_t) * (double)ys.sum;
         if (fabs(left - right) <= 1e-4 * right || t < 1e-29f) return kNear;
         return left < right ? kKept : kRefused;
     };
-    // The ids of a warp lie together, lane by lane; a lane's weights of a row stay in registers where one block holds them.
-    constexpr int kHeld = 16;
-    const int per_warp = (((vocab + kPickCtas * kWarps - 1) / (kPickCtas * kWarps)) + 31) & ~31;
-    const int begin = min(vocab, (rank * kWarps + warp) * per_warp), end = min(vocab, begin + per_warp);
-    const int blocks = (per_warp + 32 * kHeld - 1) / (32 * kHeld);  // (one up to 65,536 ids)
-    double ez[kHeld], ey[kHeld];
+    // A warp's ids lie together, 32 at a time.  Nothing of a row is kept between the two walks over it: it comes from L1
+    // again, and without the registers two CTAs are on an SM, so that one walks while the other meets its cluster.
+    const int per_warp = (((vocab + ctas * kPickWarps - 1) / (ctas * kPickWarps)) + 31) & ~31;
+    const int begin = min(vocab, (rank * kPickWarps + warp) * per_warp), end = min(vocab, begin + per_warp);
+    constexpr int kAhead = 4;
     const float *z = nullptr, *y = nullptr;
     float z_max = 0.f, y_max = 0.f;
-    auto weights = [&](int block) {
-        float xz[kHeld], xy[kHeld];
-        const int first = begin + block * 32 * kHeld + lane;
+    auto weights = [&](int first, double (&ez)[kAhead], double (&ey)[kAhead]) {  // of ids first, first + 32, ...
+        float xz[kAhead], xy[kAhead];
 #pragma unroll
-        for (int k = 0; k < kHeld; ++k) {
+        for (int k = 0; k < kAhead; ++k) {
             const int i = first + 32 * k;
             xz[k] = i < end ? z[i] : -INFINITY;
             xy[k] = y && i < end ? y[i] : -INFINITY;
         }
 #pragma unroll
-        for (int k = 0; k < kHeld; ++k) {
-            if (32 * k >= per_warp) {  // (nobody's)
-                ez[k] = ey[k] = 0.0;
-                continue;
-            }
+        for (int k = 0; k < kAhead; ++k) {
             ez[k] = weight64(s.table, xz[k], z_max, inv_t);
             ey[k] = y ? weight64(s.table, xy[k], y_max, inv_t) : 0.0;
         }
     };
-    auto exact_sums = [&](int i, double& sp, double& sq) {  // of row i, in 64 bits
+    int turn = 0;
+    double sp = 0.0, sq = 0.0;
+    auto exact_sums = [&](int i, int stopped) {  // of row i, at which warp `stopped` stopped, in 64 bits
         z = logits + (size_t)(row0 + i) * vocab;
-        z_max = row_sum(parts, (size_t)(row0 + i), n_parts, c).max;
         y = draft_logits && i < count ? draft_logits + (size_t)(draft0 + i) * vocab : nullptr;
-        if (y) y_max = row_sum(parts, (size_t)(rows + draft0 + i), n_parts, c).max;
+        z_max = s.row_max[0][stopped];
+        y_max = s.row_max[1][stopped];
         sp = sq = 0.0;
-        for (int block = 0; block < blocks; ++block) {
-            weights(block);
+        for (int i0 = begin + lane; i0 < end; i0 += 32 * kAhead) {
+            double ez[kAhead], ey[kAhead];
+            weights(i0, ez, ey);
 #pragma unroll
-            for (int k = 0; k < kHeld; ++k) {
+            for (int k = 0; k < kAhead; ++k) {
                 sp += ez[k];
                 sq += ey[k];
             }
         }
-        cluster_sum(cluster, s, sp, sq);
+        cluster_sum(cluster, s, turn, sp, sq);
+        turn ^= 1;
         if (!y) sq = 1.0;
     };
 
-    double sp = 0.0, sq = 0.0;
     int a = 0, why = kNear;
-    bool summed = false;
     for (int from = 0;;) {
-        for (int i = from + warp; i <= count; i += kWarps) {
+        for (int i = from + warp; i <= count; i += kPickWarps) {
             const int how = decide(i);
             if (how != kKept) {
                 if (lane == 0) atomicMin(&s.stop, i * 4 + how);
@@ -329,22 +331,20 @@ verify_pick_kernel(const float* __restrict__ logits, const float* __restrict__ d
         __syncthreads();
         a = s.stop >> 2;
         why = s.stop & 3;
-        __syncthreads();
-        if (tid == 0) s.stop = 0x7fffffff;
+        if (why == kNothing || greedy) break;
+        exact_sums(a, (a - from) % kPickWarps);  // (all CTAs of the cluster come here together)
         if (why != kNear) break;
-        exact_sums(a, sp, sq);  // (all CTAs of the cluster come here together)
         const int d = drafts[draft0 + a];
         const double eq = y ? weight64(s.table, y[d], y_max, inv_t) : 1.0;
-        if (!(accept_draws[draft0 + a] * eq * sp < weight64(s.table, z[d], z_max, inv_t) * sq)) {
-            summed = true;
-            break;
-        }
+        if (!(accept_draws[draft0 + a] * eq * sp < weight64(s.table, z[d], z_max, inv_t) * sq)) break;
+        if (tid == 0) s.stop = 0x7fffffff;  // (everybody has read it: they have met)
+        __syncthreads();
         from = a + 1;
     }
     if (why == kNothing || greedy) {
-        if (rank == 0 && tid < 32) {
+        if (rank == 0 && warp == 0) {
             const int best = row_sum(parts, (size_t)(row0 + a), n_parts, c).best;
-            if (tid == 0) {
+            if (lane == 0) {
                 accepted[b] = a;
                 picked[b] = why == kNothing ? -1 : best;
             }
@@ -354,79 +354,74 @@ verify_pick_kernel(const float* __restrict__ logits, const float* __restrict__ d
     // The distribution to draw from: p, or what of it the draft's distribution leaves.
     const bool all = a >= count;
     const int d = all ? -1 : drafts[draft0 + a];
-    if (!summed) exact_sums(a, sp, sq);
+    const double draw = pick_draws[b];
     const double ip = 1.0 / sp, iq = 1.0 / sq;
     bool plain = all;
-    auto masses = [&](int block) {  // into ez
-        const int first = begin + block * 32 * kHeld + lane;
+    auto masses = [&](int first, double (&m)[kAhead]) {
+        double ey[kAhead];
+        weights(first, m, ey);
 #pragma unroll
-        for (int k = 0; k < kHeld; ++k) {
-            const double p = __dmul_rn(ez[k], ip);  // (rounded like q: equal ones leave nothing)
-            ez[k] = plain ? p : y ? fmax(p - __dmul_rn(ey[k], iq), 0.0) : first + 32 * k == d ? 0.0 : p;
+        for (int k = 0; k < kAhead; ++k) {
+            const double p = __dmul_rn(m[k], ip);  // (rounded like q: equal ones leave nothing)
+            m[k] = plain ? p : y ? fmax(p - __dmul_rn(ey[k], iq), 0.0) : first + 32 * k == d ? 0.0 : p;
         }
     };
     double total, unused;
     for (;;) {
         total = unused = 0.0;
-        for (int block = 0; block < blocks; ++block) {
-            if (blocks > 1) weights(block);
-            masses(block);
+        for (int i0 = begin + lane; i0 < end; i0 += 32 * kAhead) {
+            double m[kAhead];
+            masses(i0, m);
 #pragma unroll
-            for (int k = 0; k < kHeld; ++k) total += ez[k];
+            for (int k = 0; k < kAhead; ++k) total += m[k];
         }
-        cluster_sum(cluster, s, total, unused);
+        cluster_sum(cluster, s, turn, total, unused);
+        turn ^= 1;
         if (plain || total > 0.0) break;
         plain = true;  // nothing is left: p and q are one
-        if (blocks == 1) weights(0);
     }
-    // (s.warp[0]: this CTA's warps' sums; s.cta[0] of every CTA: theirs)
-    const double target = pick_draws[b] * total;
+    // (s.warp[0]: this CTA's warps' sums; s.cta: every CTA's)
+    const double target = draw * total;
     double before = 0.0, held = 0.0;
     int last = 0;  // the last CTA with any weight
-    for (int i = 0; i < kPickCtas; ++i) {
-        const double other = cluster.map_shared_rank(&s, i)->cta[0];
+    for (int i = 0; i < ctas; ++i) {
+        const double other = s.cta[turn ^ 1][0][i];
         if (i < rank) before += other;
         if (i == rank) held = other;
         if (other > 0.0) last = i;
     }
+    if (rank == 0 && tid == 0) accepted[b] = a;
     // a draw at the very end of the sums belongs to the last id with any weight
-    if ((target >= before && target < before + held) || (rank == last && target >= before + held)) {
-        double ahead = before;
-        int last_warp = 0;
-        for (int w = 0; w < kWarps; ++w) {
-            if (w < warp) ahead += s.warp[0][w];
-            if (s.warp[0][w] > 0.0) last_warp = w;
-        }
-        const double own = s.warp[0][warp];
-        if (own > 0.0 && ((target >= ahead && target < ahead + own) || (warp == last_warp && target >= ahead + own))) {
-            int found = -1, last_id = -1;
-            for (int block = 0; block < blocks && found < 0; ++block) {
-                if (blocks > 1) {
-                    weights(block);
-                    masses(block);
-                }
+    if (!((target >= before && target < before + held) || (rank == last && target >= before + held))) return;
+    double ahead = before;
+    int last_warp = 0;
+    for (int w = 0; w < kPickWarps; ++w) {
+        if (w < warp) ahead += s.warp[0][w];
+        if (s.warp[0][w] > 0.0) last_warp = w;
+    }
+    const double own = s.warp[0][warp];
+    if (!(own > 0.0 && ((target >= ahead && target < ahead + own) || (warp == last_warp && target >= ahead + own)))) return;
+    int found = -1, last_id = -1;
+    for (int i0 = begin; i0 < end && found < 0; i0 += 32 * kAhead) {
+        double m[kAhead];
+        masses(i0 + lane, m);
 #pragma unroll
-                for (int k = 0; k < kHeld; ++k) {
-                    if (found >= 0) break;
-                    double run = ez[k];
+        for (int k = 0; k < kAhead; ++k) {
+            if (found >= 0) break;
+            double run = m[k];
 #pragma unroll
-                    for (int o = 1; o < 32; o <<= 1) {
-                        const double up = __shfl_up_sync(0xffffffffu, run, o);
-                        if (lane >= o) run += up;
-                    }
-                    const unsigned over = __ballot_sync(0xffffffffu, ez[k] > 0.0 && ahead + run > target);
-                    const unsigned some = __ballot_sync(0xffffffffu, ez[k] > 0.0);
-                    const int first = begin + (block * kHeld + k) * 32;
-                    if (over) found = first + __ffs(over) - 1;
-                    if (some) last_id = first + 31 - __clz(some);
-                    ahead += __shfl_sync(0xffffffffu, run, 31);
-                }
+            for (int o = 1; o < 32; o <<= 1) {
+                const double up = __shfl_up_sync(0xffffffffu, run, o);
+                if (lane >= o) run += up;
             }
-            if (lane == 0) picked[b] = found >= 0 ? found : last_id;
+            const unsigned over = __ballot_sync(0xffffffffu, m[k] > 0.0 && ahead + run > target);
+            const unsigned some = __ballot_sync(0xffffffffu, m[k] > 0.0);
+            if (over) found = i0 + 32 * k + __ffs(over) - 1;
+            if (some) last_id = i0 + 32 * k + 31 - __clz(some);
+            ahead += __shfl_sync(0xffffffffu, run, 31);
         }
     }
-    if (rank == 0 && tid == 0) accepted[b] = a;
-    cluster.sync();  // nobody leaves while its sums may be read
+    if (lane == 0) picked[b] = found >= 0 ? found : last_id;
 }
 
 static int verify_parts(int vocab) {
@@ -459,8 +454,21 @@ NNIS_API int nnis_verify_drafts(const float* logits, const float* draft_logits, 
     cudaError_t e = launch_dependent(verify_rows_kernel, dim3(n_parts, all_rows), kVerifyThreads, 0, stream, logits, draft_logits,
                                      first_row, temperature, n_seqs, rows, draft_rows, vocab, per, static_cast<RowSum*>(scratch));
     if (e != cudaSuccess) return (int)e;
-    e = launch_dependent(verify_pick_kernel, dim3(kPickCtas, n_seqs), kPickThreads, 0, stream, logits, draft_logits, drafts, first_row,
-                         temperature, accept_draws, pick_draws, static_cast<const RowSum*>(scratch), n_parts, rows, vocab, accepted,
-                         picked);
+    // Eight CTAs a sequence; four where eight would be more than the device holds at once.
+    cudaLaunchConfig_t cfg = {};
+    const int ctas = n_seqs * kPickCtas <= 2 * device_sms() ? kPickCtas : kPickCtas / 2;
+    cfg.gridDim = dim3(ctas, n_seqs);
+    cfg.blockDim = dim3(kPickThreads);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = ctas;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = dependent_launches() ? 2 : 1;
+    e = cudaLaunchKernelEx(&cfg, verify_pick_kernel, logits, draft_logits, drafts, first_row, temperature, accept_draws, pick_draws,
+                           static_cast<const RowSum*>(scratch), n_parts, rows, vocab, accepted, picked);
     return e == cudaSuccess ? NNIS_OK : (int)e;
 }

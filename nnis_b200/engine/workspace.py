@@ -60,6 +60,15 @@ class Workspace:
             self._buffers[key] = buf
         return buf[:count].view(*shape)
 
+    def room(self, name: str, count: int, dtype: torch.dtype) -> torch.Tensor:
+        """The buffer of at least ``count`` elements itself: for a caller that takes its address alone (a slice and a
+        view of it are 2 us of the host)."""
+        buf = self._buffers.get((name, dtype))
+        if buf is None or buf.numel() < count:
+            self.get(name, (count,), dtype)
+            buf = self._buffers[(name, dtype)]
+        return buf
+
     def kept_zero(self, name: str, shape, dtype: torch.dtype) -> torch.Tensor:
         """Like ``get``, for a buffer whose users leave every value they touched at zero again
         (an accumulator that the kernel which reads it last clears): zero when first handed out
@@ -90,6 +99,17 @@ class Workspace:
             buf = torch.zeros(max(count, 1), dtype=dtype, device=self.device)
             self._buffers[key] = buf
         return buf[:count].view(*shape)
+
+    def zeros_room(self, name: str, count: int, dtype: torch.dtype) -> torch.Tensor:
+        """The buffer of ``zeros`` of at least ``count`` elements itself: for users that leave whatever they touch at zero, so
+        that one buffer serves requests of every size (a larger one is made anew, zero)."""
+        key = (name + "#zeros_room", dtype)
+        buf = self._buffers.get(key)
+        if buf is None or buf.numel() < count:
+            if self.frozen:
+                raise RuntimeError(f"workspace buffer {name!r} would move after graph capture")
+            buf = self._buffers[key] = torch.zeros(max(count, 1), dtype=dtype, device=self.device)
+        return buf
 
     def bytes(self) -> int:
         return sum(b.numel() * b.element_size() for b in self._buffers.values()) + \
