@@ -21,6 +21,12 @@ their views, in the same order):
   kind ((shape, dtype) each) for a mixer whose state has several parts (a recurrence's
   sums and the last inputs of a short convolution, say).
 
+Sequences may share pages: ``fork`` makes a sequence that begins with another's pages instead
+of copies of them, and counts the holders of each.  A shared page is read by all and written by
+none: before a step writes into one (a sequence's last, partly filled page), ``reserve`` gives the
+writer a page of its own with a copy of the positions that it holds, for all layers and all
+sequences of the step in one launch.
+
 Lengths are per slot (all layers advance together inside a step).  Positions at
 or beyond a slot's length are never read, so a reused slot cannot see what its
 last owner left (NNIS relies on the same rule:
@@ -96,6 +102,18 @@ class _KVGroup:
         self.v = torch.zeros((*shape[:4], self.value_dim), dtype=dtype, device=device) if self.values else None
         # per slot: logical page index -> page id, -1 where given back
         self.tables: Dict[int, List[int]] = {}
+        # pages in more than one table: how many more
+        self.extra: Dict[int, int] = {}
+
+    def give(self, page: int) -> None:
+        """One table fewer holds the page; it is free when none does."""
+        more = self.extra.get(page)
+        if more is None:
+            self.pool.give(page)
+        elif more > 1:
+            self.extra[page] = more - 1
+        else:
+            del self.extra[page]
 
     def first_needed_page(self, length: int) -> int:
         """Pages before this one (but for the kept first ones) hold no key that a later position may read."""
@@ -122,6 +140,9 @@ class CacheManager:
         # counts every change of any page table, growth included: while it stands still a
         # copy of the tables of the same slots needs no look
         self.epoch = 0
+        # counts what happened to pages that several tables hold (shared, parted with, given back, moved): while it
+        # stands still, sequences share what they shared
+        self.share_epoch = 0
         self.owners: List[int] = [0] * max_slots  # how many sequences have held each slot
         self.groups: List[_KVGroup] = []
         self._views: List[Optional[Union[KVView, StateView]]] = []
@@ -215,9 +236,11 @@ class CacheManager:
         if not self.slots.is_held(slot):
             raise SlotError(f"slot {slot} is not held (freed twice?)")
         for g in self.groups:
+            if g.extra:
+                self.share_epoch += 1
             for page in g.tables.pop(slot):
                 if page >= 0:
-                    g.pool.give(page)
+                    g.give(page)
         self.lengths[slot] = 0
         self.versions[slot] += 1
         self.epoch += 1
@@ -244,10 +267,15 @@ class CacheManager:
                                 f"{self.max_positions}")
             for gi, g in enumerate(self.groups):
                 need[gi] += max(0, -(-n // PAGE_SIZE) - len(g.tables[slot]))
+        copies = [self._to_copy(g, slots, new_lengths) if g.extra else [] for g in self.groups]
         for gi, g in enumerate(self.groups):
+            need[gi] += len(copies[gi])
             if need[gi] > g.pool.free:
                 raise CacheFull(f"{need[gi]} pages wanted, {g.pool.free} of {g.pool.count} free "
                                 f"(group {gi}); raise max_tokens")
+        for g, slots_of in zip(self.groups, copies):
+            if slots_of:
+                self._copy_shared(g, slots_of)
         for slot, n in zip(slots, new_lengths):
             for g in self.groups:
                 table = g.tables[slot]
@@ -255,6 +283,42 @@ class CacheManager:
                 if more > 0:
                     table.extend(g.pool.take_many(more))
                     self.epoch += 1
+
+    def _to_copy(self, g: _KVGroup, slots: Sequence[int], new_lengths: Sequence[int]) -> List[int]:
+        """The slots that will write into a page that others hold as well: of a page's holders the last may keep it."""
+        out, parted = [], {}
+        for slot, n in zip(slots, new_lengths):
+            at = self.lengths[slot] // PAGE_SIZE
+            table = g.tables[slot]
+            if n > self.lengths[slot] and at < len(table):
+                others = g.extra.get(table[at], 0) - parted.get(table[at], 0)
+                if others > 0:
+                    parted[table[at]] = parted.get(table[at], 0) + 1
+                    out.append(slot)
+        return out
+
+    def _copy_shared(self, g: _KVGroup, slots: Sequence[int]) -> None:
+        """A page of its own for every slot that is about to write into a shared one, with the positions it holds."""
+        moves = []
+        for slot, page in zip(slots, g.pool.take_many(len(slots))):
+            at, rows = divmod(self.lengths[slot], PAGE_SIZE)
+            old = g.tables[slot][at]
+            moves.append((old, page, rows))
+            g.tables[slot][at] = page
+            g.give(old)
+            self.versions[slot] += 1
+        self.epoch += 1
+        self.share_epoch += 1
+        self._copy_pages(g, moves)
+
+    def _copy_pages(self, g: _KVGroup, moves) -> None:
+        if self.device.type == "cuda":
+            ops.copy_pages(g.k, g.v, moves)
+            return
+        for t in (g.k, g.v):  # (host tests)
+            if t is not None:
+                for src, dst, rows in moves:
+                    t[:, dst, :, :rows] = t[:, src, :, :rows]
 
     def commit(self, slots: Sequence[int], new_lengths: Sequence[int]) -> None:
         """The step has been issued: lengths advance, windowed groups give back
@@ -266,7 +330,9 @@ class CacheManager:
                     table = g.tables[slot]
                     for i in range(g.kept_pages, min(g.first_needed_page(n), len(table))):
                         if table[i] >= 0:
-                            g.pool.give(table[i])
+                            if g.extra:
+                                self.share_epoch += 1
+                            g.give(table[i])
                             table[i] = -1
                             self.epoch += 1
 
@@ -289,18 +355,23 @@ class CacheManager:
                             "(take a snapshot before the tokens that may be taken back, and restore it)")
         self._forget_from(slot, length)
 
+    @staticmethod
+    def _check_pages(slot: int, gi: int, g: _KVGroup, length: int, keep: int) -> None:
+        if any(page < 0 for page in g.tables[slot][g.first_needed_page(length):keep]):
+            raise SlotError(f"slot {slot}: group {gi} (window {g.window}) has given back pages that "
+                            f"position {length} would read")
+
     def _forget_from(self, slot: int, length: int) -> None:
         keep = -(-length // PAGE_SIZE)
         for gi, g in enumerate(self.groups):
-            table = g.tables[slot]
-            if any(page < 0 for page in table[g.first_needed_page(length):keep]):
-                raise SlotError(f"slot {slot}: group {gi} (window {g.window}) has given back pages that "
-                                f"position {length} would read")
+            self._check_pages(slot, gi, g, length, keep)
         for g in self.groups:
             table = g.tables[slot]
+            if g.extra:
+                self.share_epoch += 1
             for page in table[keep:]:
                 if page >= 0:
-                    g.pool.give(page)
+                    g.give(page)
             del table[keep:]
         self.lengths[slot] = length
         self.versions[slot] += 1
@@ -338,6 +409,71 @@ class CacheManager:
             for t, kept in zip(self._states_of(slot), snapshot.states):
                 t.copy_(kept)
 
+    # -- sequences that begin alike ------------------------------------------
+    def fork(self, slot: int, length: Optional[int] = None) -> int:
+        """A new sequence that holds the first ``length`` positions of ``slot`` (all of them by default): its slot.  The
+        pages are shared, the state of fixed size is copied; either sequence goes on by itself, and whichever writes
+        first into the last, partly filled page gets a copy of it then.  Refused, with nothing changed, where ``length``
+        is not where the sequence is and the model keeps fixed-size state (it has no earlier value), or a windowed
+        group has given back pages that the positions after ``length`` would read."""
+        if not self.slots.is_held(slot):
+            raise SlotError(f"slot {slot} is not held")
+        length = self.lengths[slot] if length is None else length
+        if not 0 <= length <= self.lengths[slot]:
+            raise SlotError(f"slot {slot}: cannot fork {length} of {self.lengths[slot]} positions")
+        if self._states and length < self.lengths[slot]:
+            raise SlotError("a sequence with fixed-size state forks where it is, not at an earlier length")
+        keep = -(-length // PAGE_SIZE)
+        for gi, g in enumerate(self.groups):
+            self._check_pages(slot, gi, g, length, keep)
+        new = self.acquire()
+        for g in self.groups:
+            table = g.tables[slot][:keep]
+            # (pages in front of the window's first that the other still holds are not needed here)
+            table = [page if i < g.kept_pages or i >= g.first_needed_page(length) else -1 for i, page in enumerate(table)]
+            g.tables[new] = table
+            for page in table:
+                if page >= 0:
+                    g.extra[page] = g.extra.get(page, 0) + 1
+        self.lengths[new] = length
+        self.share_epoch += 1
+        if self._states:
+            pieces = self._pieces_of(new)
+            if pieces:
+                pieces.take_back(self._states_of(slot))
+            else:
+                for t, kept in zip(self._states_of(new), self._states_of(slot)):
+                    t.copy_(kept)
+        return new
+
+    def shares_pages(self) -> bool:
+        """Whether any page is held by more than one sequence."""
+        return any(g.extra for g in self.groups)
+
+    def compact(self) -> List[int]:
+        """The held pages of every group move to its lowest places, so that they are ``[:, :held]`` of its storage:
+        returns how many pages have moved in each.  One launch a group, on the current stream; page lists that a
+        program has copied are out of date."""
+        moved = []
+        for g in self.groups:
+            held = g.pool.held
+            sources = [p for p in range(held, g.pool.count) if g.pool.is_held(p)]
+            targets = g.pool.take_many(len(sources))  # (the lowest free places: all below ``held``)
+            to = dict(zip(sources, targets))
+            if to:
+                self._copy_pages(g, [(a, b, PAGE_SIZE) for a, b in to.items()])
+                for slot, table in g.tables.items():
+                    if any(p in to for p in table):
+                        table[:] = [to.get(p, p) for p in table]
+                        self.versions[slot] += 1
+                g.extra = {to.get(p, p): n for p, n in g.extra.items()}
+                for page in sources:
+                    g.pool.give(page)
+                self.epoch += 1
+                self.share_epoch += 1
+            moved.append(len(to))
+        return moved
+
     def page_table(self, group: int, slot: int) -> List[int]:
         return self.groups[group].tables[slot]
 
@@ -358,6 +494,7 @@ class CacheManager:
         return {
             "slots_held": self.slots.held, "slots_total": self.slots.count,
             "pages_held": [g.pool.held for g in self.groups], "pages_total": self.pages_total,
+            "pages_shared": [len(g.extra) for g in self.groups],
             "live_tokens": sum(self.lengths[s] for s in range(self.slots.count)
                                if self.slots.is_held(s)),
             "kv_bytes": sum(t.numel() * t.element_size() for g in self.groups for t in (g.k, g.v)
@@ -368,8 +505,12 @@ class CacheManager:
         self.slots.check()
         for g in self.groups:
             g.pool.check()
-            held = [p for t in g.tables.values() for p in t if p >= 0]
-            if len(set(held)) != len(held):
+            counts: Dict[int, int] = {}
+            for table in g.tables.values():
+                for p in table:
+                    if p >= 0:
+                        counts[p] = counts.get(p, 0) + 1
+            if any(n != 1 + g.extra.get(p, 0) for p, n in counts.items()) or any(p not in counts for p in g.extra):
                 raise SlotError("a page is in two page tables")
-            if len(held) != g.pool.held:
-                raise SlotError(f"{g.pool.held} pages held, {len(held)} in page tables")
+            if len(counts) != g.pool.held:
+                raise SlotError(f"{g.pool.held} pages held, {len(counts)} in page tables")
