@@ -17,6 +17,9 @@ def __getattr__(name):
     if name in ("GenerationConfig", "GenerationRequest", "GenerationResult", "StreamControl"):
         from .engine import generate
         return getattr(generate, name)
+    if name in ("LookupDrafter", "SessionDrafter"):
+        from .engine import drafting
+        return getattr(drafting, name)
     if name == "SamplingConfig":
         from .sampling import SamplingConfig
         return SamplingConfig

@@ -446,6 +446,10 @@ class CacheManager:
                     t.copy_(kept)
         return new
 
+    def fixed_history(self) -> bool:
+        """Whether sequences cannot go back to any earlier length: some state has no earlier value, or a window gives pages back."""
+        return bool(self._states) or any(g.window > 0 for g in self.groups)
+
     def shares_pages(self) -> bool:
         """Whether any page is held by more than one sequence."""
         return any(g.extra for g in self.groups)

@@ -22,14 +22,14 @@ DEFAULT_MAX_NEW_TOKENS = 16
 GENERATE_BATCH_JSON_SCHEMA_VERSION = 1
 USAGE = """Usage:
   nnis generate --model DIR [--tokenizer FILE] --prompt TEXT | --prompt-ids IDS [--device N] [--max-new-tokens N] [--dtype bfloat16|float32] [--sample --seed U64] [--temperature F] [--top-k N] [--top-p F] [--stream]
-  nnis generate-batch --model DIR [--tokenizer FILE] --prompt TEXT [--prompt TEXT ...] | --prompt-ids IDS [--prompt-ids IDS ...] --seed U64 [--seed U64 ...] [--device N] [--max-new-tokens N] [--dtype bfloat16|float32] [--temperature F] [--top-k N] [--top-p F] [--json]
+  nnis generate-batch --model DIR [--tokenizer FILE] --prompt TEXT [--prompt TEXT ...] | --prompt-ids IDS [--prompt-ids IDS ...] --seed U64 [--seed U64 ...] [--device N] [--max-new-tokens N] [--dtype bfloat16|float32] [--temperature F] [--top-k N] [--top-p F] [--share-prefix] [--json]
   nnis validate --model DIR [--tokenizer FILE] [--json] [--output FILE]
   nnis random-model --config FILE --seed U64 --out DIR [--format hf|nnis]
 
 `validate` checks config.json, the safetensors files (tensor names, shapes and dtypes against the model that config.json names) and, when a tokenizer is given or DIR/tokenizer.json exists, that its ids fit the vocabulary; it needs no GPU and reads no tensor. `--output FILE` requires `--json` and writes the report there, never over an existing file.
 `random-model` writes a model folder with seeded random weights from a config.json (`hf`: config.json + model.safetensors; `nnis`: model.json + raw tensor files); it needs no GPU.
 
-Default decoding on `generate` is greedy. Opt-in `--sample` requires `--seed`. Optional `--temperature`, `--top-k`, and `--top-p` apply only with `--sample`. `--stream` is valid only with `--sample` and prints each token as it is emitted. `generate-batch` requires one `--seed` per prompt and always samples; `--json` emits versioned JSON. CUDA device ordinal defaults to 0."""
+Default decoding on `generate` is greedy. Opt-in `--sample` requires `--seed`. Optional `--temperature`, `--top-k`, and `--top-p` apply only with `--sample`. `--stream` is valid only with `--sample` and prints each token as it is emitted. `generate-batch` requires one `--seed` per prompt and always samples; `--json` emits versioned JSON; `--share-prefix` runs tokens that prompts begin with alike once. CUDA device ordinal defaults to 0."""
 
 
 class UsageError(Exception):
@@ -48,6 +48,7 @@ class GenerateArgs:
     sample: bool = False
     stream: bool = False
     json: bool = False
+    share_prefix: bool = False
     seeds: List[int] = field(default_factory=list)
     temperature: Optional[float] = None
     top_k: Optional[int] = None
@@ -106,12 +107,12 @@ def parse_args(argv: List[str]) -> Optional[GenerateArgs]:
     for flag in it:
         if flag in ("-h", "--help"):
             return None
-        if flag in ("--sample", "--stream", "--json"):
-            if (flag == "--json") != batch and flag == "--json":
-                raise UsageError("--json belongs to generate-batch")
-            if batch and flag != "--json":
+        if flag in ("--sample", "--stream", "--json", "--share-prefix"):
+            if not batch and flag in ("--json", "--share-prefix"):
+                raise UsageError(f"{flag} belongs to generate-batch")
+            if batch and flag in ("--sample", "--stream"):
                 raise UsageError(f"{flag} does not apply to generate-batch (it always samples)")
-            setattr(a, flag[2:], True)
+            setattr(a, flag[2:].replace("-", "_"), True)
             continue
         try:
             value = next(it)
@@ -356,7 +357,7 @@ def run(a: GenerateArgs, out=sys.stdout) -> int:
         out.flush()
 
     results = llm.generate(prompts, max_new_tokens=a.max_new_tokens, sampling=sampling,
-                           on_token=on_token if a.stream else None)
+                           on_token=on_token if a.stream else None, share_prefix=a.share_prefix)
     failed = any(not r.ok for r in results)
     if a.command == "generate":
         r = results[0]

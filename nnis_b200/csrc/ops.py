@@ -17,6 +17,7 @@ from typing import Optional
 import torch
 
 from . import build as _build
+from .shared_plan import shared_nodes, shared_units
 
 F32, BF16 = 0, 1
 _DTYPE_CODE = {torch.float32: F32, torch.bfloat16: BF16}
@@ -2839,47 +2840,81 @@ def memory_finish(o_raw: torch.Tensor, a: torch.Tensor, gate_off: int, weight: t
 
 class SharedPlan:
     """What ``attention_shared`` works through for a batch whose sequences share pages (see ``shared_plan``): good as long as
-    its rows stay at the positions that it was made for and their page lists do not change."""
+    its rows stay at the positions that it was made for and their page lists do not change (and, made with pages
+    ``ahead``, while they grow by no more)."""
 
-    def __init__(self, rows, heads, kv_heads, head_dim, dtype, counts, ints, records, seqs, cols, form):
+    def __init__(self, rows, heads, kv_heads, head_dim, dtype, counts, members, ints, records, seqs, cols):
         self.rows, self.heads, self.kv_heads, self.head_dim, self.dtype = rows, heads, kv_heads, head_dim, dtype
-        self.counts, self.ints, self.records, self.seqs, self.cols, self.form = counts, ints, records, seqs, cols, form
-        units, members = 8 * sum(counts), ints.numel() - 8 * sum(counts) - rows - 1
-        self.units, self.members, self.record = ints.data_ptr(), ints.data_ptr() + 4 * units, ints.data_ptr() + 4 * (units + members)
+        self.counts, self.members_held, self.ints, self.records, self.seqs, self.cols = counts, members, ints, records, seqs, cols
+        self.form = int(_shared_on_tensor_cores(dtype, head_dim))
+        at = ints.data_ptr()
+        self.units, self.members = at, at + 32 * sum(counts)
+        self.record = self.members + 4 * members
         # rows merged by the CTA that completes them save a launch, where a CTA has few of them to merge
         self.merged_inside = counts[2] == 0 and sum(counts) * kv_heads <= 148 and records <= 4 * rows
         self.device, self.status = ints.device, status_word(ints.device).data_ptr()
         self.launches = (not self.merged_inside) + sum(c > 0 for c in counts)
+
+    @classmethod
+    def with_room(cls, rows, heads, kv_heads, head_dim, dtype, device, room, cols) -> "SharedPlan":
+        """A plan whose units, members and records fit ``room`` (of each kind, and of members and records), to be filled."""
+        *counts, members, records = room
+        ints = torch.zeros(8 * sum(counts) + members + rows + 1, dtype=torch.int32, device=device)
+        return cls(rows, heads, kv_heads, head_dim, dtype, counts, members, ints, records, rows, cols)
+
+    def fill(self, kinds, members, record) -> None:
+        """Its contents replaced, on the current stream, by a batch's that fit (units that are left over do nothing)."""
+        import numpy as np
+        _need(all(len(k) <= c for k, c in zip(kinds, self.counts)) and len(members) <= self.members_held
+              and len(record) == self.rows + 1 and int(record[-1]) <= self.records, "shared attention: more units than the plan holds")
+        ints, at = np.zeros(self.ints.numel(), dtype=np.int32), 0
+        for kind, count in zip(kinds, self.counts):
+            ints[at:at + kind.size] = kind.reshape(-1)
+            at += 8 * count
+        ints[at:at + len(members)] = members
+        ints[at + self.members_held:] = record
+        self.ints.copy_(torch.from_numpy(ints))
 
 
 def attention_shared_takes(head_dim: int, page_size: int) -> bool:
     return page_size == 64 and head_dim % 2 == 0 and 2 <= head_dim <= 256
 
 
+def _shared_on_tensor_cores(dtype: torch.dtype, head_dim: int) -> bool:
+    return dtype == torch.bfloat16 and head_dim in (64, 128)
+
+
+def attention_shared_units(nodes, tails, seqs, heads: int, kv_heads: int, head_dim: int, dtype: torch.dtype, device):
+    """(units of every kind, members, record offsets) of a batch's tree of pages (``shared_nodes``)."""
+    sms = sm_count(device)
+    kinds = ((0, 0, 0, 0), (32, 6 * sms, 2, 16), (128, 2 * sms, 2, 1 << 20)) if _shared_on_tensor_cores(dtype, head_dim) else \
+        ((16, 4 * sms, 2, 16), (64, 4 * sms, 2, 16), (0, 0, 0, 0))
+    return shared_units(nodes, tails, seqs, heads // kv_heads, kv_heads, kinds, 1)
+
+
+def attention_shared_plan_of(nodes, tails, seqs, positions, heads: int, kv_heads: int, head_dim: int, dtype: torch.dtype,
+                             device) -> SharedPlan:
+    import numpy as np
+    kinds, members, record = attention_shared_units(nodes, tails, seqs, heads, kv_heads, head_dim, dtype, device)
+    ints = np.concatenate([k.reshape(-1) for k in kinds] + [members, record]).astype(np.int32)
+    return SharedPlan(len(seqs), heads, kv_heads, head_dim, dtype, [len(k) for k in kinds], len(members),
+                      torch.from_numpy(ints).to(device), int(record[-1]), 1 + max(seqs), max([p // 64 + 1 for p in positions] + [1]))
+
+
 def attention_shared_plan(tables, seqs, positions, heads: int, kv_heads: int, head_dim: int, dtype: torch.dtype,
                           device) -> SharedPlan:
     """The plan of a batch: ``tables`` the page list of every sequence, ``seqs`` and ``positions`` the sequence and the
     position (-1: a padding row) of every token row."""
-    import numpy as np
-    from .shared_plan import PAGE as page, shared_nodes, shared_units
     n = len(seqs)
     _need(n > 0 and len(positions) == n, "shared attention: a sequence and a position per token row")
     _need(kv_heads > 0 and heads % kv_heads == 0, "attention: heads is not a multiple of kv_heads")
-    _need(attention_shared_takes(head_dim, page), f"attention: head_dim {head_dim} is not an even size in 2..256")
+    _need(attention_shared_takes(head_dim, 64), f"attention: head_dim {head_dim} is not an even size in 2..256")
     code_of(dtype)
     for s, p in zip(seqs, positions):
         _need(0 <= s < len(tables), f"shared attention: sequence {s} of {len(tables)}")
-        _need(p < len(tables[s]) * page, f"shared attention: position {p} is beyond its sequence's {len(tables[s])} pages")
+        _need(p < len(tables[s]) * 64, f"shared attention: position {p} is beyond its sequence's {len(tables[s])} pages")
     nodes, tails = shared_nodes(tables, seqs, positions)
-    device = torch.device(device)
-    tensor = dtype == torch.bfloat16 and head_dim in (64, 128)  # (the forms on the tensor cores)
-    sms = sm_count(device)
-    kinds, members, record = shared_units(nodes, tails, seqs, heads // kv_heads, kv_heads, (
-        ((0, 0, 0, 0), (32, 6 * sms, 2, 16), (128, 2 * sms, 2, 1 << 20)) if tensor else
-        ((16, 4 * sms, 2, 16), (64, 4 * sms, 2, 16), (0, 0, 0, 0))), 1)
-    ints = np.concatenate([k.reshape(-1) for k in kinds] + [members, record]).astype(np.int32)
-    return SharedPlan(n, heads, kv_heads, head_dim, dtype, [len(k) for k in kinds], torch.from_numpy(ints).to(device),
-                      int(record[-1]), 1 + max(seqs), max([p // page + 1 for p in positions] + [1]), int(tensor))
+    return attention_shared_plan_of(nodes, tails, seqs, positions, heads, kv_heads, head_dim, dtype, torch.device(device))
 
 
 def attention_shared(q: torch.Tensor, q_stride: int, k_cache: torch.Tensor, v_cache: torch.Tensor, token_pos: torch.Tensor,

@@ -31,14 +31,14 @@ def _alike(a: Sequence[int], b: Sequence[int], low: int, high: int) -> int:
 
 
 def shared_nodes(tables: Sequence[Sequence[int]], seqs: Sequence[int], positions: Sequence[int],
-                 horizon: int = 0) -> Tuple[List[tuple], List[tuple]]:
+                 ahead: int = 0) -> Tuple[List[tuple], List[tuple]]:
     """(nodes, tails): nodes (rows, first page, end page) that several rows share, parents before children;
-    tails (row, first page, end page).  ``horizon`` > 0: tails go on to that page (rows that will grow)."""
+    tails (row, first page, end page), ``ahead`` pages longer than they are (rows that will grow)."""
     nodes: List[tuple] = []
     tails: List[tuple] = []
 
     def tail(row: int, depth: int) -> None:
-        end = max(horizon, positions[row] // PAGE + 1)
+        end = positions[row] // PAGE + 1 + ahead
         if end > depth:
             tails.append((row, depth, end))
 

@@ -24,10 +24,13 @@ from ..cache import PAGE_SIZE
 from ..csrc import ops
 from .decode import GraphDecoder
 from .engine import Engine, SequenceStep, StepError
+from .sharing import BatchUnits, rooms_of
 from .generate import (DEFAULT_MAX_NEW_TOKENS, GenerationConfig, GenerationRequest,
                        GenerationResult, Generator, StreamControl)
 
 Prompt = Union[str, Sequence[int]]
+
+MAX_SHARED_DECODERS = 8  # captured steps kept for batches whose sequences share pages
 
 
 class EngineBackend:
@@ -45,6 +48,7 @@ class EngineBackend:
         self._decoders = {}
         self._uncaptured = set()  # keys of decoders whose capture has failed for a session
         self._views = {}
+        self._shared = BatchUnits(engine)
         self._pinned = None
         self._picked = None
         self._picked_for = None
@@ -61,6 +65,9 @@ class EngineBackend:
 
     def release_slot(self, slot: int) -> None:
         self.engine.release_slot(slot)
+
+    def fork_slot(self, slot: int) -> int:
+        return self.engine.fork(slot)
 
     def step(self, batch, need_logits: bool = True):
         """Logits [len(batch) wanted rows, vocab] (or None when ``need_logits`` is
@@ -102,7 +109,7 @@ class EngineBackend:
         new_lengths = [p + 1 for p in positions]
         cache.reserve(slots, new_lengths)
         if dec is None:
-            dec = self._decoder(len(slots), max(new_lengths), need_logits)
+            dec = self._shared_decoder(slots, positions, max(new_lengths), need_logits)
         self.h2d_bytes += dec.upload(tokens, positions, slots)
         dec.launch()
         cache.commit(slots, new_lengths)
@@ -192,18 +199,43 @@ class EngineBackend:
         context = min(pages * PAGE_SIZE, self.engine.spec.max_positions)
         return bucket, context, want_logits
 
-    def _decoder(self, rows: int, max_context: int, want_logits: bool = False) -> GraphDecoder:
+    def _decoder(self, rows: int, max_context: int, want_logits: bool = False, rooms: Optional[tuple] = None) -> GraphDecoder:
         key = self._decoder_key(rows, max_context, want_logits)
+        if rooms is not None:
+            key = (*key, rooms)
+            # (what sequences share takes many forms: of the steps captured for it the least recently used goes)
+            shared = [k for k in self._decoders if len(k) > 3]
+            if key in self._decoders:
+                self._decoders[key] = self._decoders.pop(key)
+            elif len(shared) >= MAX_SHARED_DECODERS:
+                gone = self._decoders.pop(shared[0])
+                self._views = {k: v for k, v in self._views.items() if k[0] != id(gone)}
         if key not in self._decoders:
             self._decoders[key] = GraphDecoder(self.engine, *key)
         return self._decoders[key]
+
+    def _shared_decoder(self, slots: Sequence[int], positions: Sequence[int], max_context: int, want_logits: bool = False,
+                        ahead: Optional[int] = None) -> GraphDecoder:
+        """The decoder of these sequences, whose pages have been reserved: one that reads what they share once, where that pays."""
+        rows = self._decoder_key(len(slots), max_context, want_logits)[0]
+        units = self._shared.units(slots, positions, rows) if ahead is None else self._shared.units(slots, positions, rows, ahead)
+        dec = self._decoder(len(slots), max_context, want_logits, rooms_of(units))
+        if units is not None:
+            dec.plans.fill(units)
+        return dec
 
     def decode_greedy(self, rows, emit) -> None:
         """rows: (request, slot, next input token, its position, tokens still to
         pick).  Calls ``emit(request, token)`` for every pick in order; a False
         return means that sequence has ended (its slot is already given back)."""
         cache = self.engine.cache
-        dec = self._decoder(len(rows), max(pos + left + 1 for _, _, _, pos, left in rows))
+        slots, positions = [r[1] for r in rows], [r[3] for r in rows]
+        longest = max(pos + left + 1 for _, _, _, pos, left in rows)
+        if cache.shares_pages():  # (the pages that they will write into, copied together)
+            cache.reserve(slots, [p + 1 for p in positions])
+            dec = self._shared_decoder(slots, positions, longest, ahead=max(left for *_, left in rows) // PAGE_SIZE + 1)
+        else:
+            dec = self._decoder(len(rows), longest)
         live = {}
         for r, (i, slot, token, pos, left) in enumerate(rows):
             dec.set_row(r, slot, token, pos)
@@ -286,12 +318,14 @@ class LLM:
     def generate(self, prompts: Sequence[Prompt], max_new_tokens: int = DEFAULT_MAX_NEW_TOKENS,
                  sampling: Union[None, SamplingConfig, Sequence[Optional[SamplingConfig]]] = None,
                  stop_token_ids: Optional[Sequence[int]] = None,
-                 on_token: Optional[Callable[[int, int], Optional[StreamControl]]] = None
-                 ) -> List[GenerationResult]:
+                 on_token: Optional[Callable[[int, int], Optional[StreamControl]]] = None,
+                 share_prefix: bool = False) -> List[GenerationResult]:
         """Greedy unless ``sampling`` is given (one policy for all prompts or one
         per prompt).  ``stop_token_ids=None`` takes config.json's eos ids.
         ``on_token(prompt index, token)`` sees tokens as they are emitted and may return
-        ``StreamControl.STOP`` to end that prompt's generation; the others go on."""
+        ``StreamControl.STOP`` to end that prompt's generation; the others go on.
+        ``share_prefix``: prompts that begin with the same tokens (several samples of one
+        prompt, questions behind one document) run those once and share their pages."""
         stops = tuple(self.spec.stop_token_ids if stop_token_ids is None else stop_token_ids)
         if sampling is None or isinstance(sampling, SamplingConfig):
             sampling = [sampling] * len(prompts)
@@ -300,7 +334,7 @@ class LLM:
         gen = GenerationConfig(max_new_tokens=max_new_tokens, stop_token_ids=stops)
         requests = [GenerationRequest(self.encode(p) if isinstance(p, str) else list(p), gen, s)
                     for p, s in zip(prompts, sampling)]
-        return self._generator.generate(requests, on_token)
+        return self._generator.generate(requests, on_token, share_prefix)
 
     def new_session(self) -> "InferenceSession":
         return InferenceSession(self)
@@ -311,10 +345,10 @@ class InferenceSession:
 
     EAGER_TOKENS = 5  # that a session decodes before its step is captured (see ``EngineBackend.decode_logits``)
 
-    def __init__(self, llm: LLM):
+    def __init__(self, llm: LLM, slot: Optional[int] = None):
         self.llm = llm
         self.engine = llm.engine
-        self.slot = self.engine.acquire_slot()
+        self.slot = self.engine.acquire_slot() if slot is None else slot
         self._decoded = 0  # tokens that this session has decoded one by one
 
     def position(self) -> int:
@@ -340,6 +374,11 @@ class InferenceSession:
 
     def restore(self, snapshot) -> None:
         self.engine.restore(snapshot)
+
+    def fork(self) -> "InferenceSession":
+        """A second session that holds what this one does and goes on by itself: their pages are shared until one of
+        them writes into them, states are copied."""
+        return InferenceSession(self.llm, self.engine.fork(self.slot))
 
     def close(self) -> None:
         if self.slot is not None:
@@ -385,6 +424,64 @@ class InferenceSession:
         each emitted token once it has been executed; ``StreamControl.STOP`` ends the
         generation cleanly and leaves the session ready to go on."""
         return self._generate(input_ids, generation, sampling, on_token, keep_context)
+
+    def generate_drafted(self, input_ids: Sequence[int], generation: GenerationConfig, drafter, drafts: int = 4,
+                         sampling: Optional[SamplingConfig] = None,
+                         on_token: Optional[Callable[[int], Optional[StreamControl]]] = None,
+                         keep_context: bool = False) -> List[int]:
+        """Generation with drafted tokens: ``drafter`` (``drafting.LookupDrafter``, ``drafting.SessionDrafter``) proposes up to
+        ``drafts`` tokens, one step runs them all, and those stay that the model keeps.  Greedy unless ``sampling`` is
+        given (a temperature and a seed; top-k and top-p are refused): tokens are distributed as ``generate_sampled``'s without
+        the drafter, not the same for the same seed.  Every emitted token is executed, as in ``generate``."""
+        if self.engine.cache.fixed_history():
+            raise ValueError("drafted tokens that are refused are taken back: not for a model with state of fixed size or a window")
+        if drafts < 1:
+            raise ValueError(f"drafts must be positive; got {drafts}")
+        if sampling is not None and (sampling.top_k is not None or sampling.top_p is not None):
+            raise ValueError("drafted generation samples with a temperature only (no top_k, no top_p)")
+        other = getattr(getattr(drafter, "llm", None), "spec", None)
+        if other is not None and other.vocab_size != self.engine.spec.vocab_size:
+            raise ValueError(f"the drafting model has {other.vocab_size} tokens, this one {self.engine.spec.vocab_size}")
+        if not keep_context:
+            self.reset()
+        prompt = [int(t) for t in input_ids]
+        why = self.llm._generator.refusal(GenerationRequest(prompt, generation, sampling, slot=self.slot, start=self.position()))
+        if why is not None:
+            raise ValueError(why)
+        drafter.begin()
+        verifier = device_sampling.DraftVerifier(self.engine.device, self.engine.workspace, sampling)
+        told, emitted, feed, proposed, logits_of = list(prompt), [], prompt, [], None
+        while True:
+            held = self.position()
+            if proposed:
+                want = list(range(len(feed) - len(proposed) - 1, len(feed)))
+                logits = self.engine.step([SequenceStep(self.slot, feed, want)], drafted=True)
+            elif len(feed) == 1 and emitted:
+                logits = self.llm.backend.decode_logits(self.slot, feed[0], self._decoded >= self.EAGER_TOKENS).reshape(1, -1)
+                self._decoded += 1
+            else:
+                logits = self.engine.step([SequenceStep(self.slot, feed, [len(feed) - 1])])
+            kept, token = verifier.verify(logits, proposed, logits_of)
+            new, ended = proposed[:kept] + [token], False
+            for n, t in enumerate(new):
+                emitted.append(t)
+                stop = on_token is not None and on_token(t) is StreamControl.STOP
+                if stop or t in generation.stop_token_ids or len(emitted) >= generation.max_new_tokens:
+                    new, ended = new[:n + 1], True
+                    break
+            told += new
+            # what stays of the step: what was fed before the drafts, and the drafts that were emitted
+            stays = held + len(feed) - len(proposed) + min(len(new), kept)
+            if stays < self.position():
+                self.truncate(stays)
+            if ended:
+                if len(new) > kept:  # the last one came from the distribution: it is executed here
+                    self.engine.step([SequenceStep(self.slot, [token], [])])
+                return emitted
+            room = min(drafts, generation.max_new_tokens - len(emitted) - 1)
+            proposed, logits_of = drafter.propose(told, room, verifier.temperature) if room > 0 else ([], None)
+            proposed = list(proposed)[:room]
+            feed = [token, *proposed]
 
     def _generate(self, input_ids, generation, sampling, on_token, keep_context) -> List[int]:
         if not keep_context:

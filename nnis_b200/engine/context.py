@@ -76,6 +76,10 @@ class StepContext:
     next_block: object = None
     normed_rows: object = None
 
+    # ``shared``: gives an attention its plan for pages that several rows of the batch share (``sharing.SharedRows``
+    # or ``sharing.KeptPlans``); None where none do
+    shared: object = None
+
     def take_shared_norm(self, norm):
         """What the part before left of ``norm``'s work, or None; nothing is kept."""
         begun, self.shared_norm = self.shared_norm, None

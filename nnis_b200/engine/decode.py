@@ -31,6 +31,7 @@ import torch
 from ..cache import PAGE_SIZE
 from ..csrc import ops
 from .context import StepContext, sm_count
+from .sharing import KeptPlans
 from .workspace import Workspace
 
 
@@ -51,7 +52,7 @@ def chains_for(rows: int) -> int:
 
 class GraphDecoder:
     def __init__(self, engine, rows: int, max_context: int, want_logits: bool = False,
-                 chains: Optional[int] = None):
+                 rooms: Optional[tuple] = None, chains: Optional[int] = None):
         self.engine = engine
         self.want_logits = want_logits
         self.rows = rows
@@ -92,6 +93,10 @@ class GraphDecoder:
         # the chains: consecutive runs of rows, each with a context, buffers and a
         # stream of its own
         n_chains = max(1, min(chains if chains is not None else chains_for(rows), rows))
+        # pages that several rows share, read once for all of them (``rooms``: the sizes of the plans, ``sharing.rooms_of``)
+        self.plans = KeptPlans(engine, rows, self.cols, rooms) if rooms else None
+        if self.plans is not None:
+            n_chains = 1
         per = -(-rows // n_chains)
         self.chains = []
         for a in range(0, rows, per):
@@ -118,7 +123,7 @@ class GraphDecoder:
             n_tokens=n, n_seqs=n, tokens=self.tokens[a:b], token_pos=self.pos[a:b],
             token_seq=self.seq[:n], seq_slots=self.slots[a:b],
             page_tables=[t[a:b] for t in self.tables], workspace=Workspace(self.device), decode=True,
-            max_context=self.max_context, fixed_splits=splits)
+            max_context=self.max_context, fixed_splits=splits, shared=self.plans)
 
     def _query_heads(self) -> int:
         heads = [getattr(part, "heads", 1) for b in self.engine.model.blocks for part in b.parts()]

@@ -28,6 +28,7 @@ from ..weights import load_weights
 from ..weights.loader import shape_fits
 from .context import StepContext
 from .model import DecoderModel
+from .sharing import SharedRows
 from .workspace import Workspace
 
 GRAPH_MIN_TOKENS = 256  # prompt steps at least this large are captured when they recur
@@ -132,6 +133,15 @@ class Engine:
     def restore(self, snapshot) -> None:
         self.cache.restore(snapshot)
 
+    def fork(self, slot: int, length: Optional[int] = None) -> int:
+        """A new sequence (its slot) that holds the first ``length`` positions of ``slot``, all of them by default: pages are
+        shared and read once for all sequences of a decode step, states copied (see ``CacheManager.fork``)."""
+        return self.cache.fork(slot, length)
+
+    def compact(self) -> List[int]:
+        """Held pages move to the lowest places of their stores (see ``CacheManager.compact``)."""
+        return self.cache.compact()
+
     # -- the step -----------------------------------------------------------
     def _stage(self, parts: List[np.ndarray], workspace: Optional[Workspace] = None) -> torch.Tensor:
         """Int arrays -> one pinned buffer -> one async copy -> int32 device tensor."""
@@ -226,10 +236,10 @@ class Engine:
         entry["free"].record()
         return slots, new_lengths
 
-    def prepare(self, batch: Sequence[SequenceStep], workspace: Optional[Workspace] = None):
+    def prepare(self, batch: Sequence[SequenceStep], workspace: Optional[Workspace] = None, drafted: bool = False):
         """Validate, reserve pages, upload the tables; returns (ctx, want_rows,
         slots, new lengths).  ``workspace``: where the step's buffers live (the
-        engine's own unless a captured graph has one of its own)."""
+        engine's own unless a captured graph has one of its own).  ``drafted``: see ``step``."""
         workspace = workspace if workspace is not None else self.workspace
         token_arrays, wants, counts, starts = self._read(batch)
         slots = [s.slot for s in batch]
@@ -279,11 +289,15 @@ class Engine:
                 ctx.tables[name] = take(arr.size).view(arr.shape)
                 ctx.host_tables[name] = arr
                 take(-arr.size % 4)
+        if drafted or (decode and b > 1 and self.cache.shares_pages()):
+            ctx.shared = SharedRows(self, slots, seq.tolist(), pos.tolist())
         return ctx, d_want, slots, new_lengths
 
-    def step(self, batch: Sequence[SequenceStep]) -> torch.Tensor:
+    def step(self, batch: Sequence[SequenceStep], drafted: bool = False) -> torch.Tensor:
         """Run one step; returns float32 logits [wanted places, vocab] in the
-        order of the batch and of each sequence's ``want``.
+        order of the batch and of each sequence's ``want``.  ``drafted``: the sequences bring a few tokens
+        each after long contexts (drafts to be verified), so attention reads what a sequence's tokens, or
+        sequences that were forked, see alike once for all of them.
 
         Large prompt steps whose shape (token counts, start positions, number of
         wanted places) comes a second time are captured as a CUDA graph with buffers
@@ -293,7 +307,7 @@ class Engine:
         least recently used goes when there are more than ``MAX_STEP_GRAPHS``."""
         key = None
         if sum(len(s.tokens) for s in batch) >= GRAPH_MIN_TOKENS and \
-                any(len(s.tokens) > 1 for s in batch) and self._graph_safe:
+                any(len(s.tokens) > 1 for s in batch) and self._graph_safe and not drafted:
             key = (tuple(len(s.tokens) for s in batch),
                    tuple(self.cache.length(s.slot) for s in batch),  # refuses slots that are not held
                    tuple(len(s.want) for s in batch))
@@ -311,7 +325,7 @@ class Engine:
             if len(self._seen_shapes) >= MAX_SEEN_SHAPES:
                 self._seen_shapes.pop(next(iter(self._seen_shapes)))
             self._seen_shapes[key] = True
-        ctx, d_want, slots, new_lengths = self.prepare(batch)
+        ctx, d_want, slots, new_lengths = self.prepare(batch, drafted=drafted)
         logits = torch.empty((d_want.numel(), self.spec.vocab_size), dtype=torch.float32,
                              device=self.device)
         self.model.forward(ctx, d_want, logits)

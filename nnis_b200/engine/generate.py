@@ -20,8 +20,12 @@ go on where generation ended, as NNIS's sessions do
 (crates/nnis-model/src/runtime.rs:814-846, :1264-1268;
 crates/nnis-model/src/streaming.rs:14-20).
 
+With ``share_prefix`` prompts of a batch that begin with the same tokens (a page of them at least)
+run those once: one sequence takes them and is forked for the others, whose further tokens then
+run in one step; their pages are shared in the cache, and attention reads them once for all.
+
 The loop talks to a *backend* (``acquire_slot``, ``release_slot``, ``step``,
-``greedy``, ``host_rows``), so its decisions can be tested without a GPU.
+``greedy``, ``host_rows``; ``fork_slot`` for shared prefixes), so its decisions can be tested without a GPU.
 """
 from __future__ import annotations
 
@@ -89,10 +93,27 @@ def pages_needed(request: GenerationRequest) -> int:
              // PAGE_SIZE)
 
 
+def prefix_groups(requests: Sequence[GenerationRequest], indices: Sequence[int]) -> List[Tuple[List[int], int]]:
+    """(requests, tokens that all of them begin with) for every two and more of ``indices`` whose prompts begin with the same
+    page; every prompt keeps a token of its own.  Requests on a slot of their caller's take no part."""
+    by_page: Dict[tuple, List[int]] = {}
+    for i in indices:
+        if requests[i].slot is None and len(requests[i].prompt) > PAGE_SIZE:
+            by_page.setdefault(tuple(requests[i].prompt[:PAGE_SIZE]), []).append(i)
+    groups = []
+    for members in by_page.values():
+        if len(members) > 1:
+            prompts = [list(requests[i].prompt) for i in members]
+            low, high = min(prompts), max(prompts)  # (in the order of lists: what these share, all between them do)
+            most = min(map(len, prompts)) - 1
+            groups.append((members, next((n for n in range(most) if low[n] != high[n]), most)))
+    return groups
+
+
 def plan_batches(requests: Sequence[GenerationRequest], runnable: Sequence[bool], max_batch: int,
-                 max_pages: int) -> List[List[int]]:
+                 max_pages: int, share_prefix: bool = False) -> List[List[int]]:
     """Request indices per batch, in order; a batch closes when it is full or
-    the next request's pages would not fit beside it."""
+    the next request's pages would not fit beside it (pages of a shared prefix counted once)."""
     batches: List[List[int]] = []
     current: List[int] = []
     pages = 0
@@ -100,9 +121,14 @@ def plan_batches(requests: Sequence[GenerationRequest], runnable: Sequence[bool]
         if not runnable[i]:
             continue
         need = pages_needed(r)
+        if current and share_prefix:  # what the batch takes with it
+            both = [*current, i]
+            saved = sum((len(m) - 1) * (n // PAGE_SIZE) for m, n in prefix_groups(requests, both))
+            need = sum(pages_needed(requests[j]) for j in both) - saved - pages
         if current and (len(current) >= max_batch or pages + need > max_pages):
             batches.append(current)
             current, pages = [], 0
+            need = pages_needed(r)
         current.append(i)
         pages += need
     if current:
@@ -127,7 +153,8 @@ class Generator:
         self.device_sampling = device_sampling and hasattr(backend, "sample_temperature")
 
     # -- checks made before any work -------------------------------------------
-    def _refusal(self, r: GenerationRequest) -> Optional[str]:
+    def refusal(self, r: GenerationRequest) -> Optional[str]:
+        """Why the request cannot run; None where it can."""
         if len(r.prompt) == 0:
             return "the prompt is empty"
         for t in r.prompt:
@@ -193,15 +220,15 @@ class Generator:
 
     # -- the loop ------------------------------------------------------------------
     def generate(self, requests: Sequence[GenerationRequest],
-                 on_token: Optional[Callable[[int, int], Optional[StreamControl]]] = None
-                 ) -> List[GenerationResult]:
+                 on_token: Optional[Callable[[int, int], Optional[StreamControl]]] = None,
+                 share_prefix: bool = False) -> List[GenerationResult]:
         """``on_token(request index, token)`` is called as tokens are emitted; when it
         returns ``StreamControl.STOP`` that request ends there (``finish_reason``
-        "stop") and the others go on."""
+        "stop") and the others go on.  ``share_prefix``: see the module's docstring."""
         results = [GenerationResult(i) for i in range(len(requests))]
         runnable = []
         for i, r in enumerate(requests):
-            why = self._refusal(r)
+            why = self.refusal(r)
             if why is not None:
                 results[i].error, results[i].finish_reason = why, "error"
             runnable.append(why is None)
@@ -209,8 +236,8 @@ class Generator:
         samplers: Dict[int, HostLogitSampler] = {}
         self._samplers_for([i for i in range(len(requests)) if runnable[i]], requests, samplers)
         shown: Dict[int, int] = {}  # tokens of each request that the callback has been shown
-        for batch in plan_batches(requests, runnable, self.max_batch, self.max_pages):
-            failed = self._run_batch(batch, requests, results, samplers, on_token, shown)
+        for batch in plan_batches(requests, runnable, self.max_batch, self.max_pages, share_prefix):
+            failed = self._run_batch(batch, requests, results, samplers, on_token, shown, share_prefix)
             if failed is not None and len(batch) > 1:
                 # a step of the batch failed: each unfinished request again, alone;
                 # tokens that the callback has seen already are not shown again
@@ -233,7 +260,7 @@ class Generator:
                 results[i].error = f"{type(error).__name__}: {error}"
                 results[i].finish_reason = "error"
 
-    def _run_batch(self, batch, requests, results, samplers, on_token, shown) -> Optional[BaseException]:
+    def _run_batch(self, batch, requests, results, samplers, on_token, shown, share_prefix=False) -> Optional[BaseException]:
         """Runs the requests of ``batch`` together.  Returns the exception that ended
         the batch early, if any; requests it left unfinished have no finish reason.
         ``shown[i]``: how many tokens of request i the callback has been shown."""
@@ -253,11 +280,21 @@ class Generator:
             return on_token(i, t) is StreamControl.STOP
 
         try:
+            held = {i: 0 for i in batch}  # tokens of its prompt that a request's slot holds already
+            for members, tokens in prefix_groups(requests, batch) if share_prefix else ():
+                first = members[0]
+                slots[first] = self.backend.acquire_slot()
+                self.backend.step([SequenceStep(slots[first], list(requests[first].prompt[:tokens]), [])], need_logits=False)
+                for i in members:
+                    if i != first:
+                        slots[i] = self.backend.fork_slot(slots[first])
+                    held[i] = tokens
             for i in batch:
-                slots[i] = requests[i].slot if i in own else self.backend.acquire_slot()
+                if i not in slots:
+                    slots[i] = requests[i].slot if i in own else self.backend.acquire_slot()
             live = list(batch)
-            logits = self.backend.step([SequenceStep(slots[i], list(requests[i].prompt),
-                                                     [len(requests[i].prompt) - 1]) for i in live])
+            logits = self.backend.step([SequenceStep(slots[i], list(requests[i].prompt[held[i]:]),
+                                                     [len(requests[i].prompt) - held[i] - 1]) for i in live])
             if all(requests[i].sampling is None for i in batch) and \
                     getattr(self.backend, "decode_greedy", None) is not None and \
                     getattr(self.backend, "pipeline", True):

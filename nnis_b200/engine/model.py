@@ -95,6 +95,16 @@ class DecoderModel:
                 self.blocks[entry.layer].check_shared_cache(view)
             self._views.append(view)
         self._embedding_view = cache.view(len(self.spec.schedule))
+        keys = {}
+        for entry, view in zip(self.spec.schedule, self._views):
+            ask = getattr(self.blocks[entry.layer].mixer, "shared_key", None)
+            if ask is not None:
+                keys[ask(view)] = True
+        self._shared_keys = [k for k in keys if k is not None]
+
+    def shared_keys(self):
+        """The cache group and head layout of every attention that can read pages shared by several rows once."""
+        return self._shared_keys
 
     def step_tables(self, counts, starts) -> Dict[str, object]:
         """The work lists that the scheduled blocks want uploaded for a prompt step."""

@@ -1,0 +1,106 @@
+"""Which steps read shared pages once for several rows, and the plans they do it by.
+
+Rows share pages where their sequences were forked from one another (``CacheManager.fork``) and, with
+several tokens of a sequence in one step, where those see the same pages.  A step's context asks for
+the plan (``ops.SharedPlan``) of a cache group and a head layout: ``SharedRows`` makes it then, for a step
+that is launched kernel by kernel; ``KeptPlans`` holds plans of a captured step at addresses that stay.
+"""
+from __future__ import annotations
+
+from typing import Dict, Optional, Sequence, Tuple
+
+from ..cache import PAGE_SIZE
+from ..csrc import ops
+
+# Sharing has to take this many pages, and this part of them, off what the rows read one by one.
+LEAST_PAGES, LEAST_PART = 16, 0.25
+AHEAD = 8  # pages that a captured step's plan lets its sequences grow by
+
+PlanKey = Tuple[int, int, int, int]  # cache group, heads, key/value heads, head size
+
+
+def shared_tree(cache, group: int, slots: Sequence[int], seqs: Sequence[int], positions: Sequence[int], ahead: int = 0):
+    """(nodes, tails) of the rows' pages (``ops.shared_nodes``), or None where sharing does not pay."""
+    if cache.groups[group].window > 0:
+        return None
+    nodes, tails = ops.shared_nodes([cache.page_table(group, s) for s in slots], seqs, positions, ahead)
+    saved = sum((len(rows) - 1) * (b - a) for rows, a, b in nodes)
+    read = sum(p // PAGE_SIZE + 1 for p in positions if p >= 0)
+    return (nodes, tails) if saved >= max(LEAST_PAGES, LEAST_PART * read) else None
+
+
+class SharedRows:
+    """The plans of one step: the sequence (a place in ``slots``) and the position of every row."""
+
+    def __init__(self, engine, slots: Sequence[int], seqs: Sequence[int], positions: Sequence[int]):
+        self.engine, self.slots, self.seqs, self.positions = engine, slots, seqs, positions
+        self._trees: Dict[int, Optional[tuple]] = {}
+        self._plans: Dict[PlanKey, Optional[ops.SharedPlan]] = {}
+
+    def plan(self, *key) -> Optional[ops.SharedPlan]:
+        if key not in self._plans:
+            group, e = key[0], self.engine
+            if group not in self._trees:
+                self._trees[group] = shared_tree(e.cache, group, self.slots, self.seqs, self.positions)
+            tree = self._trees[group]
+            self._plans[key] = None if tree is None else ops.attention_shared_plan_of(
+                *tree, self.seqs, self.positions, *key[1:], e.dtype, e.device)
+        return self._plans[key]
+
+
+class KeptPlans:
+    """The plans of a captured step of ``rows`` rows: each as large as ``rooms`` says, its contents replaced by ``fill``."""
+
+    def __init__(self, engine, rows: int, cols: int, rooms: Sequence[Tuple[PlanKey, tuple]]):
+        self.plans = {key: ops.SharedPlan.with_room(rows, *key[1:], engine.dtype, engine.device, room, cols) for key, room in rooms}
+        self._filled = None
+
+    def plan(self, *key) -> Optional[ops.SharedPlan]:
+        return self.plans.get(key)
+
+    def fill(self, units: Dict[PlanKey, tuple]) -> None:
+        if units is not self._filled:
+            for key, plan in self.plans.items():
+                plan.fill(*units[key])
+            self._filled = units
+
+
+class BatchUnits:
+    """What a batch of single tokens shares, for captured steps: made anew when its sequences, what they share, or how
+    far they may grow have changed."""
+
+    def __init__(self, engine):
+        self.engine = engine
+        self._made_for = self._positions = self._units = None
+        self._until = 0
+
+    def units(self, slots: Sequence[int], positions: Sequence[int], rows: int, ahead: int = AHEAD) -> Optional[Dict[PlanKey, tuple]]:
+        """Per attention of the model that gains by it, its units, members and record offsets, for ``rows`` rows of which
+        the first are the sequences; None where none gains."""
+        cache = self.engine.cache
+        if len(slots) < 2 or not cache.shares_pages():
+            return None
+        made_for = (tuple(slots), cache.share_epoch, rows)
+        if made_for == self._made_for and all(0 <= now - then <= self._until for now, then in zip(positions, self._positions)):
+            return self._units
+        seqs, padding = list(range(len(slots))), rows - len(slots)
+        trees: Dict[int, Optional[tuple]] = {}
+        units = {}
+        for key in self.engine.model.shared_keys():
+            if key[0] not in trees:
+                trees[key[0]] = shared_tree(cache, key[0], slots, seqs + [0] * padding, list(positions) + [-1] * padding, ahead)
+            if trees[key[0]] is not None:
+                units[key] = ops.attention_shared_units(*trees[key[0]], seqs + [0] * padding, *key[1:], self.engine.dtype,
+                                                        self.engine.device)
+        self._made_for, self._positions, self._until = made_for, list(positions), ahead * PAGE_SIZE
+        self._units = units or None
+        return self._units
+
+
+def rooms_of(units: Optional[Dict[PlanKey, tuple]]) -> Optional[tuple]:
+    """The sizes, in powers of two, of plans that hold these units: part of a captured step's key."""
+    if units is None:
+        return None
+    up = lambda n: 0 if n == 0 else 1 << (n - 1).bit_length()
+    return tuple(sorted((key, (*(up(len(k)) for k in kinds), up(max(1, len(members))), up(max(1, int(record[-1])))))
+                        for key, (kinds, members, record) in units.items()))

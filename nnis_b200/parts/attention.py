@@ -91,6 +91,12 @@ class Attention(Part):
                 (self.kv_heads, view.page_size, self.head_dim) or view.window != self.window:
             raise ValueError("the shared cache does not fit this attention's heads or window")
 
+    def shared_key(self, view: KVView):
+        """What a plan for pages that several rows share is made for (None: this attention reads them row by row)."""
+        if self.window > 0 or not ops.attention_shared_takes(self.head_dim, view.page_size):
+            return None
+        return view.group, self.heads, self.kv_heads, self.head_dim
+
     def step_flops(self, counts, starts) -> float:
         d, nq, nkv, H = self.head_dim, self.heads, self.kv_heads, self.hidden
         tokens = sum(counts)
@@ -229,9 +235,12 @@ class Attention(Part):
         # the tensor-core decode attention: a CTA per (kv head, up to 16 query heads, slice)
         mma_decode = self.dtype == torch.bfloat16 and ctx.decode and n <= 65535 \
             and ops.attention_decode_mma_takes(d, cache.page_size)
+        # rows whose sequences begin with the same pages read those once for all of them
+        key = self.shared_key(cache) if ctx.shared is not None else None
+        shared = ctx.shared.plan(*key) if key is not None else None
         # ... or, with few sequences, short slices whose pages are all in shared memory at once
         tma_splits = ops.attention_decode_tma_plan(
-            n, nq, nkv, d, cache.page_size, table.shape[1], self.device, ctx.share) if mma_decode else 0
+            n, nq, nkv, d, cache.page_size, table.shape[1], self.device, ctx.share) if mma_decode and shared is None else 0
         if begun is not None or self._decode_kernels(ctx, n, normed=hidden is not None):
             q = ws.get("q", (n, nq * d), self.dtype)
             if begun is not None:
@@ -268,7 +277,9 @@ class Attention(Part):
                            sin, cache.k if self.own_kv else None, cache.v if self.own_kv else None,
                            nq, self.stored_kv, d, cache.page_size)
             q_buf, q_stride = qkv, qkv.shape[1]
-        if tma_splits:
+        if shared is not None:
+            ops.attention_shared(q_buf, q_stride, cache.k, cache.v, ctx.token_pos, table, shared, attn, nq, nkv, d, self.scale, ws)
+        elif tma_splits:
             partial = tickets = None
             if tma_splits > 1:
                 partial = ws.get("attn_partial", (n * nq * tma_splits * (d + 2),), torch.float32)

@@ -8,6 +8,8 @@ from typing import Optional
 import torch
 
 from ..csrc import ops
+from .config import SamplingConfig, SamplingError
+from .host import SplitMix64
 
 
 def greedy(logits: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
@@ -45,3 +47,27 @@ def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, first_row: torch.T
     them) ends its sequence there: picked is -1.  Offsets that no packed rows have give 0 and -1."""
     ops.verify_drafts(logits, drafts, first_row, temperatures, accept_draws, pick_draws, accepted, picked, draft_logits,
                       workspace)
+
+
+class DraftVerifier:
+    """``verify_drafts`` for one sequence whose drafts are host numbers: draws from a SplitMix64 of the policy's seed, an
+    accept draw a draft and then the pick's, every time; without a policy greedy."""
+
+    def __init__(self, device, workspace, sampling: Optional[SamplingConfig]):
+        self.device, self.workspace = device, workspace
+        self.temperature = 0.0 if sampling is None else float(sampling.temperature)
+        self._rng = SplitMix64(0 if sampling is None else sampling.seed)
+        self._temperatures = torch.full((1,), self.temperature, dtype=torch.float32, device=device)
+        self._out = torch.empty((2, 1), dtype=torch.int32, device=device)
+
+    def verify(self, logits: torch.Tensor, drafts, draft_logits: Optional[torch.Tensor]):
+        """(drafts kept, the token after them) by the logits' k + 1 rows; ``SamplingError`` where a row has no probability."""
+        k = len(drafts)
+        draws = torch.tensor([self._rng.next_unit_f64() for _ in range(k + 1)], dtype=torch.float64, device=self.device)
+        ints = torch.tensor([*drafts, 0, k + 1], dtype=torch.int32, device=self.device)
+        verify_drafts(logits, ints[:k], ints[k:], self._temperatures, draws[:k], draws[k:], self._out[0], self._out[1],
+                      draft_logits, self.workspace)
+        kept, token = self._out.reshape(-1).tolist()
+        if token < 0:
+            raise SamplingError("sampling softmax produced no positive finite probability mass")
+        return kept, token

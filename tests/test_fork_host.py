@@ -252,3 +252,50 @@ def test_any_order_of_forks_steps_truncations_releases_and_moves(seed):
     for s in list(w.marks):
         w.release(s)
     assert w.cache.usage()["pages_held"] == [0, 0] and not w.cache.shares_pages()
+
+
+# ---- the generation loop above it ------------------------------------------------------------------
+def test_prompts_that_begin_alike_run_that_once():
+    from nnis_b200.engine.generate import GenerationConfig, GenerationRequest, pages_needed, plan_batches, prefix_groups
+    from test_generation_host import ScriptedBackend, expected, gen
+
+    class Forking(ScriptedBackend):
+        def fork_slot(self, slot):
+            new = self.acquire_slot()
+            self.held[new] = list(self.held[slot])
+            return new
+
+    long = [(i * 7) % 50 for i in range(70)]
+    prompts = [long + [1, 2], [3], long + [1], long + [1, 2], [5] * 70, long[:PAGE_SIZE]]
+    reqs = [GenerationRequest(p, GenerationConfig(4)) for p in prompts]
+    assert prefix_groups(reqs, range(6)) == [([0, 2, 3], 70)]
+    assert prefix_groups(reqs, [0, 3]) == [([0, 3], 71)]  # (each keeps a token of its own)
+    b = Forking()
+    res = gen(b, max_batch=8).generate(reqs, share_prefix=True)
+    assert [r.token_ids for r in res] == [expected(p, 4) for p in prompts] and not b.held
+    assert [n for _, n in b.steps[0]] == [70] and sorted(n for _, n in b.steps[1]) == [1, 1, 2, 2, 64, 70]
+    plain = ScriptedBackend()
+    assert [r.token_ids for r in gen(plain, max_batch=8).generate(reqs)] == [r.token_ids for r in res]
+    assert len(plain.steps[0]) == 6
+
+    pages = [pages_needed(r) for r in reqs]
+    assert pages == [2, 1, 2, 2, 2, 2]
+    assert plan_batches(reqs, [True] * 6, 8, 5) == [[0, 1, 2], [3, 4], [5]]
+    assert plan_batches(reqs, [True] * 6, 8, 5, True) == [[0, 1, 2, 3], [4, 5]]  # 2 + 1 + 1 + 1
+    # a batch whose shared prompt fails is run request by request, without sharing
+    b = Forking(fail_on_step=1)
+    res = gen(b).generate(reqs[:3], share_prefix=True)
+    assert [r.token_ids for r in res] == [expected(p, 4) for p in prompts[:3]] and not b.held
+
+
+def test_drafts_looked_up_in_the_text():
+    from nnis_b200 import LookupDrafter
+    d = LookupDrafter(2)
+    assert d.propose([1, 2, 3, 4, 1, 2], 3, 0.0) == ([3, 4, 1], None)
+    assert d.propose([1, 2, 3, 4, 1, 2, 3], 2, 0.0) == ([4, 1], None)
+    assert d.propose([1, 2, 3, 4, 1, 2, 3, 9], 2, 0.0) == ([], None)
+    assert d.propose([7, 7], 5, 0.0) == ([7], None)  # another sequence
+    d.begin()
+    assert d.propose([5], 2, 0.0) == ([], None)
+    with pytest.raises(ValueError):
+        LookupDrafter(0)
