@@ -22,7 +22,7 @@ struct SharedUnit {   // eight ints of the plan
     int page_begin, page_end;  // columns of the page table
     int slot;         // which of each row's records it writes
     int seq;          // row of the page table that names the pages
-    int ends;         // 1: keys beyond the row's own position are hidden (all entries are of one token row)
+    int ends;         // 1 + token row: all entries are of that row, and keys beyond its position are hidden; 0: all see all
 };
 
 constexpr int kSharedPage = 64;  // keys of a page
@@ -110,32 +110,68 @@ __device__ __forceinline__ void merge_row(const float* partial, const float2* su
     }
 }
 
-// After all threads of a CTA have written their unit's records: the rows that these complete are merged here.  `done`: an
-// int per entry of shared memory.  Every thread of the CTA calls it.
+// After all threads of a CTA have written their unit's records: the rows that these complete are merged here, a thread four (or
+// two) values of an entry at a time, its records asked for eight at once.  For units whose entries have few records.  `done`: an
+// int4 per entry of shared memory that nothing else uses.  Every thread of the CTA calls it.
 template <typename T, int THREADS>
-__device__ __forceinline__ void merge_finished(const SharedArgs& a, const SharedUnit& u, int hk, int G, int* done) {
+__device__ __forceinline__ void merge_finished(const SharedArgs& a, const SharedUnit& u, int hk, int G, int4* done) {
     __syncthreads();  // (the fence below covers what the others wrote before this)
     const int* members = a.members + u.members;
+    const float2* sums = reinterpret_cast<const float2*>(a.sums);
     for (int e = threadIdx.x; e < u.entries; e += THREADS) {
         const int at = u.entry + e, row = members[at / G];
         unsigned* ticket = a.tickets + (size_t)row * a.nq + hk * G + at % G;
         __threadfence();
-        const bool last = atomicAdd(ticket, 1u) == (unsigned)(a.record[row + 1] - a.record[row]) - 1u;
+        const int first = a.record[row], count = a.record[row + 1] - first;
+        const bool last = atomicAdd(ticket, 1u) == (unsigned)count - 1u;
         if (last) *ticket = 0u;
-        done[e] = last;
+        done[e] = make_int4(last ? count : 0, first, row, hk * G + at % G);
     }
     __syncthreads();
     __threadfence();
-    for (int e = threadIdx.x >> 5; e < u.entries; e += THREADS / 32) {
-        if (!done[e]) continue;
-        const int at = u.entry + e, row = members[at / G], first = a.record[row];
-        merge_row<T, 16>(a.partial, reinterpret_cast<const float2*>(a.sums), first, a.record[row + 1] - first, row, hk * G + at % G,
-                         a.nq, a.d, static_cast<T*>(a.out));
+    const int d = a.d, pairs = d / 2;
+    for (int item = threadIdx.x; item < u.entries * pairs; item += THREADS) {
+        const int e = item / pairs, i = 2 * (item % pairs);
+        const int count = done[e].x, first = done[e].y, row = done[e].z, head = done[e].w;
+        if (!count) continue;
+        float m = -INFINITY, l = 0.f;
+        float2 acc = make_float2(0.f, 0.f);
+        constexpr int kAhead = 8;
+        for (int s0 = 0; s0 < count; s0 += kAhead) {
+            float2 ml[kAhead], v[kAhead];
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+                const size_t rec = (size_t)(first + s0 + k) * a.nq + head;
+                const bool there = s0 + k < count;
+                ml[k] = there ? __ldcg(sums + rec) : make_float2(-INFINITY, 0.f);
+                v[k] = there ? __ldcg(reinterpret_cast<const float2*>(a.partial + rec * d + i)) : make_float2(0.f, 0.f);
+            }
+            float top = m;
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k)
+                if (ml[k].y != 0.f) top = fmaxf(top, ml[k].x);
+            const float keep = m == -INFINITY ? 0.f : exp2f(m - top);
+            l *= keep;
+            acc.x *= keep;
+            acc.y *= keep;
+            m = top;
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+                if (ml[k].y == 0.f) continue;  // (a record that holds nothing is never added)
+                const float f = exp2f(ml[k].x - m);
+                l = fmaf(ml[k].y, f, l);
+                acc.x = fmaf(f, v[k].x, acc.x);
+                acc.y = fmaf(f, v[k].y, acc.y);
+            }
+        }
+        const float inv = l != 0.f ? 1.0f / l : 0.f;
+        store2(static_cast<T*>(a.out) + ((size_t)row * a.nq + head) * d + i, acc.x * inv, acc.y * inv);
     }
 }
 
 // One launch of the named form over `n_units` units; each is defined in its own file.
 cudaError_t shared_units_any(const SharedArgs& a, int n_units, int tile, bool f32, cudaStream_t stream);
+cudaError_t shared_units_warp(const SharedArgs& a, int n_units, int* status, cudaStream_t stream);
 cudaError_t shared_units_mma(const SharedArgs& a, int n_units, cudaStream_t stream);
 cudaError_t shared_units_tc(const SharedArgs& a, int n_units, int* status, cudaStream_t stream);
 

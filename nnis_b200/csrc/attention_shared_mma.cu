@@ -11,7 +11,7 @@
 
 namespace nnis {
 
-constexpr int kSmWarps = 4, kSmThreads = kSmWarps * 32, kSmEntries = 32;
+constexpr int kSmWarps = 4, kSmThreads = kSmWarps * 32;
 
 template <int D>
 constexpr int sm_stages() { return D == 64 ? 4 : 3; }
@@ -22,32 +22,37 @@ __device__ __forceinline__ void cp_async16_or_zero(void* dst, const void* src, b
 }
 
 template <int D>
-__global__ void __launch_bounds__(kSmThreads)
+__global__ void __launch_bounds__(kSmThreads, D == 64 ? 3 : 2)
 attn_shared_mma_kernel(const SharedArgs a) {
-    constexpr int CH = D / 8, NT = D / 8, KS = D / 16, STAGES = sm_stages<D>();
+    constexpr int CH = D / 8, NT = D / 8, KS = D / 16, STAGES = sm_stages<D>(), MT = 2, kSmEntries = 16 * MT;  // (MT tiles of 16 entries)
     extern __shared__ __align__(128) unsigned char smem_raw[];
     bf16* q_s = reinterpret_cast<bf16*>(smem_raw);  // [32, D] swizzled
     bf16* tiles = q_s + kSmEntries * D;             // stages x (K [64, D], V [64, D])
     __shared__ float sm_ml[kSmWarps][kSmEntries][2];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    // The plan, the positions and the page ids are older than the kernel before this one, which writes the queries and this
+    // step's keys and values: they are asked for ahead of the wait for it, the ids beside the position.
     const SharedUnit u = a.units[blockIdx.x];
     const int hk = blockIdx.y, G = a.nq / a.nkv;
     const int* members = a.members + u.members;
+    const int* table = a.page_table + (size_t)u.seq * a.table_cols + u.page_begin;
+    const int some = min(u.page_end, a.table_cols) - u.page_begin;  // (a tail may be given room to grow)
+    const int ids = lane < some ? table[lane] : -1;  // a lane a page, up to 32 of them
+    const int pos = u.ends ? a.token_pos[u.ends - 1] : 0x7fffffff;
+    const int n_pages = u.ends ? min(some, pos < 0 ? 0 : pos / kSharedPage + 1 - u.page_begin) : some;
     units_begin(a);
     const bool two = u.entries > 16;  // the second tile of 16 entries holds any
-    const int pos = u.ends ? a.token_pos[members[u.entry / G]] : 0x7fffffff;
-    const int n_pages = (u.ends ? min(u.page_end, pos < 0 ? 0 : pos / kSharedPage + 1) : u.page_end) - u.page_begin;
-    const int* table = a.page_table + (size_t)u.seq * a.table_cols + u.page_begin;
     const bf16 *k_cache = static_cast<const bf16*>(a.k_cache), *v_cache = static_cast<const bf16*>(a.v_cache);
     constexpr size_t kTile = (size_t)kSharedPage * D;
 
+    auto page_of = [&](int it) { return it < 32 ? __shfl_sync(0xffffffffu, ids, it) : table[it]; };
     // keys of page `it` that the unit's rows see (0 where the table has a gap)
     auto keys_of = [&](int it, int page) {
         return page < 0 || page >= a.pages ? 0 : u.ends ? min(kSharedPage, pos + 1 - (u.page_begin + it) * kSharedPage) : kSharedPage;
     };
     auto load_page = [&](int it) {
         if (it < n_pages) {
-            const int page = table[it], keys = keys_of(it, page);
+            const int page = page_of(it), keys = keys_of(it, page);
             const size_t from = (size_t)((keys ? page : 0) * (long long)a.nkv + hk) * kTile;
             bf16* kd = tiles + (size_t)(it % STAGES) * 2 * kTile;
             bf16* vd = kd + kTile;
@@ -72,9 +77,9 @@ attn_shared_mma_kernel(const SharedArgs a) {
         *reinterpret_cast<uint4*>(q_s + swz<D>(e, chunk)) = x;
     }
     const int r_lo = lane >> 2, c_lo = (lane & 3) * 2;
-    float o[2][NT][4], m_run[2][2], l_run[2][2];
+    float o[MT][NT][4], m_run[MT][2], l_run[MT][2];
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
+    for (int t = 0; t < MT; ++t) {
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -90,11 +95,11 @@ attn_shared_mma_kernel(const SharedArgs a) {
         load_page(it + STAGES - 1);
         const bf16* kt = tiles + (size_t)(it % STAGES) * 2 * kTile;
         const bf16* vt = kt + kTile;
-        const int keys = keys_of(it, table[it]);
-        uint32_t pa[2][4];
-        float alpha[2][2];
+        const int keys = keys_of(it, page_of(it));
+        uint32_t pa[MT][4];
+        float alpha[MT][2];
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
+        for (int t = 0; t < MT; ++t) {
             if (t && !two) break;
             float s[2][4];
 #pragma unroll
@@ -157,8 +162,8 @@ attn_shared_mma_kernel(const SharedArgs a) {
             mma_bf16(o[0][j], pa[0], vb[0], vb[1]);
             mma_bf16(o[0][j + 1], pa[0], vb[2], vb[3]);
             if (two) {
-                mma_bf16(o[1][j], pa[1], vb[0], vb[1]);
-                mma_bf16(o[1][j + 1], pa[1], vb[2], vb[3]);
+                mma_bf16(o[MT - 1][j], pa[MT - 1], vb[0], vb[1]);
+                mma_bf16(o[MT - 1][j + 1], pa[MT - 1], vb[2], vb[3]);
             }
         }
     }
@@ -166,7 +171,7 @@ attn_shared_mma_kernel(const SharedArgs a) {
     __syncthreads();  // everyone is done with the tiles: the warps' outputs meet there
     float* o_s = reinterpret_cast<float*>(smem_raw);  // [warps, 16, D], one tile of entries after the other
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
+    for (int t = 0; t < MT; ++t) {
         if (t && !two) break;
         if (t) __syncthreads();
 #pragma unroll
@@ -211,20 +216,17 @@ attn_shared_mma_kernel(const SharedArgs a) {
             *reinterpret_cast<float4*>(a.partial + rec * D + c * 4) = x;
         }
     }
-    if (a.tickets) merge_finished<bf16, kSmThreads>(a, u, hk, G, reinterpret_cast<int*>(q_s));
+    if (a.tickets) merge_finished<bf16, kSmThreads>(a, u, hk, G, reinterpret_cast<int4*>(tiles + 4 * kTile));
     units_end(a);
 }
 
 template <int D>
 static cudaError_t launch_small(const SharedArgs& a, int n_units, cudaStream_t stream) {
-    const size_t tiles = (kSmEntries * D + sm_stages<D>() * 2 * (size_t)kSharedPage * D) * sizeof(bf16);
-    const size_t merge = (size_t)kSmWarps * 16 * D * sizeof(float), smem = tiles > merge ? tiles : merge;
+    const size_t tiles = (32 * D + sm_stages<D>() * 2 * (size_t)kSharedPage * D) * sizeof(bf16);
     auto kernel = attn_shared_mma_kernel<D>;
-    if (smem > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (e != cudaSuccess) return e;
-    }
-    return launch_dependent(kernel, dim3(n_units, a.nkv), kSmThreads, smem, stream, a);
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)tiles);
+    if (e != cudaSuccess) return e;
+    return launch_dependent(kernel, dim3(n_units, a.nkv), kSmThreads, tiles, stream, a);
 }
 
 cudaError_t shared_units_mma(const SharedArgs& a, int n_units, cudaStream_t stream) {

@@ -2843,15 +2843,17 @@ class SharedPlan:
     its rows stay at the positions that it was made for and their page lists do not change (and, made with pages
     ``ahead``, while they grow by no more)."""
 
-    def __init__(self, rows, heads, kv_heads, head_dim, dtype, counts, members, ints, records, seqs, cols):
+    def __init__(self, rows, heads, kv_heads, head_dim, dtype, counts, members, ints, records, seqs, cols,
+                 most_entries=1 << 20):
         self.rows, self.heads, self.kv_heads, self.head_dim, self.dtype = rows, heads, kv_heads, head_dim, dtype
         self.counts, self.members_held, self.ints, self.records, self.seqs, self.cols = counts, members, ints, records, seqs, cols
         self.form = int(_shared_on_tensor_cores(dtype, head_dim))
         at = ints.data_ptr()
         self.units, self.members = at, at + 32 * sum(counts)
         self.record = self.members + 4 * members
-        # rows merged by the CTA that completes them save a launch, where a CTA has few of them to merge
-        self.merged_inside = counts[2] == 0 and sum(counts) * kv_heads <= 148 and records <= 4 * rows
+        # rows merged by the CTA that completes them save a launch, where a CTA has little to merge
+        self.merged_inside = most_entries * head_dim <= 1024 and counts[2] == 0 and (self.form == 0 or counts[0] == 0) \
+            and sum(counts) * kv_heads <= 148 and records <= 8 * rows
         self.device, self.status = ints.device, status_word(ints.device).data_ptr()
         self.launches = (not self.merged_inside) + sum(c > 0 for c in counts)
 
@@ -2887,8 +2889,12 @@ def _shared_on_tensor_cores(dtype: torch.dtype, head_dim: int) -> bool:
 def attention_shared_units(nodes, tails, seqs, heads: int, kv_heads: int, head_dim: int, dtype: torch.dtype, device):
     """(units of every kind, members, record offsets) of a batch's tree of pages (``shared_nodes``)."""
     sms = sm_count(device)
-    kinds = ((0, 0, 0, 0), (32, 6 * sms, 2, 16), (128, 2 * sms, 2, 1 << 20)) if _shared_on_tensor_cores(dtype, head_dim) else \
-        ((16, 4 * sms, 2, 16), (64, 4 * sms, 2, 16), (0, 0, 0, 0))
+    if _shared_on_tensor_cores(dtype, head_dim):
+        # (small units go warp by warp where they are many; else that is only a launch more)
+        pieces = sum(len(rows) * (heads // kv_heads) <= 16 for rows, *_ in nodes) + (len(tails) if heads // kv_heads <= 16 else 0)
+        kinds = ((16 if pieces * kv_heads > 2 * sms else 0, 12 * sms, 4, 16), (32, 3 * sms, 4, 16), (128, 2 * sms, 2, 1 << 20))
+    else:
+        kinds = ((16, 4 * sms, 2, 16), (64, 4 * sms, 2, 16), (0, 0, 0, 0))
     return shared_units(nodes, tails, seqs, heads // kv_heads, kv_heads, kinds, 1)
 
 
@@ -2898,7 +2904,8 @@ def attention_shared_plan_of(nodes, tails, seqs, positions, heads: int, kv_heads
     kinds, members, record = attention_shared_units(nodes, tails, seqs, heads, kv_heads, head_dim, dtype, device)
     ints = np.concatenate([k.reshape(-1) for k in kinds] + [members, record]).astype(np.int32)
     return SharedPlan(len(seqs), heads, kv_heads, head_dim, dtype, [len(k) for k in kinds], len(members),
-                      torch.from_numpy(ints).to(device), int(record[-1]), 1 + max(seqs), max([p // 64 + 1 for p in positions] + [1]))
+                      torch.from_numpy(ints).to(device), int(record[-1]), 1 + max(seqs), max([p // 64 + 1 for p in positions] + [1]),
+                      max(int(k[:, 2].max()) for k in kinds if len(k)))
 
 
 def attention_shared_plan(tables, seqs, positions, heads: int, kv_heads: int, head_dim: int, dtype: torch.dtype,

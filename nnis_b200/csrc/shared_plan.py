@@ -82,7 +82,7 @@ def shared_units(nodes: Sequence[tuple], tails: Sequence[tuple], seqs: Sequence[
     them."""
     pieces = []  # (rows, first, end, ends, kind)
     total = [0] * len(kinds)
-    for rows, a, b, ends in [(*n, 0) for n in nodes] + [([r], a, b, 1) for r, a, b in tails]:
+    for rows, a, b, ends in [(*n, 0) for n in nodes] + [([r], a, b, 1 + r) for r, a, b in tails]:
         entries = len(rows) * group
         may = [i for i, k in enumerate(kinds) if k[0] and (not ends or i <= ending)]
         kind = next((i for i in may if entries <= kinds[i][0]), may[-1])
