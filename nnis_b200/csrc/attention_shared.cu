@@ -183,11 +183,11 @@ cudaError_t shared_units_any(const SharedArgs& a, int n_units, int tile, bool f3
 }  // namespace nnis
 
 // units: n[0] units of the first kind, n[1] of the second, n[2] of the third.  `form` 0 (any even head size, float32 or
-// bfloat16): at most 16, at most 64 entries, none; `form` 1 (bfloat16, heads of 64 and 128): at most 16, 32 and 128, the last
+// bfloat16) and 2 (float32, heads of 64 and 128): at most 16, at most 64 entries, none; `form` 1 (bfloat16, heads of 64 and 128): at most 16, 32 and 128, the last
 // of which cover only positions that all their rows see.  The plan (units, members, record) is the host's, made of
 // page lists that the call's page table agrees with; page ids outside the store hold no keys.  partial: records x nq x d floats,
 // sums: records x nq x 2.  tickets (n_tokens x nq counters, zero, left zero): every row is merged by the CTA that completes it, and no
-// merge is launched (where all units are of the second kind, or `form` is 0); every row then has a record.
+// merge is launched (where all units are of the second kind, or `form` is not 1); every row then has a record.
 NNIS_API int nnis_attention_shared(const void* q, int q_stride, const void* k_cache, const void* v_cache, const int* token_pos,
                                    const int* page_table, int table_cols, const int* units, int n0, int n1, int n2,
                                    const int* members, const int* record, float* partial, float* sums, unsigned* tickets, void* out, int n_tokens,
@@ -200,10 +200,12 @@ NNIS_API int nnis_attention_shared(const void* q, int q_stride, const void* k_ca
     if (page_size != kSharedPage || d < 2 || d > 256 || d % 2 || nkv > 65535) return NNIS_ERR_UNSUPPORTED;
     const bool f32 = dtype == NNIS_DTYPE_F32;
     if (form == 1 && (f32 || (d != 64 && d != 128))) return NNIS_ERR_UNSUPPORTED;
+    if (form == 2 && (!f32 || (d != 64 && d != 128))) return NNIS_ERR_UNSUPPORTED;
+    if (form < 0 || form > 2) return NNIS_ERR_ARGUMENT;
     if ((n2 && form != 1) || (tickets && (n2 || (n0 && form == 1)))) return NNIS_ERR_UNSUPPORTED;
     if ((uintptr_t)units % 16 || (uintptr_t)partial % 16 || (uintptr_t)sums % 8) return NNIS_ERR_ALIGNMENT;
     const uintptr_t all = (uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache;
-    if (all % (form == 1 ? 16 : f32 ? 8 : 4) || (uintptr_t)out % (f32 ? 8 : 4) || (form == 1 && q_stride % 8)) return NNIS_ERR_ALIGNMENT;
+    if (all % (form ? 16 : f32 ? 8 : 4) || (uintptr_t)out % (f32 ? 8 : 4) || (form && q_stride % (f32 ? 4 : 8))) return NNIS_ERR_ALIGNMENT;
     SharedArgs a = {q,       k_cache, v_cache, token_pos, page_table, reinterpret_cast<const SharedUnit*>(units), members, record,
                     partial, sums,    tickets, out,       q_stride,   table_cols, pages,   nq,     nkv, d, scale, 0};
     // (the large units first: the small ones end what is left of the device)
@@ -212,7 +214,8 @@ NNIS_API int nnis_attention_shared(const void* q, int q_stride, const void* k_ca
         const int n = kind == 2 ? n2 : kind == 1 ? n1 : n0;
         if (!n) continue;
         a.units = first + (kind == 2 ? n0 + n1 : kind == 1 ? n0 : 0);
-        const cudaError_t e = form != 1   ? shared_units_any(a, n, kind == 1 ? 64 : 16, f32, stream)
+        const cudaError_t e = form == 0   ? shared_units_any(a, n, kind == 1 ? 64 : 16, f32, stream)
+                              : form == 2 ? shared_units_f32(a, n, kind == 1 ? 64 : 16, stream)
                               : kind == 2 ? shared_units_tc(a, n, status, stream)
                                           : kind == 1 ? shared_units_mma(a, n, stream)
                                           : shared_units_warp(a, n, status, stream);

@@ -171,6 +171,7 @@ __device__ __forceinline__ void merge_finished(const SharedArgs& a, const Shared
 
 // One launch of the named form over `n_units` units; each is defined in its own file.
 cudaError_t shared_units_any(const SharedArgs& a, int n_units, int tile, bool f32, cudaStream_t stream);
+cudaError_t shared_units_f32(const SharedArgs& a, int n_units, int tile, cudaStream_t stream);
 cudaError_t shared_units_warp(const SharedArgs& a, int n_units, int* status, cudaStream_t stream);
 cudaError_t shared_units_mma(const SharedArgs& a, int n_units, cudaStream_t stream);
 cudaError_t shared_units_tc(const SharedArgs& a, int n_units, int* status, cudaStream_t stream);

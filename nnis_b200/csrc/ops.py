@@ -2847,12 +2847,12 @@ class SharedPlan:
                  most_entries=1 << 20):
         self.rows, self.heads, self.kv_heads, self.head_dim, self.dtype = rows, heads, kv_heads, head_dim, dtype
         self.counts, self.members_held, self.ints, self.records, self.seqs, self.cols = counts, members, ints, records, seqs, cols
-        self.form = int(_shared_on_tensor_cores(dtype, head_dim))
+        self.form = _shared_form(dtype, head_dim)
         at = ints.data_ptr()
         self.units, self.members = at, at + 32 * sum(counts)
         self.record = self.members + 4 * members
         # rows merged by the CTA that completes them save a launch, where a CTA has little to merge
-        self.merged_inside = most_entries * head_dim <= 1024 and counts[2] == 0 and (self.form == 0 or counts[0] == 0) \
+        self.merged_inside = most_entries * head_dim <= 1024 and counts[2] == 0 and (self.form != 1 or counts[0] == 0) \
             and sum(counts) * kv_heads <= 148 and records <= 8 * rows
         self.device, self.status = ints.device, status_word(ints.device).data_ptr()
         self.launches = (not self.merged_inside) + sum(c > 0 for c in counts)
@@ -2882,19 +2882,21 @@ def attention_shared_takes(head_dim: int, page_size: int) -> bool:
     return page_size == 64 and head_dim % 2 == 0 and 2 <= head_dim <= 256
 
 
-def _shared_on_tensor_cores(dtype: torch.dtype, head_dim: int) -> bool:
-    return dtype == torch.bfloat16 and head_dim in (64, 128)
+def _shared_form(dtype: torch.dtype, head_dim: int) -> int:
+    """Which kernels: 1 tensor cores, 2 float32 heads of 64 and 128, 0 all others."""
+    return 0 if head_dim not in (64, 128) else 1 if dtype == torch.bfloat16 else 2
 
 
 def attention_shared_units(nodes, tails, seqs, heads: int, kv_heads: int, head_dim: int, dtype: torch.dtype, device):
     """(units of every kind, members, record offsets) of a batch's tree of pages (``shared_nodes``)."""
     sms = sm_count(device)
-    if _shared_on_tensor_cores(dtype, head_dim):
+    form = _shared_form(dtype, head_dim)
+    if form == 1:
         # (small units go warp by warp where they are many; else that is only a launch more)
         pieces = sum(len(rows) * (heads // kv_heads) <= 16 for rows, *_ in nodes) + (len(tails) if heads // kv_heads <= 16 else 0)
         kinds = ((16 if pieces * kv_heads > 2 * sms else 0, 12 * sms, 4, 16), (32, 3 * sms, 4, 16), (128, 2 * sms, 2, 1 << 20))
     else:
-        kinds = ((16, 4 * sms, 2, 16), (64, 4 * sms, 2, 16), (0, 0, 0, 0))
+        kinds = ((16, 4 * sms, 1, 16), (64, 2 * sms, 1, 16), (0, 0, 0, 0))
     return shared_units(nodes, tails, seqs, heads // kv_heads, kv_heads, kinds, 1)
 
 
@@ -2939,10 +2941,11 @@ def attention_shared(q: torch.Tensor, q_stride: int, k_cache: torch.Tensor, v_ca
             and token_pos.dtype == page_table.dtype == torch.int32 and scale > 0
             and q.device == k_cache.device == v_cache.device == token_pos.device == page_table.device == out.device == device
             and k_cache.is_contiguous() and v_cache.is_contiguous() and out.is_contiguous() and token_pos.is_contiguous()
-            and page_table.is_contiguous() and shape[0] * kv_heads < 1 << 25):
+            and page_table.is_contiguous() and shape[0] * kv_heads < 1 << 25
+            and (plan.form == 0 or (q_stride * q.element_size() % 16 == 0 and q.data_ptr() % 16 == 0))):
         raise KernelError(
             f"attention_shared: the plan is of {n} rows, {plan.heads} heads over {plan.kv_heads} of {d}, {dtype}, {plan.seqs} sequences of "
-            f"{plan.cols} pages on {device}; wanted are q [rows, heads * d] in rows of q_stride, k and v [pages < 2^25 / kv_heads, "
+            f"{plan.cols} pages on {device}; wanted are q [rows, heads * d] in rows of q_stride (of whole 16 bytes for heads of 64 and 128), k and v [pages < 2^25 / kv_heads, "
             f"kv_heads, 64, d], token_pos int32 [rows], page_table int32, out [rows, heads * d], contiguous, and a positive scale; got "
             f"q {tuple(q.shape)} of {q.dtype}, cache {tuple(shape)} of {k_cache.dtype}, out {tuple(out.shape)}, page_table "
             f"{tuple(page_table.shape)}, scale {scale}")

@@ -88,8 +88,15 @@ def shared_units(nodes: Sequence[tuple], tails: Sequence[tuple], seqs: Sequence[
         kind = next((i for i in may if entries <= kinds[i][0]), may[-1])
         pieces.append((rows, a, b, ends, kind))
         total[kind] += -(-entries // kinds[kind][0]) * (b - a) * kv_heads
-    # pages of a chunk: as many as leave every CTA of the kind the same share
-    share = [min(k[3], max(k[2], -(-t // max(1, k[1])))) if k[0] else 1 for k, t in zip(kinds, total)]
+    # pages of a chunk: as few as leave no more CTAs of the kind than it has at once (a few more would run by themselves)
+    share = [1] * len(kinds)
+    for i, (tile, ctas, least, most) in enumerate(kinds):
+        mine = [(b - a, -(-len(rows) * group // tile) * kv_heads) for rows, a, b, _, kind in pieces if kind == i]
+        if mine:
+            share[i] = min(most, max(least, -(-total[i] // ctas)))
+            while share[i] < min(most, max(n for n, _ in mine)) and sum(-(-n // share[i]) * tiles for n, tiles in mine) > ctas:
+                share[i] += 1 + share[i] // 16
+            share[i] = min(share[i], most)
     units: List[List[tuple]] = [[] for _ in kinds]
     members: List[int] = []
     slots = [0] * len(seqs)

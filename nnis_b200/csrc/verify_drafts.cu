@@ -29,7 +29,7 @@ constexpr int kVerifyThreads = 256;
 constexpr int kVerifyShare = 8192;   // logits of a row that a CTA of the first launch sums at least
 constexpr int kVerifyParts = 32;     // most CTAs a row
 constexpr int kPickThreads = 512;
-constexpr int kPickCtas = 8;         // of a cluster
+constexpr int kPickCtas = 16;        // most of a cluster
 
 struct __align__(16) RowSum {
     float max, sum;  // maximum logit, sum of exp((x - max) / T): no number where a logit is none, or +infinity
@@ -185,6 +185,7 @@ __device__ __forceinline__ double weight64(const double* table, float x, float m
 }
 
 constexpr int kPickWarps = kPickThreads / 32;
+constexpr size_t kHeldMost = 108 * 1024;  // bytes of weights that two CTAs of an SM can each keep
 
 struct PickShared {
     double table[64];                // 2^(j / 64)
@@ -222,12 +223,15 @@ __device__ __forceinline__ void cluster_sum(cg::cluster_group cluster, PickShare
     }
 }
 
+// HELD: a CTA's weights stay in shared memory between the two walks over the row (16 bytes an id).
+template <bool HELD>
 __global__ void __launch_bounds__(kPickThreads, 2)
 verify_pick_kernel(const float* __restrict__ logits, const float* __restrict__ draft_logits, const int* __restrict__ drafts,
                    const int* __restrict__ first_row, const float* __restrict__ temperature, const double* __restrict__ accept_draws,
                    const double* __restrict__ pick_draws, const RowSum* __restrict__ parts, int n_parts, int rows, int vocab,
                    int* __restrict__ accepted, int* __restrict__ picked) {
     __shared__ PickShared s;
+    extern __shared__ __align__(16) double2 held_s[];
     cg::cluster_group cluster = cg::this_cluster();
     const int b = blockIdx.y, rank = (int)cluster.block_rank(), ctas = (int)cluster.num_blocks();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -276,8 +280,7 @@ verify_pick_kernel(const float* __restrict__ logits, const float* __restrict__ d
         if (fabs(left - right) <= 1e-4 * right || t < 1e-29f) return kNear;
         return left < right ? kKept : kRefused;
     };
-    // A warp's ids lie together, 32 at a time.  Nothing of a row is kept between the two walks over it: it comes from L1
-    // again, and without the registers two CTAs are on an SM, so that one walks while the other meets its cluster.
+    // A warp's ids lie together, 32 at a time.
     const int per_warp = (((vocab + ctas * kPickWarps - 1) / (ctas * kPickWarps)) + 31) & ~31;
     const int begin = min(vocab, (rank * kPickWarps + warp) * per_warp), end = min(vocab, begin + per_warp);
     constexpr int kAhead = 4;
@@ -297,6 +300,7 @@ verify_pick_kernel(const float* __restrict__ logits, const float* __restrict__ d
             ey[k] = y ? weight64(s.table, xy[k], y_max, inv_t) : 0.0;
         }
     };
+    double2* mine = held_s + warp * per_warp;  // (a lane reads what it has written)
     int turn = 0;
     double sp = 0.0, sq = 0.0;
     auto exact_sums = [&](int i, int stopped) {  // of row i, at which warp `stopped` stopped, in 64 bits
@@ -312,6 +316,7 @@ verify_pick_kernel(const float* __restrict__ logits, const float* __restrict__ d
             for (int k = 0; k < kAhead; ++k) {
                 sp += ez[k];
                 sq += ey[k];
+                if (HELD && i0 + 32 * k < end) mine[i0 + 32 * k - begin] = make_double2(ez[k], ey[k]);
             }
         }
         cluster_sum(cluster, s, turn, sp, sq);
@@ -359,7 +364,16 @@ verify_pick_kernel(const float* __restrict__ logits, const float* __restrict__ d
     bool plain = all;
     auto masses = [&](int first, double (&m)[kAhead]) {
         double ey[kAhead];
-        weights(first, m, ey);
+        if (HELD) {
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+                const double2 e = first + 32 * k < end ? mine[first + 32 * k - begin] : make_double2(0.0, 0.0);
+                m[k] = e.x;
+                ey[k] = e.y;
+            }
+        } else {
+            weights(first, m, ey);
+        }
 #pragma unroll
         for (int k = 0; k < kAhead; ++k) {
             const double p = __dmul_rn(m[k], ip);  // (rounded like q: equal ones leave nothing)
@@ -454,11 +468,22 @@ NNIS_API int nnis_verify_drafts(const float* logits, const float* draft_logits, 
     cudaError_t e = launch_dependent(verify_rows_kernel, dim3(n_parts, all_rows), kVerifyThreads, 0, stream, logits, draft_logits,
                                      first_row, temperature, n_seqs, rows, draft_rows, vocab, per, static_cast<RowSum*>(scratch));
     if (e != cudaSuccess) return (int)e;
-    // Eight CTAs a sequence; four where eight would be more than the device holds at once.
+    // As many CTAs a sequence as the device holds at once (two an SM) for all of them, sixteen at most, four at least.  Their
+    // weights stay in shared memory where two CTAs of an SM have room for them.
     cudaLaunchConfig_t cfg = {};
-    const int ctas = n_seqs * kPickCtas <= 2 * device_sms() ? kPickCtas : kPickCtas / 2;
+    const int slots = 2 * device_sms();
+    int ctas = kPickCtas;
+    while (ctas > 4 && n_seqs * ctas > slots) ctas /= 2;
+    auto bytes_of = [&](int n) { return (size_t)16 * (((vocab + n * kPickWarps - 1) / (n * kPickWarps) + 31) & ~31) * kPickWarps; };
+    if (ctas == 4 && bytes_of(4) > kHeldMost) ctas = 8;  // (the walk saved is worth the second wave)
+    const bool held = bytes_of(ctas) <= kHeldMost;
+    auto kernel = held ? verify_pick_kernel<true> : verify_pick_kernel<false>;
+    const size_t smem = held ? bytes_of(ctas) : 0;
+    if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) != cudaSuccess) return (int)e;
+    if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) != cudaSuccess) return (int)e;
     cfg.gridDim = dim3(ctas, n_seqs);
     cfg.blockDim = dim3(kPickThreads);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -468,7 +493,7 @@ NNIS_API int nnis_verify_drafts(const float* logits, const float* draft_logits, 
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = dependent_launches() ? 2 : 1;
-    e = cudaLaunchKernelEx(&cfg, verify_pick_kernel, logits, draft_logits, drafts, first_row, temperature, accept_draws, pick_draws,
+    e = cudaLaunchKernelEx(&cfg, kernel, logits, draft_logits, drafts, first_row, temperature, accept_draws, pick_draws,
                            static_cast<const RowSum*>(scratch), n_parts, rows, vocab, accepted, picked);
     return e == cudaSuccess ? NNIS_OK : (int)e;
 }
