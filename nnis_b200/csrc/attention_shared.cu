@@ -154,7 +154,7 @@ attn_shared_merge_kernel(const float* __restrict__ partial, const float2* __rest
     const int count = record[row + 1] - first;
     pdl_wait();
     pdl_launch_dependents();
-    merge_row<T, 8>(partial, sums, first, count, row, (int)(at % nq), nq, d, out);
+    merge_row<T, 16>(partial, sums, first, count, row, (int)(at % nq), nq, d, out);
 }
 
 template <typename T, int ROWS, int NJ>
@@ -203,7 +203,7 @@ NNIS_API int nnis_attention_shared(const void* q, int q_stride, const void* k_ca
     if (form == 2 && (!f32 || (d != 64 && d != 128))) return NNIS_ERR_UNSUPPORTED;
     if (form < 0 || form > 2) return NNIS_ERR_ARGUMENT;
     if ((n2 && form != 1) || (tickets && (n2 || (n0 && form == 1)))) return NNIS_ERR_UNSUPPORTED;
-    if ((uintptr_t)units % 16 || (uintptr_t)partial % 16 || (uintptr_t)sums % 8) return NNIS_ERR_ALIGNMENT;
+    if ((uintptr_t)units % 16 || (uintptr_t)partial % 32 || (uintptr_t)sums % 8) return NNIS_ERR_ALIGNMENT;
     const uintptr_t all = (uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache;
     if (all % (form ? 16 : f32 ? 8 : 4) || (uintptr_t)out % (f32 ? 8 : 4) || (form && q_stride % (f32 ? 4 : 8))) return NNIS_ERR_ALIGNMENT;
     SharedArgs a = {q,       k_cache, v_cache, token_pos, page_table, reinterpret_cast<const SharedUnit*>(units), members, record,

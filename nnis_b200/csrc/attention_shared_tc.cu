@@ -1,15 +1,17 @@
 // Attention over shared pages on the fifth-generation tensor cores: units of up to 128 entries (token row, query head),
 // bfloat16, heads of 64 or 128.  See attention_shared.cuh for units and records.
 //
-// A CTA owns a unit and a kv head; all its entries see all keys of its pages, so nothing is masked.  Ten warps:
+// A CTA owns a unit and a kv head; all its entries see all keys of its pages, so nothing is masked.  Eleven warps:
 //   warp 0     one lane issues TMA loads: a page of K and of V [64 keys, D] per step into rings of their own (K is done with as
 //              soon as its scores are, V a softmax later);
-//   warp 1     allocates tensor memory and issues S[128, 64] = Q K^T (two buffers) and O[128, D] += P V, P from tensor
-//              memory: the next page's scores are made while this one's softmax runs;
-//   warps 2-9  stack the entries' queries into shared memory (they lie rows apart, G heads together), then softmax: two
+//   warp 1     allocates tensor memory and issues S[128, 64] = Q K^T (two buffers), the next pages' while this one's
+//              softmax runs;
+//   warp 2     issues O[128, D] += P V, P from tensor memory;
+//   warps 3-10 stack the entries' queries into shared memory (they lie rows apart, G heads together), then softmax: two
 //              warps per quarter of the rows, a thread has one row and half of a page's keys.  The halves tell each
 //              other their maximum through shared memory, so that one accumulator O serves both, and write P
-//              (bfloat16) over the scores they have read.
+//              (bfloat16) into tensor memory: with 64 values into columns of its own, so that a buffer takes its next scores as
+//              soon as the last have been read; with 128, where O takes those columns, over the scores.
 // P is rounded to bfloat16 because the tensor cores take it so (2^-9 of a weight, of either sign); sums are of the 32-bit
 // weights.  O stays in tensor memory; the maximum that P is taken against is only raised when a page exceeds it by
 // more than 8 (a factor 256, harmless in both types), then the warps wait for the products so far and multiply O.
@@ -20,7 +22,7 @@
 
 namespace nnis {
 
-constexpr int kShRows = 128, kShThreads = 320;
+constexpr int kShRows = 128, kShThreads = 352;
 constexpr uint32_t kShChunkQ = kShRows * 128, kShChunkK = kSharedPage * 128;  // bytes of 64 columns of the queries, of a page
 constexpr float kShRaise = 8.0f;
 
@@ -49,6 +51,13 @@ __device__ __forceinline__ void sh_store16(uint32_t taddr, const uint32_t (&v)[1
     tmem_store_wait();
 }
 
+// 32 bytes, a whole sector, at once: a lane's row is far from its neighbours'.
+__device__ __forceinline__ void store_sector(float* to, const uint32_t* v) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
+                 "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+}
+
 // The two warps of a quarter of the rows meet.  A warp that gives up raises the abort flag and then arrives once, so that its
 // partner, wherever it is, comes through its next meeting, sees the flag there and gives up too: no meeting waits for good.
 __device__ __forceinline__ void quarter_meet(int quarter) { asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory"); }
@@ -66,13 +75,16 @@ __global__ void __launch_bounds__(kShThreads, 2)
 attn_shared_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const SharedArgs a,
                       int* __restrict__ status) {
     constexpr int C = D / 64, kStages = sh_stages<D>();
-    constexpr uint32_t kPageBytes = C * kShChunkK, kColsO = 128, kCols = 256;
+    constexpr uint32_t kPageBytes = C * kShChunkK, kCols = 256;
+    // tensor memory: S, two buffers of 64 columns; P, 32 columns a buffer; O
+    constexpr bool kOwnP = D == 64;
+    constexpr uint32_t kP = kOwnP ? 128 : 0, kStrideP = kOwnP ? 32 : 64, kColsO = kOwnP ? 192 : 128;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char* q_s = shared_1024(smem_raw);           // C x [128, 64] swizzled
     unsigned char* k_s = q_s + C * kShChunkQ;             // stages x C x [64, 64]
     unsigned char* v_s = k_s + kStages * kPageBytes;
     __shared__ __align__(8) uint64_t k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
-    __shared__ __align__(8) uint64_t q_ready, s_full[2], p_ready[2], pv_done[2];
+    __shared__ __align__(8) uint64_t q_ready, s_full[2], s_free[2], p_ready[2], pv_done[2];
     __shared__ float half_max[2][2][kShRows], half_sum[kShRows];
     __shared__ uint32_t tmem_base_s;
     __shared__ volatile int abort_flag;
@@ -90,6 +102,7 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         mbar_init(&q_ready, 8);
         for (int b = 0; b < 2; ++b) {
             mbar_init(&s_full[b], 1);
+            mbar_init(&s_free[b], 8);  // the softmax warps
             mbar_init(&p_ready[b], 8);
             mbar_init(&pv_done[b], 1);
         }
@@ -100,7 +113,7 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = tmem_base_s;  // S, and P over it: columns 0 and 64; O: from 128 on
+    const uint32_t tmem = tmem_base_s;
     const SharedUnit u = a.units[blockIdx.x];
     const int hk = blockIdx.y, G = a.nq / a.nkv;
     const int n_pages = u.entries > 0 ? u.page_end - u.page_begin : 0;
@@ -132,75 +145,100 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             for (int j = max(0, i_v - kStages); j < i_v; ++j) mbar_wait(&v_full[j % kStages], (uint32_t)(j / kStages) & 1u);
         }
     } else if (warp == 1) {
-        constexpr uint32_t idesc_s = instr_desc(kShRows, kSharedPage), idesc_o = instr_desc(kShRows, D) | (1u << 16);  // (V: MN-major)
-        const uint64_t desc_q = smem_desc_k128(smem_addr(q_s)), desc_k0 = smem_desc_k128(smem_addr(k_s)), desc_v0 = sh_desc_v(smem_addr(v_s));
+        constexpr uint32_t idesc = instr_desc(kShRows, kSharedPage);
+        const uint64_t desc_q = smem_desc_k128(smem_addr(q_s)), desc_k0 = smem_desc_k128(smem_addr(k_s));
         bool ok = sh_wait(&q_ready, 0);
-        auto scores = [&](int i) {  // S(i) into its buffer
+        for (int i = 0; ok && i < n_pages; ++i) {
             const int s = i % kStages, b = i & 1;
-            ok = ok && sh_wait(&k_full[s], (uint32_t)(i / kStages) & 1u) && !__any_sync(0xffffffffu, abort_flag);
-            if (!ok) return;
+            ok = sh_wait(&k_full[s], (uint32_t)(i / kStages) & 1u) && !__any_sync(0xffffffffu, abort_flag);
+            // (the buffer's scores of two pages ago have been read, or the product that read P over them is over)
+            if (ok && i >= 2) ok = sh_wait(kOwnP ? &s_free[b] : &pv_done[b], (uint32_t)((i >> 1) - 1) & 1u);
+            if (!ok) break;
             tc_fence_after();
 #pragma unroll
             for (int c = 0; c < C; ++c)
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
                     warp_mma(tmem + b * 64, desc_advance(desc_q, c * kShChunkQ + k * 32),
-                             desc_advance(desc_k0, (uint32_t)s * kPageBytes + c * kShChunkK + k * 32), idesc_s, (c | k) != 0);
+                             desc_advance(desc_k0, (uint32_t)s * kPageBytes + c * kShChunkK + k * 32), idesc, (c | k) != 0);
             warp_commit(&s_full[b]);
             warp_commit(&k_empty[s]);
-        };
-        scores(0);
-        if (n_pages > 1) scores(1);
+        }
+        if (!ok && lane == 0) abort_flag = 1;
+    } else if (warp == 2) {
+        constexpr uint32_t idesc = instr_desc(kShRows, D) | (1u << 16);  // (V: MN-major)
+        const uint64_t desc_v0 = sh_desc_v(smem_addr(v_s));
+        bool ok = true;
         for (int i = 0; ok && i < n_pages; ++i) {
             const int s = i % kStages, b = i & 1;
-            ok = sh_wait(&v_full[s], (uint32_t)(i / kStages) & 1u) && sh_wait(&p_ready[b], (uint32_t)(i >> 1) & 1u) && !__any_sync(0xffffffffu, abort_flag);
+            ok = sh_wait(&v_full[s], (uint32_t)(i / kStages) & 1u) && sh_wait(&p_ready[b], (uint32_t)(i >> 1) & 1u) &&
+                 !__any_sync(0xffffffffu, abort_flag);
             if (!ok) break;
             tc_fence_after();
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-                warp_mma_ts(tmem + kColsO, tmem + b * 64 + k * 8, desc_advance(desc_v0, (uint32_t)s * kPageBytes + k * 2048), idesc_o,
-                            (i | k) != 0);
+                warp_mma_ts(tmem + kColsO, tmem + kP + b * kStrideP + k * 8, desc_advance(desc_v0, (uint32_t)s * kPageBytes + k * 2048),
+                            idesc, (i | k) != 0);
             warp_commit(&pv_done[b]);
             warp_commit(&v_empty[s]);
-            if (i + 2 < n_pages) {  // (its buffer holds P(i) until that product is over)
-                ok = sh_wait(&pv_done[b], (uint32_t)(i >> 1) & 1u);
-                scores(i + 2);
-            }
         }
         if (!ok && lane == 0) abort_flag = 1;
     } else {
-        const int quarter = warp & 3, half = (warp - 2) >> 2;
+        const int quarter = warp & 3, half = (warp - 3) >> 2;
         const int row = quarter * 32 + lane;
         const int* members = a.members + u.members;
-        {   // the queries: eight warps, a row of 128 bytes by eight lanes
+        {   // the queries: eight warps, a row of 128 bytes by eight lanes, all of a thread's on their way together
+            constexpr int kPer = kShRows * C * 8 / 256;
             const bf16* q = static_cast<const bf16*>(a.q);
-            for (int i = threadIdx.x - 64; i < kShRows * C * 8; i += kShThreads - 64) {
-                const int e = i / (C * 8), c = i % (C * 8), at = u.entry + e;
-                uint4 x = make_uint4(0, 0, 0, 0);
+            uint4 x[kPer];
+#pragma unroll
+            for (int n = 0; n < kPer; ++n) {
+                const int i = threadIdx.x - 96 + n * 256, e = i / (C * 8), c = i % (C * 8), at = u.entry + e;
+                x[n] = make_uint4(0, 0, 0, 0);
                 if (e < u.entries)
-                    x = *reinterpret_cast<const uint4*>(q + (size_t)members[at / G] * a.q_stride + (size_t)(hk * G + at % G) * D + c * 8);
-                *reinterpret_cast<uint4*>(q_s + (c >> 3) * kShChunkQ + e * 128 + (((c & 7) ^ (e & 7)) << 4)) = x;
+                    x[n] = __ldg(reinterpret_cast<const uint4*>(q + (size_t)__ldg(members + at / G) * a.q_stride + (size_t)(hk * G + at % G) * D + c * 8));
+            }
+#pragma unroll
+            for (int n = 0; n < kPer; ++n) {
+                const int i = threadIdx.x - 96 + n * 256, e = i / (C * 8), c = i % (C * 8);
+                *reinterpret_cast<uint4*>(q_s + (c >> 3) * kShChunkQ + e * 128 + (((c & 7) ^ (e & 7)) << 4)) = x[n];
             }
             fence_async_shared();
             __syncwarp();
             if (lane == 0) mbar_arrive(&q_ready);
+        }
+        int rec = -1;  // this row's record
+        if (row < u.entries) {
+            const int at = u.entry + row;
+            rec = (a.record[members[at / G]] + u.slot) * a.nq + hk * G + at % G;
         }
         const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
         const float sc = a.scale * 1.4426950408889634f;
         const bool idle = quarter * 32 >= u.entries;  // rows of no entry: their P may be anything
         float m_run = -INFINITY, l_run = 0.f;         // maximum in use (scaled, log2 units), this half's sum against it
         bool ok = true;
+        // Where the next scores come before a product is over, a page's P (and a warp's word that it is there) waits for that of
+        // two pages ago.
+        auto last_over = [&](int i) { return !kOwnP || i < 2 || sh_wait(&pv_done[i & 1], (uint32_t)((i >> 1) - 1) & 1u); };
         for (int i = 0; i < n_pages; ++i) {
             const int b = i & 1;
-            ok = sh_wait(&s_full[b], (uint32_t)(i >> 1) & 1u) && !__any_sync(0xffffffffu, abort_flag);
+            ok = sh_wait(&s_full[b], (uint32_t)(i >> 1) & 1u);
             if (!ok) break;
             if (idle) {
+                if (kOwnP && lane == 0) mbar_arrive(&s_free[b]);
+                ok = last_over(i);
+                if (!ok) break;
                 if (lane == 0) mbar_arrive(&p_ready[b]);
                 continue;
             }
             tc_fence_after();
             uint32_t sv[32];
             tmem_load32(tmem + b * 64 + half * 32 + lane_base, sv);
+            if (kOwnP) {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&s_free[b]);
+            }
             float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
             for (int c = 0; c < 32; c += 8)
@@ -247,7 +285,10 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             }
             const float2 s0 = halves(ps[0]), s1 = halves(ps[1]);
             l_run += (s0.x + s0.y) + (s1.x + s1.y);
-            sh_store16(tmem + b * 64 + half * 16 + lane_base, w);
+            ok = last_over(i);
+            if (!ok) break;
+            if (kOwnP) tc_fence_after();
+            sh_store16(tmem + kP + b * kStrideP + half * 16 + lane_base, w);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&p_ready[b]);
@@ -265,19 +306,16 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                 abort_flag = 1;
             } else {
                 tc_fence_after();
-                const int at = u.entry + row;
-                const bool real = row < u.entries;
-                const size_t rec = real ? (size_t)(a.record[members[at / G]] + u.slot) * a.nq + hk * G + at % G : 0;
+                const bool real = rec >= 0;
                 if (real && !half) reinterpret_cast<float2*>(a.sums)[rec] = make_float2(m_run, l_run + half_sum[row]);
-                float* dst = a.partial + rec * D + half * (D / 2);
+                float* dst = a.partial + (size_t)rec * D + half * (D / 2);
 #pragma unroll
                 for (int h = 0; h < D / 64; ++h) {
                     uint32_t ov[32];
                     tmem_load32(tmem + kColsO + half * (D / 2) + h * 32 + lane_base, ov);
                     if (real) {
 #pragma unroll
-                        for (int c = 0; c < 32; c += 4)
-                            *reinterpret_cast<uint4*>(dst + h * 32 + c) = make_uint4(ov[c], ov[c + 1], ov[c + 2], ov[c + 3]);
+                        for (int c = 0; c < 32; c += 8) store_sector(dst + h * 32 + c, ov + c);
                     }
                 }
             }

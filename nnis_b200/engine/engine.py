@@ -290,7 +290,7 @@ class Engine:
                 ctx.host_tables[name] = arr
                 take(-arr.size % 4)
         if drafted or (decode and b > 1 and self.cache.shares_pages()):
-            ctx.shared = SharedRows(self, slots, seq.tolist(), pos.tolist())
+            ctx.shared = SharedRows(self, slots, seq.tolist(), pos.tolist(), not decode)
         return ctx, d_want, slots, new_lengths
 
     def step(self, batch: Sequence[SequenceStep], drafted: bool = False) -> torch.Tensor:

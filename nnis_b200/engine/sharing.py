@@ -12,28 +12,36 @@ from typing import Dict, Optional, Sequence, Tuple
 from ..cache import PAGE_SIZE
 from ..csrc import ops
 
-# Sharing has to take this many pages, and this part of them, off what the rows read one by one.
-LEAST_PAGES, LEAST_PART = 16, 0.25
+# Bytes of keys and values that sharing has to take off what the rows of a layer read one by one: it costs a launch or two more
+# and a merge.  us a layer of a decode step, one by one -> shared, bfloat16, bytes saved: 9 heads over 3 of 64, 8 rows behind 64
+# pages (22 MB) 7.2 -> 9.6, 4 behind 256 (38 MB) 14.5 -> 12.4, 16 behind 64 (47 MB) 12.9 -> 10.0, 64 behind 256 137 -> 19; 32 over 32 of
+# 64, 8 behind 4 (15 MB) 5.2 -> 7.6, 4 behind 16 (25 MB) 10.2 -> 7.8, 2 behind 64 (34 MB) 15.5 -> 11; 32 over 8 of 128, 8 behind 16
+# (29 MB) 10.9 -> 13.4, 16 behind 16 (63 MB) 14.9 -> 10.8.
+LEAST_BYTES = 32 << 20
 AHEAD = 8  # pages that a captured step's plan lets its sequences grow by
 
 PlanKey = Tuple[int, int, int, int]  # cache group, heads, key/value heads, head size
 
 
-def shared_tree(cache, group: int, slots: Sequence[int], seqs: Sequence[int], positions: Sequence[int], ahead: int = 0):
+def shared_tree(cache, group: int, slots: Sequence[int], seqs: Sequence[int], positions: Sequence[int], least_bytes: int,
+                ahead: int = 0):
     """(nodes, tails) of the rows' pages (``ops.shared_nodes``), or None where sharing does not pay."""
-    if cache.groups[group].window > 0:
+    g = cache.groups[group]
+    if g.window > 0:
         return None
     nodes, tails = ops.shared_nodes([cache.page_table(group, s) for s in slots], seqs, positions, ahead)
     saved = sum((len(rows) - 1) * (b - a) for rows, a, b in nodes)
-    read = sum(p // PAGE_SIZE + 1 for p in positions if p >= 0)
-    return (nodes, tails) if saved >= max(LEAST_PAGES, LEAST_PART * read) else None
+    return (nodes, tails) if saved and saved * PAGE_SIZE * g.kv_heads * (g.head_dim + g.value_dim) * g.k.element_size() >= least_bytes \
+        else None
 
 
 class SharedRows:
-    """The plans of one step: the sequence (a place in ``slots``) and the position of every row."""
+    """The plans of one step: the sequence (a place in ``slots``) and the position of every row.  ``drafted``: a sequence brings
+    several tokens, for which the kernels of prompts would walk its pages with a tile hardly filled: any sharing pays."""
 
-    def __init__(self, engine, slots: Sequence[int], seqs: Sequence[int], positions: Sequence[int]):
+    def __init__(self, engine, slots: Sequence[int], seqs: Sequence[int], positions: Sequence[int], drafted: bool):
         self.engine, self.slots, self.seqs, self.positions = engine, slots, seqs, positions
+        self._least = 0 if drafted else LEAST_BYTES
         self._trees: Dict[int, Optional[tuple]] = {}
         self._plans: Dict[PlanKey, Optional[ops.SharedPlan]] = {}
 
@@ -41,7 +49,7 @@ class SharedRows:
         if key not in self._plans:
             group, e = key[0], self.engine
             if group not in self._trees:
-                self._trees[group] = shared_tree(e.cache, group, self.slots, self.seqs, self.positions)
+                self._trees[group] = shared_tree(e.cache, group, self.slots, self.seqs, self.positions, self._least)
             tree = self._trees[group]
             self._plans[key] = None if tree is None else ops.attention_shared_plan_of(
                 *tree, self.seqs, self.positions, *key[1:], e.dtype, e.device)
@@ -88,7 +96,8 @@ class BatchUnits:
         units = {}
         for key in self.engine.model.shared_keys():
             if key[0] not in trees:
-                trees[key[0]] = shared_tree(cache, key[0], slots, seqs + [0] * padding, list(positions) + [-1] * padding, ahead)
+                trees[key[0]] = shared_tree(cache, key[0], slots, seqs + [0] * padding, list(positions) + [-1] * padding,
+                                              LEAST_BYTES, ahead)
             if trees[key[0]] is not None:
                 units[key] = ops.attention_shared_units(*trees[key[0]], seqs + [0] * padding, *key[1:], self.engine.dtype,
                                                         self.engine.device)

@@ -13,6 +13,13 @@ SHARED = dict(architectures=["LlamaForCausalLM"], model_type="llama", vocab_size
               torch_dtype="bfloat16")
 
 
+@pytest.fixture(autouse=True)
+def share_whatever_can_be(monkeypatch):
+    """The models here are small: sharing would not pay."""
+    from nnis_b200.engine import sharing
+    monkeypatch.setattr(sharing, "LEAST_BYTES", 1)
+
+
 @pytest.fixture(scope="module")
 def folder(tmp_path_factory):
     return make_model(str(tmp_path_factory.mktemp("shared")), SHARED, 3)
