@@ -162,10 +162,9 @@ static cudaError_t launch_any(const SharedArgs& a, int n_units, cudaStream_t str
     const int ds = ((a.d + 3) & ~3) + 4, tile = 16 * ROWS;
     const size_t smem = ((size_t)(tile + kSharedPage) * ds + (size_t)tile * 68) * sizeof(float);
     auto kernel = attn_shared_any_kernel<T, ROWS, NJ>;
-    if (smem > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (e != cudaSuccess) return e;
-    }
+    static std::atomic<int> held[16];
+    const cudaError_t e = allow_shared(kernel, smem, held);
+    if (e != cudaSuccess) return e;
     return launch_dependent(kernel, dim3(n_units, a.nkv), kAnyThreads, smem, stream, a);
 }
 

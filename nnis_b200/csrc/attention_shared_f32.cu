@@ -164,7 +164,8 @@ template <int D, int ROWS>
 static cudaError_t launch_f32(const SharedArgs& a, int n_units, cudaStream_t stream) {
     const size_t smem = ((size_t)(16 * ROWS + kSharedPage) * (D + 4) + (size_t)kSharedPage * D + (size_t)16 * ROWS * (kSharedPage + 4)) * sizeof(float);
     auto kernel = attn_shared_f32_kernel<D, ROWS>;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    static std::atomic<int> held[16];
+    const cudaError_t e = allow_shared(kernel, smem, held);
     if (e != cudaSuccess) return e;
     return launch_dependent(kernel, dim3(n_units, a.nkv), kF32Threads, smem, stream, a);
 }

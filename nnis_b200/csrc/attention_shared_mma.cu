@@ -224,7 +224,8 @@ template <int D>
 static cudaError_t launch_small(const SharedArgs& a, int n_units, cudaStream_t stream) {
     const size_t tiles = (32 * D + sm_stages<D>() * 2 * (size_t)kSharedPage * D) * sizeof(bf16);
     auto kernel = attn_shared_mma_kernel<D>;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)tiles);
+    static std::atomic<int> held[16];
+    const cudaError_t e = allow_shared(kernel, tiles, held);
     if (e != cudaSuccess) return e;
     return launch_dependent(kernel, dim3(n_units, a.nkv), kSmThreads, tiles, stream, a);
 }

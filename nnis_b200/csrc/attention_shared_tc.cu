@@ -338,7 +338,8 @@ static cudaError_t launch_tc(const SharedArgs& a, int n_units, int* status, cuda
         return cudaErrorInvalidValue;
     const size_t smem = 1024 + (D / 64) * (size_t)kShChunkQ + 2 * sh_stages<D>() * (size_t)(D / 64) * kShChunkK;
     auto kernel = attn_shared_tc_kernel<D>;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    static std::atomic<int> held[16];
+    const cudaError_t e = allow_shared(kernel, smem, held);
     if (e != cudaSuccess) return e;
     return launch_dependent(kernel, dim3(n_units, a.nkv), kShThreads, smem, stream, map_k, map_v, a, status);
 }

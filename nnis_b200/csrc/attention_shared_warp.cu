@@ -233,7 +233,8 @@ static cudaError_t launch_warp(const SharedArgs& a, int n_units, int* status, cu
     constexpr int W = wp_warps<D>();
     const size_t smem = 1024 + (size_t)W * 2 * kSharedPage * D * 2;
     auto kernel = attn_shared_warp_kernel<D>;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    static std::atomic<int> held[16];
+    const cudaError_t e = allow_shared(kernel, smem, held);
     if (e != cudaSuccess) return e;
     const int items = n_units * a.nkv, sms = device_sms();
     return launch_dependent(kernel, dim3(items < sms ? items : sms), W * 32, smem, stream, map_k, map_v, a, items, status);

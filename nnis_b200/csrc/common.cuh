@@ -7,6 +7,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #define NNIS_OK 0
 // Negative codes are argument errors found on the host before any launch;
 // positive codes are cudaError_t values of the launch itself.
@@ -100,6 +102,18 @@ inline int device_sms() {
     const bool known = cudaGetDevice(&device) == cudaSuccess &&
                        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) == cudaSuccess && sms > 0;
     return known ? sms : 148;
+}
+
+// Lets `kernel` have `bytes` of dynamic shared memory on the current device; `held` (16 zeros of the caller's, one place a device)
+// is what it may have already, so that the driver is asked once and not at every launch.
+template <typename Kernel>
+inline cudaError_t allow_shared(Kernel kernel, size_t bytes, std::atomic<int>* held) {
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess || (device < 16 && held[device].load(std::memory_order_relaxed) >= (int)bytes)) return e;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == cudaSuccess && device < 16) held[device].store((int)bytes, std::memory_order_relaxed);
+    return e;
 }
 
 // Launch `kernel` as a programmatic dependent of the kernel before it on the stream: it may

@@ -62,17 +62,22 @@ def _stream() -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
-_P, _I, _L, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
+def _types(letters: str):
+    return [{"p": ctypes.c_void_p, "i": ctypes.c_int, "f": ctypes.c_float}[c] for c in letters]
+
+
+# Entry points that take plain numbers for their arguments (p: an address, i: an int, f: a float): a call with thirty arguments
+# wrapped one by one costs the host 8 us, this one 3.
+_ENTRY_TYPES = {"nnis_copy_pages": "ppiiiiiipiip", "nnis_verify_scratch": "iii", "nnis_verify_drafts": "ppppppppiiippp",
+                "nnis_attention_shared": "pippppipiiippppppiiiiiifiipp"}
 _entries = {}
 
 
-def _entry(name: str, *types):
-    """An entry point that takes plain numbers for its arguments (made once: a call with thirty arguments wrapped one by one,
-    and the library asked for, costs the host 8 us, this one 3)."""
+def _entry(name: str):
     fn = _entries.get(name)
     if fn is None:
         fn = getattr(_lib(), name)
-        fn.argtypes = types
+        fn.argtypes = _types(_ENTRY_TYPES[name])
         _entries[name] = fn
     return fn
 
@@ -202,7 +207,7 @@ def copy_pages(k: torch.Tensor, v: Optional[torch.Tensor], moves) -> None:
         ints = array.array("i", src + dst + rows)
     except (TypeError, ValueError, OverflowError) as error:
         raise KernelError(f"copy_pages: moves are (source page, target page, rows), whole numbers: {error}") from None
-    code = _entry("nnis_copy_pages", _P, _P, _I, _I, _I, _I, _I, _I, _P, _I, _I, _P)(
+    code = _entry("nnis_copy_pages")(
         k.data_ptr(), None if v is None else v.data_ptr(), layers, pages, heads, page_size, k_row, v_row, ints.buffer_info()[0],
         len(src), sm_count(k.device), _stream_here())
     if code == -1:
@@ -431,9 +436,9 @@ def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, first_row: torch.T
         with torch.cuda.device(device):
             return verify_drafts(logits, drafts, first_row, temperatures, accept_draws, pick_draws, accepted, picked,
                                  draft_logits, workspace)
-    need = _entry("nnis_verify_scratch", _I, _I, _I)(rows, drafted, vocab)
+    need = _entry("nnis_verify_scratch")(rows, drafted, vocab)
     scratch = workspace.room("verify_sums", need // 4, f32)
-    _check(_entry("nnis_verify_drafts", _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _P, _P, _P)(
+    _check(_entry("nnis_verify_drafts")(
         logits.data_ptr(), draft_logits.data_ptr() if draft_logits is not None and drafted else None, drafts.data_ptr(),
         first_row.data_ptr(), temperatures.data_ptr(), accept_draws.data_ptr(), pick_draws.data_ptr(), scratch.data_ptr(), b, rows,
         vocab, accepted.data_ptr(), picked.data_ptr(), _stream_here()), "verify_drafts", 2)
@@ -2957,8 +2962,7 @@ def attention_shared(q: torch.Tensor, q_stride: int, k_cache: torch.Tensor, v_ca
     at = workspace.room("attn_shared_records", held * (d + 2), torch.float32).data_ptr()
     tickets = workspace.zeros_room("attn_shared_tickets", n * heads, torch.int32).data_ptr() if plan.merged_inside else None
     n0, n1, n2 = plan.counts
-    _check(_entry("nnis_attention_shared", _P, _I, _P, _P, _P, _P, _I, _P, _I, _I, _I, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I,
-                  _I, _F, _I, _I, _P, _P)(
+    _check(_entry("nnis_attention_shared")(
         q.data_ptr(), q_stride, k_cache.data_ptr(), v_cache.data_ptr(), token_pos.data_ptr(), page_table.data_ptr(),
         page_table.shape[1], plan.units, n0, n1, n2, plan.members, plan.record, at, at + 4 * held * d, tickets, out.data_ptr(), n,
         heads, kv_heads, d, shape[0], 64, scale, F32 if dtype == torch.float32 else BF16, plan.form, plan.status, _stream_here()),

@@ -185,53 +185,49 @@ __device__ __forceinline__ double weight64(const double* table, float x, float m
 }
 
 constexpr int kPickWarps = kPickThreads / 32;
-constexpr size_t kHeldMost = 108 * 1024;  // bytes of weights that two CTAs of an SM can each keep
 
 struct PickShared {
     double table[64];                // 2^(j / 64)
-    double warp[2][kPickWarps];
-    double cta[2][2][kPickCtas];     // every CTA's sums, written by them: [turn][which][rank]
-    float row_max[2][kPickWarps];    // of the row at which a warp stopped
+    double warp[4][kPickWarps];
+    double cta[2][4][kPickCtas];     // every CTA's sums, written by them: [turn][which][rank]
+    float row_max[2][kPickWarps], row_sum[2][kPickWarps];  // of the row at which a warp stopped
     int stop;
 };
 
-// Sum over the whole cluster of up to two values a thread, every thread gets both.  Each CTA tells all others its sums, in
+// Sums over the whole cluster of four values a thread; every thread gets all.  Each CTA tells all others its sums, in
 // one of two places by turns: a place is written again only when everybody has met once more.
-__device__ __forceinline__ void cluster_sum(cg::cluster_group cluster, PickShared& s, int turn, double& a, double& b) {
+__device__ __forceinline__ void cluster_sums(cg::cluster_group cluster, PickShared& s, int turn, double (&v)[4]) {
     const int lane = threadIdx.x & 31;
-    a = warp_sum64(a);
-    b = warp_sum64(b);
-    if (lane == 0) {
-        s.warp[0][threadIdx.x >> 5] = a;
-        s.warp[1][threadIdx.x >> 5] = b;
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+        v[n] = warp_sum64(v[n]);
+        if (lane == 0) s.warp[n][threadIdx.x >> 5] = v[n];
     }
     __syncthreads();
     const int ctas = (int)cluster.num_blocks();
     if (threadIdx.x < 32) {
-        a = warp_sum64(lane < kPickWarps ? s.warp[0][lane] : 0.0);
-        b = warp_sum64(lane < kPickWarps ? s.warp[1][lane] : 0.0);
-        if (lane < 2 * ctas) {
-            PickShared* other = cluster.map_shared_rank(&s, lane >> 1);
-            other->cta[turn][lane & 1][cluster.block_rank()] = lane & 1 ? b : a;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) v[n] = warp_sum64(lane < kPickWarps ? s.warp[n][lane] : 0.0);
+        if (lane < ctas) {
+            PickShared* other = cluster.map_shared_rank(&s, lane);
+#pragma unroll
+            for (int n = 0; n < 4; ++n) other->cta[turn][n][cluster.block_rank()] = v[n];
         }
     }
     cluster.sync();
-    a = b = 0.0;
-    for (int i = 0; i < ctas; ++i) {
-        a += s.cta[turn][0][i];
-        b += s.cta[turn][1][i];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+        v[n] = 0.0;
+        for (int i = 0; i < ctas; ++i) v[n] += s.cta[turn][n][i];
     }
 }
 
-// HELD: a CTA's weights stay in shared memory between the two walks over the row (16 bytes an id).
-template <bool HELD>
 __global__ void __launch_bounds__(kPickThreads, 2)
 verify_pick_kernel(const float* __restrict__ logits, const float* __restrict__ draft_logits, const int* __restrict__ drafts,
                    const int* __restrict__ first_row, const float* __restrict__ temperature, const double* __restrict__ accept_draws,
                    const double* __restrict__ pick_draws, const RowSum* __restrict__ parts, int n_parts, int rows, int vocab,
                    int* __restrict__ accepted, int* __restrict__ picked) {
     __shared__ PickShared s;
-    extern __shared__ __align__(16) double2 held_s[];
     cg::cluster_group cluster = cg::this_cluster();
     const int b = blockIdx.y, rank = (int)cluster.block_rank(), ctas = (int)cluster.num_blocks();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -269,6 +265,8 @@ verify_pick_kernel(const float* __restrict__ logits, const float* __restrict__ d
         if (lane == 0) {
             s.row_max[0][warp] = zs.max;
             s.row_max[1][warp] = ys.max;
+            s.row_sum[0][warp] = zs.sum;
+            s.row_sum[1][warp] = ys.sum;
         }
         if (!(zs.sum >= 0.f) || zs.max == -INFINITY || zs.max == INFINITY) return kNothing;
         if (!drafted) return kRefused;
@@ -300,28 +298,34 @@ verify_pick_kernel(const float* __restrict__ logits, const float* __restrict__ d
             ey[k] = y ? weight64(s.table, xy[k], y_max, inv_t) : 0.0;
         }
     };
-    double2* mine = held_s + warp * per_warp;  // (a lane reads what it has written)
+    // The sums of row i, at which warp `stopped` stopped, in 64 bits: of p's weights, of q's, and of both over the ids where p is
+    // the larger, by the sums in 32 bits.  The last two give what q leaves of p, sum p[more] / sum p - sum q[more] / sum q,
+    // without a second walk: an id on the wrong side of that line has p and q within 2e-5 of one another, and counts for as much.
     int turn = 0;
-    double sp = 0.0, sq = 0.0;
-    auto exact_sums = [&](int i, int stopped) {  // of row i, at which warp `stopped` stopped, in 64 bits
+    double sums[4];
+    auto walk = [&](int i, int stopped, int without) {
         z = logits + (size_t)(row0 + i) * vocab;
         y = draft_logits && i < count ? draft_logits + (size_t)(draft0 + i) * vocab : nullptr;
         z_max = s.row_max[0][stopped];
         y_max = s.row_max[1][stopped];
-        sp = sq = 0.0;
+        const double zt = s.row_sum[0][stopped], yt = s.row_sum[1][stopped];
+#pragma unroll
+        for (int n = 0; n < 4; ++n) sums[n] = 0.0;
         for (int i0 = begin + lane; i0 < end; i0 += 32 * kAhead) {
             double ez[kAhead], ey[kAhead];
             weights(i0, ez, ey);
 #pragma unroll
             for (int k = 0; k < kAhead; ++k) {
-                sp += ez[k];
-                sq += ey[k];
-                if (HELD && i0 + 32 * k < end) mine[i0 + 32 * k - begin] = make_double2(ez[k], ey[k]);
+                sums[0] += ez[k];
+                sums[1] += ey[k];
+                const bool more = y ? ez[k] * yt > ey[k] * zt : i0 + 32 * k != without;
+                sums[2] += more ? ez[k] : 0.0;
+                sums[3] += more ? ey[k] : 0.0;
             }
         }
-        cluster_sum(cluster, s, turn, sp, sq);
+        cluster_sums(cluster, s, turn, sums);
         turn ^= 1;
-        if (!y) sq = 1.0;
+        if (!y) sums[1] = 1.0;
     };
 
     int a = 0, why = kNear;
@@ -337,11 +341,11 @@ verify_pick_kernel(const float* __restrict__ logits, const float* __restrict__ d
         a = s.stop >> 2;
         why = s.stop & 3;
         if (why == kNothing || greedy) break;
-        exact_sums(a, (a - from) % kPickWarps);  // (all CTAs of the cluster come here together)
+        const int d = a < count ? drafts[draft0 + a] : -1;
+        walk(a, (a - from) % kPickWarps, d);  // (all CTAs of the cluster come here together)
         if (why != kNear) break;
-        const int d = drafts[draft0 + a];
         const double eq = y ? weight64(s.table, y[d], y_max, inv_t) : 1.0;
-        if (!(accept_draws[draft0 + a] * eq * sp < weight64(s.table, z[d], z_max, inv_t) * sq)) break;
+        if (!(accept_draws[draft0 + a] * eq * sums[0] < weight64(s.table, z[d], z_max, inv_t) * sums[1])) break;
         if (tid == 0) s.stop = 0x7fffffff;  // (everybody has read it: they have met)
         __syncthreads();
         from = a + 1;
@@ -357,49 +361,44 @@ verify_pick_kernel(const float* __restrict__ logits, const float* __restrict__ d
         return;
     }
     // The distribution to draw from: p, or what of it the draft's distribution leaves.
-    const bool all = a >= count;
-    const int d = all ? -1 : drafts[draft0 + a];
-    const double draw = pick_draws[b];
-    const double ip = 1.0 / sp, iq = 1.0 / sq;
-    bool plain = all;
+    const int d = a < count ? drafts[draft0 + a] : -1;
+    const double ip = 1.0 / sums[0], iq = y ? 1.0 / sums[1] : 0.0;
+    bool plain = a >= count;
     auto masses = [&](int first, double (&m)[kAhead]) {
         double ey[kAhead];
-        if (HELD) {
-#pragma unroll
-            for (int k = 0; k < kAhead; ++k) {
-                const double2 e = first + 32 * k < end ? mine[first + 32 * k - begin] : make_double2(0.0, 0.0);
-                m[k] = e.x;
-                ey[k] = e.y;
-            }
-        } else {
-            weights(first, m, ey);
-        }
+        weights(first, m, ey);
 #pragma unroll
         for (int k = 0; k < kAhead; ++k) {
             const double p = __dmul_rn(m[k], ip);  // (rounded like q: equal ones leave nothing)
             m[k] = plain ? p : y ? fmax(p - __dmul_rn(ey[k], iq), 0.0) : first + 32 * k == d ? 0.0 : p;
         }
     };
-    double total, unused;
-    for (;;) {
-        total = unused = 0.0;
-        for (int i0 = begin + lane; i0 < end; i0 += 32 * kAhead) {
-            double m[kAhead];
-            masses(i0, m);
+    // Masses of warps and CTAs, from their sums over the ids where p is the larger.  Where q leaves little (or, by
+    // rounding, nothing) of p the line between those ids is too coarse: the masses are summed id by id.
+    double mp = ip, mq = iq, total = mp * sums[2] - mq * sums[3];
+    if (!plain && (!(total >= 0.01) || t < 1e-29f)) {
+        mp = 1.0;
+        mq = 0.0;
+        for (;;) {
+            sums[0] = sums[1] = sums[2] = sums[3] = 0.0;
+            for (int i0 = begin + lane; i0 < end; i0 += 32 * kAhead) {
+                double m[kAhead];
+                masses(i0, m);
 #pragma unroll
-            for (int k = 0; k < kAhead; ++k) total += m[k];
+                for (int k = 0; k < kAhead; ++k) sums[2] += m[k];
+            }
+            cluster_sums(cluster, s, turn, sums);
+            turn ^= 1;
+            total = sums[2];
+            if (plain || total > 0.0) break;
+            plain = true;  // nothing is left: p and q are one
         }
-        cluster_sum(cluster, s, turn, total, unused);
-        turn ^= 1;
-        if (plain || total > 0.0) break;
-        plain = true;  // nothing is left: p and q are one
     }
-    // (s.warp[0]: this CTA's warps' sums; s.cta: every CTA's)
-    const double target = draw * total;
+    const double target = pick_draws[b] * total;
     double before = 0.0, held = 0.0;
     int last = 0;  // the last CTA with any weight
     for (int i = 0; i < ctas; ++i) {
-        const double other = s.cta[turn ^ 1][0][i];
+        const double other = fmax(mp * s.cta[turn ^ 1][2][i] - mq * s.cta[turn ^ 1][3][i], 0.0);
         if (i < rank) before += other;
         if (i == rank) held = other;
         if (other > 0.0) last = i;
@@ -407,16 +406,22 @@ verify_pick_kernel(const float* __restrict__ logits, const float* __restrict__ d
     if (rank == 0 && tid == 0) accepted[b] = a;
     // a draw at the very end of the sums belongs to the last id with any weight
     if (!((target >= before && target < before + held) || (rank == last && target >= before + held))) return;
-    double ahead = before;
+    double ahead = before, own = 0.0;
     int last_warp = 0;
     for (int w = 0; w < kPickWarps; ++w) {
-        if (w < warp) ahead += s.warp[0][w];
-        if (s.warp[0][w] > 0.0) last_warp = w;
+        const double other = fmax(mp * s.warp[2][w] - mq * s.warp[3][w], 0.0);
+        if (w < warp) ahead += other;
+        if (w == warp) own = other;
+        if (other > 0.0) last_warp = w;
     }
-    const double own = s.warp[0][warp];
     if (!(own > 0.0 && ((target >= ahead && target < ahead + own) || (warp == last_warp && target >= ahead + own)))) return;
     int found = -1, last_id = -1;
-    for (int i0 = begin; i0 < end && found < 0; i0 += 32 * kAhead) {
+    for (int i0 = begin; found < 0; i0 += 32 * kAhead) {
+        if (i0 >= end) {
+            if (last_id >= 0 || plain) break;
+            plain = true;  // (only ids of equal p and q are here, on the line by a rounding: one of them by p)
+            i0 = begin;
+        }
         double m[kAhead];
         masses(i0 + lane, m);
 #pragma unroll
@@ -468,22 +473,20 @@ NNIS_API int nnis_verify_drafts(const float* logits, const float* draft_logits, 
     cudaError_t e = launch_dependent(verify_rows_kernel, dim3(n_parts, all_rows), kVerifyThreads, 0, stream, logits, draft_logits,
                                      first_row, temperature, n_seqs, rows, draft_rows, vocab, per, static_cast<RowSum*>(scratch));
     if (e != cudaSuccess) return (int)e;
-    // As many CTAs a sequence as the device holds at once (two an SM) for all of them, sixteen at most, four at least.  Their
-    // weights stay in shared memory where two CTAs of an SM have room for them.
+    // As many CTAs a sequence as the device holds at once (two an SM) for all of them, sixteen at most, four at least.
     cudaLaunchConfig_t cfg = {};
-    const int slots = 2 * device_sms();
+    static const int slots = 2 * device_sms();
     int ctas = kPickCtas;
     while (ctas > 4 && n_seqs * ctas > slots) ctas /= 2;
-    auto bytes_of = [&](int n) { return (size_t)16 * (((vocab + n * kPickWarps - 1) / (n * kPickWarps) + 31) & ~31) * kPickWarps; };
-    if (ctas == 4 && bytes_of(4) > kHeldMost) ctas = 8;  // (the walk saved is worth the second wave)
-    const bool held = bytes_of(ctas) <= kHeldMost;
-    auto kernel = held ? verify_pick_kernel<true> : verify_pick_kernel<false>;
-    const size_t smem = held ? bytes_of(ctas) : 0;
-    if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) != cudaSuccess) return (int)e;
-    if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) != cudaSuccess) return (int)e;
+    static std::atomic<int> large[16];
+    int device = 0;
+    if ((e = cudaGetDevice(&device)) != cudaSuccess) return (int)e;
+    if (device >= 16 || !large[device].load(std::memory_order_relaxed)) {  // (sixteen CTAs a cluster are asked for once)
+        if ((e = cudaFuncSetAttribute(verify_pick_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) != cudaSuccess) return (int)e;
+        if (device < 16) large[device].store(1, std::memory_order_relaxed);
+    }
     cfg.gridDim = dim3(ctas, n_seqs);
     cfg.blockDim = dim3(kPickThreads);
-    cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -493,7 +496,7 @@ NNIS_API int nnis_verify_drafts(const float* logits, const float* draft_logits, 
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = dependent_launches() ? 2 : 1;
-    e = cudaLaunchKernelEx(&cfg, kernel, logits, draft_logits, drafts, first_row, temperature, accept_draws, pick_draws,
+    e = cudaLaunchKernelEx(&cfg, verify_pick_kernel, logits, draft_logits, drafts, first_row, temperature, accept_draws, pick_draws,
                            static_cast<const RowSum*>(scratch), n_parts, rows, vocab, accepted, picked);
     return e == cudaSuccess ? NNIS_OK : (int)e;
 }
