@@ -168,20 +168,25 @@ __device__ __forceinline__ double warp_sum64(double v) {
     return v;
 }
 
-// exp((x - max) / T) in 64 bits for x <= max: 2^(k / 64) from a table times the series of exp(r), |r| <= ln 2 / 128, to r^5 (what is
-// left out is 3e-17), after P. T. P. Tang's table-driven method (ACM TOMS 15, 1989).  Ten operations where
-// the library's exp, good to the last place, takes twice that: the sums of a row are bound by them.
-__device__ __forceinline__ double weight64(const double* table, float x, float max, double inv_t) {
-    const double t = ((double)x - (double)max) * inv_t;
-    if (!(t > -700.0) || x == -INFINITY) return t <= -700.0 || x == -INFINITY ? 0.0 : t;  // (too small to count; no number stays none)
-    constexpr double kRound = 6755399441055744.0;     // 1.5 * 2^52: adding it rounds to a whole number, in the low word
-    double k = fma(t, 92.33248261689366, kRound);     // 64 / ln 2
+// exp((x - max) / T) in 64 bits for x <= max: with u = 64 (x - max) / (T ln 2) and k the whole number next to it, 2^(k / 64) from a
+// table times the series of 2^((u - k) / 64) to the fourth power (what is left out is 4e-14), after P. T. P. Tang's
+// table-driven method (ACM TOMS 15, 1989).  Twenty instructions where the library's exp, good to the last place, takes twice as many and
+// the sums of a row are bound by them.
+struct Scale {
+    double per;    // 64 / (T ln 2)
+    double max;    // the row's maximum
+    float lowest;  // below it (700 T under the maximum, and at -infinity) a weight is zero
+};
+__device__ __forceinline__ Scale scale64(float max, double inv_t, float t) {
+    return {inv_t * 92.33248261689366, (double)max, fmaxf(-FLT_MAX, max - 700.f * t)};
+}
+__device__ __forceinline__ double weight64(const double* table, float x, const Scale& c) {
+    constexpr double kRound = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to a whole number, in the low word
+    const double u = ((double)x - c.max) * c.per, k = u + kRound, f = u - (k - kRound);
     const int n = __double2loint(k);
-    k -= kRound;
-    const double r = fma(k, -3.623510646634843e-19, fma(k, -0.010830424696249145, t));  // ln 2 / 64 in two parts
-    const double p = fma(fma(fma(fma(r, 1.0 / 120.0, 1.0 / 24.0), r, 1.0 / 6.0), r, 0.5), r * r, r);
-    const double e = table[n & 63], w = fma(e, p, e);
-    return __hiloint2double(__double2hiint(w) + (n >> 6) * (1 << 20), __double2loint(w));
+    const double p = fma(fma(fma(5.732851688640402e-10, f, 2.1173137155464776e-07), f, 5.86490495505617e-05), f, 0.010830424696249145);
+    const double e = table[n & 63], w = fma(e * f, p, e);
+    return x >= c.lowest ? __hiloint2double(__double2hiint(w) + (n & ~63) * (1 << 14), __double2loint(w)) : 0.0;
 }
 
 constexpr int kPickWarps = kPickThreads / 32;
@@ -273,8 +278,8 @@ verify_pick_kernel(const float* __restrict__ logits, const float* __restrict__ d
         if (greedy) return d == zs.best ? kKept : kRefused;
         if (!(ys.sum >= 0.f) || ys.max == -INFINITY || ys.max == INFINITY) return kNothing;
         if (!known) return kRefused;
-        const double eq = other ? weight64(s.table, yd, ys.max, inv_t) : 1.0;
-        const double left = u * eq * (double)zs.sum, right = weight64(s.table, zd, zs.max, inv_t) * (double)ys.sum;
+        const double eq = other ? weight64(s.table, yd, scale64(ys.max, inv_t, t)) : 1.0;
+        const double left = u * eq * (double)zs.sum, right = weight64(s.table, zd, scale64(zs.max, inv_t, t)) * (double)ys.sum;
         if (fabs(left - right) <= 1e-4 * right || t < 1e-29f) return kNear;
         return left < right ? kKept : kRefused;
     };
@@ -283,8 +288,9 @@ verify_pick_kernel(const float* __restrict__ logits, const float* __restrict__ d
     const int begin = min(vocab, (rank * kPickWarps + warp) * per_warp), end = min(vocab, begin + per_warp);
     constexpr int kAhead = 4;
     const float *z = nullptr, *y = nullptr;
-    float z_max = 0.f, y_max = 0.f;
-    auto weights = [&](int first, double (&ez)[kAhead], double (&ey)[kAhead]) {  // of ids first, first + 32, ...
+    Scale zc = {}, yc = {};
+    float line = 0.f;  // p is larger than q where z - y lies above it (by the sums in 32 bits)
+    auto weights = [&](int first, double (&ez)[kAhead], double (&ey)[kAhead], unsigned& more) {  // of ids first, first + 32, ...
         float xz[kAhead], xy[kAhead];
 #pragma unroll
         for (int k = 0; k < kAhead; ++k) {
@@ -294,33 +300,36 @@ verify_pick_kernel(const float* __restrict__ logits, const float* __restrict__ d
         }
 #pragma unroll
         for (int k = 0; k < kAhead; ++k) {
-            ez[k] = weight64(s.table, xz[k], z_max, inv_t);
-            ey[k] = y ? weight64(s.table, xy[k], y_max, inv_t) : 0.0;
+            ez[k] = weight64(s.table, xz[k], zc);
+            ey[k] = y ? weight64(s.table, xy[k], yc) : 0.0;
+            more |= xz[k] - xy[k] > line ? 1u << k : 0u;
         }
     };
     // The sums of row i, at which warp `stopped` stopped, in 64 bits: of p's weights, of q's, and of both over the ids where p is
     // the larger, by the sums in 32 bits.  The last two give what q leaves of p, sum p[more] / sum p - sum q[more] / sum q,
-    // without a second walk: an id on the wrong side of that line has p and q within 2e-5 of one another, and counts for as much.
+    // without a second walk: an id on the wrong side of that line has p and q within some 2e-5 of one another, and counts for as much.
     int turn = 0;
     double sums[4];
     auto walk = [&](int i, int stopped, int without) {
         z = logits + (size_t)(row0 + i) * vocab;
         y = draft_logits && i < count ? draft_logits + (size_t)(draft0 + i) * vocab : nullptr;
-        z_max = s.row_max[0][stopped];
-        y_max = s.row_max[1][stopped];
-        const double zt = s.row_sum[0][stopped], yt = s.row_sum[1][stopped];
+        zc = scale64(s.row_max[0][stopped], inv_t, t);
+        yc = scale64(s.row_max[1][stopped], inv_t, t);
+        line = y ? s.row_max[0][stopped] - s.row_max[1][stopped] + t * logf(s.row_sum[0][stopped] / s.row_sum[1][stopped]) : -INFINITY;
 #pragma unroll
         for (int n = 0; n < 4; ++n) sums[n] = 0.0;
         for (int i0 = begin + lane; i0 < end; i0 += 32 * kAhead) {
             double ez[kAhead], ey[kAhead];
-            weights(i0, ez, ey);
+            unsigned more = 0;
+            weights(i0, ez, ey, more);
 #pragma unroll
             for (int k = 0; k < kAhead; ++k) {
                 sums[0] += ez[k];
                 sums[1] += ey[k];
-                const bool more = y ? ez[k] * yt > ey[k] * zt : i0 + 32 * k != without;
-                sums[2] += more ? ez[k] : 0.0;
-                sums[3] += more ? ey[k] : 0.0;
+                if ((more >> k & 1u) && i0 + 32 * k != without) {
+                    sums[2] += ez[k];
+                    sums[3] += ey[k];
+                }
             }
         }
         cluster_sums(cluster, s, turn, sums);
@@ -342,10 +351,10 @@ verify_pick_kernel(const float* __restrict__ logits, const float* __restrict__ d
         why = s.stop & 3;
         if (why == kNothing || greedy) break;
         const int d = a < count ? drafts[draft0 + a] : -1;
-        walk(a, (a - from) % kPickWarps, d);  // (all CTAs of the cluster come here together)
+        walk(a, (a - from) % kPickWarps, draft_logits ? -1 : d);  // (all CTAs of the cluster come here together)
         if (why != kNear) break;
-        const double eq = y ? weight64(s.table, y[d], y_max, inv_t) : 1.0;
-        if (!(accept_draws[draft0 + a] * eq * sums[0] < weight64(s.table, z[d], z_max, inv_t) * sums[1])) break;
+        const double eq = y ? weight64(s.table, y[d], yc) : 1.0;
+        if (!(accept_draws[draft0 + a] * eq * sums[0] < weight64(s.table, z[d], zc) * sums[1])) break;
         if (tid == 0) s.stop = 0x7fffffff;  // (everybody has read it: they have met)
         __syncthreads();
         from = a + 1;
@@ -366,7 +375,8 @@ verify_pick_kernel(const float* __restrict__ logits, const float* __restrict__ d
     bool plain = a >= count;
     auto masses = [&](int first, double (&m)[kAhead]) {
         double ey[kAhead];
-        weights(first, m, ey);
+        unsigned more = 0;
+        weights(first, m, ey, more);
 #pragma unroll
         for (int k = 0; k < kAhead; ++k) {
             const double p = __dmul_rn(m[k], ip);  // (rounded like q: equal ones leave nothing)
