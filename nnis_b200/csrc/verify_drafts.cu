@@ -167,6 +167,21 @@ __device__ __forceinline__ double warp_sum64(double v) {
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
+// The same over either half of a warp: sixteen values, in every lane if both halves hold them.
+__device__ __forceinline__ double half_sum64(double v) {
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+// Sum of the lanes up to this one, of sixteen.
+__device__ __forceinline__ double half_scan64(double v) {
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) {
+        const double up = __shfl_up_sync(0xffffffffu, v, o, 16);
+        if ((threadIdx.x & 15) >= o) v += up;
+    }
+    return v;
+}
 
 // exp((x - max) / T) in 64 bits for x <= max: with u = 64 (x - max) / (T ln 2) and k the whole number next to it, 2^(k / 64) from a
 // table times the series of 2^((u - k) / 64) to the fourth power (what is left out is 4e-14), after P. T. P. Tang's
@@ -209,10 +224,10 @@ __device__ __forceinline__ void cluster_sums(cg::cluster_group cluster, PickShar
         if (lane == 0) s.warp[n][threadIdx.x >> 5] = v[n];
     }
     __syncthreads();
-    const int ctas = (int)cluster.num_blocks();
+    const int ctas = (int)cluster.num_blocks(), at = lane & 15;  // (chains of 64-bit sums are slow: trees of sixteen)
     if (threadIdx.x < 32) {
 #pragma unroll
-        for (int n = 0; n < 4; ++n) v[n] = warp_sum64(lane < kPickWarps ? s.warp[n][lane] : 0.0);
+        for (int n = 0; n < 4; ++n) v[n] = half_sum64(s.warp[n][at]);
         if (lane < ctas) {
             PickShared* other = cluster.map_shared_rank(&s, lane);
 #pragma unroll
@@ -221,11 +236,9 @@ __device__ __forceinline__ void cluster_sums(cg::cluster_group cluster, PickShar
     }
     cluster.sync();
 #pragma unroll
-    for (int n = 0; n < 4; ++n) {
-        v[n] = 0.0;
-        for (int i = 0; i < ctas; ++i) v[n] += s.cta[turn][n][i];
-    }
+    for (int n = 0; n < 4; ++n) v[n] = half_sum64(at < ctas ? s.cta[turn][n][at] : 0.0);
 }
+static_assert(kPickWarps == 16 && kPickCtas == 16, "sums of sixteen");
 
 __global__ void __launch_bounds__(kPickThreads, 2)
 verify_pick_kernel(const float* __restrict__ logits, const float* __restrict__ draft_logits, const int* __restrict__ drafts,
@@ -405,26 +418,22 @@ verify_pick_kernel(const float* __restrict__ logits, const float* __restrict__ d
         }
     }
     const double target = pick_draws[b] * total;
-    double before = 0.0, held = 0.0;
-    int last = 0;  // the last CTA with any weight
-    for (int i = 0; i < ctas; ++i) {
-        const double other = fmax(mp * s.cta[turn ^ 1][2][i] - mq * s.cta[turn ^ 1][3][i], 0.0);
-        if (i < rank) before += other;
-        if (i == rank) held = other;
-        if (other > 0.0) last = i;
-    }
+    // Where in the row the target lies: the CTAs' masses, lane by lane, then the warps'.  A draw at the very end of the
+    // sums belongs to the last id with any weight.
+    auto place = [&](double mass, double from, int mine, double& ahead) {
+        const double upto = half_scan64(mass);
+        const unsigned some = __ballot_sync(0xffffffffu, mass > 0.0) & 0xffffu;
+        const int last = some ? 31 - __clz(some) : 0;
+        const double own = __shfl_sync(0xffffffffu, mass, mine), end_of = from + __shfl_sync(0xffffffffu, upto, mine);
+        const double begin_of = from + (mine ? __shfl_sync(0xffffffffu, upto, mine - 1) : 0.0);
+        ahead = begin_of;
+        return own > 0.0 && target >= begin_of && (target < end_of || mine == last);
+    };
     if (rank == 0 && tid == 0) accepted[b] = a;
-    // a draw at the very end of the sums belongs to the last id with any weight
-    if (!((target >= before && target < before + held) || (rank == last && target >= before + held))) return;
-    double ahead = before, own = 0.0;
-    int last_warp = 0;
-    for (int w = 0; w < kPickWarps; ++w) {
-        const double other = fmax(mp * s.warp[2][w] - mq * s.warp[3][w], 0.0);
-        if (w < warp) ahead += other;
-        if (w == warp) own = other;
-        if (other > 0.0) last_warp = w;
-    }
-    if (!(own > 0.0 && ((target >= ahead && target < ahead + own) || (warp == last_warp && target >= ahead + own)))) return;
+    const int at = lane & 15;
+    double before, ahead;
+    if (!place(at < ctas ? fmax(mp * s.cta[turn ^ 1][2][at] - mq * s.cta[turn ^ 1][3][at], 0.0) : 0.0, 0.0, rank, before)) return;
+    if (!place(fmax(mp * s.warp[2][at] - mq * s.warp[3][at], 0.0), before, warp, ahead)) return;
     int found = -1, last_id = -1;
     for (int i0 = begin; found < 0; i0 += 32 * kAhead) {
         if (i0 >= end) {
