@@ -13,7 +13,7 @@ used here in process.
 from __future__ import annotations
 
 import warnings
-from typing import Callable, List, Optional, Sequence, Union
+from typing import Callable, Dict, List, Optional, Sequence, Union
 
 import numpy as np
 import torch
@@ -49,6 +49,7 @@ class EngineBackend:
         self._uncaptured = set()  # keys of decoders whose capture has failed for a session
         self._views = {}
         self._shared = BatchUnits(engine)
+        self._drafted: Dict[int, BatchUnits] = {}  # by number of tokens
         self._pinned = None
         self._picked = None
         self._picked_for = None
@@ -130,6 +131,27 @@ class EngineBackend:
         if dec is None or not 0 <= token < engine.spec.vocab_size:
             return engine.step([SequenceStep(slot, [token], [0])])[0]  # (which says what is wrong with a token)
         return self._replay([slot], [token], True, dec).logits[0]
+
+    def drafted_logits(self, slot: int, tokens: List[int], again: bool) -> torch.Tensor:
+        """Logits [tokens, vocab] of one sequence's next tokens, a token and drafts after it.  From the third such step on
+        (``again``) it is a captured step whose rows are the tokens: what a sequence of the SmolLM2-135M shape waits for is
+        then 0.6 ms instead of the 8 of its launches from Python one by one."""
+        engine, cache, n = self.engine, self.engine.cache, len(tokens)
+        vocab = engine.spec.vocab_size
+        if not again or self.decode_greedy is None or not engine.model.all_share or n > self.max_rows \
+                or not all(0 <= t < vocab for t in tokens):
+            return engine.step([SequenceStep(slot, tokens, list(range(n)))], drafted=True)
+        held = cache.length(slot)
+        positions = list(range(held, held + n))
+        cache.reserve([slot], [held + n])
+        rows = self._decoder_key(n, held + n, True)[0]
+        units = self._drafted.setdefault(n, BatchUnits(engine, drafted=True)).units([slot] * n, positions, rows)
+        dec = self._decoder(n, held + n, True, rooms_of(units))
+        dec.plans.fill(units)
+        self.h2d_bytes += dec.upload(tokens, positions, [slot] * n)
+        dec.launch()
+        cache.commit([slot], [held + n])
+        return dec.logits[:n]
 
     def _captured(self, key) -> Optional[GraphDecoder]:
         """The decoder of this key with its graph, captured now.  Where that fails (no memory for its buffers, say) None,
@@ -350,6 +372,7 @@ class InferenceSession:
         self.engine = llm.engine
         self.slot = self.engine.acquire_slot() if slot is None else slot
         self._decoded = 0  # tokens that this session has decoded one by one
+        self._drafted = 0  # steps with drafts that it has run
 
     def position(self) -> int:
         return self.engine.cache.length(self.slot)
@@ -454,8 +477,8 @@ class InferenceSession:
         while True:
             held = self.position()
             if proposed:
-                want = list(range(len(feed) - len(proposed) - 1, len(feed)))
-                logits = self.engine.step([SequenceStep(self.slot, feed, want)], drafted=True)
+                logits = self.llm.backend.drafted_logits(self.slot, feed, self._drafted >= 2)
+                self._drafted += 1
             elif len(feed) == 1 and emitted:
                 logits = self.llm.backend.decode_logits(self.slot, feed[0], self._decoded >= self.EAGER_TOKENS).reshape(1, -1)
                 self._decoded += 1

@@ -14,6 +14,9 @@ import torch
 from ..sampling import device as device_sampling
 
 
+CAPTURED = 16  # most tokens that a drafting model takes by a captured step
+
+
 class LookupDrafter:
     """Drafts what followed the last time that the sequence's last ``ngram`` tokens (or fewer, down to one) came up in it."""
 
@@ -74,7 +77,13 @@ class SessionDrafter:
         same = next((i for i, (a, b) in enumerate(zip(self._held, tokens)) if a != b), min(len(self._held), len(tokens)))
         same = min(same, len(tokens) - 1)  # (the last token's logits are wanted)
         self.session.truncate(same)
-        logits = engine.step([SequenceStep(self.session.slot, tokens[same:], [len(tokens) - same - 1])])
+        fresh, backend, slot = tokens[same:], self.llm.backend, self.session.slot
+        if len(fresh) == 1:
+            logits = backend.decode_logits(slot, fresh[0], True)
+        elif len(fresh) <= CAPTURED:
+            logits = backend.drafted_logits(slot, fresh, True)[-1]
+        else:
+            logits = engine.step([SequenceStep(slot, fresh, [len(fresh) - 1])])
         vocab, drafts = engine.spec.vocab_size, []
         kept = torch.empty((count, vocab), dtype=torch.float32, device=engine.device) if temperature > 0 else None
         picked = torch.empty(1, dtype=torch.int32, device=engine.device)
@@ -87,6 +96,6 @@ class SessionDrafter:
                 device_sampling.greedy(logits.reshape(1, -1), picked)
             drafts.append(int(picked.item()))
             if i + 1 < count:
-                logits = self.llm.backend.decode_logits(self.session.slot, drafts[-1], True)
+                logits = backend.decode_logits(slot, drafts[-1], True)
         self._held = tokens + drafts[:-1]
         return drafts, kept

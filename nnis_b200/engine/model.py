@@ -100,7 +100,12 @@ class DecoderModel:
             ask = getattr(self.blocks[entry.layer].mixer, "shared_key", None)
             if ask is not None:
                 keys[ask(view)] = True
+            else:
+                keys[None] = True
         self._shared_keys = [k for k in keys if k is not None]
+        # every mixer can: a captured step may bring several tokens of one sequence (kernels of other mixers ask for pages
+        # ahead of the kernel that writes them, which is sound only for a step's single token)
+        self.all_share = None not in keys
 
     def shared_keys(self):
         """The cache group and head layout of every attention that can read pages shared by several rows once."""

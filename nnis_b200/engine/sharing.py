@@ -31,8 +31,7 @@ def shared_tree(cache, group: int, slots: Sequence[int], seqs: Sequence[int], po
         return None
     nodes, tails = ops.shared_nodes([cache.page_table(group, s) for s in slots], seqs, positions, ahead)
     saved = sum((len(rows) - 1) * (b - a) for rows, a, b in nodes)
-    return (nodes, tails) if saved and saved * PAGE_SIZE * g.kv_heads * (g.head_dim + g.value_dim) * g.k.element_size() >= least_bytes \
-        else None
+    return (nodes, tails) if saved * PAGE_SIZE * g.kv_heads * (g.head_dim + g.value_dim) * g.k.element_size() >= least_bytes else None
 
 
 class SharedRows:
@@ -75,10 +74,10 @@ class KeptPlans:
 
 class BatchUnits:
     """What a batch of single tokens shares, for captured steps: made anew when its sequences, what they share, or how
-    far they may grow have changed."""
+    far they may grow have changed.  ``drafted``: the rows are tokens of one sequence, which share whatever they see alike."""
 
-    def __init__(self, engine):
-        self.engine = engine
+    def __init__(self, engine, drafted: bool = False):
+        self.engine, self.drafted = engine, drafted
         self._made_for = self._positions = self._units = None
         self._until = 0
 
@@ -86,9 +85,9 @@ class BatchUnits:
         """Per attention of the model that gains by it, its units, members and record offsets, for ``rows`` rows of which
         the first are the sequences; None where none gains."""
         cache = self.engine.cache
-        if len(slots) < 2 or not cache.shares_pages():
+        if not self.drafted and (len(slots) < 2 or not cache.shares_pages()):
             return None
-        made_for = (tuple(slots), cache.share_epoch, rows)
+        made_for = (tuple(slots), None if self.drafted else cache.share_epoch, rows)  # (a plan names columns of a table, not pages)
         if made_for == self._made_for and all(0 <= now - then <= self._until for now, then in zip(positions, self._positions)):
             return self._units
         seqs, padding = list(range(len(slots))), rows - len(slots)
@@ -97,7 +96,7 @@ class BatchUnits:
         for key in self.engine.model.shared_keys():
             if key[0] not in trees:
                 trees[key[0]] = shared_tree(cache, key[0], slots, seqs + [0] * padding, list(positions) + [-1] * padding,
-                                              LEAST_BYTES, ahead)
+                                              0 if self.drafted else LEAST_BYTES, ahead)
             if trees[key[0]] is not None:
                 units[key] = ops.attention_shared_units(*trees[key[0]], seqs + [0] * padding, *key[1:], self.engine.dtype,
                                                         self.engine.device)

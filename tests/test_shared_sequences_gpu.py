@@ -258,3 +258,42 @@ def test_designs_with_states_and_windows_fork_and_refuse_drafts(tmp_path):
         if llm.engine.cache.fixed_history():
             with pytest.raises(ValueError):
                 llm.new_session().generate_drafted([1, 2], GenerationConfig(4), LookupDrafter())
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_captured_steps_of_drafts(folder, dtype):
+    """Several tokens of a sequence as rows of a captured step, over page ends, with tokens taken back between them, two
+    sessions and two numbers of tokens in turn, one of them forked: logits as token by token."""
+    from nnis_b200 import LLM
+    from nnis_b200.engine import SequenceStep
+    llm = LLM(folder, dtype=dtype, max_tokens=1 << 14, max_batch=16)
+    engine, backend = llm.engine, llm.backend
+    a, b = engine.acquire_slot(), engine.acquire_slot()
+    history = {a: tokens(70, 1270), b: tokens(71, 60)}
+    for s, h in history.items():
+        engine.step([SequenceStep(s, h, [])])
+    for turn in range(24):
+        if turn == 12:
+            c = engine.fork(a)
+            history[c] = list(history[a])
+        for s, n in ((a, 5), (b, 3 if turn % 2 else 5)):
+            new = tokens(1000 + 10 * turn + s, n)
+            got = backend.drafted_logits(s, new, True).cpu().numpy()
+            keep = 1 + turn % n
+            if turn % 6 == 0:
+                other = engine.acquire_slot()
+                engine.step([SequenceStep(other, history[s], [])])
+                want = np.concatenate([engine.step([SequenceStep(other, [t], [0])]).cpu().numpy() for t in new])
+                engine.release_slot(other)
+                assert close(got, want, dtype), (turn, s)
+            history[s] += new[:keep]
+            engine.truncate(s, len(history[s]))
+            engine.cache.check()
+    for s in (a, c):  # what was forked is as it was
+        t = tokens(5, 1)
+        got = engine.step([SequenceStep(s, t, [0])])[0].cpu().numpy()
+        other = engine.acquire_slot()
+        want = engine.step([SequenceStep(other, history[s] + t, [len(history[s])])])[0].cpu().numpy()
+        engine.release_slot(other)
+        assert close(got, want, dtype)
+    engine.check_status()
