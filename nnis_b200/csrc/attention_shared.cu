@@ -184,7 +184,8 @@ cudaError_t shared_units_any(const SharedArgs& a, int n_units, int tile, bool f3
 // units: n[0] units of the first kind, n[1] of the second, n[2] of the third.  `form` 0 (any even head size, float32 or
 // bfloat16) and 2 (float32, heads of 64 and 128): at most 16, at most 64 entries, none; `form` 1 (bfloat16, heads of 64 and 128): at most 16, 32 and 128, the last
 // of which cover only positions that all their rows see.  The plan (units, members, record) is the host's, made of
-// page lists that the call's page table agrees with; page ids outside the store hold no keys.  partial: records x nq x d floats,
+// page lists that the call's page table agrees with; a page id outside the store holds no keys (zeros in units of the third kind of
+// form 1).  partial: records x nq x d floats,
 // sums: records x nq x 2.  tickets (n_tokens x nq counters, zero, left zero): every row is merged by the CTA that completes it, and no
 // merge is launched (where all units are of the second kind, or `form` is not 1); every row then has a record.
 NNIS_API int nnis_attention_shared(const void* q, int q_stride, const void* k_cache, const void* v_cache, const int* token_pos,

@@ -194,7 +194,7 @@ def copy_pages(k: torch.Tensor, v: Optional[torch.Tensor], moves) -> None:
         _need(v.dim() == 5 and v.shape[:4] == k.shape[:4] and v.device == k.device and v.numel() > 0,
               "copy_pages: v [layers, pages, kv_heads, page_size, value dim] beside k")
         v_row = v.shape[4] * v.element_size()
-    _need(k_row % 4 == 0 and v_row % 4 == 0, "copy_pages: rows of a multiple of four bytes")
+    _need(k_row % 2 == 0 and v_row % 2 == 0, "copy_pages: rows of a multiple of two bytes")
     _need(layers <= 65535 and heads * page_size * max(k_row, v_row) < 2 ** 32, "copy_pages: at most 65,535 layers, pages below 4 GB")
     if not moves:
         return
@@ -2927,6 +2927,7 @@ def attention_shared_plan(tables, seqs, positions, heads: int, kv_heads: int, he
     for s, p in zip(seqs, positions):
         _need(0 <= s < len(tables), f"shared attention: sequence {s} of {len(tables)}")
         _need(p < len(tables[s]) * 64, f"shared attention: position {p} is beyond its sequence's {len(tables[s])} pages")
+        _need(p < 0 or min(tables[s][:p // 64 + 1]) >= 0, f"shared attention: sequence {s} lacks a page that position {p} reads")
     nodes, tails = shared_nodes(tables, seqs, positions)
     return attention_shared_plan_of(nodes, tails, seqs, positions, heads, kv_heads, head_dim, dtype, torch.device(device))
 

@@ -63,8 +63,8 @@ static cudaError_t launch_moves(void* k, void* v, int layers, int pages, int kv_
         p.rows[i] = rows[i];
         most = rows[i] > most ? rows[i] : most;
     }
-    const bool wide = ((uintptr_t)k | (uintptr_t)v | (uintptr_t)k_row | (uintptr_t)(v ? v_row : 0)) % 16 == 0;
-    const int unit = wide ? 16 : 4, tensors = v ? 2 : 1;
+    const uintptr_t all = (uintptr_t)k | (uintptr_t)v | (uintptr_t)k_row | (uintptr_t)(v ? v_row : 0);
+    const int unit = all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : 2, tensors = v ? 2 : 1;
     const long long words = (long long)kv_heads * most * (k_row > v_row ? k_row : v_row) / unit;
     const long long ctas = (long long)n * tensors * layers;
     long long share = (words + 1023) / 1024;                // four words a thread
@@ -73,25 +73,25 @@ static cudaError_t launch_moves(void* k, void* v, int layers, int pages, int kv_
     if (share < 1) share = 1;
     if (share > 65535) share = 65535;
     const dim3 grid((unsigned)(n * tensors), (unsigned)layers, (unsigned)share);
-    if (wide) copy_pages_kernel<uint4, N><<<grid, 256, 0, stream>>>(p, k, v, pages, kv_heads, page_size, k_row / 16, v_row / 16);
-    else copy_pages_kernel<uint32_t, N><<<grid, 256, 0, stream>>>(p, k, v, pages, kv_heads, page_size, k_row / 4, v_row / 4);
+    auto kernel = unit == 16 ? copy_pages_kernel<uint4, N> : unit == 4 ? copy_pages_kernel<uint32_t, N> : copy_pages_kernel<uint16_t, N>;
+    kernel<<<grid, 256, 0, stream>>>(p, k, v, pages, kv_heads, page_size, k_row / unit, v_row / unit);
     return cudaGetLastError();
 }
 
 }  // namespace nnis
 
-// k and v (or null): [layers, pages, kv_heads, page_size, row] with rows of `k_row` and `v_row` bytes, multiples of 4.
+// k and v (or null): [layers, pages, kv_heads, page_size, row] with rows of `k_row` and `v_row` bytes, multiples of 2.
 // moves, on the host: `count` sources, then targets, then numbers of rows (0 to page_size).  NNIS_ERR_ARGUMENT, with nothing
 // copied, where a page is outside the store, the target of two moves, or a target and a source.
 NNIS_API int nnis_copy_pages(void* k, void* v, int layers, int pages, int kv_heads, int page_size, int k_row, int v_row,
                              const int* moves, int count, int sms, cudaStream_t stream) {
     using namespace nnis;
-    if (!k || !moves || count < 0 || layers <= 0 || pages <= 0 || kv_heads <= 0 || page_size <= 0 || k_row <= 0 || k_row % 4 ||
-        (v && (v_row <= 0 || v_row % 4)))
+    if (!k || !moves || count < 0 || layers <= 0 || pages <= 0 || kv_heads <= 0 || page_size <= 0 || k_row <= 0 || k_row % 2 ||
+        (v && (v_row <= 0 || v_row % 2)))
         return NNIS_ERR_ARGUMENT;
     const long long page_bytes = (long long)kv_heads * page_size * (k_row > v_row ? k_row : v_row);
-    if (layers > 65535 || page_bytes / 4 >= (1LL << 31)) return NNIS_ERR_UNSUPPORTED;
-    if (((uintptr_t)k | (uintptr_t)v) % 4) return NNIS_ERR_ALIGNMENT;
+    if (layers > 65535 || page_bytes / 2 >= (1LL << 31)) return NNIS_ERR_UNSUPPORTED;
+    if (((uintptr_t)k | (uintptr_t)v) % 2) return NNIS_ERR_ALIGNMENT;
     const int *src = moves, *dst = moves + count, *rows = moves + 2 * count;
     unsigned char* seen = static_cast<unsigned char*>(calloc((size_t)pages, 1));  // 1: a source, 2: a target
     if (!seen) return (int)cudaErrorMemoryAllocation;

@@ -258,7 +258,8 @@ verify_pick_kernel(const float* __restrict__ logits, const float* __restrict__ d
     const double inv_t = greedy ? 1.0 : 1.0 / (double)t;
     pdl_wait();
     pdl_launch_dependents();
-    if (row0 < b || count < 0 || row0 + count >= rows) {  // (offsets that no packed rows have: the whole cluster leaves)
+    // (offsets that no packed rows have: the whole cluster leaves)
+    if (row0 < b || count < 0 || row0 + count >= rows || draft0 + count > rows - (int)gridDim.y) {
         if (rank == 0 && tid == 0) {
             accepted[b] = 0;
             picked[b] = -1;

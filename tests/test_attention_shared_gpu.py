@@ -221,7 +221,8 @@ def test_shared_attention_refuses():
     plan_of = lambda **kw: o.attention_shared_plan(**{**dict(tables=[[0, 1], [0, 2]], seqs=[0, 1], positions=[70, 80], heads=4,
                                                              kv_heads=2, head_dim=64, dtype=torch.float32, device=DEV), **kw})
     for bad in (dict(seqs=[0, 2]), dict(positions=[70, 128]), dict(positions=[1]), dict(heads=3), dict(head_dim=63),
-                dict(head_dim=258), dict(dtype=torch.float16), dict(seqs=[], positions=[])):
+                dict(head_dim=258), dict(dtype=torch.float16), dict(seqs=[], positions=[]),
+                dict(tables=[[0, -1], [0, 2]])):
         with pytest.raises(o.KernelError):
             plan_of(**bad)
     plan, ws = plan_of(), Workspace(torch.device(DEV))

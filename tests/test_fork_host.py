@@ -299,3 +299,11 @@ def test_drafts_looked_up_in_the_text():
     assert d.propose([5], 2, 0.0) == ([], None)
     with pytest.raises(ValueError):
         LookupDrafter(0)
+
+
+def test_the_command_line_shares_prefixes_of_batches_only():
+    from nnis_b200.cli.main import UsageError, parse_args
+    batch = ["generate-batch", "--model", "m", "--prompt-ids", "1,2", "--prompt-ids", "1,3", "--seed", "1", "--seed", "2"]
+    assert not parse_args(batch).share_prefix and parse_args([*batch, "--share-prefix"]).share_prefix
+    with pytest.raises(UsageError):
+        parse_args(["generate", "--model", "m", "--prompt-ids", "1,2", "--share-prefix"])

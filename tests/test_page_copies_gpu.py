@@ -12,10 +12,10 @@ def ops():
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
-@pytest.mark.parametrize("layers,heads,dim,vdim", [(1, 1, 2, 2), (3, 3, 64, 64), (2, 5, 48, 30), (2, 1, 66, 0), (30, 2, 128, 64)])
+@pytest.mark.parametrize("layers,heads,dim,vdim", [(1, 1, 2, 2), (3, 3, 64, 64), (2, 5, 48, 30), (2, 1, 66, 0), (30, 2, 128, 64), (2, 1, 33, 0), (1, 3, 5, 7)])
 @pytest.mark.parametrize("case", ["one row", "ragged", "whole", "one source", "mixed"])
 def test_rows_of_pages_are_copied(dtype, layers, heads, dim, vdim, case):
-    """Rows from one to all, words of 16 and of 4 bytes, values of another size or none, no rows at all."""
+    """Rows from one to all, words of 16, 4 and 2 bytes, values of another size or none, no rows at all."""
     g = torch.Generator().manual_seed(layers * dim)
     pages = 23
     k = torch.randn((layers, pages, heads, 64, dim), generator=g).to(dtype).to(DEV)

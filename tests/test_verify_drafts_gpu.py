@@ -200,7 +200,9 @@ def test_equal_distributions_leave_the_target_itself():
 def test_offsets_that_no_rows_have():
     z = torch.randn((6, 50), generator=torch.Generator().manual_seed(1))
     a, p = run(z, [1, 1, 1], [0, 0, 0], [1.0] * 3, [0.5] * 3, [0.5] * 3, first=[0, 5, 4, 9])
-    assert a[1] == 0 and p[1] == -1 and a[2] == 0 and p[2] == -1
+    assert a == [0, 0, 0] and p == [-1, -1, -1]  # (more drafts than there are, rows that run back, rows beyond the last)
+    a, p = run(z, [1, 1, 1], [0, 0, 0], [1.0] * 3, [0.5] * 3, [0.5] * 3, first=[-2, 2, 2, 6])
+    assert a[:2] == [0, 0] and p[:2] == [-1, -1]
 
 
 def test_verify_in_a_graph_and_on_another_stream():
