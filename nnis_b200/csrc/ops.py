@@ -2899,9 +2899,10 @@ def attention_shared_units(nodes, tails, seqs, heads: int, kv_heads: int, head_d
     if form == 1:
         # (small units go warp by warp where they are many; else that is only a launch more)
         pieces = sum(len(rows) * (heads // kv_heads) <= 16 for rows, *_ in nodes) + (len(tails) if heads // kv_heads <= 16 else 0)
-        kinds = ((16 if pieces * kv_heads > 2 * sms else 0, 12 * sms, 1, 16), (32, 3 * sms, 4, 16), (128, 2 * sms, 2, 1 << 20))
+        kinds = ((16 if pieces * kv_heads > 2 * sms else 0, 12 * sms, 1, 16, True), (32, 3 * sms, 4, 16, False),
+                 (128, 2 * sms, 2, 1 << 20, False))
     else:
-        kinds = ((16, 4 * sms, 1, 16), (64, 2 * sms, 1, 16), (0, 0, 0, 0))
+        kinds = ((16, 4 * sms, 1, 16, False), (64, 2 * sms, 1, 16, False), (0, 0, 0, 0, False))
     return shared_units(nodes, tails, seqs, heads // kv_heads, kv_heads, kinds, 1)
 
 

@@ -6,9 +6,11 @@ import pytest
 
 from nnis_b200.csrc.shared_plan import PAGE, shared_nodes, shared_units
 
-# (most entries, CTAs at once, fewest and most pages of a chunk) per kind, the last kind that takes ends
-KINDS = [((16, 600, 1, 16), (32, 400, 4, 16), (128, 300, 2, 1 << 20)), ((0, 0, 0, 0), (32, 8, 2, 16), (128, 8, 2, 100)),
-         ((16, 8, 1, 3), (64, 600, 2, 16), (0, 0, 0, 0)), ((16, 1, 4, 16), (64, 1, 4, 16), (0, 0, 0, 0))]
+NONE = (0, 0, 0, 0, False)
+# (most entries, CTAs at once, fewest and most pages of a chunk, from a queue) per kind
+KINDS = [((16, 600, 1, 16, True), (32, 400, 4, 16, False), (128, 300, 2, 1 << 20, False)),
+         (NONE, (32, 8, 2, 16, False), (128, 8, 2, 100, False)),
+         ((16, 8, 1, 3, True), (64, 600, 2, 16, False), NONE), ((16, 1, 4, 16, False), (64, 1, 4, 16, False), NONE)]
 
 
 def batch(seed):
@@ -76,6 +78,7 @@ def test_chunks_fit_the_device_where_they_can():
     """A kind's CTAs are no more than it has at once unless its pieces alone are."""
     tables = [list(range(62)) + [100 + r] for r in range(24)]
     nodes, tails = shared_nodes(tables, range(24), [62 * PAGE + 9] * 24)
-    units, _, _ = shared_units(nodes, tails, range(24), 1, 32, ((16, 1776, 1, 16), (32, 444, 4, 16), (128, 296, 2, 1 << 20)), 1)
+    units, _, _ = shared_units(nodes, tails, range(24), 1, 32, ((16, 1776, 1, 16, True), (32, 444, 4, 16, False),
+                                                                          (128, 296, 2, 1 << 20, False)), 1)
     assert len(units[1]) * 32 <= 444 and sum(u[4] - u[3] for u in units[1].tolist()) == 62
     assert len(units[0]) == 24
