@@ -11,10 +11,15 @@
 // Two launches.  The first sums every row once, in 32 bits (CTA: a share of a row; running maximum and sum, argmax).  In the
 // second a cluster of CTAs takes a sequence: the drafts are decided in order from the rows' sums and the two logits of the
 // draft itself, in 64 bits; a decision within 1e-4 of its border is taken again with the row's sums in 64 bits
-// (the sums' 32-bit error is below 1e-5: terms 17 bits of exponent at most where they count, 2e-6; 32 and
-// fewer additions a thread, 2e-6).  Then the one row that is drawn from is summed in 64 bits, each
-// CTA a range of ids and each warp a range of that, because a draw may fall next to a border between two of 50,000
-// tokens, and p - q cancels: 32 bits would pick another token every few hundred draws.
+// (the sums' 32-bit error is below 4e-5: exponents of 17 bits at most where they count, 2e-6, and 2^-24 for each of a
+// thread's additions one after another, 5 with 300,000 logits, 520 with the most that are taken, 2^26).  Then the one row that is
+// drawn from is summed in 64 bits, each CTA a range of ids and each warp a range of that, because a draw may fall next to a
+// border between two of 50,000 tokens, and p - q cancels: 32 bits would pick another token every few hundred draws.  That walk
+// sums p, q and both over the ids where p is the larger, so what q leaves of p needs no second one; only where it leaves next to
+// nothing are the masses summed id by id.
+//
+// The first launch is bound by bytes: 960 rows of 49,152 (189 MB) 37.5 us, 5.0 TB/s; nine rows 3.7.  The second by 64-bit
+// arithmetic (an SM has few such units) and, with few sequences, by its chain of steps: draft, row, cluster, pick.
 #include <cooperative_groups.h>
 #include <float.h>
 
@@ -418,7 +423,7 @@ verify_pick_kernel(const float* __restrict__ logits, const float* __restrict__ d
             plain = true;  // nothing is left: p and q are one
         }
     }
-    const double target = pick_draws[b] * total;
+    const double target = fmin(fmax(pick_draws[b], 0.0), 1.0) * total;  // (a draw of another range, or no number, is its next end)
     // Where in the row the target lies: the CTAs' masses, lane by lane, then the warps'.  A draw at the very end of the
     // sums belongs to the last id with any weight.
     auto place = [&](double mass, double from, int mine, double& ahead) {
@@ -490,13 +495,15 @@ NNIS_API int nnis_verify_drafts(const float* logits, const float* draft_logits, 
         return NNIS_ERR_ARGUMENT;
     const int draft_rows = rows - n_seqs, all_rows = rows + (draft_logits ? draft_rows : 0);
     if (draft_rows > 0 && (!drafts || !accept_draws)) return NNIS_ERR_ARGUMENT;
-    if (all_rows > 65535 || n_seqs > 65535 || vocab > (1 << 30)) return NNIS_ERR_UNSUPPORTED;
+    if (all_rows > 65535 || n_seqs > 65535 || vocab > (1 << 26)) return NNIS_ERR_UNSUPPORTED;
     if ((uintptr_t)scratch % 16) return NNIS_ERR_ALIGNMENT;
     const int n_parts = verify_parts(rows + draft_rows, vocab), per = (vocab + n_parts - 1) / n_parts;
     cudaError_t e = launch_dependent(verify_rows_kernel, dim3(n_parts, all_rows), kVerifyThreads, 0, stream, logits, draft_logits,
                                      first_row, temperature, n_seqs, rows, draft_rows, vocab, per, static_cast<RowSum*>(scratch));
     if (e != cudaSuccess) return (int)e;
-    // As many CTAs a sequence as the device holds at once (two an SM) for all of them, sixteen at most, four at least.
+    // As many CTAs a sequence as the device holds at once (two an SM) for all of them, sixteen at most, four at least: a row of
+    // 49,152 is walked in 9.8 us by sixteen, 15.4 by eight (24 sequences), 32 by four (64 sequences, which eight would
+    // take in two turns).
     cudaLaunchConfig_t cfg = {};
     static const int slots = 2 * device_sms();
     int ctas = kPickCtas;

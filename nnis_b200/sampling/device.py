@@ -42,7 +42,7 @@ def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, first_row: torch.T
     With p and q the softmax of the rows over the temperature, a draft is kept iff draw * q(draft) < p(draft)
     (q = 1 without draft logits).  ``accepted[b]`` (int32): the drafts before the first that is not kept; ``picked[b]``
     (int32): the token after them, drawn with ``pick_draws[b]`` (float64) in id order from max(p - q, 0) where a draft was
-    not kept and from p where all were.  Temperature 0 (or less): a draft is kept iff it is the argmax, which is also the pick.
+    not kept and from p where all were (a draw outside [0, 1] is taken for its next end, NaN for 0).  Temperature 0 (or less): a draft is kept iff it is the argmax, which is also the pick.
     An id outside the vocabulary is never kept.  A row without probability (all logits -inf, a NaN or +inf among
     them) ends its sequence there: picked is -1.  Offsets that no packed rows have give 0 and -1."""
     ops.verify_drafts(logits, drafts, first_row, temperatures, accept_draws, pick_draws, accepted, picked, draft_logits,

@@ -205,6 +205,21 @@ def test_offsets_that_no_rows_have():
     assert a[:2] == [0, 0] and p[:2] == [-1, -1]
 
 
+@pytest.mark.parametrize("model", [True, False])
+def test_pick_draws_of_another_range(model):
+    """Below 0 and NaN: the first id with any mass; from 1 on: the last.  Nothing is left unwritten."""
+    counts = [0, 1, 0, 1, 0, 1]
+    logits, _, drafts, temps, accept, _, draft_logits = make_case(5, counts, 4099, model=model)
+    logits[:, :3], logits[:, -2:] = -math.inf, -math.inf
+    accept = [1.0 - 2.0 ** -53] * 3
+    if draft_logits is not None:
+        draft_logits = draft_logits.flip(0).contiguous()
+    case = lambda picks: (logits, counts, drafts, temps, accept, picks, draft_logits)
+    low, high = plain(*case([0.0] * 6)), plain(*case([1.0] * 6))
+    assert run(*case([-0.25, -0.25, math.nan, math.nan, -math.inf, -1e-300])) == low
+    assert run(*case([1.0, 1.0, 1.5, 1.5, math.inf, math.inf])) == high
+
+
 def test_verify_in_a_graph_and_on_another_stream():
     from nnis_b200.engine.workspace import Workspace
     from nnis_b200.sampling import device
