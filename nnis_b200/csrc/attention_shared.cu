@@ -4,7 +4,8 @@
 // A CTA owns a unit and a kv head: a tile of 16 or 64 entries (token row, query head) over the unit's pages.  A page of K
 // comes into shared memory as float32, scores of tile x 64 keys are sums in registers (a thread: 1 or 4 entries x 4 keys),
 // the softmax's running maximum and sum are a half-warp's shuffles, the weights go to shared memory and the outputs, a
-// thread's 1 or 4 entries x d / 16 values, are added up in registers while the page's V replaces its K.
+// thread's 1 or 4 entries x d / 16 values, are added up in registers while the page's V replaces its K.  It is the form that is
+// right for every size, not a fast one: its loads wait for its products.
 #include "attention_shared.cuh"
 
 namespace nnis {

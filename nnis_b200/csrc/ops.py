@@ -400,7 +400,7 @@ def _verify_refused(logits, drafts, first_row, temperatures, accept_draws, pick_
     rows, vocab = logits.shape
     b = first_row.numel() - 1
     _need(1 <= b <= rows, f"verify: first_row holds one number more than there are sequences; got {b + 1} for {rows} rows")
-    _need(rows <= 32767 and vocab <= 1 << 30, "verify: at most 32,767 rows")
+    _need(rows <= 32767 and vocab <= 1 << 26, "verify: at most 32,767 rows of at most 2^26 logits")
     drafted = rows - b
     for t, name in ((drafts, "drafts"), (first_row, "first_row"), (accepted, "accepted"), (picked, "picked")):
         _need(t.dtype == torch.int32, f"verify: {name} int32")
@@ -422,7 +422,7 @@ def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, first_row: torch.T
     b, device, i32, f32, f64 = first_row.numel() - 1, logits.device, torch.int32, torch.float32, torch.float64
     rows, vocab = logits.shape if logits.dim() == 2 else (0, 0)
     drafted = rows - b
-    good = 1 <= b <= rows <= 32767 and 0 < vocab <= 1 << 30
+    good = 1 <= b <= rows <= 32767 and 0 < vocab <= 1 << 26
     for t, dtype, count in ((logits, f32, rows * vocab), (drafts, i32, drafted), (first_row, i32, b + 1), (temperatures, f32, b),
                             (accept_draws, f64, drafted), (pick_draws, f64, b), (accepted, i32, b), (picked, i32, b)):
         good = good and t.dtype == dtype and t.numel() == count and t.device == device and t.is_contiguous()
@@ -2856,7 +2856,8 @@ class SharedPlan:
         at = ints.data_ptr()
         self.units, self.members = at, at + 32 * sum(counts)
         self.record = self.members + 4 * members
-        # rows merged by the CTA that completes them save a launch, where a CTA has little to merge
+        # rows merged by the CTA that completes them save a launch, where a CTA has little to merge: 2 rows of 3 units each
+        # 11.5 us instead of 13; where a unit's entries have much (8 rows of 14 records) its kernel takes 12 to 16 us for 7.4 and 4.1
         self.merged_inside = most_entries * head_dim <= 1024 and counts[2] == 0 and (self.form != 1 or counts[0] == 0) \
             and sum(counts) * kv_heads <= 148 and records <= 8 * rows
         self.device, self.status = ints.device, status_word(ints.device).data_ptr()
@@ -2897,7 +2898,9 @@ def attention_shared_units(nodes, tails, seqs, heads: int, kv_heads: int, head_d
     sms = sm_count(device)
     form = _shared_form(dtype, head_dim)
     if form == 1:
-        # (small units go warp by warp where they are many; else that is only a launch more)
+        # Small units go warp by warp where they are many (64 rows of a page each, 32 heads: 21 -> 15.5 us); else that is only a
+        # launch more.  From 33 entries on tcgen05: units of 17 to 32 there took two prompts' 24 rows 54 us as mma.sync's 56, but
+        # 8 rows of 3 heads 15.8 for 13.6.
         pieces = sum(len(rows) * (heads // kv_heads) <= 16 for rows, *_ in nodes) + (len(tails) if heads // kv_heads <= 16 else 0)
         kinds = ((16 if pieces * kv_heads > 2 * sms else 0, 12 * sms, 1, 16, True), (32, 3 * sms, 4, 16, False),
                  (128, 2 * sms, 2, 1 << 20, False))

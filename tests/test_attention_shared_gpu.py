@@ -165,6 +165,35 @@ def test_only_padding_rows(dtype):
     check([[0], [0, 1]], [0, 1], [-1, -1], 2, 4, 2, 64, dtype)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(9, 3, 64), (32, 32, 64), (16, 2, 128), (6, 3, 48)])
+@pytest.mark.parametrize("members", [2, 9, 70])
+def test_a_query_that_is_no_number_gives_none(dtype, heads, kv_heads, dim, members):
+    """All scores of one (row, head) are NaN: its output is, and no other's."""
+    from nnis_b200.engine.workspace import Workspace
+    tables, seqs, positions, pages = build(11, [5], members, 1, [1, 64, 100])
+    g = torch.Generator().manual_seed(3)
+    k = torch.randn((pages, kv_heads, 64, dim), generator=g).to(dtype).to(DEV)
+    v = torch.randn((pages, kv_heads, 64, dim), generator=g).to(dtype).to(DEV)
+    q = torch.randn((len(seqs), heads * dim), generator=g).to(dtype).to(DEV)
+    cols = max(map(len, tables))
+    table = torch.tensor([t + [-1] * (cols - len(t)) for t in tables], dtype=torch.int32, device=DEV)
+    pos = torch.tensor(positions, dtype=torch.int32, device=DEV)
+    plan = ops().attention_shared_plan(tables, seqs, positions, heads, kv_heads, dim, dtype, DEV)
+    outs = []
+    for spoilt in (False, True):
+        if spoilt:
+            q[1, 2 * dim + 1] = math.nan
+        out = torch.empty_like(q)
+        ops().attention_shared(q, heads * dim, k, v, pos, table, plan, out, heads, kv_heads, dim, 0.1, Workspace(torch.device(DEV)))
+        outs.append(out.view(-1, heads, dim).double())
+    clean, got = outs
+    assert torch.isnan(got[1, 2]).all()
+    got[1, 2] = clean[1, 2]
+    # (either is off by at most 1.5 * 2^-8 of the largest value, see ``check``)
+    assert ((got - clean).abs() <= 3 * 2 ** -8 * v.abs().max().item()).all()
+
+
 def test_pages_beyond_32_bit_offsets():
     """A store of more than 2^32 bytes and 2^31 values: pages at its end."""
     from nnis_b200.engine.workspace import Workspace
