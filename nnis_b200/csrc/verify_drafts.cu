@@ -25,6 +25,7 @@
 
 #include "async_copy.cuh"
 #include "common.cuh"
+#include "fma_pairs.cuh"
 
 namespace nnis {
 
@@ -54,24 +55,101 @@ __device__ __forceinline__ float weight32(float x) {
     return y;
 }
 
-// (m, s, best) of two sets of ids
-__device__ __forceinline__ RowSum joined(const RowSum& a, const RowSum& b, float c) {
-    RowSum r;
-    r.max = fmaxf(a.max, b.max);
-    r.best = a.max > b.max || (a.max == b.max && a.best < b.best) ? a.best : b.best;
-    const float base = r.max == -INFINITY ? 0.f : r.max;
-    r.sum = a.sum * weight32((a.max - base) * c) + b.sum * weight32((b.max - base) * c);
-    return r;
+// Of the lanes of groups of LANES: the sums together, in every lane, and with BEST the id of the maximum, the lower among equals.
+template <int LANES, bool BEST>
+__device__ __forceinline__ RowSum joined(RowSum x, float c) {
+    float max = x.max;
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) max = fmaxf(max, __shfl_xor_sync(0xffffffffu, max, o));
+    x.sum *= weight32((x.max - (max == -INFINITY ? 0.f : max)) * c);
+    if (x.max != max) x.best = 0x7fffffff;
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) {
+        x.sum += __shfl_xor_sync(0xffffffffu, x.sum, o);
+        if (BEST) x.best = min(x.best, __shfl_xor_sync(0xffffffffu, x.best, o));
+    }
+    x.max = max;
+    return x;
+}
+
+__device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigned long long b) {
+    unsigned long long d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+// A thread's share of a row's ids from `begin` on, below `end`.  BEST: with the id of the maximum (greedy rows; else it is any).
+template <bool BEST>
+__device__ __forceinline__ RowSum thread_sum(const float* __restrict__ row, int begin, int end, float c) {
+    // (32 bits: the maximum is taken off first, exactly, so that a large one costs no digits)
+    RowSum mine = {-INFINITY, 0.f, 0x7fffffff};
+    constexpr int kAhead = 4;  // quads a thread has on their way
+    // quads from the row's first 16-byte boundary on; the first threads take what lies before it and what is left behind them
+    const int head = min(end - begin, (int)((4 - (((uintptr_t)(row + begin) >> 2) & 3)) & 3)), quads = (end - begin - head) / 4;
+    const float4* row4 = reinterpret_cast<const float4*>(row + begin + head);
+    for (int at = threadIdx.x; at < quads; at += kAhead * kVerifyThreads) {
+        float4 x[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const int w = at + i * kVerifyThreads;
+            x[i] = w < quads ? __ldcs(row4 + w) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        }
+        float m = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) m = max3(max3(m, x[i].x, x[i].y), x[i].z, x[i].w);
+        if (m > mine.max) {
+            mine.sum *= weight32((mine.max - m) * c);
+            mine.max = m;
+            if (BEST) {
+#pragma unroll
+                for (int i = kAhead - 1; i >= 0; --i) {
+                    const int id = begin + head + 4 * (at + i * kVerifyThreads);
+                    mine.best = x[i].x == m ? id : x[i].y == m ? id + 1 : x[i].z == m ? id + 2 : x[i].w == m ? id + 3 : mine.best;
+                }
+            }
+        }
+        const unsigned long long off = both(mine.max == -INFINITY ? 0.f : -mine.max), cc = both(c);
+        unsigned long long sum[2] = {0ull, 0ull};
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const float2 u = halves(mul2(add2(h ? pair_of(x[i].z, x[i].w) : pair_of(x[i].x, x[i].y), off), cc));
+                sum[h] = add2(sum[h], pair_of(weight32(u.x), weight32(u.y)));  // (a NaN or +infinity makes the sum one)
+            }
+        const float2 s = halves(add2(sum[0], sum[1]));
+        mine.sum += s.x + s.y;
+    }
+    const int tail = begin + head + 4 * quads;
+    if (head > 0 || tail < end) {  // at most six, a thread each
+        const int t = threadIdx.x, id = t < head ? begin + t : tail + t - head;
+        if (id < end && (t < head || t < head + 3)) {
+            const float x = row[id];
+            if (x > mine.max) {
+                mine.sum *= weight32((mine.max - x) * c);
+                mine.max = x;
+                mine.best = id;
+            } else if (BEST && x == mine.max) {
+                mine.best = min(mine.best, id);
+            }
+            mine.sum += weight32((x - (mine.max == -INFINITY ? 0.f : mine.max)) * c);
+        }
+    }
+    return mine;
 }
 
 __global__ void __launch_bounds__(kVerifyThreads)
 verify_rows_kernel(const float* __restrict__ logits, const float* __restrict__ draft_logits, const int* __restrict__ first_row,
-                   const float* __restrict__ temperature, int n_seqs, int rows, int draft_rows, int vocab, int per,
-                   RowSum* __restrict__ parts) {
+                   const float* __restrict__ temperature, int n_seqs, int rows, int vocab, int per, RowSum* __restrict__ parts) {
     pdl_wait();
     pdl_launch_dependents();
     __shared__ RowSum warp_sum_s[kVerifyThreads / 32];
-    const int r = blockIdx.y;
+    const int r = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const bool of_draft = r >= rows;
     // the row's sequence: the last one that begins at or before it
     int lo = 0, hi = n_seqs - 1;
@@ -84,70 +162,14 @@ verify_rows_kernel(const float* __restrict__ logits, const float* __restrict__ d
     const float c = scale_of(t);
     const float* row = of_draft ? draft_logits + (size_t)(r - rows) * vocab : logits + (size_t)r * vocab;
     const int begin = min(vocab, (int)blockIdx.x * per), end = min(vocab, begin + per);
-    // (32 bits: the maximum is taken off first, exactly, so that a large one costs no digits)
-    RowSum mine = {-INFINITY, 0.f, 0x7fffffff};
-    constexpr int kAhead = 4;  // quads a thread has on their way
-    auto take = [&](const float (&x)[4 * kAhead], int at, int step) {  // x[i] has the id at + step * (i / 4) + i % 4
-        float m = x[0];
-#pragma unroll
-        for (int i = 1; i < 4 * kAhead; ++i) m = fmaxf(m, x[i]);
-        if (m > mine.max) {
-            mine.sum *= weight32((mine.max - m) * c);
-            mine.max = m;
-#pragma unroll
-            for (int i = 4 * kAhead - 1; i >= 0; --i)
-                if (x[i] == m) mine.best = at + step * (i / 4) + i % 4;
-        }
-        const float base = mine.max == -INFINITY ? 0.f : mine.max;
-        float s[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int i = 0; i < 4 * kAhead; ++i) s[i & 3] += weight32((x[i] - base) * c);  // (a NaN or +infinity makes the sum one)
-        mine.sum += (s[0] + s[1]) + (s[2] + s[3]);
-    };
-    // quads from the row's first 16-byte boundary on; thread 0 takes what lies before it and what is left behind them
-    const int head = min(end - begin, (int)((4 - (((uintptr_t)(row + begin) >> 2) & 3)) & 3)), quads = (end - begin - head) / 4;
-    const float4* row4 = reinterpret_cast<const float4*>(row + begin + head);
-    for (int at = threadIdx.x; at < quads; at += kAhead * kVerifyThreads) {
-        float x[4 * kAhead];
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-            const int w = at + i * kVerifyThreads;
-            const float4 v = w < quads ? __ldcs(row4 + w) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-            x[4 * i] = v.x;
-            x[4 * i + 1] = v.y;
-            x[4 * i + 2] = v.z;
-            x[4 * i + 3] = v.w;
-        }
-        take(x, begin + head + 4 * at, 4 * kVerifyThreads);
-    }
-    if (threadIdx.x == 0) {
-        float x[4 * kAhead];
-        const int tail = begin + head + 4 * quads;
-#pragma unroll
-        for (int i = 0; i < 4 * kAhead; ++i) x[i] = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < 3; ++i) {
-            if (i < head) x[i] = row[begin + i];
-            if (tail + i < end) x[4 + i] = row[tail + i];
-        }
-        RowSum kept = mine;
-        mine = {-INFINITY, 0.f, 0x7fffffff};
-        take(x, begin, tail - begin);
-        mine = joined(kept, mine, c);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        RowSum other;
-        other.max = __shfl_xor_sync(0xffffffffu, mine.max, o);
-        other.sum = __shfl_xor_sync(0xffffffffu, mine.sum, o);
-        other.best = __shfl_xor_sync(0xffffffffu, mine.best, o);
-        mine = joined(mine, other, c);
-    }
-    if ((threadIdx.x & 31) == 0) warp_sum_s[threadIdx.x >> 5] = mine;
+    const bool greedy = !(t > 0.f);
+    RowSum mine = greedy ? joined<32, true>(thread_sum<true>(row, begin, end, c), c)
+                         : joined<32, false>(thread_sum<false>(row, begin, end, c), c);
+    if (lane == 0) warp_sum_s[warp] = mine;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < kVerifyThreads / 32; ++w) mine = joined(mine, warp_sum_s[w], c);
-        parts[(size_t)r * gridDim.x + blockIdx.x] = mine;
+    if (warp == 0) {
+        mine = joined<kVerifyThreads / 32, true>(warp_sum_s[lane % (kVerifyThreads / 32)], c);
+        if (lane == 0) parts[(size_t)r * gridDim.x + blockIdx.x] = mine;
     }
 }
 
@@ -155,16 +177,9 @@ verify_rows_kernel(const float* __restrict__ logits, const float* __restrict__ d
 __device__ __forceinline__ RowSum row_sum(const RowSum* __restrict__ parts, size_t row, int n_parts, float c) {
     const int lane = threadIdx.x & 31;
     RowSum mine = {-INFINITY, 0.f, 0x7fffffff};
-    const int part = n_parts <= 8 ? lane & 7 : lane;  // (few parts: each eighth of the warp joins them all)
+    const int part = n_parts <= 8 ? lane & 7 : lane;  // (few parts: each quarter of the warp joins them all)
     if (part < n_parts) mine = parts[row * n_parts + part];
-    for (int o = n_parts <= 8 ? 4 : 16; o > 0; o >>= 1) {
-        RowSum other;
-        other.max = __shfl_xor_sync(0xffffffffu, mine.max, o);
-        other.sum = __shfl_xor_sync(0xffffffffu, mine.sum, o);
-        other.best = __shfl_xor_sync(0xffffffffu, mine.best, o);
-        mine = joined(mine, other, c);
-    }
-    return mine;
+    return n_parts <= 8 ? joined<8, true>(mine, c) : joined<32, true>(mine, c);
 }
 
 __device__ __forceinline__ double warp_sum64(double v) {
@@ -215,8 +230,9 @@ struct PickShared {
     double table[64];                // 2^(j / 64)
     double warp[4][kPickWarps];
     double cta[2][4][kPickCtas];     // every CTA's sums, written by them: [turn][which][rank]
+    double chunk[kPickWarps];        // the warps' shares of the ids among which the pick lies
     float row_max[2][kPickWarps], row_sum[2][kPickWarps];  // of the row at which a warp stopped
-    int stop;
+    int stop, found, last;
 };
 
 // Sums over the whole cluster of four values a thread; every thread gets all.  Each CTA tells all others its sums, in
@@ -255,34 +271,53 @@ verify_pick_kernel(const float* __restrict__ logits, const float* __restrict__ d
     const int b = blockIdx.y, rank = (int)cluster.block_rank(), ctas = (int)cluster.num_blocks();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid < 64) s.table[tid] = exp2((double)tid * (1.0 / 64.0));
-    if (tid == 0) s.stop = 0x7fffffff;
+    if (tid == 0) {
+        s.stop = s.found = 0x7fffffff;
+        s.last = -1;
+    }
+    // (What the call was given is older than the first launch, which has waited for it: it is read under that launch's end.)
     const int row0 = first_row[b], draft0 = row0 - b, count = first_row[b + 1] - row0 - 1;
     const float t = temperature[b];
     const bool greedy = !(t > 0.f);
     const float c = scale_of(t);
     const double inv_t = greedy ? 1.0 : 1.0 / (double)t;
+    const bool good = row0 >= b && count >= 0 && row0 + count < rows && draft0 + count <= rows - (int)gridDim.y;
+    // A warp's draft: its logits in the two rows.
+    struct Draft {
+        int id;
+        float z, y;
+        double draw;
+    };
+    auto draft_of = [&](int i) {
+        Draft x = {-1, 0.f, 0.f, 0.0};
+        if (i < count) {
+            x.id = drafts[draft0 + i];
+            x.draw = accept_draws[draft0 + i];
+            if (x.id >= 0 && x.id < vocab && !greedy) {
+                x.z = logits[(size_t)(row0 + i) * vocab + x.id];
+                if (draft_logits) x.y = draft_logits[(size_t)(draft0 + i) * vocab + x.id];
+            }
+        }
+        return x;
+    };
+    Draft mine = draft_of(good ? warp : count);
+    cluster.sync();  // (all of the cluster run: their shared memory may be written)
     pdl_wait();
     pdl_launch_dependents();
-    // (offsets that no packed rows have: the whole cluster leaves)
-    if (row0 < b || count < 0 || row0 + count >= rows || draft0 + count > rows - (int)gridDim.y) {
+    if (!good) {  // (offsets that no packed rows have: the whole cluster leaves)
         if (rank == 0 && tid == 0) {
             accepted[b] = 0;
             picked[b] = -1;
         }
         return;
     }
-    cluster.sync();  // (all of the cluster run: their shared memory may be written)
 
     // The drafts, a warp each: where the first one lies that is not kept for sure, and why (every CTA of the cluster for
     // itself, all alike).
     enum { kKept, kRefused, kNothing, kNear };
-    auto decide = [&](int i) -> int {
+    auto decide = [&](int i, const Draft& x) -> int {
         const bool drafted = i < count, other = drafted && draft_logits && !greedy;
-        const int d = drafted ? drafts[draft0 + i] : -1;
-        const double u = drafted ? accept_draws[draft0 + i] : 0.0;
-        const bool known = d >= 0 && d < vocab;
-        const float zd = known ? logits[(size_t)(row0 + i) * vocab + d] : 0.f;
-        const float yd = known && other ? draft_logits[(size_t)(draft0 + i) * vocab + d] : 0.f;
+        const bool known = x.id >= 0 && x.id < vocab;
         const RowSum zs = row_sum(parts, (size_t)(row0 + i), n_parts, c);
         RowSum ys = {0.f, 1.f, 0};
         if (other) ys = row_sum(parts, (size_t)(rows + draft0 + i), n_parts, c);
@@ -294,11 +329,11 @@ verify_pick_kernel(const float* __restrict__ logits, const float* __restrict__ d
         }
         if (!(zs.sum >= 0.f) || zs.max == -INFINITY || zs.max == INFINITY) return kNothing;
         if (!drafted) return kRefused;
-        if (greedy) return d == zs.best ? kKept : kRefused;
+        if (greedy) return x.id == zs.best ? kKept : kRefused;
         if (!(ys.sum >= 0.f) || ys.max == -INFINITY || ys.max == INFINITY) return kNothing;
         if (!known) return kRefused;
-        const double eq = other ? weight64(s.table, yd, scale64(ys.max, inv_t, t)) : 1.0;
-        const double left = u * eq * (double)zs.sum, right = weight64(s.table, zd, scale64(zs.max, inv_t, t)) * (double)ys.sum;
+        const double eq = other ? weight64(s.table, x.y, scale64(ys.max, inv_t, t)) : 1.0;
+        const double left = x.draw * eq * (double)zs.sum, right = weight64(s.table, x.z, scale64(zs.max, inv_t, t)) * (double)ys.sum;
         if (fabs(left - right) <= 1e-4 * right || t < 1e-29f) return kNear;
         return left < right ? kKept : kRefused;
     };
@@ -309,20 +344,9 @@ verify_pick_kernel(const float* __restrict__ logits, const float* __restrict__ d
     const float *z = nullptr, *y = nullptr;
     Scale zc = {}, yc = {};
     float line = 0.f;  // p is larger than q where z - y lies above it (by the sums in 32 bits)
-    auto weights = [&](int first, double (&ez)[kAhead], double (&ey)[kAhead], unsigned& more) {  // of ids first, first + 32, ...
-        float xz[kAhead], xy[kAhead];
+    auto ask = [&](const float* row, int first, float (&x)[kAhead]) {  // logits of ids first, first + 32, ...
 #pragma unroll
-        for (int k = 0; k < kAhead; ++k) {
-            const int i = first + 32 * k;
-            xz[k] = i < end ? z[i] : -INFINITY;
-            xy[k] = y && i < end ? y[i] : -INFINITY;
-        }
-#pragma unroll
-        for (int k = 0; k < kAhead; ++k) {
-            ez[k] = weight64(s.table, xz[k], zc);
-            ey[k] = y ? weight64(s.table, xy[k], yc) : 0.0;
-            more |= xz[k] - xy[k] > line ? 1u << k : 0u;
-        }
+        for (int k = 0; k < kAhead; ++k) x[k] = first + 32 * k < end ? row[first + 32 * k] : -INFINITY;
     };
     // The sums of row i, at which warp `stopped` stopped, in 64 bits: of p's weights, of q's, and of both over the ids where p is
     // the larger, by the sums in 32 bits.  The last two give what q leaves of p, sum p[more] / sum p - sum q[more] / sum q,
@@ -337,17 +361,38 @@ verify_pick_kernel(const float* __restrict__ logits, const float* __restrict__ d
         line = y ? s.row_max[0][stopped] - s.row_max[1][stopped] + t * logf(s.row_sum[0][stopped] / s.row_sum[1][stopped]) : -INFINITY;
 #pragma unroll
         for (int n = 0; n < 4; ++n) sums[n] = 0.0;
-        for (int i0 = begin + lane; i0 < end; i0 += 32 * kAhead) {
-            double ez[kAhead], ey[kAhead];
-            unsigned more = 0;
-            weights(i0, ez, ey, more);
+        float xz[kAhead], xy[kAhead];
+        if (y) {
+            ask(z, begin + lane, xz);
+            ask(y, begin + lane, xy);
+            for (int i0 = begin + lane; i0 < end; i0 += 32 * kAhead) {
+                float next_z[kAhead], next_y[kAhead];  // (on their way while these are worked)
+                ask(z, i0 + 32 * kAhead, next_z);
+                ask(y, i0 + 32 * kAhead, next_y);
 #pragma unroll
-            for (int k = 0; k < kAhead; ++k) {
-                sums[0] += ez[k];
-                sums[1] += ey[k];
-                if ((more >> k & 1u) && i0 + 32 * k != without) {
-                    sums[2] += ez[k];
-                    sums[3] += ey[k];
+                for (int k = 0; k < kAhead; ++k) {
+                    const double ez = weight64(s.table, xz[k], zc), ey = weight64(s.table, xy[k], yc);
+                    sums[0] += ez;
+                    sums[1] += ey;
+                    if (xz[k] - xy[k] > line) {
+                        sums[2] += ez;
+                        sums[3] += ey;
+                    }
+                    xz[k] = next_z[k];
+                    xy[k] = next_y[k];
+                }
+            }
+        } else {
+            ask(z, begin + lane, xz);
+            for (int i0 = begin + lane; i0 < end; i0 += 32 * kAhead) {
+                float next_z[kAhead];
+                ask(z, i0 + 32 * kAhead, next_z);
+#pragma unroll
+                for (int k = 0; k < kAhead; ++k) {
+                    const double ez = weight64(s.table, xz[k], zc);
+                    sums[0] += ez;
+                    if (i0 + 32 * k != without) sums[2] += ez;
+                    xz[k] = next_z[k];
                 }
             }
         }
@@ -359,11 +404,12 @@ verify_pick_kernel(const float* __restrict__ logits, const float* __restrict__ d
     int a = 0, why = kNear;
     for (int from = 0;;) {
         for (int i = from + warp; i <= count; i += kPickWarps) {
-            const int how = decide(i);
+            const int how = decide(i, mine);
             if (how != kKept) {
                 if (lane == 0) atomicMin(&s.stop, i * 4 + how);
                 break;
             }
+            mine = draft_of(i + kPickWarps);
         }
         __syncthreads();
         a = s.stop >> 2;
@@ -377,6 +423,7 @@ verify_pick_kernel(const float* __restrict__ logits, const float* __restrict__ d
         if (tid == 0) s.stop = 0x7fffffff;  // (everybody has read it: they have met)
         __syncthreads();
         from = a + 1;
+        mine = draft_of(from + warp);
     }
     if (why == kNothing || greedy) {
         if (rank == 0 && warp == 0) {
@@ -392,15 +439,9 @@ verify_pick_kernel(const float* __restrict__ logits, const float* __restrict__ d
     const int d = a < count ? drafts[draft0 + a] : -1;
     const double ip = 1.0 / sums[0], iq = y ? 1.0 / sums[1] : 0.0;
     bool plain = a >= count;
-    auto masses = [&](int first, double (&m)[kAhead]) {
-        double ey[kAhead];
-        unsigned more = 0;
-        weights(first, m, ey, more);
-#pragma unroll
-        for (int k = 0; k < kAhead; ++k) {
-            const double p = __dmul_rn(m[k], ip);  // (rounded like q: equal ones leave nothing)
-            m[k] = plain ? p : y ? fmax(p - __dmul_rn(ey[k], iq), 0.0) : first + 32 * k == d ? 0.0 : p;
-        }
+    auto mass = [&](int i, float xz, float xy) {  // of id i
+        const double p = __dmul_rn(weight64(s.table, xz, zc), ip);  // (rounded like q: equal ones leave nothing)
+        return plain ? p : y ? fmax(p - __dmul_rn(weight64(s.table, xy, yc), iq), 0.0) : i == d ? 0.0 : p;
     };
     // Masses of warps and CTAs, from their sums over the ids where p is the larger.  Where q leaves little (or, by
     // rounding, nothing) of p the line between those ids is too coarse: the masses are summed id by id.
@@ -410,12 +451,7 @@ verify_pick_kernel(const float* __restrict__ logits, const float* __restrict__ d
         mq = 0.0;
         for (;;) {
             sums[0] = sums[1] = sums[2] = sums[3] = 0.0;
-            for (int i0 = begin + lane; i0 < end; i0 += 32 * kAhead) {
-                double m[kAhead];
-                masses(i0, m);
-#pragma unroll
-                for (int k = 0; k < kAhead; ++k) sums[2] += m[k];
-            }
+            for (int i = begin + lane; i < end; i += 32) sums[2] += mass(i, z[i], y ? y[i] : 0.f);
             cluster_sums(cluster, s, turn, sums);
             turn ^= 1;
             total = sums[2];
@@ -426,48 +462,49 @@ verify_pick_kernel(const float* __restrict__ logits, const float* __restrict__ d
     const double target = fmin(fmax(pick_draws[b], 0.0), 1.0) * total;  // (a draw of another range, or no number, is its next end)
     // Where in the row the target lies: the CTAs' masses, lane by lane, then the warps'.  A draw at the very end of the
     // sums belongs to the last id with any weight.
-    auto place = [&](double mass, double from, int mine, double& ahead) {
+    auto place = [&](double mass, double& ahead) {  // of sixteen; `ahead`: what lies before the first, then before the one
         const double upto = half_scan64(mass);
         const unsigned some = __ballot_sync(0xffffffffu, mass > 0.0) & 0xffffu;
-        const int last = some ? 31 - __clz(some) : 0;
-        const double own = __shfl_sync(0xffffffffu, mass, mine), end_of = from + __shfl_sync(0xffffffffu, upto, mine);
-        const double begin_of = from + (mine ? __shfl_sync(0xffffffffu, upto, mine - 1) : 0.0);
-        ahead = begin_of;
-        return own > 0.0 && target >= begin_of && (target < end_of || mine == last);
+        const unsigned over = __ballot_sync(0xffffffffu, mass > 0.0 && target < ahead + upto) & 0xffffu;
+        const int one = over ? __ffs(over) - 1 : some ? 31 - __clz(some) : 0;
+        const double before = __shfl_sync(0xffffffffu, upto, max(one - 1, 0));
+        if (one) ahead += before;
+        return one;
     };
     if (rank == 0 && tid == 0) accepted[b] = a;
     const int at = lane & 15;
-    double before, ahead;
-    if (!place(at < ctas ? fmax(mp * s.cta[turn ^ 1][2][at] - mq * s.cta[turn ^ 1][3][at], 0.0) : 0.0, 0.0, rank, before)) return;
-    if (!place(fmax(mp * s.warp[2][at] - mq * s.warp[3][at], 0.0), before, warp, ahead)) return;
-    int found = -1, last_id = -1;
-    for (int i0 = begin; found < 0; i0 += 32 * kAhead) {
-        if (i0 >= end) {
-            if (last_id >= 0 || plain) break;
+    double ahead = 0.0;
+    if (place(at < ctas ? fmax(mp * s.cta[turn ^ 1][2][at] - mq * s.cta[turn ^ 1][3][at], 0.0) : 0.0, ahead) != rank) return;
+    // The CTA goes through that warp's ids together.
+    const int of = place(fmax(mp * s.warp[2][at] - mq * s.warp[3][at], 0.0), ahead);
+    const int first = min(vocab, (rank * kPickWarps + of) * per_warp), behind = min(vocab, first + per_warp);
+    for (int i0 = first;; i0 += kPickThreads) {
+        if (i0 >= behind) {
+            if (s.last >= 0 || plain) break;
             plain = true;  // (only ids of equal p and q are here, on the line by a rounding: one of them by p)
-            i0 = begin;
+            i0 = first;
         }
-        double m[kAhead];
-        masses(i0 + lane, m);
+        const int i = i0 + tid;
+        const double m = i < behind ? mass(i, z[i], y ? y[i] : 0.f) : 0.0;
+        double run = m;
 #pragma unroll
-        for (int k = 0; k < kAhead; ++k) {
-            if (found >= 0) break;
-            double run = m[k];
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const double up = __shfl_up_sync(0xffffffffu, run, o);
-                if (lane >= o) run += up;
-            }
-            const unsigned over = __ballot_sync(0xffffffffu, m[k] > 0.0 && ahead + run > target);
-            const unsigned some = __ballot_sync(0xffffffffu, m[k] > 0.0);
-            if (over) found = i0 + 32 * k + __ffs(over) - 1;
-            if (some) last_id = i0 + 32 * k + 31 - __clz(some);
-            ahead += __shfl_sync(0xffffffffu, run, 31);
+        for (int o = 1; o < 32; o <<= 1) {
+            const double up = __shfl_up_sync(0xffffffffu, run, o);
+            if (lane >= o) run += up;
         }
+        if (lane == 31) s.chunk[warp] = run;
+        __syncthreads();
+        const double upto = half_scan64(s.chunk[at]), before = __shfl_sync(0xffffffffu, upto, max(warp - 1, 0));
+        if (m > 0.0) {  // (written between the two meetings, read between the second and the next turn's first)
+            atomicMax(&s.last, i);
+            if (ahead + ((warp ? before : 0.0) + run) > target) atomicMin(&s.found, i);
+        }
+        ahead += __shfl_sync(0xffffffffu, upto, 15);
+        __syncthreads();
+        if (s.found < vocab) break;
     }
-    if (lane == 0) picked[b] = found >= 0 ? found : last_id;
+    if (tid == 0) picked[b] = s.found < vocab ? s.found : s.last;
 }
-
 // CTAs a row: shares of 8,192 logits, of 4,096 where all rows together are no more than four CTAs an SM then (nine rows of 49,152:
 // 4.4 -> 3.6 us; 960 rows 37.5 us with 8,192 and more, 49 with 4,096).
 static int verify_parts(long long rows, int vocab) {
@@ -499,7 +536,7 @@ NNIS_API int nnis_verify_drafts(const float* logits, const float* draft_logits, 
     if ((uintptr_t)scratch % 16) return NNIS_ERR_ALIGNMENT;
     const int n_parts = verify_parts(rows + draft_rows, vocab), per = (vocab + n_parts - 1) / n_parts;
     cudaError_t e = launch_dependent(verify_rows_kernel, dim3(n_parts, all_rows), kVerifyThreads, 0, stream, logits, draft_logits,
-                                     first_row, temperature, n_seqs, rows, draft_rows, vocab, per, static_cast<RowSum*>(scratch));
+                                     first_row, temperature, n_seqs, rows, vocab, per, static_cast<RowSum*>(scratch));
     if (e != cudaSuccess) return (int)e;
     // As many CTAs a sequence as the device holds at once (two an SM) for all of them, sixteen at most, four at least: a row of
     // 49,152 is walked in 9.8 us by sixteen, 15.4 by eight (24 sequences), 32 by four (64 sequences, which eight would
