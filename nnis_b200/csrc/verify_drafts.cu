@@ -173,24 +173,17 @@ verify_rows_kernel(const float* __restrict__ logits, const float* __restrict__ d
     }
 }
 
-// A row's parts joined by a warp (at most 32 of them); every lane gets the result.
-__device__ __forceinline__ RowSum row_sum(const RowSum* __restrict__ parts, size_t row, int n_parts, float c) {
-    const int lane = threadIdx.x & 31;
-    RowSum mine = {-INFINITY, 0.f, 0x7fffffff};
-    const int part = n_parts <= 8 ? lane & 7 : lane;  // (few parts: each quarter of the warp joins them all)
-    if (part < n_parts) mine = parts[row * n_parts + part];
-    return n_parts <= 8 ? joined<8, true>(mine, c) : joined<32, true>(mine, c);
+// A row's parts, a lane each (at most 32; up to eight are asked for by each quarter of the warp), and the row of them, in every lane.
+__device__ __forceinline__ RowSum part_of(const RowSum* __restrict__ parts, size_t row, int n_parts) {
+    const int part = n_parts <= 8 ? threadIdx.x & 7 : threadIdx.x & 31;
+    return part < n_parts ? parts[row * n_parts + part] : RowSum{-INFINITY, 0.f, 0x7fffffff};
+}
+__device__ __forceinline__ RowSum row_of(const RowSum& part, int n_parts, float c) {
+    return n_parts <= 8 ? joined<8, true>(part, c) : joined<32, true>(part, c);
 }
 
-__device__ __forceinline__ double warp_sum64(double v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
-}
-// The same over either half of a warp: sixteen values, in every lane if both halves hold them.
-__device__ __forceinline__ double half_sum64(double v) {
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+__device__ __forceinline__ double sum64(double v, int from, int to) {  // over lanes that differ in these bits
+    for (int o = from; o >= to; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
 // Sum of the lanes up to this one, of sixteen.
@@ -236,28 +229,26 @@ struct PickShared {
 };
 
 // Sums over the whole cluster of four values a thread; every thread gets all.  Each CTA tells all others its sums, in
-// one of two places by turns: a place is written again only when everybody has met once more.
+// one of two places by turns: a place is written again only when everybody has met once more.  A quarter of a warp has one of
+// the four values from the start (shuffles are what sums of a warp's doubles cost).
 __device__ __forceinline__ void cluster_sums(cg::cluster_group cluster, PickShared& s, int turn, double (&v)[4]) {
-    const int lane = threadIdx.x & 31;
-#pragma unroll
-    for (int n = 0; n < 4; ++n) {
-        v[n] = warp_sum64(v[n]);
-        if (lane == 0) s.warp[n][threadIdx.x >> 5] = v[n];
-    }
+    const int lane = threadIdx.x & 31, n = lane >> 3, at = lane & 7;
+    const bool high = lane & 16, odd = lane & 8;
+    const double a = high ? v[2] : v[0], b = high ? v[3] : v[1];
+    const double x = a + __shfl_xor_sync(0xffffffffu, high ? v[0] : v[2], 16), y = b + __shfl_xor_sync(0xffffffffu, high ? v[1] : v[3], 16);
+    double one = (odd ? y : x) + __shfl_xor_sync(0xffffffffu, odd ? x : y, 8);
+    one = sum64(one, 4, 1);
+    if (at == 0) s.warp[n][threadIdx.x >> 5] = one;
     __syncthreads();
-    const int ctas = (int)cluster.num_blocks(), at = lane & 15;  // (chains of 64-bit sums are slow: trees of sixteen)
+    const int ctas = (int)cluster.num_blocks();
     if (threadIdx.x < 32) {
-#pragma unroll
-        for (int n = 0; n < 4; ++n) v[n] = half_sum64(s.warp[n][at]);
-        if (lane < ctas) {
-            PickShared* other = cluster.map_shared_rank(&s, lane);
-#pragma unroll
-            for (int n = 0; n < 4; ++n) other->cta[turn][n][cluster.block_rank()] = v[n];
-        }
+        one = sum64(s.warp[n][at] + s.warp[n][at + 8], 4, 1);
+        for (int r = at; r < ctas; r += 8) cluster.map_shared_rank(&s, r)->cta[turn][n][cluster.block_rank()] = one;
     }
     cluster.sync();
+    one = sum64((at < ctas ? s.cta[turn][n][at] : 0.0) + (at + 8 < ctas ? s.cta[turn][n][at + 8] : 0.0), 4, 1);
 #pragma unroll
-    for (int n = 0; n < 4; ++n) v[n] = half_sum64(at < ctas ? s.cta[turn][n][at] : 0.0);
+    for (int k = 0; k < 4; ++k) v[k] = __shfl_sync(0xffffffffu, one, 8 * k);
 }
 static_assert(kPickWarps == 16 && kPickCtas == 16, "sums of sixteen");
 
@@ -318,9 +309,10 @@ verify_pick_kernel(const float* __restrict__ logits, const float* __restrict__ d
     auto decide = [&](int i, const Draft& x) -> int {
         const bool drafted = i < count, other = drafted && draft_logits && !greedy;
         const bool known = x.id >= 0 && x.id < vocab;
-        const RowSum zs = row_sum(parts, (size_t)(row0 + i), n_parts, c);
-        RowSum ys = {0.f, 1.f, 0};
-        if (other) ys = row_sum(parts, (size_t)(rows + draft0 + i), n_parts, c);
+        RowSum zs = part_of(parts, (size_t)(row0 + i), n_parts), ys = {0.f, 1.f, 0};
+        if (other) ys = part_of(parts, (size_t)(rows + draft0 + i), n_parts);
+        zs = row_of(zs, n_parts, c);
+        if (other) ys = row_of(ys, n_parts, c);
         if (lane == 0) {
             s.row_max[0][warp] = zs.max;
             s.row_max[1][warp] = ys.max;
@@ -427,7 +419,7 @@ verify_pick_kernel(const float* __restrict__ logits, const float* __restrict__ d
     }
     if (why == kNothing || greedy) {
         if (rank == 0 && warp == 0) {
-            const int best = row_sum(parts, (size_t)(row0 + a), n_parts, c).best;
+            const int best = row_of(part_of(parts, (size_t)(row0 + a), n_parts), n_parts, c).best;
             if (lane == 0) {
                 accepted[b] = a;
                 picked[b] = why == kNothing ? -1 : best;
