@@ -18,8 +18,9 @@
 // sums p, q and both over the ids where p is the larger, so what q leaves of p needs no second one; only where it leaves next to
 // nothing are the masses summed id by id.
 //
-// The first launch is bound by bytes: 960 rows of 49,152 (189 MB) 37.5 us, 5.0 TB/s; nine rows 3.7.  The second by 64-bit
-// arithmetic (an SM has few such units) and, with few sequences, by its chain of steps: draft, row, cluster, pick.
+// The first launch is bound by bytes: 960 rows of 49,152 (189 MB) 33 us, 5.7 TB/s; nine rows 3.7.  The second by the instructions of
+// its 64-bit weights (45 a pair of logits, a third of them of 64 bits) and, with few sequences, by its chain of steps: draft,
+// row, cluster, pick.  Both in turns, the next sequences' rows beside the last ones' picks, were slower (62 us for 58).
 #include <cooperative_groups.h>
 #include <float.h>
 
@@ -196,31 +197,49 @@ __device__ __forceinline__ double half_scan64(double v) {
     return v;
 }
 
-// exp((x - max) / T) in 64 bits for x <= max: with u = 64 (x - max) / (T ln 2) and k the whole number next to it, 2^(k / 64) from a
-// table times the series of 2^((u - k) / 64) to the fourth power (what is left out is 4e-14), after P. T. P. Tang's
-// table-driven method (ACM TOMS 15, 1989).  Twenty instructions where the library's exp, good to the last place, takes twice as many and
-// the sums of a row are bound by them.
+// exp((x - max) / T) in 64 bits for x <= max: with u = 64 (x - max) / (T ln 2) and k a whole number next to it, 2^(k / 64) from a
+// table times the series of 2^((u - k) / 64) to the fourth power (what is left out is 5e-14), after P. T. P. Tang's
+// table-driven method (ACM TOMS 15, 1989).  k is found in 32 bits (off by 0.01 at most from rounding u), so that seven
+// instructions are of 64 bits, which the device has half as many units for; the sums of a row are bound by them.
 struct Scale {
-    double per;    // 64 / (T ln 2)
-    double max;    // the row's maximum
-    float lowest;  // below it (700 T under the maximum, and at -infinity) a weight is zero
+    double per;          // 64 / (T ln 2)
+    double max;          // the row's maximum
+    float per32, max32;  // the same
+    float lowest;        // below it (700 T under the maximum, and at -infinity) a weight is zero
 };
 __device__ __forceinline__ Scale scale64(float max, double inv_t, float t) {
-    return {inv_t * 92.33248261689366, (double)max, fmaxf(-FLT_MAX, max - 700.f * t)};
+    const double per = inv_t * 92.33248261689366;
+    // (a temperature below 1e-35 leaves the maximum alone: 64 / T is beyond 32 bits)
+    return {per, (double)max, fminf((float)per, FLT_MAX), max, t < 1e-35f ? max : fmaxf(-FLT_MAX, max - 700.f * t)};
+}
+// (In constant memory, from where an instruction takes them: as numbers in the code each costs two moves whenever it is used.)
+__constant__ double kSeries[4] = {5.732851688640402e-10, 2.1173137155464776e-07, 5.86490495505617e-05, 0.010830424696249145};
+
+// The table holds 2^(j / 64) less j 2^14 in its high word, so that adding k 2^14 there leaves 2^(k / 64).
+__device__ __forceinline__ double table_entry(int j) {
+    const double e = exp2((double)j * (1.0 / 64.0));
+    return __hiloint2double(__double2hiint(e) - (j << 14), __double2loint(e));
+}
+// (Where x lies below the lowest, and where it is -infinity, it may be anything.)
+__device__ __forceinline__ double weight64_above(const double* table, float x, const Scale& c) {
+    constexpr float kRound = 12582912.f;  // 1.5 * 2^23: adding it rounds to a whole number, in the low bits
+    const float k = fmaf(x - c.max32, c.per32, kRound);
+    const int n = __float_as_int(k);
+    const double f = fma((double)x - c.max, c.per, (double)(kRound - k));
+    const double p = fma(fma(fma(kSeries[0], f, kSeries[1]), f, kSeries[2]), f, kSeries[3]);
+    const double j = *reinterpret_cast<const double*>(reinterpret_cast<const char*>(table) + ((n << 3) & 504));
+    const double e = __hiloint2double(__double2hiint(j) + (n << 14), __double2loint(j));
+    return fma(e * f, p, e);
 }
 __device__ __forceinline__ double weight64(const double* table, float x, const Scale& c) {
-    constexpr double kRound = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to a whole number, in the low word
-    const double u = ((double)x - c.max) * c.per, k = u + kRound, f = u - (k - kRound);
-    const int n = __double2loint(k);
-    const double p = fma(fma(fma(5.732851688640402e-10, f, 2.1173137155464776e-07), f, 5.86490495505617e-05), f, 0.010830424696249145);
-    const double e = table[n & 63], w = fma(e * f, p, e);
-    return x >= c.lowest ? __hiloint2double(__double2hiint(w) + (n & ~63) * (1 << 14), __double2loint(w)) : 0.0;
+    const double w = weight64_above(table, x, c);
+    return x >= c.lowest ? w : 0.0;
 }
 
 constexpr int kPickWarps = kPickThreads / 32;
 
 struct PickShared {
-    double table[64];                // 2^(j / 64)
+    double table[64];                // see table_entry
     double warp[4][kPickWarps];
     double cta[2][4][kPickCtas];     // every CTA's sums, written by them: [turn][which][rank]
     double chunk[kPickWarps];        // the warps' shares of the ids among which the pick lies
@@ -261,7 +280,7 @@ verify_pick_kernel(const float* __restrict__ logits, const float* __restrict__ d
     cg::cluster_group cluster = cg::this_cluster();
     const int b = blockIdx.y, rank = (int)cluster.block_rank(), ctas = (int)cluster.num_blocks();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    if (tid < 64) s.table[tid] = exp2((double)tid * (1.0 / 64.0));
+    if (tid < 64) s.table[tid] = table_entry(tid);
     if (tid == 0) {
         s.stop = s.found = 0x7fffffff;
         s.last = -1;
@@ -337,8 +356,13 @@ verify_pick_kernel(const float* __restrict__ logits, const float* __restrict__ d
     Scale zc = {}, yc = {};
     float line = 0.f;  // p is larger than q where z - y lies above it (by the sums in 32 bits)
     auto ask = [&](const float* row, int first, float (&x)[kAhead]) {  // logits of ids first, first + 32, ...
+        if (first - lane + 32 * kAhead <= end) {
 #pragma unroll
-        for (int k = 0; k < kAhead; ++k) x[k] = first + 32 * k < end ? row[first + 32 * k] : -INFINITY;
+            for (int k = 0; k < kAhead; ++k) x[k] = row[first + 32 * k];
+        } else {
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) x[k] = first + 32 * k < end ? row[first + 32 * k] : -INFINITY;
+        }
     };
     // The sums of row i, at which warp `stopped` stopped, in 64 bits: of p's weights, of q's, and of both over the ids where p is
     // the larger, by the sums in 32 bits.  The last two give what q leaves of p, sum p[more] / sum p - sum q[more] / sum q,
@@ -363,13 +387,14 @@ verify_pick_kernel(const float* __restrict__ logits, const float* __restrict__ d
                 ask(y, i0 + 32 * kAhead, next_y);
 #pragma unroll
                 for (int k = 0; k < kAhead; ++k) {
-                    const double ez = weight64(s.table, xz[k], zc), ey = weight64(s.table, xy[k], yc);
-                    sums[0] += ez;
-                    sums[1] += ey;
-                    if (xz[k] - xy[k] > line) {
-                        sums[2] += ez;
-                        sums[3] += ey;
+                    const double ez = weight64_above(s.table, xz[k], zc), ey = weight64_above(s.table, xy[k], yc);
+                    const bool any = xy[k] >= yc.lowest, more = xz[k] - xy[k] > line;
+                    if (xz[k] >= zc.lowest) {
+                        sums[0] += ez;
+                        if (more) sums[2] += ez;
                     }
+                    if (any) sums[1] += ey;
+                    if (any && more) sums[3] += ey;
                     xz[k] = next_z[k];
                     xy[k] = next_y[k];
                 }
@@ -381,9 +406,10 @@ verify_pick_kernel(const float* __restrict__ logits, const float* __restrict__ d
                 ask(z, i0 + 32 * kAhead, next_z);
 #pragma unroll
                 for (int k = 0; k < kAhead; ++k) {
-                    const double ez = weight64(s.table, xz[k], zc);
-                    sums[0] += ez;
-                    if (i0 + 32 * k != without) sums[2] += ez;
+                    const double ez = weight64_above(s.table, xz[k], zc);
+                    const bool any = xz[k] >= zc.lowest;
+                    if (any) sums[0] += ez;
+                    if (any && i0 + 32 * k != without) sums[2] += ez;
                     xz[k] = next_z[k];
                 }
             }
@@ -530,9 +556,9 @@ NNIS_API int nnis_verify_drafts(const float* logits, const float* draft_logits, 
     cudaError_t e = launch_dependent(verify_rows_kernel, dim3(n_parts, all_rows), kVerifyThreads, 0, stream, logits, draft_logits,
                                      first_row, temperature, n_seqs, rows, vocab, per, static_cast<RowSum*>(scratch));
     if (e != cudaSuccess) return (int)e;
-    // As many CTAs a sequence as the device holds at once (two an SM) for all of them, sixteen at most, four at least: a row of
-    // 49,152 is walked in 9.8 us by sixteen, 15.4 by eight (24 sequences), 32 by four (64 sequences, which eight would
-    // take in two turns).
+    // As many CTAs a sequence as the device holds at once (two an SM) for all of them, sixteen at most, four at least: the launch takes
+    // 9.2 us with sixteen (one sequence, rows of 49,152), 10.4 with eight (24 sequences), 21 with four (64 sequences, which eight
+    // would take in two turns).
     cudaLaunchConfig_t cfg = {};
     static const int slots = 2 * device_sms();
     int ctas = kPickCtas;
