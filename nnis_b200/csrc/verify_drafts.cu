@@ -524,7 +524,7 @@ verify_pick_kernel(const float* __restrict__ logits, const float* __restrict__ d
     if (tid == 0) picked[b] = s.found < vocab ? s.found : s.last;
 }
 // CTAs a row: shares of 8,192 logits, of 4,096 where all rows together are no more than four CTAs an SM then (nine rows of 49,152:
-// 4.4 -> 3.6 us; 960 rows 37.5 us with 8,192 and more, 49 with 4,096).
+// 4.4 -> 3.7 us; 144 rows 9.2 us with 8,192, 9.7 with 4,096, 960 rows 33 and 41).
 static int verify_parts(long long rows, int vocab) {
     const int fine = (vocab + kVerifyShare / 2 - 1) / (kVerifyShare / 2);
     const int n = rows * fine <= 600 ? fine : (vocab + kVerifyShare - 1) / kVerifyShare;
@@ -557,7 +557,7 @@ NNIS_API int nnis_verify_drafts(const float* logits, const float* draft_logits, 
                                      first_row, temperature, n_seqs, rows, vocab, per, static_cast<RowSum*>(scratch));
     if (e != cudaSuccess) return (int)e;
     // As many CTAs a sequence as the device holds at once (two an SM) for all of them, sixteen at most, four at least: the launch takes
-    // 9.2 us with sixteen (one sequence, rows of 49,152), 10.4 with eight (24 sequences), 21 with four (64 sequences, which eight
+    // 9.8 us with sixteen (one sequence, rows of 49,152), 10.7 with eight (24 sequences), 21.5 with four (64 sequences, which eight
     // would take in two turns).
     cudaLaunchConfig_t cfg = {};
     static const int slots = 2 * device_sms();
