@@ -6,6 +6,8 @@
 // the softmax's running maximum and sum are a half-warp's shuffles, the weights go to shared memory and the outputs, a
 // thread's 1 or 4 entries x d / 16 values, are added up in registers while the page's V replaces its K.  It is the form that is
 // right for every size, not a fast one: its loads wait for its products.
+#include <string.h>
+
 #include "attention_shared.cuh"
 
 namespace nnis {
@@ -189,12 +191,30 @@ cudaError_t shared_units_any(const SharedArgs& a, int n_units, int tile, bool f3
 // form 1).  partial: records x nq x d floats,
 // sums: records x nq x 2.  tickets (n_tokens x nq counters, zero, left zero): every row is merged by the CTA that completes it, and no
 // merge is launched (where all units are of the second kind, or `form` is not 1); every row then has a record.
-NNIS_API int nnis_attention_shared(const void* q, int q_stride, const void* k_cache, const void* v_cache, const int* token_pos,
-                                   const int* page_table, int table_cols, const int* units, int n0, int n1, int n2,
-                                   const int* members, const int* record, float* partial, float* sums, unsigned* tickets, void* out, int n_tokens,
-                                   int nq, int nkv, int d, int pages, int page_size, float scale, int dtype, int form, int* status,
-                                   cudaStream_t stream) {
+struct SharedCall {
+    const void* q;
+    int q_stride;
+    const void *k_cache, *v_cache;
+    const int *token_pos, *page_table;
+    int table_cols;
+    const int* units;
+    int n0, n1, n2;
+    const int *members, *record;
+    float *partial, *sums;
+    unsigned* tickets;
+    void* out;
+    int n_tokens, nq, nkv, d, pages, page_size;
+    float scale;
+    int dtype, form;
+    int* status;
+    cudaStream_t stream;
+};
+NNIS_API int nnis_attention_shared(const void* call) {
     using namespace nnis;
+    SharedCall c;
+    memcpy(&c, call, sizeof c);
+    const auto [q, q_stride, k_cache, v_cache, token_pos, page_table, table_cols, units, n0, n1, n2, members, record, partial, sums,
+                tickets, out, n_tokens, nq, nkv, d, pages, page_size, scale, dtype, form, status, stream] = c;
     if (n_tokens <= 0 || nq <= 0 || nkv <= 0 || nq % nkv || table_cols <= 0 || n0 < 0 || n1 < 0 || n2 < 0 || pages <= 0 || !record ||
         !partial || !sums || !(scale > 0.f) || (n0 + n1 + n2 > 0 && (!units || !members)))
         return NNIS_ERR_ARGUMENT;

@@ -11,6 +11,7 @@ import array
 import ctypes
 import functools
 import math
+import struct
 import os
 from typing import Optional
 
@@ -62,31 +63,40 @@ def _stream() -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
-def _types(letters: str):
-    return [{"p": ctypes.c_void_p, "i": ctypes.c_int, "f": ctypes.c_float}[c] for c in letters]
-
-
-# Entry points that take plain numbers for their arguments (p: an address, i: an int, f: a float): a call with thirty arguments
-# wrapped one by one costs the host 8 us, this one 3.
-_ENTRY_TYPES = {"nnis_copy_pages": "ppiiiiiipiip", "nnis_verify_scratch": "iii", "nnis_verify_drafts": "ppppppppiiippp",
-                "nnis_attention_shared": "pippppipiiippppppiiiiiifiipp"}
+# Entry points that take their arguments as one record, a C struct of these fields (p: an address, i: an int, f: a float; an address
+# comes last, so that neither side pads the end): thirty arguments wrapped one by one cost the host 8 us, as plain numbers
+# 2.4, in a record 0.6.
+_ENTRY_FIELDS = {"nnis_copy_pages": "ppiiiiiipiip", "nnis_verify_drafts": "ppppppppiiippp",
+                 "nnis_attention_shared": "pippppipiiippppppiiiiiifiipp"}
 _entries = {}
 
 
 def _entry(name: str):
-    fn = _entries.get(name)
-    if fn is None:
+    call = _entries.get(name)
+    if call is None:
         fn = getattr(_lib(), name)
-        fn.argtypes = _types(_ENTRY_TYPES[name])
-        _entries[name] = fn
-    return fn
+        fn.argtypes = [ctypes.c_char_p]
+        pack = struct.Struct("@" + _ENTRY_FIELDS[name].replace("p", "P")).pack
+
+        def call(*args) -> int:
+            try:
+                record = pack(*args)
+            except (struct.error, OverflowError) as error:
+                raise KernelError(f"{name}: {error}") from None
+            return fn(record)
+
+        _entries[name] = call
+    return call
 
 
-def _stream_here() -> int:
-    """The current stream of the current device as a number."""
+_device_now = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def _stream_of(index: int) -> int:
+    """The current stream of device ``index`` as a number."""
     if _raw_stream is not None:
-        return _raw_stream(torch.cuda.current_device())
-    return torch.cuda.current_stream().cuda_stream
+        return _raw_stream(index)
+    return torch.cuda.current_stream(index).cuda_stream
 
 
 def _ptr(t: Optional[torch.Tensor]) -> ctypes.c_void_p:
@@ -186,21 +196,21 @@ def copy_pages(k: torch.Tensor, v: Optional[torch.Tensor], moves) -> None:
     """Pages copied inside the store for all layers at once: for every (source page, target page, rows) of ``moves`` the
     first ``rows`` positions of the target become the source's.  k: [layers, pages, kv_heads, page_size, dim], v the same with
     its own dim, or None.  A page that is a target is the target of one move and the source of none."""
-    _cuda(k, v)
-    _need(k.dim() == 5 and k.numel() > 0, "copy_pages: k [layers, pages, kv_heads, page_size, dim]")
-    layers, pages, heads, page_size, dim = k.shape
-    k_row, v_row = dim * k.element_size(), 0
-    if v is not None:
-        _need(v.dim() == 5 and v.shape[:4] == k.shape[:4] and v.device == k.device and v.numel() > 0,
-              "copy_pages: v [layers, pages, kv_heads, page_size, value dim] beside k")
-        v_row = v.shape[4] * v.element_size()
-    _need(k_row % 2 == 0 and v_row % 2 == 0, "copy_pages: rows of a multiple of two bytes")
-    _need(layers <= 65535 and heads * page_size * max(k_row, v_row) < 2 ** 32, "copy_pages: at most 65,535 layers, pages below 4 GB")
+    shape, index = k.shape, k.get_device()
+    if len(shape) != 5 or index < 0 or not k.is_contiguous() or not shape.numel() or (
+            v is not None and (v.dim() != 5 or v.shape[:4] != shape[:4] or v.get_device() != index or not v.is_contiguous() or not v.numel())):
+        _cuda(k, v)
+        raise KernelError("copy_pages: k [layers, pages, kv_heads, page_size, dim], and v [layers, pages, kv_heads, page_size, value "
+                          f"dim] beside it; got {tuple(shape)} and {None if v is None else tuple(v.shape)}")
+    layers, pages, heads, page_size, dim = shape
+    k_row = dim * k.element_size()
+    v_row = 0 if v is None else v.shape[4] * v.element_size()
+    if (k_row | v_row) % 2 or layers > 65535 or heads * page_size * max(k_row, v_row) >= 2 ** 32:
+        raise KernelError("copy_pages: rows of a multiple of two bytes, at most 65,535 layers, pages below 4 GB")
     if not moves:
         return
-    device = k.device.index
-    if torch.cuda.current_device() != device:
-        with torch.cuda.device(device):
+    if _device_now() != index:
+        with torch.cuda.device(index):
             return copy_pages(k, v, moves)
     try:  # (a list of 63 moves read number by number in Python takes 40 us, as three rows 7)
         src, dst, rows = zip(*moves, strict=True)
@@ -208,8 +218,8 @@ def copy_pages(k: torch.Tensor, v: Optional[torch.Tensor], moves) -> None:
     except (TypeError, ValueError, OverflowError) as error:
         raise KernelError(f"copy_pages: moves are (source page, target page, rows), whole numbers: {error}") from None
     code = _entry("nnis_copy_pages")(
-        k.data_ptr(), None if v is None else v.data_ptr(), layers, pages, heads, page_size, k_row, v_row, ints.buffer_info()[0],
-        len(src), sm_count(k.device), _stream_here())
+        k.data_ptr(), 0 if v is None else v.data_ptr(), layers, pages, heads, page_size, k_row, v_row, ints.buffer_info()[0],
+        len(src), _sm_count.get(index) or sm_count(k.device), _stream_of(index))
     if code == -1:
         _moves_refused(moves, pages, page_size)
     _check(code, "copy_pages", -(-len(src) // 1024))
@@ -419,29 +429,38 @@ def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, first_row: torch.T
                   accept_draws: torch.Tensor, pick_draws: torch.Tensor, accepted: torch.Tensor, picked: torch.Tensor,
                   draft_logits: Optional[torch.Tensor], workspace) -> None:
     """See ``sampling.device.verify_drafts``."""
-    b, device, i32, f32, f64 = first_row.numel() - 1, logits.device, torch.int32, torch.float32, torch.float64
-    rows, vocab = logits.shape if logits.dim() == 2 else (0, 0)
+    b, index, i32, f32, f64 = first_row.numel() - 1, logits.get_device(), torch.int32, torch.float32, torch.float64
+    shape = logits.shape
+    rows, vocab = shape if len(shape) == 2 else (0, 0)
     drafted = rows - b
-    good = 1 <= b <= rows <= 32767 and 0 < vocab <= 1 << 26
-    for t, dtype, count in ((logits, f32, rows * vocab), (drafts, i32, drafted), (first_row, i32, b + 1), (temperatures, f32, b),
-                            (accept_draws, f64, drafted), (pick_draws, f64, b), (accepted, i32, b), (picked, i32, b)):
-        good = good and t.dtype == dtype and t.numel() == count and t.device == device and t.is_contiguous()
-    if draft_logits is not None:
-        good = good and draft_logits.dtype == f32 and draft_logits.shape == (drafted, vocab) and draft_logits.device == device \
-            and draft_logits.is_contiguous()
-    if not good or device.type != "cuda":
+    if not (1 <= b <= rows <= 32767 and 0 < vocab <= 1 << 26 and index >= 0
+            and logits.dtype is f32 and drafts.dtype is first_row.dtype is accepted.dtype is picked.dtype is i32
+            and temperatures.dtype is f32 and accept_draws.dtype is pick_draws.dtype is f64
+            and drafts.numel() == accept_draws.numel() == drafted
+            and temperatures.numel() == pick_draws.numel() == accepted.numel() == picked.numel() == b
+            and drafts.get_device() == first_row.get_device() == temperatures.get_device() == accept_draws.get_device()
+            == pick_draws.get_device() == accepted.get_device() == picked.get_device() == index
+            and logits.is_contiguous() and drafts.is_contiguous() and first_row.is_contiguous() and temperatures.is_contiguous()
+            and accept_draws.is_contiguous() and pick_draws.is_contiguous() and accepted.is_contiguous() and picked.is_contiguous()
+            and (draft_logits is None or (draft_logits.dtype is f32 and draft_logits.shape == (drafted, vocab)
+                                          and draft_logits.get_device() == index and draft_logits.is_contiguous()))):
         _verify_refused(logits, drafts, first_row, temperatures, accept_draws, pick_draws, accepted, picked, draft_logits)
         raise KernelError("verify: arguments that are not taken")
-    if torch.cuda.current_device() != device.index:
-        with torch.cuda.device(device):
+    if _device_now() != index:
+        with torch.cuda.device(index):
             return verify_drafts(logits, drafts, first_row, temperatures, accept_draws, pick_draws, accepted, picked,
                                  draft_logits, workspace)
-    need = _entry("nnis_verify_scratch")(rows, drafted, vocab)
-    scratch = workspace.room("verify_sums", need // 4, f32)
+    scratch = workspace.room("verify_sums", _verify_scratch(rows, drafted, vocab) // 4, f32)
     _check(_entry("nnis_verify_drafts")(
-        logits.data_ptr(), draft_logits.data_ptr() if draft_logits is not None and drafted else None, drafts.data_ptr(),
+        logits.data_ptr(), draft_logits.data_ptr() if draft_logits is not None and drafted else 0, drafts.data_ptr(),
         first_row.data_ptr(), temperatures.data_ptr(), accept_draws.data_ptr(), pick_draws.data_ptr(), scratch.data_ptr(), b, rows,
-        vocab, accepted.data_ptr(), picked.data_ptr(), _stream_here()), "verify_drafts", 2)
+        vocab, accepted.data_ptr(), picked.data_ptr(), _stream_of(index)), "verify_drafts", 2)
+
+
+@functools.lru_cache(maxsize=1024)
+def _verify_scratch(rows: int, drafted: int, vocab: int) -> int:
+    """Bytes of scratch that these sizes need."""
+    return _lib().nnis_verify_scratch(rows, drafted, vocab)
 
 
 EPI_STORE, EPI_STORE_F32, EPI_ADD_F32, EPI_GATED, EPI_QKV, EPI_ARGMAX = 0, 1, 2, 3, 4, 5
@@ -2860,7 +2879,8 @@ class SharedPlan:
         # 11.5 us instead of 13; where a unit's entries have much (8 rows of 14 records) its kernel takes 12 to 16 us for 7.4 and 4.1
         self.merged_inside = most_entries * head_dim <= 1024 and counts[2] == 0 and (self.form != 1 or counts[0] == 0) \
             and sum(counts) * kv_heads <= 148 and records <= 8 * rows
-        self.device, self.status = ints.device, status_word(ints.device).data_ptr()
+        self.device, self.index, self.status = ints.device, ints.get_device(), status_word(ints.device).data_ptr()
+        self.code, self.item = _DTYPE_CODE[dtype], dtype.itemsize
         self.launches = (not self.merged_inside) + sum(c > 0 for c in counts)
 
     @classmethod
@@ -2941,34 +2961,35 @@ def attention_shared(q: torch.Tensor, q_stride: int, k_cache: torch.Tensor, v_ca
                      scale: float, workspace) -> None:
     """Causal attention of packed query tokens over the paged cache, pages that several rows share read once for all of them.
     ``plan``: ``attention_shared_plan`` of the same rows, positions and page lists."""
-    n, d, dtype, device = plan.rows, plan.head_dim, plan.dtype, plan.device
-    shape = k_cache.shape
+    n, d, dtype, index = plan.rows, plan.head_dim, plan.dtype, plan.index
+    shape, q_shape, table_shape = k_cache.shape, q.shape, page_table.shape
     if not (heads == plan.heads and kv_heads == plan.kv_heads and head_dim == d and len(shape) == 4 and shape[1] == kv_heads
             and shape[2] == 64 and shape[3] == d and v_cache.shape == shape and out.shape == (n, heads * d)
-            and q.dim() == 2 and q.shape[0] >= n and q.stride() == (q_stride, 1) and q_stride >= heads * d
-            and token_pos.numel() >= n and page_table.dim() == 2 and page_table.shape[0] >= plan.seqs
-            and page_table.shape[1] >= plan.cols and q.dtype == k_cache.dtype == v_cache.dtype == out.dtype == dtype
-            and token_pos.dtype == page_table.dtype == torch.int32 and scale > 0
-            and q.device == k_cache.device == v_cache.device == token_pos.device == page_table.device == out.device == device
+            and len(q_shape) == 2 and q_shape[0] >= n and q.stride() == (q_stride, 1) and q_stride >= heads * d
+            and token_pos.numel() >= n and len(table_shape) == 2 and table_shape[0] >= plan.seqs and table_shape[1] >= plan.cols
+            and q.dtype is k_cache.dtype is v_cache.dtype is out.dtype is dtype
+            and token_pos.dtype is page_table.dtype is torch.int32 and scale > 0
+            and q.get_device() == k_cache.get_device() == v_cache.get_device() == token_pos.get_device() == page_table.get_device()
+            == out.get_device() == index
             and k_cache.is_contiguous() and v_cache.is_contiguous() and out.is_contiguous() and token_pos.is_contiguous()
             and page_table.is_contiguous() and shape[0] * kv_heads < 1 << 25
-            and (plan.form == 0 or (q_stride * q.element_size() % 16 == 0 and q.data_ptr() % 16 == 0))):
+            and (plan.form == 0 or (q_stride * plan.item % 16 == 0 and q.data_ptr() % 16 == 0))):
         raise KernelError(
             f"attention_shared: the plan is of {n} rows, {plan.heads} heads over {plan.kv_heads} of {d}, {dtype}, {plan.seqs} sequences of "
-            f"{plan.cols} pages on {device}; wanted are q [rows, heads * d] in rows of q_stride (of whole 16 bytes for heads of 64 and 128), k and v [pages < 2^25 / kv_heads, "
+            f"{plan.cols} pages on {plan.device}; wanted are q [rows, heads * d] in rows of q_stride (of whole 16 bytes for heads of 64 and 128), k and v [pages < 2^25 / kv_heads, "
             f"kv_heads, 64, d], token_pos int32 [rows], page_table int32, out [rows, heads * d], contiguous, and a positive scale; got "
             f"q {tuple(q.shape)} of {q.dtype}, cache {tuple(shape)} of {k_cache.dtype}, out {tuple(out.shape)}, page_table "
             f"{tuple(page_table.shape)}, scale {scale}")
-    if torch.cuda.current_device() != device.index:
-        with torch.cuda.device(device):
+    if _device_now() != index:
+        with torch.cuda.device(index):
             return attention_shared(q, q_stride, k_cache, v_cache, token_pos, page_table, plan, out, heads, kv_heads, head_dim,
                                     scale, workspace)
     held = max(1, plan.records) * heads
     at = workspace.room("attn_shared_records", held * (d + 2), torch.float32).data_ptr()
-    tickets = workspace.zeros_room("attn_shared_tickets", n * heads, torch.int32).data_ptr() if plan.merged_inside else None
+    tickets = workspace.zeros_room("attn_shared_tickets", n * heads, torch.int32).data_ptr() if plan.merged_inside else 0
     n0, n1, n2 = plan.counts
     _check(_entry("nnis_attention_shared")(
         q.data_ptr(), q_stride, k_cache.data_ptr(), v_cache.data_ptr(), token_pos.data_ptr(), page_table.data_ptr(),
-        page_table.shape[1], plan.units, n0, n1, n2, plan.members, plan.record, at, at + 4 * held * d, tickets, out.data_ptr(), n,
-        heads, kv_heads, d, shape[0], 64, scale, F32 if dtype == torch.float32 else BF16, plan.form, plan.status, _stream_here()),
+        table_shape[1], plan.units, n0, n1, n2, plan.members, plan.record, at, at + 4 * held * d, tickets, out.data_ptr(), n,
+        heads, kv_heads, d, shape[0], 64, scale, plan.code, plan.form, plan.status, _stream_of(index)),
         "attention_shared", plan.launches)

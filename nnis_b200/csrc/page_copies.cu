@@ -6,6 +6,7 @@
 // pages of 30 layers (48 MB read and written) 13 us; 24 whole pages of 24 layers of 32 heads (1.2 GB) 193 us, 0.97 of the
 // measured copy rate; one page of 30 layers 2.8 us.
 #include <stdlib.h>
+#include <string.h>
 
 #include "async_copy.cuh"
 #include "common.cuh"
@@ -85,9 +86,18 @@ static cudaError_t launch_moves(void* k, void* v, int layers, int pages, int kv_
 // k and v (or null): [layers, pages, kv_heads, page_size, row] with rows of `k_row` and `v_row` bytes, multiples of 2.
 // moves, on the host: `count` sources, then targets, then numbers of rows (0 to page_size).  NNIS_ERR_ARGUMENT, with nothing
 // copied, where a page is outside the store, the target of two moves, or a target and a source.
-NNIS_API int nnis_copy_pages(void* k, void* v, int layers, int pages, int kv_heads, int page_size, int k_row, int v_row,
-                             const int* moves, int count, int sms, cudaStream_t stream) {
+struct CopyCall {
+    void *k, *v;
+    int layers, pages, kv_heads, page_size, k_row, v_row;
+    const int* moves;
+    int count, sms;
+    cudaStream_t stream;
+};
+NNIS_API int nnis_copy_pages(const void* call) {
     using namespace nnis;
+    CopyCall c;
+    memcpy(&c, call, sizeof c);
+    const auto [k, v, layers, pages, kv_heads, page_size, k_row, v_row, moves, count, sms, stream] = c;
     if (!k || !moves || count < 0 || layers <= 0 || pages <= 0 || kv_heads <= 0 || page_size <= 0 || k_row <= 0 || k_row % 2 ||
         (v && (v_row <= 0 || v_row % 2)))
         return NNIS_ERR_ARGUMENT;

@@ -23,6 +23,7 @@
 // row, cluster, pick.  Both in turns, the next sequences' rows beside the last ones' picks, were slower (62 us for 58).
 #include <cooperative_groups.h>
 #include <float.h>
+#include <string.h>
 
 #include "async_copy.cuh"
 #include "common.cuh"
@@ -541,10 +542,22 @@ NNIS_API long long nnis_verify_scratch(int rows, int draft_rows, int vocab) {
 
 // first_row: n_seqs + 1 offsets into the packed rows of `logits` [rows, vocab], the last one `rows`; draft rows (drafts,
 // accept_draws, draft_logits or null) lie without the sequences' last rows.
-NNIS_API int nnis_verify_drafts(const float* logits, const float* draft_logits, const int* drafts, const int* first_row,
-                                const float* temperature, const double* accept_draws, const double* pick_draws, void* scratch,
-                                int n_seqs, int rows, int vocab, int* accepted, int* picked, cudaStream_t stream) {
+struct VerifyCall {
+    const float *logits, *draft_logits;
+    const int *drafts, *first_row;
+    const float* temperature;
+    const double *accept_draws, *pick_draws;
+    void* scratch;
+    int n_seqs, rows, vocab;
+    int *accepted, *picked;
+    cudaStream_t stream;
+};
+NNIS_API int nnis_verify_drafts(const void* call) {
     using namespace nnis;
+    VerifyCall v;
+    memcpy(&v, call, sizeof v);
+    const auto [logits, draft_logits, drafts, first_row, temperature, accept_draws, pick_draws, scratch, n_seqs, rows, vocab, accepted,
+                picked, stream] = v;
     if (n_seqs <= 0 || rows < n_seqs || vocab <= 0 || !logits || !first_row || !temperature || !pick_draws || !scratch || !accepted ||
         !picked)
         return NNIS_ERR_ARGUMENT;
