@@ -212,10 +212,10 @@ def copy_pages(k: torch.Tensor, v: Optional[torch.Tensor], moves) -> None:
     if _device_now() != index:
         with torch.cuda.device(index):
             return copy_pages(k, v, moves)
-    try:  # (a list of 63 moves read number by number in Python takes 40 us, as three rows 7)
+    try:  # (a list of 63 moves read number by number in Python takes 40 us, as three rows 7, packed 5)
         src, dst, rows = zip(*moves, strict=True)
-        ints = array.array("i", src + dst + rows)
-    except (TypeError, ValueError, OverflowError) as error:
+        ints = array.array("i", struct.pack(f"{3 * len(src)}i", *src, *dst, *rows))
+    except (TypeError, ValueError, struct.error) as error:
         raise KernelError(f"copy_pages: moves are (source page, target page, rows), whole numbers: {error}") from None
     code = _entry("nnis_copy_pages")(
         k.data_ptr(), 0 if v is None else v.data_ptr(), layers, pages, heads, page_size, k_row, v_row, ints.buffer_info()[0],

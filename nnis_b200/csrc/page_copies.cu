@@ -13,7 +13,7 @@
 
 namespace nnis {
 
-constexpr int kMoves = 1024, kFewMoves = 32;  // of a launch: 12 KB of parameters, 384 bytes (2 us of the host less)
+constexpr int kMoves = 1024, kSomeMoves = 128, kFewMoves = 32;  // of a launch: 12 KB of parameters, 1.5 KB, 384 bytes (2 us of the host less)
 
 template <int N>
 struct PageMoves {
@@ -120,7 +120,7 @@ NNIS_API int nnis_copy_pages(const void* call) {
     if (!good) return NNIS_ERR_ARGUMENT;
     for (int first = 0; first < count; first += kMoves) {
         const int n = count - first < kMoves ? count - first : kMoves;
-        auto launch = n <= kFewMoves ? launch_moves<kFewMoves> : launch_moves<kMoves>;
+        auto launch = n <= kFewMoves ? launch_moves<kFewMoves> : n <= kSomeMoves ? launch_moves<kSomeMoves> : launch_moves<kMoves>;
         const cudaError_t e = launch(k, v, layers, pages, kv_heads, page_size, k_row, v_row, src + first, dst + first, rows + first, n,
                                      sms, stream);
         if (e != cudaSuccess) return (int)e;
