@@ -56,6 +56,13 @@ __device__ __forceinline__ void units_end(const SharedArgs& a) {
     if (a.beside) pdl_wait();
 }
 
+// 2^x for a weight: one that would be denormal is zero (exp2f keeps it, by four instructions instead of one).
+__device__ __forceinline__ float sh_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 // Adds up one (token row, head)'s records: a warp; lane s holds the weights of records s, s + 32, ..., every lane sums its pairs of
 // values over the records in their order, AHEAD records asked for at a time.  Where no record holds a key the result is zero.
 template <typename T, int AHEAD>

@@ -108,12 +108,12 @@ attn_shared_f32_kernel(const SharedArgs a) {
 #pragma unroll
             for (int w = 8; w > 0; w >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
             const float m_new = fmaxf(m_run[r], mx), base = m_new == -INFINITY ? 0.f : m_new;
-            const float alpha = exp2f(m_run[r] - base);
+            const float alpha = sh_ex2(m_run[r] - base);
             m_run[r] = m_new;
             float sum = 0.f;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float p = exp2f(s[r][i] - base);
+                const float p = sh_ex2(s[r][i] - base);
                 sum += p;
                 p_s[(ty * ROWS + r) * kPs + tx + 16 * i] = p;
             }

@@ -138,14 +138,14 @@ attn_shared_mma_kernel(const SharedArgs a) {
                 mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
                 const float mn = fmaxf(m_run[t][r], mx[r]);
                 base[r] = mn == -INFINITY ? 0.f : mn;  // nothing seen yet: no inf - inf
-                alpha[t][r] = exp2f(m_run[t][r] - base[r]);
+                alpha[t][r] = sh_ex2(m_run[t][r] - base[r]);
                 m_run[t][r] = mn;
             }
             float sum[2] = {0.f, 0.f};
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                const float p0 = exp2f(s[j][0] - base[0]), p1 = exp2f(s[j][1] - base[0]);
-                const float p2 = exp2f(s[j][2] - base[1]), p3 = exp2f(s[j][3] - base[1]);
+                const float p0 = sh_ex2(s[j][0] - base[0]), p1 = sh_ex2(s[j][1] - base[0]);
+                const float p2 = sh_ex2(s[j][2] - base[1]), p3 = sh_ex2(s[j][3] - base[1]);
                 sum[0] += p0 + p1;
                 sum[1] += p2 + p3;
                 pa[t][j * 2] = pack_bf16(p0, p1);
@@ -153,10 +153,12 @@ attn_shared_mma_kernel(const SharedArgs a) {
             }
 #pragma unroll
             for (int r = 0; r < 2; ++r) l_run[t][r] = l_run[t][r] * alpha[t][r] + sum[r];
+            if (__any_sync(0xffffffffu, alpha[t][0] != 1.f || alpha[t][1] != 1.f)) {
 #pragma unroll
-            for (int j = 0; j < NT; ++j)
+                for (int j = 0; j < NT; ++j)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[t][j][e] *= alpha[t][e >> 1];
+                    for (int e = 0; e < 4; ++e) o[t][j][e] *= alpha[t][e >> 1];
+            }
         }
 #pragma unroll
         for (int j = 0; j < NT; j += 2) {

@@ -35,11 +35,6 @@ constexpr float kShRaise = 8.0f;
 template <int D>
 constexpr int sh_stages() { return D == 64 ? 4 : 2; }
 
-__device__ __forceinline__ float sh_ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 __device__ __forceinline__ float sh_max3(float a, float b, float c) {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));

@@ -159,14 +159,14 @@ attn_shared_warp_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
                 mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
                 const float mn = fmaxf(m_run[r], mx[r]);
                 base[r] = mn == -INFINITY ? 0.f : mn;  // nothing seen yet: no inf - inf
-                alpha[r] = exp2f(m_run[r] - base[r]);
+                alpha[r] = sh_ex2(m_run[r] - base[r]);
                 m_run[r] = mn;
             }
             uint32_t pa[4][4];  // four k-steps of 16 keys
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const float p0 = exp2f(s[j][0] - base[0]), p1 = exp2f(s[j][1] - base[0]);
-                const float p2 = exp2f(s[j][2] - base[1]), p3 = exp2f(s[j][3] - base[1]);
+                const float p0 = sh_ex2(s[j][0] - base[0]), p1 = sh_ex2(s[j][1] - base[0]);
+                const float p2 = sh_ex2(s[j][2] - base[1]), p3 = sh_ex2(s[j][3] - base[1]);
                 sum[0] += p0 + p1;
                 sum[1] += p2 + p3;
                 pa[j >> 1][(j & 1) * 2] = pack_bf16(p0, p1);
@@ -183,10 +183,12 @@ attn_shared_warp_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
                 fence_async_shared();  // (the next page comes by the other proxy)
                 __syncwarp();
             }
+            if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
 #pragma unroll
-            for (int j = 0; j < NT; ++j)
+                for (int j = 0; j < NT; ++j)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[j][e] *= alpha[e >> 1];
+                    for (int e = 0; e < 4; ++e) o[j][e] *= alpha[e >> 1];
+            }
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
