@@ -64,42 +64,45 @@ __device__ __forceinline__ float sh_ex2(float x) {
 }
 
 // Adds up one (token row, head)'s records: a warp; lane s holds the weights of records s, s + 32, ..., every lane sums its pairs of
-// values over the records in their order, AHEAD records asked for at a time.  Where no record holds a key the result is zero.
+// values over the records in their order, AHEAD records asked for at a time, the first ones before any weight is known.  Where no
+// record holds a key the result is zero.
 template <typename T, int AHEAD>
 __device__ __forceinline__ void merge_row(const float* partial, const float2* sums, int first, int count, int row, int head, int nq,
                                           int d, T* out) {
     const int lane = threadIdx.x & 31;
     const size_t rec = (size_t)first * nq + head;
-    float m = -INFINITY;
-    for (int s = lane; s < count; s += 32) {
-        const float2 x = __ldcg(sums + rec + (size_t)s * nq);
+    auto ask_sum = [&](int s) { return s < count ? __ldcg(sums + rec + (size_t)s * nq) : make_float2(-INFINITY, 0.f); };
+    auto ask = [&](int s0, int j, float2 (&v)[AHEAD]) {
+        const int i = 2 * (lane + 32 * j);
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k)
+            v[k] = s0 + k < count && i < d ? __ldcg(reinterpret_cast<const float2*>(partial + (rec + (size_t)(s0 + k) * nq) * d + i))
+                                           : make_float2(0.f, 0.f);
+    };
+    float2 own = ask_sum(lane), v[AHEAD];
+    ask(0, 0, v);
+    float m = own.y != 0.f ? own.x : -INFINITY;
+    for (int s = lane + 32; s < count; s += 32) {
+        const float2 x = ask_sum(s);
         if (x.y != 0.f) m = fmaxf(m, x.x);
     }
     m = warp_max(m);
     float2 acc[4] = {};
     float l = 0.f;
     for (int s0 = 0; s0 < count; s0 += 32) {
-        float w = 0.f;
-        if (s0 + lane < count) {
-            const float2 x = __ldcg(sums + rec + (size_t)(s0 + lane) * nq);
-            w = x.y != 0.f ? exp2f(x.x - m) : 0.f;
-            l += x.y * w;
-        }
-        const int here = min(32, count - s0);
-        for (int s = 0; s < here; s += AHEAD) {
+        if (s0) own = ask_sum(s0 + lane);
+        const float w = own.y != 0.f ? exp2f(own.x - m) : 0.f;
+        l += own.y * w;
+        const int end = min(32, count - s0);
+        for (int s = 0; s < end; s += AHEAD) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 if (j * 64 >= d) break;
-                const int i = 2 * (lane + 32 * j);
-                float2 v[AHEAD];
-#pragma unroll
-                for (int k = 0; k < AHEAD; ++k)
-                    v[k] = s + k < here && i < d ? __ldcg(reinterpret_cast<const float2*>(partial + (rec + (size_t)(s0 + s + k) * nq) * d + i))
-                                                 : make_float2(0.f, 0.f);
+                if (s0 + s + j) ask(s0 + s, j, v);
 #pragma unroll
                 for (int k = 0; k < AHEAD; ++k) {
                     const float f = __shfl_sync(0xffffffffu, w, (s + k) & 31);
-                    if (s + k < here && f != 0.f) {  // (a record that holds nothing is never added)
+                    if (s + k < end && f != 0.f) {  // (a record that holds nothing is never added)
                         acc[j].x = fmaf(f, v[k].x, acc[j].x);
                         acc[j].y = fmaf(f, v[k].y, acc[j].y);
                     }
