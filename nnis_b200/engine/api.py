@@ -455,7 +455,8 @@ class InferenceSession:
         """Generation with drafted tokens: ``drafter`` (``drafting.LookupDrafter``, ``drafting.SessionDrafter``) proposes up to
         ``drafts`` tokens, one step runs them all, and those stay that the model keeps.  Greedy unless ``sampling`` is
         given (a temperature and a seed; top-k and top-p are refused): tokens are distributed as ``generate_sampled``'s without
-        the drafter, not the same for the same seed.  Every emitted token is executed, as in ``generate``."""
+        the drafter, not the same for the same seed.  Every emitted token is executed, as in ``generate``; where a
+        callback raises, the session holds no draft that it has not been shown."""
         if self.engine.cache.fixed_history():
             raise ValueError("drafted tokens that are refused are taken back: not for a model with state of fixed size or a window")
         if drafts < 1:
@@ -484,17 +485,23 @@ class InferenceSession:
                 self._decoded += 1
             else:
                 logits = self.engine.step([SequenceStep(self.slot, feed, [len(feed) - 1])])
-            kept, token = verifier.verify(logits, proposed, logits_of)
-            new, ended = proposed[:kept] + [token], False
-            for n, t in enumerate(new):
-                emitted.append(t)
-                stop = on_token is not None and on_token(t) is StreamControl.STOP
-                if stop or t in generation.stop_token_ids or len(emitted) >= generation.max_new_tokens:
-                    new, ended = new[:n + 1], True
-                    break
+            fed, kept, shown = held + len(feed) - len(proposed), 0, 0  # the session's length without any draft
+            try:
+                kept, token = verifier.verify(logits, proposed, logits_of)
+                new, ended = proposed[:kept] + [token], False
+                for n, t in enumerate(new):
+                    stop = on_token is not None and on_token(t) is StreamControl.STOP
+                    emitted.append(t)
+                    shown = n + 1
+                    if stop or t in generation.stop_token_ids or len(emitted) >= generation.max_new_tokens:
+                        new, ended = new[:n + 1], True
+                        break
+            except BaseException:  # (no draft stays that has not been emitted)
+                self.truncate(fed + min(shown, kept))
+                raise
             told += new
             # what stays of the step: what was fed before the drafts, and the drafts that were emitted
-            stays = held + len(feed) - len(proposed) + min(len(new), kept)
+            stays = fed + min(len(new), kept)
             if stays < self.position():
                 self.truncate(stays)
             if ended:

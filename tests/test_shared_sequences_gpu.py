@@ -193,6 +193,29 @@ def test_drafted_greedy_generation_is_greedy_generation(folder, small_folder):
     llm.engine.check_status()
 
 
+@pytest.mark.parametrize("at", [0, 1, 3, 6])
+def test_a_callback_that_raises_leaves_no_draft_behind(folder, at):
+    """The session holds the prompt and emitted tokens alone, and goes on from there."""
+    from nnis_b200 import LLM, GenerationConfig, SessionDrafter
+    llm = LLM(folder, dtype="float32", max_tokens=1 << 13, max_batch=8)
+    prompt, shown = tokens(6, 40) * 5, []
+
+    def on_token(token):
+        if len(shown) == at:
+            raise KeyError("enough")
+        shown.append(token)
+
+    s = llm.new_session()
+    with pytest.raises(KeyError):
+        s.generate_drafted(prompt, GenerationConfig(30), SessionDrafter(llm), drafts=4, on_token=on_token)
+    held = s.position()
+    assert len(prompt) <= held <= len(prompt) + len(shown)
+    assert shown == llm.new_session().generate(prompt, GenerationConfig(30))[:at]
+    ref = llm.new_session()
+    ref.prefill(prompt + shown[:held - len(prompt)])
+    assert close(s.decode_one(3), ref.decode_one(3), "float32")
+
+
 def test_drafted_sampling_draws_from_the_target(folder, small_folder):
     """The first two tokens over 600 seeds, by a drafter of another distribution: as often as the target's probabilities say.
     A count of 600 draws is within 4.5 standard deviations of its mean, sqrt(600 p (1 - p)) each, for all of some 20
