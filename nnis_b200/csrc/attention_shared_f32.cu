@@ -6,7 +6,7 @@
 // values of the outputs (sums over four keys at a time), so a product of four by four takes eight loads of 16 bytes.  Rows
 // beyond the last visible key are filled with zeros instead of read.  With 64 entries bound by the multiply-adds (1 us each of
 // scores and outputs a page and SM at heads of 64), with 16 by shared memory; both products are true float32.  16 rows of 9 heads
-// over 3 behind 2,000 tokens: 11.0 us the units of 64, 6.9 those of 16 beside them (the form for any head size: 19 and 16).
+// over 3 behind 2,000 tokens: 10.8 us the units of 64, 6.9 those of 16 beside them (the form for any head size: 19 and 16).
 #include "attention_shared.cuh"
 #include "fma_pairs.cuh"
 

@@ -20,7 +20,7 @@
 // Two CTAs an SM, so that one's softmax runs under the other's waits.  A page of 128 entries takes 1,095 clocks of an SM (2,190
 // with two CTAs), of which its 8,192 exponentials are 512; the tensor pipe is busy a fifth of the time.  To that come 5 to 8 us
 // a launch: set-up, queries from all over, the first page, records.  64 rows of 15 heads over 5 behind 16,384 tokens
-// (bytes 3.3 us, exponentials 3.4): 17.8 us; 16 sequences of 5 tokens, 32 heads of 128 over 8, behind 8,190: 23.9 us.  Tried and slower: one CTA an
+// (bytes 3.3 us, exponentials 3.4): 17.6 us; 16 sequences of 5 tokens, 32 heads of 128 over 8, behind 8,190: 23.9 us.  Tried and slower: one CTA an
 // SM with two tiles (256 entries) and 128 keys a step, 23.6 us where this took 20.2, 36 where it took 30.
 #include "attention_shared.cuh"
 #include "fma_pairs.cuh"

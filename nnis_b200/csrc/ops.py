@@ -2875,8 +2875,9 @@ class SharedPlan:
         at = ints.data_ptr()
         self.units, self.members = at, at + 32 * sum(counts)
         self.record = self.members + 4 * members
-        # rows merged by the CTA that completes them save a launch, where a CTA has little to merge: 2 rows of 3 units each
-        # 11.5 us instead of 13; where a unit's entries have much (8 rows of 14 records) its kernel takes 12 to 16 us for 7.4 and 4.1
+        # Rows merged by the CTA that completes them save a launch, which is what a small call by itself waits for: 2 rows of two
+        # records 9.4 us instead of 10.6, 4 of five 10.3 instead of 10.6, but 8 of 17 25 instead of 10.6.  On the device alone the
+        # merge kernel is the faster (5.2 us for 6.2, 6.7 for 9.4), so plans of captured steps leave it to that.
         self.merged_inside = most_entries * head_dim <= 1024 and counts[2] == 0 and (self.form != 1 or counts[0] == 0) \
             and sum(counts) * kv_heads <= 148 and records <= 8 * rows
         self.device, self.index, self.status = ints.device, ints.get_device(), status_word(ints.device).data_ptr()
