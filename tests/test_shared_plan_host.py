@@ -82,3 +82,15 @@ def test_chunks_fit_the_device_where_they_can():
                                                                           (128, 296, 2, 1 << 20, False)), 1)
     assert len(units[1]) * 32 <= 444 and sum(u[4] - u[3] for u in units[1].tolist()) == 62
     assert len(units[0]) == 24
+
+
+def test_entry_points_refuse_empty_records():
+    """Argument errors are found before anything is launched; numbers that no field holds are the caller's error."""
+    from nnis_b200.csrc import ops
+    for name, fields in ops._ENTRY_FIELDS.items():
+        call = ops._entry(name)
+        zeros = [0.0 if c == "f" else 0 for c in fields]
+        assert call(*zeros) == -1
+        for i, c in enumerate(fields):
+            with pytest.raises(ops.KernelError):
+                call(*zeros[:i], {"p": 1 << 64, "i": 1 << 31, "f": "one"}[c], *zeros[i + 1:])
