@@ -233,7 +233,7 @@ class EngineBackend:
                 gone = self._decoders.pop(shared[0])
                 self._views = {k: v for k, v in self._views.items() if k[0] != id(gone)}
         if key not in self._decoders:
-            self._decoders[key] = GraphDecoder(self.engine, *key)
+            self._decoders[key] = GraphDecoder(self.engine, *key[:3], rooms=rooms)
         return self._decoders[key]
 
     def _shared_decoder(self, slots: Sequence[int], positions: Sequence[int], max_context: int, want_logits: bool = False,

@@ -52,7 +52,7 @@ def chains_for(rows: int) -> int:
 
 class GraphDecoder:
     def __init__(self, engine, rows: int, max_context: int, want_logits: bool = False,
-                 rooms: Optional[tuple] = None, chains: Optional[int] = None):
+                 chains: Optional[int] = None, rooms: Optional[tuple] = None):
         self.engine = engine
         self.want_logits = want_logits
         self.rows = rows
