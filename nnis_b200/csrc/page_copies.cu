@@ -39,12 +39,24 @@ copy_pages_kernel(const __grid_constant__ PageMoves<N> moves, void* k, void* v, 
     const unsigned total = words * runs, step = gridDim.z * 256u;
     if (total == 0) return;
     constexpr int kAhead = 4;  // words a thread has on their way
+    unsigned at = blockIdx.z * 256u + threadIdx.x;
+    W word[kAhead];
+    if (runs == 1) {
+        for (; at < total; at += kAhead * step) {
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i)
+                if (at + i * step < total) word[i] = from[at + i * step];
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i)
+                if (at + i * step < total) to[at + i * step] = word[i];
+        }
+        return;
+    }
     // Where in a run a thread's next word lies follows from the last one's place: a division a word made the launch wait for its
     // instructions (63 forks' pages 12.9 us, without 12.0).
-    unsigned at = blockIdx.z * 256u + threadIdx.x, run = at / words, in_run = at - run * words;
+    unsigned run = at / words, in_run = at - run * words;
     const unsigned more_runs = step / words, more = step - more_runs * words;
     for (; at < total; at += kAhead * step) {
-        W word[kAhead];
         unsigned place[kAhead];  // (a page has less than 2^31 words)
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
