@@ -238,9 +238,10 @@ class EngineBackend:
 
     def _shared_decoder(self, slots: Sequence[int], positions: Sequence[int], max_context: int, want_logits: bool = False,
                         ahead: Optional[int] = None) -> GraphDecoder:
-        """The decoder of these sequences, whose pages have been reserved: one that reads what they share once, where that pays."""
+        """The decoder of these sequences, whose pages have been reserved: one that reads what they share once, where that
+        pays.  ``ahead``: pages that they will grow by before the caller asks again (None: it asks at every step)."""
         rows = self._decoder_key(len(slots), max_context, want_logits)[0]
-        units = self._shared.units(slots, positions, rows) if ahead is None else self._shared.units(slots, positions, rows, ahead)
+        units = self._shared.units(slots, positions, rows, ahead)
         dec = self._decoder(len(slots), max_context, want_logits, rooms_of(units))
         if units is not None:
             dec.plans.fill(units)

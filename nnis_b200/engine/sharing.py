@@ -18,7 +18,7 @@ from ..csrc import ops
 # 64, 8 behind 4 (15 MB) 5.2 -> 7.6, 4 behind 16 (25 MB) 10.2 -> 7.8, 2 behind 64 (34 MB) 15.5 -> 11; 32 over 8 of 128, 8 behind 16
 # (29 MB) 10.9 -> 13.4, 16 behind 16 (63 MB) 14.9 -> 10.8.
 LEAST_BYTES = 32 << 20
-AHEAD = 8  # pages that a captured step's plan lets its sequences grow by
+AHEAD = 8  # pages that the plan of a step which is looked at every time lets its sequences grow by
 
 PlanKey = Tuple[int, int, int, int]  # cache group, heads, key/value heads, head size
 
@@ -73,23 +73,26 @@ class KeptPlans:
 
 
 class BatchUnits:
-    """What a batch of single tokens shares, for captured steps: made anew when its sequences, what they share, or how
-    far they may grow have changed.  ``drafted``: the rows are tokens of one sequence, which share whatever they see alike."""
+    """What a batch of single tokens shares, for captured steps: made anew when its sequences or what they share have
+    changed, or when they grow beyond what it reaches.  ``drafted``: the rows are tokens of one sequence, which share whatever they see alike."""
 
     def __init__(self, engine, drafted: bool = False):
         self.engine, self.drafted = engine, drafted
         self._made_for = self._positions = self._units = None
         self._until = 0
 
-    def units(self, slots: Sequence[int], positions: Sequence[int], rows: int, ahead: int = AHEAD) -> Optional[Dict[PlanKey, tuple]]:
+    def units(self, slots: Sequence[int], positions: Sequence[int], rows: int, ahead: Optional[int] = None) -> Optional[Dict[PlanKey, tuple]]:
         """Per attention of the model that gains by it, its units, members and record offsets, for ``rows`` rows of which
-        the first are the sequences; None where none gains."""
+        the first are the sequences; None where none gains.  ``ahead``: they cover as many pages beyond these positions, for a
+        caller that does not ask again while its sequences grow; None: these positions, for one that asks at every step."""
         cache = self.engine.cache
         if not self.drafted and (len(slots) < 2 or not cache.shares_pages()):
             return None
         made_for = (tuple(slots), None if self.drafted else cache.share_epoch, rows)  # (a plan names columns of a table, not pages)
-        if made_for == self._made_for and all(0 <= now - then <= self._until for now, then in zip(positions, self._positions)):
+        reach = (ahead or 0) * PAGE_SIZE
+        if made_for == self._made_for and all(0 <= now - then <= self._until - reach for now, then in zip(positions, self._positions)):
             return self._units
+        ahead = AHEAD if ahead is None else ahead
         seqs, padding = list(range(len(slots))), rows - len(slots)
         trees: Dict[int, Optional[tuple]] = {}
         units = {}
