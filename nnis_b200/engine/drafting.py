@@ -11,6 +11,7 @@ from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
 
+from ..sampling import SplitMix64
 from ..sampling import device as device_sampling
 
 
@@ -51,14 +52,18 @@ class LookupDrafter:
 class SessionDrafter:
     """Drafts with a second, smaller model of the same vocabulary: an ``LLM`` of its own, a session of which follows the
     sequence.  With a temperature its tokens are drawn at that temperature, from a generator of the drafter's own
-    (``seed``), and come with their logits; greedy drafts are its likeliest tokens."""
+    (``seed``, of a stream that no policy's seed gives), and come with their logits; greedy drafts are its likeliest tokens."""
+
+    STREAM = 0x6472616674657273  # told apart from policies' seeds by it
 
     def __init__(self, llm, seed: int = 0):
         if llm.engine.cache.fixed_history():
             raise ValueError("a drafting model goes back over refused tokens: it keeps no state of fixed size and no window")
         self.llm = llm
         self.session = llm.new_session()
-        self._rng = device_sampling.seed_states([seed], llm.engine.device)
+        # The verification draws from SplitMix64 of the policy's seed.  With that state here the numbers that drew the drafts would
+        # decide about them, too, and what is kept would no longer be distributed as the target's: the state is one mixed from the seed.
+        self._rng = device_sampling.seed_states([SplitMix64(seed ^ self.STREAM).next_u64()], llm.engine.device)
         self._held: List[int] = []  # the tokens that the session has executed
 
     def begin(self) -> None:
