@@ -144,9 +144,11 @@ class EngineBackend:
         held = cache.length(slot)
         positions = list(range(held, held + n))
         cache.reserve([slot], [held + n])
-        rows = self._decoder_key(n, held + n, True)[0]
-        units = self._drafted.setdefault(n, BatchUnits(engine, drafted=True)).units([slot] * n, positions, rows)
-        dec = self._decoder(n, held + n, True, rooms_of(units))
+        key = self._decoder_key(n, held + n, True)
+        units = self._drafted.setdefault(n, BatchUnits(engine, drafted=True)).units([slot] * n, positions, key[0])
+        dec = self._captured((*key, rooms_of(units)))
+        if dec is None:
+            return engine.step([SequenceStep(slot, tokens, list(range(n)))], drafted=True)
         dec.plans.fill(units)
         self.h2d_bytes += dec.upload(tokens, positions, [slot] * n)
         dec.launch()
@@ -154,12 +156,12 @@ class EngineBackend:
         return dec.logits[:n]
 
     def _captured(self, key) -> Optional[GraphDecoder]:
-        """The decoder of this key with its graph, captured now.  Where that fails (no memory for its buffers, say) None,
-        and it is not tried again."""
+        """The decoder of this key with its graph, captured now if it has none.  Where that fails (no memory for its buffers,
+        say) None, and it is not tried again."""
+        if key in self._uncaptured:
+            return None
         try:
-            if key not in self._decoders:
-                self._decoders[key] = GraphDecoder(self.engine, *key)
-            self._decoders[key].capture()
+            self._made(key).capture()
         except RuntimeError as error:
             self._decoders.pop(key, None)
             self._uncaptured.add(key)
@@ -223,8 +225,11 @@ class EngineBackend:
 
     def _decoder(self, rows: int, max_context: int, want_logits: bool = False, rooms: Optional[tuple] = None) -> GraphDecoder:
         key = self._decoder_key(rows, max_context, want_logits)
-        if rooms is not None:
-            key = (*key, rooms)
+        return self._made(key if rooms is None else (*key, rooms))
+
+    def _made(self, key) -> GraphDecoder:
+        """The decoder of this key: (rows, positions, whether it gives logits) and, if sequences share pages, its plans' sizes."""
+        if len(key) > 3:
             # (what sequences share takes many forms: of the steps captured for it the least recently used goes)
             shared = [k for k in self._decoders if len(k) > 3]
             if key in self._decoders:
@@ -233,7 +238,7 @@ class EngineBackend:
                 gone = self._decoders.pop(shared[0])
                 self._views = {k: v for k, v in self._views.items() if k[0] != id(gone)}
         if key not in self._decoders:
-            self._decoders[key] = GraphDecoder(self.engine, *key[:3], rooms=rooms)
+            self._decoders[key] = GraphDecoder(self.engine, *key[:3], rooms=key[3] if len(key) > 3 else None)
         return self._decoders[key]
 
     def _shared_decoder(self, slots: Sequence[int], positions: Sequence[int], max_context: int, want_logits: bool = False,

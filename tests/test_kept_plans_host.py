@@ -131,3 +131,47 @@ def test_units_that_are_kept_reach_as_far_as_they_are_asked_to():
     assert reach(660, 16)[0] is again and reach(900)[0] is again and reach(660, 3)[0] is again
     further, end = reach(700, 16)
     assert further is not again and end >= 700 + 16 * PAGE_SIZE
+
+
+@pytest.mark.parametrize("fails", ["buffers", "capture"])
+def test_drafted_steps_that_cannot_be_captured_are_launched_kernel_by_kernel(monkeypatch, fails):
+    """No memory for a captured step's buffers, or for its graph: a warning, the step by the engine, and no second try."""
+    from nnis_b200.engine import api
+    engine = make_engine()
+    tries, steps = [], []
+
+    class Fails:
+        graph = None
+
+        def __init__(self, *a, **k):
+            tries.append(1)
+            if fails == "buffers":
+                raise torch.cuda.OutOfMemoryError("out of memory")
+            self.plans = SimpleNamespace(fill=lambda units: None)
+
+        def upload(self, *a):
+            return 0
+
+        def capture(self):
+            raise RuntimeError("out of memory")
+
+        launch = capture
+
+    def step(batch, drafted=False):
+        assert drafted
+        steps.append([(s.slot, list(s.tokens), list(s.want)) for s in batch])
+        engine.step_in_portions(batch, 100)
+        return "logits"
+
+    monkeypatch.setattr(api, "GraphDecoder", Fails)
+    engine.step = step
+    backend = EngineBackend(engine)
+    slot = engine.acquire_slot()
+    engine.cache.reserve([slot], [100])
+    engine.cache.commit([slot], [100])
+    with pytest.warns(RuntimeWarning, match="could not be captured"):
+        assert backend.drafted_logits(slot, [1, 2, 3], True) == "logits"
+    assert backend.drafted_logits(slot, [4, 5, 6], True) == "logits"
+    assert steps == [[(slot, [1, 2, 3], [0, 1, 2])], [(slot, [4, 5, 6], [0, 1, 2])]]
+    assert len(tries) == 1 and not backend._decoders and engine.cache.length(slot) == 106
+    engine.cache.check()
