@@ -45,8 +45,9 @@ struct SharedArgs {
     int beside;          // 1: the launch before this one is of the same call and runs beside it
 };
 
-// Programmatic dependent launch among the units' kernels of a call: the first waits for the kernel before the call (queries, and
-// this step's keys and values) before it lets the second start, so the second need not wait to begin, only to end: whoever
+// Programmatic dependent launch among the units' kernels of a call: the first waits for the kernel before the call (queries, this
+// step's keys and values, and as a caller may write them there, too, positions and page tables; ahead of it only the plan is read, which
+// is copied from the host) before it lets the second start, so the second need not wait to begin, only to end: whoever
 // waits for it then waits for both.
 __device__ __forceinline__ void units_begin(const SharedArgs& a) {
     if (!a.beside) pdl_wait();

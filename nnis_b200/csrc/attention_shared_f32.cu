@@ -25,12 +25,12 @@ attn_shared_f32_kernel(const SharedArgs a) {
     float* p_s = v_s + kSharedPage * D;         // [tile, 68]
     const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
     const SharedUnit u = a.units[blockIdx.x];
+    units_begin(a);
     const int hk = blockIdx.y, G = a.nq / a.nkv;
     const int* members = a.members + u.members;
     const int* table = a.page_table + (size_t)u.seq * a.table_cols;
     const int pos = u.ends ? a.token_pos[u.ends - 1] : 0x7fffffff;
     const int n_pages = min(a.table_cols, u.ends ? min(u.page_end, pos < 0 ? 0 : pos / kSharedPage + 1) : u.page_end);
-    units_begin(a);
 
     auto keys_of = [&](int it, int page) {  // keys of a page that the unit's rows see (0 where the table has a gap)
         return page < 0 || page >= a.pages ? 0 : u.ends ? min(kSharedPage, pos + 1 - it * kSharedPage) : kSharedPage;

@@ -33,9 +33,8 @@ attn_shared_mma_kernel(const SharedArgs a) {
     bf16* tiles = q_s + kSmEntries * D;             // stages x (K [64, D], V [64, D])
     __shared__ float sm_ml[kSmWarps][kSmEntries][2];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    // The plan, the positions and the page ids are older than the kernel before this one, which writes the queries and this
-    // step's keys and values: they are asked for ahead of the wait for it, the ids beside the position.
-    const SharedUnit u = a.units[blockIdx.x];
+    const SharedUnit u = a.units[blockIdx.x];  // (the plan comes from the host: it is asked for ahead of the wait)
+    units_begin(a);
     const int hk = blockIdx.y, G = a.nq / a.nkv;
     const int* members = a.members + u.members;
     const int* table = a.page_table + (size_t)u.seq * a.table_cols + u.page_begin;
@@ -43,7 +42,6 @@ attn_shared_mma_kernel(const SharedArgs a) {
     const int ids = lane < some ? table[lane] : -1;  // a lane a page, up to 32 of them
     const int pos = u.ends ? a.token_pos[u.ends - 1] : 0x7fffffff;
     const int n_pages = u.ends ? min(some, pos < 0 ? 0 : pos / kSharedPage + 1 - u.page_begin) : some;
-    units_begin(a);
     const bool two = u.entries > 16;  // the second tile of 16 entries holds any
     const bf16 *k_cache = static_cast<const bf16*>(a.k_cache), *v_cache = static_cast<const bf16*>(a.v_cache);
     constexpr size_t kTile = (size_t)kSharedPage * D;

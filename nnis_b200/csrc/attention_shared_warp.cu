@@ -45,8 +45,7 @@ attn_shared_warp_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
     const int r_lo = lane >> 2, c_lo = (lane & 3) * 2;
     const float sc = a.scale * kLog2e;
 
-    // What is known of an item ahead of its turn; the plan, the positions and the page ids are older than the kernel before
-    // this one (which writes the queries and this step's keys and values).
+    // What is known of an item ahead of its turn.
     struct Item {
         SharedUnit u;
         int hk, ids, pos, pages;
@@ -80,9 +79,10 @@ attn_shared_warp_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
     auto at = [&](unsigned char* tile, int row, int chunk) { return tile + (chunk >> 3) * kChunk + row * 128 + (((chunk & 7) ^ (row & 7)) << 4); };
 
     int i = warp * gridDim.x + blockIdx.x;  // (neighbouring items go to different SMs)
-    Item now = look(unit_of(i), i);
+    const SharedUnit u_first = unit_of(i);  // (the plan comes from the host: it is asked for ahead of the wait)
     SharedUnit u_next = unit_of(i + stride);
     units_begin(a);
+    Item now = look(u_first, i);
     uint32_t k_turn = 0, v_turn = 0;
     int n_pages = i < n_items ? pages_of(now) : 0;
     bool ok = true, asked = false;  // whether this item's first page is on its way

@@ -1,0 +1,46 @@
+"""Attention over shared pages, called as a program may call it: right behind the kernels that write what it reads."""
+import math
+
+import pytest
+import torch
+
+from test_attention_shared_gpu import build, check
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+def ops():
+    from nnis_b200.csrc import ops as o
+    return o
+
+
+FORMS = [(9, 3, 64, torch.bfloat16, 3), (32, 32, 64, torch.bfloat16, 40), (8, 2, 64, torch.bfloat16, 40), (16, 2, 128, torch.bfloat16, 9),
+         (9, 3, 64, torch.float32, 9), (6, 2, 128, torch.float32, 20), (6, 3, 48, torch.bfloat16, 5), (4, 1, 96, torch.float32, 9)]
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,dtype,members", FORMS)
+def test_positions_and_page_tables_written_by_the_kernel_before(heads, kv_heads, dim, dtype, members):
+    """Positions by a kernel that lets the next one start before it has written them, page tables just before that: every form sees
+    what they wrote, call after call.  (Positions are right only in that kernel's results: one behind them before it, and tables
+    name the wrong pages.)"""
+    from nnis_b200.engine.workspace import Workspace
+    o, held = ops(), {}
+    tables, seqs, positions, pages = build(12, [5], members, 1, [2, 65, 130])
+
+    def keep(go):
+        held.update(zip(go.__code__.co_freevars, (c.cell_contents for c in go.__closure__)))
+        pos, table, n = held["pos"], held["table"], len(positions)
+        pos0, table0 = pos - 1, table.flip(0).contiguous()
+        real_pos, real_table = pos.clone(), table.clone()
+        none = torch.zeros(n, dtype=torch.int32, device=DEV)
+        for _ in range(20):
+            held["out"].fill_(77.0)
+            pos.copy_(pos0)
+            table.copy_(table0)
+            table.copy_(real_table)
+            o.advance(none.clone(), pos, none)
+            go()
+        assert torch.equal(pos, real_pos)
+
+    check(tables, seqs, positions, pages, heads, kv_heads, dim, dtype, seed=5, call=keep)
