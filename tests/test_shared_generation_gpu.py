@@ -34,33 +34,32 @@ def logits_alone(llm, prompt, emitted):
 
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 @pytest.mark.parametrize("last", [1, 9])
-def test_greedy_steps_far_behind_a_shared_prompt(folder, dtype, last):
+def test_greedy_steps_far_behind_a_shared_prompt(folder, dtype, last, monkeypatch):
     """Prompts that differ in their last token (or nine) and 700 tokens after them, eleven pages: every step's logits, and the
     tokens picked from them."""
     from nnis_b200 import LLM
     from nnis_b200.csrc import ops
+    from nnis_b200.engine.api import EngineBackend
+    from nnis_b200.engine.decode import GraphDecoder
     llm = LLM(folder, dtype=dtype, max_tokens=1 << 14, max_batch=8)
     document = tokens(2, 1100)
     prompts = [document + [7 + i] * last for i in range(5)]
-    steps, used, real, made = [], [], ops.attention_shared, llm.backend._decoder
+    steps, used, real, made, launch = [], [], ops.attention_shared, EngineBackend._decoder, GraphDecoder.launch
 
-    def with_logits(rows, max_context, want_logits=False, rooms=None):
-        dec = made(rows, max_context, True, rooms)
-        if max_context > 1200:  # the generation's
-            launch = dec.launch
-            dec.launch = lambda: (launch(), steps.append(dec.logits[:5].cpu().numpy()))
-        return dec
+    def launch_and_keep(dec):
+        launch(dec)
+        steps.append(dec.logits[:5].cpu().numpy())
 
-    llm.backend._decoder = with_logits
-    ops.attention_shared = lambda *a: (used.append(1), real(*a))[1]
-    try:
-        results = llm.generate(prompts, max_new_tokens=700, share_prefix=True, stop_token_ids=[])
-    finally:
-        ops.attention_shared = real
-    assert used and all(r.ok and len(r.token_ids) == 700 for r in results) and len(steps) == 699
+    # (of the classes, so that no model outlives the test in a cycle)
+    monkeypatch.setattr(EngineBackend, "_decoder", lambda self, rows, context, want=False, rooms=None: made(self, rows, context, True, rooms))
+    monkeypatch.setattr(GraphDecoder, "launch", launch_and_keep)
+    monkeypatch.setattr(ops, "attention_shared", lambda *a: (used.append(1), real(*a))[1])
+    results = llm.generate(prompts, max_new_tokens=700, share_prefix=True, stop_token_ids=[])
+    assert used and all(r.ok and len(r.token_ids) == 700 for r in results)
+    assert len(steps) == 699 + (last == 1)  # (one token of a prompt's own runs as such a step, too)
     limit = F32_REL_TO_MAX if dtype == "float32" else BF16_REL_TO_MAX
     for row, (prompt, r) in enumerate(zip(prompts, results)):
-        want, got = logits_alone(llm, prompt, r.token_ids)[1:], np.stack([s[row] for s in steps])
+        want, got = logits_alone(llm, prompt, r.token_ids)[1:], np.stack([s[row] for s in steps[-699:]])
         off = np.abs(got - want).max(axis=1) / np.maximum(1.0, np.abs(want).max(axis=1))
         assert off.max() <= limit, (row, int(off.argmax()), float(off.max()))
         assert (got.argmax(axis=1) == r.token_ids[1:]).all()
