@@ -34,6 +34,7 @@ attn_shared_any_kernel(const SharedArgs a) {
     const int pos = u.ends ? a.token_pos[u.ends - 1] : 0x7fffffff;
     const int n_pages = min(a.table_cols, u.ends ? min(u.page_end, pos < 0 ? 0 : pos / kSharedPage + 1) : u.page_end);
     const int* table = a.page_table + (size_t)u.seq * a.table_cols;
+    if (tid == 0) units_end_check(a, u, pos);
     const T* q = static_cast<const T*>(a.q);
 
     for (int i = tid; i < kTile * ds; i += kAnyThreads) {
@@ -238,7 +239,7 @@ NNIS_API int nnis_attention_shared(const void* call) {
     const uintptr_t all = (uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache;
     if (all % (form ? 16 : f32 ? 8 : 4) || (uintptr_t)out % (f32 ? 8 : 4) || (form && q_stride % (f32 ? 4 : 8))) return NNIS_ERR_ALIGNMENT;
     SharedArgs a = {q,       k_cache, v_cache, token_pos, page_table, reinterpret_cast<const SharedUnit*>(units), members, record,
-                    partial, sums,    tickets, out,       q_stride,   table_cols, pages,   nq,     nkv, d, scale, 0};
+                    partial, sums,    tickets, out,       q_stride,   table_cols, pages,   nq,     nkv, d, scale, status, 0};
     // (the large units first: the small ones end what is left of the device)
     const SharedUnit* first = a.units;
     for (int kind = 2; kind >= 0; --kind) {
@@ -247,9 +248,9 @@ NNIS_API int nnis_attention_shared(const void* call) {
         a.units = first + (kind == 2 ? n0 + n1 : kind == 1 ? n0 : 0);
         const cudaError_t e = form == 0   ? shared_units_any(a, n, kind == 1 ? 64 : 16, f32, stream)
                               : form == 2 ? shared_units_f32(a, n, kind == 1 ? 64 : 16, stream)
-                              : kind == 2 ? shared_units_tc(a, n, status, stream)
+                              : kind == 2 ? shared_units_tc(a, n, stream)
                                           : kind == 1 ? shared_units_mma(a, n, stream)
-                                          : shared_units_warp(a, n, status, stream);
+                                          : shared_units_warp(a, n, stream);
         if (e != cudaSuccess) return (int)e;
         a.beside = 1;
     }

@@ -42,6 +42,7 @@ struct SharedArgs {
     void* out;           // [tokens, nq, d]
     int q_stride, table_cols, pages, nq, nkv, d;
     float scale;
+    int* status;         // see units_end_check; null: nobody is told
     int beside;          // 1: the launch before this one is of the same call and runs beside it
 };
 
@@ -55,6 +56,13 @@ __device__ __forceinline__ void units_begin(const SharedArgs& a) {
 }
 __device__ __forceinline__ void units_end(const SharedArgs& a) {
     if (a.beside) pdl_wait();
+}
+
+// A unit that ends a row's pages and does not reach the row's position (the row has gone on beyond what its plan was made for) tells the
+// status word: the keys behind it are not seen.  One thread's work.
+__device__ __forceinline__ void units_end_check(const SharedArgs& a, const SharedUnit& u, int pos) {
+    if (u.ends && pos >= 0 && pos / kSharedPage >= u.page_end && a.status && a.record[u.ends - 1] + u.slot + 1 == a.record[u.ends])
+        atomicExch(a.status, 2);
 }
 
 // 2^x for a weight: one that would be denormal is zero (exp2f keeps it, by four instructions instead of one).
@@ -183,8 +191,8 @@ __device__ __forceinline__ void merge_finished(const SharedArgs& a, const Shared
 // One launch of the named form over `n_units` units; each is defined in its own file.
 cudaError_t shared_units_any(const SharedArgs& a, int n_units, int tile, bool f32, cudaStream_t stream);
 cudaError_t shared_units_f32(const SharedArgs& a, int n_units, int tile, cudaStream_t stream);
-cudaError_t shared_units_warp(const SharedArgs& a, int n_units, int* status, cudaStream_t stream);
+cudaError_t shared_units_warp(const SharedArgs& a, int n_units, cudaStream_t stream);
 cudaError_t shared_units_mma(const SharedArgs& a, int n_units, cudaStream_t stream);
-cudaError_t shared_units_tc(const SharedArgs& a, int n_units, int* status, cudaStream_t stream);
+cudaError_t shared_units_tc(const SharedArgs& a, int n_units, cudaStream_t stream);
 
 }  // namespace nnis

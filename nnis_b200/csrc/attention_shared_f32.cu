@@ -31,6 +31,7 @@ attn_shared_f32_kernel(const SharedArgs a) {
     const int* table = a.page_table + (size_t)u.seq * a.table_cols;
     const int pos = u.ends ? a.token_pos[u.ends - 1] : 0x7fffffff;
     const int n_pages = min(a.table_cols, u.ends ? min(u.page_end, pos < 0 ? 0 : pos / kSharedPage + 1) : u.page_end);
+    if (tid == 0) units_end_check(a, u, pos);
 
     auto keys_of = [&](int it, int page) {  // keys of a page that the unit's rows see (0 where the table has a gap)
         return page < 0 || page >= a.pages ? 0 : u.ends ? min(kSharedPage, pos + 1 - it * kSharedPage) : kSharedPage;

@@ -42,6 +42,7 @@ attn_shared_mma_kernel(const SharedArgs a) {
     const int ids = lane < some ? table[lane] : -1;  // a lane a page, up to 32 of them
     const int pos = u.ends ? a.token_pos[u.ends - 1] : 0x7fffffff;
     const int n_pages = u.ends ? min(some, pos < 0 ? 0 : pos / kSharedPage + 1 - u.page_begin) : some;
+    if (tid == 0) units_end_check(a, u, pos);
     const bool two = u.entries > 16;  // the second tile of 16 entries holds any
     const bf16 *k_cache = static_cast<const bf16*>(a.k_cache), *v_cache = static_cast<const bf16*>(a.v_cache);
     constexpr size_t kTile = (size_t)kSharedPage * D;

@@ -73,8 +73,7 @@ __device__ __forceinline__ uint64_t sh_desc_v(uint32_t addr) {
 
 template <int D>
 __global__ void __launch_bounds__(kShThreads, 2)
-attn_shared_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const SharedArgs a,
-                      int* __restrict__ status) {
+attn_shared_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const SharedArgs a) {
     constexpr int C = D / 64, kStages = sh_stages<D>();
     constexpr uint32_t kPageBytes = C * kShChunkK, kCols = 256;
     // tensor memory: S, two buffers of 64 columns; P, 32 columns a buffer; O
@@ -324,7 +323,7 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         tc_fence_before();
     }
     __syncthreads();
-    if (abort_flag && threadIdx.x == 0 && status) atomicExch(status, 1);
+    if (abort_flag && threadIdx.x == 0 && a.status) atomicExch(a.status, 1);
     if (warp == 1) {
         tc_fence_after();
         tmem_dealloc(tmem, kCols);
@@ -332,7 +331,7 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
 }
 
 template <int D>
-static cudaError_t launch_tc(const SharedArgs& a, int n_units, int* status, cudaStream_t stream) {
+static cudaError_t launch_tc(const SharedArgs& a, int n_units, cudaStream_t stream) {
     CUtensorMap map_k, map_v;
     const long long rows = (long long)a.pages * a.nkv * kSharedPage;
     if (!make_map(&map_k, a.k_cache, rows, D, kSharedPage) || !make_map(&map_v, a.v_cache, rows, D, kSharedPage))
@@ -342,11 +341,11 @@ static cudaError_t launch_tc(const SharedArgs& a, int n_units, int* status, cuda
     static std::atomic<int> held[16];
     const cudaError_t e = allow_shared(kernel, smem, held);
     if (e != cudaSuccess) return e;
-    return launch_dependent(kernel, dim3(n_units, a.nkv), kShThreads, smem, stream, map_k, map_v, a, status);
+    return launch_dependent(kernel, dim3(n_units, a.nkv), kShThreads, smem, stream, map_k, map_v, a);
 }
 
-cudaError_t shared_units_tc(const SharedArgs& a, int n_units, int* status, cudaStream_t stream) {
-    return a.d == 64 ? launch_tc<64>(a, n_units, status, stream) : launch_tc<128>(a, n_units, status, stream);
+cudaError_t shared_units_tc(const SharedArgs& a, int n_units, cudaStream_t stream) {
+    return a.d == 64 ? launch_tc<64>(a, n_units, stream) : launch_tc<128>(a, n_units, stream);
 }
 
 }  // namespace nnis

@@ -22,7 +22,7 @@ constexpr int wp_warps() { return D == 64 ? 12 : 6; }
 template <int D>
 __global__ void __launch_bounds__(wp_warps<D>() * 32, 1)
 attn_shared_warp_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const SharedArgs a,
-                        int n_items, int* __restrict__ status) {
+                        int n_items) {
     constexpr int C = D / 64, NT = D / 8, KS = D / 16, W = wp_warps<D>();
     constexpr uint32_t kBytes = kSharedPage * D * 2, kChunk = kSharedPage * 128;  // of a page's K or V, of 64 columns of it
     extern __shared__ __align__(1024) unsigned char smem_raw[];
@@ -90,6 +90,7 @@ attn_shared_warp_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
         const Item next = look(u_next, i + stride);
         u_next = unit_of(i + 2 * stride);
         const int next_pages = i + stride < n_items ? pages_of(next) : 0;
+        if (lane == 0) units_end_check(a, now.u, now.pos);
         const int* members = a.members + now.u.members;
         if (n_pages > 0 && !asked) {
             const int page = id_of(now, 0);
@@ -222,14 +223,14 @@ attn_shared_warp_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_
     if (!ok) {  // no copy may land after the CTA has left
         mbar_wait(k_bar, k_turn);
         mbar_wait(v_bar, v_turn);
-        if (lane == 0 && status) atomicExch(status, 1);
+        if (lane == 0 && a.status) atomicExch(a.status, 1);
     }
     __syncthreads();
     units_end(a);
 }
 
 template <int D>
-static cudaError_t launch_warp(const SharedArgs& a, int n_units, int* status, cudaStream_t stream) {
+static cudaError_t launch_warp(const SharedArgs& a, int n_units, cudaStream_t stream) {
     CUtensorMap map_k, map_v;
     const long long rows = (long long)a.pages * a.nkv * kSharedPage;
     if (!make_map(&map_k, a.k_cache, rows, D, kSharedPage) || !make_map(&map_v, a.v_cache, rows, D, kSharedPage))
@@ -241,11 +242,11 @@ static cudaError_t launch_warp(const SharedArgs& a, int n_units, int* status, cu
     const cudaError_t e = allow_shared(kernel, smem, held);
     if (e != cudaSuccess) return e;
     const int items = n_units * a.nkv, sms = device_sms();
-    return launch_dependent(kernel, dim3(items < sms ? items : sms), W * 32, smem, stream, map_k, map_v, a, items, status);
+    return launch_dependent(kernel, dim3(items < sms ? items : sms), W * 32, smem, stream, map_k, map_v, a, items);
 }
 
-cudaError_t shared_units_warp(const SharedArgs& a, int n_units, int* status, cudaStream_t stream) {
-    return a.d == 64 ? launch_warp<64>(a, n_units, status, stream) : launch_warp<128>(a, n_units, status, stream);
+cudaError_t shared_units_warp(const SharedArgs& a, int n_units, cudaStream_t stream) {
+    return a.d == 64 ? launch_warp<64>(a, n_units, stream) : launch_warp<128>(a, n_units, stream);
 }
 
 }  // namespace nnis

@@ -475,7 +475,8 @@ _status = {}
 
 
 def status_word(device) -> torch.Tensor:
-    """One int32 per device that kernels set when a bounded wait runs out."""
+    """One int32 per device that kernels set when a bounded wait runs out (1), or where a plan of shared pages ends before one of its
+    rows does (2)."""
     key = torch.device(device).index or 0
     if key not in _status:
         _status[key] = torch.zeros(1, dtype=torch.int32, device=device)
@@ -483,11 +484,13 @@ def status_word(device) -> torch.Tensor:
 
 
 def check_status(device) -> None:
-    """Raise if a kernel gave up a wait since the last check (synchronises)."""
+    """Raise if a kernel gave up a wait, or met a plan too short, since the last check (synchronises)."""
     word = status_word(device)
-    if int(word.item()) != 0:
+    why = int(word.item())
+    if why != 0:
         word.zero_()
-        raise KernelError("a kernel gave up waiting for an asynchronous copy; results are invalid")
+        raise KernelError("attention_shared: a row's position lies beyond the pages of its plan; results are invalid" if why == 2 else
+                          "a kernel gave up waiting for an asynchronous copy; results are invalid")
 
 
 def gemv_grid(m: int, n: int, k: int, device) -> int:
@@ -2865,7 +2868,7 @@ def memory_finish(o_raw: torch.Tensor, a: torch.Tensor, gate_off: int, weight: t
 class SharedPlan:
     """What ``attention_shared`` works through for a batch whose sequences share pages (see ``shared_plan``): good as long as
     its rows stay at the positions that it was made for and their page lists do not change (and, made with pages
-    ``ahead``, while they grow by no more)."""
+    ``ahead``, while they grow by no more: a row that has grown beyond the end of its plan sets the status word)."""
 
     def __init__(self, rows, heads, kv_heads, head_dim, dtype, counts, members, ints, records, seqs, cols,
                  most_entries=1 << 20):

@@ -44,3 +44,40 @@ def test_positions_and_page_tables_written_by_the_kernel_before(heads, kv_heads,
         assert torch.equal(pos, real_pos)
 
     check(tables, seqs, positions, pages, heads, kv_heads, dim, dtype, seed=5, call=keep)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,dtype,members", FORMS)
+def test_a_row_beyond_the_end_of_its_plan_sets_the_status_word(heads, kv_heads, dim, dtype, members):
+    """One row of a batch a page behind what its plan was made for; at the plan's own positions, on its last page and for padding rows
+    nothing is set.  (Tables and store have the page: nothing is out of range.)"""
+    from nnis_b200.engine.workspace import Workspace
+    o = ops()
+    tables, seqs, positions, pages = build(13, [5], members, 1, [2, 65, 130])
+    plan = o.attention_shared_plan(tables, seqs, positions, heads, kv_heads, dim, dtype, DEV)
+    k = torch.randn((pages, kv_heads, 64, dim), device=DEV).to(dtype)
+    q = torch.randn((len(seqs), heads * dim), device=DEV).to(dtype)
+    table = torch.zeros((len(tables), 12), dtype=torch.int32)
+    for i, t in enumerate(tables):
+        table[i, :len(t)] = torch.tensor(t)
+    table, out = table.to(DEV), torch.empty_like(q)
+
+    def run(at):
+        o.attention_shared(q, heads * dim, k, k, torch.tensor(at, dtype=torch.int32, device=DEV), table, plan, out, heads, kv_heads, dim,
+                           0.1, Workspace(torch.device(DEV)))
+
+    o.check_status(DEV)
+    run(positions)
+    o.check_status(DEV)
+    run([p // 64 * 64 + 63 for p in positions])
+    run([-1] * len(positions))
+    o.check_status(DEV)
+    padded = o.attention_shared_plan(tables, seqs, [-1, *positions[1:-1], -1], heads, kv_heads, dim, dtype, DEV)
+    o.attention_shared(q, heads * dim, k, k, torch.tensor([-1, *positions[1:-1], -1], dtype=torch.int32, device=DEV), table, padded, out,
+                       heads, kv_heads, dim, 0.1, Workspace(torch.device(DEV)))
+    o.check_status(DEV)
+    for row in (0, len(positions) - 1):
+        run([p // 64 * 64 + 64 if r == row else p for r, p in enumerate(positions)])
+        with pytest.raises(o.KernelError, match="beyond the pages of its plan"):
+            o.check_status(DEV)
+        o.check_status(DEV)
+    assert math.isfinite(float(out.float().sum()))
