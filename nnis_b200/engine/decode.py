@@ -32,7 +32,7 @@ from ..cache import PAGE_SIZE
 from ..csrc import ops
 from .context import StepContext, sm_count
 from .sharing import KeptPlans
-from .workspace import Workspace
+from .workspace import Workspace, recording
 
 
 def chains_for(rows: int) -> int:
@@ -168,7 +168,7 @@ class GraphDecoder:
             ctx.workspace.frozen = True
         graph = torch.cuda.CUDAGraph()
         before = ops.launch_count()
-        with torch.cuda.graph(graph):
+        with recording(graph):
             self._body()
         self.launches_per_step = ops.launch_count() - before
         self.graph = graph

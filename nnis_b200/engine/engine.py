@@ -29,7 +29,7 @@ from ..weights.loader import shape_fits
 from .context import StepContext
 from .model import DecoderModel
 from .sharing import SharedRows
-from .workspace import Workspace
+from .workspace import Workspace, recording
 
 GRAPH_MIN_TOKENS = 256  # prompt steps at least this large are captured when they recur
 MAX_STEP_GRAPHS = 4     # captured prompt steps kept (each holds buffers of its own)
@@ -350,7 +350,7 @@ class Engine:
         result = logits.clone()
         workspace.frozen = True
         graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(graph):
+        with recording(graph):
             self.model.forward(ctx, d_want, logits)
         self.cache.commit(slots, new_lengths)
         self._seen_shapes.pop(key, None)

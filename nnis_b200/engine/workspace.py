@@ -7,9 +7,25 @@ holds the old address.
 """
 from __future__ import annotations
 
+import contextlib
+import gc
 from typing import Dict, Tuple
 
 import torch
+
+
+@contextlib.contextmanager
+def recording(graph: torch.cuda.CUDAGraph):
+    """Records what is launched into ``graph``.  Python's collector waits meanwhile: an object that it finds then may hold a graph
+    of its own (a model that was left in a cycle), and to free one is not permitted while a stream records."""
+    collects = gc.isenabled()
+    gc.disable()
+    try:
+        with torch.cuda.graph(graph):
+            yield
+    finally:
+        if collects:
+            gc.enable()
 
 
 class Workspace:
