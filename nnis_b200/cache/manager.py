@@ -34,6 +34,7 @@ crates/nnis-rt/src/kv_cache.rs:368-395).
 """
 from __future__ import annotations
 
+import contextlib
 from dataclasses import dataclass
 from typing import Dict, List, Optional, Sequence, Tuple, Union
 
@@ -143,6 +144,7 @@ class CacheManager:
         # counts what happened to pages that several tables hold (shared, parted with, given back, moved): while it
         # stands still, sequences share what they shared
         self.share_epoch = 0
+        self._in_place = 0  # callers for which held pages stay where they are (see ``in_place``)
         self.owners: List[int] = [0] * max_slots  # how many sequences have held each slot
         self.groups: List[_KVGroup] = []
         self._views: List[Optional[Union[KVView, StateView]]] = []
@@ -454,10 +456,23 @@ class CacheManager:
         """Whether any page is held by more than one sequence."""
         return any(g.extra for g in self.groups)
 
+    @contextlib.contextmanager
+    def in_place(self):
+        """While it lasts ``compact`` is refused: for a caller whose steps read pages by lists that nothing brings up to date, as those
+        of a sequence are that has ended and that others still share pages with."""
+        self._in_place += 1
+        try:
+            yield
+        finally:
+            self._in_place -= 1
+
     def compact(self) -> List[int]:
         """The held pages of every group move to its lowest places, so that they are ``[:, :held]`` of its storage:
         returns how many pages have moved in each.  One launch a group, on the current stream; page lists that a
-        program has copied are out of date."""
+        program has copied are out of date.  Refused, with nothing moved, from within a greedy generation of sequences that
+        share pages (a callback of it)."""
+        if self._in_place:
+            raise SlotError("pages cannot move while a generation whose sequences share them runs")
         moved = []
         for g in self.groups:
             held = g.pool.held

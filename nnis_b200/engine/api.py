@@ -12,6 +12,7 @@ used here in process.
 """
 from __future__ import annotations
 
+import contextlib
 import warnings
 from typing import Callable, Dict, List, Optional, Sequence, Union
 
@@ -264,6 +265,13 @@ class EngineBackend:
             dec = self._shared_decoder(slots, positions, longest, ahead=max(left for *_, left in rows) // PAGE_SIZE + 1)
         else:
             dec = self._decoder(len(rows), longest)
+        # (shared pages are read by the table of the first of their sequences, which stays as it is when that one ends)
+        with cache.in_place() if dec.plans is not None else contextlib.nullcontext():
+            self._greedy_steps(dec, rows, emit)
+
+    def _greedy_steps(self, dec: GraphDecoder, rows, emit) -> None:
+        """``decode_greedy`` by the given decoder."""
+        cache = self.engine.cache
         live = {}
         for r, (i, slot, token, pos, left) in enumerate(rows):
             dec.set_row(r, slot, token, pos)

@@ -5,7 +5,7 @@ from types import SimpleNamespace
 import pytest
 import torch
 
-from nnis_b200.cache import PAGE_SIZE, CacheManager, KVRequest
+from nnis_b200.cache import PAGE_SIZE, CacheManager, KVRequest, SlotError
 from nnis_b200.csrc import ops
 from nnis_b200.engine import sharing
 from nnis_b200.engine.api import EngineBackend
@@ -175,3 +175,48 @@ def test_drafted_steps_that_cannot_be_captured_are_launched_kernel_by_kernel(mon
     assert steps == [[(slot, [1, 2, 3], [0, 1, 2])], [(slot, [4, 5, 6], [0, 1, 2])]]
     assert len(tries) == 1 and not backend._decoders and engine.cache.length(slot) == 106
     engine.cache.check()
+
+
+@pytest.mark.parametrize("share", [True, False])
+def test_pages_stay_where_they_are_while_a_generation_shares_them(share):
+    """A callback that compacts the cache after the sequence has ended by whose table the others read what they share: refused, with
+    nothing moved; without shared pages, and afterwards, they move."""
+    engine = make_engine()
+    cache = engine.cache
+
+    class Plain(Recorder):
+        def launch(self):
+            self.reach = {r: 1 << 20 for r in range(self.rows)}
+            super().launch()
+
+    class AnyBackend(Backend):
+        def _decoder(self, rows, max_context, want_logits=False, rooms=None):
+            made = (Recorder if rooms else Plain)(self._decoder_key(rows, max_context, want_logits)[0])
+            if not rooms:
+                made.plans = None
+            return made
+
+    first = cache.acquire()  # (its pages lie in front of the generation's, and are given back in the middle of it)
+    cache.reserve([first], [300])
+    cache.commit([first], [300])
+    seen, refused, moved = [0] * 4, [], []
+
+    def on_token(i, token):
+        seen[i] += 1
+        if i == 1 and seen[i] == 20:
+            cache.release(first)
+            before = [list(t) for t in cache.groups[0].tables.values()]
+            try:
+                moved.append(cache.compact())
+            except SlotError:
+                refused.append(before == [list(t) for t in cache.groups[0].tables.values()])
+
+    prompt = [i % VOCAB for i in range(1001)]
+    requests = [GenerationRequest(prompt + [i], GenerationConfig(5 if i == 0 else 40)) for i in range(4)]
+    results = Generator(AnyBackend(engine), VOCAB, 1 << 14, 8, 1 << 15).generate(requests, on_token, share_prefix=share)
+    assert [r.error for r in results] == [None] * 4
+    assert (refused, len(moved)) == (([True], 0) if share else ([], 1))
+    slot = cache.acquire()
+    assert cache.compact() == [0] and cache.usage()["pages_held"] == [0]
+    cache.release(slot)
+    cache.check()
