@@ -157,7 +157,7 @@ verify_rows_kernel(const float* __restrict__ logits, const float* __restrict__ d
     int lo = 0, hi = n_seqs - 1;
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
-        if (first_row[mid] - (of_draft ? mid : 0) <= (of_draft ? r - rows : r)) lo = mid;
+        if (first_row[mid] <= (of_draft ? r - rows + mid : r)) lo = mid;
         else hi = mid - 1;
     }
     const float t = temperature[lo];
@@ -287,12 +287,14 @@ verify_pick_kernel(const float* __restrict__ logits, const float* __restrict__ d
         s.last = -1;
     }
     // (What the call was given is older than the first launch, which has waited for it: it is read under that launch's end.)
-    const int row0 = first_row[b], draft0 = row0 - b, count = first_row[b + 1] - row0 - 1;
+    const int row0 = first_row[b], row_end = first_row[b + 1];
+    // (compared, not subtracted: offsets may be any numbers; good ones leave as many draft rows as there are drafts)
+    const bool good = row0 >= b && row_end > row0 && row_end <= rows && row_end - b <= rows - (int)gridDim.y + 1;
+    const int draft0 = good ? row0 - b : 0, count = good ? row_end - row0 - 1 : 0;
     const float t = temperature[b];
     const bool greedy = !(t > 0.f);
     const float c = scale_of(t);
     const double inv_t = greedy ? 1.0 : 1.0 / (double)t;
-    const bool good = row0 >= b && count >= 0 && row0 + count < rows && draft0 + count <= rows - (int)gridDim.y;
     // A warp's draft: its logits in the two rows.
     struct Draft {
         int id;
@@ -311,7 +313,7 @@ verify_pick_kernel(const float* __restrict__ logits, const float* __restrict__ d
         }
         return x;
     };
-    Draft mine = draft_of(good ? warp : count);
+    Draft mine = draft_of(warp);
     cluster.sync();  // (all of the cluster run: their shared memory may be written)
     pdl_wait();
     pdl_launch_dependents();
