@@ -8,6 +8,7 @@
 #include <stdint.h>
 
 #include <atomic>
+#include <mutex>
 
 #define NNIS_OK 0
 // Negative codes are argument errors found on the host before any launch;
@@ -105,14 +106,18 @@ inline int device_sms() {
 }
 
 // Lets `kernel` have `bytes` of dynamic shared memory on the current device; `held` (16 zeros of the caller's, one place a device)
-// is what it may have already, so that the driver is asked once and not at every launch.
+// is what it may have already, so that the driver is asked once and not at every launch.  Threads that ask for different sizes of one
+// kernel take turns: the smaller one set last would refuse the other's launch.
 template <typename Kernel>
 inline cudaError_t allow_shared(Kernel kernel, size_t bytes, std::atomic<int>* held) {
     int device = 0;
     cudaError_t e = cudaGetDevice(&device);
-    if (e != cudaSuccess || (device < 16 && held[device].load(std::memory_order_relaxed) >= (int)bytes)) return e;
+    if (e != cudaSuccess || (device < 16 && held[device].load(std::memory_order_acquire) >= (int)bytes)) return e;
+    static std::mutex turns;
+    const std::lock_guard<std::mutex> turn(turns);
+    if (device < 16 && held[device].load(std::memory_order_relaxed) >= (int)bytes) return cudaSuccess;
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-    if (e == cudaSuccess && device < 16) held[device].store((int)bytes, std::memory_order_relaxed);
+    if (e == cudaSuccess && device < 16) held[device].store((int)bytes, std::memory_order_release);
     return e;
 }
 

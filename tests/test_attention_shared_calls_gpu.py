@@ -81,3 +81,46 @@ def test_a_row_beyond_the_end_of_its_plan_sets_the_status_word(heads, kv_heads, 
             o.check_status(DEV)
         o.check_status(DEV)
     assert math.isfinite(float(out.float().sum()))
+
+
+def test_two_threads_at_once():
+    """Two head sizes of one kernel, each on a stream and a workspace of its own, as often as one alone: the same to the bit."""
+    import threading
+    from nnis_b200.engine.workspace import Workspace
+    o, work = ops(), []
+    for seed, dim in ((1, 30), (2, 62)):
+        tables, seqs, positions, pages = build(20 + seed, [5], 6, 1, [2, 65, 130])
+        g = torch.Generator(device=DEV).manual_seed(seed)
+        k = torch.randn((pages, 2, 64, dim), generator=g, device=DEV)
+        q = torch.randn((len(seqs), 6 * dim), generator=g, device=DEV)
+        cols = max(map(len, tables))
+        table = torch.tensor([t + [-1] * (cols - len(t)) for t in tables], dtype=torch.int32, device=DEV)
+        at = torch.tensor(positions, dtype=torch.int32, device=DEV)
+        plan = o.attention_shared_plan(tables, seqs, positions, 6, 2, dim, torch.float32, DEV)
+        ws = Workspace(torch.device(DEV))
+        work.append(lambda out, q=q, k=k, at=at, table=table, plan=plan, dim=dim, ws=ws:
+                    o.attention_shared(q, 6 * dim, k, k, at, table, plan, out, 6, 2, dim, 0.1, ws))
+        work[-1].like = q
+    got, errors = [[], []], []
+
+    def run(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream(DEV)):
+                for _ in range(30):
+                    got[i].append(torch.empty_like(work[i].like))
+                    work[i](got[i][-1])
+                torch.cuda.current_stream().synchronize()
+        except Exception as error:
+            errors.append(error)
+
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=run, args=(i,)) for i in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    for i in (0, 1):
+        want = torch.empty_like(work[i].like)
+        work[i](want)
+        assert all(torch.equal(x, want) for x in got[i])
