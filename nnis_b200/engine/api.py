@@ -525,6 +525,7 @@ class InferenceSession:
             room = min(drafts, generation.max_new_tokens - len(emitted) - 1)
             proposed, logits_of = drafter.propose(told, room, verifier.temperature) if room > 0 else ([], None)
             proposed = list(proposed)[:room]
+            logits_of = logits_of[:len(proposed)] if proposed and logits_of is not None else None
             feed = [token, *proposed]
 
     def _generate(self, input_ids, generation, sampling, on_token, keep_context) -> List[int]:

@@ -41,3 +41,56 @@ def test_a_drafter_of_the_policys_seed_draws_numbers_of_its_own(offset):
         for place in range(3):
             counts[place, tokens[place]] += 1
     assert (np.abs(counts / n - p) <= 4.5 * np.sqrt(p * (1 - p) / n)).all(), counts / n
+
+
+class FakeSession:
+    """``InferenceSession.generate_drafted`` over a model that continues every token by the next number."""
+
+    def __init__(self, monkeypatch, vocab=50):
+        from nnis_b200.engine import api
+        self.length, self.seen = 0, []
+        row = lambda tokens: torch.nn.functional.one_hot(torch.tensor([(t + 1) % vocab for t in tokens]), vocab).float()
+
+        def step(batch):
+            s, = batch
+            self.length += len(s.tokens)
+            return row([s.tokens[w] for w in s.want]) if s.want else None
+
+        def drafted(slot, tokens, again):
+            self.length += len(tokens)
+            return row(tokens)
+
+        def verify(verifier, logits, drafts, draft_logits):
+            self.seen.append((len(drafts), None if draft_logits is None else tuple(draft_logits.shape)))
+            picks = logits.argmax(1).tolist()
+            kept = next((i for i, d in enumerate(drafts) if d != picks[i]), len(drafts))
+            return kept, picks[kept]
+
+        engine = SimpleNamespace(cache=SimpleNamespace(fixed_history=lambda: False, length=lambda slot: self.length),
+                                 spec=SimpleNamespace(vocab_size=vocab, max_positions=1000), device=torch.device("cpu"), workspace=None,
+                                 acquire_slot=lambda: 0, release_slot=lambda slot: setattr(self, "length", 0), step=step,
+                                 truncate=lambda slot, n: setattr(self, "length", n))
+        backend = SimpleNamespace(drafted_logits=drafted, decode_logits=lambda slot, token, again: drafted(slot, [token], again)[0])
+        monkeypatch.setattr(api.device_sampling.DraftVerifier, "verify", verify)
+        self.session = api.InferenceSession(SimpleNamespace(engine=engine, backend=backend,
+                                                            _generator=SimpleNamespace(refusal=lambda request: None)))
+
+
+@pytest.mark.parametrize("surplus", [0, 3])
+@pytest.mark.parametrize("wrong", [False, True])
+def test_drafts_beyond_the_room_are_dropped_with_their_logits(monkeypatch, surplus, wrong):
+    """A drafter that gives more tokens than it was asked for, each with its logits, or none but logits all the same."""
+    from nnis_b200 import GenerationConfig
+
+    class Drafter:
+        begin = lambda self: None
+
+        def propose(self, tokens, count, temperature):
+            n = count + surplus if len(tokens) % 3 else 0
+            drafts = [(tokens[-1] + 1 + i + (i == 1 and wrong)) % 50 for i in range(n)]
+            return drafts, torch.zeros((count + surplus, 50))
+
+    fake = FakeSession(monkeypatch)
+    got = fake.session.generate_drafted([5], GenerationConfig(17), Drafter(), drafts=4)
+    assert got == list(range(6, 23)) and fake.length == 18
+    assert any(n for n, _ in fake.seen) and all(n <= 4 and shape == ((n, 50) if n else None) for n, shape in fake.seen)
