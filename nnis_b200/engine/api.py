@@ -477,7 +477,11 @@ class InferenceSession:
             raise ValueError(f"drafts must be positive; got {drafts}")
         if sampling is not None and (sampling.top_k is not None or sampling.top_p is not None):
             raise ValueError("drafted generation samples with a temperature only (no top_k, no top_p)")
-        other = getattr(getattr(drafter, "llm", None), "spec", None)
+        llm = getattr(drafter, "llm", None)
+        there = getattr(getattr(llm, "engine", None), "device", self.engine.device)
+        if (there.index or 0) != (self.engine.device.index or 0):
+            raise ValueError(f"the drafting model is on {there}, this one on {self.engine.device}")
+        other = getattr(llm, "spec", None)
         if other is not None and other.vocab_size != self.engine.spec.vocab_size:
             raise ValueError(f"the drafting model has {other.vocab_size} tokens, this one {self.engine.spec.vocab_size}")
         if not keep_context:

@@ -50,8 +50,8 @@ class LookupDrafter:
 
 
 class SessionDrafter:
-    """Drafts with a second, smaller model of the same vocabulary: an ``LLM`` of its own, a session of which follows the
-    sequence.  With a temperature its tokens are drawn at that temperature, from a generator of the drafter's own
+    """Drafts with a second, smaller model of the same vocabulary on the same device: an ``LLM`` of its own, a session of which
+    follows the sequence.  With a temperature its tokens are drawn at that temperature, from a generator of the drafter's own
     (``seed``, of a stream that no policy's seed gives), and come with their logits; greedy drafts are its likeliest tokens."""
 
     STREAM = 0x6472616674657273  # told apart from policies' seeds by it

@@ -124,3 +124,24 @@ def test_two_threads_at_once():
         want = torch.empty_like(work[i].like)
         work[i](want)
         assert all(torch.equal(x, want) for x in got[i])
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,dtype,members", FORMS)
+def test_the_same_call_gives_the_same_bits(heads, kv_heads, dim, dtype, members):
+    """No order of units, records or merges changes a result, and neither does what the workspace held."""
+    from nnis_b200.engine.workspace import Workspace
+    o = ops()
+    tables, seqs, positions, pages = build(14, [9], members, 2, [2, 65, 130])
+    plan = o.attention_shared_plan(tables, seqs, positions, heads, kv_heads, dim, dtype, DEV)
+    k, v = (torch.randn((pages, kv_heads, 64, dim), device=DEV).to(dtype) for _ in range(2))
+    q = (2.0 * torch.randn((len(seqs), heads * dim), device=DEV)).to(dtype)
+    cols = max(map(len, tables))
+    table = torch.tensor([t + [-1] * (cols - len(t)) for t in tables], dtype=torch.int32, device=DEV)
+    at, ws, first = torch.tensor(positions, dtype=torch.int32, device=DEV), Workspace(torch.device(DEV)), None
+    for turn in range(30):
+        out = torch.full_like(q, 77.0)
+        if turn:
+            ws.room("attn_shared_records", 1, torch.float32).fill_(math.nan if turn % 2 else 3.0)
+        o.attention_shared(q, heads * dim, k, v, at, table, plan, out, heads, kv_heads, dim, 0.1, ws)
+        first = out if first is None else first
+        assert torch.equal(out, first)

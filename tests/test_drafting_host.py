@@ -94,3 +94,20 @@ def test_drafts_beyond_the_room_are_dropped_with_their_logits(monkeypatch, surpl
     got = fake.session.generate_drafted([5], GenerationConfig(17), Drafter(), drafts=4)
     assert got == list(range(6, 23)) and fake.length == 18
     assert any(n for n, _ in fake.seen) and all(n <= 4 and shape == ((n, 50) if n else None) for n, shape in fake.seen)
+
+
+def test_a_drafting_model_on_another_device_is_refused(monkeypatch):
+    """Its kernels would be launched on this one's: the current device is the model's that runs."""
+    from nnis_b200 import GenerationConfig
+    fake = FakeSession(monkeypatch)
+    fake.session.engine.device = torch.device("cuda:0")
+    monkeypatch.setattr("nnis_b200.engine.api.device_sampling.DraftVerifier.__init__", lambda self, *a: setattr(self, "temperature", 0.0))
+    drafter = drafter_of(0)
+    drafter.llm.spec = SimpleNamespace(vocab_size=50)
+    drafter.llm.engine.device = torch.device("cuda:1")
+    with pytest.raises(ValueError, match="cuda:1"):
+        fake.session.generate_drafted([5], GenerationConfig(4), drafter)
+    assert fake.length == 0 and not fake.seen
+    drafter.llm.engine.device = torch.device("cuda")  # (the first, however it is named)
+    drafter.begin, drafter.propose = lambda: None, lambda tokens, count, temperature: ([], None)
+    assert fake.session.generate_drafted([5], GenerationConfig(4), drafter) == [6, 7, 8, 9]
