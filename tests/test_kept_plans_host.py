@@ -93,6 +93,7 @@ def make_engine(max_tokens=1 << 15):
 @pytest.fixture(autouse=True)
 def share_whatever_can_be(monkeypatch):
     monkeypatch.setattr(sharing, "LEAST_BYTES", 1)
+    monkeypatch.setattr(sharing, "PAGE_COST", {})
     monkeypatch.setattr(ops, "sm_count", lambda device: 148)
 
 

@@ -65,3 +65,40 @@ def test_greedy_steps_far_behind_a_shared_prompt(folder, dtype, last, monkeypatc
         assert (got.argmax(axis=1) == r.token_ids[1:]).all()
     llm.engine.check_status()
     assert llm.engine.cache.usage()["pages_held"] == [0]
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("name", ["A", "B", "C"])
+def test_other_head_sizes_read_shared_pages_once(tmp_path, name, dtype, monkeypatch):
+    """Forked sequences of other head layouts, where the rule of what pays would have them read row by row: captured steps' logits
+    are those of sequences of their own."""
+    from helpers import CONFIGS
+    from nnis_b200 import LLM
+    from nnis_b200.csrc import ops
+    from nnis_b200.engine import SequenceStep, sharing
+    monkeypatch.setattr(sharing, "PAGE_COST", {})
+    used, real = [], ops.attention_shared
+    monkeypatch.setattr(ops, "attention_shared", lambda *a: (used.append(1), real(*a))[1])
+    vocab = CONFIGS[name]["vocab_size"]
+    llm = LLM(make_model(str(tmp_path), {**CONFIGS[name], "max_position_embeddings": 2048}, 11), dtype=dtype, max_tokens=1 << 14, max_batch=8)
+    engine, limit = llm.engine, F32_REL_TO_MAX if dtype == "float32" else BF16_REL_TO_MAX
+    document = tokens(3, 1000, vocab)
+    first = engine.acquire_slot()
+    engine.step([SequenceStep(first, document, [])])
+    slots = [first] + [engine.fork(first) for _ in range(4)]
+    history = {s: list(document) for s in slots}
+    for turn in range(70):
+        new = tokens(200 + turn, 5, vocab)
+        logits = llm.backend.step([SequenceStep(s, [t], [0]) for s, t in zip(slots, new)])
+        for s, t in zip(slots, new):
+            history[s].append(t)
+        if turn in (0, 24, 25, 69):
+            got, other = logits.float().cpu().numpy(), engine.acquire_slot()
+            for r, s in enumerate(slots):
+                engine.release_slot(other)
+                other = engine.acquire_slot()
+                want = engine.step([SequenceStep(other, history[s], [len(history[s]) - 1])])[0].cpu().numpy()
+                assert np.abs(got[r] - want).max() <= limit * max(1.0, float(np.abs(want).max())), (turn, r)
+            engine.release_slot(other)
+    assert used
+    engine.check_status()
