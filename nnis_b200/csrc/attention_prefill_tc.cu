@@ -58,11 +58,6 @@ constexpr float kTcLog2e = 1.4426950408889634f;
 constexpr int kTcPartial = kTcD + 2;  // floats per row of a chunk's result: O, maximum, sum
 constexpr float kTcRaise = 8.0f;  // log2 of how far a page's maximum may exceed the one in use
 
-__device__ __forceinline__ float max3(float a, float b, float c) {
-    float d;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-    return d;
-}
 
 // 2^x for x <= 0 or so; -inf gives 0, denormal results are flushed
 __device__ __forceinline__ float ex2(float x) {

@@ -10,6 +10,7 @@
 // merge 3.3 more; 24 rows of 32 heads behind each of two prompts of 4,001 tokens (65 MB): 24.0 us.
 // P is rounded to bfloat16 for the tensor cores (2^-9 of a weight, of either sign), sums are of the 32-bit weights.
 #include "attention_shared.cuh"
+#include "fma_pairs.cuh"
 #include "mma_helpers.cuh"
 
 namespace nnis {
@@ -18,11 +19,6 @@ constexpr int kSmWarps = 4, kSmThreads = kSmWarps * 32;
 
 template <int D>
 constexpr int sm_stages() { return D == 64 ? 4 : 3; }
-
-// 16 bytes, or zeros where there is nothing to read (src is any valid address then)
-__device__ __forceinline__ void cp_async16_or_zero(void* dst, const void* src, bool there) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(dst)), "l"(src), "r"(there ? 16 : 0) : "memory");
-}
 
 template <int D>
 __global__ void __launch_bounds__(kSmThreads, D == 64 ? 3 : 2)
@@ -62,8 +58,8 @@ attn_shared_mma_kernel(const SharedArgs a) {
             for (int i = 0; i < kSharedPage * CH / kSmThreads; ++i) {
                 const int c = tid + i * kSmThreads, row = c / CH, chunk = c % CH;
                 const bool there = row < keys;
-                cp_async16_or_zero(kd + swz<D>(row, chunk), k_cache + from + (there ? (size_t)c * 8 : 0), there);
-                cp_async16_or_zero(vd + swz<D>(row, chunk), v_cache + from + (there ? (size_t)c * 8 : 0), there);
+                copy16_or_zero(kd + swz<D>(row, chunk), k_cache + from + (there ? (size_t)c * 8 : 0), there);
+                copy16_or_zero(vd + swz<D>(row, chunk), v_cache + from + (there ? (size_t)c * 8 : 0), there);
             }
         }
         cp_async_commit();

@@ -14,8 +14,7 @@
 //              soon as the last have been read; with 128, where O takes those columns, over the scores.
 // P is rounded to bfloat16 because the tensor cores take it so (2^-9 of a weight, of either sign); sums are of the 32-bit
 // weights.  O stays in tensor memory; the maximum that P is taken against is only raised when a page exceeds it by
-// more than 8 (a factor 256, harmless in both types), then the warps wait for the products so far and multiply O.
-// Every wait is bounded; one that runs out raises an abort flag, all warps meet at the end and tensor memory is freed.
+// more than 8 (a factor 256, harmless in both types), then the warps wait for the products so far and multiply O.  // Every wait is bounded; one that runs out raises an abort flag, all warps meet at the end and tensor memory is freed.
 //
 // Two CTAs an SM, so that one's softmax runs under the other's waits.  A page of 128 entries takes 1,095 clocks of an SM (2,190
 // with two CTAs), of which its 8,192 exponentials are 512; the tensor pipe is busy a fifth of the time.  To that come 5 to 8 us
@@ -35,11 +34,6 @@ constexpr float kShRaise = 8.0f;
 template <int D>
 constexpr int sh_stages() { return D == 64 ? 4 : 2; }
 
-__device__ __forceinline__ float sh_max3(float a, float b, float c) {
-    float d;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-    return d;
-}
 __device__ __forceinline__ bool sh_wait(uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); }
 
 __device__ __forceinline__ void sh_store16(uint32_t taddr, const uint32_t (&v)[16]) {
@@ -243,7 +237,7 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
 #pragma unroll
             for (int c = 0; c < 32; c += 8)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) mx[e] = sh_max3(mx[e], __uint_as_float(sv[c + 2 * e]), __uint_as_float(sv[c + 2 * e + 1]));
+                for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], __uint_as_float(sv[c + 2 * e]), __uint_as_float(sv[c + 2 * e + 1]));
             const float mine = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
             half_max[b][half][row] = mine;
             tc_fence_before();

@@ -62,11 +62,6 @@ __device__ __forceinline__ float wide_ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ float wide_max3(float a, float b, float c) {
-    float d;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-    return d;
-}
 
 // Wait of a thread that has nothing else to do: it may stay suspended for up to two microseconds per try.  False after
 // `limit` tries (a quarter of a second).
@@ -410,8 +405,8 @@ attn_wide_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             for (int c = 0; c < 32; c += 4)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    mx[e] = wide_max3(mx[e], __uint_as_float(sa[c + 2 * e]), __uint_as_float(sa[c + 2 * e + 1]));
-                    mx[2 + e] = wide_max3(mx[2 + e], __uint_as_float(sb[c + 2 * e]), __uint_as_float(sb[c + 2 * e + 1]));
+                    mx[e] = max3(mx[e], __uint_as_float(sa[c + 2 * e]), __uint_as_float(sa[c + 2 * e + 1]));
+                    mx[2 + e] = max3(mx[2 + e], __uint_as_float(sb[c + 2 * e]), __uint_as_float(sb[c + 2 * e + 1]));
                 }
             const float m_new = fmaxf(m_run, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc);
             const bool raise = m_run != -INFINITY && m_new > m_run + kWideRaise;

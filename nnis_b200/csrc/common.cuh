@@ -93,6 +93,12 @@ __device__ __forceinline__ float warp_max(float v) {
     return v;
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
 // Whether kernels are launched as programmatic dependents of the kernel before them
 // (NNIS_PDL=0 turns it off everywhere); defined in elementwise.cu.
 bool dependent_launches();

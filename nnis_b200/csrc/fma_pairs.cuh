@@ -35,7 +35,7 @@ __device__ __forceinline__ unsigned long long pair_of(float a, float b) {
 }
 
 // 16 bytes to shared memory, or 16 zero bytes where the source does not exist (`src` is any valid address then).
-__device__ __forceinline__ void copy16_or_zero(float* dst, const float* src, bool there) {
+__device__ __forceinline__ void copy16_or_zero(void* dst, const void* src, bool there) {
     const uint32_t to = (uint32_t)__cvta_generic_to_shared(dst);
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
