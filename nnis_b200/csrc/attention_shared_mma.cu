@@ -8,7 +8,7 @@
 // Bound by the bytes of K and V where units are many (three CTAs an SM, pages of three more ahead each), by a unit's trips to memory
 // (plan, page id, page, records: 3.5 us for a page) where they are few.  8 rows of 9 heads over 3 behind 4,032 tokens: 8.5 us, the
 // merge 3.3 more; 24 rows of 32 heads behind each of two prompts of 4,001 tokens (65 MB): 24.0 us.
-// P is rounded to bfloat16 for the tensor cores (2^-9 of a weight, of either sign), sums are of the 32-bit weights.
+// P is rounded to bfloat16 for the tensor cores (up to 2^-8 of a weight, of either sign), sums are of the 32-bit weights.
 #include "attention_shared.cuh"
 #include "fma_pairs.cuh"
 #include "mma_helpers.cuh"

@@ -8,7 +8,7 @@
 // (six at 128 values) warps an SM that is 192 KB on its way.  Scores and outputs are mma.sync products, a warp has all keys of
 // its page, and nothing is shared among warps.  Bound by the bytes of K and V: 51 rows of 32 heads, tails of one to five pages and three
 // long ones (188 MB), 37 us, 5.1 TB/s.
-// P is rounded to bfloat16 for the tensor cores (2^-9 of a weight, of either sign), sums are of the 32-bit weights.
+// P is rounded to bfloat16 for the tensor cores (up to 2^-8 of a weight, of either sign), sums are of the 32-bit weights.
 // Every wait is bounded; a warp whose wait runs out sets the status word and leaves.
 #include "attention_shared.cuh"
 #include "mma_helpers.cuh"

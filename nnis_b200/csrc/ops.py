@@ -2882,7 +2882,7 @@ class SharedPlan:
         # records 9.4 us instead of 10.6, 4 of five 10.3 instead of 10.6, but 8 of 17 25 instead of 10.6.  On the device alone the
         # merge kernel is the faster (5.2 us for 6.2, 6.7 for 9.4), so plans of captured steps leave it to that.
         self.merged_inside = most_entries * head_dim <= 1024 and counts[2] == 0 and (self.form != 1 or counts[0] == 0) \
-            and sum(counts) * kv_heads <= 148 and records <= 8 * rows
+            and sum(counts) * kv_heads <= sm_count(ints.device) and records <= 8 * rows
         self.device, self.index, self.status = ints.device, ints.get_device(), status_word(ints.device).data_ptr()
         self.code, self.item = _DTYPE_CODE[dtype], dtype.itemsize
         self.launches = (not self.merged_inside) + sum(c > 0 for c in counts)
@@ -2922,9 +2922,11 @@ def attention_shared_units(nodes, tails, seqs, heads: int, kv_heads: int, head_d
     sms = sm_count(device)
     form = _shared_form(dtype, head_dim)
     if form == 1:
-        # Small units go warp by warp where they are many (64 rows of a page each, 32 heads: 21 -> 15.5 us); else that is only a
-        # launch more.  From 33 entries on tcgen05: units of 17 to 32 there took two prompts' 24 rows 54 us as mma.sync's 56, but
-        # 8 rows of 3 heads 15.8 for 13.6.
+        # Small units go warp by warp, dealt to the warps by turns, where they are many (64 rows of a page each, 32 heads: 21 -> 15.5
+        # us); else that is only a launch more.  From 33 entries on tcgen05: units of 17 to 32 there took two prompts' 24 rows 54 us as
+        # mma.sync's 56, but 8 rows of 3 heads 15.8 for 13.6; 33 to 64 entries take (us, tcgen05 and mma.sync) 14.2 and 14.6 with
+        # 33 of 9 heads over 3 behind 256 pages, 9.4 and 9.1 behind 64, 15.5 and 19.4 with 48 of 15 over 5, 23.0 and 41.0 with 36 of 32
+        # over 8 of 128, 13.0 and 17.3 with 33 of 32 over 32 behind 16 pages.
         pieces = sum(len(rows) * (heads // kv_heads) <= 16 for rows, *_ in nodes) + (len(tails) if heads // kv_heads <= 16 else 0)
         kinds = ((16 if pieces * kv_heads > 2 * sms else 0, 12 * sms, 1, 16, True), (32, 3 * sms, 4, 16, False),
                  (128, 2 * sms, 2, 1 << 20, False))

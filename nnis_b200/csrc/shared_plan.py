@@ -77,9 +77,9 @@ def shared_units(nodes: Sequence[tuple], tails: Sequence[tuple], seqs: Sequence[
                  kinds: Sequence[tuple], ending: int):
     """(units of every kind [*, 8], members, record offsets [rows + 1]).
 
-    ``kinds``: (most entries of a unit, CTAs of the kind that the device holds at once, fewest and most pages of a chunk, whether
-    the device takes units from a queue), entries ascending, 0 where the kernel has no such kind; ``ending``: the last kind that takes units whose rows end inside
-    them."""
+    ``kinds``: (most entries of a unit, CTAs of the kind that the device holds at once, or warps of a kind that goes warp by warp,
+    fewest and most pages of a chunk, whether each of those takes several units in turn), entries ascending, 0 where the kernel
+    has no such kind; ``ending``: the last kind that takes units whose rows end inside them."""
     pieces = []  # (rows, first, end, ends, kind)
     total = [0] * len(kinds)
     for rows, a, b, ends in [(*n, 0) for n in nodes] + [([r], a, b, 1 + r) for r, a, b in tails]:
@@ -89,13 +89,14 @@ def shared_units(nodes: Sequence[tuple], tails: Sequence[tuple], seqs: Sequence[
         pieces.append((rows, a, b, ends, kind))
         total[kind] += -(-entries // kinds[kind][0]) * (b - a) * kv_heads
     # pages of a chunk: as few as leave no more CTAs of the kind than it has at once (a few more would run by themselves), or,
-    # from a queue, an even share of all pages
+    # of units dealt in turn, an even share of all pages
     share = [1] * len(kinds)
-    for i, (tile, ctas, least, most, queue) in enumerate(kinds):
+    for i, (tile, ctas, least, most, dealt) in enumerate(kinds):
         mine = [(b - a, -(-len(rows) * group // tile) * kv_heads) for rows, a, b, _, kind in pieces if kind == i]
         if mine:
             share[i] = min(most, max(least, -(-total[i] // ctas)))
-            while not queue and share[i] < min(most, max(n for n, _ in mine)) and sum(-(-n // share[i]) * tiles for n, tiles in mine) > ctas:
+            while not dealt and share[i] < min(most, max(n for n, _ in mine)) and \
+                    sum(-(-n // share[i]) * tiles for n, tiles in mine) > ctas:
                 share[i] += 1 + share[i] // 16
             share[i] = min(share[i], most)
     units: List[List[tuple]] = [[] for _ in kinds]
