@@ -102,3 +102,39 @@ def test_other_head_sizes_read_shared_pages_once(tmp_path, name, dtype, monkeypa
             engine.release_slot(other)
     assert used
     engine.check_status()
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_a_step_of_many_drafted_sequences(folder, dtype):
+    """Forked sequences and one of its own with two to six tokens each in one step, wanted places in any order: the logits of steps
+    that do not share, and what follows them."""
+    from nnis_b200 import LLM
+    from nnis_b200.engine import SequenceStep
+    llm = LLM(folder, dtype=dtype, max_tokens=1 << 14, max_batch=16)
+    engine, limit = llm.engine, F32_REL_TO_MAX if dtype == "float32" else BF16_REL_TO_MAX
+    first, lone = engine.acquire_slot(), engine.acquire_slot()
+    history = {first: tokens(80, 830), lone: tokens(81, 100)}
+    for s, h in history.items():
+        engine.step([SequenceStep(s, h, [])])
+    for _ in range(3):
+        new = engine.fork(first)
+        history[new] = list(history[first])
+    for turn in range(4):
+        batch, want = [], []
+        for i, s in enumerate(history):
+            fresh = tokens(900 + 10 * turn + i, 2 + (i + turn) % 5)
+            places = list(range(len(fresh)))[::-1 if i % 2 else 1]
+            batch.append(SequenceStep(s, fresh, places))
+            other = engine.acquire_slot()
+            want.append(engine.step([SequenceStep(other, history[s] + fresh, [len(history[s]) + p for p in places])]).cpu().numpy())
+            engine.release_slot(other)
+        got = engine.step(batch, drafted=True).cpu().numpy()
+        want = np.concatenate(want)
+        assert got.shape == want.shape
+        assert (np.abs(got - want).max(axis=1) <= limit * np.maximum(1.0, np.abs(want).max(axis=1))).all()
+        for i, s in enumerate(batch):
+            keep = len(s.tokens) - i % 2
+            history[s.slot] += s.tokens[:keep]
+            engine.truncate(s.slot, len(history[s.slot]))
+        engine.cache.check()
+    engine.check_status()
