@@ -16,7 +16,7 @@
 // weights.  O stays in tensor memory; the maximum that P is taken against is only raised when a page exceeds it by
 // more than 8 (a factor 256, harmless in both types), then the warps wait for the products so far and multiply O.  So the largest
 // weight is not the 1 that it is against the running maximum, and is rounded too: 0.0023 of the outputs' norm from 64 bits, where the
-// mma.sync units' are 0.0018 and the outputs' own rounding is 0.0017.
+// mma.sync units' are 0.0017 to 0.0019 and the outputs' own rounding is 0.0017.
 // Every wait is bounded; one that runs out raises an abort flag, all warps meet at the end and tensor memory is freed.
 //
 // Two CTAs an SM, so that one's softmax runs under the other's waits.  A page of 128 entries takes 1,095 clocks of an SM (2,190

@@ -221,3 +221,26 @@ def test_pages_stay_where_they_are_while_a_generation_shares_them(share):
     assert cache.compact() == [0] and cache.usage()["pages_held"] == [0]
     cache.release(slot)
     cache.check()
+
+
+@pytest.mark.parametrize("tokens", [2, 5, 64])
+def test_drafted_steps_are_captured_whatever_the_batch(monkeypatch, tokens):
+    """A model for one sequence (``max_batch=1``) takes a token and its drafts by a captured step."""
+    from nnis_b200.engine import api
+    engine = make_engine()
+    monkeypatch.setattr(api, "GraphDecoder", lambda engine, rows, context, want_logits, rooms: made.append(rows) or Drafted(rows))
+    made, launched = [], []
+
+    class Drafted(Recorder):
+        graph, capture = None, lambda self: None
+
+        def launch(self):
+            launched.append(dict(self.positions))
+            self.logits = torch.zeros((self.rows, VOCAB))
+
+    backend = EngineBackend(engine, 1)
+    slot = engine.acquire_slot()
+    engine.cache.reserve([slot], [100])
+    engine.cache.commit([slot], [100])
+    assert backend.drafted_logits(slot, [3] * tokens, True).shape == (tokens, VOCAB)
+    assert launched == [{r: 100 + r for r in range(tokens)}] and made[0] >= tokens
