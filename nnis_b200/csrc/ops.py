@@ -2966,7 +2966,8 @@ def attention_shared(q: torch.Tensor, q_stride: int, k_cache: torch.Tensor, v_ca
                      page_table: torch.Tensor, plan: SharedPlan, out: torch.Tensor, heads: int, kv_heads: int, head_dim: int,
                      scale: float, workspace) -> None:
     """Causal attention of packed query tokens over the paged cache, pages that several rows share read once for all of them.
-    ``plan``: ``attention_shared_plan`` of the same rows, positions and page lists."""
+    ``plan``: ``attention_shared_plan`` of the same rows, positions and page lists.  All tensors may be written by the kernel
+    right before; a row that lies beyond the pages of its plan is answered without the keys there and sets the status word."""
     n, d, dtype, index = plan.rows, plan.head_dim, plan.dtype, plan.index
     shape, q_shape, table_shape = k_cache.shape, q.shape, page_table.shape
     if not (heads == plan.heads and kv_heads == plan.kv_heads and head_dim == d and len(shape) == 4 and shape[1] == kv_heads
