@@ -145,3 +145,13 @@ def test_the_same_call_gives_the_same_bits(heads, kv_heads, dim, dtype, members)
         o.attention_shared(q, heads * dim, k, v, at, table, plan, out, heads, kv_heads, dim, 0.1, ws)
         first = out if first is None else first
         assert torch.equal(out, first)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,dtype", [(4, 1, 64, torch.bfloat16), (2, 2, 128, torch.bfloat16), (4, 1, 64, torch.float32),
+                                                      (2, 1, 16, torch.bfloat16)])
+def test_thousands_of_rows(heads, kv_heads, dim, dtype):
+    """2,000 sequences behind two pages; 300 tokens of one sequence, the same position twice among them."""
+    tables, seqs, positions, pages = build(15, [2], 2000, 0, [1, 40, 64, 70])
+    check(tables, seqs, positions, pages, heads, kv_heads, dim, dtype, seed=6)
+    positions = [399 - i for i in range(299)] + [399]
+    check([list(range(7))], [0] * 300, positions, 7, heads, kv_heads, dim, dtype, seed=7)

@@ -138,3 +138,22 @@ def test_a_step_of_many_drafted_sequences(folder, dtype):
             engine.truncate(s.slot, len(history[s.slot]))
         engine.cache.check()
     engine.check_status()
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_sampled_tokens_behind_a_shared_prompt(folder, dtype):
+    """Each prompt's tokens are drawn from its own logits: every drawn token is one that its policy can draw (of the 50 likeliest, by
+    logits that are off by the type's tolerance on either side), lengths are whole, and a second run draws the same."""
+    from nnis_b200 import LLM, SamplingConfig
+    llm = LLM(folder, dtype=dtype, max_tokens=1 << 14, max_batch=8)
+    document = tokens(4, 1100)
+    prompts = [document + [7 + i] * (1 + 3 * i) for i in range(6)]
+    sampling = [SamplingConfig(seed=i, temperature=0.9, top_k=50) for i in range(6)]
+    drawn = [llm.generate(prompts, max_new_tokens=90, share_prefix=True, sampling=sampling, stop_token_ids=[]) for _ in range(2)]
+    assert all(r.ok and len(r.token_ids) == 90 for run in drawn for r in run)
+    assert [r.token_ids for r in drawn[0]] == [r.token_ids for r in drawn[1]]
+    limit = 2 * (F32_REL_TO_MAX if dtype == "float32" else BF16_REL_TO_MAX)
+    for prompt, r in zip(prompts, drawn[0]):
+        logits = logits_alone(llm, prompt, r.token_ids)
+        line = np.sort(logits, axis=1)[:, -50]
+        assert (logits[np.arange(90), r.token_ids] >= line - limit * np.maximum(1.0, np.abs(logits).max(axis=1))).all()
