@@ -32,7 +32,7 @@ from .generate import (DEFAULT_MAX_NEW_TOKENS, GenerationConfig, GenerationReque
 Prompt = Union[str, Sequence[int]]
 
 MAX_SHARED_DECODERS = 8  # captured steps kept for batches whose sequences share pages
-MAX_DRAFTED_ROWS = 64  # most tokens of one sequence that a captured step takes, however few sequences a batch may hold
+DRAFTED_ROWS = 64  # tokens of one sequence that a captured step takes, however few sequences a batch may hold
 
 
 class EngineBackend:
@@ -140,7 +140,7 @@ class EngineBackend:
         then 0.6 ms instead of the 8 of its launches from Python one by one."""
         engine, cache, n = self.engine, self.engine.cache, len(tokens)
         vocab = engine.spec.vocab_size
-        if not again or self.decode_greedy is None or not engine.model.all_share or n > MAX_DRAFTED_ROWS \
+        if not again or self.decode_greedy is None or not engine.model.all_share or n > max(self.max_rows, DRAFTED_ROWS) \
                 or not all(0 <= t < vocab for t in tokens):
             return engine.step([SequenceStep(slot, tokens, list(range(n)))], drafted=True)
         held = cache.length(slot)

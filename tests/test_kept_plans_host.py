@@ -223,9 +223,9 @@ def test_pages_stay_where_they_are_while_a_generation_shares_them(share):
     cache.check()
 
 
-@pytest.mark.parametrize("tokens", [2, 5, 64])
-def test_drafted_steps_are_captured_whatever_the_batch(monkeypatch, tokens):
-    """A model for one sequence (``max_batch=1``) takes a token and its drafts by a captured step."""
+@pytest.mark.parametrize("tokens,most", [(2, 1), (5, 1), (64, 1), (64, 4), (100, 100)])
+def test_drafted_steps_are_captured_whatever_the_batch(monkeypatch, tokens, most):
+    """A model for one sequence (``max_batch=1``), or for many, takes a token and its drafts by a captured step."""
     from nnis_b200.engine import api
     engine = make_engine()
     monkeypatch.setattr(api, "GraphDecoder", lambda engine, rows, context, want_logits, rooms: made.append(rows) or Drafted(rows))
@@ -238,7 +238,7 @@ def test_drafted_steps_are_captured_whatever_the_batch(monkeypatch, tokens):
             launched.append(dict(self.positions))
             self.logits = torch.zeros((self.rows, VOCAB))
 
-    backend = EngineBackend(engine, 1)
+    backend = EngineBackend(engine, most)
     slot = engine.acquire_slot()
     engine.cache.reserve([slot], [100])
     engine.cache.commit([slot], [100])
