@@ -479,7 +479,7 @@ class InferenceSession:
         if sampling is not None and (sampling.top_k is not None or sampling.top_p is not None):
             raise ValueError("drafted generation samples with a temperature only (no top_k, no top_p)")
         llm = getattr(drafter, "llm", None)
-        there = getattr(getattr(llm, "engine", None), "device", self.engine.device)
+        there = torch.device(getattr(getattr(llm, "engine", None), "device", self.engine.device))
         if (there.index or 0) != (self.engine.device.index or 0):
             raise ValueError(f"the drafting model is on {there}, this one on {self.engine.device}")
         other = getattr(llm, "spec", None)

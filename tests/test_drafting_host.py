@@ -108,6 +108,7 @@ def test_a_drafting_model_on_another_device_is_refused(monkeypatch):
     with pytest.raises(ValueError, match="cuda:1"):
         fake.session.generate_drafted([5], GenerationConfig(4), drafter)
     assert fake.length == 0 and not fake.seen
-    drafter.llm.engine.device = torch.device("cuda")  # (the first, however it is named)
     drafter.begin, drafter.propose = lambda: None, lambda tokens, count, temperature: ([], None)
-    assert fake.session.generate_drafted([5], GenerationConfig(4), drafter) == [6, 7, 8, 9]
+    for first in (torch.device("cuda"), "cuda:0", "cuda"):  # (however it is named)
+        drafter.llm.engine.device = first
+        assert fake.session.generate_drafted([5], GenerationConfig(4), drafter) == [6, 7, 8, 9]
