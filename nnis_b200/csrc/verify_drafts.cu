@@ -152,7 +152,7 @@ verify_rows_kernel(const float* __restrict__ logits, const float* __restrict__ d
     int lo = 0, hi = n_seqs - 1;
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
-        if (first_row[mid] <= (of_draft ? r - rows + mid : r)) lo = mid;
+        if ((int)((unsigned)first_row[mid] - (of_draft ? (unsigned)mid : 0u)) <= (of_draft ? r - rows : r)) lo = mid;
         else hi = mid - 1;
     }
     const float t = temperature[lo];
@@ -282,14 +282,15 @@ verify_pick_kernel(const float* __restrict__ logits, const float* __restrict__ d
         s.last = -1;
     }
     // (What the call was given is older than the first launch, which has waited for it: it is read under that launch's end.)
+    // (Offsets may be any numbers: differences wrap, and count for nothing where a comparison says that no packed rows have them.)
     const int row0 = first_row[b], row_end = first_row[b + 1];
-    // (compared, not subtracted: offsets may be any numbers; good ones leave as many draft rows as there are drafts)
-    const bool good = row0 >= b && row_end > row0 && row_end <= rows && row_end - b <= rows - (int)gridDim.y + 1;
-    const int draft0 = good ? row0 - b : 0, count = good ? row_end - row0 - 1 : 0;
+    const int draft0 = (int)((unsigned)row0 - (unsigned)b), count = (int)((unsigned)row_end - (unsigned)row0 - 1u);
     const float t = temperature[b];
     const bool greedy = !(t > 0.f);
     const float c = scale_of(t);
     const double inv_t = greedy ? 1.0 : 1.0 / (double)t;
+    // (good ones leave as many draft rows as there are drafts)
+    const bool good = row0 >= b && row_end > row0 && row_end <= rows && row_end - b <= rows - (int)gridDim.y + 1;
     // A warp's draft: its logits in the two rows.
     struct Draft {
         int id;
@@ -308,7 +309,7 @@ verify_pick_kernel(const float* __restrict__ logits, const float* __restrict__ d
         }
         return x;
     };
-    Draft mine = draft_of(warp);
+    Draft mine = draft_of(good ? warp : count);
     cluster.sync();  // (all of the cluster run: their shared memory may be written)
     pdl_wait();
     pdl_launch_dependents();
