@@ -182,7 +182,7 @@ def _codes(pages, kv_heads, dim, gen):
     top = codes.abs().amax(-1, keepdim=True)
     codes = torch.round(codes * (127.0 / top)).to(torch.int8)
     spread = torch.rand(shape[:3], generator=gen, device="cuda") * 0.5 + 0.75
-    return codes, (top[..., 0] / 127.0) * spread
+    return codes, top[..., 0] / 127.0 * spread
 
 
 def _prepare_cache(case, gen):
@@ -246,7 +246,8 @@ def run(state):
 def _rows_to_codes(x):
     """float32 rows -> (codes as float32, scales)."""
     top = x.abs().amax(-1, keepdim=True)
-    return torch.round(x * (127.0 / top)), top / 127.0
+    most = torch.full_like(top, 127.0)  # (a quotient of two tensors is rounded once; by a number it is a product with a reciprocal)
+    return torch.round(x * (most / top)), top / most
 
 
 def _run_cache(s):
