@@ -67,7 +67,10 @@ def _stream() -> ctypes.c_void_p:
 # comes last, so that neither side pads the end): thirty arguments wrapped one by one cost the host 8 us, as plain numbers
 # 2.4, in a record 0.6.
 _ENTRY_FIELDS = {"nnis_copy_pages": "ppiiiiiipiip", "nnis_verify_drafts": "ppppppppiiippp",
-                 "nnis_attention_shared": "pippppipiiippppppiiiiiifiipp"}
+                 "nnis_attention_shared": "pippppipiiippppppiiiiiifiipp",
+                 "nnis_rope_store_int8": "pppppppppppiiiiiiiiiip", "nnis_read_pages_int8": "ppppppppiiiiiiiiip",
+                 "nnis_attention_int8": "ppppppppppiiiiiiiiiifiip", "nnis_quantize_rows": "pppiiiip",
+                 "nnis_linear_int8": "pppppppiiiiiip"}
 _entries = {}
 
 
@@ -3000,3 +3003,220 @@ def attention_shared(q: torch.Tensor, q_stride: int, k_cache: torch.Tensor, v_ca
         table_shape[1], plan.units, n0, n1, n2, plan.members, plan.record, at, at + 4 * held * d, tickets, out.data_ptr(), n,
         heads, kv_heads, d, shape[0], 64, scale, plan.code, plan.form, plan.status, _stream_of(index)),
         "attention_shared", plan.launches)
+
+
+# ---- 8 bits: codes and scales (int8_rows.cuh) -------------------------------------------------------------
+def _wanted(what: str, **tensors) -> None:
+    """Says of each (tensor, dtype, shape) what is wrong with it (the calls below come here only when something is)."""
+    for name, (t, dtype, shape) in tensors.items():
+        if t is None:
+            continue
+        _need(t.dtype == dtype, f"{what}: {name} is {t.dtype}, wanted {dtype}")
+        _need(len(t.shape) == len(shape) and all(w is None or w == g for w, g in zip(shape, t.shape)),
+              f"{what}: {name} is {tuple(t.shape)}, wanted {tuple('any' if w is None else w for w in shape)}")
+        _need(t.is_contiguous(), f"{what}: {name} is not contiguous")
+    devices = {t.device for t, _, _ in tensors.values() if t is not None}
+    _need(all(d.type == "cuda" for d in devices), f"{what}: kernels take CUDA tensors only (there is no CPU path)")
+    _need(len(devices) == 1, f"{what}: tensors on several devices: {sorted(map(str, devices))}")
+
+
+def _store8(what: str, k, v, k_scales, v_scales, kv_heads: int, head_dim: int, page_size: int) -> dict:
+    pages = k.shape[0] if k.dim() else 0
+    _need(kv_heads > 0 and page_size > 0 and head_dim % 2 == 0 and 2 <= head_dim <= 256,
+          f"{what}: even head sizes up to 256, at least one head and a page of one position; got {kv_heads} heads of {head_dim}, "
+          f"pages of {page_size}")
+    codes, scales = (pages, kv_heads, page_size, head_dim), (pages, kv_heads, page_size)
+    return {"k": (k, torch.int8, codes), "v": (v, torch.int8, codes), "k_scales": (k_scales, torch.float32, scales),
+            "v_scales": (v_scales, torch.float32, scales)}
+
+
+def _good(*wanted) -> bool:
+    """Whether every (tensor, dtype, shape) is a contiguous tensor of that kind on the first one's CUDA device."""
+    index = wanted[0][0].get_device()
+    return index >= 0 and all(t.dtype is dtype and t.shape == shape and t.get_device() == index and t.is_contiguous()
+                              for t, dtype, shape in wanted)
+
+
+def rope_store_int8(qkv: torch.Tensor, q: torch.Tensor, token_pos: torch.Tensor, token_seq: torch.Tensor, page_table: torch.Tensor,
+                    cos: Optional[torch.Tensor], sin: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
+                    k_scales: torch.Tensor, v_scales: torch.Tensor, heads: int, kv_heads: int, head_dim: int, page_size: int) -> None:
+    """The rows' q heads rotated into ``q`` [n, heads * d] and their k (rotated, rounded to the rows' type) and v heads put into
+    the cache of 8-bit codes: k, v int8 [pages, kv_heads, page_size, d], k_scales, v_scales float32 [pages, kv_heads,
+    page_size].  A head x gets the codes rint(x * (127 / top)) and the scale top / 127, top = max |x|.  ``qkv`` [n, (heads +
+    2 kv_heads) * d] float32 or bfloat16 is left as it is.  ``cos`` and ``sin`` None: nothing is rotated.  A row at position -1, or
+    beyond the angles, writes nothing; one whose page the table does not name stores nothing.  No two rows of a call have the same
+    sequence and position."""
+    d, n = head_dim, qkv.shape[0] if qkv.dim() else 0
+    pages, seqs, cols = k.shape[0] if k.dim() else 0, page_table.shape[0], page_table.shape[-1]
+    codes, scales, half = (pages, kv_heads, page_size, d), (pages, kv_heads, page_size), (cos.shape[0] if cos is not None else 0, d // 2)
+    if not (d % 2 == 0 and 2 <= d <= 256 and heads > 0 and kv_heads > 0 and page_size > 0 and qkv.dtype in _DTYPE_CODE
+            and _good((qkv, qkv.dtype, (n, (heads + 2 * kv_heads) * d)), (q, qkv.dtype, (n, heads * d)), (k, torch.int8, codes),
+                      (v, torch.int8, codes), (k_scales, torch.float32, scales), (v_scales, torch.float32, scales),
+                      (page_table, torch.int32, (seqs, cols)))
+            and token_pos.dtype is token_seq.dtype is torch.int32 and token_pos.numel() >= n and token_seq.numel() >= n
+            and _good((qkv, qkv.dtype, qkv.shape), (token_pos, torch.int32, token_pos.shape), (token_seq, torch.int32, token_seq.shape))
+            and (cos is None) == (sin is None)
+            and (cos is None or _good((qkv, qkv.dtype, qkv.shape), (cos, torch.float32, half), (sin, torch.float32, half)))):
+        code_of(qkv.dtype)
+        _need(heads > 0, "rope_store_int8: at least one query head")
+        _need((cos is None) == (sin is None), "rope_store_int8: cos and sin, or neither")
+        _need(token_pos.numel() >= n and token_seq.numel() >= n, f"rope_store_int8: a position and a sequence for each of {n} rows")
+        _wanted("rope_store_int8", qkv=(qkv, qkv.dtype, (None, (heads + 2 * kv_heads) * d)), q=(q, qkv.dtype, (n, heads * d)),
+                **_store8("rope_store_int8", k, v, k_scales, v_scales, kv_heads, d, page_size),
+                token_pos=(token_pos, torch.int32, token_pos.shape), token_seq=(token_seq, torch.int32, token_seq.shape),
+                page_table=(page_table, torch.int32, (None, None)), cos=(cos, torch.float32, (None, d // 2)),
+                sin=(sin, torch.float32, half))
+        raise KernelError("rope_store_int8: bad argument")
+    if n == 0:
+        return
+    index = qkv.get_device()
+    if _device_now() != index:
+        with torch.cuda.device(index):
+            return rope_store_int8(qkv, q, token_pos, token_seq, page_table, cos, sin, k, v, k_scales, v_scales, heads, kv_heads, d,
+                                   page_size)
+    _check(_entry("nnis_rope_store_int8")(
+        qkv.data_ptr(), q.data_ptr(), token_pos.data_ptr(), token_seq.data_ptr(), page_table.data_ptr(),
+        0 if cos is None else cos.data_ptr(), 0 if sin is None else sin.data_ptr(), k.data_ptr(), v.data_ptr(), k_scales.data_ptr(),
+        v_scales.data_ptr(), _DTYPE_CODE[qkv.dtype], seqs, cols, half[0], pages, n, heads, kv_heads, d, page_size,
+        _stream_of(index)), "rope_store_int8")
+
+
+def read_pages_int8(k: torch.Tensor, v: torch.Tensor, k_scales: torch.Tensor, v_scales: torch.Tensor, page_table: torch.Tensor,
+                    local_table: torch.Tensor, k_out: torch.Tensor, v_out: torch.Tensor) -> None:
+    """Pages of the 8-bit cache read back: for every place (sequence, column) of ``local_table`` that names a page of the outputs,
+    int32 [sequences, columns], -1 where none is wanted, that page becomes the values, code times scale, of the page that
+    ``page_table`` names in the same place.  k, v int8 [pages, kv_heads, page_size, d], their scales float32 [pages, kv_heads,
+    page_size]; k_out, v_out float32 or bfloat16 [out_pages, kv_heads, page_size, d].  A page id outside its store is passed over."""
+    shape, seqs, cols, local_cols = k.shape, local_table.shape[0], page_table.shape[-1], local_table.shape[-1]
+    outs, dtype = (k_out.shape[0] if k_out.dim() else 0, *shape[1:]), k_out.dtype
+    if not (len(shape) == 4 and dtype in _DTYPE_CODE
+            and _good((k, torch.int8, shape), (v, torch.int8, shape), (k_scales, torch.float32, shape[:3]),
+                      (v_scales, torch.float32, shape[:3]), (page_table, torch.int32, (page_table.shape[0], cols)),
+                      (local_table, torch.int32, (seqs, local_cols)), (k_out, dtype, outs), (v_out, dtype, outs))
+            and page_table.shape[0] >= seqs and cols >= local_cols):
+        code_of(dtype)
+        _need(len(shape) == 4, f"read_pages_int8: k is int8 [pages, kv_heads, page_size, d]; got {tuple(shape)}")
+        _wanted("read_pages_int8", **_store8("read_pages_int8", k, v, k_scales, v_scales, shape[1], shape[3], shape[2]),
+                page_table=(page_table, torch.int32, (None, None)), local_table=(local_table, torch.int32, (None, None)),
+                k_out=(k_out, dtype, (None, *shape[1:])), v_out=(v_out, dtype, outs))
+        raise KernelError(f"read_pages_int8: local_table {tuple(local_table.shape)} reaches beyond page_table {tuple(page_table.shape)}")
+    if not local_table.numel() or not outs[0] or not k.numel():
+        return
+    index = k.get_device()
+    if _device_now() != index:
+        with torch.cuda.device(index):
+            return read_pages_int8(k, v, k_scales, v_scales, page_table, local_table, k_out, v_out)
+    _check(_entry("nnis_read_pages_int8")(
+        k.data_ptr(), v.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), page_table.data_ptr(), local_table.data_ptr(),
+        k_out.data_ptr(), v_out.data_ptr(), cols, seqs, local_cols, _DTYPE_CODE[dtype], shape[0], outs[0], shape[1], shape[2],
+        shape[3], _stream_of(index)), "read_pages_int8")
+
+
+def attention_int8_splits(n: int, heads: int, keys: int, device) -> int:
+    """Into how many slices the keys of a row are cut where ``n`` rows of ``heads`` heads see at most ``keys`` of them: a warp a slice,
+    sixteen warps an SM, at least 128 keys each, at most 64."""
+    return max(1, min(16 * sm_count(device) // max(1, n * heads), -(-keys // 128), 64))
+
+
+def attention_int8(q: torch.Tensor, q_stride: int, k: torch.Tensor, v: torch.Tensor, k_scales: torch.Tensor, v_scales: torch.Tensor,
+                   token_pos: torch.Tensor, token_seq: torch.Tensor, page_table: torch.Tensor, out: torch.Tensor, heads: int,
+                   kv_heads: int, head_dim: int, window: int, scale: float, workspace) -> None:
+    """Causal attention of packed query rows over the cache of 8-bit codes (``rope_store_int8``): a row at position p of its sequence
+    sees the keys up to p, the last ``window`` of them where that is not 0.  q float32 or bfloat16, rows ``q_stride`` apart, out [n,
+    heads * d] of its type.  A position whose page the table does not name, or beyond it, holds no key; a row that sees none (a
+    padding row at position -1 among them) is zero.  Every row of a call reads its keys by itself: for single tokens and a few
+    drafted ones (prompts read their pages back and take the kernels of the 16-bit cache)."""
+    d, dtype, (n, width) = head_dim, q.dtype, out.shape
+    pages, seqs, cols, page_size = k.shape[0], page_table.shape[0], page_table.shape[-1], k.shape[2] if k.dim() == 4 else 0
+    codes, scales = (pages, kv_heads, page_size, d), (pages, kv_heads, page_size)
+    if not (d % 2 == 0 and 2 <= d <= 256 and heads > 0 and kv_heads > 0 and heads % kv_heads == 0 and page_size > 0 and window >= 0
+            and scale > 0 and dtype in _DTYPE_CODE and q.dim() == 2 and q.shape[0] >= n and q.stride() == (q_stride, 1)
+            and q.shape[1] >= heads * d <= q_stride < 1 << 31 and q.get_device() == k.get_device() and heads <= 65535
+            and _good((k, torch.int8, codes), (v, torch.int8, codes), (k_scales, torch.float32, scales),
+                      (v_scales, torch.float32, scales), (out, dtype, (n, heads * d)), (page_table, torch.int32, (seqs, cols)),
+                      (token_pos, torch.int32, token_pos.shape), (token_seq, torch.int32, token_seq.shape))
+            and token_pos.numel() >= n and token_seq.numel() >= n):
+        code_of(dtype)
+        _wanted("attention_int8", **_store8("attention_int8", k, v, k_scales, v_scales, kv_heads, d, page_size),
+                out=(out, dtype, (n, heads * d)), page_table=(page_table, torch.int32, (None, None)),
+                token_pos=(token_pos, torch.int32, token_pos.shape), token_seq=(token_seq, torch.int32, token_seq.shape))
+        raise KernelError(
+            f"attention_int8: wanted are heads a multiple of kv_heads, a window of 0 or more, a positive scale, a position and a "
+            f"sequence for every row, and q [rows, heads * d] in rows of q_stride on the cache's device; got {heads} heads over "
+            f"{kv_heads}, window {window}, scale {scale}, q {tuple(q.shape)} in strides {q.stride()} (q_stride {q_stride}) on "
+            f"{q.device}, out {tuple(out.shape)}, {token_pos.numel()} positions, {token_seq.numel()} sequences")
+    if n == 0:
+        return
+    index = k.get_device()
+    if _device_now() != index:
+        with torch.cuda.device(index):
+            return attention_int8(q, q_stride, k, v, k_scales, v_scales, token_pos, token_seq, page_table, out, heads, kv_heads, d,
+                                  window, scale, workspace)
+    keys = cols * page_size
+    splits = attention_int8_splits(n, heads, min(keys, window) if window else keys, k.device)
+    partial = workspace.room("attn_int8_partial", n * heads * splits * (d + 2), torch.float32).data_ptr() if splits > 1 else 0
+    _check(_entry("nnis_attention_int8")(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), token_pos.data_ptr(),
+        token_seq.data_ptr(), page_table.data_ptr(), out.data_ptr(), partial, q_stride, seqs, cols, pages, n, heads, kv_heads, d,
+        page_size, window, scale, splits, _DTYPE_CODE[dtype], _stream_of(index)), "attention_int8", 2 if splits > 1 else 1)
+
+
+def int8_width(k: int) -> int:
+    """Bytes of a row of ``k`` codes of a matrix or of tokens: a multiple of 16, zero behind the codes."""
+    return -(-k // 16) * 16
+
+
+def quantize_rows(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor) -> None:
+    """Every row of x [rows, k], float32 or bfloat16, in rows of any stride, as 8-bit codes rint(x * (127 / top)) and the scale top /
+    127, top = max |x|: codes int8 [rows, int8_width(k)], scales float32 [rows].  A row of zeros has the scale zero; one that holds
+    an infinity or a NaN has the scale NaN and codes of zero."""
+    code = code_of(x.dtype)
+    _need(x.dim() == 2 and (x.shape[1] == 1 or x.stride(1) == 1) and x.shape[1] > 0,
+          f"quantize_rows: x [rows, k >= 1], a row's values beside one another; got {tuple(x.shape)} in strides {x.stride()}")
+    rows, k = x.shape
+    _wanted("quantize_rows", codes=(codes, torch.int8, (rows, int8_width(k))), scales=(scales, torch.float32, (rows,)))
+    _need(codes.device == x.device, "quantize_rows: tensors on several devices")
+    if rows == 0:
+        return
+    index = x.get_device()
+    if _device_now() != index:
+        with torch.cuda.device(index):
+            return quantize_rows(x, codes, scales)
+    stride = x.stride(0) if rows > 1 else k
+    _check(_entry("nnis_quantize_rows")(x.data_ptr(), codes.data_ptr(), scales.data_ptr(), stride, code, rows, k, _stream_of(index)),
+           "quantize_rows")
+
+
+def linear_int8(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, bias: Optional[torch.Tensor], out: torch.Tensor, mode: int,
+                workspace) -> None:
+    """y = x . W^T (+ bias) with the rows of x put into 8-bit codes with a scale for every token (``quantize_rows``), W held in such
+    codes with a scale for every row, w int8 [n, int8_width(k)], and the codes multiplied as whole numbers: the sum is exact, and
+    one float32 product with each scale follows.  x [m, k] float32 or bfloat16, bias float32 [n] or None.  ``mode``: STORE (out of
+    x's type [m, n]), STORE_F32 or ADD_F32 (float32 [m, n], written or added to), GEMM_GATED (w = [gate; up] rows, out of x's type [m, n /
+    2] = silu(gate) * up).  k at most 133,136: beyond it a sum could pass 32 bits."""
+    dtype = x.dtype
+    (m, k), (rows, width) = x.shape, w.shape
+    n = rows // 2 if mode == GEMM_GATED else rows
+    kept = dtype if mode in (STORE, GEMM_GATED) else torch.float32
+    if not (dtype in _DTYPE_CODE and 0 < k <= 133136 and mode in (STORE, STORE_F32, ADD_F32, GEMM_GATED) and n > 0
+            and (mode != GEMM_GATED or rows % 2 == 0) and (k == 1 or x.stride(1) == 1) and x.get_device() == w.get_device()
+            and _good((w, torch.int8, (rows, int8_width(k))), (w_scales, torch.float32, (rows,)), (out, kept, (m, n)))
+            and (bias is None or _good((w, torch.int8, w.shape), (bias, torch.float32, (rows,))))):
+        code_of(dtype)
+        _need(mode in (STORE, STORE_F32, ADD_F32, GEMM_GATED), f"linear_int8: mode {mode}")
+        _need(mode != GEMM_GATED or rows % 2 == 0, f"linear_int8: {rows} rows are no gate and up")
+        _wanted("linear_int8", w=(w, torch.int8, (rows, int8_width(k))), w_scales=(w_scales, torch.float32, (rows,)),
+                bias=(bias, torch.float32, (rows,)), out=(out, kept, (m, n)))
+        raise KernelError(f"linear_int8: x [m, k] with 0 < k <= 133136 and a row's values beside one another, on w's device; got "
+                          f"{tuple(x.shape)} in strides {x.stride()} on {x.device}")
+    if m == 0:
+        return
+    index = w.get_device()
+    if _device_now() != index:
+        with torch.cuda.device(index):
+            return linear_int8(x, w, w_scales, bias, out, mode, workspace)
+    codes = workspace.room("int8_codes", m * width, torch.int8)
+    scales = workspace.room("int8_scales", m, torch.float32)
+    _check(_entry("nnis_linear_int8")(
+        x.data_ptr(), w.data_ptr(), w_scales.data_ptr(), 0 if bias is None else bias.data_ptr(), out.data_ptr(), codes.data_ptr(),
+        scales.data_ptr(), x.stride(0) if m > 1 else k, m, n, k, mode, _DTYPE_CODE[dtype], _stream_of(index)), "linear_int8", 2)

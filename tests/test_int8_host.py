@@ -1,0 +1,118 @@
+"""What the operators of 8-bit codes refuse, and their plain forms (no GPU)."""
+import pytest
+import torch
+
+import int8_plain as plain
+
+I8, F32, BF16, I32 = torch.int8, torch.float32, torch.bfloat16, torch.int32
+
+
+def empty(*shape, dtype=F32):
+    return torch.zeros(shape, dtype=dtype)
+
+
+def store_args(**change):
+    a = dict(qkv=empty(5, 5 * 64, dtype=BF16), q=empty(5, 3 * 64, dtype=BF16), pos=empty(5, dtype=I32), seq=empty(5, dtype=I32),
+             table=empty(2, 3, dtype=I32), cos=empty(9, 32), sin=empty(9, 32), k=empty(4, 1, 64, 64, dtype=I8), v=empty(4, 1, 64, 64, dtype=I8),
+             ks=empty(4, 1, 64), vs=empty(4, 1, 64), heads=3, kv_heads=1, d=64, page=64)
+    a.update(change)
+    return list(a.values())
+
+
+@pytest.mark.parametrize("change,why", [
+    (dict(), "CUDA tensors only"), (dict(qkv=empty(5, 5 * 64, dtype=torch.float16)), "float16"), (dict(q=empty(5, 3 * 64)), "q is"),
+    (dict(q=empty(4, 3 * 64, dtype=BF16)), "q is"), (dict(k=empty(4, 1, 64, 64)), "k is"), (dict(v=empty(3, 1, 64, 64, dtype=I8)), "v is"),
+    (dict(ks=empty(4, 1, 63)), "k_scales is"), (dict(vs=empty(4, 1, 64, dtype=BF16)), "v_scales is"), (dict(pos=empty(4, dtype=I32)), "each of 5 rows"),
+    (dict(seq=empty(5, dtype=torch.int64)), "token_seq is"), (dict(table=empty(6, dtype=I32)), "page_table is"), (dict(sin=None), "cos and sin"),
+    (dict(cos=empty(9, 31)), "cos is"), (dict(sin=empty(8, 32)), "sin is"), (dict(heads=0), "query head"), (dict(d=63), "even head sizes"),
+    (dict(kv_heads=0), "even head sizes"), (dict(qkv=empty(5, 6 * 64, dtype=BF16)[:, 64:]), "not contiguous")])
+def test_writing_refuses(change, why):
+    from nnis_b200.csrc import ops
+    with pytest.raises(ops.KernelError, match=why):
+        ops.rope_store_int8(*store_args(**change))
+
+
+def read_args(**change):
+    a = dict(k=empty(4, 2, 64, 64, dtype=I8), v=empty(4, 2, 64, 64, dtype=I8), ks=empty(4, 2, 64), vs=empty(4, 2, 64), table=empty(2, 3, dtype=I32),
+             local=empty(2, 3, dtype=I32), ko=empty(5, 2, 64, 64, dtype=BF16), vo=empty(5, 2, 64, 64, dtype=BF16))
+    a.update(change)
+    return list(a.values())
+
+
+@pytest.mark.parametrize("change,why", [
+    (dict(), "CUDA tensors only"), (dict(k=empty(4, 2, 64, 64)), "k is"), (dict(k=empty(4, 64, 64, dtype=I8)), "k is int8"),
+    (dict(vs=empty(4, 64, 2)), "v_scales is"), (dict(local=empty(2, 3, dtype=torch.int64)), "local_table is"), (dict(vo=empty(5, 2, 64, 64)), "v_out is"),
+    (dict(ko=empty(5, 2, 64, 63, dtype=BF16)), "k_out is"), (dict(vo=empty(4, 2, 64, 64, dtype=BF16)), "v_out is"),
+    (dict(ko=empty(5, 2, 64, 64, dtype=torch.float16)), "float16")])
+def test_reading_refuses(change, why):
+    from nnis_b200.csrc import ops
+    with pytest.raises(ops.KernelError, match=why):
+        ops.read_pages_int8(*read_args(**change))
+
+
+def attend_args(**change):
+    a = dict(q=empty(5, 6 * 64, dtype=BF16), stride=6 * 64, k=empty(4, 2, 64, 64, dtype=I8), v=empty(4, 2, 64, 64, dtype=I8), ks=empty(4, 2, 64),
+             vs=empty(4, 2, 64), pos=empty(5, dtype=I32), seq=empty(5, dtype=I32), table=empty(2, 3, dtype=I32), out=empty(5, 6 * 64, dtype=BF16),
+             heads=6, kv_heads=2, d=64, window=0, scale=0.125, ws=None)
+    a.update(change)
+    return list(a.values())
+
+
+@pytest.mark.parametrize("change,why", [
+    (dict(), "CUDA tensors only"), (dict(q=empty(5, 6 * 64)), "out is"), (dict(out=empty(5, 5 * 64, dtype=BF16)), "out is"), (dict(k=empty(4, 2, 64, 64)), "k is"),
+    (dict(ks=empty(4, 2, 64, 1)), "k_scales is"), (dict(pos=empty(5)), "token_pos is"), (dict(table=empty(2, 3)), "page_table is"),
+    (dict(q=empty(5, 6 * 64, dtype=torch.float16), out=empty(5, 6 * 64, dtype=torch.float16)), "float16")])
+def test_attention_refuses(change, why):
+    from nnis_b200.csrc import ops
+    with pytest.raises(ops.KernelError, match=why):
+        ops.attention_int8(*attend_args(**change))
+
+
+def product_args(**change):
+    a = dict(x=empty(5, 40, dtype=BF16), w=empty(12, 48, dtype=I8), ws=empty(12), bias=None, out=empty(5, 12, dtype=BF16), mode=0, space=None)
+    a.update(change)
+    return list(a.values())
+
+
+@pytest.mark.parametrize("change,why", [
+    (dict(), "CUDA tensors only"), (dict(x=empty(5, 40, dtype=torch.float16)), "float16"), (dict(w=empty(12, 40, dtype=I8)), "w is"), (dict(w=empty(12, 48)), "w is"),
+    (dict(ws=empty(11)), "w_scales is"), (dict(bias=empty(12, dtype=BF16)), "bias is"), (dict(out=empty(5, 12)), "out is"), (dict(mode=1), "out is"),
+    (dict(mode=3), "out is"), (dict(mode=7), "mode 7"), (dict(w=empty(11, 48, dtype=I8), mode=3), "no gate and up")])
+def test_products_refuse(change, why):
+    from nnis_b200.csrc import ops
+    with pytest.raises(ops.KernelError, match=why):
+        ops.linear_int8(*product_args(**change))
+
+
+@pytest.mark.parametrize("x,codes,scales,why", [
+    (empty(3, 20), empty(3, 32, dtype=I8), empty(3), "CUDA tensors only"), (empty(3, 20), empty(3, 20, dtype=I8), empty(3), "codes is"),
+    (empty(3, 20), empty(3, 32, dtype=I8), empty(4), "scales is"), (empty(20, 3).T, empty(3, 32, dtype=I8), empty(3), "beside one another"),
+    (empty(3, 0), empty(3, 0, dtype=I8), empty(3), "k >= 1"), (empty(3, 20, dtype=torch.float16), empty(3, 32, dtype=I8), empty(3), "float16")])
+def test_codes_of_rows_refuse(x, codes, scales, why):
+    from nnis_b200.csrc import ops
+    with pytest.raises(ops.KernelError, match=why):
+        ops.quantize_rows(x, codes, scales)
+
+
+def test_codes_are_within_half_a_step():
+    x = torch.randn((200, 64), generator=torch.Generator().manual_seed(0))
+    codes, scales = plain.codes_of(x)
+    assert codes.abs().amax() == 127
+    assert ((codes.double() * scales.double()[:, None] - x.double()).abs() <= x.abs().amax(1, keepdim=True).double() / 254 * (1 + 2.0 ** -20)).all()
+
+
+def test_codes_of_bfloat16_rows_are_the_exact_quotients():
+    """Every pair of a value and a top of 8 significant bits: the code is the exact quotient's, ties to even; half of the top, 63.5 steps,
+    may go either way."""
+    top = torch.arange(128, 256, dtype=F32)
+    for e in (1.0, 0.5, 0.25, 2.0 ** -6):
+        x = torch.arange(128, 256, dtype=F32) * e
+        rows = torch.stack((x[None].expand(128, -1), top[:, None].expand(-1, 128)), -1)
+        rows = rows[(x[None] <= top[:, None])]
+        codes, _ = plain.codes_of(rows)
+        whole = (rows[:, 0].double() * 127).div(rows[:, 1].double(), rounding_mode="floor")
+        part = rows[:, 0].double() * 127 - whole * rows[:, 1].double()  # (exact)
+        up = (2 * part > rows[:, 1]) | ((2 * part == rows[:, 1]) & (whole % 2 == 1))
+        half = 2 * rows[:, 0] == rows[:, 1]
+        assert torch.equal(codes[~half, 0].double(), (whole + up)[~half])
+        assert ((codes[half, 0] == 63) | (codes[half, 0] == 64)).all()

@@ -1,0 +1,142 @@
+"""Rows and matrices held in 8-bit codes, and their products."""
+import pytest
+import torch
+
+import int8_plain as plain
+
+pytestmark = pytest.mark.gpu
+TYPES = [torch.bfloat16, torch.float32]
+
+
+def coded(w):
+    """A matrix's codes in rows of whole 16 bytes, and its scales, made on the GPU."""
+    from nnis_b200.csrc import ops
+    codes = torch.full((w.shape[0], ops.int8_width(w.shape[1])), 55, dtype=torch.int8, device="cuda")
+    scales = torch.empty(w.shape[0], device="cuda")
+    ops.quantize_rows(w.cuda(), codes, scales)
+    return codes, scales
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,k", [(1, 1), (3, 15), (5, 16), (7, 17), (2, 511), (4, 576), (3, 2048), (2, 8192), (1, 20001), (300, 40)])
+def test_rows_become_codes(dtype, rows, k):
+    """To the last bit, zeros behind each row; rows further apart than they are long too."""
+    x = torch.randn((rows, k), generator=torch.Generator().manual_seed(k)).to(dtype)
+    if rows > 2:
+        x[1] = 0
+        x[2, k // 2] = float("nan")
+    for view in (x.cuda(), torch.cat((x, x), 1).cuda()[:, :k]):
+        codes, scales = coded(view)
+        want, want_scales = plain.codes_of(x)
+        assert torch.equal(codes[:, :k].cpu(), want) and (codes[:, k:] == 0).all()
+        assert torch.equal(torch.nan_to_num(scales.cpu(), nan=-9.0), torch.nan_to_num(want_scales, nan=-9.0))
+
+
+def check(dtype, m, n, k, mode, bias=False, seed=0, stride=0):
+    from nnis_b200.csrc import ops
+    from nnis_b200.engine.workspace import Workspace
+    gen = torch.Generator().manual_seed(seed + m + n + k)
+    rows = 2 * n if mode == ops.GEMM_GATED else n
+    x = (torch.randn((m, k), generator=gen) * (0.1 + 2 * torch.rand((m, 1), generator=gen))).to(dtype)
+    w, w_scales = coded(torch.randn((rows, k), generator=gen) * k ** -0.5)
+    b = torch.randn(rows, generator=gen) if bias else None
+    want, bound = plain.product(x, w.cpu(), k, w_scales.cpu(), b, mode == ops.GEMM_GATED)
+    kept = dtype if mode in (ops.STORE, ops.GEMM_GATED) else torch.float32
+    out = torch.randn((m, n), generator=gen).to(kept).cuda()
+    before = out.cpu().double()
+    given = torch.full((m, k + stride), float("nan"), dtype=dtype, device="cuda")
+    given[:, :k] = x.cuda()
+    ops.linear_int8(given[:, :k], w, w_scales, b.cuda() if bias else None, out, mode, Workspace(torch.device("cuda")))
+    if mode == ops.ADD_F32:
+        want = want + before
+        bound = bound + 2.0 ** -24 * want.abs()
+    got = out.cpu().double()
+    assert ((got - want).abs() <= bound).all(), float(((got - want).abs() / bound).max())
+
+
+SIZES = [(1, 960, 576), (2, 130, 64), (3, 1, 16), (8, 512, 2048), (9, 577, 300), (16, 64, 8192), (17, 96, 33), (33, 200, 1000), (64, 640, 576),
+         (65, 129, 17), (128, 256, 256), (130, 257, 515), (1, 1, 1), (5, 8192, 128), (300, 72, 4104), (257, 1000, 576)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,n,k", SIZES)
+@pytest.mark.parametrize("mode", [0, 1, 2, 3])
+def test_products(dtype, m, n, k, mode):
+    check(dtype, m, n, k, mode)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,n,k", [(1, 960, 576), (7, 65, 40), (40, 130, 700), (200, 384, 512)])
+@pytest.mark.parametrize("mode", [0, 1, 2, 3])
+def test_products_with_a_bias_and_rows_further_apart(dtype, m, n, k, mode):
+    check(dtype, m, n, k, mode, bias=True, seed=1, stride=3)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_a_large_product(dtype):
+    check(dtype, 1500, 1100, 2056, 0)
+
+
+@pytest.mark.parametrize("m", [1, 20, 200])
+@pytest.mark.parametrize("k", [8192, 133136])
+def test_the_largest_sums(m, k):
+    """All codes at their ends: the sum is the largest that k allows, exact to its last bit."""
+    from nnis_b200.csrc import ops
+    from nnis_b200.engine.workspace import Workspace
+    x = torch.full((m, k), -1.0, dtype=torch.bfloat16, device="cuda")
+    w, w_scales = coded(torch.full((70, k), 1.0))
+    out = torch.empty((m, 70), device="cuda")
+    ops.linear_int8(x, w, w_scales, None, out, ops.STORE_F32, Workspace(torch.device("cuda")))
+    one = torch.tensor(1.0) / torch.tensor(127.0)
+    want = torch.tensor(float(-127 * 127 * k)) * one * one
+    assert (out.cpu() == want).all()
+
+
+@pytest.mark.parametrize("m", [1, 40, 300])
+def test_tokens_that_are_no_numbers_stay_alone(m):
+    """An infinity or a NaN in a token, or in a row of the matrix, makes NaN of that row or column of the output, of no others."""
+    from nnis_b200.csrc import ops
+    from nnis_b200.engine.workspace import Workspace
+    gen = torch.Generator().manual_seed(3)
+    x, w = torch.randn((m, 64), generator=gen).to(torch.bfloat16), torch.randn((96, 64), generator=gen)
+    if m > 1:
+        x[m // 2, 3] = float("inf")
+    w[17, 5] = float("nan")
+    codes, scales = coded(w)
+    out = torch.empty((m, 96), dtype=torch.bfloat16, device="cuda")
+    ops.linear_int8(x.cuda(), codes, scales, None, out, ops.STORE, Workspace(torch.device("cuda")))
+    want = torch.zeros((m, 96), dtype=torch.bool)
+    want[:, 17] = True
+    if m > 1:
+        want[m // 2] = True
+    assert torch.equal(torch.isnan(out).cpu(), want)
+
+
+def test_products_on_a_stream_and_in_a_graph():
+    """Two products that share a workspace, one after the other, captured and replayed with other rows."""
+    from nnis_b200.csrc import ops
+    from nnis_b200.engine.workspace import Workspace
+    gen = torch.Generator().manual_seed(4)
+    w1, s1 = coded(torch.randn((2 * 256, 128), generator=gen))
+    w2, s2 = coded(torch.randn((128, 256), generator=gen))
+    x = torch.randn((24, 128), generator=gen).to(torch.bfloat16).cuda()
+    act, out, ws = torch.empty((24, 256), dtype=torch.bfloat16, device="cuda"), torch.zeros((24, 128), device="cuda"), Workspace(torch.device("cuda"))
+
+    def step():
+        ops.linear_int8(x, w1, s1, None, act, ops.GEMM_GATED, ws)
+        ops.linear_int8(act, w2, s2, None, out, ops.STORE_F32, ws)
+
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        step()
+    stream.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for _ in range(2):
+        x.copy_(torch.randn((24, 128), generator=gen).to(torch.bfloat16))
+        graph.replay()
+        first = out.clone()
+        step()
+        assert torch.equal(first, out)
