@@ -15,6 +15,8 @@ their views, in the same order):
   With ``values=False`` the group keeps one tensor only (``v`` is None): rows that
   serve as keys and carry the values inside them, as latent attention's do.
   ``value_dim`` gives the values a size of their own (0: the keys' size).
+  With ``codes`` the group holds 8-bit codes, ``k, v`` int8 of that shape, and a scale for every position and head,
+  ``k_scales, v_scales: [entries, pages, kv_heads, page_size]`` float32 (``ops.rope_store_int8`` writes them).
 * ``StateRequest`` - a fixed-size tensor per sequence, ``[slots, *shape]``,
   zeroed when a slot is taken: the state of a recurrent mixer (retention's
   ``[heads, dim, vdim]`` in float32).  ``extra`` lists further tensors of the same
@@ -54,6 +56,7 @@ class KVRequest:
     values: bool = True  # False: no storage for values (the key rows carry them)
     value_dim: int = 0  # size of a value head; 0: head_dim
     keep_first: int = 0  # first positions of a sequence that a windowed group keeps
+    codes: bool = False  # 8-bit codes with a scale for every position and head, in place of the cache's type
 
 
 @dataclass(frozen=True)
@@ -83,6 +86,8 @@ class KVView:
     window: int
     keep_first: int = 0
     ahead: int = 0  # elements from k (and v) to those of the group's layer that runs next; 0: none
+    k_scales: Optional[torch.Tensor] = None  # [pages, kv_heads, page_size] float32 where k and v are 8-bit codes
+    v_scales: Optional[torch.Tensor] = None
 
 
 @dataclass
@@ -92,19 +97,32 @@ class StateView:
 
 
 class _KVGroup:
-    def __init__(self, key: Tuple[int, int, int, bool, int, int], entries: List[int], pages: int,
+    def __init__(self, key: Tuple[int, int, int, bool, int, int, bool], entries: List[int], pages: int,
                  dtype: torch.dtype, device: torch.device):
-        self.kv_heads, self.head_dim, self.window, self.values, self.value_dim, self.keep_first = key
+        self.kv_heads, self.head_dim, self.window, self.values, self.value_dim, self.keep_first, self.codes = key
+        if self.codes and not self.values:
+            raise ValueError("a cache of 8-bit codes holds keys and values")
         self.kept_pages = -(-self.keep_first // PAGE_SIZE)  # these never go back while the sequence lives
         self.entries = entries
         self.pool = FreeList(pages, "page")
         shape = (len(entries), pages, self.kv_heads, PAGE_SIZE, self.head_dim)
+        dtype = torch.int8 if self.codes else dtype
         self.k = torch.zeros(shape, dtype=dtype, device=device)
         self.v = torch.zeros((*shape[:4], self.value_dim), dtype=dtype, device=device) if self.values else None
+        self.k_scales = torch.zeros(shape[:4], device=device) if self.codes else None
+        self.v_scales = torch.zeros(shape[:4], device=device) if self.codes else None
         # per slot: logical page index -> page id, -1 where given back
         self.tables: Dict[int, List[int]] = {}
         # pages in more than one table: how many more
         self.extra: Dict[int, int] = {}
+
+    def stores(self) -> List[torch.Tensor]:
+        """Everything that pages hold: keys, values, scales."""
+        return [t for t in (self.k, self.v, self.k_scales, self.v_scales) if t is not None]
+
+    def position_bytes(self) -> int:
+        """Bytes of one position in one layer."""
+        return self.kv_heads * ((self.head_dim + self.value_dim) * self.k.element_size() + (8 if self.codes else 0))
 
     def give(self, page: int) -> None:
         """One table fewer holds the page; it is free when none does."""
@@ -148,7 +166,7 @@ class CacheManager:
         self.owners: List[int] = [0] * max_slots  # how many sequences have held each slot
         self.groups: List[_KVGroup] = []
         self._views: List[Optional[Union[KVView, StateView]]] = []
-        by_key: Dict[Tuple[int, int, int, bool, int, int], List[int]] = {}
+        by_key: Dict[Tuple[int, int, int, bool, int, int, bool], List[int]] = {}
         # an entry that asks for several things: each is served like an entry's own request, and
         # the entry's view is the tuple of what they get
         spans: List[Optional[Tuple[int, int]]] = []
@@ -165,7 +183,7 @@ class CacheManager:
             if isinstance(r, KVRequest):
                 by_key.setdefault((r.kv_heads, r.head_dim, r.window, bool(r.values),
                                    (r.value_dim or r.head_dim) if r.values else 0,
-                                   r.keep_first if r.window > 0 else 0), []).append(i)
+                                   r.keep_first if r.window > 0 else 0, bool(r.codes)), []).append(i)
         group_of: Dict[int, Tuple[int, int]] = {}
         for key, entries in by_key.items():
             g = _KVGroup(key, entries, self.pages_total, dtype, self.device)
@@ -181,7 +199,8 @@ class CacheManager:
                 g = self.groups[gi]
                 nxt = (j + 1) % len(g.entries)  # (after the last layer: the first, in the next step)
                 self._views.append(KVView(gi, g.k[j], g.v[j] if g.values else None, PAGE_SIZE, g.window,
-                                          g.keep_first, (nxt - j) * g.k[0].numel()))
+                                          g.keep_first, (nxt - j) * g.k[0].numel(),
+                                          g.k_scales[j] if g.codes else None, g.v_scales[j] if g.codes else None))
             elif isinstance(r, StateRequest):
                 made = [torch.zeros((max_slots, *shape), dtype=dtype, device=self.device)
                         for shape, dtype in ((r.shape, r.dtype), *r.extra)]
@@ -316,11 +335,12 @@ class CacheManager:
     def _copy_pages(self, g: _KVGroup, moves) -> None:
         if self.device.type == "cuda":
             ops.copy_pages(g.k, g.v, moves)
+            if g.codes:
+                ops.copy_pages(g.k_scales.unsqueeze(-1), g.v_scales.unsqueeze(-1), moves)
             return
-        for t in (g.k, g.v):  # (host tests)
-            if t is not None:
-                for src, dst, rows in moves:
-                    t[:, dst, :, :rows] = t[:, src, :, :rows]
+        for t in g.stores():  # (host tests)
+            for src, dst, rows in moves:
+                t[:, dst, :, :rows] = t[:, src, :, :rows]
 
     def commit(self, slots: Sequence[int], new_lengths: Sequence[int]) -> None:
         """The step has been issued: lengths advance, windowed groups give back
@@ -499,13 +519,12 @@ class CacheManager:
     def kv_bytes_per_token(self) -> int:
         """Bytes of keys and values that one position of one sequence holds over all
         layers (a windowed group counted like a full one)."""
-        return sum(len(g.entries) * g.kv_heads * (g.head_dim + g.value_dim) * g.k.element_size()
-                   for g in self.groups)
+        return sum(len(g.entries) * g.position_bytes() for g in self.groups)
 
     def kv_bytes_read(self, length: int) -> int:
         """Bytes of keys and values that one more token of a sequence of ``length`` positions reads over all
         layers: a windowed group's window and kept first positions, the whole of another's."""
-        return sum(len(g.entries) * g.kv_heads * (g.head_dim + g.value_dim) * g.k.element_size()
+        return sum(len(g.entries) * g.position_bytes()
                    * (min(length, g.window + g.keep_first) if g.window > 0 else length) for g in self.groups)
 
     # -- telemetry (crates/nnis-rt/src/kv_telemetry.rs:42-80) ----------------
@@ -516,8 +535,7 @@ class CacheManager:
             "pages_shared": [len(g.extra) for g in self.groups],
             "live_tokens": sum(self.lengths[s] for s in range(self.slots.count)
                                if self.slots.is_held(s)),
-            "kv_bytes": sum(t.numel() * t.element_size() for g in self.groups for t in (g.k, g.v)
-                            if t is not None),
+            "kv_bytes": sum(t.numel() * t.element_size() for g in self.groups for t in g.stores()),
         }
 
     def check(self) -> None:

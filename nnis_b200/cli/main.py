@@ -21,15 +21,15 @@ DEFAULT_DEVICE_ORDINAL = 0
 DEFAULT_MAX_NEW_TOKENS = 16
 GENERATE_BATCH_JSON_SCHEMA_VERSION = 1
 USAGE = """Usage:
-  nnis generate --model DIR [--tokenizer FILE] --prompt TEXT | --prompt-ids IDS [--device N] [--max-new-tokens N] [--dtype bfloat16|float32] [--sample --seed U64] [--temperature F] [--top-k N] [--top-p F] [--stream]
-  nnis generate-batch --model DIR [--tokenizer FILE] --prompt TEXT [--prompt TEXT ...] | --prompt-ids IDS [--prompt-ids IDS ...] --seed U64 [--seed U64 ...] [--device N] [--max-new-tokens N] [--dtype bfloat16|float32] [--temperature F] [--top-k N] [--top-p F] [--share-prefix] [--json]
+  nnis generate --model DIR [--tokenizer FILE] --prompt TEXT | --prompt-ids IDS [--device N] [--max-new-tokens N] [--dtype bfloat16|float32] [--cache-dtype int8] [--weight-dtype int8] [--sample --seed U64] [--temperature F] [--top-k N] [--top-p F] [--stream]
+  nnis generate-batch --model DIR [--tokenizer FILE] --prompt TEXT [--prompt TEXT ...] | --prompt-ids IDS [--prompt-ids IDS ...] --seed U64 [--seed U64 ...] [--device N] [--max-new-tokens N] [--dtype bfloat16|float32] [--cache-dtype int8] [--weight-dtype int8] [--temperature F] [--top-k N] [--top-p F] [--share-prefix] [--json]
   nnis validate --model DIR [--tokenizer FILE] [--json] [--output FILE]
   nnis random-model --config FILE --seed U64 --out DIR [--format hf|nnis]
 
 `validate` checks config.json, the safetensors files (tensor names, shapes and dtypes against the model that config.json names) and, when a tokenizer is given or DIR/tokenizer.json exists, that its ids fit the vocabulary; it needs no GPU and reads no tensor. `--output FILE` requires `--json` and writes the report there, never over an existing file.
 `random-model` writes a model folder with seeded random weights from a config.json (`hf`: config.json + model.safetensors; `nnis`: model.json + raw tensor files); it needs no GPU.
 
-Default decoding on `generate` is greedy. Opt-in `--sample` requires `--seed`. Optional `--temperature`, `--top-k`, and `--top-p` apply only with `--sample`. `--stream` is valid only with `--sample` and prints each token as it is emitted. `generate-batch` requires one `--seed` per prompt and always samples; `--json` emits versioned JSON; `--share-prefix` runs tokens that prompts begin with alike once. CUDA device ordinal defaults to 0."""
+Default decoding on `generate` is greedy. Opt-in `--sample` requires `--seed`. Optional `--temperature`, `--top-k`, and `--top-p` apply only with `--sample`. `--stream` is valid only with `--sample` and prints each token as it is emitted. `generate-batch` requires one `--seed` per prompt and always samples; `--json` emits versioned JSON; `--share-prefix` runs tokens that prompts begin with alike once. `--cache-dtype int8` holds keys and values in 8 bits, `--weight-dtype int8` the layers' matrices. CUDA device ordinal defaults to 0."""
 
 
 class UsageError(Exception):
@@ -45,6 +45,8 @@ class GenerateArgs:
     device_ordinal: int = DEFAULT_DEVICE_ORDINAL
     max_new_tokens: int = DEFAULT_MAX_NEW_TOKENS
     dtype: str = "bfloat16"
+    cache_dtype: Optional[str] = None
+    weight_dtype: Optional[str] = None
     sample: bool = False
     stream: bool = False
     json: bool = False
@@ -138,6 +140,10 @@ def parse_args(argv: List[str]) -> Optional[GenerateArgs]:
             if value not in ("bfloat16", "float32"):
                 raise UsageError(f"--dtype must be bfloat16 or float32; got {value!r}")
             a.dtype = value
+        elif flag in ("--cache-dtype", "--weight-dtype"):
+            if value != "int8":
+                raise UsageError(f"{flag} must be int8 (without it, as --dtype says); got {value!r}")
+            setattr(a, flag[2:].replace("-", "_"), value)
         elif flag == "--seed":
             a.seeds.append(_unsigned(flag, value))
         elif flag == "--temperature":
@@ -339,7 +345,8 @@ def run(a: GenerateArgs, out=sys.stdout) -> int:
     prompts = a.prompts if a.prompts else a.prompt_ids
     llm = LLM(a.model_dir, dtype=a.dtype, device_ordinal=a.device_ordinal,
               tokenizer_file=a.tokenizer_file, max_batch=max(1, len(prompts)),
-              max_tokens=max(4096, sum(len(p) for p in prompts) + len(prompts) * (a.max_new_tokens + 64)))
+              max_tokens=max(4096, sum(len(p) for p in prompts) + len(prompts) * (a.max_new_tokens + 64)),
+              cache_dtype=a.cache_dtype, weight_dtype=a.weight_dtype)
 
     def text_of(ids):
         return llm.decode(ids) if llm.tokenizer is not None else " ".join(str(i) for i in ids)

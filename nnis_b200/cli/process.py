@@ -10,7 +10,7 @@ the record, :266-306 the call).  This is the same for ``bin/nnis generate``;
 ``nnis_b200.LLM`` is the in-process entry point.
 
 Additions: ``prompt_ids`` instead of ``prompt`` (then no tokenizer is needed and
-ids are printed), and ``dtype``.
+ids are printed), ``dtype``, and ``cache_dtype`` and ``weight_dtype`` ("int8": held in 8 bits).
 """
 from __future__ import annotations
 
@@ -169,7 +169,8 @@ def write_new_json(path: str, value: Dict[str, Any]) -> None:
 def execute(model_dir: str, tokenizer_file: Optional[str] = None, prompt: Optional[str] = None,
             device_ordinal: int = 0, max_new_tokens: int = 16, result_path: Optional[str] = None,
             timeout_seconds: float = DEFAULT_TIMEOUT_SECONDS, nnis_bin: Optional[str] = None,
-            prompt_ids: Optional[Sequence[int]] = None, dtype: str = "bfloat16") -> Dict[str, Any]:
+            prompt_ids: Optional[Sequence[int]] = None, dtype: str = "bfloat16", cache_dtype: Optional[str] = None,
+            weight_dtype: Optional[str] = None) -> Dict[str, Any]:
     """Greedy generation in a child process; the record is returned and, with
     ``result_path``, written there.  Raises ProcessContractError before anything
     runs, TimeoutError at the deadline, RuntimeError when the child fails."""
@@ -177,12 +178,17 @@ def execute(model_dir: str, tokenizer_file: Optional[str] = None, prompt: Option
                   timeout_seconds)
     if dtype not in ("bfloat16", "float32"):
         raise ProcessContractError(f"dtype must be bfloat16 or float32; got {dtype!r}")
+    if cache_dtype not in (None, "int8") or weight_dtype not in (None, "int8"):
+        raise ProcessContractError(f"cache_dtype and weight_dtype must be None or int8; got {cache_dtype!r} and {weight_dtype!r}")
     if result_path is not None and os.path.lexists(result_path):
         raise ProcessContractError(f"result path exists already: {result_path}")
     binary = nnis_bin if nnis_bin is not None else default_binary()
     command = [binary] if os.access(binary, os.X_OK) else [sys.executable, binary]
     command += ["generate", "--model", model_dir, "--device", str(device_ordinal),
                 "--max-new-tokens", str(max_new_tokens), "--dtype", dtype]
+    for flag, value in (("--cache-dtype", cache_dtype), ("--weight-dtype", weight_dtype)):
+        if value is not None:
+            command += [flag, value]
     if tokenizer_file is not None:
         command += ["--tokenizer", tokenizer_file]
     if prompt is not None:
@@ -196,6 +202,8 @@ def execute(model_dir: str, tokenizer_file: Optional[str] = None, prompt: Option
     inputs = {"model_directory": model_dir, "tokenizer_file": tokenizer_file, "prompt": prompt,
               "prompt_ids": list(prompt_ids) if prompt_ids is not None else None,
               "device_ordinal": device_ordinal, "max_new_tokens": max_new_tokens, "dtype": dtype}
+    if cache_dtype is not None or weight_dtype is not None:
+        inputs.update(cache_dtype=cache_dtype, weight_dtype=weight_dtype)
     result = build_result(inputs, stdout, stderr)
     if result_path is not None:
         write_new_json(result_path, result)

@@ -3112,6 +3112,10 @@ def read_pages_int8(k: torch.Tensor, v: torch.Tensor, k_scales: torch.Tensor, v_
         shape[3], _stream_of(index)), "read_pages_int8")
 
 
+# A prompt step whose sequences bring at most this many tokens each attends over the codes row by row; others read their pages back.
+INT8_ROWS_AT_ONCE = 16
+
+
 def attention_int8_splits(n: int, heads: int, keys: int, device) -> int:
     """Into how many slices the keys of a row are cut where ``n`` rows of ``heads`` heads see at most ``keys`` of them: a warp a slice,
     sixteen warps an SM, at least 128 keys each, at most 64."""

@@ -326,13 +326,17 @@ class LLM:
                  device: Optional[str] = None, max_tokens: Optional[int] = None,
                  max_batch: int = 64, tokenizer_file: Optional[str] = None,
                  pipeline_decode: bool = True, device_sampling: bool = False,
-                 max_step_tokens: int = 16384):
+                 max_step_tokens: int = 16384, cache_dtype: Optional[str] = None, weight_dtype: Optional[str] = None):
+        """``cache_dtype="int8"``: keys and values are held in 8-bit codes with a scale for every position and head, half the bytes of
+        bfloat16 to keep and to read.  ``weight_dtype="int8"``: the layers' matrices in 8-bit codes with a scale for each output
+        channel, multiplied with each token's activations in 8-bit codes as whole numbers; embedding and head keep their type.
+        Either, both or none; refused with a ValueError for models whose layers have no such form (``Llama`` has both)."""
         device = device if device is not None else f"cuda:{int(device_ordinal)}"
         self.max_batch = max_batch
         if max_tokens is None:
             max_tokens = 1 << 17
         self.engine = Engine.from_dir(model_dir, dtype=dtype, device=device, max_tokens=max_tokens,
-                                      max_slots=max(max_batch, 1))
+                                      max_slots=max(max_batch, 1), cache_dtype=cache_dtype, weight_dtype=weight_dtype)
         self.spec = self.engine.spec
         self.tokenizer = load_tokenizer(tokenizer_file) if tokenizer_file else None
         self.backend = EngineBackend(self.engine, max_batch, pipeline_decode, max_step_tokens)

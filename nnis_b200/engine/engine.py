@@ -65,12 +65,14 @@ def require_cuda(device) -> torch.device:
 
 class Engine:
     def __init__(self, spec: ModelSpec, tensors: Mapping[str, torch.Tensor], dtype="bfloat16",
-                 device="cuda:0", max_tokens: int = 1 << 16, max_slots: Optional[int] = None):
+                 device="cuda:0", max_tokens: int = 1 << 16, max_slots: Optional[int] = None,
+                 cache_dtype: Optional[str] = None, weight_dtype: Optional[str] = None):
+        """``cache_dtype`` and ``weight_dtype``: "int8" holds the cache, the blocks' matrices in 8 bits (``DecoderModel``)."""
         self.device = require_cuda(device)
         self.dtype = _DTYPES[dtype]
         self.spec = spec
         torch.cuda.set_device(self.device)
-        self.model = DecoderModel(spec, self.dtype, self.device)
+        self.model = DecoderModel(spec, self.dtype, self.device, cache_dtype, weight_dtype)
         self.model.load(tensors)
         pages = -(-max_tokens // PAGE_SIZE)
         self.max_slots = max_slots if max_slots is not None else min(pages, 1024)

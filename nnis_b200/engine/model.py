@@ -16,7 +16,11 @@ from ..weights.loader import WeightSpec
 
 
 class DecoderModel:
-    def __init__(self, spec: ModelSpec, dtype: torch.dtype, device: torch.device):
+    def __init__(self, spec: ModelSpec, dtype: torch.dtype, device: torch.device, cache_dtype: Optional[str] = None,
+                 weight_dtype: Optional[str] = None):
+        """``cache_dtype`` "int8": keys and values are held in 8-bit codes with a scale for every position and head.
+        ``weight_dtype`` "int8": the blocks' matrices are held in 8-bit codes with a scale for each output channel (embedding and
+        head keep their type).  None: as ``dtype`` says.  Both are refused for a model with a part that has no such form."""
         spec.validate()
         if dtype not in (torch.float32, torch.bfloat16):
             raise ValueError(f"compute dtype must be float32 or bfloat16; got {dtype}")
@@ -24,6 +28,7 @@ class DecoderModel:
         self.embedding = EMBEDDINGS.build(spec.embedding.kind, spec.embedding.params, "", dtype,
                                           self.device)
         self.blocks = [BLOCKS.build(layer.block, layer, dtype, self.device) for layer in spec.layers]
+        self._in_int8(cache_dtype, weight_dtype)
         self.final_norm = NORMS.build(spec.final_norm.kind, spec.final_norm.params, "", dtype,
                                       self.device)
         self.head = HEADS.build(spec.head.kind, spec.head.params, "", dtype, self.device)
@@ -40,6 +45,21 @@ class DecoderModel:
             if entry.cache_of is not None and wants is not None:
                 raise ValueError(f"schedule[{i}] reads the cache of entry {entry.cache_of} but its "
                                  f"mixer writes one of its own")
+
+    def _in_int8(self, cache_dtype: Optional[str], weight_dtype: Optional[str]) -> None:
+        for what, value in (("cache_dtype", cache_dtype), ("weight_dtype", weight_dtype)):
+            if value not in (None, "int8"):
+                raise ValueError(f"{what} must be None or 'int8'; got {value!r}")
+        self.weights_in_int8 = weight_dtype == "int8"
+        for layer, block in enumerate(self.blocks):
+            if cache_dtype == "int8" and block.mixer is not None:
+                if getattr(block.mixer, "cache_in_int8", None) is not None:
+                    block.mixer.cache_in_int8()
+                else:
+                    raise ValueError(f"cache_dtype='int8': layer {layer}'s mixer ({type(block.mixer).__name__}) has no 8-bit cache")
+            for part in block.parts() if self.weights_in_int8 else ():
+                if getattr(part, "hold_int8", None) is None and any(w.role == "matrix" for w in part.weight_specs().values()):
+                    raise ValueError(f"weight_dtype='int8': layer {layer}'s {type(part).__name__} has no 8-bit product")
 
     # -- weights ------------------------------------------------------------
     def weight_specs(self) -> Dict[str, WeightSpec]:
@@ -61,6 +81,11 @@ class DecoderModel:
     def load(self, tensors: Mapping[str, torch.Tensor]) -> None:
         for part in (self.embedding, *self.blocks, self.final_norm, self.head):
             part.load(tensors)
+        if self.weights_in_int8:
+            for block in self.blocks:
+                for part in block.parts():
+                    if getattr(part, "hold_int8", None) is not None:
+                        part.hold_int8()
         self._enter_tensors = {name: tensors[name].to(torch.float32).contiguous() for name, _ in self._enter_names}
 
     def parameter_bytes(self) -> int:

@@ -11,6 +11,10 @@ params: hidden_size, heads, kv_heads, head_dim, bias, window (0: all keys),
 position (a PartSpec), names {q, k, v, o}, kv ("own" | "shared").  With
 ``kv == "shared"`` the part has no k/v projection and reads the cache that the
 model hands it (another schedule entry's).
+
+The cache may be held in 8 bits (``cache_in_int8``) and the matrices too (``hold_int8``).  With an 8-bit cache the rows are
+projected, then rotated and put into codes by one kernel; single tokens, and a few of a sequence, read the codes as they are, and a
+prompt step reads its sequences' pages back into scratch, a layer at a time, and takes the kernels of the 16-bit (or float32) cache.
 """
 from __future__ import annotations
 
@@ -24,10 +28,12 @@ from ..cache import PAGE_SIZE, KVRequest, KVView
 from ..csrc import ops
 from ..weights.loader import WeightSpec
 from .base import MIXERS, POSITIONS, Part, begin_norm
-from .linear import ADD_F32, STORE, linear
+from .linear import ADD_F32, STORE, Int8Matrix, linear, matrix_bytes
 
 
 class Attention(Part):
+    codes = False  # the cache holds 8-bit codes
+
     def __init__(self, params, prefix, dtype, device):
         super().__init__(params, prefix, dtype, device)
         self.hidden = int(params["hidden_size"])
@@ -78,22 +84,30 @@ class Attention(Part):
                                    0).contiguous()
             self.b_o = tensors[self.tensor_name(self.names["o"], "bias")]
 
+    def hold_int8(self) -> None:
+        """The loaded matrices become 8-bit codes with a scale for each output channel."""
+        self.w_qkv, self.w_o = Int8Matrix.of(self.w_qkv), Int8Matrix.of(self.w_o)
+
     def parameter_bytes(self) -> int:
-        return sum(t.numel() * t.element_size() for t in (self.w_qkv, self.w_o, self.b_qkv, self.b_o)
-                   if t is not None)
+        return sum(matrix_bytes(t) for t in (self.w_qkv, self.w_o, self.b_qkv, self.b_o))
 
     # -- cache ------------------------------------------------------------
+    def cache_in_int8(self) -> None:
+        """Keys and values are held in 8-bit codes with a scale for every position and head."""
+        self.codes = True
+
     def cache_request(self) -> Optional[KVRequest]:
-        return KVRequest(self.kv_heads, self.head_dim, self.window) if self.own_kv else None
+        return KVRequest(self.kv_heads, self.head_dim, self.window, codes=self.codes) if self.own_kv else None
 
     def check_shared_cache(self, view: KVView) -> None:
         if not isinstance(view, KVView) or tuple(view.k.shape[1:]) != \
-                (self.kv_heads, view.page_size, self.head_dim) or view.window != self.window:
+                (self.kv_heads, view.page_size, self.head_dim) or view.window != self.window \
+                or (view.k_scales is not None) != self.codes:
             raise ValueError("the shared cache does not fit this attention's heads or window")
 
     def shared_key(self, view: KVView):
         """What a plan for pages that several rows share is made for (None: this attention reads them row by row)."""
-        if self.window > 0 or not ops.attention_shared_takes(self.head_dim, view.page_size):
+        if self.window > 0 or self.codes or not ops.attention_shared_takes(self.head_dim, view.page_size):
             return None
         return view.group, self.heads, self.kv_heads, self.head_dim
 
@@ -114,6 +128,23 @@ class Attention(Part):
     def _wide_plan_name(self) -> str:
         return f"prefill_wide/window{self.window}/heads{self.heads}"
 
+    def _read_back_name(self) -> str:
+        return f"int8_pages/window{self.window}"
+
+    def _read_back_table(self, counts, starts):
+        """Which pages of an 8-bit cache a prompt step reads back, and to which places: [sequences, columns], -1 for pages that lie
+        before every window.  None where every sequence brings few tokens: their rows read the codes as they are."""
+        if max(counts) <= ops.INT8_ROWS_AT_ONCE:
+            return None
+        spans = [(max(0, s - self.window + 1) // PAGE_SIZE if self.window > 0 else 0, -(-(s + c) // PAGE_SIZE))
+                 for c, s in zip(counts, starts)]
+        table = np.full((len(spans), max(b for _, b in spans)), -1, dtype=np.int32)
+        at = 0
+        for row, (a, b) in zip(table, spans):
+            row[a:b] = np.arange(at, at + b - a)
+            at += b - a
+        return table, at
+
     TILES_64 = "prefill_mma/tiles64"  # (sequence, first query) per 64 queries of the step
 
     def step_tables(self, counts, starts, have=()):
@@ -122,7 +153,24 @@ class Attention(Part):
         and number of heads, where they pay; else the 64-query tiles of the
         mma.sync kernel (head sizes 64 and 128), the same for every layer.  In float32
         the units of the tensor cores' kernel (head size 64) where it pays; 64-query tiles, the ones
-        with the most keys first, for other head sizes and for steps of single pages, where those pay."""
+        with the most keys first, for other head sizes and for steps of single pages, where those pay.
+        With an 8-bit cache, before all: the pages to read back."""
+        if self.codes:
+            name = self._read_back_name()
+            if name + "/pages" in have:  # (a layer of this window has asked)
+                places, read = {}, None
+            else:
+                read = self._read_back_table(counts, starts)
+                places = {name + "/pages": np.asarray([read[1] if read else 0], dtype=np.int32)}
+                if read:
+                    places[name] = read[0]
+            if max(counts) <= ops.INT8_ROWS_AT_ONCE:
+                return places
+            places.update(self._kernel_tables(counts, starts, have))
+            return places
+        return self._kernel_tables(counts, starts, have)
+
+    def _kernel_tables(self, counts, starts, have):
         if self.dtype != torch.bfloat16:
             split, name = self._split_f32(self.heads * self.head_dim), self._tile_f32_name()
             tables: Dict[str, object] = {}
@@ -179,12 +227,12 @@ class Attention(Part):
     # -- run --------------------------------------------------------------
     def _decode_kernels(self, ctx, n: int, normed: bool = False) -> bool:
         """The fused bfloat16 decode kernel for q, k, v: few rows, one token each."""
-        return (self.dtype == torch.bfloat16 and ctx.decode
+        return (self.dtype == torch.bfloat16 and ctx.decode and not self.codes and not isinstance(self.w_qkv, Int8Matrix)
                 and self.head_dim % 16 == 0 and self.position_in_kernel
                 and ops.gemv_pays(n, self.w_qkv.shape[0], self.hidden, ops.EPI_QKV, self.device, normed))
 
     def _fused_out(self, ctx, n: int) -> bool:
-        return (self.dtype == torch.bfloat16 and ctx.decode
+        return (self.dtype == torch.bfloat16 and ctx.decode and not isinstance(self.w_o, Int8Matrix)
                 and ops.gemv_pays(n, self.hidden, self.heads * self.head_dim, ops.EPI_ADD_F32,
                                   self.device))
 
@@ -194,7 +242,7 @@ class Attention(Part):
     def shares_norm(self, norm, ctx, n: int) -> bool:
         """Whether the q, k, v projection can end a norm that the projection before it began."""
         return (getattr(norm, "kind", None) == "rmsnorm" and self.dtype == torch.bfloat16 and ctx.decode
-                and self.head_dim % 16 == 0 and self.position_in_kernel
+                and not self.codes and not isinstance(self.w_qkv, Int8Matrix) and self.head_dim % 16 == 0 and self.position_in_kernel
                 and ops.gemv_shares_norm(n, self.w_qkv.shape[0], self.hidden, ops.EPI_QKV, self.device))
 
     def forward(self, x: torch.Tensor, ctx, residual: torch.Tensor, cache: KVView) -> None:
@@ -233,7 +281,7 @@ class Attention(Part):
         cos, sin = tables if tables is not None else (None, None)
         attn = ws.get("attn", (n, nq * d), self.dtype)
         # the tensor-core decode attention: a CTA per (kv head, up to 16 query heads, slice)
-        mma_decode = self.dtype == torch.bfloat16 and ctx.decode and n <= 65535 \
+        mma_decode = self.dtype == torch.bfloat16 and ctx.decode and n <= 65535 and not self.codes \
             and ops.attention_decode_mma_takes(d, cache.page_size)
         # rows whose sequences begin with the same pages read those once for all of them
         key = self.shared_key(cache) if ctx.shared is not None else None
@@ -258,7 +306,8 @@ class Attention(Part):
                           # pages before its wait: it may start together with this one
                           release_early=tma_splits > 0)
             q_buf, q_stride = q, nq * d
-        elif self.dtype == torch.bfloat16 and ops.gemm_tc_qkv_takes(d) and self.position_in_kernel \
+        elif self.dtype == torch.bfloat16 and not self.codes and not isinstance(self.w_qkv, Int8Matrix) \
+                and ops.gemm_tc_qkv_takes(d) and self.position_in_kernel \
                 and ops.gemm_tc_takes(n, self.w_qkv.shape[0], self.hidden):
             # tensor-core product with bias, RoPE and the cache store in its epilogue
             q = ws.get("q", (n, nq * d), self.dtype)
@@ -270,14 +319,25 @@ class Attention(Part):
             q_buf, q_stride = q, nq * d
         else:
             qkv = ws.get("qkv", (n, (nq + 2 * self.stored_kv) * d), self.dtype)
-            linear(x, self.w_qkv, self.b_qkv, qkv, STORE)
+            linear(x, self.w_qkv, self.b_qkv, qkv, STORE, ws, decode=ctx.decode and self.codes)
             if not self.position_in_kernel:  # an encoding with arithmetic of its own
                 self.position.apply(qkv, ctx, nq, self.stored_kv, d)
-            ops.rope_store(qkv, ctx.token_pos, ctx.token_seq, table if self.own_kv else None, cos,
-                           sin, cache.k if self.own_kv else None, cache.v if self.own_kv else None,
-                           nq, self.stored_kv, d, cache.page_size)
-            q_buf, q_stride = qkv, qkv.shape[1]
-        if shared is not None:
+            if self.codes and self.own_kv:
+                q_buf, q_stride = ws.get("q", (n, nq * d), self.dtype), nq * d
+                ops.rope_store_int8(qkv, q_buf, ctx.token_pos, ctx.token_seq, table, cos, sin, cache.k, cache.v, cache.k_scales,
+                                    cache.v_scales, nq, nkv, d, cache.page_size)
+            else:
+                ops.rope_store(qkv, ctx.token_pos, ctx.token_seq, table if self.own_kv else None, cos,
+                               sin, cache.k if self.own_kv else None, cache.v if self.own_kv else None,
+                               nq, self.stored_kv, d, cache.page_size)
+                q_buf, q_stride = qkv, qkv.shape[1]
+        from_codes = self.codes and (ctx.decode or self._read_back_name() not in ctx.tables)
+        if self.codes and not from_codes:
+            cache, table = self._read_back(ctx, cache, table)
+        if from_codes:
+            ops.attention_int8(q_buf, q_stride, cache.k, cache.v, cache.k_scales, cache.v_scales, ctx.token_pos, ctx.token_seq, table,
+                               attn, nq, nkv, d, self.window, self.scale, ws)
+        elif shared is not None:
             ops.attention_shared(q_buf, q_stride, cache.k, cache.v, ctx.token_pos, table, shared, attn, nq, nkv, d, self.scale, ws)
         elif tma_splits:
             partial = tickets = None
@@ -353,6 +413,15 @@ class Attention(Part):
                           split=ops.gemv_split(n, *self.w_o.shape, ws))
         else:
             linear(attn, self.w_o, self.b_o, residual, ADD_F32, ws)
+
+    def _read_back(self, ctx, cache: KVView, table: torch.Tensor):
+        """A prompt step's pages of an 8-bit cache as values of the operands' type in scratch: a view of them and their page table."""
+        name, ws = self._read_back_name(), ctx.workspace
+        local, pages = ctx.tables[name], int(ctx.host_tables[name + "/pages"][0])
+        shape = (pages, self.kv_heads, cache.page_size, self.head_dim)
+        k, v = ws.get("int8_k_read", shape, self.dtype), ws.get("int8_v_read", shape, self.dtype)
+        ops.read_pages_int8(cache.k, cache.v, cache.k_scales, cache.v_scales, table, local, k, v)
+        return KVView(cache.group, k, v, cache.page_size, cache.window), local
 
 
 MIXERS.register("attention", Attention)

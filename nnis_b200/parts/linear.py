@@ -9,7 +9,8 @@ projection plans (crates/nnis-model/src/projection_plan.rs:10-90).
 """
 from __future__ import annotations
 
-from typing import Optional
+from dataclasses import dataclass
+from typing import Optional, Union
 
 import torch
 
@@ -18,13 +19,43 @@ from ..csrc import ops
 STORE, STORE_F32, ADD_F32 = ops.STORE, ops.STORE_F32, ops.ADD_F32
 
 
-def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor], out: torch.Tensor,
+@dataclass
+class Int8Matrix:
+    """A matrix [n, k] held in 8-bit codes with a scale for each of its rows (``ops.quantize_rows``), a projection's output channels."""
+    codes: torch.Tensor   # int8 [n, ops.int8_width(k)]
+    scales: torch.Tensor  # float32 [n]
+    shape: tuple
+
+    @classmethod
+    def of(cls, weight: torch.Tensor) -> "Int8Matrix":
+        n, k = weight.shape
+        codes = torch.empty((n, ops.int8_width(k)), dtype=torch.int8, device=weight.device)
+        scales = torch.empty(n, dtype=torch.float32, device=weight.device)
+        ops.quantize_rows(weight, codes, scales)
+        return cls(codes, scales, (n, k))
+
+    def bytes(self) -> int:
+        return self.codes.numel() + 4 * self.scales.numel()
+
+
+def matrix_bytes(weight: Union[None, torch.Tensor, Int8Matrix]) -> int:
+    """Bytes of a matrix or a bias as it is held; 0 for None."""
+    if weight is None:
+        return 0
+    return weight.bytes() if isinstance(weight, Int8Matrix) else weight.numel() * weight.element_size()
+
+
+def linear(x: torch.Tensor, weight: Union[torch.Tensor, Int8Matrix], bias: Optional[torch.Tensor], out: torch.Tensor,
            mode: int, workspace=None, decode: bool = False) -> None:
     """``workspace``: the step's buffers (``engine.workspace.Workspace``); with it the adding
     tensor-core product may cut a long K among several CTAs per tile (few rows, few tiles),
     which needs scratch for their partial sums.  ``decode``: the step brings one token per
     sequence; a bfloat16 product of few rows then runs as a decode projection kernel (weights
-    by bulk copies ahead of the wait for the kernel before) where that kernel takes the shape."""
+    by bulk copies ahead of the wait for the kernel before) where that kernel takes the shape.
+    A matrix in 8-bit codes is multiplied as such, which needs the workspace."""
+    if isinstance(weight, Int8Matrix):
+        ops.linear_int8(x, weight.codes, weight.scales, bias, out, mode, workspace)
+        return
     m, (n, k) = x.shape[0], weight.shape
     if decode and x.dtype == torch.bfloat16 and ops.gemv_pays(m, n, k, mode, x.device):
         split = ops.gemv_split(m, n, k, workspace) if mode == ADD_F32 and workspace is not None else None

@@ -21,7 +21,7 @@ import torch
 from ..csrc import ops
 from ..weights.loader import WeightSpec
 from .base import FEED_FORWARDS, Part, begin_norm
-from .linear import ADD_F32, STORE_F32, linear
+from .linear import ADD_F32, STORE_F32, Int8Matrix, linear, matrix_bytes
 
 
 class GatedMLP(Part):
@@ -63,9 +63,12 @@ class GatedMLP(Part):
                                    tensors[self.tensor_name(n["up"], "bias")]], 0).contiguous()
             self.b_down = tensors[self.tensor_name(n["down"], "bias")]
 
+    def hold_int8(self) -> None:
+        """The loaded matrices become 8-bit codes with a scale for each output channel."""
+        self.w_gu, self.w_down = Int8Matrix.of(self.w_gu), Int8Matrix.of(self.w_down)
+
     def parameter_bytes(self) -> int:
-        return sum(t.numel() * t.element_size()
-                   for t in (self.w_gu, self.w_down, self.b_gu, self.b_down) if t is not None)
+        return sum(matrix_bytes(t) for t in (self.w_gu, self.w_down, self.b_gu, self.b_down))
 
     def step_flops(self, counts, starts) -> float:
         return 2.0 * 3 * self.hidden * self.inter * sum(counts)
@@ -73,10 +76,10 @@ class GatedMLP(Part):
     def _fused_gate_up(self, ctx, n: int, normed: bool = False) -> bool:
         """The fused bfloat16 decode kernel for gate/up (few rows, one token each)."""
         return (self.dtype == torch.bfloat16 and ctx.decode and self.fused_act is not None
-                and ops.gemv_pays(n, 2 * self.inter, self.hidden, ops.EPI_GATED, self.device, normed))
+                and not isinstance(self.w_gu, Int8Matrix) and ops.gemv_pays(n, 2 * self.inter, self.hidden, ops.EPI_GATED, self.device, normed))
 
     def _fused_down(self, ctx, n: int) -> bool:
-        return (self.dtype == torch.bfloat16 and ctx.decode
+        return (self.dtype == torch.bfloat16 and ctx.decode and not isinstance(self.w_down, Int8Matrix)
                 and ops.gemv_pays(n, self.hidden, self.inter, ops.EPI_ADD_F32, self.device))
 
     def fuses_norm(self, norm, ctx, n: int) -> bool:
@@ -85,7 +88,7 @@ class GatedMLP(Part):
     def shares_norm(self, norm, ctx, n: int) -> bool:
         """Whether gate/up can end a norm that the projection before it began."""
         return (getattr(norm, "kind", None) == "rmsnorm" and self.dtype == torch.bfloat16 and ctx.decode
-                and self.fused_act is not None
+                and self.fused_act is not None and not isinstance(self.w_gu, Int8Matrix)
                 and ops.gemv_shares_norm(n, 2 * self.inter, self.hidden, ops.EPI_GATED, self.device))
 
     def forward(self, x: torch.Tensor, ctx, residual: torch.Tensor) -> None:
@@ -110,6 +113,11 @@ class GatedMLP(Part):
             ops.gemv_bf16(self.w_gu, self.b_gu, act, ops.EPI_GATED, x=x, hidden=hidden,
                           norm_weight=norm.weight if norm is not None else None,
                           eps=norm.eps if norm is not None else 0.0, m=n, act=self.fused_act)
+        elif isinstance(self.w_gu, Int8Matrix):
+            if self.activation == "silu":  # (in the product's epilogue)
+                ops.linear_int8(x, self.w_gu.codes, self.w_gu.scales, self.b_gu, act, ops.GEMM_GATED, ws)
+            else:
+                self._activate_apart(x, act, ctx)
         elif self.activation == "silu" and self.dtype == torch.bfloat16 \
                 and ops.gemm_tc_takes(n, 2 * self.inter, self.hidden):
             # tensor-core product with the activation in its epilogue
@@ -125,19 +133,23 @@ class GatedMLP(Part):
             # the same product with the clamped activation in its epilogue
             ops.gemm_tc_glu_clamp(x, self.w_gu, self.b_gu, act, self.limit, self.alpha)
         else:
-            gate_up = ws.get("gate_up", (n, 2 * self.inter), torch.float32)
-            linear(x, self.w_gu, self.b_gu, gate_up, STORE_F32, decode=ctx.decode)
-            if self.activation == "silu":
-                ops.silu_mul(gate_up, act)
-            elif self.activation == "gelu_tanh":
-                ops.gelu_mul(gate_up, act)
-            else:
-                ops.glu_clamp(gate_up, act, self.limit, self.alpha)
+            self._activate_apart(x, act, ctx)
         if self._fused_down(ctx, n):
             ops.gemv_bf16(self.w_down, self.b_down, residual, ops.EPI_ADD_F32, x=act,
                           emit=begin_norm(ctx, n, self.hidden), split=ops.gemv_split(n, self.hidden, self.inter, ws))
         else:
             linear(act, self.w_down, self.b_down, residual, ADD_F32, ws)
+
+    def _activate_apart(self, x: torch.Tensor, act: torch.Tensor, ctx) -> None:
+        """Gate and up as a float32 product, the activation by a kernel of its own."""
+        gate_up = ctx.workspace.get("gate_up", (x.shape[0], 2 * self.inter), torch.float32)
+        linear(x, self.w_gu, self.b_gu, gate_up, STORE_F32, ctx.workspace, decode=ctx.decode)
+        if self.activation == "silu":
+            ops.silu_mul(gate_up, act)
+        elif self.activation == "gelu_tanh":
+            ops.gelu_mul(gate_up, act)
+        else:
+            ops.glu_clamp(gate_up, act, self.limit, self.alpha)
 
 
 class DenseMLP(Part):
@@ -171,8 +183,12 @@ class DenseMLP(Part):
         self.w_up = tensors[self.tensor_name(self.names["up"])]
         self.w_down = tensors[self.tensor_name(self.names["down"])]
 
+    def hold_int8(self) -> None:
+        """The loaded matrices become 8-bit codes with a scale for each output channel."""
+        self.w_up, self.w_down = Int8Matrix.of(self.w_up), Int8Matrix.of(self.w_down)
+
     def parameter_bytes(self) -> int:
-        return sum(t.numel() * t.element_size() for t in (self.w_up, self.w_down))
+        return sum(matrix_bytes(t) for t in (self.w_up, self.w_down))
 
     def step_flops(self, counts, starts) -> float:
         return 2.0 * 2 * self.hidden * self.inter * sum(counts)
@@ -183,14 +199,15 @@ class DenseMLP(Part):
         kind = self.ACTIVATIONS[self.activation]
         act = ws.get("act", (n, self.inter), self.dtype)
         # bfloat16: the activation rides in the first product's epilogue (the float32 sums, rounded once)
-        if self.dtype == torch.bfloat16 and ctx.decode and ops.gemv_pays(n, self.inter, self.hidden, ops.EPI_STORE,
-                                                                         x.device):
+        codes = isinstance(self.w_up, Int8Matrix)
+        if self.dtype == torch.bfloat16 and ctx.decode and not codes and ops.gemv_pays(n, self.inter, self.hidden, ops.EPI_STORE,
+                                                                                       x.device):
             ops.gemv_bf16(self.w_up, None, act, ops.EPI_STORE, x=x, act=self.FUSED[kind])
-        elif self.dtype == torch.bfloat16 and ops.gemm_tc_takes(n, self.inter, self.hidden):
+        elif self.dtype == torch.bfloat16 and not codes and ops.gemm_tc_takes(n, self.inter, self.hidden):
             ops.gemm_tc_act(x, self.w_up, None, act, self.FUSED[kind])
         else:
             up = ws.get("mlp_up", (n, self.inter), torch.float32)
-            linear(x, self.w_up, None, up, STORE_F32, decode=ctx.decode)
+            linear(x, self.w_up, None, up, STORE_F32, ws, decode=ctx.decode)
             ops.act_rows(up, act, kind)
         linear(act, self.w_down, None, residual, ADD_F32, ws, decode=ctx.decode)
 

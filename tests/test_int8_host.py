@@ -116,3 +116,81 @@ def test_codes_of_bfloat16_rows_are_the_exact_quotients():
         half = 2 * rows[:, 0] == rows[:, 1]
         assert torch.equal(codes[~half, 0].double(), (whole + up)[~half])
         assert ((codes[half, 0] == 63) | (codes[half, 0] == 64)).all()
+
+
+# ---- the cache, the model and the command line --------------------------------------------------
+def test_pages_of_codes_are_copied_with_their_scales():
+    from nnis_b200.cache import CacheManager, KVRequest
+    cache = CacheManager([KVRequest(2, 8, codes=True)] * 3 + [KVRequest(2, 8)], F32, torch.device("cpu"), 64 * 8, 4, 1000)
+    codes, wide = cache.groups
+    assert (codes.k.dtype, wide.k.dtype, codes.k_scales.shape, wide.k_scales) == (I8, F32, (3, 8, 2, 64), None)
+    view = cache.view(1)
+    assert view.k_scales.shape == (8, 2, 64) and view.v_scales.data_ptr() == codes.v_scales[1].data_ptr() and cache.view(3).k_scales is None
+    a = cache.acquire()
+    cache.reserve([a], [70])
+    cache.commit([a], [70])
+    for t in codes.stores():
+        t[:, cache.page_table(0, a)[1], :, :6] = 9
+    b = cache.fork(a)
+    cache.reserve([b], [71])
+    cache.commit([b], [71])
+    mine, copy = cache.page_table(0, a)[1], cache.page_table(0, b)[1]
+    assert mine != copy and all((t[:, copy, :, :6] == 9).all() and (t[:, copy, :, 6:] == 0).all() for t in codes.stores())
+    assert cache.kv_bytes_per_token() == 3 * 2 * (16 + 8) + 2 * 16 * 4
+    assert cache.kv_bytes_read(10) == 10 * cache.kv_bytes_per_token()
+    assert cache.usage()["kv_bytes"] == 8 * 64 * cache.kv_bytes_per_token()
+    cache.check()
+
+
+def test_a_cache_of_codes_without_values_is_refused():
+    from nnis_b200.cache import CacheManager, KVRequest
+    with pytest.raises(ValueError, match="keys and values"):
+        CacheManager([KVRequest(1, 8, values=False, codes=True)], F32, torch.device("cpu"), 64, 1, 64)
+
+
+def test_models_without_an_8_bit_form_are_refused():
+    import nafezen_models
+    from helpers import TINY_A
+    from nnis_b200.config import config_from_dict
+    from nnis_b200.engine.model import DecoderModel
+    cpu = torch.device("cpu")
+    llama, other = config_from_dict(TINY_A).to_spec(), config_from_dict(nafezen_models.CONFIGS["mixed"]).to_spec()
+    model = DecoderModel(llama, F32, cpu, "int8", "int8")
+    assert all(r is None or r.codes for r in model.cache_requests())
+    assert not any(r is not None and r.codes for r in DecoderModel(llama, F32, cpu).cache_requests())
+    for args, why in ((("int8", None), "no 8-bit cache"), ((None, "int8"), "no 8-bit product")):
+        with pytest.raises(ValueError, match=why):
+            DecoderModel(other, F32, cpu, *args)
+    for args in (("fp8", None), (None, "int4")):
+        with pytest.raises(ValueError, match="must be None or 'int8'"):
+            DecoderModel(llama, F32, cpu, *args)
+
+
+def test_pages_that_a_prompt_step_reads_back():
+    from nnis_b200.config import config_from_dict
+    from nnis_b200.csrc import ops
+    from nnis_b200.engine.model import DecoderModel
+    from helpers import TINY_A
+    spec = config_from_dict(TINY_A).to_spec()
+    mixer = DecoderModel(spec, BF16, torch.device("cpu"), "int8").blocks[0].mixer
+    few, many = ops.INT8_ROWS_AT_ONCE, ops.INT8_ROWS_AT_ONCE + 1
+    name = mixer._read_back_name()
+    assert name not in mixer.step_tables([few, 1], [100, 0])
+    tables = mixer.step_tables([1, many, 64], [100, 64, 0])
+    assert tables[name].tolist() == [[0, 1], [2, 3], [4, -1]] and tables[name + "/pages"].tolist() == [5]
+    assert name not in mixer.step_tables([many], [0], tuple(tables))  # (another layer has asked)
+    mixer.window = 70
+    assert mixer._read_back_table([many, 20], [200, 63])[0].tolist() == [[-1, -1, 0, 1], [2, 3, -1, -1]]
+
+
+def test_flags_of_the_command_line():
+    from nnis_b200.cli.main import UsageError, parse_args
+    from nnis_b200.cli.process import ProcessContractError, execute
+    base = ["generate", "--model", "m", "--prompt-ids", "1,2"]
+    a = parse_args([*base, "--cache-dtype", "int8"])
+    assert (a.cache_dtype, a.weight_dtype) == ("int8", None) and parse_args([*base, "--weight-dtype", "int8"]).weight_dtype == "int8"
+    for flag in ("--cache-dtype", "--weight-dtype"):
+        with pytest.raises(UsageError, match="must be int8"):
+            parse_args([*base, flag, "float32"])
+    with pytest.raises((ProcessContractError, ValueError)):
+        execute("m", prompt_ids=[1], cache_dtype="fp8")
