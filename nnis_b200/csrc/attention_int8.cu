@@ -6,24 +6,11 @@
 #include <float.h>
 #include <string.h>
 
+#include "attention_int8.cuh"
 #include "attention_merge.cuh"
 #include "int8_rows.cuh"
 
 namespace nnis {
-
-struct Attend8 {
-    const void* q;
-    long long q_stride;
-    const int8_t *k, *v;
-    const float *k_scales, *v_scales;
-    const int *token_pos, *token_seq, *page_table;
-    int table_rows, table_cols, pages;
-    void* out;
-    float* partial;
-    int n, nq, nkv, d, page_size, window;
-    float scale;
-    int splits;
-};
 
 template <typename T, int R>
 __global__ void __launch_bounds__(128) attn_int8_warp_kernel(const __grid_constant__ Attend8 p) {
@@ -127,31 +114,46 @@ static cudaError_t launch_warps8(const Attend8& p, cudaStream_t stream) {
 
 }  // namespace nnis
 
-// `partial`: n * nq * splits * (d + 2) floats where splits > 1.
+// slice_pages 0: a warp a row, head and slice, `partial` n * nq * splits * (d + 2) floats where splits > 1.  slice_pages > 0: the tensor
+// cores' kernel (heads of 32, 64, 96, 128, pages of 64), rows_at_once rows of a sequence together, slices of that many pages that
+// cover the whole table, `partial` n * nq * splits * (d + 4) floats and n * nkv * (heads of rows_at_once rows / 8, rounded up)
+// tickets where splits > 1.
 struct Attend8Call {
     const void *q, *k, *v;
     const float *k_scales, *v_scales;
     const int *token_pos, *token_seq, *page_table;
     void* out;
     float* partial;
+    unsigned* tickets;
+    int* status;
     int q_stride, table_rows, table_cols, pages, n, nq, nkv, d, page_size, window;
     float scale;
-    int splits, dtype;
+    int splits, slice_pages, rows_at_once, dtype;
     cudaStream_t stream;
 };
 NNIS_API int nnis_attention_int8(const void* call) {
     using namespace nnis;
     Attend8Call c;
     memcpy(&c, call, sizeof c);
-    const auto [q, k, v, k_scales, v_scales, token_pos, token_seq, page_table, out, partial, q_stride, table_rows, table_cols, pages, n,
-                nq, nkv, d, page_size, window, scale, splits, dtype, stream] = c;
+    const auto [q, k, v, k_scales, v_scales, token_pos, token_seq, page_table, out, partial, tickets, status, q_stride, table_rows, table_cols, pages, n,
+                nq, nkv, d, page_size, window, scale, splits, slice_pages, rows_at_once, dtype, stream] = c;
     if (n <= 0 || nq <= 0 || nkv <= 0 || nq % nkv || table_rows <= 0 || table_cols <= 0 || pages <= 0 || page_size <= 0 || window < 0 ||
         splits < 1 || (splits > 1 && !partial) || !q || !k || !v || !k_scales || !v_scales || !out)
         return NNIS_ERR_ARGUMENT;
     if (d < 2 || d % 2 || d > 256 || nq > 65535 || splits > 64) return NNIS_ERR_UNSUPPORTED;
     if (((uintptr_t)k | (uintptr_t)v) % 4) return NNIS_ERR_ALIGNMENT;
+    const bool aligned = (uintptr_t)q % 16 == 0 && q_stride % 4 == 0;
     const Attend8 p{q, q_stride, (const int8_t*)k, (const int8_t*)v, k_scales, v_scales, token_pos, token_seq, page_table, table_rows,
-                    table_cols, pages, out, partial, n, nq, nkv, d, page_size, window, scale, splits};
+                    table_cols, pages, out, partial, n, nq, nkv, d, page_size, window, scale, splits, slice_pages, rows_at_once, 0, aligned,
+                    tickets, status};
+    if (slice_pages > 0) {
+        if (page_size != 64 || (d != 32 && d != 64 && d != 96 && d != 128) || (dtype != NNIS_DTYPE_F32 && dtype != NNIS_DTYPE_BF16))
+            return NNIS_ERR_UNSUPPORTED;
+        if (rows_at_once < 1 || !status || (splits > 1 && !tickets) || (long long)splits * slice_pages < table_cols) return NNIS_ERR_ARGUMENT;
+        if (((uintptr_t)k | (uintptr_t)v | (uintptr_t)k_scales | (uintptr_t)v_scales | (uintptr_t)out | (uintptr_t)partial) % 16)
+            return NNIS_ERR_ALIGNMENT;
+        return (int)attend_int8_mma(p, dtype == NNIS_DTYPE_F32, stream);
+    }
     if (dtype == NNIS_DTYPE_F32) return (int)launch_warps8<float>(p, stream);
     if (dtype == NNIS_DTYPE_BF16) return (int)launch_warps8<bf16>(p, stream);
     return NNIS_ERR_UNSUPPORTED;

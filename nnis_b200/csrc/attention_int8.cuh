@@ -1,0 +1,37 @@
+// What the kernels of attention over the 8-bit cache are given.
+#pragma once
+
+#include <limits.h>
+
+#include <type_traits>
+
+#include "common.cuh"
+
+namespace nnis {
+
+struct Attend8 {
+    const void* q;
+    long long q_stride;
+    const int8_t *k, *v;
+    const float *k_scales, *v_scales;
+    const int *token_pos, *token_seq, *page_table;
+    int table_rows, table_cols, pages;
+    void* out;
+    float* partial;  // records of slices
+    int n, nq, nkv, d, page_size, window;
+    float scale;
+    int splits;      // most slices of a row
+    // the tensor cores' kernel
+    int slice_pages, rows_at_once, tiles, aligned;
+    unsigned* tickets;  // n * nkv * tiles, zero between launches
+    int* status;
+};
+
+// Pages that a warp has on their way or in use (two of heads of 128: a CTA's 135 KB).
+__host__ __device__ constexpr int stages8(int d) { return d <= 64 ? 3 : 2; }
+
+__device__ __forceinline__ void fence_async_shared8() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+cudaError_t attend_int8_mma(Attend8 p, bool f32, cudaStream_t stream);
+
+}  // namespace nnis

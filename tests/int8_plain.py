@@ -44,8 +44,9 @@ def attention(q, k, v, k_scales, v_scales, positions, seqs, table, heads, kv_hea
     Of a score: sums and products of float32 are (d + 4) roundings of at most 2^-24 of the magnitudes' sum; a query held in
     16-bit codes (``exact_q`` False) is off by at most half a step, top / 65,024, per value.  A weight's relative error is that
     of its exponent, twice (its own and the maximum's), two roundings of 2^-11 where it is held in 16 bits (else of 2^-22, an
-    exponential's), and as much again through the sum that it is divided by; a weight below 2^-14 of the row's largest is held to
-    2^-25 of it.  The output is rounded to half a step of its type."""
+    exponential's), and as much again through the sum that it is divided by; what a weight times its value's scale is below 2^-29 of
+    the largest times the largest is held to 2^-39 of it (float16 behind a factor of 2^15, next to a power of two above the scales).
+    The output is rounded to half a step of its type."""
     n, d = q.shape[0], q.shape[1] // heads
     per, dtype = heads // kv_heads, q.dtype
     out, bound = torch.zeros((n, heads, d), dtype=torch.float64), torch.zeros((n, heads, d), dtype=torch.float64)
@@ -71,8 +72,8 @@ def attention(q, k, v, k_scales, v_scales, positions, seqs, table, heads, kv_hea
                 off = off + x.abs().max() / 65024 * keys.abs().sum(1).max() * scale
             rounding = 2.0 ** -22 if exact_q else 2.0 ** -11
             relative = 2 * (math.expm1(2 * float(off)) + 2 * rounding + len(at) * 2.0 ** -24)
-            small = 0.0 if exact_q else 2.0 ** -24 * float(p.max())
-            bound[r, h] = (relative * p + small) @ values.abs() + torch.finfo(dtype).eps / 2 * out[r, h].abs() + 1e-30
+            small = 2.0 ** -38 * float(p.max()) * float(v_scales[page, h // per, slot].max())
+            bound[r, h] = relative * p @ values.abs() + small * v[page, h // per, slot].double().abs().sum(0) + torch.finfo(dtype).eps / 2 * out[r, h].abs() + 1e-30
     return out.reshape(n, -1), bound.reshape(n, -1)
 
 
