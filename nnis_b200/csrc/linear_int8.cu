@@ -6,10 +6,9 @@
 
 #include "async_copy.cuh"
 #include "int8_rows.cuh"
+#include "linear_int8.cuh"
 
 namespace nnis {
-
-enum { INT8_STORE = 0, INT8_STORE_F32 = 1, INT8_ADD_F32 = 2, INT8_GATED = 3 };
 
 struct Quantize8 {
     const void* x;
@@ -61,78 +60,6 @@ __global__ void __launch_bounds__(128) quantize_rows_kernel(const __grid_constan
     if (threadIdx.x == 0) p.scales[blockIdx.x] = r.scale;
 }
 
-struct Linear8 {
-    const int8_t *x, *w;
-    const float *xs, *ws, *bias;
-    void* out;
-    int m, n, kp;  // n: columns of the output; a gated product's w has 2 n rows, gate before up
-};
-
-__device__ __forceinline__ float silu_gate(float gate, float up) { return __fdividef(gate, 1.0f + __expf(-gate)) * up; }
-
-template <typename T, int MODE>
-__device__ __forceinline__ void put_value(void* out, size_t at, float y) {
-    if (MODE == INT8_STORE || MODE == INT8_GATED) reinterpret_cast<T*>(out)[at] = from_float<T>(y);
-    else if (MODE == INT8_STORE_F32) reinterpret_cast<float*>(out)[at] = y;
-    else reinterpret_cast<float*>(out)[at] += y;
-}
-
-// Tiles of 64 x 64 outputs on the CUDA cores, four codes a product.
-template <typename T, int MODE>
-__global__ void __launch_bounds__(256) linear_int8_dots_kernel(const __grid_constant__ Linear8 p) {
-    constexpr int NB = MODE == INT8_GATED ? 2 : 1;
-    __shared__ uint32_t xs[64][17], ws[NB][64][17];
-    pdl_wait();
-    pdl_launch_dependents();
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, m0 = blockIdx.y * 64, n0 = blockIdx.x * 64;
-    int acc[NB][4][4] = {};
-    for (int k0 = 0; k0 < p.kp; k0 += 64) {
-        for (int i = threadIdx.x; i < 64 * 16; i += 256) {
-            const int r = i >> 4, c = i & 15;
-            const bool in = k0 + c * 4 < p.kp;
-            xs[r][c] = in && m0 + r < p.m ? *reinterpret_cast<const uint32_t*>(p.x + (size_t)(m0 + r) * p.kp + k0 + c * 4) : 0u;
-#pragma unroll
-            for (int b = 0; b < NB; ++b)
-                ws[b][r][c] = in && n0 + r < p.n
-                    ? *reinterpret_cast<const uint32_t*>(p.w + ((size_t)b * p.n + n0 + r) * p.kp + k0 + c * 4) : 0u;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int c = 0; c < 16; ++c)
-#pragma unroll
-            for (int b = 0; b < NB; ++b)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        acc[b][i][j] = __dp4a((int)xs[ty * 4 + i][c], (int)ws[b][tx + 16 * j][c], acc[b][i][j]);
-        __syncthreads();
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int m = m0 + ty * 4 + i, n = n0 + tx + 16 * j;
-            if (m >= p.m || n >= p.n) continue;
-            float y[NB];
-#pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                const size_t row = (size_t)b * p.n + n;
-                y[b] = (float)acc[b][i][j] * p.xs[m] * p.ws[row] + (p.bias ? p.bias[row] : 0.f);
-            }
-            put_value<T, MODE>(p.out, (size_t)m * p.n + n, NB == 2 ? silu_gate(y[0], y[NB - 1]) : y[0]);
-        }
-}
-
-template <typename T>
-static cudaError_t launch_dots(const Linear8& p, int mode, cudaStream_t stream) {
-    const dim3 grid((unsigned)((p.n + 63) / 64), (unsigned)((p.m + 63) / 64));
-    auto kernel = mode == INT8_STORE ? linear_int8_dots_kernel<T, INT8_STORE>
-                  : mode == INT8_STORE_F32 ? linear_int8_dots_kernel<T, INT8_STORE_F32>
-                  : mode == INT8_ADD_F32 ? linear_int8_dots_kernel<T, INT8_ADD_F32> : linear_int8_dots_kernel<T, INT8_GATED>;
-    return launch_dependent(kernel, grid, 256, 0, stream, p);
-}
-
 template <typename T>
 static cudaError_t launch_quantize(const Quantize8& p, cudaStream_t stream) {
     const bool quads = p.k % 4 == 0 && p.x_stride % 4 == 0 && (uintptr_t)p.x % (4 * sizeof(T)) == 0;
@@ -170,22 +97,25 @@ struct Linear8Call {
     const float *ws, *bias;
     void *out, *codes;
     float* scales;
-    int x_stride, m, n, k, mode, dtype;
+    int* status;
+    int x_stride, m, n, k, mode, dtype, sms, unused;
     cudaStream_t stream;
 };
 NNIS_API int nnis_linear_int8(const void* call) {
     using namespace nnis;
     Linear8Call c;
     memcpy(&c, call, sizeof c);
-    const auto [x, w, ws, bias, out, codes, scales, x_stride, m, n, k, mode, dtype, stream] = c;
+    const auto [x, w, ws, bias, out, codes, scales, status, x_stride, m, n, k, mode, dtype, sms, unused, stream] = c;
+    (void)unused;
     const int kp = (k + 15) / 16 * 16;
     if (!x || !w || !ws || !out || !codes || !scales || m <= 0 || n <= 0 || k <= 0 || x_stride < k || mode < 0 || mode > 3)
         return NNIS_ERR_ARGUMENT;
-    if (k > 133136 || (m + 63) / 64 > 65535 || (dtype != NNIS_DTYPE_F32 && dtype != NNIS_DTYPE_BF16)) return NNIS_ERR_UNSUPPORTED;
+    if (k > 133136 || (dtype != NNIS_DTYPE_F32 && dtype != NNIS_DTYPE_BF16)) return NNIS_ERR_UNSUPPORTED;
     if (((uintptr_t)codes | (uintptr_t)w) % 16) return NNIS_ERR_ALIGNMENT;
     const Quantize8 q{x, x_stride, (int8_t*)codes, scales, m, k, kp};
     const cudaError_t e = dtype == NNIS_DTYPE_F32 ? launch_quantize<float>(q, stream) : launch_quantize<bf16>(q, stream);
     if (e != cudaSuccess) return (int)e;
-    const Linear8 p{(const int8_t*)codes, (const int8_t*)w, scales, ws, bias, out, m, n, kp};
-    return (int)(dtype == NNIS_DTYPE_F32 ? launch_dots<float>(p, mode, stream) : launch_dots<bf16>(p, mode, stream));
+    const Linear8 p{(const int8_t*)codes, (const int8_t*)w, scales, ws, bias, out, m, n, kp, status, 0};
+    if (m <= 32) return (int)linear_int8_few(p, mode, dtype == NNIS_DTYPE_F32, stream);
+    return linear_int8_tc(p, mode, dtype == NNIS_DTYPE_F32, sms > 0 ? sms : 148, stream);
 }

@@ -1,0 +1,31 @@
+// What the products of 8-bit codes are given, and what becomes of their sums.
+#pragma once
+
+#include "common.cuh"
+
+namespace nnis {
+
+enum { INT8_STORE = 0, INT8_STORE_F32 = 1, INT8_ADD_F32 = 2, INT8_GATED = 3 };
+
+struct Linear8 {
+    const int8_t *x, *w;
+    const float *xs, *ws, *bias;
+    void* out;
+    int m, n, kp;  // n: columns of the output; a gated product's w has 2 n rows, gate before up
+    int* status;
+    int out_by_tma;
+};
+
+// silu(gate) * up with the two approximate instructions (2^x and 1 / x, relative error about 1e-7 each)
+__device__ __forceinline__ float silu_gate(float gate, float up) {
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(gate * -1.4426950408889634f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+    return gate * r * up;
+}
+
+// `x` put into codes; the product of few rows; of many (tcgen05).  `f32`: the operands' type is float32.
+cudaError_t linear_int8_few(const Linear8& p, int mode, bool f32, cudaStream_t stream);
+int linear_int8_tc(Linear8 p, int mode, bool f32, int sms, cudaStream_t stream);
+
+}  // namespace nnis

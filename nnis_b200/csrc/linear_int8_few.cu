@@ -1,0 +1,110 @@
+// Products of 8-bit codes with few rows (decode steps), bound by the bytes of W: a CTA's eight warps share 16 rows of W (gated: 16 gate
+// and the 16 up rows), each takes every eighth run of 64 places of K straight into registers, and multiplies them (mma.sync, signed
+// bytes, W as the 16-row operand) with up to 64 rows of x; the eight sums, whole numbers, are added in shared memory.
+//
+// Any order of K serves a sum: a lane holds 16 bytes of a row that lie side by side, so that a warp's load of 8 rows takes whole
+// 64-byte runs and no byte is moved afterwards.  The first loads of W go out ahead of the wait for the kernel that makes x's codes.
+#include <type_traits>
+
+#include "async_copy.cuh"
+#include "linear_int8.cuh"
+
+namespace nnis {
+
+constexpr int kFewWarps = 8;
+
+__device__ __forceinline__ uint4 load_w(const int8_t* p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ void few_mma(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// NT: tiles of 8 rows of x.
+template <typename T, bool ADD, bool GATED, int NT>
+__global__ void __launch_bounds__(kFewWarps * 32) linear_int8_few_kernel(const __grid_constant__ Linear8 p) {
+    constexpr int NB = GATED ? 2 : 1, kAhead = GATED ? 2 : 4;  // runs of K that a lane asks for at once
+    constexpr int kSums = NB * 16 * NT * 8;
+    __shared__ int sums[kFewWarps][kSums];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int n0 = blockIdx.x * 16, runs = (p.kp + 63) / 64;
+    const uint4 none = {0u, 0u, 0u, 0u};
+    uint4 w[kAhead][NB][2];
+    auto load = [&](int first) {
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const int k = (first + i * kFewWarps) * 64 + 16 * t;
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    w[i][b][h] = k < p.kp && n0 + g + 8 * h < p.n ? load_w(p.w + ((size_t)b * p.n + n0 + g + 8 * h) * p.kp + k) : none;
+        }
+    };
+    load(warp);
+    pdl_wait();
+    pdl_launch_dependents();
+    int acc[NB][NT][4] = {};
+    for (int first = warp; first < runs; first += kAhead * kFewWarps) {
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const int k = (first + i * kFewWarps) * 64 + 16 * t;
+#pragma unroll
+            for (int c = 0; c < NT; ++c) {
+                const int m = 8 * c + g;
+                const uint4 x = k < p.kp && m < p.m ? *reinterpret_cast<const uint4*>(p.x + (size_t)m * p.kp + k) : none;
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    few_mma(acc[b][c], w[i][b][0].x, w[i][b][1].x, w[i][b][0].y, w[i][b][1].y, x.x, x.y);
+                    few_mma(acc[b][c], w[i][b][0].z, w[i][b][1].z, w[i][b][0].w, w[i][b][1].w, x.z, x.w);
+                }
+            }
+        }
+        if (first + kAhead * kFewWarps < runs) load(first + kAhead * kFewWarps);
+    }
+    // sums[token][row of W]: a lane's are rows g and g + 8, tokens 2 t and 2 t + 1 of each tile
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int c = 0; c < NT; ++c)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                sums[warp][((b * NT + c) * 8 + 2 * t + (i & 1)) * 16 + g + 8 * (i >> 1)] = acc[b][c][i];
+    __syncthreads();
+    for (int at = threadIdx.x; at < NT * 128; at += kFewWarps * 32) {
+        const int m = at >> 4, n = n0 + (at & 15);
+        if (m >= p.m || n >= p.n) continue;
+        const float xs = p.xs[m];
+        float y[NB];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            int sum = 0;
+#pragma unroll
+            for (int v = 0; v < kFewWarps; ++v) sum += sums[v][b * NT * 128 + at];
+            const size_t row = (size_t)b * p.n + n;
+            y[b] = (float)sum * xs * p.ws[row] + (p.bias ? p.bias[row] : 0.f);
+        }
+        const float value = GATED ? silu_gate(y[0], y[NB - 1]) : y[0];
+        T* out = reinterpret_cast<T*>(p.out) + (size_t)m * p.n + n;
+        *out = from_float<T>(ADD ? to_float(*out) + value : value);
+    }
+}
+
+template <typename T, bool ADD, bool GATED>
+static cudaError_t launch_few(const Linear8& p, cudaStream_t stream) {
+    auto kernel = p.m <= 8 ? linear_int8_few_kernel<T, ADD, GATED, 1> : p.m <= 16 ? linear_int8_few_kernel<T, ADD, GATED, 2>
+                  : linear_int8_few_kernel<T, ADD, GATED, 4>;
+    return launch_dependent(kernel, (unsigned)((p.n + 15) / 16), kFewWarps * 32, 0, stream, p);
+}
+
+cudaError_t linear_int8_few(const Linear8& p, int mode, bool f32, cudaStream_t stream) {
+    if (mode == INT8_GATED) return f32 ? launch_few<float, false, true>(p, stream) : launch_few<bf16, false, true>(p, stream);
+    if (mode == INT8_ADD_F32) return launch_few<float, true, false>(p, stream);
+    return f32 || mode == INT8_STORE_F32 ? launch_few<float, false, false>(p, stream) : launch_few<bf16, false, false>(p, stream);
+}
+
+}  // namespace nnis

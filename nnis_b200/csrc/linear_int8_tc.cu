@@ -1,0 +1,297 @@
+// Products of 8-bit codes with many rows on the fifth-generation tensor cores: sums of products of signed bytes in 32 bits (tcgen05.mma,
+// kind::i8), exact, in tensor memory; the epilogue multiplies each by its token's and its channel's scale.
+//
+// Roles as in the bfloat16 product: lane 0 of warp 0 loads tiles of x, lane 0 of warp 2 tiles of W (128 places of K, a row of the 128-byte
+// swizzle, a stage), one lane of warp 1 issues the products, warps 2 to 9 read tensor memory, scale, and send boxes of 32 rows x
+// 128 bytes out by TMA.  A byte is a place of K, so a stage of as many bytes carries twice the products of bfloat16's at twice the rate:
+// the same bytes a cycle are asked of L2, 64 for each SM of a pair of CTAs that share a tile of 256 x 256 (gated: 128 gate and the 128
+// up columns), 128 for a CTA of its own with a tile of 128 x 128 (gated: 64 and 64), which is for products of fewer tiles.
+// Every wait is bounded; a wait that runs out sets the status word, and all warps still meet at the end and free tensor memory.
+#include "linear_int8.cuh"
+#include "tcgen05_helpers.cuh"
+
+namespace nnis {
+
+constexpr int kRows8 = 128, kSlice8 = 128, kThreads8 = 320, kEpilogueWarps8 = 8;
+constexpr uint32_t kTileBytes8 = kRows8 * kSlice8;  // x's tile, and W's: 128 rows in either form
+
+// T: the output's type; ADD: into float32.  BN: columns of a tile's products, gate and up together.
+template <typename T, bool ADD, bool GATED, bool PAIR, int STAGES>
+__global__ void __launch_bounds__(kThreads8, STAGES <= 3 ? 2 : 1)
+linear_int8_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
+                      const __grid_constant__ CUtensorMap map_out, const __grid_constant__ Linear8 p) {
+    constexpr int BN = PAIR ? 256 : 128, kOutCols = GATED ? BN / 2 : BN;  // columns of the output that the tile makes
+    constexpr int kLoads = GATED ? 2 : 1, kLoadRows = 128 / kLoads;       // of W, by each CTA: 128 rows in one or two boxes
+    constexpr uint32_t kTmemCols = BN;
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* base = shared_1024(smem_raw);
+    __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES], done;
+    __shared__ uint32_t tmem_s;
+    __shared__ volatile int abort_flag;
+    __shared__ float scales[BN], biases[BN];
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = PAIR ? cluster_rank() : 0;
+    const int m0 = blockIdx.x * kRows8, n0 = blockIdx.y * kOutCols;
+    const int slices = (p.kp + kSlice8 - 1) / kSlice8;
+    if (threadIdx.x == 32) {
+        prefetch_tensormap(&map_x);
+        prefetch_tensormap(&map_w);
+        if (p.out_by_tma) prefetch_tensormap(&map_out);
+    }
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(&full[s], 2);
+            mbar_init(&empty[s], 1);
+        }
+        mbar_init(&done, 1);
+        abort_flag = 0;
+        mbar_fence_init();
+    }
+    if (warp == 1) {
+        if constexpr (PAIR) pair_tmem_alloc(&tmem_s, kTmemCols);
+        else tmem_alloc(&tmem_s, kTmemCols);
+    }
+    tc_fence_before();
+    __syncthreads();
+    if constexpr (PAIR) cluster_meet();
+    tc_fence_after();
+    const uint32_t tmem = tmem_s;
+
+    // Each CTA of a pair loads its 128 rows of x and half of the tile's rows of W; the bytes of both count on the first one's barrier.
+    auto load = [&](bool of_x, int slice) {
+        const int s = slice % STAGES;
+        unsigned char* to = base + (size_t)s * 2 * kTileBytes8 + (of_x ? 0 : kTileBytes8);
+        const int w_row = n0 + (int)rank * kLoadRows;
+        if constexpr (PAIR) {
+            const uint32_t bar = leader_addr(&full[s]);
+            if (rank == 0) mbar_expect_tx(&full[s], 2 * kTileBytes8);
+            if (of_x) pair_load_2d(to, &map_x, slice * kSlice8, m0, bar);
+            else
+#pragma unroll
+                for (int h = 0; h < kLoads; ++h) pair_load_2d(to + h * kLoadRows * kSlice8, &map_w, slice * kSlice8, h * p.n + w_row, bar);
+        } else {
+            mbar_expect_tx(&full[s], kTileBytes8);
+            if (of_x) tma_load_2d(to, &map_x, slice * kSlice8, m0, &full[s]);
+            else
+#pragma unroll
+                for (int h = 0; h < kLoads; ++h) tma_load_2d(to + h * kLoadRows * kSlice8, &map_w, slice * kSlice8, h * p.n + w_row, &full[s]);
+        }
+    };
+    // W does not depend on the kernel before: its first stages are asked for ahead of the wait
+    int ahead = 0;
+    if (warp == 2 && lane == 0)
+        for (; ahead < slices && ahead < STAGES; ++ahead) load(false, ahead);
+    pdl_wait();
+    pdl_launch_dependents();
+
+    if (lane == 0 && (warp == 0 || warp == 2)) {
+        for (int i = warp == 0 ? 0 : ahead; i < slices; ++i) {
+            if (i >= STAGES && !mbar_wait(&empty[i % STAGES], (uint32_t)(i / STAGES - 1) & 1u)) {
+                abort_flag = 1;
+                break;
+            }
+            if (abort_flag) break;
+            load(warp == 0, i);
+        }
+    }
+    __syncwarp();
+    if (warp == 1) {
+        if (lane == 0 && rank == 0) {
+            constexpr uint32_t idesc = instr_desc_i8(PAIR ? 256 : 128, BN);
+            const uint64_t desc_x = smem_desc_k128(smem_addr(base)), desc_w = smem_desc_k128(smem_addr(base + kTileBytes8));
+            bool ok = true;
+            for (int i = 0; i < slices; ++i) {
+                const int s = i % STAGES;
+                if (!mbar_wait(&full[s], (uint32_t)(i / STAGES) & 1u) || abort_flag) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {  // 32 places of K each
+                    const uint64_t a = desc_advance(desc_x, s * 2 * kTileBytes8 + k * 32), b = desc_advance(desc_w, s * 2 * kTileBytes8 + k * 32);
+                    if constexpr (PAIR) pair_mma_i8(tmem, a, b, idesc, (i | k) != 0);
+                    else tc_mma_i8(tmem, a, b, idesc, (i | k) != 0);
+                }
+                if constexpr (PAIR) pair_commit(&empty[s]);
+                else tc_commit(&empty[s]);
+            }
+            if (!ok) {
+                abort_flag = 1;
+                if constexpr (PAIR) follower_set(&abort_flag, 1);
+            }
+            if constexpr (PAIR) pair_commit(&done);
+            else tc_commit(&done);
+        }
+    } else if (warp >= 2) {
+        const int quarter = warp & 3, group = (warp - 2) >> 2, row = quarter * 32 + lane, m = m0 + row;
+        // the tile's scales and biases, in the order of its products' columns: of a pair's gate and up, the first CTA's gate and up
+        // rows, then the second's
+        for (int c = threadIdx.x - 64; c < BN; c += kEpilogueWarps8 * 32) {
+            int col = c, up = 0;
+            if (GATED) {
+                up = c / kLoadRows % 2;
+                col = c / (2 * kLoadRows) * kLoadRows + c % kLoadRows;
+            }
+            const bool in = n0 + col < p.n;
+            scales[c] = in ? p.ws[(size_t)up * p.n + n0 + col] : 0.f;
+            biases[c] = in && p.bias ? p.bias[(size_t)up * p.n + n0 + col] : 0.f;
+        }
+        asm volatile("bar.sync 1, %0;" ::"n"(kEpilogueWarps8 * 32) : "memory");
+        const float xs = m < p.m ? p.xs[m] : 0.f;
+        bool ok = mbar_wait(&done, 0);
+        ok = __all_sync(0xffffffffu, ok) && !abort_flag;
+        if (!ok) {
+            abort_flag = 1;
+        } else {
+            tc_fence_after();
+            constexpr int kBoxCols = 128 / (int)sizeof(T), kSlots = 2;
+            const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
+            unsigned char* boxes = base + (size_t)(warp - 2) * (kSlots * 4096);
+            // (a tile's rows beyond the last: nothing to send)
+            const bool sends = m0 + quarter * 32 < p.m;
+#pragma unroll 1
+            for (int b = group, i = 0; b < kOutCols / kBoxCols && n0 + b * kBoxCols < p.n && sends; b += 2, ++i) {
+                unsigned char* box = boxes + (i % kSlots) * 4096;
+                if (p.out_by_tma && i >= kSlots) {
+                    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kSlots - 1) : "memory");
+                    __syncwarp();
+                }
+#pragma unroll 1
+                for (int c0 = b * kBoxCols; c0 < (b + 1) * kBoxCols; c0 += 32) {
+                    uint32_t v[32], u[32];
+                    const int at = GATED ? c0 / kLoadRows * 2 * kLoadRows + c0 % kLoadRows : c0;
+                    tmem_load32_issue(lanes + (uint32_t)at, v);
+                    if constexpr (GATED) tmem_load32_issue(lanes + (uint32_t)(at + kLoadRows), u);
+                    tmem_load_wait();
+                    float y[32];
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4) {
+                        const float4 s4 = *reinterpret_cast<const float4*>(scales + at + j), b4 = *reinterpret_cast<const float4*>(biases + at + j);
+                        y[j] = (float)(int)v[j] * xs * s4.x + b4.x;
+                        y[j + 1] = (float)(int)v[j + 1] * xs * s4.y + b4.y;
+                        y[j + 2] = (float)(int)v[j + 2] * xs * s4.z + b4.z;
+                        y[j + 3] = (float)(int)v[j + 3] * xs * s4.w + b4.w;
+                        if constexpr (GATED) {
+                            const float4 t4 = *reinterpret_cast<const float4*>(scales + at + kLoadRows + j);
+                            const float4 c4 = *reinterpret_cast<const float4*>(biases + at + kLoadRows + j);
+                            y[j] = silu_gate(y[j], (float)(int)u[j] * xs * t4.x + c4.x);
+                            y[j + 1] = silu_gate(y[j + 1], (float)(int)u[j + 1] * xs * t4.y + c4.y);
+                            y[j + 2] = silu_gate(y[j + 2], (float)(int)u[j + 2] * xs * t4.z + c4.z);
+                            y[j + 3] = silu_gate(y[j + 3], (float)(int)u[j + 3] * xs * t4.w + c4.w);
+                        }
+                    }
+                    if (p.out_by_tma) {
+                        if constexpr (sizeof(T) == 2) {
+                            const int unit = c0 % 64 / 8;
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                uint32_t w[4];
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    __nv_bfloat162 two = __floats2bfloat162_rn(y[8 * j + 2 * e], y[8 * j + 2 * e + 1]);
+                                    w[e] = *reinterpret_cast<uint32_t*>(&two);
+                                }
+                                *reinterpret_cast<uint4*>(box + lane * 128 + (((unit + j) ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                            }
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 8; ++j)
+                                *reinterpret_cast<float4*>(box + lane * 128 + ((j ^ (lane & 7)) << 4)) =
+                                    make_float4(y[4 * j], y[4 * j + 1], y[4 * j + 2], y[4 * j + 3]);
+                        }
+                    } else if (m < p.m) {
+                        T* out = reinterpret_cast<T*>(p.out) + (size_t)m * p.n + n0 + c0;
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            if (n0 + c0 + j < p.n) out[j] = from_float<T>(ADD ? to_float(out[j]) + y[j] : y[j]);
+                    }
+                }
+                if (p.out_by_tma) {
+                    fence_async_shared();
+                    __syncwarp();
+                    if (lane == 0) {
+                        if (ADD) tma_add_2d(&map_out, n0 + b * kBoxCols, m0 + quarter * 32, box);
+                        else tma_store_2d(&map_out, n0 + b * kBoxCols, m0 + quarter * 32, box);
+                        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                    }
+                }
+            }
+            if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if constexpr (PAIR) cluster_meet();
+    if (warp == 1) {
+        tc_fence_after();
+        if constexpr (PAIR) pair_tmem_dealloc(tmem, kTmemCols);
+        else tmem_dealloc(tmem, kTmemCols);
+    }
+    if constexpr (PAIR) cluster_meet();
+    if (threadIdx.x == 0 && abort_flag && p.status) atomicExch(p.status, 3);
+}
+
+template <typename T, bool ADD, bool GATED, bool PAIR, int STAGES>
+static cudaError_t launch_tc8(const CUtensorMap& mx, const CUtensorMap& mw, const CUtensorMap& mo, const Linear8& p, cudaStream_t stream) {
+    constexpr size_t smem = (size_t)STAGES * 2 * kTileBytes8 + 1024;
+    static_assert(STAGES * 2 * kTileBytes8 >= kEpilogueWarps8 * 2 * 4096, "the epilogue's boxes fit the ring");
+    auto kernel = linear_int8_tc_kernel<T, ADD, GATED, PAIR, STAGES>;
+    static std::atomic<int> held[16];
+    cudaError_t e = allow_shared(kernel, smem, held);
+    if (e != cudaSuccess) return e;
+    constexpr int kOutCols = (PAIR ? 256 : 128) / (GATED ? 2 : 1);
+    const unsigned tiles = (unsigned)((p.m + kRows8 - 1) / kRows8);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(PAIR ? (tiles + 1) / 2 * 2 : tiles, (unsigned)((p.n + kOutCols - 1) / kOutCols));
+    cfg.blockDim = dim3(kThreads8);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    int attrs = 0;
+    if (PAIR) {
+        attr[attrs].id = cudaLaunchAttributeClusterDimension;
+        attr[attrs].val.clusterDim.x = 2;
+        attr[attrs].val.clusterDim.y = 1;
+        attr[attrs++].val.clusterDim.z = 1;
+    }
+    if (dependent_launches()) {
+        attr[attrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[attrs++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    cfg.attrs = attr;
+    cfg.numAttrs = attrs;
+    return cudaLaunchKernelEx(&cfg, kernel, mx, mw, mo, p);
+}
+
+// Three stages let two CTAs share an SM, so that one's epilogue runs under the other's products; six where there are no more CTAs than SMs.
+template <typename T, bool ADD, bool GATED>
+static cudaError_t launch_tc8_of(const CUtensorMap& mx, const CUtensorMap& mw, const CUtensorMap& mo, const Linear8& p, bool pair, bool alone,
+                                 cudaStream_t stream) {
+    if (pair) return alone ? launch_tc8<T, ADD, GATED, true, 6>(mx, mw, mo, p, stream) : launch_tc8<T, ADD, GATED, true, 3>(mx, mw, mo, p, stream);
+    return alone ? launch_tc8<T, ADD, GATED, false, 6>(mx, mw, mo, p, stream) : launch_tc8<T, ADD, GATED, false, 3>(mx, mw, mo, p, stream);
+}
+
+int linear_int8_tc(Linear8 p, int mode, bool f32, int sms, cudaStream_t stream) {
+    const bool gated = mode == INT8_GATED, wide = f32 || mode == INT8_STORE_F32 || mode == INT8_ADD_F32;
+    const long tiles = (p.m + 127) / 128, pair_cols = gated ? 128 : 256, single_cols = gated ? 64 : 128;
+    const long pairs = (tiles + 1) / 2 * 2 * ((p.n + pair_cols - 1) / pair_cols), singles = tiles * ((p.n + single_cols - 1) / single_cols);
+    const bool pair = 5 * pairs >= 3 * sms;
+    if ((p.n + single_cols - 1) / single_cols > 65535) return NNIS_ERR_UNSUPPORTED;
+    CUtensorMap mx, mw, mo;
+    const int bytes = wide ? 4 : 2;
+    if (!make_map(&mx, p.x, p.m, p.kp, kRows8, 0, 1) || !make_map(&mw, p.w, (gated ? 2LL : 1LL) * p.n, p.kp, gated ? 64 : 128, 0, 1))
+        return NNIS_ERR_UNSUPPORTED;
+    p.out_by_tma = (uintptr_t)p.out % 16 == 0 && (long long)p.n * bytes % 16 == 0 && make_map(&mo, p.out, p.m, p.n, 32, 0, bytes);
+    if (!p.out_by_tma) mo = mx;
+    const bool alone = (pair ? pairs : singles) <= sms;
+    if (gated)
+        return (int)(f32 ? launch_tc8_of<float, false, true>(mx, mw, mo, p, pair, alone, stream)
+                         : launch_tc8_of<bf16, false, true>(mx, mw, mo, p, pair, alone, stream));
+    if (mode == INT8_ADD_F32) return (int)launch_tc8_of<float, true, false>(mx, mw, mo, p, pair, alone, stream);
+    return (int)(wide ? launch_tc8_of<float, false, false>(mx, mw, mo, p, pair, alone, stream)
+                      : launch_tc8_of<bf16, false, false>(mx, mw, mo, p, pair, alone, stream));
+}
+
+}  // namespace nnis

@@ -70,7 +70,7 @@ _ENTRY_FIELDS = {"nnis_copy_pages": "ppiiiiiipiip", "nnis_verify_drafts": "ppppp
                  "nnis_attention_shared": "pippppipiiippppppiiiiiifiipp",
                  "nnis_rope_store_int8": "pppppppppppiiiiiiiiiip", "nnis_read_pages_int8": "ppppppppiiiiiiiiip",
                  "nnis_attention_int8": "ppppppppppppiiiiiiiiiifiiiip", "nnis_quantize_rows": "pppiiiip",
-                 "nnis_linear_int8": "pppppppiiiiiip"}
+                 "nnis_linear_int8": "ppppppppiiiiiiiip"}
 _entries = {}
 
 
@@ -3046,18 +3046,24 @@ def rope_store_int8(qkv: torch.Tensor, q: torch.Tensor, token_pos: torch.Tensor,
     2 kv_heads) * d] float32 or bfloat16 is left as it is.  ``cos`` and ``sin`` None: nothing is rotated.  A row at position -1, or
     beyond the angles, writes nothing; one whose page the table does not name stores nothing.  No two rows of a call have the same
     sequence and position."""
-    d, n = head_dim, qkv.shape[0] if qkv.dim() else 0
-    pages, seqs, cols = k.shape[0] if k.dim() else 0, page_table.shape[0], page_table.shape[-1]
-    codes, scales, half = (pages, kv_heads, page_size, d), (pages, kv_heads, page_size), (cos.shape[0] if cos is not None else 0, d // 2)
-    if not (d % 2 == 0 and 2 <= d <= 256 and heads > 0 and kv_heads > 0 and page_size > 0 and qkv.dtype in _DTYPE_CODE
-            and _good((qkv, qkv.dtype, (n, (heads + 2 * kv_heads) * d)), (q, qkv.dtype, (n, heads * d)), (k, torch.int8, codes),
-                      (v, torch.int8, codes), (k_scales, torch.float32, scales), (v_scales, torch.float32, scales),
-                      (page_table, torch.int32, (seqs, cols)))
-            and token_pos.dtype is token_seq.dtype is torch.int32 and token_pos.numel() >= n and token_seq.numel() >= n
-            and _good((qkv, qkv.dtype, qkv.shape), (token_pos, torch.int32, token_pos.shape), (token_seq, torch.int32, token_seq.shape))
-            and (cos is None) == (sin is None)
-            and (cos is None or _good((qkv, qkv.dtype, qkv.shape), (cos, torch.float32, half), (sin, torch.float32, half)))):
-        code_of(qkv.dtype)
+    d, dtype, index, turns = head_dim, qkv.dtype, k.get_device(), cos is not None
+    shape, rows, q_shape, table_shape, per_head = k.shape, qkv.shape, q.shape, page_table.shape, k_scales.shape
+    n, half = rows[0] if rows else 0, cos.shape if turns else (0, d // 2)
+    if not (len(shape) == 4 and len(rows) == len(q_shape) == len(table_shape) == len(half) == 2 and shape[1] == kv_heads
+            and shape[2] == page_size and shape[3] == d and v.shape == shape and per_head == shape[:3] and v_scales.shape == per_head
+            and rows[1] == (heads + 2 * kv_heads) * d and q_shape[0] == n and q_shape[1] == heads * d
+            and 2 <= d <= 256 and d % 2 == 0 and heads > 0 and kv_heads > 0 and page_size > 0 and dtype in _DTYPE_CODE and q.dtype is dtype
+            and k.dtype is v.dtype is torch.int8 and k_scales.dtype is v_scales.dtype is torch.float32
+            and token_pos.dtype is token_seq.dtype is page_table.dtype is torch.int32
+            and token_pos.numel() >= n <= token_seq.numel()
+            and 0 <= index == v.get_device() == k_scales.get_device() == v_scales.get_device() == q.get_device() == qkv.get_device()
+            == token_pos.get_device() == token_seq.get_device() == page_table.get_device()
+            and k.is_contiguous() and v.is_contiguous() and k_scales.is_contiguous() and v_scales.is_contiguous() and q.is_contiguous()
+            and qkv.is_contiguous() and token_pos.is_contiguous() and token_seq.is_contiguous() and page_table.is_contiguous()
+            and turns == (sin is not None)
+            and (not turns or (half[1] == d // 2 and sin.shape == half and cos.dtype is sin.dtype is torch.float32
+                               and cos.get_device() == sin.get_device() == index and cos.is_contiguous() and sin.is_contiguous()))):
+        code_of(dtype)
         _need(heads > 0, "rope_store_int8: at least one query head")
         _need((cos is None) == (sin is None), "rope_store_int8: cos and sin, or neither")
         _need(token_pos.numel() >= n and token_seq.numel() >= n, f"rope_store_int8: a position and a sequence for each of {n} rows")
@@ -3065,19 +3071,18 @@ def rope_store_int8(qkv: torch.Tensor, q: torch.Tensor, token_pos: torch.Tensor,
                 **_store8("rope_store_int8", k, v, k_scales, v_scales, kv_heads, d, page_size),
                 token_pos=(token_pos, torch.int32, token_pos.shape), token_seq=(token_seq, torch.int32, token_seq.shape),
                 page_table=(page_table, torch.int32, (None, None)), cos=(cos, torch.float32, (None, d // 2)),
-                sin=(sin, torch.float32, half))
+                sin=(sin, torch.float32, (half[0] if half else 0, d // 2)))
         raise KernelError("rope_store_int8: bad argument")
     if n == 0:
         return
-    index = qkv.get_device()
     if _device_now() != index:
         with torch.cuda.device(index):
             return rope_store_int8(qkv, q, token_pos, token_seq, page_table, cos, sin, k, v, k_scales, v_scales, heads, kv_heads, d,
                                    page_size)
     _check(_entry("nnis_rope_store_int8")(
         qkv.data_ptr(), q.data_ptr(), token_pos.data_ptr(), token_seq.data_ptr(), page_table.data_ptr(),
-        0 if cos is None else cos.data_ptr(), 0 if sin is None else sin.data_ptr(), k.data_ptr(), v.data_ptr(), k_scales.data_ptr(),
-        v_scales.data_ptr(), _DTYPE_CODE[qkv.dtype], seqs, cols, half[0], pages, n, heads, kv_heads, d, page_size,
+        cos.data_ptr() if turns else 0, sin.data_ptr() if turns else 0, k.data_ptr(), v.data_ptr(), k_scales.data_ptr(),
+        v_scales.data_ptr(), _DTYPE_CODE[dtype], table_shape[0], table_shape[1], half[0], shape[0], n, heads, kv_heads, d, page_size,
         _stream_of(index)), "rope_store_int8")
 
 
@@ -3087,28 +3092,31 @@ def read_pages_int8(k: torch.Tensor, v: torch.Tensor, k_scales: torch.Tensor, v_
     int32 [sequences, columns], -1 where none is wanted, that page becomes the values, code times scale, of the page that
     ``page_table`` names in the same place.  k, v int8 [pages, kv_heads, page_size, d], their scales float32 [pages, kv_heads,
     page_size]; k_out, v_out float32 or bfloat16 [out_pages, kv_heads, page_size, d].  A page id outside its store is passed over."""
-    shape, seqs, cols, local_cols = k.shape, local_table.shape[0], page_table.shape[-1], local_table.shape[-1]
-    outs, dtype = (k_out.shape[0] if k_out.dim() else 0, *shape[1:]), k_out.dtype
-    if not (len(shape) == 4 and dtype in _DTYPE_CODE
-            and _good((k, torch.int8, shape), (v, torch.int8, shape), (k_scales, torch.float32, shape[:3]),
-                      (v_scales, torch.float32, shape[:3]), (page_table, torch.int32, (page_table.shape[0], cols)),
-                      (local_table, torch.int32, (seqs, local_cols)), (k_out, dtype, outs), (v_out, dtype, outs))
-            and page_table.shape[0] >= seqs and cols >= local_cols):
+    shape, places, table_shape, outs, dtype, index = k.shape, local_table.shape, page_table.shape, k_out.shape, k_out.dtype, k.get_device()
+    if not (len(shape) == len(outs) == 4 and len(places) == len(table_shape) == 2 and outs[1:] == shape[1:] and v.shape == shape
+            and v_out.shape == outs and k_scales.shape == shape[:3] and v_scales.shape == shape[:3] and shape[1] > 0 and shape[2] > 0
+            and 2 <= shape[3] <= 256 and shape[3] % 2 == 0
+            and table_shape[0] >= places[0] and table_shape[1] >= places[1] and dtype in _DTYPE_CODE and v_out.dtype is dtype
+            and k.dtype is v.dtype is torch.int8 and k_scales.dtype is v_scales.dtype is torch.float32
+            and page_table.dtype is local_table.dtype is torch.int32
+            and 0 <= index == v.get_device() == k_scales.get_device() == v_scales.get_device() == k_out.get_device() == v_out.get_device()
+            == page_table.get_device() == local_table.get_device()
+            and k.is_contiguous() and v.is_contiguous() and k_scales.is_contiguous() and v_scales.is_contiguous()
+            and k_out.is_contiguous() and v_out.is_contiguous() and page_table.is_contiguous() and local_table.is_contiguous()):
         code_of(dtype)
         _need(len(shape) == 4, f"read_pages_int8: k is int8 [pages, kv_heads, page_size, d]; got {tuple(shape)}")
         _wanted("read_pages_int8", **_store8("read_pages_int8", k, v, k_scales, v_scales, shape[1], shape[3], shape[2]),
                 page_table=(page_table, torch.int32, (None, None)), local_table=(local_table, torch.int32, (None, None)),
-                k_out=(k_out, dtype, (None, *shape[1:])), v_out=(v_out, dtype, outs))
+                k_out=(k_out, dtype, (None, *shape[1:])), v_out=(v_out, dtype, (outs[0] if outs else 0, *shape[1:])))
         raise KernelError(f"read_pages_int8: local_table {tuple(local_table.shape)} reaches beyond page_table {tuple(page_table.shape)}")
     if not local_table.numel() or not outs[0] or not k.numel():
         return
-    index = k.get_device()
     if _device_now() != index:
         with torch.cuda.device(index):
             return read_pages_int8(k, v, k_scales, v_scales, page_table, local_table, k_out, v_out)
     _check(_entry("nnis_read_pages_int8")(
         k.data_ptr(), v.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), page_table.data_ptr(), local_table.data_ptr(),
-        k_out.data_ptr(), v_out.data_ptr(), cols, seqs, local_cols, _DTYPE_CODE[dtype], shape[0], outs[0], shape[1], shape[2],
+        k_out.data_ptr(), v_out.data_ptr(), table_shape[1], places[0], places[1], _DTYPE_CODE[dtype], shape[0], outs[0], shape[1], shape[2],
         shape[3], _stream_of(index)), "read_pages_int8")
 
 
@@ -3122,6 +3130,7 @@ def attention_int8_splits(n: int, heads: int, keys: int, device) -> int:
     return max(1, min(16 * sm_count(device) // max(1, n * heads), -(-keys // 128), 64))
 
 
+@functools.lru_cache(maxsize=4096)
 def attention_int8_plan(n: int, seqs: int, heads: int, kv_heads: int, d: int, cols: int, window: int, sms: int):
     """(slices, pages of a slice, rows taken together) of the tensor cores' kernel: rows of a sequence lie together, as many as come on
     each, up to 64 queries a key/value head; slices cover the table, at most 64, as short as fills the device."""
@@ -3145,17 +3154,23 @@ def attention_int8(q: torch.Tensor, q_stride: int, k: torch.Tensor, v: torch.Ten
     heads * d] of its type.  A position whose page the table does not name, or beyond it, holds no key; a row that sees none (a
     padding row at position -1 among them) is zero.  Every row of a call reads its keys by itself: for single tokens and a few
     drafted ones (prompts read their pages back and take the kernels of the 16-bit cache)."""
-    d, dtype, (n, width) = head_dim, q.dtype, out.shape
-    pages, seqs, cols, page_size = k.shape[0], page_table.shape[0], page_table.shape[-1], k.shape[2] if k.dim() == 4 else 0
-    codes, scales = (pages, kv_heads, page_size, d), (pages, kv_heads, page_size)
-    if not (d % 2 == 0 and 2 <= d <= 256 and heads > 0 and kv_heads > 0 and heads % kv_heads == 0 and page_size > 0 and window >= 0
-            and scale > 0 and dtype in _DTYPE_CODE and q.dim() == 2 and q.shape[0] >= n and q.stride() == (q_stride, 1)
-            and q.shape[1] >= heads * d <= q_stride < 1 << 31 and q.get_device() == k.get_device() and heads <= 65535
-            and _good((k, torch.int8, codes), (v, torch.int8, codes), (k_scales, torch.float32, scales),
-                      (v_scales, torch.float32, scales), (out, dtype, (n, heads * d)), (page_table, torch.int32, (seqs, cols)),
-                      (token_pos, torch.int32, token_pos.shape), (token_seq, torch.int32, token_seq.shape))
-            and token_pos.numel() >= n and token_seq.numel() >= n):
+    # (checked in one expression: a call of its own for each tensor costs the host 3 us more)
+    d, dtype, index = head_dim, q.dtype, k.get_device()
+    shape, q_shape, out_shape, table_shape, per_head = k.shape, q.shape, out.shape, page_table.shape, k_scales.shape
+    if not (len(shape) == 4 and len(q_shape) == len(out_shape) == len(table_shape) == 2 and shape[1] == kv_heads and shape[3] == d
+            and v.shape == shape and per_head == shape[:3] and v_scales.shape == per_head and out_shape[1] == heads * d
+            and q_shape[0] >= out_shape[0] and q_shape[1] >= heads * d <= q_stride < 1 << 31 and q.stride() == (q_stride, 1)
+            and 2 <= d <= 256 and d % 2 == 0 and 0 < heads <= 65535 and kv_heads > 0 and heads % kv_heads == 0 and shape[2] > 0
+            and window >= 0 and scale > 0 and dtype in _DTYPE_CODE and out.dtype is dtype
+            and k.dtype is v.dtype is torch.int8 and k_scales.dtype is v_scales.dtype is torch.float32
+            and token_pos.dtype is token_seq.dtype is page_table.dtype is torch.int32
+            and token_pos.numel() >= out_shape[0] <= token_seq.numel()
+            and 0 <= index == v.get_device() == k_scales.get_device() == v_scales.get_device() == q.get_device() == out.get_device()
+            == token_pos.get_device() == token_seq.get_device() == page_table.get_device()
+            and k.is_contiguous() and v.is_contiguous() and k_scales.is_contiguous() and v_scales.is_contiguous() and out.is_contiguous()
+            and token_pos.is_contiguous() and token_seq.is_contiguous() and page_table.is_contiguous()):
         code_of(dtype)
+        n, page_size = out_shape[0] if out_shape else 0, shape[2] if len(shape) == 4 else 1
         _wanted("attention_int8", **_store8("attention_int8", k, v, k_scales, v_scales, kv_heads, d, page_size),
                 out=(out, dtype, (n, heads * d)), page_table=(page_table, torch.int32, (None, None)),
                 token_pos=(token_pos, torch.int32, token_pos.shape), token_seq=(token_seq, torch.int32, token_seq.shape))
@@ -3164,16 +3179,16 @@ def attention_int8(q: torch.Tensor, q_stride: int, k: torch.Tensor, v: torch.Ten
             f"sequence for every row, and q [rows, heads * d] in rows of q_stride on the cache's device; got {heads} heads over "
             f"{kv_heads}, window {window}, scale {scale}, q {tuple(q.shape)} in strides {q.stride()} (q_stride {q_stride}) on "
             f"{q.device}, out {tuple(out.shape)}, {token_pos.numel()} positions, {token_seq.numel()} sequences")
+    n, pages, page_size, (seqs, cols) = out_shape[0], shape[0], shape[2], table_shape
     if n == 0:
         return
-    index = k.get_device()
     if _device_now() != index:
         with torch.cuda.device(index):
             return attention_int8(q, q_stride, k, v, k_scales, v_scales, token_pos, token_seq, page_table, out, heads, kv_heads, d,
                                   window, scale, workspace)
     tickets = status = slice_pages = rows = 0
-    if page_size == 64 and d in (32, 64, 96, 128) \
-            and not (k.data_ptr() | v.data_ptr() | k_scales.data_ptr() | v_scales.data_ptr() | out.data_ptr()) % 16:
+    at = k.data_ptr(), v.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), out.data_ptr()
+    if page_size == 64 and d in (32, 64, 96, 128) and not (at[0] | at[1] | at[2] | at[3] | at[4]) % 16:
         splits, slice_pages, rows = attention_int8_plan(n, seqs, heads, kv_heads, d, cols, window, _sm_count.get(index) or sm_count(k.device))
         partial = workspace.room("attn_int8_records", n * heads * splits * (d + 4), torch.float32).data_ptr() if splits > 1 else 0
         tickets = workspace.zeros_room("attn_int8_tickets", n * kv_heads * -(-rows * (heads // kv_heads) // 8), torch.int32).data_ptr() \
@@ -3184,9 +3199,8 @@ def attention_int8(q: torch.Tensor, q_stride: int, k: torch.Tensor, v: torch.Ten
         splits = attention_int8_splits(n, heads, min(keys, window) if window else keys, k.device)
         partial = workspace.room("attn_int8_partial", n * heads * splits * (d + 2), torch.float32).data_ptr() if splits > 1 else 0
     _check(_entry("nnis_attention_int8")(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), token_pos.data_ptr(),
-        token_seq.data_ptr(), page_table.data_ptr(), out.data_ptr(), partial, tickets, status, q_stride, seqs, cols, pages, n, heads,
-        kv_heads, d, page_size, window, scale, splits, slice_pages, rows, _DTYPE_CODE[dtype], _stream_of(index)),
+        q.data_ptr(), at[0], at[1], at[2], at[3], token_pos.data_ptr(), token_seq.data_ptr(), page_table.data_ptr(), at[4], partial,
+        tickets, status, q_stride, seqs, cols, pages, n, heads, kv_heads, d, page_size, window, scale, splits, slice_pages, rows, _DTYPE_CODE[dtype], _stream_of(index)),
         "attention_int8", 2 if splits > 1 and not slice_pages else 1)
 
 
@@ -3248,4 +3262,5 @@ def linear_int8(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, bias: 
     scales = workspace.room("int8_scales", m, torch.float32)
     _check(_entry("nnis_linear_int8")(
         x.data_ptr(), w.data_ptr(), w_scales.data_ptr(), 0 if bias is None else bias.data_ptr(), out.data_ptr(), codes.data_ptr(),
-        scales.data_ptr(), x.stride(0) if m > 1 else k, m, n, k, mode, _DTYPE_CODE[dtype], _stream_of(index)), "linear_int8", 2)
+        scales.data_ptr(), status_word(w.device).data_ptr(), x.stride(0) if m > 1 else k, m, n, k, mode, _DTYPE_CODE[dtype],
+        _sm_count.get(index) or sm_count(w.device), 0, _stream_of(index)), "linear_int8", 2)

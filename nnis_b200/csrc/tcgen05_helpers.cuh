@@ -202,6 +202,23 @@ __device__ __forceinline__ void pair_mma(uint32_t d_tmem, uint64_t a_desc, uint6
         ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
+// The same products of whole numbers: signed bytes, 32-bit sums, 32 places of K each.
+__device__ __forceinline__ void tc_mma_i8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void pair_mma_i8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
 // One arrival on both CTAs' copies of the barrier when the products issued so far are complete.
 __device__ __forceinline__ void pair_commit(uint64_t* bar) {
     asm volatile(
@@ -252,6 +269,15 @@ __host__ __device__ constexpr uint32_t instr_desc(int m, int n) {
          | ((uint32_t)(m >> 4) << 24);  // M / 16
 }
 
+// kind::i8 instruction descriptor: signed bytes x signed bytes -> 32-bit whole numbers, both K-major.
+__host__ __device__ constexpr uint32_t instr_desc_i8(int m, int n) {
+    return (2u << 4)                    // accumulator int32
+         | (1u << 7)                    // A signed
+         | (1u << 10)                   // B signed
+         | ((uint32_t)(n >> 3) << 17)   // N / 8
+         | ((uint32_t)(m >> 4) << 24);  // M / 16
+}
+
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
                                   const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                                   const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
@@ -271,7 +297,7 @@ static inline EncodeTiledFn encode_tiled() {
     return fn;
 }
 
-// [rows, K] row-major bfloat16 or float32 (`elem_bytes` 2 or 4; rows `row_stride`
+// [rows, K] row-major bfloat16, float32 or bytes (`elem_bytes` 2, 4 or 1; rows `row_stride`
 // elements apart; 0: packed), boxes of box_rows x 128 bytes, 128-byte swizzle.  Encoding a map costs the host a
 // microsecond or two and a step encodes hundreds (weights, caches and workspace
 // buffers at the same addresses every time), so the last maps are kept by key.
@@ -307,7 +333,7 @@ static inline bool make_map(CUtensorMap* map, const void* ptr, long long rows, i
     cuuint64_t strides[1] = {(cuuint64_t)(row_stride > 0 ? row_stride : K) * (cuuint64_t)elem_bytes};
     cuuint32_t box[2] = {128u / (cuuint32_t)elem_bytes, (cuuint32_t)box_rows};  // one 128-byte swizzle row
     cuuint32_t elem[2] = {1, 1};
-    if (fn(map, elem_bytes == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(ptr), dims, strides, box, elem,
+    if (fn(map, elem_bytes == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : elem_bytes == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(ptr), dims, strides, box, elem,
            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
         return false;
