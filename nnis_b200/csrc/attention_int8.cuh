@@ -22,13 +22,13 @@ struct Attend8 {
     float scale;
     int splits;      // most slices of a row
     // the tensor cores' kernel
-    int slice_pages, rows_at_once, tiles, aligned;
+    int slice_pieces, rows_at_once, tiles, aligned;
     unsigned* tickets;  // n * nkv * tiles, zero between launches
     int* status;
 };
 
-// Pages that a warp has on their way or in use (two of heads of 128: a CTA's 135 KB).
-__host__ __device__ constexpr int stages8(int d) { return d <= 64 ? 3 : 2; }
+// Pieces of 32 positions that a warp has on their way or in use.
+__host__ __device__ constexpr int stages8(int d) { return 3; }
 
 __device__ __forceinline__ void fence_async_shared8() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 

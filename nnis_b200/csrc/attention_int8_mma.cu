@@ -14,9 +14,9 @@
 // side by side in shared memory as the copies bring it: a thread of the key product holds bytes [t D / 4, (t + 1) D / 4) of a
 // position's row, of the value product bytes [g D / 8, (g + 1) D / 8) of positions 4 t to 4 t + 3 (g = lane / 4, t = lane % 4).
 //
-// A CTA: four warps, (run of rows with one sequence, key/value head, tile of queries, slice of pages); a warp takes every fourth page of
-// the slice through a ring of its own, filled by bulk copies, so that nothing meets before the slice's end.  Slices are of a fixed
-// number of pages, so sequences of all lengths are cut into equal pieces; the slice that ends last joins them.
+// A CTA: four warps, (run of rows with one sequence, key/value head, tile of queries, slice of positions); a warp takes every fourth piece
+// of 32 positions of the slice through a ring of its own, filled by bulk copies, so that nothing meets before the slice's end.  Slices are of a
+// fixed number of pieces, so sequences of all lengths are cut into equal pieces; the slice that ends last joins them.
 #include <float.h>
 #include <string.h>
 
@@ -28,9 +28,9 @@
 
 namespace nnis {
 
-constexpr int kPage8 = 64, kWarps8 = 4;
+constexpr int kPage8 = 64, kPiece8 = 32, kWarps8 = 4;  // positions of a page, and of what a warp takes at a time
 
-__host__ __device__ constexpr int stage_bytes8(int d) { return 2 * kPage8 * d + 2 * kPage8 * 4; }
+__host__ __device__ constexpr int stage_bytes8(int d) { return 2 * kPiece8 * d + 2 * kPiece8 * 4; }
 
 __device__ __forceinline__ void mma_s8(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -113,15 +113,16 @@ __global__ void __launch_bounds__(kWarps8 * 32) attn_int8_mma_kernel(const __gri
     using T = std::conditional_t<F32, float, bf16>;
     constexpr int kStage = stage_bytes8(D), kTile = 8 * MT, kSteps = D / 32, kWords = D / 16, kValueWords = D / 32, kCols = D / 8;
     constexpr int kOuts = F32 ? MT : (MT + 1) / 2;  // products of the weights per step of 16 positions
-    constexpr int kStages = stages8(D);
+    constexpr int kStages = stages8(D), kScores = kPiece8 / 4;  // (a lane's positions of a piece: 16 s + 4 t + 0 to 3)
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ __align__(8) uint64_t full[kWarps8][kStages];
-    __shared__ int joins;
+    __shared__ int joins, piece_in[kWarps8][kStages];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    if (lane == 0)
+    if (lane == 0) {  // (a warp's barriers are its own)
         for (int s = 0; s < kStages; ++s) mbar_init(&full[warp][s], 1);
-    mbar_fence_init();
-    __syncthreads();
+        mbar_fence_init();
+    }
+    __syncwarp();
     pdl_wait();
     pdl_launch_dependents();
 
@@ -131,9 +132,27 @@ __global__ void __launch_bounds__(kWarps8 * 32) attn_int8_mma_kernel(const __gri
     unit /= p.tiles;
     const int hk = unit % p.nkv, row_first = unit / p.nkv * p.rows_at_once, row_end = min(p.n, row_first + p.rows_at_once);
     unsigned char* ring = smem + (size_t)warp * kStages * kStage;
-    int filled = 0, used = 0;  // pages asked for and met, over all runs
+    int filled = 0, used = 0;  // pieces asked for and met, over all runs
 
     for (int r0 = row_first, r1; r0 < row_end; r0 = r1) {
+        // ---- the queries of as many rows as the run may have are asked for beside its sequence and positions, before anything waits
+        const int e0 = tile * kTile;
+        float x[MT][D / 4];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            const int e = min(e0 + 8 * i + g, (row_end - r0) * per - 1);
+            const T* q = reinterpret_cast<const T*>(p.q) + (size_t)(r0 + e / per) * p.q_stride + (size_t)(hk * per + e % per) * D + t * (D / 4);
+            if (p.aligned) {
+#pragma unroll
+                for (int c = 0; c < D / 4; c += 4) {
+                    const float4 v = load4(q + c);
+                    x[i][c] = v.x; x[i][c + 1] = v.y; x[i][c + 2] = v.z; x[i][c + 3] = v.w;
+                }
+            } else {
+#pragma unroll
+                for (int c = 0; c < D / 4; ++c) x[i][c] = to_float(q[c]);
+            }
+        }
         // ---- the run, its keys and this slice's part of them (the same for every thread of the CTA)
         const int seq = p.token_seq[r0];
         int top_pos = -1, low = INT_MAX, low_pos = INT_MAX, top_low = 0;
@@ -146,38 +165,44 @@ __global__ void __launch_bounds__(kWarps8 * 32) attn_int8_mma_kernel(const __gri
             low = min(low, lo);
             top_low = max(top_low, lo);
         }
-        const int entries = (r1 - r0) * per, e0 = tile * kTile;
+        const int entries = (r1 - r0) * per;
         if (e0 >= entries) continue;
         const bool known = seq >= 0 && seq < p.table_rows && top_pos >= 0;
         const int* table = p.page_table + (size_t)(known ? seq : 0) * p.table_cols;
-        const int page_low = known ? low / kPage8 : 0, page_top = known ? min(top_pos / kPage8 + 1, p.table_cols) : 0;
-        const int slices = max(1, (page_top - page_low + p.slice_pages - 1) / p.slice_pages);
+        constexpr int kHalves = kPage8 / kPiece8;
+        const int piece_low = known ? low / kPiece8 : 0, piece_top = known ? (int)min((long long)top_pos / kPiece8 + 1, (long long)kHalves * p.table_cols) : 0;
+        const int slices = max(1, (piece_top - piece_low + p.slice_pieces - 1) / p.slice_pieces);
         if (slice >= slices) continue;
-        const int first = page_low + slice * p.slice_pages, last = min(page_top, first + p.slice_pages);
+        const int first = piece_low + slice * p.slice_pieces, last = min(piece_top, first + p.slice_pieces);
 
-        // ---- copies: this warp's pages are first + warp, + 4, ...; ids outside the store are passed over
-        auto next_page = [&](int page) {
-            while (page < last && (unsigned)table[page] >= (unsigned)p.pages) page += kWarps8;
-            return page;
-        };
-        int to_fill = next_page(first + warp), page = to_fill;
+        // ---- copies: this warp's pieces are first + warp, + 4, ...; those of pages outside the store are passed over
+        // (the next piece's page is asked for as a piece is filled, and looked at when its turn comes)
+        int next = first + warp, page = next < last ? table[next / kHalves] : -1;
         auto fill = [&]() {
-            if (to_fill >= last) return;
-            if (lane == 0) {
+            while (next < last && (unsigned)page >= (unsigned)p.pages) {
+                next += kWarps8;
+                page = next < last ? table[next / kHalves] : -1;
+            }
+            if (next >= last) return;
+            if (lane < 4) {  // (keys, values and the scales of each: one copy a lane)
                 unsigned char* at = ring + (filled % kStages) * kStage;
                 uint64_t* bar = &full[warp][filled % kStages];
-                const size_t head = (size_t)table[to_fill] * p.nkv + hk;
-                mbar_expect_tx(bar, kStage);
-                bulk_load(at, p.k + head * kPage8 * D, kPage8 * D, bar);
-                bulk_load(at + 2 * kPage8 * D, p.k_scales + head * kPage8, kPage8 * 4, bar);
-                bulk_load(at + kPage8 * D, p.v + head * kPage8 * D, kPage8 * D, bar);
-                bulk_load(at + 2 * kPage8 * D + kPage8 * 4, p.v_scales + head * kPage8, kPage8 * 4, bar);
+                const size_t row = ((size_t)page * p.nkv + hk) * kPage8 + next % kHalves * kPiece8;
+                if (lane == 0) {
+                    mbar_expect_tx(bar, kStage);
+                    piece_in[warp][filled % kStages] = next;
+                }
+                const void* from = lane < 2 ? (const void*)((lane == 0 ? p.k : p.v) + row * D) : (const void*)((lane == 2 ? p.k_scales : p.v_scales) + row);
+                bulk_load(at + (lane < 2 ? lane * kPiece8 * D : 2 * kPiece8 * D + (lane - 2) * kPiece8 * 4), from,
+                          lane < 2 ? kPiece8 * D : kPiece8 * 4, bar);
             }
             ++filled;
-            to_fill = next_page(to_fill + kWarps8);
+            next += kWarps8;
+            page = next < last ? table[next / kHalves] : -1;
         };
 #pragma unroll 1
         for (int s = 0; s < kStages; ++s) fill();
+        __syncwarp();
 
         // ---- the tile's queries as whole numbers
         uint32_t qa[MT][kSteps][4], ql[F32 ? MT : 1][F32 ? kSteps : 1][2];
@@ -185,27 +210,11 @@ __global__ void __launch_bounds__(kWarps8 * 32) attn_int8_mma_kernel(const __gri
         int pos_of[MT], low_of[MT];
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
-            const int e = e0 + 8 * i + g, row = r0 + min(e, entries - 1) / per, head = hk * per + min(e, entries - 1) % per;
-            pos_of[i] = e < entries && known ? p.token_pos[row] : -1;
+            const int e = e0 + 8 * i + g;
+            pos_of[i] = e < entries && known ? p.token_pos[r0 + e / per] : -1;
             low_of[i] = p.window > 0 ? max(0, pos_of[i] - p.window + 1) : 0;
-            float x[D / 4];
-            const T* q = reinterpret_cast<const T*>(p.q) + (size_t)row * p.q_stride + (size_t)head * D + t * (D / 4);
-#pragma unroll
-            for (int c = 0; c < D / 4; ++c) x[c] = 0.f;
-            if (pos_of[i] >= 0) {
-                if (p.aligned) {
-#pragma unroll
-                    for (int c = 0; c < D / 4; c += 4) {
-                        const float4 v = load4(q + c);
-                        x[c] = v.x; x[c + 1] = v.y; x[c + 2] = v.z; x[c + 3] = v.w;
-                    }
-                } else {
-#pragma unroll
-                    for (int c = 0; c < D / 4; ++c) x[c] = to_float(q[c]);
-                }
-            }
             uint32_t hi[kWords], mid[kWords], lo[kWords];
-            factor[i] = query_codes<D, F32>(x, hi, mid, lo) * p.scale * 1.4426950408889634f;
+            factor[i] = query_codes<D, F32>(x[i], hi, mid, lo) * p.scale * 1.4426950408889634f;
 #pragma unroll
             for (int s = 0; s < kSteps; ++s) {
                 qa[i][s][0] = hi[2 * s];
@@ -224,20 +233,21 @@ __global__ void __launch_bounds__(kWarps8 * 32) attn_int8_mma_kernel(const __gri
         float unit_t = 0.f, inverse_t = 0.f;  // T and 2^15 / T
 
 #pragma unroll 1
-        for (; page < last; page = next_page(page + kWarps8)) {
+        while (used < filled) {
+            const int piece = piece_in[warp][used % kStages];
             const unsigned char* at = ring + (used % kStages) * kStage;
             if (!mbar_wait(&full[warp][used % kStages], (uint32_t)(used / kStages) & 1u)) {
                 if (lane == 0) atomicExch(p.status, 1);
                 break;
             }
-            const float* ks = reinterpret_cast<const float*>(at + 2 * kPage8 * D);
-            const float* vs = ks + kPage8;
-            const int key0 = page * kPage8 + 4 * t;
-            const bool whole = page * kPage8 >= top_low && page * kPage8 + kPage8 - 1 <= low_pos;
+            const float* ks = reinterpret_cast<const float*>(at + 2 * kPiece8 * D);
+            const float* vs = ks + kPiece8;
+            const int key0 = piece * kPiece8 + 4 * t;
+            const bool whole = piece * kPiece8 >= top_low && piece * kPiece8 + kPiece8 - 1 <= low_pos;
             // ---- scores, in units of log 2: position 16 s + 4 t + i is value i of step s
-            float sc[MT][16];
+            float sc[MT][kScores];
 #pragma unroll
-            for (int s = 0; s < 4; ++s) {
+            for (int s = 0; s < kScores / 4; ++s) {
                 int acc[MT][2][4] = {}, acl[F32 ? MT : 1][2][4] = {};
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
@@ -273,20 +283,20 @@ __global__ void __launch_bounds__(kWarps8 * 32) attn_int8_mma_kernel(const __gri
 #pragma unroll
                 for (int i = 0; i < MT; ++i)
 #pragma unroll
-                    for (int c = 0; c < 16; ++c) {
+                    for (int c = 0; c < kScores; ++c) {
                         const int key = key0 + 16 * (c >> 2) + (c & 3);
                         if (key > pos_of[i] || key < low_of[i]) sc[i][c] = -INFINITY;
                     }
             }
             // ---- T grows to a power of two above the scales of the positions that anyone sees
-            float ts[16], t_most = 0.f;
+            float ts[kScores], t_most = 0.f;
 #pragma unroll
-            for (int s = 0; s < 4; ++s) {
+            for (int s = 0; s < kScores / 4; ++s) {
                 const float4 scales = *reinterpret_cast<const float4*>(vs + 16 * s + 4 * t);
                 ts[4 * s] = scales.x; ts[4 * s + 1] = scales.y; ts[4 * s + 2] = scales.z; ts[4 * s + 3] = scales.w;
             }
 #pragma unroll
-            for (int c = 0; c < 16; ++c) {
+            for (int c = 0; c < kScores; ++c) {
                 const int key = key0 + 16 * (c >> 2) + (c & 3);
                 if (whole || (key >= low && key <= top_pos)) t_most = fmaxf(t_most, ts[c]);
             }
@@ -305,7 +315,7 @@ __global__ void __launch_bounds__(kWarps8 * 32) attn_int8_mma_kernel(const __gri
             for (int i = 0; i < MT; ++i) {
                 float most = sc[i][0];
 #pragma unroll
-                for (int c = 1; c < 16; ++c) most = fmaxf(most, sc[i][c]);
+                for (int c = 1; c < kScores; ++c) most = fmaxf(most, sc[i][c]);
                 most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
                 most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
                 const float now = fmaxf(m[i], most), base = now == -INFINITY ? 0.f : now;
@@ -313,7 +323,7 @@ __global__ void __launch_bounds__(kWarps8 * 32) attn_int8_mma_kernel(const __gri
                 m[i] = now;
                 float sum = 0.f;
 #pragma unroll
-                for (int c = 0; c < 16; ++c) {
+                for (int c = 0; c < kScores; ++c) {
                     sc[i][c] = ex2_8(sc[i][c] - base);
                     sum += sc[i][c];
                 }
@@ -338,7 +348,7 @@ __global__ void __launch_bounds__(kWarps8 * 32) attn_int8_mma_kernel(const __gri
             }
             // ---- outputs
 #pragma unroll
-            for (int s = 0; s < 4; ++s) {
+            for (int s = 0; s < kScores / 4; ++s) {
                 uint32_t a[kOuts][4];
 #pragma unroll
                 for (int u = 0; u < kOuts; ++u)
@@ -367,7 +377,7 @@ __global__ void __launch_bounds__(kWarps8 * 32) attn_int8_mma_kernel(const __gri
                     }
                 uint32_t vw[4][kValueWords];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) load_words<kValueWords>(vw[r], at + kPage8 * D + (16 * s + 4 * t + r) * D + g * (D / 8));
+                for (int r = 0; r < 4; ++r) load_words<kValueWords>(vw[r], at + kPiece8 * D + (16 * s + 4 * t + r) * D + g * (D / 8));
 #pragma unroll
                 for (int w = 0; w < kValueWords; ++w) {
                     uint32_t c0 = vw[0][w] ^ 0x80808080u, c1 = vw[1][w] ^ 0x80808080u, c2 = vw[2][w] ^ 0x80808080u, c3 = vw[3][w] ^ 0x80808080u;

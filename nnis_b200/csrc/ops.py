@@ -3132,18 +3132,18 @@ def attention_int8_splits(n: int, heads: int, keys: int, device) -> int:
 
 @functools.lru_cache(maxsize=4096)
 def attention_int8_plan(n: int, seqs: int, heads: int, kv_heads: int, d: int, cols: int, window: int, sms: int):
-    """(slices, pages of a slice, rows taken together) of the tensor cores' kernel: rows of a sequence lie together, as many as come on
-    each, up to 64 queries a key/value head; slices cover the table, at most 64, as short as fills the device."""
+    """(slices, runs of 32 positions in a slice, rows taken together) of the tensor cores' kernel: rows of a sequence lie together, as
+    many as come on each, up to 64 queries a key/value head; slices cover the table, at most 64, as short as fills the device."""
     per = heads // kv_heads
     rows = max(1, min(-(-n // max(1, seqs)), 64 // per))
     units = -(-n // rows) * kv_heads * -(-rows * per // 16)
-    seen = min(cols, (window + rows + 62) // 64 + 1) if window else cols
-    resident = sms * (1 if d == 128 else 2 if d >= 64 else 4)
-    pages = max(4, -(-seen * units // (INT8_WAVES * resident)), -(-cols // 64))
-    return -(-cols // pages), pages, rows
+    seen = min(2 * cols, (window + rows + 30) // 32 + 1) if window else 2 * cols
+    resident = sms * (4 if d <= 64 else 2)
+    pieces = max(INT8_LEAST_PIECES, -(-seen * units // resident), -(-2 * cols // 64))
+    return -(-2 * cols // pieces), pieces, rows
 
 
-INT8_WAVES = 2
+INT8_LEAST_PIECES = 8
 
 
 def attention_int8(q: torch.Tensor, q_stride: int, k: torch.Tensor, v: torch.Tensor, k_scales: torch.Tensor, v_scales: torch.Tensor,
@@ -3186,10 +3186,10 @@ def attention_int8(q: torch.Tensor, q_stride: int, k: torch.Tensor, v: torch.Ten
         with torch.cuda.device(index):
             return attention_int8(q, q_stride, k, v, k_scales, v_scales, token_pos, token_seq, page_table, out, heads, kv_heads, d,
                                   window, scale, workspace)
-    tickets = status = slice_pages = rows = 0
+    tickets = status = slice_pieces = rows = 0
     at = k.data_ptr(), v.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), out.data_ptr()
     if page_size == 64 and d in (32, 64, 96, 128) and not (at[0] | at[1] | at[2] | at[3] | at[4]) % 16:
-        splits, slice_pages, rows = attention_int8_plan(n, seqs, heads, kv_heads, d, cols, window, _sm_count.get(index) or sm_count(k.device))
+        splits, slice_pieces, rows = attention_int8_plan(n, seqs, heads, kv_heads, d, cols, window, _sm_count.get(index) or sm_count(k.device))
         partial = workspace.room("attn_int8_records", n * heads * splits * (d + 4), torch.float32).data_ptr() if splits > 1 else 0
         tickets = workspace.zeros_room("attn_int8_tickets", n * kv_heads * -(-rows * (heads // kv_heads) // 8), torch.int32).data_ptr() \
             if splits > 1 else 0
@@ -3200,8 +3200,8 @@ def attention_int8(q: torch.Tensor, q_stride: int, k: torch.Tensor, v: torch.Ten
         partial = workspace.room("attn_int8_partial", n * heads * splits * (d + 2), torch.float32).data_ptr() if splits > 1 else 0
     _check(_entry("nnis_attention_int8")(
         q.data_ptr(), at[0], at[1], at[2], at[3], token_pos.data_ptr(), token_seq.data_ptr(), page_table.data_ptr(), at[4], partial,
-        tickets, status, q_stride, seqs, cols, pages, n, heads, kv_heads, d, page_size, window, scale, splits, slice_pages, rows, _DTYPE_CODE[dtype], _stream_of(index)),
-        "attention_int8", 2 if splits > 1 and not slice_pages else 1)
+        tickets, status, q_stride, seqs, cols, pages, n, heads, kv_heads, d, page_size, window, scale, splits, slice_pieces, rows, _DTYPE_CODE[dtype], _stream_of(index)),
+        "attention_int8", 2 if splits > 1 and not slice_pieces else 1)
 
 
 def int8_width(k: int) -> int:
