@@ -22,13 +22,15 @@ struct Attend8 {
     float scale;
     int splits;      // most slices of a row
     // the tensor cores' kernel
-    int slice_pieces, rows_at_once, tiles, aligned;
+    int slice_pieces, rows_at_once, tiles, aligned, cluster;  // cluster: CTAs that share a slice, at most 8
     unsigned* tickets;  // n * nkv * tiles, zero between launches
     int* status;
 };
 
-// Pieces of 32 positions that a warp has on their way or in use.
-__host__ __device__ constexpr int stages8(int d) { return 3; }
+// Positions that a warp takes at a time (what each time costs beside its positions is a third of 32 positions of 64 values), and how
+// many such pieces it has on their way or in use: three CTAs an SM with heads of 64, two with 96 and 128.
+__host__ __device__ constexpr int piece8(int d) { return d <= 64 ? 64 : 32; }
+__host__ __device__ constexpr int stages8(int d) { return d <= 64 ? 2 : 3; }
 
 __device__ __forceinline__ void fence_async_shared8() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 

@@ -28,14 +28,20 @@
 
 namespace nnis {
 
-constexpr int kPage8 = 64, kPiece8 = 32, kWarps8 = 4;  // positions of a page, and of what a warp takes at a time
+constexpr int kPage8 = 64, kWarps8 = 4;
 
-__host__ __device__ constexpr int stage_bytes8(int d) { return 2 * kPiece8 * d + 2 * kPiece8 * 4; }
+__host__ __device__ constexpr int stage_bytes8(int d) { return 2 * piece8(d) * (d + 4); }
 
 __device__ __forceinline__ void mma_s8(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// The same without sums before it
+__device__ __forceinline__ void mma_s8_first(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(0));
 }
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -56,6 +62,39 @@ __device__ __forceinline__ uint32_t code_halves(uint32_t pair, uint32_t select) 
     const uint32_t biased = __byte_perm(pair, 0x64646464u, select), bias = 0x64806480u;  // 1,024 + 128
     const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&biased), *reinterpret_cast<const __half2*>(&bias));
     return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+constexpr int kMostCluster8 = 8;
+// Every thread of every CTA of the cluster
+__device__ __forceinline__ void cluster_sync8() {
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// What lies at the same place of the shared memory of the cluster's CTA `rank`
+__device__ __forceinline__ uint32_t peer_addr(const void* p, int rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_addr(p)), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float2 peer_load2(const float* p, int rank) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(peer_addr(p, rank)) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 peer_load4(const float* p, int rank) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(peer_addr(p, rank)) : "memory");
+    return v;
+}
+
+__device__ __forceinline__ void add_part(float4& sum, float& total, const float4& v, float l, float share) {
+    total = fmaf(share, l, total);
+    sum.x = fmaf(share, v.x, sum.x);
+    sum.y = fmaf(share, v.y, sum.y);
+    sum.z = fmaf(share, v.z, sum.z);
+    sum.w = fmaf(share, v.w, sum.w);
 }
 
 template <int N>
@@ -109,14 +148,14 @@ __device__ __forceinline__ float query_codes(const float (&x)[D / 4], uint32_t (
 }
 
 template <int D, bool F32, int MT>
-__global__ void __launch_bounds__(kWarps8 * 32) attn_int8_mma_kernel(const __grid_constant__ Attend8 p) {
+__global__ void __launch_bounds__(kWarps8 * 32, D <= 32 ? 4 : D <= 64 ? 3 : 2) attn_int8_mma_kernel(const __grid_constant__ Attend8 p) {
     using T = std::conditional_t<F32, float, bf16>;
     constexpr int kStage = stage_bytes8(D), kTile = 8 * MT, kSteps = D / 32, kWords = D / 16, kValueWords = D / 32, kCols = D / 8;
     constexpr int kOuts = F32 ? MT : (MT + 1) / 2;  // products of the weights per step of 16 positions
-    constexpr int kStages = stages8(D), kScores = kPiece8 / 4;  // (a lane's positions of a piece: 16 s + 4 t + 0 to 3)
+    constexpr int kPiece8 = piece8(D), kStages = stages8(D), kScores = kPiece8 / 4;  // (a lane's positions of a piece: 16 s + 4 t + 0 to 3)
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ __align__(8) uint64_t full[kWarps8][kStages];
-    __shared__ int joins, piece_in[kWarps8][kStages];
+    __shared__ int joins;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     if (lane == 0) {  // (a warp's barriers are its own)
         for (int s = 0; s < kStages; ++s) mbar_init(&full[warp][s], 1);
@@ -126,13 +165,21 @@ __global__ void __launch_bounds__(kWarps8 * 32) attn_int8_mma_kernel(const __gri
     pdl_wait();
     pdl_launch_dependents();
 
-    const int per = p.nq / p.nkv, slice = blockIdx.y;
+    const int per = p.nq / p.nkv, slice = blockIdx.y / p.cluster, rank = blockIdx.y % p.cluster;
     int unit = blockIdx.x;
     const int tile = unit % p.tiles;
     unit /= p.tiles;
     const int hk = unit % p.nkv, row_first = unit / p.nkv * p.rows_at_once, row_end = min(p.n, row_first + p.rows_at_once);
     unsigned char* ring = smem + (size_t)warp * kStages * kStage;
-    int filled = 0, used = 0;  // pieces asked for and met, over all runs
+    int stage = 0;  // the ring's next, over all runs, and the phase of its barrier
+    uint32_t phase = 0;
+    // what lane 0 to 3 copies of a piece: codes of keys, of values, scales of keys, of values
+    const bool codes = lane < 2;
+    const unsigned char* mine = codes ? reinterpret_cast<const unsigned char*>(lane == 0 ? p.k : p.v)
+                                      : reinterpret_cast<const unsigned char*>(lane == 2 ? p.k_scales : p.v_scales);
+    const uint32_t row_bytes = codes ? D : 4, piece_bytes = kPiece8 * row_bytes, page_bytes = (uint32_t)p.nkv * kPage8 * row_bytes;
+    const uint32_t to_lane = codes ? lane * kPiece8 * D : 2 * kPiece8 * D + (lane & 1) * kPiece8 * 4;
+    mine += (size_t)hk * kPage8 * row_bytes;
 
     for (int r0 = row_first, r1; r0 < row_end; r0 = r1) {
         // ---- the queries of as many rows as the run may have are asked for beside its sequence and positions, before anything waits
@@ -171,38 +218,33 @@ __global__ void __launch_bounds__(kWarps8 * 32) attn_int8_mma_kernel(const __gri
         const int* table = p.page_table + (size_t)(known ? seq : 0) * p.table_cols;
         constexpr int kHalves = kPage8 / kPiece8;
         const int piece_low = known ? low / kPiece8 : 0, piece_top = known ? (int)min((long long)top_pos / kPiece8 + 1, (long long)kHalves * p.table_cols) : 0;
+        // a slice's pieces are dealt out to all warps of its cluster
         const int slices = max(1, (piece_top - piece_low + p.slice_pieces - 1) / p.slice_pieces);
         if (slice >= slices) continue;
-        const int first = piece_low + slice * p.slice_pieces, last = min(piece_top, first + p.slice_pieces);
+        const int first = piece_low + slice * p.slice_pieces, last = min(piece_top, first + p.slice_pieces), step = kWarps8 * p.cluster;
 
-        // ---- copies: this warp's pieces are first + warp, + 4, ...; those of pages outside the store are passed over
-        // (the next piece's page is asked for as a piece is filled, and looked at when its turn comes)
-        int next = first + warp, page = next < last ? table[next / kHalves] : -1;
-        auto fill = [&]() {
+        // ---- copies: this warp's pieces are every step-th; those of pages outside the store are passed over.  The next
+        // piece's page is asked for as a piece is copied, and looked at when its turn comes.
+        int next = first + rank * kWarps8 + warp, page = next < last ? table[(unsigned)next / kHalves] : -1;
+        auto copy = [&](int to) {  // the piece that is copied to this stage, -1 where none is left
             while (next < last && (unsigned)page >= (unsigned)p.pages) {
-                next += kWarps8;
-                page = next < last ? table[next / kHalves] : -1;
+                next += step;
+                page = next < last ? table[(unsigned)next / kHalves] : -1;
             }
-            if (next >= last) return;
-            if (lane < 4) {  // (keys, values and the scales of each: one copy a lane)
-                unsigned char* at = ring + (filled % kStages) * kStage;
-                uint64_t* bar = &full[warp][filled % kStages];
-                const size_t row = ((size_t)page * p.nkv + hk) * kPage8 + next % kHalves * kPiece8;
-                if (lane == 0) {
-                    mbar_expect_tx(bar, kStage);
-                    piece_in[warp][filled % kStages] = next;
-                }
-                const void* from = lane < 2 ? (const void*)((lane == 0 ? p.k : p.v) + row * D) : (const void*)((lane == 2 ? p.k_scales : p.v_scales) + row);
-                bulk_load(at + (lane < 2 ? lane * kPiece8 * D : 2 * kPiece8 * D + (lane - 2) * kPiece8 * 4), from,
-                          lane < 2 ? kPiece8 * D : kPiece8 * 4, bar);
+            if (next >= last) return -1;
+            if (lane < 4) {
+                if (lane == 0) mbar_expect_tx(&full[warp][to], kStage);
+                bulk_load(ring + to * kStage + to_lane, mine + (size_t)(unsigned)page * page_bytes + (unsigned)next % kHalves * piece_bytes, piece_bytes,
+                          &full[warp][to]);
             }
-            ++filled;
-            next += kWarps8;
-            page = next < last ? table[next / kHalves] : -1;
+            const int piece = next;
+            next += step;
+            page = next < last ? table[(unsigned)next / kHalves] : -1;
+            return piece;
         };
-#pragma unroll 1
-        for (int s = 0; s < kStages; ++s) fill();
-        __syncwarp();
+        int queue[kStages];
+#pragma unroll
+        for (int s = 0; s < kStages; ++s) queue[s] = copy(stage + s < kStages ? stage + s : stage + s - kStages);
 
         // ---- the tile's queries as whole numbers
         uint32_t qa[MT][kSteps][4], ql[F32 ? MT : 1][F32 ? kSteps : 1][2];
@@ -233,10 +275,10 @@ __global__ void __launch_bounds__(kWarps8 * 32) attn_int8_mma_kernel(const __gri
         float unit_t = 0.f, inverse_t = 0.f;  // T and 2^15 / T
 
 #pragma unroll 1
-        while (used < filled) {
-            const int piece = piece_in[warp][used % kStages];
-            const unsigned char* at = ring + (used % kStages) * kStage;
-            if (!mbar_wait(&full[warp][used % kStages], (uint32_t)(used / kStages) & 1u)) {
+        while (queue[0] >= 0) {
+            const int piece = queue[0];
+            const unsigned char* at = ring + stage * kStage;
+            if (!mbar_wait(&full[warp][stage], phase)) {
                 if (lane == 0) atomicExch(p.status, 1);
                 break;
             }
@@ -248,7 +290,7 @@ __global__ void __launch_bounds__(kWarps8 * 32) attn_int8_mma_kernel(const __gri
             float sc[MT][kScores];
 #pragma unroll
             for (int s = 0; s < kScores / 4; ++s) {
-                int acc[MT][2][4] = {}, acl[F32 ? MT : 1][2][4] = {};
+                int acc[MT][2][4], acl[F32 ? MT : 1][2][4];
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     uint32_t w[kWords];
@@ -257,10 +299,12 @@ __global__ void __launch_bounds__(kWarps8 * 32) attn_int8_mma_kernel(const __gri
                     for (int i = 0; i < MT; ++i)
 #pragma unroll
                         for (int k = 0; k < kSteps; ++k) {
-                            mma_s8(acc[i][j], qa[i][k], w[2 * k], w[2 * k + 1]);
+                            if (k == 0) mma_s8_first(acc[i][j], qa[i][k], w[2 * k], w[2 * k + 1]);
+                            else mma_s8(acc[i][j], qa[i][k], w[2 * k], w[2 * k + 1]);
                             if constexpr (F32) {
                                 const uint32_t a[4] = {ql[i][k][0], 0u, ql[i][k][1], 0u};
-                                mma_s8(acl[i][j], a, w[2 * k], w[2 * k + 1]);
+                                if (k == 0) mma_s8_first(acl[i][j], a, w[2 * k], w[2 * k + 1]);
+                                else mma_s8(acl[i][j], a, w[2 * k], w[2 * k + 1]);
                             }
                         }
                 }
@@ -279,61 +323,61 @@ __global__ void __launch_bounds__(kWarps8 * 32) attn_int8_mma_kernel(const __gri
                         sc[i][4 * s + c] = sum * factor[i] * key_scale[c];
                     }
             }
-            if (!whole) {
-#pragma unroll
-                for (int i = 0; i < MT; ++i)
-#pragma unroll
-                    for (int c = 0; c < kScores; ++c) {
-                        const int key = key0 + 16 * (c >> 2) + (c & 3);
-                        if (key > pos_of[i] || key < low_of[i]) sc[i][c] = -INFINITY;
-                    }
-            }
-            // ---- T grows to a power of two above the scales of the positions that anyone sees
-            float ts[kScores], t_most = 0.f;
+            float ts[kScores];
 #pragma unroll
             for (int s = 0; s < kScores / 4; ++s) {
                 const float4 scales = *reinterpret_cast<const float4*>(vs + 16 * s + 4 * t);
                 ts[4 * s] = scales.x; ts[4 * s + 1] = scales.y; ts[4 * s + 2] = scales.z; ts[4 * s + 3] = scales.w;
             }
-#pragma unroll
-            for (int c = 0; c < kScores; ++c) {
-                const int key = key0 + 16 * (c >> 2) + (c & 3);
-                if (whole || (key >= low && key <= top_pos)) t_most = fmaxf(t_most, ts[c]);
-            }
-            t_most = fmaxf(t_most, __shfl_xor_sync(0xffffffffu, t_most, 1));
-            t_most = fmaxf(t_most, __shfl_xor_sync(0xffffffffu, t_most, 2));
-            float grown = 1.f;
-            if (t_most >= unit_t && t_most >= 0x1p-100f) {
-                const uint32_t bits = min((__float_as_uint(t_most) & 0x7f800000u) + 0x00800000u, 0x7e800000u);  // (at most 2^126)
-                grown = unit_t * __uint_as_float(0x7f000000u - bits);  // T before / T now
-                unit_t = __uint_as_float(bits);
-                inverse_t = __uint_as_float(0x7f000000u - bits) * 32768.f;
-            }
-            // ---- weights
-            float shrink[MT];
-#pragma unroll
-            for (int i = 0; i < MT; ++i) {
-                float most = sc[i][0];
-#pragma unroll
-                for (int c = 1; c < kScores; ++c) most = fmaxf(most, sc[i][c]);
-                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-                const float now = fmaxf(m[i], most), base = now == -INFINITY ? 0.f : now;
-                shrink[i] = ex2_8(m[i] - base);
-                m[i] = now;
-                float sum = 0.f;
+            // (a value's scale that is no number must not meet a weight of zero: nobody's positions have none, and where one row of
+            // several sees such a value and another does not, the weights are looked at one by one)
+            bool looks = false;
+            if (!whole) {
 #pragma unroll
                 for (int c = 0; c < kScores; ++c) {
-                    sc[i][c] = ex2_8(sc[i][c] - base);
-                    sum += sc[i][c];
-                }
-                l[i] = l[i] * shrink[i] + sum;
-                shrink[i] *= grown;
-            }
-            bool same = true;
+                    const int key = key0 + 16 * (c >> 2) + (c & 3);
+                    if (key < low || key > top_pos) ts[c] = 0.f;
+                    looks = looks || ts[c] != ts[c];
 #pragma unroll
-            for (int i = 0; i < MT; ++i) same = same && shrink[i] == 1.f;
-            if (!__all_sync(0xffffffffu, same)) {
+                    for (int i = 0; i < MT; ++i)
+                        if (key > pos_of[i] || key < low_of[i]) sc[i][c] = -INFINITY;
+                }
+                looks = __any_sync(0xffffffffu, looks);
+            }
+            float t_most = ts[0];
+#pragma unroll
+            for (int c = 1; c < kScores; ++c) t_most = fmaxf(t_most, ts[c]);
+            float most[MT];
+            bool rises = t_most >= unit_t;
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                most[i] = sc[i][0];
+#pragma unroll
+                for (int c = 1; c < kScores; ++c) most[i] = fmaxf(most[i], sc[i][c]);
+                rises = rises || most[i] > m[i];
+            }
+            // ---- only where some maximum or T has risen are they joined and what has been added up brought in line
+            if (__any_sync(0xffffffffu, rises)) {
+                t_most = fmaxf(t_most, __shfl_xor_sync(0xffffffffu, t_most, 1));
+                t_most = fmaxf(t_most, __shfl_xor_sync(0xffffffffu, t_most, 2));
+                float grown = 1.f;
+                if (t_most >= unit_t && t_most >= 0x1p-100f) {
+                    const uint32_t bits = min((__float_as_uint(t_most) & 0x7f800000u) + 0x00800000u, 0x7e800000u);  // (at most 2^126)
+                    grown = unit_t * __uint_as_float(0x7f000000u - bits);  // T before / T now
+                    unit_t = __uint_as_float(bits);
+                    inverse_t = __uint_as_float(0x7f000000u - bits) * 32768.f;
+                }
+                float shrink[MT];
+#pragma unroll
+                for (int i = 0; i < MT; ++i) {
+                    most[i] = fmaxf(most[i], __shfl_xor_sync(0xffffffffu, most[i], 1));
+                    most[i] = fmaxf(most[i], __shfl_xor_sync(0xffffffffu, most[i], 2));
+                    const float now = fmaxf(m[i], most[i]);
+                    shrink[i] = now == -INFINITY ? 1.f : ex2_8(m[i] - now);
+                    m[i] = now;
+                    l[i] *= shrink[i];
+                    shrink[i] *= grown;
+                }
 #pragma unroll
                 for (int u = 0; u < kOuts; ++u) {
                     const float a = shrink[F32 ? u : 2 * u], b = F32 ? a : 2 * u + 1 < MT ? shrink[2 * u + 1 < MT ? 2 * u + 1 : 0] : 1.f;
@@ -346,6 +390,25 @@ __global__ void __launch_bounds__(kWarps8 * 32) attn_int8_mma_kernel(const __gri
                     }
                 }
             }
+            // ---- weights, then times the values' scales
+#pragma unroll
+            for (int c = 0; c < kScores; ++c) ts[c] *= inverse_t;
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                const float base = m[i] == -INFINITY ? 0.f : m[i];
+#pragma unroll
+                for (int c = 0; c < kScores; ++c) {
+                    sc[i][c] = ex2_8(sc[i][c] - base);
+                    l[i] += sc[i][c];
+                }
+                if (looks) {
+#pragma unroll
+                    for (int c = 0; c < kScores; ++c) sc[i][c] = sc[i][c] == 0.f ? 0.f : sc[i][c] * ts[c];
+                } else {
+#pragma unroll
+                    for (int c = 0; c < kScores; ++c) sc[i][c] *= ts[c];
+                }
+            }
             // ---- outputs
 #pragma unroll
             for (int s = 0; s < kScores / 4; ++s) {
@@ -355,24 +418,14 @@ __global__ void __launch_bounds__(kWarps8 * 32) attn_int8_mma_kernel(const __gri
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {  // positions 4 t + 2 half, + 1
                         const int c = 4 * s + 2 * half;
-                        float w[2][2];
-#pragma unroll
-                        for (int i = 0; i < 2; ++i)
-#pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                const int mt = F32 ? u : 2 * u + i < MT ? 2 * u + i : 0;
-                                const float weight = sc[mt][c + e];
-                                // (a scale that is no number, where nobody looks, must not meet a weight of zero)
-                                w[i][e] = whole || weight != 0.f ? weight * (ts[c + e] * inverse_t) : 0.f;
-                            }
                         if constexpr (F32) {
-                            const uint32_t h = half2_bits(w[0][0], w[0][1]);
+                            const uint32_t h = half2_bits(sc[u][c], sc[u][c + 1]);
                             const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
                             a[u][2 * half] = h;
-                            a[u][2 * half + 1] = half2_bits(w[0][0] - f.x, w[0][1] - f.y);
+                            a[u][2 * half + 1] = half2_bits(sc[u][c] - f.x, sc[u][c + 1] - f.y);
                         } else {
-                            a[u][2 * half] = half2_bits(w[0][0], w[0][1]);
-                            a[u][2 * half + 1] = 2 * u + 1 < MT ? half2_bits(w[1][0], w[1][1]) : 0u;
+                            a[u][2 * half] = half2_bits(sc[2 * u][c], sc[2 * u][c + 1]);
+                            a[u][2 * half + 1] = 2 * u + 1 < MT ? half2_bits(sc[2 * u + 1 < MT ? 2 * u + 1 : 0][c], sc[2 * u + 1 < MT ? 2 * u + 1 : 0][c + 1]) : 0u;
                         }
                     }
                 uint32_t vw[4][kValueWords];
@@ -391,9 +444,14 @@ __global__ void __launch_bounds__(kWarps8 * 32) attn_int8_mma_kernel(const __gri
                         for (int u = 0; u < kOuts; ++u) mma_f16(o[u][4 * w + c], a[u], b0[c], b1[c]);
                 }
             }
-            ++used;
             __syncwarp();  // every lane is done with the stage
-            fill();
+#pragma unroll
+            for (int s = 0; s + 1 < kStages; ++s) queue[s] = queue[s + 1];
+            queue[kStages - 1] = copy(stage);
+            if (++stage == kStages) {
+                stage = 0;
+                phase ^= 1u;
+            }
         }
 
         // ---- the four warps' parts are joined: [queries][D] sums, then maxima and sums of weights, in the warp's own ring
@@ -425,9 +483,23 @@ __global__ void __launch_bounds__(kWarps8 * 32) attn_int8_mma_kernel(const __gri
         __syncthreads();
         const int count = min(kTile, entries - e0);
         auto warp_part = [&](int w) { return reinterpret_cast<const float*>(smem + (size_t)w * kStages * kStage); };
+        float* together = reinterpret_cast<float*>(smem) + kTile * (D + 2);  // (behind the first warp's part)
+        auto place_of = [&](int e) { return (size_t)(r0 + (e0 + e) / per) * p.nq + hk * per + (e0 + e) % per; };
+        auto write = [&](int e, int d, const float4& sum, float total) {
+            const float inv = total == 0.f ? 0.f : 1.f / total;
+            store4(reinterpret_cast<T*>(p.out) + place_of(e) * D + d, make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv));
+        };
+        auto put = [&](int e, int d, const float4& sum, float most, float total) {  // the slice's sums: the output, or a record of them
+            if (slices == 1) {
+                write(e, d, sum, total);
+                return;
+            }
+            float* rec = p.partial + (place_of(e) * p.splits + slice) * (D + 4);
+            __stcg(reinterpret_cast<float4*>(rec + 4 + d), sum);
+            if (d == 0) __stcg(reinterpret_cast<float2*>(rec), make_float2(most, total));
+        };
         for (int at = threadIdx.x; at < count * (D / 4); at += kWarps8 * 32) {
             const int e = at / (D / 4), d = at % (D / 4) * 4;
-            const int row = r0 + (e0 + e) / per, head = hk * per + (e0 + e) % per;
             float most = -INFINITY, total = 0.f;
             float4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -436,28 +508,47 @@ __global__ void __launch_bounds__(kWarps8 * 32) attn_int8_mma_kernel(const __gri
 #pragma unroll
             for (int w = 0; w < kWarps8; ++w) {
                 const float* part = warp_part(w);
-                const float share = ex2_8(part[kTile * D + 2 * e] - base);
-                const float4 v = *reinterpret_cast<const float4*>(part + e * D + d);
-                total = fmaf(share, part[kTile * D + 2 * e + 1], total);
-                sum.x = fmaf(share, v.x, sum.x);
-                sum.y = fmaf(share, v.y, sum.y);
-                sum.z = fmaf(share, v.z, sum.z);
-                sum.w = fmaf(share, v.w, sum.w);
+                add_part(sum, total, *reinterpret_cast<const float4*>(part + e * D + d), part[kTile * D + 2 * e + 1],
+                         ex2_8(part[kTile * D + 2 * e] - base));
             }
-            const size_t place = (size_t)row * p.nq + head;
-            if (slices == 1) {
-                const float inv = total == 0.f ? 0.f : 1.f / total;
-                store4(reinterpret_cast<T*>(p.out) + place * D + d, make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv));
+            if (p.cluster > 1) {
+                *reinterpret_cast<float4*>(together + e * D + d) = sum;
+                if (d == 0) *reinterpret_cast<float2*>(together + kTile * D + 2 * e) = make_float2(most, total);
             } else {
-                float* rec = p.partial + (place * p.splits + slice) * (D + 4);
-                __stcg(reinterpret_cast<float4*>(rec + 4 + d), sum);
-                if (d == 0) __stcg(reinterpret_cast<float2*>(rec), make_float2(most, total));
+                put(e, d, sum, most, total);
+            }
+        }
+        if (p.cluster > 1) {
+            // ---- the cluster's CTAs share out the outputs and read each other's sums
+            cluster_sync8();
+            for (int at = rank * kWarps8 * 32 + threadIdx.x; at < count * (D / 4); at += p.cluster * kWarps8 * 32) {
+                const int e = at / (D / 4), d = at % (D / 4) * 4;
+                float2 ml[kMostCluster8];
+                float4 v[kMostCluster8];
+                float most = -INFINITY, total = 0.f;
+                float4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int c = 0; c < kMostCluster8; ++c)
+                    if (c < p.cluster) {
+                        ml[c] = peer_load2(together + kTile * D + 2 * e, c);
+                        v[c] = peer_load4(together + e * D + d, c);
+                        most = fmaxf(most, ml[c].x);
+                    }
+                const float base = most == -INFINITY ? 0.f : most;
+#pragma unroll
+                for (int c = 0; c < kMostCluster8; ++c)
+                    if (c < p.cluster) add_part(sum, total, v[c], ml[c].y, ex2_8(ml[c].x - base));
+                put(e, d, sum, most, total);
             }
         }
         if (slices > 1) {
-            // ---- the slice that ends last joins the others' records, in their order
+            // ---- the slice that ends last joins the others' records, in their order (a fence of every thread: one thread's release for
+            // all of them took 3 us longer)
             __threadfence();
             __syncthreads();
+        }
+        if (p.cluster > 1) cluster_sync8();  // every record of the slice is out, and nobody reads this CTA's sums any more
+        if (slices > 1 && rank == 0) {
             if (threadIdx.x == 0) {
                 unsigned* ticket = p.tickets + ((size_t)r0 * p.nkv + hk) * p.tiles + tile;
                 unsigned old;
@@ -469,26 +560,33 @@ __global__ void __launch_bounds__(kWarps8 * 32) attn_int8_mma_kernel(const __gri
             if (joins) {
                 for (int at = threadIdx.x; at < count * (D / 4); at += kWarps8 * 32) {
                     const int e = at / (D / 4), d = at % (D / 4) * 4;
-                    const size_t place = (size_t)(r0 + (e0 + e) / per) * p.nq + hk * per + (e0 + e) % per;
-                    const float* rec = p.partial + place * p.splits * (D + 4);
+                    const float* rec = p.partial + place_of(e) * p.splits * (D + 4);
                     float most = -INFINITY, total = 0.f;
                     float4 sum = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 8
-                    for (int s = 0; s < slices; ++s) most = fmaxf(most, __ldcg(rec + (size_t)s * (D + 4)));
-                    const float base = most == -INFINITY ? 0.f : most;
-#pragma unroll 8
-                    for (int s = 0; s < slices; ++s) {
-                        const float2 ml = __ldcg(reinterpret_cast<const float2*>(rec + (size_t)s * (D + 4)));
-                        const float4 v = __ldcg(reinterpret_cast<const float4*>(rec + (size_t)s * (D + 4) + 4 + d));
-                        const float share = ex2_8(ml.x - base);
-                        total = fmaf(share, ml.y, total);
-                        sum.x = fmaf(share, v.x, sum.x);
-                        sum.y = fmaf(share, v.y, sum.y);
-                        sum.z = fmaf(share, v.z, sum.z);
-                        sum.w = fmaf(share, v.w, sum.w);
+                    constexpr int kAhead = 8;  // records asked for at once
+                    for (int s0 = 0; s0 < slices; s0 += kAhead) {
+                        float2 ml[kAhead];
+                        float4 v[kAhead];
+                        float now = most;
+#pragma unroll
+                        for (int s = 0; s < kAhead; ++s) {
+                            ml[s] = make_float2(-INFINITY, 0.f);
+                            v[s] = make_float4(0.f, 0.f, 0.f, 0.f);
+                            if (s0 + s < slices) {
+                                ml[s] = __ldcg(reinterpret_cast<const float2*>(rec + (size_t)(s0 + s) * (D + 4)));
+                                v[s] = __ldcg(reinterpret_cast<const float4*>(rec + (size_t)(s0 + s) * (D + 4) + 4 + d));
+                            }
+                        }
+#pragma unroll
+                        for (int s = 0; s < kAhead; ++s) now = fmaxf(now, ml[s].x);
+                        const float base = now == -INFINITY ? 0.f : now, before = ex2_8(most - base);
+                        total *= before;
+                        sum = make_float4(sum.x * before, sum.y * before, sum.z * before, sum.w * before);
+                        most = now;
+#pragma unroll
+                        for (int s = 0; s < kAhead; ++s) add_part(sum, total, v[s], ml[s].y, ex2_8(ml[s].x - base));
                     }
-                    const float inv = total == 0.f ? 0.f : 1.f / total;
-                    store4(reinterpret_cast<T*>(p.out) + place * D + d, make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv));
+                    write(e, d, sum, total);
                 }
             }
         }
@@ -500,12 +598,28 @@ __global__ void __launch_bounds__(kWarps8 * 32) attn_int8_mma_kernel(const __gri
 template <int D, bool F32, int MT>
 static cudaError_t launch_mma8(const Attend8& p, unsigned units, cudaStream_t stream) {
     constexpr size_t smem = (size_t)kWarps8 * stages8(D) * stage_bytes8(D);
-    static_assert(stages8(D) * stage_bytes8(D) >= 8 * MT * (D + 2) * 4, "a warp's part of the outputs fits its ring");
+    static_assert(stages8(D) * stage_bytes8(D) >= 2 * 8 * MT * (D + 2) * 4, "a warp's part of the outputs fits its ring, twice in the first");
     auto kernel = attn_int8_mma_kernel<D, F32, MT>;
     static std::atomic<int> held[16];
     const cudaError_t e = allow_shared(kernel, smem, held);
     if (e != cudaSuccess) return e;
-    return launch_dependent(kernel, dim3(units, (unsigned)p.splits), kWarps8 * 32, smem, stream, p);
+    const dim3 grid(units, (unsigned)(p.splits * p.cluster));
+    if (p.cluster == 1) return launch_dependent(kernel, grid, kWarps8 * 32, smem, stream, p);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(kWarps8 * 32);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 1;
+    attr[0].val.clusterDim.y = (unsigned)p.cluster;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = dependent_launches() ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 
 template <int D>

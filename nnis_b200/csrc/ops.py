@@ -69,7 +69,7 @@ def _stream() -> ctypes.c_void_p:
 _ENTRY_FIELDS = {"nnis_copy_pages": "ppiiiiiipiip", "nnis_verify_drafts": "ppppppppiiippp",
                  "nnis_attention_shared": "pippppipiiippppppiiiiiifiipp",
                  "nnis_rope_store_int8": "pppppppppppiiiiiiiiiip", "nnis_read_pages_int8": "ppppppppiiiiiiiiip",
-                 "nnis_attention_int8": "ppppppppppppiiiiiiiiiifiiiip", "nnis_quantize_rows": "pppiiiip",
+                 "nnis_attention_int8": "ppppppppppppiiiiiiiiiifiiiiiip", "nnis_quantize_rows": "pppiiiip",
                  "nnis_linear_int8": "ppppppppiiiiiiiip"}
 _entries = {}
 
@@ -3132,18 +3132,24 @@ def attention_int8_splits(n: int, heads: int, keys: int, device) -> int:
 
 @functools.lru_cache(maxsize=4096)
 def attention_int8_plan(n: int, seqs: int, heads: int, kv_heads: int, d: int, cols: int, window: int, sms: int):
-    """(slices, runs of 32 positions in a slice, rows taken together) of the tensor cores' kernel: rows of a sequence lie together, as
-    many as come on each, up to 64 queries a key/value head; slices cover the table, at most 64, as short as fills the device."""
-    per = heads // kv_heads
+    """(slices, pieces of a slice, rows taken together, CTAs of a slice's cluster) of the tensor cores' kernel; a piece is 64 positions,
+    32 for heads of 96 and 128.  Rows of a sequence lie together, as many as come on each, up to 64 queries a key/value head."""
+    per, half = heads // kv_heads, 1 if d <= 64 else 2
     rows = max(1, min(-(-n // max(1, seqs)), 64 // per))
     units = -(-n // rows) * kv_heads * -(-rows * per // 16)
-    seen = min(2 * cols, (window + rows + 30) // 32 + 1) if window else 2 * cols
-    resident = sms * (4 if d <= 64 else 2)
-    pieces = max(INT8_LEAST_PIECES, -(-seen * units // resident), -(-2 * cols // 64))
-    return -(-2 * cols // pieces), pieces, rows
-
-
-INT8_LEAST_PIECES = 8
+    length = 64 // half
+    seen = min(half * cols, (window + rows + length - 2) // length + 1) if window else half * cols
+    # CTAs a unit (a run of rows, a key/value head, a tile of queries): as many as the device holds at once where that is one to three, half
+    # of that beyond, since a cluster's and a join's meeting cost what two pieces do.  us with 1, 2, 4, 8, 16 CTAs a unit: 192 units of 64
+    # pieces 30.5, 25.1, 30.7; 160 of 8 to 16 pieces 10.2, 10.1, 14.1; 256 of 32 pieces 21.6, 26.3; 48 of 32 pieces (float32) 14.5, 10.6,
+    # 9.4, 10.7; 24 of 64 pieces 23.4, 15.2, 10.1, 8.8, 12.8; 3 of 256 pieces 82, 45, 25, 15.2, 11.6, and with 64 8.7.
+    held = sms * (4 if d <= 32 else 3 if d <= 64 else 2) // units
+    ctas = min(held if held < 4 else held // 2, -(-seen // 2) if seen <= 8 else -(-seen // 4))
+    ctas = 1 << max(0, ctas.bit_length() - 1)
+    cluster = min(8, ctas)
+    slices = min(64, ctas // cluster)
+    pieces = -(-half * cols // slices)
+    return -(-half * cols // pieces), pieces, rows, cluster
 
 
 def attention_int8(q: torch.Tensor, q_stride: int, k: torch.Tensor, v: torch.Tensor, k_scales: torch.Tensor, v_scales: torch.Tensor,
@@ -3186,10 +3192,10 @@ def attention_int8(q: torch.Tensor, q_stride: int, k: torch.Tensor, v: torch.Ten
         with torch.cuda.device(index):
             return attention_int8(q, q_stride, k, v, k_scales, v_scales, token_pos, token_seq, page_table, out, heads, kv_heads, d,
                                   window, scale, workspace)
-    tickets = status = slice_pieces = rows = 0
+    tickets = status = slice_pieces = rows = cluster = 0
     at = k.data_ptr(), v.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), out.data_ptr()
     if page_size == 64 and d in (32, 64, 96, 128) and not (at[0] | at[1] | at[2] | at[3] | at[4]) % 16:
-        splits, slice_pieces, rows = attention_int8_plan(n, seqs, heads, kv_heads, d, cols, window, _sm_count.get(index) or sm_count(k.device))
+        splits, slice_pieces, rows, cluster = attention_int8_plan(n, seqs, heads, kv_heads, d, cols, window, _sm_count.get(index) or sm_count(k.device))
         partial = workspace.room("attn_int8_records", n * heads * splits * (d + 4), torch.float32).data_ptr() if splits > 1 else 0
         tickets = workspace.zeros_room("attn_int8_tickets", n * kv_heads * -(-rows * (heads // kv_heads) // 8), torch.int32).data_ptr() \
             if splits > 1 else 0
@@ -3200,7 +3206,7 @@ def attention_int8(q: torch.Tensor, q_stride: int, k: torch.Tensor, v: torch.Ten
         partial = workspace.room("attn_int8_partial", n * heads * splits * (d + 2), torch.float32).data_ptr() if splits > 1 else 0
     _check(_entry("nnis_attention_int8")(
         q.data_ptr(), at[0], at[1], at[2], at[3], token_pos.data_ptr(), token_seq.data_ptr(), page_table.data_ptr(), at[4], partial,
-        tickets, status, q_stride, seqs, cols, pages, n, heads, kv_heads, d, page_size, window, scale, splits, slice_pieces, rows, _DTYPE_CODE[dtype], _stream_of(index)),
+        tickets, status, q_stride, seqs, cols, pages, n, heads, kv_heads, d, page_size, window, scale, splits, slice_pieces, rows, cluster, _DTYPE_CODE[dtype], 0, _stream_of(index)),
         "attention_int8", 2 if splits > 1 and not slice_pieces else 1)
 
 
