@@ -18,22 +18,62 @@ struct Quantize8 {
     int rows, k, kp;
 };
 
-// A CTA a row.
-template <typename T, bool QUADS>
+// WARPS warps a row, its values in registers between the two looks at them: CHUNKS runs of eight a lane.
+template <typename T, int WARPS, int CHUNKS>
 __global__ void __launch_bounds__(128) quantize_rows_kernel(const __grid_constant__ Quantize8 p) {
+    __shared__ uint32_t tops[4];
+    pdl_wait();
+    pdl_launch_dependents();
+    constexpr int kLanes = WARPS * 32;
+    const int row = blockIdx.x * (4 / WARPS) + threadIdx.x / kLanes, lane = threadIdx.x % kLanes;
+    const T* x = reinterpret_cast<const T*>(p.x) + (size_t)row * p.x_stride;
+    float v[CHUNKS][8];
+    uint32_t top = 0;
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) {
+        const int i = (c * kLanes + lane) * 8;
+        if (row < p.rows && i < p.k) {
+            const float4 a = load4(x + i), b = load4(x + i + 4);
+            v[c][0] = a.x; v[c][1] = a.y; v[c][2] = a.z; v[c][3] = a.w;
+            v[c][4] = b.x; v[c][5] = b.y; v[c][6] = b.z; v[c][7] = b.w;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[c][e] = 0.f;
+        }
+    }
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = max(top, magnitude_bits(v[c][e]));
+    top = group_max<32>(top);
+    if (WARPS > 1) {
+        if (threadIdx.x % 32 == 0) tops[threadIdx.x / 32] = top;
+        __syncthreads();
+        top = max(max(tops[0], tops[1]), max(tops[2], tops[3]));
+    }
+    if (row >= p.rows) return;
+    const RowScale r = row_scale(top);
+    const uint32_t good = good_row(r.scale);
+    int8_t* codes = p.codes + (size_t)row * p.kp;
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) {
+        const int i = (c * kLanes + lane) * 8;
+        if (i >= p.kp) continue;
+        *reinterpret_cast<uint2*>(codes + i) = make_uint2(code_word(v[c][0], v[c][1], v[c][2], v[c][3], r.inverse, good),
+                                                          code_word(v[c][4], v[c][5], v[c][6], v[c][7], r.inverse, good));
+    }
+    if (lane == 0) p.scales[row] = r.scale;
+}
+
+// Any row: a CTA each, read twice.
+template <typename T>
+__global__ void __launch_bounds__(128) quantize_rows_any_kernel(const __grid_constant__ Quantize8 p) {
     __shared__ uint32_t tops[4];
     pdl_wait();
     pdl_launch_dependents();
     const T* x = reinterpret_cast<const T*>(p.x) + (size_t)blockIdx.x * p.x_stride;
     uint32_t top = 0;
-    if (QUADS) {
-        for (int i = threadIdx.x * 4; i < p.k; i += 512) {
-            const float4 v = load4(x + i);
-            top = max(top, max(max(magnitude_bits(v.x), magnitude_bits(v.y)), max(magnitude_bits(v.z), magnitude_bits(v.w))));
-        }
-    } else {
-        for (int i = threadIdx.x; i < p.k; i += 128) top = max(top, magnitude_bits(to_float(x[i])));
-    }
+    for (int i = threadIdx.x; i < p.k; i += 128) top = max(top, magnitude_bits(to_float(x[i])));
     top = group_max<32>(top);
     if (threadIdx.x % 32 == 0) tops[threadIdx.x / 32] = top;
     __syncthreads();
@@ -42,19 +82,9 @@ __global__ void __launch_bounds__(128) quantize_rows_kernel(const __grid_constan
     int8_t* codes = p.codes + (size_t)blockIdx.x * p.kp;
     for (int i = threadIdx.x * 4; i < p.kp; i += 512) {
         int c[4] = {0, 0, 0, 0};
-        if (QUADS) {
-            if (i < p.k) {
-                const float4 v = load4(x + i);
-                c[0] = row_code(v.x, r.inverse);
-                c[1] = row_code(v.y, r.inverse);
-                c[2] = row_code(v.z, r.inverse);
-                c[3] = row_code(v.w, r.inverse);
-            }
-        } else {
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (i + j < p.k) c[j] = row_code(to_float(x[i + j]), r.inverse);
-        }
+        for (int j = 0; j < 4; ++j)
+            if (i + j < p.k) c[j] = row_code(to_float(x[i + j]), r.inverse);
         *reinterpret_cast<uint32_t*>(codes + i) = pack_codes(c[0], c[1], c[2], c[3]);
     }
     if (threadIdx.x == 0) p.scales[blockIdx.x] = r.scale;
@@ -62,8 +92,15 @@ __global__ void __launch_bounds__(128) quantize_rows_kernel(const __grid_constan
 
 template <typename T>
 static cudaError_t launch_quantize(const Quantize8& p, cudaStream_t stream) {
-    const bool quads = p.k % 4 == 0 && p.x_stride % 4 == 0 && (uintptr_t)p.x % (4 * sizeof(T)) == 0;
-    return launch_dependent(quads ? quantize_rows_kernel<T, true> : quantize_rows_kernel<T, false>, (unsigned)p.rows, 128, 0, stream, p);
+    const bool eights = p.k % 8 == 0 && p.x_stride % 8 == 0 && (uintptr_t)p.x % (4 * sizeof(T)) == 0;
+    if (!eights || p.kp > 8192) return launch_dependent(quantize_rows_any_kernel<T>, (unsigned)p.rows, 128, 0, stream, p);
+    // (a warp a row up to 1,024 values, and up to 2,048 where rows are many)
+    if (p.kp <= 1024 || (p.kp <= 2048 && p.rows >= 1024)) {
+        auto kernel = p.kp <= 512 ? quantize_rows_kernel<T, 1, 2> : p.kp <= 1024 ? quantize_rows_kernel<T, 1, 4> : quantize_rows_kernel<T, 1, 8>;
+        return launch_dependent(kernel, (unsigned)((p.rows + 3) / 4), 128, 0, stream, p);
+    }
+    auto kernel = p.kp <= 2048 ? quantize_rows_kernel<T, 4, 2> : p.kp <= 4096 ? quantize_rows_kernel<T, 4, 4> : quantize_rows_kernel<T, 4, 8>;
+    return launch_dependent(kernel, (unsigned)p.rows, 128, 0, stream, p);
 }
 
 }  // namespace nnis

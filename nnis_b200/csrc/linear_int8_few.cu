@@ -11,7 +11,6 @@
 
 namespace nnis {
 
-constexpr int kFewWarps = 8;
 
 __device__ __forceinline__ uint4 load_w(const int8_t* p) {
     uint4 v;
@@ -24,28 +23,26 @@ __device__ __forceinline__ void few_mma(int (&c)[4], uint32_t a0, uint32_t a1, u
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// NT: tiles of 8 rows of x.
-template <typename T, bool ADD, bool GATED, int NT>
+// NT: tiles of 8 rows of x; kFewWarps: 8, or 16 where there are fewer CTAs than SMs and a long K.
+template <typename T, bool ADD, bool GATED, int NT, int kFewWarps>
 __global__ void __launch_bounds__(kFewWarps * 32) linear_int8_few_kernel(const __grid_constant__ Linear8 p) {
-    constexpr int NB = GATED ? 2 : 1, kAhead = GATED ? 2 : 4;  // runs of K that a lane asks for at once
+    constexpr int NB = GATED ? 2 : 1, kAhead = GATED ? 2 : 4;  // runs of K that a lane has asked for
     constexpr int kSums = NB * 16 * NT * 8;
     __shared__ int sums[kFewWarps][kSums];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int n0 = blockIdx.x * 16, runs = (p.kp + 63) / 64;
     const uint4 none = {0u, 0u, 0u, 0u};
     uint4 w[kAhead][NB][2];
-    auto load = [&](int first) {
+    auto load = [&](int i, int run) {
+        const int k = run * 64 + 16 * t;
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-            const int k = (first + i * kFewWarps) * 64 + 16 * t;
+        for (int b = 0; b < NB; ++b)
 #pragma unroll
-            for (int b = 0; b < NB; ++b)
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-                    w[i][b][h] = k < p.kp && n0 + g + 8 * h < p.n ? load_w(p.w + ((size_t)b * p.n + n0 + g + 8 * h) * p.kp + k) : none;
-        }
+            for (int h = 0; h < 2; ++h)
+                w[i][b][h] = k < p.kp && n0 + g + 8 * h < p.n ? load_w(p.w + ((size_t)b * p.n + n0 + g + 8 * h) * p.kp + k) : none;
     };
-    load(warp);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) load(i, warp + i * kFewWarps);
     pdl_wait();
     pdl_launch_dependents();
     int acc[NB][NT][4] = {};
@@ -63,8 +60,8 @@ __global__ void __launch_bounds__(kFewWarps * 32) linear_int8_few_kernel(const _
                     few_mma(acc[b][c], w[i][b][0].z, w[i][b][1].z, w[i][b][0].w, w[i][b][1].w, x.z, x.w);
                 }
             }
+            load(i, first + (i + kAhead) * kFewWarps);
         }
-        if (first + kAhead * kFewWarps < runs) load(first + kAhead * kFewWarps);
     }
     // sums[token][row of W]: a lane's are rows g and g + 8, tokens 2 t and 2 t + 1 of each tile
 #pragma unroll
@@ -96,9 +93,14 @@ __global__ void __launch_bounds__(kFewWarps * 32) linear_int8_few_kernel(const _
 
 template <typename T, bool ADD, bool GATED>
 static cudaError_t launch_few(const Linear8& p, cudaStream_t stream) {
-    auto kernel = p.m <= 8 ? linear_int8_few_kernel<T, ADD, GATED, 1> : p.m <= 16 ? linear_int8_few_kernel<T, ADD, GATED, 2>
-                  : linear_int8_few_kernel<T, ADD, GATED, 4>;
-    return launch_dependent(kernel, (unsigned)((p.n + 15) / 16), kFewWarps * 32, 0, stream, p);
+    const unsigned ctas = (unsigned)((p.n + 15) / 16);
+    if (!GATED && ctas <= 148 && p.kp >= 2048 && p.m <= 16) {
+        auto kernel = p.m <= 8 ? linear_int8_few_kernel<T, ADD, GATED, 1, 16> : linear_int8_few_kernel<T, ADD, GATED, 2, 16>;
+        return launch_dependent(kernel, ctas, 512, 0, stream, p);
+    }
+    auto kernel = p.m <= 8 ? linear_int8_few_kernel<T, ADD, GATED, 1, 8> : p.m <= 16 ? linear_int8_few_kernel<T, ADD, GATED, 2, 8>
+                  : linear_int8_few_kernel<T, ADD, GATED, 4, 8>;
+    return launch_dependent(kernel, ctas, 256, 0, stream, p);
 }
 
 cudaError_t linear_int8_few(const Linear8& p, int mode, bool f32, cudaStream_t stream) {
