@@ -128,7 +128,7 @@ struct Attend8Call {
     int* status;
     int q_stride, table_rows, table_cols, pages, n, nq, nkv, d, page_size, window;
     float scale;
-    int splits, slice_pieces, rows_at_once, cluster, dtype, unused;
+    int splits, slice_pieces, rows_at_once, cluster, dtype, padding;
     cudaStream_t stream;
 };
 NNIS_API int nnis_attention_int8(const void* call) {
@@ -136,8 +136,8 @@ NNIS_API int nnis_attention_int8(const void* call) {
     Attend8Call c;
     memcpy(&c, call, sizeof c);
     const auto [q, k, v, k_scales, v_scales, token_pos, token_seq, page_table, out, partial, tickets, status, q_stride, table_rows, table_cols, pages, n,
-                nq, nkv, d, page_size, window, scale, splits, slice_pieces, rows_at_once, cluster, dtype, unused, stream] = c;
-    (void)unused;
+                nq, nkv, d, page_size, window, scale, splits, slice_pieces, rows_at_once, cluster, dtype, padding, stream] = c;
+    (void)padding;
     if (n <= 0 || nq <= 0 || nkv <= 0 || nq % nkv || table_rows <= 0 || table_cols <= 0 || pages <= 0 || page_size <= 0 || window < 0 ||
         splits < 1 || (splits > 1 && !partial) || !q || !k || !v || !k_scales || !v_scales || !out)
         return NNIS_ERR_ARGUMENT;

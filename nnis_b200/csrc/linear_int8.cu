@@ -135,15 +135,15 @@ struct Linear8Call {
     void *out, *codes;
     float* scales;
     int* status;
-    int x_stride, m, n, k, mode, dtype, sms, unused;
+    int x_stride, m, n, k, mode, dtype, sms, padding;
     cudaStream_t stream;
 };
 NNIS_API int nnis_linear_int8(const void* call) {
     using namespace nnis;
     Linear8Call c;
     memcpy(&c, call, sizeof c);
-    const auto [x, w, ws, bias, out, codes, scales, status, x_stride, m, n, k, mode, dtype, sms, unused, stream] = c;
-    (void)unused;
+    const auto [x, w, ws, bias, out, codes, scales, status, x_stride, m, n, k, mode, dtype, sms, padding, stream] = c;
+    (void)padding;
     const int kp = (k + 15) / 16 * 16;
     if (!x || !w || !ws || !out || !codes || !scales || m <= 0 || n <= 0 || k <= 0 || x_stride < k || mode < 0 || mode > 3)
         return NNIS_ERR_ARGUMENT;
@@ -153,6 +153,9 @@ NNIS_API int nnis_linear_int8(const void* call) {
     const cudaError_t e = dtype == NNIS_DTYPE_F32 ? launch_quantize<float>(q, stream) : launch_quantize<bf16>(q, stream);
     if (e != cudaSuccess) return (int)e;
     const Linear8 p{(const int8_t*)codes, (const int8_t*)w, scales, ws, bias, out, m, n, kp, status, 0};
-    if (m <= 32) return (int)linear_int8_few(p, mode, dtype == NNIS_DTYPE_F32, stream);
+    // us by few rows' kernel / by tcgen05: 16 rows 16,384 x 2,048 13.2 / 13.7, 2,048 x 8,192 8.8 / 11; 32 rows 960 x 576 4.5 / 5.9,
+    // 2,048 x 2,048 6.1 / 6.4, 6,144 x 2,048 9.1 / 8.2, 2,048 x 8,192 14.4 / 11.1, 16,384 x 2,048 18.0 / 13.5
+    const long long bytes = (long long)(mode == INT8_GATED ? 2 : 1) * n * kp;
+    if (m <= 16 || (m <= 32 && bytes < 8 << 20)) return (int)linear_int8_few(p, mode, dtype == NNIS_DTYPE_F32, stream);
     return linear_int8_tc(p, mode, dtype == NNIS_DTYPE_F32, sms > 0 ? sms : 148, stream);
 }

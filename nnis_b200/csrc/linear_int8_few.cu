@@ -1,5 +1,5 @@
-// Products of 8-bit codes with few rows (decode steps), bound by the bytes of W: a CTA's eight warps share 16 rows of W (gated: 16 gate
-// and the 16 up rows), each takes every eighth run of 64 places of K straight into registers, and multiplies them (mma.sync, signed
+// Products of 8-bit codes with few rows (decode steps), bound by the bytes of W: a CTA's eight warps share 16 rows of W (gated: 8 gate
+// and the 8 up rows), each takes every eighth run of 64 places of K straight into registers, and multiplies them (mma.sync, signed
 // bytes, W as the 16-row operand) with up to 64 rows of x; the eight sums, whole numbers, are added in shared memory.
 //
 // Any order of K serves a sum: a lane holds 16 bytes of a row that lie side by side, so that a warp's load of 8 rows takes whole
@@ -26,26 +26,25 @@ __device__ __forceinline__ void few_mma(int (&c)[4], uint32_t a0, uint32_t a1, u
 // NT: tiles of 8 rows of x; kFewWarps: 8, or 16 where there are fewer CTAs than SMs and a long K.
 template <typename T, bool ADD, bool GATED, int NT, int kFewWarps>
 __global__ void __launch_bounds__(kFewWarps * 32) linear_int8_few_kernel(const __grid_constant__ Linear8 p) {
-    constexpr int NB = GATED ? 2 : 1, kAhead = GATED ? 2 : 4;  // runs of K that a lane has asked for
-    constexpr int kSums = NB * 16 * NT * 8;
-    __shared__ int sums[kFewWarps][kSums];
+    constexpr int kAhead = 4, kOut = GATED ? 8 : 16;  // runs of K that a lane has asked for; outputs of a CTA and row of x
+    __shared__ int sums[kFewWarps][NT * 128];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int n0 = blockIdx.x * 16, runs = (p.kp + 63) / 64;
+    const int n0 = blockIdx.x * kOut, runs = (p.kp + 63) / 64;
     const uint4 none = {0u, 0u, 0u, 0u};
-    uint4 w[kAhead][NB][2];
+    // row g of the operand's 16, and row g + 8: of a gated product the same output's gate and up
+    const int8_t* rows[2] = {p.w + (size_t)(n0 + g) * p.kp, p.w + ((size_t)n0 + g + (GATED ? p.n : 8)) * p.kp};
+    const bool in[2] = {n0 + g < p.n, n0 + g + (GATED ? 0 : 8) < p.n};
+    uint4 w[kAhead][2];
     auto load = [&](int i, int run) {
         const int k = run * 64 + 16 * t;
 #pragma unroll
-        for (int b = 0; b < NB; ++b)
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-                w[i][b][h] = k < p.kp && n0 + g + 8 * h < p.n ? load_w(p.w + ((size_t)b * p.n + n0 + g + 8 * h) * p.kp + k) : none;
+        for (int h = 0; h < 2; ++h) w[i][h] = k < p.kp && in[h] ? load_w(rows[h] + k) : none;
     };
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) load(i, warp + i * kFewWarps);
     pdl_wait();
     pdl_launch_dependents();
-    int acc[NB][NT][4] = {};
+    int acc[NT][4] = {};
     for (int first = warp; first < runs; first += kAhead * kFewWarps) {
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
@@ -54,47 +53,38 @@ __global__ void __launch_bounds__(kFewWarps * 32) linear_int8_few_kernel(const _
             for (int c = 0; c < NT; ++c) {
                 const int m = 8 * c + g;
                 const uint4 x = k < p.kp && m < p.m ? *reinterpret_cast<const uint4*>(p.x + (size_t)m * p.kp + k) : none;
-#pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    few_mma(acc[b][c], w[i][b][0].x, w[i][b][1].x, w[i][b][0].y, w[i][b][1].y, x.x, x.y);
-                    few_mma(acc[b][c], w[i][b][0].z, w[i][b][1].z, w[i][b][0].w, w[i][b][1].w, x.z, x.w);
-                }
+                few_mma(acc[c], w[i][0].x, w[i][1].x, w[i][0].y, w[i][1].y, x.x, x.y);
+                few_mma(acc[c], w[i][0].z, w[i][1].z, w[i][0].w, w[i][1].w, x.z, x.w);
             }
             load(i, first + (i + kAhead) * kFewWarps);
         }
     }
     // sums[token][row of W]: a lane's are rows g and g + 8, tokens 2 t and 2 t + 1 of each tile
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
+    for (int c = 0; c < NT; ++c)
 #pragma unroll
-        for (int c = 0; c < NT; ++c)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                sums[warp][((b * NT + c) * 8 + 2 * t + (i & 1)) * 16 + g + 8 * (i >> 1)] = acc[b][c][i];
+        for (int i = 0; i < 4; ++i) sums[warp][(c * 8 + 2 * t + (i & 1)) * 16 + g + 8 * (i >> 1)] = acc[c][i];
     __syncthreads();
-    for (int at = threadIdx.x; at < NT * 128; at += kFewWarps * 32) {
-        const int m = at >> 4, n = n0 + (at & 15);
+    auto value = [&](int m, int row_in, size_t row) {
+        int sum = 0;
+#pragma unroll
+        for (int v = 0; v < kFewWarps; ++v) sum += sums[v][m * 16 + row_in];
+        return (float)sum * p.xs[m] * p.ws[row] + (p.bias ? p.bias[row] : 0.f);
+    };
+    for (int at = threadIdx.x; at < NT * 8 * kOut; at += kFewWarps * 32) {
+        const int m = at / kOut, c = at % kOut, n = n0 + c;
         if (m >= p.m || n >= p.n) continue;
-        const float xs = p.xs[m];
-        float y[NB];
-#pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            int sum = 0;
-#pragma unroll
-            for (int v = 0; v < kFewWarps; ++v) sum += sums[v][b * NT * 128 + at];
-            const size_t row = (size_t)b * p.n + n;
-            y[b] = (float)sum * xs * p.ws[row] + (p.bias ? p.bias[row] : 0.f);
-        }
-        const float value = GATED ? silu_gate(y[0], y[NB - 1]) : y[0];
+        float y = value(m, c, (size_t)n);
+        if (GATED) y = silu_gate(y, value(m, 8 + c, (size_t)p.n + n));
         T* out = reinterpret_cast<T*>(p.out) + (size_t)m * p.n + n;
-        *out = from_float<T>(ADD ? to_float(*out) + value : value);
+        *out = from_float<T>(ADD ? to_float(*out) + y : y);
     }
 }
 
 template <typename T, bool ADD, bool GATED>
 static cudaError_t launch_few(const Linear8& p, cudaStream_t stream) {
-    const unsigned ctas = (unsigned)((p.n + 15) / 16);
-    if (!GATED && ctas <= 148 && p.kp >= 2048 && p.m <= 16) {
+    const unsigned ctas = (unsigned)((p.n + (GATED ? 7 : 15)) / (GATED ? 8 : 16));
+    if (ctas <= 148 && p.kp >= 2048 && p.m <= 16) {
         auto kernel = p.m <= 8 ? linear_int8_few_kernel<T, ADD, GATED, 1, 16> : linear_int8_few_kernel<T, ADD, GATED, 2, 16>;
         return launch_dependent(kernel, ctas, 512, 0, stream, p);
     }

@@ -6,6 +6,8 @@
 // 128 bytes out by TMA.  A byte is a place of K, so a stage of as many bytes carries twice the products of bfloat16's at twice the rate:
 // the same bytes a cycle are asked of L2, 64 for each SM of a pair of CTAs that share a tile of 256 x 256 (gated: 128 gate and the 128
 // up columns), 128 for a CTA of its own with a tile of 128 x 128 (gated: 64 and 64), which is for products of fewer tiles.
+// Where tiles are fewer than half of the SMs (some hundred rows at most), a cluster of up to eight CTAs shares a tile's K; their sums,
+// whole numbers, are added through the cluster's shared memory (64 rows through 1.7B's down projection, 16 tiles: 26.2 -> 11.5 us).
 // Every wait is bounded; a wait that runs out sets the status word, and all warps still meet at the end and free tensor memory.
 #include "linear_int8.cuh"
 #include "tcgen05_helpers.cuh"
@@ -13,10 +15,20 @@
 namespace nnis {
 
 constexpr int kRows8 = 128, kSlice8 = 128, kThreads8 = 320, kEpilogueWarps8 = 8;
+constexpr int kSumsRow8 = 132;  // of a tile's sums in shared memory: a row of 128 and a gap that keeps rows off one another's banks
 constexpr uint32_t kTileBytes8 = kRows8 * kSlice8;  // x's tile, and W's: 128 rows in either form
 
-// T: the output's type; ADD: into float32.  BN: columns of a tile's products, gate and up together.
-template <typename T, bool ADD, bool GATED, bool PAIR, int STAGES>
+// The addresses of the cluster's CTAs' copies of a place in shared memory, and four sums there
+__device__ __forceinline__ int4 peer_sums(const int* p, int rank) {
+    uint32_t at;
+    int4 v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_addr(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+    return v;
+}
+
+// T: the output's type; ADD: into float32; SPLIT: gridDim.z CTAs of a cluster share a tile's K.  BN: columns of a tile's products, gate and up together.
+template <typename T, bool ADD, bool GATED, bool PAIR, int STAGES, bool SPLIT = false>
 __global__ void __launch_bounds__(kThreads8, STAGES <= 3 ? 2 : 1)
 linear_int8_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
                       const __grid_constant__ CUtensorMap map_out, const __grid_constant__ Linear8 p) {
@@ -33,7 +45,8 @@ linear_int8_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = PAIR ? cluster_rank() : 0;
     const int m0 = blockIdx.x * kRows8, n0 = blockIdx.y * kOutCols;
-    const int slices = (p.kp + kSlice8 - 1) / kSlice8;
+    const int all_slices = (p.kp + kSlice8 - 1) / kSlice8, per_cta = SPLIT ? (all_slices + (int)gridDim.z - 1) / (int)gridDim.z : all_slices;
+    const int first_slice = SPLIT ? (int)blockIdx.z * per_cta : 0, slices = SPLIT ? min(per_cta, all_slices - first_slice) : all_slices;
     if (threadIdx.x == 32) {
         prefetch_tensormap(&map_x);
         prefetch_tensormap(&map_w);
@@ -59,8 +72,8 @@ linear_int8_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
     const uint32_t tmem = tmem_s;
 
     // Each CTA of a pair loads its 128 rows of x and half of the tile's rows of W; the bytes of both count on the first one's barrier.
-    auto load = [&](bool of_x, int slice) {
-        const int s = slice % STAGES;
+    auto load = [&](bool of_x, int i) {
+        const int s = i % STAGES, slice = first_slice + i;
         unsigned char* to = base + (size_t)s * 2 * kTileBytes8 + (of_x ? 0 : kTileBytes8);
         const int w_row = n0 + (int)rank * kLoadRows;
         if constexpr (PAIR) {
@@ -150,7 +163,19 @@ linear_int8_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
             const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
             unsigned char* boxes = base + (size_t)(warp - 2) * (kSlots * 4096);
             // (a tile's rows beyond the last: nothing to send)
-            const bool sends = m0 + quarter * 32 < p.m;
+            const bool sends = !SPLIT && m0 + quarter * 32 < p.m;
+            if constexpr (SPLIT) {  // this CTA's sums to its own shared memory
+                int* mine = reinterpret_cast<int*>(base) + (size_t)row * kSumsRow8;
+#pragma unroll 1
+                for (int c0 = group * 32; c0 < BN; c0 += 64) {
+                    uint32_t v[32];
+                    tmem_load32(lanes + (uint32_t)c0, v);
+                    if (m < p.m)
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            *reinterpret_cast<int4*>(mine + c0 + 4 * j) = make_int4((int)v[4 * j], (int)v[4 * j + 1], (int)v[4 * j + 2], (int)v[4 * j + 3]);
+                }
+            }
 #pragma unroll 1
             for (int b = group, i = 0; b < kOutCols / kBoxCols && n0 + b * kBoxCols < p.n && sends; b += 2, ++i) {
                 unsigned char* box = boxes + (i % kSlots) * 4096;
@@ -221,9 +246,38 @@ linear_int8_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
             if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
         }
     }
+    if constexpr (SPLIT) {
+        cluster_meet();  // every CTA's sums are there (whether or not a wait ran out: the status word says so)
+        constexpr int kQuads = kOutCols / 4;
+        const int rows = min(kRows8, p.m - m0), parts = (int)gridDim.z;
+        for (int at = (int)blockIdx.z * kThreads8 + threadIdx.x; at < rows * kQuads; at += parts * kThreads8) {
+            const int r = at / kQuads, c = at % kQuads * 4;
+            if (n0 + c >= p.n) continue;
+            const int* from = reinterpret_cast<const int*>(base) + (size_t)r * kSumsRow8 + c;
+            int4 v = {0, 0, 0, 0}, u = {0, 0, 0, 0};
+            for (int z = 0; z < parts; ++z) {
+                const int4 a = peer_sums(from, z);
+                v = make_int4(v.x + a.x, v.y + a.y, v.z + a.z, v.w + a.w);
+                if (GATED) {
+                    const int4 b = peer_sums(from + kLoadRows, z);
+                    u = make_int4(u.x + b.x, u.y + b.y, u.z + b.z, u.w + b.w);
+                }
+            }
+            const float xs = p.xs[m0 + r];
+            const int vs[4] = {v.x, v.y, v.z, v.w}, us[4] = {u.x, u.y, u.z, u.w};
+            T* out = reinterpret_cast<T*>(p.out) + (size_t)(m0 + r) * p.n + n0 + c;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (n0 + c + j >= p.n) break;
+                float y = (float)vs[j] * xs * scales[c + j] + biases[c + j];
+                if (GATED) y = silu_gate(y, (float)us[j] * xs * scales[kLoadRows + c + j] + biases[kLoadRows + c + j]);
+                out[j] = from_float<T>(ADD ? to_float(out[j]) + y : y);
+            }
+        }
+    }
     tc_fence_before();
     __syncthreads();
-    if constexpr (PAIR) cluster_meet();
+    if constexpr (PAIR || SPLIT) cluster_meet();
     if (warp == 1) {
         tc_fence_after();
         if constexpr (PAIR) pair_tmem_dealloc(tmem, kTmemCols);
@@ -233,28 +287,30 @@ linear_int8_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
     if (threadIdx.x == 0 && abort_flag && p.status) atomicExch(p.status, 3);
 }
 
-template <typename T, bool ADD, bool GATED, bool PAIR, int STAGES>
-static cudaError_t launch_tc8(const CUtensorMap& mx, const CUtensorMap& mw, const CUtensorMap& mo, const Linear8& p, cudaStream_t stream) {
+template <typename T, bool ADD, bool GATED, bool PAIR, int STAGES, bool SPLIT = false>
+static cudaError_t launch_tc8(const CUtensorMap& mx, const CUtensorMap& mw, const CUtensorMap& mo, const Linear8& p, cudaStream_t stream,
+                              int parts = 1) {
     constexpr size_t smem = (size_t)STAGES * 2 * kTileBytes8 + 1024;
     static_assert(STAGES * 2 * kTileBytes8 >= kEpilogueWarps8 * 2 * 4096, "the epilogue's boxes fit the ring");
-    auto kernel = linear_int8_tc_kernel<T, ADD, GATED, PAIR, STAGES>;
+    static_assert(!SPLIT || STAGES * 2 * kTileBytes8 >= kRows8 * kSumsRow8 * 4, "a tile's sums fit the ring");
+    auto kernel = linear_int8_tc_kernel<T, ADD, GATED, PAIR, STAGES, SPLIT>;
     static std::atomic<int> held[16];
     cudaError_t e = allow_shared(kernel, smem, held);
     if (e != cudaSuccess) return e;
     constexpr int kOutCols = (PAIR ? 256 : 128) / (GATED ? 2 : 1);
     const unsigned tiles = (unsigned)((p.m + kRows8 - 1) / kRows8);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(PAIR ? (tiles + 1) / 2 * 2 : tiles, (unsigned)((p.n + kOutCols - 1) / kOutCols));
+    cfg.gridDim = dim3(PAIR ? (tiles + 1) / 2 * 2 : tiles, (unsigned)((p.n + kOutCols - 1) / kOutCols), (unsigned)parts);
     cfg.blockDim = dim3(kThreads8);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     int attrs = 0;
-    if (PAIR) {
+    if (PAIR || SPLIT) {
         attr[attrs].id = cudaLaunchAttributeClusterDimension;
-        attr[attrs].val.clusterDim.x = 2;
+        attr[attrs].val.clusterDim.x = PAIR ? 2 : 1;
         attr[attrs].val.clusterDim.y = 1;
-        attr[attrs++].val.clusterDim.z = 1;
+        attr[attrs++].val.clusterDim.z = (unsigned)parts;
     }
     if (dependent_launches()) {
         attr[attrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -268,7 +324,8 @@ static cudaError_t launch_tc8(const CUtensorMap& mx, const CUtensorMap& mw, cons
 // Three stages let two CTAs share an SM, so that one's epilogue runs under the other's products; six where there are no more CTAs than SMs.
 template <typename T, bool ADD, bool GATED>
 static cudaError_t launch_tc8_of(const CUtensorMap& mx, const CUtensorMap& mw, const CUtensorMap& mo, const Linear8& p, bool pair, bool alone,
-                                 cudaStream_t stream) {
+                                 int parts, cudaStream_t stream) {
+    if (parts > 1) return launch_tc8<T, ADD, GATED, false, 6, true>(mx, mw, mo, p, stream, parts);
     if (pair) return alone ? launch_tc8<T, ADD, GATED, true, 6>(mx, mw, mo, p, stream) : launch_tc8<T, ADD, GATED, true, 3>(mx, mw, mo, p, stream);
     return alone ? launch_tc8<T, ADD, GATED, false, 6>(mx, mw, mo, p, stream) : launch_tc8<T, ADD, GATED, false, 3>(mx, mw, mo, p, stream);
 }
@@ -286,12 +343,23 @@ int linear_int8_tc(Linear8 p, int mode, bool f32, int sms, cudaStream_t stream) 
     p.out_by_tma = (uintptr_t)p.out % 16 == 0 && (long long)p.n * bytes % 16 == 0 && make_map(&mo, p.out, p.m, p.n, 32, 0, bytes);
     if (!p.out_by_tma) mo = mx;
     const bool alone = (pair ? pairs : singles) <= sms;
+    // CTAs that share a tile's K, two runs of 128 places each at least, none of them empty: clusters have to find their SMs side by side,
+    // and where they would fill the device some wait for a second turn.  us with 2, 3, 4, 8: 16 tiles (64 x 2,048 x 2,048) 8.8, 7.8, 6.8,
+    // 11.0; x 8,192 17.3, 13.7, 11.5, 15.9; 8 tiles (64 x 960 x 2,560) 9.4, 8.1, 7.3, 6.8; 32 tiles (256 x 2,048 x 8,192) 20.7, 17.3,
+    // 15.3; 48 tiles (64 x 6,144 x 2,048) 8.9, 14.1.
+    const int slices = (p.kp + kSlice8 - 1) / kSlice8;
+    int parts = pair ? 1 : 16 * singles <= sms ? 8 : 32 * singles <= 7 * sms ? 4 : 16 * singles <= 7 * sms ? 2 : 1;
+    if (parts > slices / 2) parts = slices / 2;
+    if (parts > 1) {
+        const int each = (slices + parts - 1) / parts;
+        parts = (slices + each - 1) / each;
+    }
     if (gated)
-        return (int)(f32 ? launch_tc8_of<float, false, true>(mx, mw, mo, p, pair, alone, stream)
-                         : launch_tc8_of<bf16, false, true>(mx, mw, mo, p, pair, alone, stream));
-    if (mode == INT8_ADD_F32) return (int)launch_tc8_of<float, true, false>(mx, mw, mo, p, pair, alone, stream);
-    return (int)(wide ? launch_tc8_of<float, false, false>(mx, mw, mo, p, pair, alone, stream)
-                      : launch_tc8_of<bf16, false, false>(mx, mw, mo, p, pair, alone, stream));
+        return (int)(f32 ? launch_tc8_of<float, false, true>(mx, mw, mo, p, pair, alone, parts, stream)
+                         : launch_tc8_of<bf16, false, true>(mx, mw, mo, p, pair, alone, parts, stream));
+    if (mode == INT8_ADD_F32) return (int)launch_tc8_of<float, true, false>(mx, mw, mo, p, pair, alone, parts, stream);
+    return (int)(wide ? launch_tc8_of<float, false, false>(mx, mw, mo, p, pair, alone, parts, stream)
+                      : launch_tc8_of<bf16, false, false>(mx, mw, mo, p, pair, alone, parts, stream));
 }
 
 }  // namespace nnis
