@@ -22,15 +22,16 @@ struct Attend8 {
     float scale;
     int splits;      // most slices of a row
     // the tensor cores' kernel
-    int slice_pieces, rows_at_once, tiles, aligned, cluster;  // cluster: CTAs that share a slice, at most 8
+    int slice_pieces, rows_at_once, tiles, aligned, cluster;  // cluster: CTAs that share a slice, at most 8; 0: a warp a unit
+    int tile_eights, units;  // a tile's queries / 8
     unsigned* tickets;  // n * nkv * tiles, zero between launches
     int* status;
 };
 
 // Positions that a warp takes at a time (what each time costs beside its positions is a third of 32 positions of 64 values), and how
-// many such pieces it has on their way or in use: three CTAs an SM with heads of 64, two with 96 and 128.
+// many such pieces it has on their way or in use: three CTAs an SM, four with heads of 32.
 __host__ __device__ constexpr int piece8(int d) { return d <= 64 ? 64 : 32; }
-__host__ __device__ constexpr int stages8(int d) { return d <= 64 ? 2 : 3; }
+__host__ __device__ constexpr int stages8(int d) { return d <= 96 ? 2 : 3; }
 
 __device__ __forceinline__ void fence_async_shared8() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 

@@ -147,8 +147,9 @@ __device__ __forceinline__ float query_codes(const float (&x)[D / 4], uint32_t (
     return none ? __uint_as_float(0x7fc00000u) : zero ? 0.f : __fdiv_rn(__uint_as_float(top), kMost);
 }
 
-template <int D, bool F32, int MT>
-__global__ void __launch_bounds__(kWarps8 * 32, D <= 32 ? 4 : D <= 64 ? 3 : 2) attn_int8_mma_kernel(const __grid_constant__ Attend8 p) {
+// SOLO: a warp a unit, its whole range of keys, for many rows with few keys.
+template <int D, bool F32, int MT, bool SOLO>
+__global__ void __launch_bounds__(kWarps8 * 32, D <= 32 ? 4 : D <= 96 ? 3 : 2) attn_int8_mma_kernel(const __grid_constant__ Attend8 p) {
     using T = std::conditional_t<F32, float, bf16>;
     constexpr int kStage = stage_bytes8(D), kTile = 8 * MT, kSteps = D / 32, kWords = D / 16, kValueWords = D / 32, kCols = D / 8;
     constexpr int kOuts = F32 ? MT : (MT + 1) / 2;  // products of the weights per step of 16 positions
@@ -166,7 +167,8 @@ __global__ void __launch_bounds__(kWarps8 * 32, D <= 32 ? 4 : D <= 64 ? 3 : 2) a
     pdl_launch_dependents();
 
     const int per = p.nq / p.nkv, slice = blockIdx.y / p.cluster, rank = blockIdx.y % p.cluster;
-    int unit = blockIdx.x;
+    int unit = SOLO ? blockIdx.x * kWarps8 + warp : blockIdx.x;
+    if (SOLO && unit >= p.units) return;  // (whole warps: nothing below meets in this form)
     const int tile = unit % p.tiles;
     unit /= p.tiles;
     const int hk = unit % p.nkv, row_first = unit / p.nkv * p.rows_at_once, row_end = min(p.n, row_first + p.rows_at_once);
@@ -220,12 +222,13 @@ __global__ void __launch_bounds__(kWarps8 * 32, D <= 32 ? 4 : D <= 64 ? 3 : 2) a
         const int piece_low = known ? low / kPiece8 : 0, piece_top = known ? (int)min((long long)top_pos / kPiece8 + 1, (long long)kHalves * p.table_cols) : 0;
         // a slice's pieces are dealt out to all warps of its cluster
         const int slices = max(1, (piece_top - piece_low + p.slice_pieces - 1) / p.slice_pieces);
-        if (slice >= slices) continue;
-        const int first = piece_low + slice * p.slice_pieces, last = min(piece_top, first + p.slice_pieces), step = kWarps8 * p.cluster;
+        if (!SOLO && slice >= slices) continue;
+        const int first = SOLO ? piece_low : piece_low + slice * p.slice_pieces, last = SOLO ? piece_top : min(piece_top, first + p.slice_pieces);
+        const int step = SOLO ? 1 : kWarps8 * p.cluster;
 
         // ---- copies: this warp's pieces are every step-th; those of pages outside the store are passed over.  The next
         // piece's page is asked for as a piece is copied, and looked at when its turn comes.
-        int next = first + rank * kWarps8 + warp, page = next < last ? table[(unsigned)next / kHalves] : -1;
+        int next = SOLO ? first : first + rank * kWarps8 + warp, page = next < last ? table[(unsigned)next / kHalves] : -1;
         auto copy = [&](int to) {  // the piece that is copied to this stage, -1 where none is left
             while (next < last && (unsigned)page >= (unsigned)p.pages) {
                 next += step;
@@ -454,6 +457,33 @@ __global__ void __launch_bounds__(kWarps8 * 32, D <= 32 ? 4 : D <= 64 ? 3 : 2) a
             }
         }
 
+        if constexpr (SOLO) {
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                const bool sees = pos_of[i] >= 0;
+                l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+                l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+                const float inv = sees && l[i] != 0.f ? unit_t * (1.f / 32768.f) / l[i] : 0.f;
+                const int e = e0 + 8 * i + g;
+                if (e >= entries) continue;
+                T* row = reinterpret_cast<T*>(p.out) + ((size_t)(r0 + e / per) * p.nq + hk * per + e % per) * D + t * (D / 4);
+#pragma unroll
+                for (int half = 0; half < 2; ++half)
+#pragma unroll
+                    for (int c = 0; c < kCols; c += 4) {
+                        float y[4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            if constexpr (F32) y[j] = o[i][c + j][half] + o[i][c + j][2 + half];
+                            else y[j] = o[i / 2][c + j][2 * (i & 1) + half];
+                            y[j] = sees ? y[j] * inv : 0.f;
+                        }
+                        store4(row + half * (D / 8) + c, make_float4(y[0], y[1], y[2], y[3]));
+                    }
+            }
+            __syncwarp();
+            continue;
+        }
         // ---- the four warps' parts are joined: [queries][D] sums, then maxima and sums of weights, in the warp's own ring
         float* sums = reinterpret_cast<float*>(ring);
         float* stats = sums + kTile * D;
@@ -595,16 +625,16 @@ __global__ void __launch_bounds__(kWarps8 * 32, D <= 32 ? 4 : D <= 64 ? 3 : 2) a
     }
 }
 
-template <int D, bool F32, int MT>
+template <int D, bool F32, int MT, bool SOLO>
 static cudaError_t launch_mma8(const Attend8& p, unsigned units, cudaStream_t stream) {
     constexpr size_t smem = (size_t)kWarps8 * stages8(D) * stage_bytes8(D);
     static_assert(stages8(D) * stage_bytes8(D) >= 2 * 8 * MT * (D + 2) * 4, "a warp's part of the outputs fits its ring, twice in the first");
-    auto kernel = attn_int8_mma_kernel<D, F32, MT>;
+    auto kernel = attn_int8_mma_kernel<D, F32, MT, SOLO>;
     static std::atomic<int> held[16];
     const cudaError_t e = allow_shared(kernel, smem, held);
     if (e != cudaSuccess) return e;
-    const dim3 grid(units, (unsigned)(p.splits * p.cluster));
-    if (p.cluster == 1) return launch_dependent(kernel, grid, kWarps8 * 32, smem, stream, p);
+    const dim3 grid(SOLO ? (units + kWarps8 - 1) / kWarps8 : units, SOLO ? 1u : (unsigned)(p.splits * p.cluster));
+    if (SOLO || p.cluster == 1) return launch_dependent(kernel, grid, kWarps8 * 32, smem, stream, p);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(kWarps8 * 32);
@@ -624,15 +654,19 @@ static cudaError_t launch_mma8(const Attend8& p, unsigned units, cudaStream_t st
 
 template <int D>
 static cudaError_t launch_mma8_of(const Attend8& p, bool f32, int mt, unsigned units, cudaStream_t stream) {
-    if (f32) return launch_mma8<D, true, 1>(p, units, stream);
-    return mt == 1 ? launch_mma8<D, false, 1>(p, units, stream) : launch_mma8<D, false, 2>(p, units, stream);
+    if (p.cluster == 0)
+        return f32 ? launch_mma8<D, true, 1, true>(p, units, stream) : mt == 1 ? launch_mma8<D, false, 1, true>(p, units, stream)
+                                                                            : launch_mma8<D, false, 2, true>(p, units, stream);
+    return f32 ? launch_mma8<D, true, 1, false>(p, units, stream) : mt == 1 ? launch_mma8<D, false, 1, false>(p, units, stream)
+                                                                         : launch_mma8<D, false, 2, false>(p, units, stream);
 }
 
 cudaError_t attend_int8_mma(Attend8 p, bool f32, cudaStream_t stream) {
-    const int per = p.nq / p.nkv, entries = p.rows_at_once * per, mt = f32 || entries <= 8 ? 1 : 2;
+    const int per = p.nq / p.nkv, entries = p.rows_at_once * per, mt = f32 ? 1 : p.tile_eights;
     p.tiles = (entries + 8 * mt - 1) / (8 * mt);
     const long long units = (long long)((p.n + p.rows_at_once - 1) / p.rows_at_once) * p.nkv * p.tiles;
     if (units > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
+    p.units = (int)units;
     switch (p.d) {
         case 32: return launch_mma8_of<32>(p, f32, mt, (unsigned)units, stream);
         case 64: return launch_mma8_of<64>(p, f32, mt, (unsigned)units, stream);

@@ -3132,24 +3132,39 @@ def attention_int8_splits(n: int, heads: int, keys: int, device) -> int:
 
 @functools.lru_cache(maxsize=4096)
 def attention_int8_plan(n: int, seqs: int, heads: int, kv_heads: int, d: int, cols: int, window: int, sms: int):
-    """(slices, pieces of a slice, rows taken together, CTAs of a slice's cluster) of the tensor cores' kernel; a piece is 64 positions,
+    """(slices, pieces of a slice, rows taken together, CTAs of a slice's cluster or 0 for a warp a unit, eights of queries in a
+    tile) of the tensor cores' kernel; a piece is 64 positions,
     32 for heads of 96 and 128.  Rows of a sequence lie together, as many as come on each, up to 64 queries a key/value head."""
     per, half = heads // kv_heads, 1 if d <= 64 else 2
     rows = max(1, min(-(-n // max(1, seqs)), 64 // per))
-    units = -(-n // rows) * kv_heads * -(-rows * per // 16)
     length = 64 // half
     seen = min(half * cols, (window + rows + length - 2) // length + 1) if window else half * cols
-    # CTAs a unit (a run of rows, a key/value head, a tile of queries): as many as the device holds at once where that is one to three, half
-    # of that beyond, since a cluster's and a join's meeting cost what two pieces do.  us with 1, 2, 4, 8, 16 CTAs a unit: 192 units of 64
-    # pieces 30.5, 25.1, 30.7; 160 of 8 to 16 pieces 10.2, 10.1, 14.1; 256 of 32 pieces 21.6, 26.3; 48 of 32 pieces (float32) 14.5, 10.6,
-    # 9.4, 10.7; 24 of 64 pieces 23.4, 15.2, 10.1, 8.8, 12.8; 3 of 256 pieces 82, 45, 25, 15.2, 11.6, and with 64 8.7.
-    held = sms * (4 if d <= 32 else 3 if d <= 64 else 2) // units
-    ctas = min(held if held < 4 else held // 2, -(-seen // 2) if seen <= 8 else -(-seen // 4))
-    ctas = 1 << max(0, ctas.bit_length() - 1)
+    resident = sms * (4 if d <= 32 else 3 if d <= 96 else 2)
+    # tiles of 8 queries, of 16 where those of 8 would take the device more than one turn.  us in tiles of 8 / 16: five rows of four heads of
+    # 128, 16 sequences of 4,000 (384 or 256 units of 296 at once) 101 / 65; 20 heads of 64, 64 sequences of 4,096 (192 units) 23 / 29;
+    # two rows of eight heads of 128, 2 sequences of 706 7.2 / 10.0
+    runs = -(-n // rows) * kv_heads
+    eights = 2 if rows * per > 8 and runs * -(-rows * per // 8) > resident else 1
+    units = runs * -(-rows * per // (8 * eights))
+    # A warp a unit where units are many and short: us by four warps / one: 1,760 units of one piece 18.6 / 6.4, 2,048 of two 25.4 / 14.8,
+    # of eight 39.8 / 37.4, of 16 58.6 / 66.1; 512 (heads of 128) of ten 20.5 / 16.5, of 32 36.7 / 39.7.
+    if units >= resident and seen <= INT8_ALONE_PIECES:
+        return 1, half * cols, rows, 0, eights
+    # CTAs a unit (a run of rows, a key/value head, a tile of queries): up to half of what the device holds at once, since a cluster's and a
+    # join's meeting cost what two pieces do; all of it where that is two, or where eight pieces are left to each.  us with 1, 2, 4, 8,
+    # 16 CTAs a unit: 192 units of 64 pieces 30.5, 25.1, 30.7; 160 of 8 to 16 pieces 10.2, 10.1, 14.1; 256 of 32 pieces 21.6, 26.3; 48 of
+    # 32 pieces (float32) 14.5, 10.6, 9.4, 10.7; 48 of 64 pieces 25.0, 16.4, 12.8, 11.8; 24 of 64 pieces 23.4, 15.2, 10.1, 8.8, 12.8; 3 of
+    # 256 pieces 82, 45, 25, 15.2, 11.6, and with 64 8.7.
+    held, most, ctas = resident // units, -(-seen // 2) if seen <= 8 else -(-seen // 3), 1
+    while 2 * ctas <= min(held, most) and (ctas == 1 or 4 * ctas <= held or seen >= 16 * ctas):
+        ctas *= 2
     cluster = min(8, ctas)
     slices = min(64, ctas // cluster)
     pieces = -(-half * cols // slices)
-    return -(-half * cols // pieces), pieces, rows, cluster
+    return -(-half * cols // pieces), pieces, rows, cluster, eights
+
+
+INT8_ALONE_PIECES = 10
 
 
 def attention_int8(q: torch.Tensor, q_stride: int, k: torch.Tensor, v: torch.Tensor, k_scales: torch.Tensor, v_scales: torch.Tensor,
@@ -3192,10 +3207,10 @@ def attention_int8(q: torch.Tensor, q_stride: int, k: torch.Tensor, v: torch.Ten
         with torch.cuda.device(index):
             return attention_int8(q, q_stride, k, v, k_scales, v_scales, token_pos, token_seq, page_table, out, heads, kv_heads, d,
                                   window, scale, workspace)
-    tickets = status = slice_pieces = rows = cluster = 0
+    tickets = status = slice_pieces = rows = cluster = eights = 0
     at = k.data_ptr(), v.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), out.data_ptr()
     if page_size == 64 and d in (32, 64, 96, 128) and not (at[0] | at[1] | at[2] | at[3] | at[4]) % 16:
-        splits, slice_pieces, rows, cluster = attention_int8_plan(n, seqs, heads, kv_heads, d, cols, window, _sm_count.get(index) or sm_count(k.device))
+        splits, slice_pieces, rows, cluster, eights = attention_int8_plan(n, seqs, heads, kv_heads, d, cols, window, _sm_count.get(index) or sm_count(k.device))
         partial = workspace.room("attn_int8_records", n * heads * splits * (d + 4), torch.float32).data_ptr() if splits > 1 else 0
         tickets = workspace.zeros_room("attn_int8_tickets", n * kv_heads * -(-rows * (heads // kv_heads) // 8), torch.int32).data_ptr() \
             if splits > 1 else 0
@@ -3206,7 +3221,7 @@ def attention_int8(q: torch.Tensor, q_stride: int, k: torch.Tensor, v: torch.Ten
         partial = workspace.room("attn_int8_partial", n * heads * splits * (d + 2), torch.float32).data_ptr() if splits > 1 else 0
     _check(_entry("nnis_attention_int8")(
         q.data_ptr(), at[0], at[1], at[2], at[3], token_pos.data_ptr(), token_seq.data_ptr(), page_table.data_ptr(), at[4], partial,
-        tickets, status, q_stride, seqs, cols, pages, n, heads, kv_heads, d, page_size, window, scale, splits, slice_pieces, rows, cluster, _DTYPE_CODE[dtype], 0, _stream_of(index)),
+        tickets, status, q_stride, seqs, cols, pages, n, heads, kv_heads, d, page_size, window, scale, splits, slice_pieces, rows, cluster, eights, _DTYPE_CODE[dtype], _stream_of(index)),
         "attention_int8", 2 if splits > 1 and not slice_pieces else 1)
 
 
