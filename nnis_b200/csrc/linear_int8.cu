@@ -126,8 +126,8 @@ NNIS_API int nnis_quantize_rows(const void* call) {
     return NNIS_ERR_UNSUPPORTED;
 }
 
-// x [m, k] (rows `x_stride` apart) is put into `codes` [m, kp] and `scales` [m], w [n (gated: 2 n), kp] codes, ws their scales, bias
-// float32 like ws or null, out [m, n]: `dtype` (x's) in the modes 0 (store) and 3 (gated: silu(first half of w's rows) * the
+// x [m, k] (rows `x_stride` apart) is put into `codes` [m, kp] and `scales` [m] (or, one row or two, into shared memory), w [n (gated: 2
+// n), kp] codes, ws their scales, bias float32 like ws or null, out [m, n]: `dtype` (x's) in the modes 0 (store) and 3 (gated: silu(first half of w's rows) * the
 // second), float32 in 1 (store) and 2 (add).
 struct Linear8Call {
     const void *x, *w;
@@ -149,13 +149,16 @@ NNIS_API int nnis_linear_int8(const void* call) {
         return NNIS_ERR_ARGUMENT;
     if (k > 133136 || (dtype != NNIS_DTYPE_F32 && dtype != NNIS_DTYPE_BF16)) return NNIS_ERR_UNSUPPORTED;
     if (((uintptr_t)codes | (uintptr_t)w) % 16) return NNIS_ERR_ALIGNMENT;
+    const bool f32 = dtype == NNIS_DTYPE_F32;
+    const Linear8 p{(const int8_t*)codes, (const int8_t*)w, scales, ws, bias, out, m, n, kp, status, 0, x, x_stride, k};
+    const int held = sms > 0 ? sms : 148;
+    if (linear_int8_fuses(p, mode == INT8_GATED, f32, held)) return (int)linear_int8_few(p, mode, f32, true, stream);
     const Quantize8 q{x, x_stride, (int8_t*)codes, scales, m, k, kp};
-    const cudaError_t e = dtype == NNIS_DTYPE_F32 ? launch_quantize<float>(q, stream) : launch_quantize<bf16>(q, stream);
+    const cudaError_t e = f32 ? launch_quantize<float>(q, stream) : launch_quantize<bf16>(q, stream);
     if (e != cudaSuccess) return (int)e;
-    const Linear8 p{(const int8_t*)codes, (const int8_t*)w, scales, ws, bias, out, m, n, kp, status, 0};
     // us by few rows' kernel / by tcgen05: 16 rows 16,384 x 2,048 13.2 / 13.7, 2,048 x 8,192 8.8 / 11; 32 rows 960 x 576 4.5 / 5.9,
     // 2,048 x 2,048 6.1 / 6.4, 6,144 x 2,048 9.1 / 8.2, 2,048 x 8,192 14.4 / 11.1, 16,384 x 2,048 18.0 / 13.5
     const long long bytes = (long long)(mode == INT8_GATED ? 2 : 1) * n * kp;
-    if (m <= 16 || (m <= 32 && bytes < 8 << 20)) return (int)linear_int8_few(p, mode, dtype == NNIS_DTYPE_F32, stream);
-    return linear_int8_tc(p, mode, dtype == NNIS_DTYPE_F32, sms > 0 ? sms : 148, stream);
+    if (m <= 16 || (m <= 32 && bytes < 8 << 20)) return (int)linear_int8_few(p, mode, f32, false, stream);
+    return linear_int8_tc(p, mode, f32, held, stream);
 }

@@ -14,6 +14,8 @@ struct Linear8 {
     int m, n, kp;  // n: columns of the output; a gated product's w has 2 n rows, gate before up
     int* status;
     int out_by_tma;
+    const void* values;  // x before it is put into codes, rows `x_stride` apart, k values each
+    int x_stride, k;
 };
 
 // silu(gate) * up with the two approximate instructions (2^x and 1 / x, relative error about 1e-7 each)
@@ -24,8 +26,10 @@ __device__ __forceinline__ float silu_gate(float gate, float up) {
     return gate * r * up;
 }
 
-// `x` put into codes; the product of few rows; of many (tcgen05).  `f32`: the operands' type is float32.
-cudaError_t linear_int8_few(const Linear8& p, int mode, bool f32, cudaStream_t stream);
+// The product of few rows (`fused`: rows that are still values), whether they are few enough for that; of many (tcgen05).  `f32`: the
+// operands' type is float32.
+bool linear_int8_fuses(const Linear8& p, bool gated, bool f32, int sms);
+cudaError_t linear_int8_few(const Linear8& p, int mode, bool f32, bool fused, cudaStream_t stream);
 int linear_int8_tc(Linear8 p, int mode, bool f32, int sms, cudaStream_t stream);
 
 }  // namespace nnis
