@@ -321,3 +321,105 @@ def test_a_step_is_written_read_back_and_attended_over(dtype):
                                dtype == torch.float32)
     # (the values read back are rounded to float32: half a step of each)
     assert ((out.cpu().double() - want.reshape(1, -1)).abs() <= 1.01 * bound + 1e-6).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv_heads,d", [(6, 3, 64), (6, 3, 128), (3, 3, 96), (8, 4, 32)])
+def test_many_short_rows(dtype, heads, kv_heads, d):
+    """Two hundred sequences of one to three hundred positions, a key/value head of each the work of one warp; padding rows and holes."""
+    gen = torch.Generator().manual_seed(16)
+    lengths = (1 + torch.randint(0, 300, (200,), generator=gen)).tolist()
+    table, pages = place(lengths, gen)
+    table[7][0] = -1
+    table[9] = [-1] * len(table[9])
+    positions = [-1 if i % 50 == 3 else n - 1 for i, n in enumerate(lengths)]
+    check(dtype, heads, kv_heads, d, positions, list(range(200)), table, pages, seed=7)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv_heads,d,tokens,context,window", [(20, 1, 64, 3, 700, 0), (20, 1, 128, 3, 300, 0), (20, 1, 64, 5, 200, 90)])
+def test_many_rows_of_many_queries(dtype, heads, kv_heads, d, tokens, context, window):
+    """Sixty sequences' drafted tokens with twenty queries a key/value head: tiles of sixteen queries, the last of a run partly empty."""
+    gen = torch.Generator().manual_seed(17)
+    lengths = [context - 7 * (i % 9) for i in range(60)]
+    table, pages = place(lengths, gen)
+    positions = [n - tokens + j for n in lengths for j in range(tokens)]
+    check(dtype, heads, kv_heads, d, positions, [i for i in range(60) for _ in range(tokens)], table, pages, window=window, seed=8)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [64, 96, 40])
+def test_queries_and_stores_at_any_address(dtype, d):
+    """Rows of queries an odd number of values apart; codes that begin at no multiple of sixteen bytes."""
+    from nnis_b200.csrc import ops
+    from nnis_b200.engine.workspace import Workspace
+    gen = torch.Generator().manual_seed(18)
+    table, pages = place([130, 70], gen)
+    check(dtype, 4, 2, d, [129, 69, 3], [0, 1, 1], table, pages, seed=9, stride=4 * d + 1)
+    k, ks = plain.store(pages, 2, d, gen)
+    v, vs = plain.store(pages, 2, d, gen)
+    moved = []
+    for t in (k, v):
+        flat = torch.empty(t.numel() + 4, dtype=torch.int8, device="cuda")[4:].view(t.shape)
+        flat.copy_(t)
+        moved.append(flat)
+    q = torch.randn((3, 4 * d), generator=gen).to(dtype)
+    want, bound = plain.attention(q, k, v, ks, vs, [129, 69, 3], [0, 1, 1], table, 4, 2, 0, d ** -0.5, dtype == torch.float32)
+    out = torch.empty_like(q, device="cuda")
+    i32 = [torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([129, 69, 3], [0, 1, 1], table)]
+    ops.attention_int8(q.cuda(), 4 * d, *moved, *cuda(ks, vs), *i32, out, 4, 2, d, 0, d ** -0.5, Workspace(torch.device("cuda")))
+    assert ((out.cpu().double() - want).abs() <= bound).all()
+    with pytest.raises(ops.KernelError, match="misaligned"):
+        ops.rope_store_int8(torch.zeros((3, 8 * d), dtype=dtype, device="cuda"), q.cuda(), *i32, None, None, *moved, *cuda(ks, vs), 4, 2, d, PAGE)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_other_page_sizes(dtype):
+    """Pages of 16 positions take the kernel of any size."""
+    from nnis_b200.csrc import ops
+    from nnis_b200.engine.workspace import Workspace
+    gen = torch.Generator().manual_seed(19)
+    d, page = 64, 16
+    x = torch.randn((5, 2, page, d), generator=gen)
+    k, ks = plain.codes_of(x)
+    v, vs = plain.codes_of(torch.randn((5, 2, page, d), generator=gen))
+    q = torch.randn((2, 4 * d), generator=gen).to(dtype)
+    table, positions = [[3, 1, 4], [0, 2, -1]], [40, 17]
+    out = torch.empty_like(q, device="cuda")
+    ops.attention_int8(q.cuda(), 4 * d, *cuda(k, v, ks, vs, torch.tensor(positions, dtype=torch.int32), torch.tensor([0, 1], dtype=torch.int32),
+                                              torch.tensor(table, dtype=torch.int32)), out, 4, 2, d, 0, 0.125, Workspace(torch.device("cuda")))
+    for r, (pages, pos) in enumerate(zip(table, positions)):
+        keys, values = ((c[pages].double() * s[pages].double()[..., None]).transpose(0, 1).reshape(2, -1, d)[:, :pos + 1]
+                        for c, s in ((k, ks), (v, vs)))
+        h = q[r].double().view(2, 2, d)
+        want = torch.softmax(torch.einsum("hgd,hnd->hgn", h, keys) * 0.125, -1) @ values
+        # (scores of at most some ten, weights and sums of float32, the output rounded once)
+        tolerance = 1e-5 * values.abs().amax() + torch.finfo(dtype).eps / 2 * want.abs()
+        assert ((out[r].cpu().double().view(2, 2, d) - want).abs() <= tolerance).all()
+
+
+def test_tickets_and_records_serve_calls_of_all_sizes():
+    """One workspace, calls that cut their keys into slices and calls that do not, in turn: each call's answer is its own, and repeats to
+    the last bit."""
+    from nnis_b200.csrc import ops
+    from nnis_b200.engine.workspace import Workspace
+    ws, gen, kept = Workspace(torch.device("cuda")), torch.Generator().manual_seed(20), []
+    for lengths, heads, kv_heads in (([5000], 9, 3), ([300] * 40, 6, 2), ([4000, 100], 4, 1), ([16000], 3, 1), ([64], 9, 3)):
+        table, pages = place(lengths, gen)
+        k, ks = plain.store(pages, kv_heads, 64, gen)
+        v, vs = plain.store(pages, kv_heads, 64, gen)
+        q = torch.randn((len(lengths), heads * 64), generator=gen).to(torch.bfloat16)
+        args = cuda(k, v, ks, vs, torch.tensor([n - 1 for n in lengths], dtype=torch.int32), torch.arange(len(lengths), dtype=torch.int32),
+                    torch.tensor(table, dtype=torch.int32))
+        kept.append((q.cuda(), args, heads, kv_heads))
+
+    def run(q, args, heads, kv_heads, space):
+        out = torch.empty_like(q)
+        ops.attention_int8(q, heads * 64, *args, out, heads, kv_heads, 64, 0, 0.125, space)
+        return out
+
+    alone = [run(*c, Workspace(torch.device("cuda"))) for c in kept]
+    for _ in range(3):
+        for c, want in zip(kept, alone):
+            assert torch.equal(run(*c, ws), want)
+    ops.check_status("cuda:0")

@@ -194,3 +194,18 @@ def test_flags_of_the_command_line():
             parse_args([*base, flag, "float32"])
     with pytest.raises((ProcessContractError, ValueError)):
         execute("m", prompt_ids=[1], cache_dtype="fp8")
+
+
+@pytest.mark.parametrize("d", [32, 64, 96, 128])
+def test_plans_of_attention_cover_every_key(d):
+    """Slices cover the table, clusters and tiles are what the kernel takes, and records fit a call's buffer."""
+    from nnis_b200.csrc import ops
+    for n, seqs in ((1, 1), (7, 7), (64, 64), (80, 16), (300, 300), (5, 400), (3000, 7)):
+        for heads, kv_heads in ((9, 3), (32, 32), (20, 1), (64, 1), (16, 2)):
+            for cols in (1, 2, 3, 63, 64, 500, 4096):
+                for window in (0, 1, 64, 5000):
+                    slices, pieces, rows, cluster, eights = ops.attention_int8_plan(n, seqs, heads, kv_heads, d, cols, window, 148)
+                    per_page = 1 if d <= 64 else 2
+                    assert 1 <= slices <= 64 and slices * pieces >= per_page * cols and (slices - 1) * pieces < per_page * cols
+                    assert cluster in (0, 1, 2, 4, 8) and (cluster > 0 or slices == 1) and eights in (1, 2)
+                    assert 1 <= rows <= max(1, 64 // (heads // kv_heads)) and slices * cluster <= 65535
