@@ -90,6 +90,65 @@ __global__ void __launch_bounds__(128) quantize_rows_any_kernel(const __grid_con
     if (threadIdx.x == 0) p.scales[blockIdx.x] = r.scale;
 }
 
+// A norm's rows put into codes: y = x / sqrt(mean(x^2) + eps) * w, rounded to T as the norm by itself would be, its codes and scale.  A CTA a
+// row, the row and the weights in registers.
+template <typename T, int Q>
+__global__ void __launch_bounds__(256)
+rmsnorm_int8_kernel(const float* __restrict__ x, const float* __restrict__ w, int8_t* __restrict__ codes, float* __restrict__ scales,
+                    int width, int kp, float eps) {
+    __shared__ float partial[8];
+    __shared__ uint32_t tops[8];
+    const int tid = threadIdx.x, n4 = width >> 2;
+    float4 g[Q], v[Q];
+#pragma unroll
+    for (int j = 0; j < Q; ++j) g[j] = tid + 256 * j < n4 ? load4(w + 4 * (tid + 256 * j)) : make_float4(0.f, 0.f, 0.f, 0.f);
+    pdl_wait();  // (the weights depend on no kernel)
+    pdl_launch_dependents();
+    const float* in = x + (size_t)blockIdx.x * width;
+    float ss = 0.f;
+#pragma unroll
+    for (int j = 0; j < Q; ++j) {
+        v[j] = tid + 256 * j < n4 ? load4(in + 4 * (tid + 256 * j)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        ss = fmaf(v[j].x, v[j].x, fmaf(v[j].y, v[j].y, fmaf(v[j].z, v[j].z, fmaf(v[j].w, v[j].w, ss))));
+    }
+    ss = warp_sum(ss);
+    if ((tid & 31) == 0) partial[tid >> 5] = ss;
+    __syncthreads();
+    float total = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) total += partial[k];
+    const float s = 1.0f / sqrtf(total * (1.0f / (float)width) + eps);
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < Q; ++j) {
+        v[j] = make_float4(to_float(from_float<T>((v[j].x * s) * g[j].x)), to_float(from_float<T>((v[j].y * s) * g[j].y)),
+                           to_float(from_float<T>((v[j].z * s) * g[j].z)), to_float(from_float<T>((v[j].w * s) * g[j].w)));
+        top = max(top, max(max(magnitude_bits(v[j].x), magnitude_bits(v[j].y)), max(magnitude_bits(v[j].z), magnitude_bits(v[j].w))));
+    }
+    top = group_max<32>(top);
+    if ((tid & 31) == 0) tops[tid >> 5] = top;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 8; ++k) top = max(top, tops[k]);
+    const RowScale r = row_scale(top);
+    const uint32_t good = good_row(r.scale);
+    int8_t* out = codes + (size_t)blockIdx.x * kp;
+#pragma unroll
+    for (int j = 0; j < Q; ++j) {
+        const int i = 4 * (tid + 256 * j);
+        if (i < kp) *reinterpret_cast<uint32_t*>(out + i) = i < width ? code_word(v[j].x, v[j].y, v[j].z, v[j].w, r.inverse, good) : 0u;
+    }
+    if (tid == 0) scales[blockIdx.x] = r.scale;
+}
+
+template <typename T>
+static cudaError_t launch_rmsnorm8(const float* x, const float* w, int8_t* codes, float* scales, int rows, int width, int kp, float eps,
+                                   cudaStream_t stream) {
+    auto kernel = kp <= 1024 ? rmsnorm_int8_kernel<T, 1> : kp <= 2048 ? rmsnorm_int8_kernel<T, 2> : kp <= 4096 ? rmsnorm_int8_kernel<T, 4>
+                  : rmsnorm_int8_kernel<T, 8>;
+    return launch_dependent(kernel, (unsigned)rows, 256, 0, stream, x, w, codes, scales, width, kp, eps);
+}
+
 template <typename T>
 static cudaError_t launch_quantize(const Quantize8& p, cudaStream_t stream) {
     const bool eights = p.k % 8 == 0 && p.x_stride % 8 == 0 && (uintptr_t)p.x % (4 * sizeof(T)) == 0;
@@ -126,35 +185,58 @@ NNIS_API int nnis_quantize_rows(const void* call) {
     return NNIS_ERR_UNSUPPORTED;
 }
 
+// Rows x [rows, width] float32 through an RMS norm with `weight`, rounded to `dtype`, as codes [rows, kp] and scales [rows].
+struct Rmsnorm8Call {
+    const float *x, *weight;
+    void* codes;
+    float* scales;
+    int rows, width, dtype;
+    float eps;
+    cudaStream_t stream;
+};
+NNIS_API int nnis_rmsnorm_int8(const void* call) {
+    using namespace nnis;
+    Rmsnorm8Call c;
+    memcpy(&c, call, sizeof c);
+    const auto [x, weight, codes, scales, rows, width, dtype, eps, stream] = c;
+    if (!x || !weight || !codes || !scales || rows <= 0 || width <= 0 || !(eps > 0.f)) return NNIS_ERR_ARGUMENT;
+    if (width % 4 || width > 8192) return NNIS_ERR_UNSUPPORTED;
+    if (((uintptr_t)x | (uintptr_t)weight | (uintptr_t)codes) % 16) return NNIS_ERR_ALIGNMENT;
+    const int kp = (width + 15) / 16 * 16;
+    if (dtype == NNIS_DTYPE_F32) return (int)launch_rmsnorm8<float>(x, weight, (int8_t*)codes, scales, rows, width, kp, eps, stream);
+    if (dtype == NNIS_DTYPE_BF16) return (int)launch_rmsnorm8<bf16>(x, weight, (int8_t*)codes, scales, rows, width, kp, eps, stream);
+    return NNIS_ERR_UNSUPPORTED;
+}
+
 // x [m, k] (rows `x_stride` apart) is put into `codes` [m, kp] and `scales` [m] (or, one row or two, into shared memory), w [n (gated: 2
 // n), kp] codes, ws their scales, bias float32 like ws or null, out [m, n]: `dtype` (x's) in the modes 0 (store) and 3 (gated: silu(first half of w's rows) * the
-// second), float32 in 1 (store) and 2 (add).
+// second), float32 in 1 (store) and 2 (add).  `coded`:
+// `codes` and `scales` are there already.
 struct Linear8Call {
     const void *x, *w;
     const float *ws, *bias;
     void *out, *codes;
     float* scales;
     int* status;
-    int x_stride, m, n, k, mode, dtype, sms, padding;
+    int x_stride, m, n, k, mode, dtype, sms, coded;
     cudaStream_t stream;
 };
 NNIS_API int nnis_linear_int8(const void* call) {
     using namespace nnis;
     Linear8Call c;
     memcpy(&c, call, sizeof c);
-    const auto [x, w, ws, bias, out, codes, scales, status, x_stride, m, n, k, mode, dtype, sms, padding, stream] = c;
-    (void)padding;
+    const auto [x, w, ws, bias, out, codes, scales, status, x_stride, m, n, k, mode, dtype, sms, coded, stream] = c;
     const int kp = (k + 15) / 16 * 16;
-    if (!x || !w || !ws || !out || !codes || !scales || m <= 0 || n <= 0 || k <= 0 || x_stride < k || mode < 0 || mode > 3)
+    if ((!x && !coded) || !w || !ws || !out || !codes || !scales || m <= 0 || n <= 0 || k <= 0 || (!coded && x_stride < k) || mode < 0 || mode > 3)
         return NNIS_ERR_ARGUMENT;
     if (k > 133136 || (dtype != NNIS_DTYPE_F32 && dtype != NNIS_DTYPE_BF16)) return NNIS_ERR_UNSUPPORTED;
     if (((uintptr_t)codes | (uintptr_t)w) % 16) return NNIS_ERR_ALIGNMENT;
     const bool f32 = dtype == NNIS_DTYPE_F32;
     const Linear8 p{(const int8_t*)codes, (const int8_t*)w, scales, ws, bias, out, m, n, kp, status, 0, x, x_stride, k};
     const int held = sms > 0 ? sms : 148;
-    if (linear_int8_fuses(p, mode == INT8_GATED, f32, held)) return (int)linear_int8_few(p, mode, f32, true, stream);
+    if (!coded && linear_int8_fuses(p, mode == INT8_GATED, f32, held)) return (int)linear_int8_few(p, mode, f32, true, stream);
     const Quantize8 q{x, x_stride, (int8_t*)codes, scales, m, k, kp};
-    const cudaError_t e = f32 ? launch_quantize<float>(q, stream) : launch_quantize<bf16>(q, stream);
+    const cudaError_t e = coded ? cudaSuccess : f32 ? launch_quantize<float>(q, stream) : launch_quantize<bf16>(q, stream);
     if (e != cudaSuccess) return (int)e;
     // us by few rows' kernel / by tcgen05: 16 rows 16,384 x 2,048 13.2 / 13.7, 2,048 x 8,192 8.8 / 11; 32 rows 960 x 576 4.5 / 5.9,
     // 2,048 x 2,048 6.1 / 6.4, 6,144 x 2,048 9.1 / 8.2, 2,048 x 8,192 14.4 / 11.1, 16,384 x 2,048 18.0 / 13.5

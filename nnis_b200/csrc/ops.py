@@ -69,7 +69,7 @@ def _stream() -> ctypes.c_void_p:
 _ENTRY_FIELDS = {"nnis_copy_pages": "ppiiiiiipiip", "nnis_verify_drafts": "ppppppppiiippp",
                  "nnis_attention_shared": "pippppipiiippppppiiiiiifiipp",
                  "nnis_rope_store_int8": "pppppppppppiiiiiiiiiip", "nnis_read_pages_int8": "ppppppppiiiiiiiiip",
-                 "nnis_attention_int8": "ppppppppppppiiiiiiiiiifiiiiiip", "nnis_quantize_rows": "pppiiiip",
+                 "nnis_attention_int8": "ppppppppppppiiiiiiiiiifiiiiiip", "nnis_quantize_rows": "pppiiiip", "nnis_rmsnorm_int8": "ppppiiifp",
                  "nnis_linear_int8": "ppppppppiiiiiiiip"}
 _entries = {}
 
@@ -3120,8 +3120,12 @@ def read_pages_int8(k: torch.Tensor, v: torch.Tensor, k_scales: torch.Tensor, v_
         shape[3], _stream_of(index)), "read_pages_int8")
 
 
-# A prompt step whose sequences bring at most this many tokens each attends over the codes row by row; others read their pages back.
-INT8_ROWS_AT_ONCE = 16
+# A prompt step whose sequences bring at most this many tokens each attends over the codes row by row; others read their pages back and
+# take the kernels of the 16-bit or float32 cache.  us by rows / read back, 9 query and 3 key/value heads of 64, bfloat16: eight sequences
+# of 4,000, 8 tokens 15 / 39, 16 tokens 24 / 40, 24 tokens 61 / 40; one of 4,000, 64 tokens 17 / 24; float32: eight of 1,000, 32 tokens
+# 28 / 37, eight of 4,000 76 / 112; 32 and 8 heads of 128, eight of 4,000: bfloat16 16 tokens 66 / 185, 24 tokens 132 / 159, float32
+# 64 tokens 373 / 1,761.
+INT8_ROWS_AT_ONCE = {torch.bfloat16: 16, torch.float32: 64}
 
 
 def attention_int8_splits(n: int, heads: int, keys: int, device) -> int:
@@ -3249,6 +3253,53 @@ def quantize_rows(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor) ->
     stride = x.stride(0) if rows > 1 else k
     _check(_entry("nnis_quantize_rows")(x.data_ptr(), codes.data_ptr(), scales.data_ptr(), stride, code, rows, k, _stream_of(index)),
            "quantize_rows")
+
+
+def rmsnorm_int8_takes(width: int) -> bool:
+    return width % 4 == 0 and width <= 8192
+
+
+def rmsnorm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float, codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype) -> None:
+    """``rmsnorm`` to ``dtype`` and ``quantize_rows`` in one: x float32 [n, width], a width of a multiple of 4 up to 8,192; codes int8 [n,
+    int8_width(width)], scales float32 [n]."""
+    n, width = x.shape
+    _need(rmsnorm_int8_takes(width) and eps > 0, f"rmsnorm_int8: a width of a multiple of 4 up to 8,192 and a positive eps; got {width}, {eps}")
+    _wanted("rmsnorm_int8", x=(x, torch.float32, (n, width)), weight=(weight, torch.float32, (width,)),
+            codes=(codes, torch.int8, (n, int8_width(width))), scales=(scales, torch.float32, (n,)))
+    code = code_of(dtype)
+    if n == 0:
+        return
+    index = x.get_device()
+    if _device_now() != index:
+        with torch.cuda.device(index):
+            return rmsnorm_int8(x, weight, eps, codes, scales, dtype)
+    _check(_entry("nnis_rmsnorm_int8")(x.data_ptr(), weight.data_ptr(), codes.data_ptr(), scales.data_ptr(), n, width, code, eps,
+                                       _stream_of(index)), "rmsnorm_int8")
+
+
+def linear_int8_coded(codes: torch.Tensor, scales: torch.Tensor, k: int, w: torch.Tensor, w_scales: torch.Tensor,
+                      bias: Optional[torch.Tensor], out: torch.Tensor, mode: int) -> None:
+    """``linear_int8`` of rows that are codes already (``rmsnorm_int8``, ``quantize_rows``): codes int8 [m, int8_width(k)], scales float32
+    [m]; in the modes STORE and GEMM_GATED out is float32 or bfloat16."""
+    m, rows = codes.shape[0], w.shape[0]
+    n = rows // 2 if mode == GEMM_GATED else rows
+    _need(mode in (STORE, STORE_F32, ADD_F32, GEMM_GATED) and 0 < k <= 133136 and (mode != GEMM_GATED or rows % 2 == 0) and n > 0,
+          f"linear_int8_coded: mode {mode}, k {k}, {rows} rows of w")
+    kept = out.dtype if mode in (STORE, GEMM_GATED) else torch.float32
+    code = code_of(out.dtype)
+    _wanted("linear_int8_coded", codes=(codes, torch.int8, (m, int8_width(k))), scales=(scales, torch.float32, (m,)),
+            w=(w, torch.int8, (rows, int8_width(k))), w_scales=(w_scales, torch.float32, (rows,)), bias=(bias, torch.float32, (rows,)),
+            out=(out, kept, (m, n)))
+    if m == 0:
+        return
+    index = w.get_device()
+    if _device_now() != index:
+        with torch.cuda.device(index):
+            return linear_int8_coded(codes, scales, k, w, w_scales, bias, out, mode)
+    _check(_entry("nnis_linear_int8")(
+        0, w.data_ptr(), w_scales.data_ptr(), 0 if bias is None else bias.data_ptr(), out.data_ptr(), codes.data_ptr(), scales.data_ptr(),
+        status_word(w.device).data_ptr(), 0, m, n, k, mode, code, _sm_count.get(index) or sm_count(w.device), 1, _stream_of(index)),
+        "linear_int8_coded")
 
 
 def linear_int8(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, bias: Optional[torch.Tensor], out: torch.Tensor, mode: int,

@@ -28,7 +28,7 @@ from ..cache import PAGE_SIZE, KVRequest, KVView
 from ..csrc import ops
 from ..weights.loader import WeightSpec
 from .base import MIXERS, POSITIONS, Part, begin_norm
-from .linear import ADD_F32, STORE, Int8Matrix, linear, matrix_bytes
+from .linear import ADD_F32, STORE, Int8Matrix, linear, matrix_bytes, normed_codes
 
 
 class Attention(Part):
@@ -134,7 +134,7 @@ class Attention(Part):
     def _read_back_table(self, counts, starts):
         """Which pages of an 8-bit cache a prompt step reads back, and to which places: [sequences, columns], -1 for pages that lie
         before every window.  None where every sequence brings few tokens: their rows read the codes as they are."""
-        if max(counts) <= ops.INT8_ROWS_AT_ONCE:
+        if max(counts) <= ops.INT8_ROWS_AT_ONCE[self.dtype]:
             return None
         spans = [(max(0, s - self.window + 1) // PAGE_SIZE if self.window > 0 else 0, -(-(s + c) // PAGE_SIZE))
                  for c, s in zip(counts, starts)]
@@ -164,7 +164,7 @@ class Attention(Part):
                 places = {name + "/pages": np.asarray([read[1] if read else 0], dtype=np.int32)}
                 if read:
                     places[name] = read[0]
-            if max(counts) <= ops.INT8_ROWS_AT_ONCE:
+            if max(counts) <= ops.INT8_ROWS_AT_ONCE[self.dtype]:
                 return places
             places.update(self._kernel_tables(counts, starts, have))
             return places
@@ -237,6 +237,8 @@ class Attention(Part):
                                   self.device))
 
     def fuses_norm(self, norm, ctx, n: int) -> bool:
+        if isinstance(self.w_qkv, Int8Matrix):  # (the norm puts its rows into codes)
+            return getattr(norm, "kind", None) == "rmsnorm" and ops.rmsnorm_int8_takes(self.hidden)
         return getattr(norm, "kind", None) == "rmsnorm" and self._decode_kernels(ctx, n, normed=True)
 
     def shares_norm(self, norm, ctx, n: int) -> bool:
@@ -319,7 +321,11 @@ class Attention(Part):
             q_buf, q_stride = q, nq * d
         else:
             qkv = ws.get("qkv", (n, (nq + 2 * self.stored_kv) * d), self.dtype)
-            linear(x, self.w_qkv, self.b_qkv, qkv, STORE, ws, decode=ctx.decode and self.codes)
+            if norm is not None:
+                codes, scales = normed_codes(hidden, norm, self.dtype, ws)
+                ops.linear_int8_coded(codes, scales, self.hidden, self.w_qkv.codes, self.w_qkv.scales, self.b_qkv, qkv, STORE)
+            else:
+                linear(x, self.w_qkv, self.b_qkv, qkv, STORE, ws, decode=ctx.decode and self.codes)
             if not self.position_in_kernel:  # an encoding with arithmetic of its own
                 self.position.apply(qkv, ctx, nq, self.stored_kv, d)
             if self.codes and self.own_kv:

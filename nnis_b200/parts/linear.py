@@ -45,6 +45,15 @@ def matrix_bytes(weight: Union[None, torch.Tensor, Int8Matrix]) -> int:
     return weight.bytes() if isinstance(weight, Int8Matrix) else weight.numel() * weight.element_size()
 
 
+def normed_codes(hidden: torch.Tensor, norm, dtype: torch.dtype, workspace):
+    """(codes, scales) of a norm's rows, for products of 8-bit matrices that read the same rows."""
+    n, width = hidden.shape
+    codes = workspace.get("int8_normed_codes", (n, ops.int8_width(width)), torch.int8)
+    scales = workspace.get("int8_normed_scales", (n,), torch.float32)
+    ops.rmsnorm_int8(hidden, norm.weight, norm.eps, codes, scales, dtype)
+    return codes, scales
+
+
 def linear(x: torch.Tensor, weight: Union[torch.Tensor, Int8Matrix], bias: Optional[torch.Tensor], out: torch.Tensor,
            mode: int, workspace=None, decode: bool = False) -> None:
     """``workspace``: the step's buffers (``engine.workspace.Workspace``); with it the adding

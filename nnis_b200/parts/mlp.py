@@ -21,7 +21,7 @@ import torch
 from ..csrc import ops
 from ..weights.loader import WeightSpec
 from .base import FEED_FORWARDS, Part, begin_norm
-from .linear import ADD_F32, STORE_F32, Int8Matrix, linear, matrix_bytes
+from .linear import ADD_F32, STORE_F32, Int8Matrix, linear, matrix_bytes, normed_codes
 
 
 class GatedMLP(Part):
@@ -83,6 +83,8 @@ class GatedMLP(Part):
                 and ops.gemv_pays(n, self.hidden, self.inter, ops.EPI_ADD_F32, self.device))
 
     def fuses_norm(self, norm, ctx, n: int) -> bool:
+        if isinstance(self.w_gu, Int8Matrix):  # (the norm puts its rows into codes)
+            return getattr(norm, "kind", None) == "rmsnorm" and self.activation == "silu" and ops.rmsnorm_int8_takes(self.hidden)
         return getattr(norm, "kind", None) == "rmsnorm" and self._fused_gate_up(ctx, n, normed=True)
 
     def shares_norm(self, norm, ctx, n: int) -> bool:
@@ -114,7 +116,10 @@ class GatedMLP(Part):
                           norm_weight=norm.weight if norm is not None else None,
                           eps=norm.eps if norm is not None else 0.0, m=n, act=self.fused_act)
         elif isinstance(self.w_gu, Int8Matrix):
-            if self.activation == "silu":  # (in the product's epilogue)
+            if norm is not None:
+                codes, scales = normed_codes(hidden, norm, self.dtype, ws)
+                ops.linear_int8_coded(codes, scales, self.hidden, self.w_gu.codes, self.w_gu.scales, self.b_gu, act, ops.GEMM_GATED)
+            elif self.activation == "silu":  # (in the product's epilogue)
                 ops.linear_int8(x, self.w_gu.codes, self.w_gu.scales, self.b_gu, act, ops.GEMM_GATED, ws)
             else:
                 self._activate_apart(x, act, ctx)

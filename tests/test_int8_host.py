@@ -173,7 +173,7 @@ def test_pages_that_a_prompt_step_reads_back():
     from helpers import TINY_A
     spec = config_from_dict(TINY_A).to_spec()
     mixer = DecoderModel(spec, BF16, torch.device("cpu"), "int8").blocks[0].mixer
-    few, many = ops.INT8_ROWS_AT_ONCE, ops.INT8_ROWS_AT_ONCE + 1
+    few, many = ops.INT8_ROWS_AT_ONCE[BF16], ops.INT8_ROWS_AT_ONCE[BF16] + 1
     name = mixer._read_back_name()
     assert name not in mixer.step_tables([few, 1], [100, 0])
     tables = mixer.step_tables([1, many, 64], [100, 64, 0])
@@ -209,3 +209,20 @@ def test_plans_of_attention_cover_every_key(d):
                     assert 1 <= slices <= 64 and slices * pieces >= per_page * cols and (slices - 1) * pieces < per_page * cols
                     assert cluster in (0, 1, 2, 4, 8) and (cluster > 0 or slices == 1) and eights in (1, 2)
                     assert 1 <= rows <= max(1, 64 // (heads // kv_heads)) and slices * cluster <= 65535
+
+
+def test_norms_and_coded_rows_refuse():
+    from nnis_b200.csrc import ops
+    x, w, codes, scales = empty(3, 20), empty(20), empty(3, 32, dtype=I8), empty(3)
+    for args, why in (((x, w, 1e-5, codes, scales, BF16), "CUDA tensors only"), ((x, w, 0.0, codes, scales, BF16), "positive eps"),
+                      ((empty(3, 21), empty(21), 1e-5, codes, scales, BF16), "multiple of 4"), ((x, empty(21), 1e-5, codes, scales, BF16), "weight is"),
+                      ((x, w, 1e-5, empty(3, 20, dtype=I8), scales, BF16), "codes is"), ((x.to(BF16), w, 1e-5, codes, scales, BF16), "x is")):
+        with pytest.raises(ops.KernelError, match=why):
+            ops.rmsnorm_int8(*args)
+    m, ms = empty(12, 32, dtype=I8), empty(12)
+    for args, why in (((codes, scales, 20, m, ms, None, empty(3, 12), 0), "CUDA tensors only"), ((codes, scales, 40, m, ms, None, empty(3, 12), 0), "codes is"),
+                      ((codes, empty(4), 20, m, ms, None, empty(3, 12), 0), "scales is"), ((codes, scales, 20, m, ms, empty(11), empty(3, 12), 0), "bias is"),
+                      ((codes, scales, 20, m, ms, None, empty(3, 12), 3), "out is"), ((codes, scales, 20, m, ms, None, empty(3, 12, dtype=BF16), 1), "out is"),
+                      ((codes, scales, 20, m, ms, None, empty(3, 12), 9), "mode 9")):
+        with pytest.raises(ops.KernelError, match=why):
+            ops.linear_int8_coded(*args)

@@ -152,7 +152,7 @@ def test_few_tokens_after_a_long_context_read_the_codes(dtype, tmp_path, monkeyp
     assert calls[2:] == ["attention_int8"] * 2
     for s, n in zip(slots, (500, 501)):
         engine.truncate(s, n)
-    many = engine.step([SequenceStep(slots[0], tokens(6, 5) + tokens(8, 20), range(5)), SequenceStep(slots[1], tokens(7, 1), [0])]).cpu().numpy()
+    many = engine.step([SequenceStep(slots[0], tokens(6, 5) + tokens(8, 70), range(5)), SequenceStep(slots[1], tokens(7, 1), [0])]).cpu().numpy()
     assert calls[4:] == ["read_pages_int8"] * 2
     near(few, many, dtype)
 

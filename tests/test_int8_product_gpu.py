@@ -140,3 +140,28 @@ def test_products_on_a_stream_and_in_a_graph():
         first = out.clone()
         step()
         assert torch.equal(first, out)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,width", [(1, 4), (3, 20), (7, 576), (40, 2048), (2, 8192), (5, 1028), (300, 64)])
+def test_a_norm_and_codes_in_one(dtype, n, width):
+    """The codes of the norm's rows: a value may fall to the neighbouring code where the norm's sums, in another order, end an ulp apart."""
+    from nnis_b200.csrc import ops
+    gen = torch.Generator().manual_seed(width)
+    x, w = torch.randn((n, width), generator=gen).cuda(), (1 + 0.1 * torch.randn(width, generator=gen)).cuda()
+    normed = torch.empty((n, width), dtype=dtype, device="cuda")
+    ops.rmsnorm(x, w, 1e-5, normed)
+    codes, scales = coded(normed)
+    got, got_scales = torch.full_like(codes, 77), torch.empty_like(scales)
+    ops.rmsnorm_int8(x, w, 1e-5, got, got_scales, dtype)
+    # sums of `width` squares in two orders differ by up to width roundings of 2^-24 each, their roots by half of that; a few roundings
+    # follow, then one of `dtype` that may fall otherwise, in a value or in its row's largest
+    step = torch.finfo(dtype).eps + (width + 8) * 2.0 ** -24
+    assert ((got_scales - scales).abs() <= 1.01 * step * scales).all() and (got[:, width:] == 0).all()
+    assert (got.int() - codes.int()).abs().max() <= 1 + int(2 * 127 * step)
+    out, want = torch.empty((n, 24), device="cuda"), torch.empty((n, 24), device="cuda")
+    m, s = coded(torch.randn((24, width), generator=gen))
+    ops.linear_int8_coded(codes, scales, width, m, s, None, out, ops.STORE)
+    from nnis_b200.engine.workspace import Workspace
+    ops.linear_int8(normed, m, s, None, want, ops.STORE_F32, Workspace(torch.device("cuda")))
+    assert torch.equal(out, want)
