@@ -3330,9 +3330,13 @@ def linear_int8(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, bias: 
     if _device_now() != index:
         with torch.cuda.device(index):
             return linear_int8(x, w, w_scales, bias, out, mode, workspace)
+    sms = _sm_count.get(index) or sm_count(w.device)
+    # (what the library does: one or two rows become codes in the product's own kernel)
+    fused = m <= 2 and -(-n // (8 if mode == GEMM_GATED else 16)) <= sms and width <= 16384 and k % 8 == 0 \
+        and (m == 1 or x.stride(0) % 8 == 0) and x.data_ptr() % (16 if dtype == torch.float32 else 8) == 0
     codes = workspace.room("int8_codes", m * width, torch.int8)
     scales = workspace.room("int8_scales", m, torch.float32)
     _check(_entry("nnis_linear_int8")(
         x.data_ptr(), w.data_ptr(), w_scales.data_ptr(), 0 if bias is None else bias.data_ptr(), out.data_ptr(), codes.data_ptr(),
         scales.data_ptr(), status_word(w.device).data_ptr(), x.stride(0) if m > 1 else k, m, n, k, mode, _DTYPE_CODE[dtype],
-        _sm_count.get(index) or sm_count(w.device), 0, _stream_of(index)), "linear_int8", 2)
+        sms, 0, _stream_of(index)), "linear_int8", 1 if fused else 2)

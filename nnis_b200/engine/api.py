@@ -148,10 +148,11 @@ class EngineBackend:
         cache.reserve([slot], [held + n])
         key = self._decoder_key(n, held + n, True)
         units = self._drafted.setdefault(n, BatchUnits(engine, drafted=True)).units([slot] * n, positions, key[0])
-        dec = self._captured((*key, rooms_of(units)))
+        dec = self._captured(key if units is None else (*key, rooms_of(units)))
         if dec is None:
             return engine.step([SequenceStep(slot, tokens, list(range(n)))], drafted=True)
-        dec.plans.fill(units)
+        if units is not None:
+            dec.plans.fill(units)
         self.h2d_bytes += dec.upload(tokens, positions, [slot] * n)
         dec.launch()
         cache.commit([slot], [held + n])

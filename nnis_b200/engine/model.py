@@ -122,14 +122,14 @@ class DecoderModel:
         self._embedding_view = cache.view(len(self.spec.schedule))
         keys = {}
         for entry, view in zip(self.spec.schedule, self._views):
-            ask = getattr(self.blocks[entry.layer].mixer, "shared_key", None)
-            if ask is not None:
-                keys[ask(view)] = True
-            else:
-                keys[None] = True
+            mixer = self.blocks[entry.layer].mixer
+            ask = getattr(mixer, "shared_key", None)
+            key = ask(view) if ask is not None else None
+            if key is not None or not getattr(mixer, "rows_apart", False):
+                keys[key] = True
         self._shared_keys = [k for k in keys if k is not None]
-        # every mixer can: a captured step may bring several tokens of one sequence (kernels of other mixers ask for pages
-        # ahead of the kernel that writes them, which is sound only for a step's single token)
+        # every mixer can, or reads nothing ahead of the kernel that writes it: a captured step may bring several tokens of one
+        # sequence (kernels of other mixers ask for pages ahead of that, which is sound only for a step's single token)
         self.all_share = None not in keys
 
     def shared_keys(self):

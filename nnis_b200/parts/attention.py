@@ -105,6 +105,12 @@ class Attention(Part):
                 or (view.k_scales is not None) != self.codes:
             raise ValueError("the shared cache does not fit this attention's heads or window")
 
+    @property
+    def rows_apart(self) -> bool:
+        """Rows of a captured step may be several tokens of one sequence although no plan brings them together: attention over codes
+        reads nothing ahead of the kernel that writes it."""
+        return self.codes
+
     def shared_key(self, view: KVView):
         """What a plan for pages that several rows share is made for (None: this attention reads them row by row)."""
         if self.window > 0 or self.codes or not ops.attention_shared_takes(self.head_dim, view.page_size):

@@ -194,3 +194,38 @@ def test_the_command_line(tmp_path, capsys):
     assert run(parse_args(["generate", "--model", made, "--prompt-ids", "1,2,3", "--max-new-tokens", "4", "--cache-dtype", "int8",
                            "--weight-dtype", "int8"]), out) == 0
     assert out.getvalue().strip()
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_drafted_steps_are_captured(dtype, tmp_path, monkeypatch):
+    """Over an 8-bit cache a sequence's drafted tokens run as a replayed step, a row each; the logits are those of a prompt of the same
+    tokens."""
+    from nnis_b200 import LLM, GenerationConfig, LookupDrafter
+    from nnis_b200.engine import SequenceStep
+    from nnis_b200.engine.decode import GraphDecoder
+    llm = LLM(make_model(str(tmp_path), SHARED, 3), dtype=dtype, max_tokens=1 << 13, max_batch=4, cache_dtype="int8")
+    launched, launch = [], GraphDecoder.launch
+    monkeypatch.setattr(GraphDecoder, "launch", lambda self: (launched.append(self.rows), launch(self))[1])
+    engine, backend = llm.engine, llm.backend
+    slot, fed = engine.acquire_slot(), tokens(30, 122)
+    engine.step([SequenceStep(slot, fed, [])])
+    for turn, count in enumerate((5, 5, 3, 8, 1, 5)):  # (over the end of a page)
+        drafted = tokens(40 + turn, count)
+        got = backend.drafted_logits(slot, drafted, True).cpu().numpy()
+        alone = engine.acquire_slot()
+        want = engine.step([SequenceStep(alone, fed + drafted, list(range(len(fed), len(fed) + count)))]).cpu().numpy()
+        engine.release_slot(alone)
+        near(got, want, dtype)
+        kept = max(1, count - turn % 3)  # some are rejected
+        fed = fed + drafted[:kept]
+        engine.truncate(slot, len(fed))
+    assert len(launched) == 6 and set(launched) == {1, 4, 8}
+    engine.release_slot(slot)
+    phrase = tokens(50, 12) * 6
+    want = llm.generate([phrase], max_new_tokens=40, stop_token_ids=[])[0].token_ids
+    before = len(launched)
+    got = list(llm.new_session().generate_drafted(phrase, GenerationConfig(40), LookupDrafter(), drafts=4))
+    assert len(launched) > before
+    if dtype == "float32":
+        assert got == want
+    engine.check_status()
