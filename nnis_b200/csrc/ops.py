@@ -3144,11 +3144,13 @@ def attention_int8_plan(n: int, seqs: int, heads: int, kv_heads: int, d: int, co
     length = 64 // half
     seen = min(half * cols, (window + rows + length - 2) // length + 1) if window else half * cols
     resident = sms * (4 if d <= 32 else 3 if d <= 96 else 2)
-    # tiles of 8 queries, of 16 where those of 8 would take the device more than one turn.  us in tiles of 8 / 16: five rows of four heads of
-    # 128, 16 sequences of 4,000 (384 or 256 units of 296 at once) 101 / 65; 20 heads of 64, 64 sequences of 4,096 (192 units) 23 / 29;
-    # two rows of eight heads of 128, 2 sequences of 706 7.2 / 10.0
+    # tiles of 8 queries; of 16 where those of 8 would take the device more than one turn, and with heads beyond 64, whose tiles of 8 leave
+    # the tensor cores waiting, where four CTAs a unit fill it.  us in tiles of 8 / 16, each with its best number of CTAs: five rows of four
+    # heads of 128, 16 sequences of 4,000 94 / 65, 4 of 8,000 54 / 42; 24 heads of 128, 64 sequences of 4,000 52 / 40, 8 of 4,000 14.2 /
+    # 17.4; 20 heads of 64, 64 sequences of 4,096 23 / 29; five rows of three heads of 64, 64 sequences of 2,000 22.8 / 22.1
     runs = -(-n // rows) * kv_heads
-    eights = 2 if rows * per > 8 and runs * -(-rows * per // 8) > resident else 1
+    turns = resident // (runs * -(-rows * per // 16))
+    eights = 2 if rows * per > 8 and (runs * -(-rows * per // 8) > resident or (d > 64 and turns <= 4)) else 1
     units = runs * -(-rows * per // (8 * eights))
     # A warp a unit where units are many and short: us by four warps / one: 1,760 units of one piece 18.6 / 6.4, 2,048 of two 25.4 / 14.8,
     # of eight 39.8 / 37.4, of 16 58.6 / 66.1; 512 (heads of 128) of ten 20.5 / 16.5, of 32 36.7 / 39.7.
