@@ -33,18 +33,18 @@ constexpr int kPage8 = 64, kWarps8 = 4;
 __host__ __device__ constexpr int stage_bytes8(int d) { return 2 * piece8(d) * (d + 4); }
 
 __device__ __forceinline__ void mma_s8(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 // The same without sums before it
 __device__ __forceinline__ void mma_s8_first(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
                  : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(0));
 }
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -294,23 +294,25 @@ __global__ void __launch_bounds__(kWarps8 * 32, D <= 32 ? 4 : D <= 96 ? 3 : 2) a
 #pragma unroll
             for (int s = 0; s < kScores / 4; ++s) {
                 int acc[MT][2][4], acl[F32 ? MT : 1][2][4];
+                uint32_t w[2][kWords];
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    uint32_t w[kWords];
-                    load_words<kWords>(w, at + (16 * s + 4 * (g >> 1) + 2 * j + (g & 1)) * D + t * (D / 4));
+                for (int j = 0; j < 2; ++j)
+                    load_words<kWords>(w[j], at + (16 * s + 4 * (g >> 1) + 2 * j + (g & 1)) * D + t * (D / 4));
+                // (products that follow one another belong to different sums: a warp waits some 30 cycles for one that its next adds to)
+#pragma unroll
+                for (int k = 0; k < kSteps; ++k)
 #pragma unroll
                     for (int i = 0; i < MT; ++i)
 #pragma unroll
-                        for (int k = 0; k < kSteps; ++k) {
-                            if (k == 0) mma_s8_first(acc[i][j], qa[i][k], w[2 * k], w[2 * k + 1]);
-                            else mma_s8(acc[i][j], qa[i][k], w[2 * k], w[2 * k + 1]);
+                        for (int j = 0; j < 2; ++j) {
+                            if (k == 0) mma_s8_first(acc[i][j], qa[i][k], w[j][2 * k], w[j][2 * k + 1]);
+                            else mma_s8(acc[i][j], qa[i][k], w[j][2 * k], w[j][2 * k + 1]);
                             if constexpr (F32) {
                                 const uint32_t a[4] = {ql[i][k][0], 0u, ql[i][k][1], 0u};
-                                if (k == 0) mma_s8_first(acl[i][j], a, w[2 * k], w[2 * k + 1]);
-                                else mma_s8(acl[i][j], a, w[2 * k], w[2 * k + 1]);
+                                if (k == 0) mma_s8_first(acl[i][j], a, w[j][2 * k], w[j][2 * k + 1]);
+                                else mma_s8(acl[i][j], a, w[j][2 * k], w[j][2 * k + 1]);
                             }
                         }
-                }
                 const float4 scales = *reinterpret_cast<const float4*>(ks + 16 * s + 4 * t);
                 const float key_scale[4] = {scales.x, scales.y, scales.z, scales.w};
 #pragma unroll
