@@ -16,14 +16,24 @@ struct Quantize8 {
     int8_t* codes;
     float* scales;
     int rows, k, kp;
+    int matrix;  // 1: the rows may be a matrix's, which products ask for ahead of their wait
 };
+
+// A product's kernel loads codes of its matrix before it waits for the kernel ahead of it.  So a kernel that may make a matrix lets nothing
+// start before its end, by when its codes are out; one that makes a product's own x lets the product start at once.
+__device__ __forceinline__ void release_early(const Quantize8& p) {
+    if (!p.matrix) pdl_launch_dependents();
+}
+__device__ __forceinline__ void release_late(const Quantize8& p) {
+    if (p.matrix) __threadfence();
+}
 
 // WARPS warps a row, its values in registers between the two looks at them: CHUNKS runs of eight a lane.
 template <typename T, int WARPS, int CHUNKS>
 __global__ void __launch_bounds__(128) quantize_rows_kernel(const __grid_constant__ Quantize8 p) {
     __shared__ uint32_t tops[4];
     pdl_wait();
-    pdl_launch_dependents();
+    release_early(p);
     constexpr int kLanes = WARPS * 32;
     const int row = blockIdx.x * (4 / WARPS) + threadIdx.x / kLanes, lane = threadIdx.x % kLanes;
     const T* x = reinterpret_cast<const T*>(p.x) + (size_t)row * p.x_stride;
@@ -63,6 +73,7 @@ __global__ void __launch_bounds__(128) quantize_rows_kernel(const __grid_constan
                                                           code_word(v[c][4], v[c][5], v[c][6], v[c][7], r.inverse, good));
     }
     if (lane == 0) p.scales[row] = r.scale;
+    release_late(p);
 }
 
 // Any row: a CTA each, read twice.
@@ -70,7 +81,7 @@ template <typename T>
 __global__ void __launch_bounds__(128) quantize_rows_any_kernel(const __grid_constant__ Quantize8 p) {
     __shared__ uint32_t tops[4];
     pdl_wait();
-    pdl_launch_dependents();
+    release_early(p);
     const T* x = reinterpret_cast<const T*>(p.x) + (size_t)blockIdx.x * p.x_stride;
     uint32_t top = 0;
     for (int i = threadIdx.x; i < p.k; i += 128) top = max(top, magnitude_bits(to_float(x[i])));
@@ -88,6 +99,7 @@ __global__ void __launch_bounds__(128) quantize_rows_any_kernel(const __grid_con
         *reinterpret_cast<uint32_t*>(codes + i) = pack_codes(c[0], c[1], c[2], c[3]);
     }
     if (threadIdx.x == 0) p.scales[blockIdx.x] = r.scale;
+    release_late(p);
 }
 
 // A norm's rows put into codes: y = x / sqrt(mean(x^2) + eps) * w, rounded to T as the norm by itself would be, its codes and scale.  A CTA a
@@ -179,7 +191,7 @@ NNIS_API int nnis_quantize_rows(const void* call) {
     const auto [x, codes, scales, x_stride, dtype, rows, k, stream] = c;
     if (!x || !codes || !scales || rows <= 0 || k <= 0 || k > 0x7ffffff0 || x_stride < k) return NNIS_ERR_ARGUMENT;
     if ((uintptr_t)codes % 16) return NNIS_ERR_ALIGNMENT;
-    const Quantize8 p{x, x_stride, (int8_t*)codes, scales, rows, k, (k + 15) / 16 * 16};
+    const Quantize8 p{x, x_stride, (int8_t*)codes, scales, rows, k, (k + 15) / 16 * 16, 1};
     if (dtype == NNIS_DTYPE_F32) return (int)launch_quantize<float>(p, stream);
     if (dtype == NNIS_DTYPE_BF16) return (int)launch_quantize<bf16>(p, stream);
     return NNIS_ERR_UNSUPPORTED;
@@ -235,7 +247,7 @@ NNIS_API int nnis_linear_int8(const void* call) {
     const Linear8 p{(const int8_t*)codes, (const int8_t*)w, scales, ws, bias, out, m, n, kp, status, 0, x, x_stride, k};
     const int held = sms > 0 ? sms : 148;
     if (!coded && linear_int8_fuses(p, mode == INT8_GATED, f32, held)) return (int)linear_int8_few(p, mode, f32, true, stream);
-    const Quantize8 q{x, x_stride, (int8_t*)codes, scales, m, k, kp};
+    const Quantize8 q{x, x_stride, (int8_t*)codes, scales, m, k, kp, 0};
     const cudaError_t e = coded ? cudaSuccess : f32 ? launch_quantize<float>(q, stream) : launch_quantize<bf16>(q, stream);
     if (e != cudaSuccess) return (int)e;
     // us by few rows' kernel / by tcgen05: 16 rows 16,384 x 2,048 13.2 / 13.7, 2,048 x 8,192 8.8 / 11; 32 rows 960 x 576 4.5 / 5.9,

@@ -165,3 +165,37 @@ def test_a_norm_and_codes_in_one(dtype, n, width):
     from nnis_b200.engine.workspace import Workspace
     ops.linear_int8(normed, m, s, None, want, ops.STORE_F32, Workspace(torch.device("cuda")))
     assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("m,n,k,is_coded", [(1, 512, 16384, False), (2, 960, 8192, False), (1, 576, 960, False), (8, 512, 20000, True), (64, 512, 20000, True),
+                                           (512, 4096, 2048, True)])
+def test_a_matrix_that_was_just_put_into_codes(m, n, k, is_coded):
+    """The product right behind the kernel that makes its matrix, in a graph, reads the new codes: products ask for their matrix ahead of
+    their wait."""
+    from nnis_b200.csrc import ops
+    from nnis_b200.engine.workspace import Workspace
+    ws, gen = Workspace(torch.device("cuda")), torch.Generator("cuda").manual_seed(n + k)
+    x, w = (torch.randn((rows, k), generator=gen, device="cuda").bfloat16() for rows in (m, n))
+    (codes, scales), (x_codes, x_scales) = coded(w), coded(x)
+    out = torch.zeros((m, n), dtype=torch.bfloat16, device="cuda")
+
+    def product():
+        if is_coded:
+            ops.linear_int8_coded(x_codes, x_scales, k, codes, scales, None, out, ops.STORE)
+        else:
+            ops.linear_int8(x, codes, scales, None, out, ops.STORE, ws)
+    product()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.quantize_rows(w, codes, scales)
+        product()
+    for _ in range(5):
+        w.copy_(torch.randn((n, k), generator=gen, device="cuda").bfloat16())
+        torch.cuda.synchronize()
+        graph.replay()
+        got = out.clone()
+        torch.cuda.synchronize()
+        product()
+        assert torch.equal(got, out)
+    del graph
