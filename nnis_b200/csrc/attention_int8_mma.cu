@@ -15,7 +15,7 @@
 // position's row, of the value product bytes [g D / 8, (g + 1) D / 8) of positions 4 t to 4 t + 3 (g = lane / 4, t = lane % 4).
 //
 // A CTA: four warps, (run of rows with one sequence, key/value head, tile of queries, slice of positions); a warp takes every fourth piece
-// of 32 positions of the slice through a ring of its own, filled by bulk copies, so that nothing meets before the slice's end.  Slices are of a
+// of 64 or 32 positions of the slice through a ring of its own, filled by bulk copies, so that nothing meets before the slice's end.  Slices are of a
 // fixed number of pieces, so sequences of all lengths are cut into equal pieces; the slice that ends last joins them.
 #include <float.h>
 #include <string.h>
@@ -166,7 +166,7 @@ __global__ void __launch_bounds__(kWarps8 * 32, D <= 32 ? 4 : D <= 96 ? 3 : 2) a
     pdl_wait();
     pdl_launch_dependents();
 
-    const int per = p.nq / p.nkv, slice = blockIdx.y / p.cluster, rank = blockIdx.y % p.cluster;
+    const int per = p.nq / p.nkv, slice = SOLO ? 0 : blockIdx.y / p.cluster, rank = SOLO ? 0 : blockIdx.y % p.cluster;
     int unit = SOLO ? blockIdx.x * kWarps8 + warp : blockIdx.x;
     if (SOLO && unit >= p.units) return;  // (whole warps: nothing below meets in this form)
     const int tile = unit % p.tiles;
@@ -283,6 +283,12 @@ __global__ void __launch_bounds__(kWarps8 * 32, D <= 32 ? 4 : D <= 96 ? 3 : 2) a
             const unsigned char* at = ring + stage * kStage;
             if (!mbar_wait(&full[warp][stage], phase)) {
                 if (lane == 0) atomicExch(p.status, 1);
+                // (copies that are on their way do not outlive the CTA)
+#pragma unroll
+                for (int s = 1; s < kStages; ++s) {
+                    const int to = stage + s < kStages ? stage + s : stage + s - kStages;
+                    if (queue[s] >= 0) mbar_wait(&full[warp][to], to < stage ? phase ^ 1u : phase);
+                }
                 break;
             }
             const float* ks = reinterpret_cast<const float*>(at + 2 * kPiece8 * D);
