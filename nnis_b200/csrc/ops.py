@@ -3055,7 +3055,7 @@ def rope_store_int8(qkv: torch.Tensor, q: torch.Tensor, token_pos: torch.Tensor,
             and 2 <= d <= 256 and d % 2 == 0 and heads > 0 and kv_heads > 0 and page_size > 0 and dtype in _DTYPE_CODE and q.dtype is dtype
             and k.dtype is v.dtype is torch.int8 and k_scales.dtype is v_scales.dtype is torch.float32
             and token_pos.dtype is token_seq.dtype is page_table.dtype is torch.int32
-            and token_pos.numel() >= n <= token_seq.numel()
+            and token_pos.numel() >= n <= token_seq.numel() and (shape[0] > 0 and table_shape[0] > 0 and table_shape[1] > 0 or not n)
             and 0 <= index == v.get_device() == k_scales.get_device() == v_scales.get_device() == q.get_device() == qkv.get_device()
             == token_pos.get_device() == token_seq.get_device() == page_table.get_device()
             and k.is_contiguous() and v.is_contiguous() and k_scales.is_contiguous() and v_scales.is_contiguous() and q.is_contiguous()
@@ -3066,6 +3066,7 @@ def rope_store_int8(qkv: torch.Tensor, q: torch.Tensor, token_pos: torch.Tensor,
         code_of(dtype)
         _need(heads > 0, "rope_store_int8: at least one query head")
         _need((cos is None) == (sin is None), "rope_store_int8: cos and sin, or neither")
+        _need(not n or (k.numel() > 0 and page_table.numel() > 0), "rope_store_int8: a store and a page table of at least one page")
         _need(token_pos.numel() >= n and token_seq.numel() >= n, f"rope_store_int8: a position and a sequence for each of {n} rows")
         _wanted("rope_store_int8", qkv=(qkv, qkv.dtype, (None, (heads + 2 * kv_heads) * d)), q=(q, qkv.dtype, (n, heads * d)),
                 **_store8("rope_store_int8", k, v, k_scales, v_scales, kv_heads, d, page_size),
@@ -3091,7 +3092,8 @@ def read_pages_int8(k: torch.Tensor, v: torch.Tensor, k_scales: torch.Tensor, v_
     """Pages of the 8-bit cache read back: for every place (sequence, column) of ``local_table`` that names a page of the outputs,
     int32 [sequences, columns], -1 where none is wanted, that page becomes the values, code times scale, of the page that
     ``page_table`` names in the same place.  k, v int8 [pages, kv_heads, page_size, d], their scales float32 [pages, kv_heads,
-    page_size]; k_out, v_out float32 or bfloat16 [out_pages, kv_heads, page_size, d].  A page id outside its store is passed over."""
+    page_size]; k_out, v_out float32 or bfloat16 [out_pages, kv_heads, page_size, d].  A page id outside its store is passed over.
+    No two places name the same page of the outputs."""
     shape, places, table_shape, outs, dtype, index = k.shape, local_table.shape, page_table.shape, k_out.shape, k_out.dtype, k.get_device()
     if not (len(shape) == len(outs) == 4 and len(places) == len(table_shape) == 2 and outs[1:] == shape[1:] and v.shape == shape
             and v_out.shape == outs and k_scales.shape == shape[:3] and v_scales.shape == shape[:3] and shape[1] > 0 and shape[2] > 0
@@ -3188,7 +3190,8 @@ def attention_int8(q: torch.Tensor, q_stride: int, k: torch.Tensor, v: torch.Ten
             and v.shape == shape and per_head == shape[:3] and v_scales.shape == per_head and out_shape[1] == heads * d
             and q_shape[0] >= out_shape[0] and q_shape[1] >= heads * d <= q_stride < 1 << 31 and q.stride() == (q_stride, 1)
             and 2 <= d <= 256 and d % 2 == 0 and 0 < heads <= 65535 and kv_heads > 0 and heads % kv_heads == 0 and shape[2] > 0
-            and window >= 0 and scale > 0 and dtype in _DTYPE_CODE and out.dtype is dtype
+            and 0 <= window < 1 << 31 and 0 < scale < math.inf and dtype in _DTYPE_CODE and out.dtype is dtype
+            and (shape[0] > 0 and table_shape[0] > 0 and table_shape[1] > 0 or not out_shape[0])
             and k.dtype is v.dtype is torch.int8 and k_scales.dtype is v_scales.dtype is torch.float32
             and token_pos.dtype is token_seq.dtype is page_table.dtype is torch.int32
             and token_pos.numel() >= out_shape[0] <= token_seq.numel()
@@ -3198,6 +3201,7 @@ def attention_int8(q: torch.Tensor, q_stride: int, k: torch.Tensor, v: torch.Ten
             and token_pos.is_contiguous() and token_seq.is_contiguous() and page_table.is_contiguous()):
         code_of(dtype)
         n, page_size = out_shape[0] if out_shape else 0, shape[2] if len(shape) == 4 else 1
+        _need(not n or (k.numel() > 0 and page_table.numel() > 0), "attention_int8: a store and a page table of at least one page")
         _wanted("attention_int8", **_store8("attention_int8", k, v, k_scales, v_scales, kv_heads, d, page_size),
                 out=(out, dtype, (n, heads * d)), page_table=(page_table, torch.int32, (None, None)),
                 token_pos=(token_pos, torch.int32, token_pos.shape), token_seq=(token_seq, torch.int32, token_seq.shape))
@@ -3264,6 +3268,7 @@ def rmsnorm_int8_takes(width: int) -> bool:
 def rmsnorm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float, codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype) -> None:
     """``rmsnorm`` to ``dtype`` and ``quantize_rows`` in one: x float32 [n, width], a width of a multiple of 4 up to 8,192; codes int8 [n,
     int8_width(width)], scales float32 [n]."""
+    _need(x.dim() == 2, f"rmsnorm_int8: x [n, width]; got {tuple(x.shape)}")
     n, width = x.shape
     _need(rmsnorm_int8_takes(width) and eps > 0, f"rmsnorm_int8: a width of a multiple of 4 up to 8,192 and a positive eps; got {width}, {eps}")
     _wanted("rmsnorm_int8", x=(x, torch.float32, (n, width)), weight=(weight, torch.float32, (width,)),
@@ -3283,6 +3288,7 @@ def linear_int8_coded(codes: torch.Tensor, scales: torch.Tensor, k: int, w: torc
                       bias: Optional[torch.Tensor], out: torch.Tensor, mode: int) -> None:
     """``linear_int8`` of rows that are codes already (``rmsnorm_int8``, ``quantize_rows``): codes int8 [m, int8_width(k)], scales float32
     [m]; in the modes STORE and GEMM_GATED out is float32 or bfloat16."""
+    _need(codes.dim() == 2 == w.dim(), f"linear_int8_coded: codes [m, width] and w [rows, width]; got {tuple(codes.shape)} and {tuple(w.shape)}")
     m, rows = codes.shape[0], w.shape[0]
     n = rows // 2 if mode == GEMM_GATED else rows
     _need(mode in (STORE, STORE_F32, ADD_F32, GEMM_GATED) and 0 < k <= 133136 and (mode != GEMM_GATED or rows % 2 == 0) and n > 0,
@@ -3312,6 +3318,8 @@ def linear_int8(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, bias: 
     x's type [m, n]), STORE_F32 or ADD_F32 (float32 [m, n], written or added to), GEMM_GATED (w = [gate; up] rows, out of x's type [m, n /
     2] = silu(gate) * up).  k at most 133,136: beyond it a sum could pass 32 bits."""
     dtype = x.dtype
+    if not x.dim() == 2 == w.dim():
+        raise KernelError(f"linear_int8: x [m, k] and w [rows, width]; got {tuple(x.shape)} and {tuple(w.shape)}")
     (m, k), (rows, width) = x.shape, w.shape
     n = rows // 2 if mode == GEMM_GATED else rows
     kept = dtype if mode in (STORE, GEMM_GATED) else torch.float32

@@ -226,3 +226,34 @@ def test_norms_and_coded_rows_refuse():
                       ((codes, scales, 20, m, ms, None, empty(3, 12), 9), "mode 9")):
         with pytest.raises(ops.KernelError, match=why):
             ops.linear_int8_coded(*args)
+
+
+@pytest.mark.parametrize("change,why", [
+    (dict(window=1 << 31), "a window of 0 or more"), (dict(scale=float("inf")), "a positive scale"), (dict(scale=float("nan")), "a positive scale"),
+    (dict(table=empty(2, 0, dtype=I32)), "at least one page"), (dict(table=empty(0, 3, dtype=I32)), "at least one page"),
+    (dict(k=empty(0, 2, 64, 64, dtype=I8), v=empty(0, 2, 64, 64, dtype=I8), ks=empty(0, 2, 64), vs=empty(0, 2, 64)), "at least one page")])
+def test_attention_without_a_page_or_a_scale_is_refused(change, why, monkeypatch):
+    """(with the tensors taken for a GPU's: what is refused for where it lies is refused first)"""
+    from nnis_b200.csrc import ops
+    monkeypatch.setattr(ops, "_wanted", lambda what, **tensors: None)
+    with pytest.raises(ops.KernelError, match=why):
+        ops.attention_int8(*attend_args(**change))
+
+
+@pytest.mark.parametrize("change", [dict(table=empty(2, 0, dtype=I32)),
+                                    dict(k=empty(0, 1, 64, 64, dtype=I8), v=empty(0, 1, 64, 64, dtype=I8), ks=empty(0, 1, 64), vs=empty(0, 1, 64))])
+def test_writing_without_a_page_is_refused(change):
+    from nnis_b200.csrc import ops
+    with pytest.raises(ops.KernelError, match="at least one page"):
+        ops.rope_store_int8(*store_args(**change))
+
+
+def test_operands_of_other_ranks_are_refused():
+    from nnis_b200.csrc import ops
+    for change in (dict(x=empty(5, 1, 40, dtype=BF16)), dict(x=empty(40, dtype=BF16)), dict(w=empty(48, dtype=I8))):
+        with pytest.raises(ops.KernelError, match=r"x \[m, k\] and w"):
+            ops.linear_int8(*product_args(**change))
+    with pytest.raises(ops.KernelError, match=r"codes \[m, width\]"):
+        ops.linear_int8_coded(empty(48, dtype=I8), empty(1), 40, empty(12, 48, dtype=I8), empty(12), None, empty(1, 12), ops.STORE)
+    with pytest.raises(ops.KernelError, match=r"x \[n, width\]"):
+        ops.rmsnorm_int8(empty(64), empty(64), 1e-5, empty(1, 64, dtype=I8), empty(1), BF16)
