@@ -223,7 +223,7 @@ NNIS_API int nnis_rmsnorm_int8(const void* call) {
 // x [m, k] (rows `x_stride` apart) is put into `codes` [m, kp] and `scales` [m] (or, one row or two, into shared memory), w [n (gated: 2
 // n), kp] codes, ws their scales, bias float32 like ws or null, out [m, n]: `dtype` (x's) in the modes 0 (store) and 3 (gated: silu(first half of w's rows) * the
 // second), float32 in 1 (store) and 2 (add).  `coded`:
-// `codes` and `scales` are there already.
+// `codes` and `scales` are there already.  Both may be null for rows that go into shared memory.
 struct Linear8Call {
     const void *x, *w;
     const float *ws, *bias;
@@ -239,7 +239,7 @@ NNIS_API int nnis_linear_int8(const void* call) {
     memcpy(&c, call, sizeof c);
     const auto [x, w, ws, bias, out, codes, scales, status, x_stride, m, n, k, mode, dtype, sms, coded, stream] = c;
     const int kp = (k + 15) / 16 * 16;
-    if ((!x && !coded) || !w || !ws || !out || !codes || !scales || m <= 0 || n <= 0 || k <= 0 || (!coded && x_stride < k) || mode < 0 || mode > 3)
+    if ((!x && !coded) || !w || !ws || !out || (coded && (!codes || !scales)) || m <= 0 || n <= 0 || k <= 0 || (!coded && x_stride < k) || mode < 0 || mode > 3)
         return NNIS_ERR_ARGUMENT;
     if (k > 133136 || (dtype != NNIS_DTYPE_F32 && dtype != NNIS_DTYPE_BF16)) return NNIS_ERR_UNSUPPORTED;
     if (((uintptr_t)codes | (uintptr_t)w) % 16) return NNIS_ERR_ALIGNMENT;
@@ -247,6 +247,7 @@ NNIS_API int nnis_linear_int8(const void* call) {
     const Linear8 p{(const int8_t*)codes, (const int8_t*)w, scales, ws, bias, out, m, n, kp, status, 0, x, x_stride, k};
     const int held = sms > 0 ? sms : 148;
     if (!coded && linear_int8_fuses(p, mode == INT8_GATED, f32, held)) return (int)linear_int8_few(p, mode, f32, true, stream);
+    if (!codes || !scales) return NNIS_ERR_ARGUMENT;
     const Quantize8 q{x, x_stride, (int8_t*)codes, scales, m, k, kp, 0};
     const cudaError_t e = coded ? cudaSuccess : f32 ? launch_quantize<float>(q, stream) : launch_quantize<bf16>(q, stream);
     if (e != cudaSuccess) return (int)e;

@@ -67,10 +67,7 @@ def _stream() -> ctypes.c_void_p:
 # comes last, so that neither side pads the end): thirty arguments wrapped one by one cost the host 8 us, as plain numbers
 # 2.4, in a record 0.6.
 _ENTRY_FIELDS = {"nnis_copy_pages": "ppiiiiiipiip", "nnis_verify_drafts": "ppppppppiiippp",
-                 "nnis_attention_shared": "pippppipiiippppppiiiiiifiipp",
-                 "nnis_rope_store_int8": "pppppppppppiiiiiiiiiip", "nnis_read_pages_int8": "ppppppppiiiiiiiiip",
-                 "nnis_attention_int8": "ppppppppppppiiiiiiiiiifiiiiiip", "nnis_quantize_rows": "pppiiiip", "nnis_rmsnorm_int8": "ppppiiifp",
-                 "nnis_linear_int8": "ppppppppiiiiiiiip"}
+                 "nnis_attention_shared": "pippppipiiippppppiiiiiifiipp"}
 _entries = {}
 
 
@@ -3030,11 +3027,69 @@ def _store8(what: str, k, v, k_scales, v_scales, kv_heads: int, head_dim: int, p
             "v_scales": (v_scales, torch.float32, scales)}
 
 
-def _good(*wanted) -> bool:
-    """Whether every (tensor, dtype, shape) is a contiguous tensor of that kind on the first one's CUDA device."""
-    index = wanted[0][0].get_device()
-    return index >= 0 and all(t.dtype is dtype and t.shape == shape and t.get_device() == index and t.is_contiguous()
-                              for t, dtype, shape in wanted)
+# What the calls below take: the names of numbers that are given, then a line for every tensor: its name, its type ("any": float32 or
+# bfloat16, one of them in all of a call; "?": or None; ">n": packed, n elements or more, in any shape; "/s": rows at a distance of s elements,
+# others are packed), its sizes.  A name stands for one value in all lines (host_tensors.cu).  And the fields of each entry's record.
+_STORE8 = ("k int8 pages kv_heads page d", "v int8 pages kv_heads page d", "k_scales float32 pages kv_heads page",
+           "v_scales float32 pages kv_heads page")
+_CODED8 = ("codes int8 m coded", "scales float32 m", "w int8 rows width", "w_scales float32 rows", "bias float32? rows")
+_VALUES8 = ("x any/stride m k", "w int8 rows width", "w_scales float32 rows", "bias float32? rows")
+_CALLS8 = {
+    "rope_store_int8": ("kv_heads page d", *_STORE8, "qkv any n wide", "q any n q_wide", "token_pos int32>n", "token_seq int32>n",
+                        "page_table int32 seqs cols", "cos float32? angles half", "sin float32? angles half"),
+    "read_pages_int8": ("", *_STORE8, "page_table int32 seqs cols", "local_table int32 places columns", "k_out any outs kv_heads page d",
+                        "v_out any outs kv_heads page d"),
+    "attention_int8": ("kv_heads d", *_STORE8, "out any n wide", "q any/stride rows q_wide", "token_pos int32>n", "token_seq int32>n",
+                       "page_table int32 seqs cols"),
+    "quantize_rows": ("", "x any/stride rows k", "codes int8 rows width", "scales float32 rows"),
+    "rmsnorm_int8": ("", "x float32 n wide", "weight float32 wide", "codes int8 n width", "scales float32 n"),
+    "linear_int8": ("", *_VALUES8, "out any m n"), "linear_int8/float32": ("", *_VALUES8, "out float32 m n"),
+    "linear_int8_coded": ("", *_CODED8, "out any m n"), "linear_int8_coded/float32": ("", *_CODED8, "out float32 m n")}
+_RECORDS8 = {"nnis_rope_store_int8": "pppppppppppiiiiiiiiiip", "nnis_read_pages_int8": "ppppppppiiiiiiiiip",
+             "nnis_attention_int8": "ppppppppppppiiiiiiiiiifiiiiiip", "nnis_quantize_rows": "pppiiiip", "nnis_rmsnorm_int8": "ppppiiifp",
+             "nnis_linear_int8": "ppppppppiiiiiiiip"}
+_TYPES8 = {"any": 0, "float32": 1, "int8": 2, "int32": 3}
+_host_functions = {}
+
+
+def _described(given: str, *lines: str, device_type: int = 2) -> bytes:
+    """What ``_CALLS8`` says of a call in the bytes that the native check reads (devices by the exchange interface's numbers, 2: CUDA)."""
+    names = given.split()
+    count = len(names)
+
+    def symbol(name: str) -> int:
+        if name not in names:
+            names.append(name)
+        return names.index(name)
+
+    tensors = []
+    for line in lines:
+        _, kind, *sizes = line.split()
+        least, distance = kind.partition(">")[2], kind.partition("/")[2]
+        kind = kind.partition(">")[0].partition("/")[0]
+        sizes = [symbol(size) for size in ([least] if least else sizes)]
+        tensors.append(bytes((_TYPES8[kind.rstrip("?")], 1 if least else 2 if distance else 0, kind.endswith("?"), len(sizes), *sizes,
+                              *([symbol(distance)] if distance else []))))
+    return bytes((count, len(names), len(lines), device_type)) + b"".join(tensors)
+
+
+def _native(name: str):
+    """The native check of a call of ``_CALLS8`` (its result: None, or the device, the float type's code, the values of all names that
+    are not given, in the order of the lines, sizes before distances, and the addresses), or an entry of ``_RECORDS8``."""
+    lib = _build.load_locked()
+    if not _host_functions:
+        pointer = ctypes.pythonapi.PyCapsule_GetPointer
+        pointer.restype, pointer.argtypes = ctypes.c_void_p, [ctypes.py_object, ctypes.c_char_p]
+        capsule = getattr(torch.Tensor, "__dlpack_c_exchange_api__", None)
+        _need(capsule is not None, "this torch publishes no exchange interface for native code (torch.Tensor.__dlpack_c_exchange_api__)")
+        code = lib.nnis_tensors_begin(ctypes.c_void_p(pointer(capsule, b"dlpack_exchange_api")), ctypes.py_object(torch.Tensor))
+        _need(code == 0, "this torch's exchange interface for native code is not the one that the library was built for")
+        lib.nnis_host_function.restype = ctypes.py_object
+    entry = name in _RECORDS8
+    told = struct.pack("@P", ctypes.cast(getattr(_lib(), name), ctypes.c_void_p).value) + _RECORDS8[name].encode() + b"\0" if entry \
+        else _described(*_CALLS8[name])
+    _host_functions[name] = made = lib.nnis_host_function(ctypes.c_int(1 if entry else 0), ctypes.py_object(told))
+    return made
 
 
 def rope_store_int8(qkv: torch.Tensor, q: torch.Tensor, token_pos: torch.Tensor, token_seq: torch.Tensor, page_table: torch.Tensor,
@@ -3046,23 +3101,16 @@ def rope_store_int8(qkv: torch.Tensor, q: torch.Tensor, token_pos: torch.Tensor,
     2 kv_heads) * d] float32 or bfloat16 is left as it is.  ``cos`` and ``sin`` None: nothing is rotated.  A row at position -1, or
     beyond the angles, writes nothing; one whose page the table does not name stores nothing.  No two rows of a call have the same
     sequence and position."""
-    d, dtype, index, turns = head_dim, qkv.dtype, k.get_device(), cos is not None
-    shape, rows, q_shape, table_shape, per_head = k.shape, qkv.shape, q.shape, page_table.shape, k_scales.shape
-    n, half = rows[0] if rows else 0, cos.shape if turns else (0, d // 2)
-    if not (len(shape) == 4 and len(rows) == len(q_shape) == len(table_shape) == len(half) == 2 and shape[1] == kv_heads
-            and shape[2] == page_size and shape[3] == d and v.shape == shape and per_head == shape[:3] and v_scales.shape == per_head
-            and rows[1] == (heads + 2 * kv_heads) * d and q_shape[0] == n and q_shape[1] == heads * d
-            and 2 <= d <= 256 and d % 2 == 0 and heads > 0 and kv_heads > 0 and page_size > 0 and dtype in _DTYPE_CODE and q.dtype is dtype
-            and k.dtype is v.dtype is torch.int8 and k_scales.dtype is v_scales.dtype is torch.float32
-            and token_pos.dtype is token_seq.dtype is page_table.dtype is torch.int32
-            and token_pos.numel() >= n <= token_seq.numel() and (shape[0] > 0 and table_shape[0] > 0 and table_shape[1] > 0 or not n)
-            and 0 <= index == v.get_device() == k_scales.get_device() == v_scales.get_device() == q.get_device() == qkv.get_device()
-            == token_pos.get_device() == token_seq.get_device() == page_table.get_device()
-            and k.is_contiguous() and v.is_contiguous() and k_scales.is_contiguous() and v_scales.is_contiguous() and q.is_contiguous()
-            and qkv.is_contiguous() and token_pos.is_contiguous() and token_seq.is_contiguous() and page_table.is_contiguous()
-            and turns == (sin is not None)
-            and (not turns or (half[1] == d // 2 and sin.shape == half and cos.dtype is sin.dtype is torch.float32
-                               and cos.get_device() == sin.get_device() == index and cos.is_contiguous() and sin.is_contiguous()))):
+    d, turns = head_dim, cos is not None
+    facts = (_host_functions.get("rope_store_int8") or _native("rope_store_int8"))(
+        kv_heads, page_size, d, k, v, k_scales, v_scales, qkv, q, token_pos, token_seq, page_table, cos, sin)
+    if facts is not None:
+        (index, code, pages, n, wide, q_wide, seqs, cols, angles, half, at_k, at_v, at_ks, at_vs, at_qkv, at_q, at_pos, at_seq, at_table,
+         at_cos, at_sin) = facts
+    if facts is None or not (wide == (heads + 2 * kv_heads) * d and q_wide == heads * d and 2 <= d <= 256 and d % 2 == 0 and heads > 0
+                             and kv_heads > 0 and page_size > 0 and turns == (sin is not None) and (not turns or half == d // 2)
+                             and (pages > 0 and seqs > 0 and cols > 0 or not n)):
+        dtype, n, half = qkv.dtype, qkv.shape[0] if qkv.dim() else 0, cos.shape if turns else (0, d // 2)
         code_of(dtype)
         _need(heads > 0, "rope_store_int8: at least one query head")
         _need((cos is None) == (sin is None), "rope_store_int8: cos and sin, or neither")
@@ -3080,11 +3128,9 @@ def rope_store_int8(qkv: torch.Tensor, q: torch.Tensor, token_pos: torch.Tensor,
         with torch.cuda.device(index):
             return rope_store_int8(qkv, q, token_pos, token_seq, page_table, cos, sin, k, v, k_scales, v_scales, heads, kv_heads, d,
                                    page_size)
-    _check(_entry("nnis_rope_store_int8")(
-        qkv.data_ptr(), q.data_ptr(), token_pos.data_ptr(), token_seq.data_ptr(), page_table.data_ptr(),
-        cos.data_ptr() if turns else 0, sin.data_ptr() if turns else 0, k.data_ptr(), v.data_ptr(), k_scales.data_ptr(),
-        v_scales.data_ptr(), _DTYPE_CODE[dtype], table_shape[0], table_shape[1], half[0], shape[0], n, heads, kv_heads, d, page_size,
-        _stream_of(index)), "rope_store_int8")
+    _check((_host_functions.get("nnis_rope_store_int8") or _native("nnis_rope_store_int8"))(
+        at_qkv, at_q, at_pos, at_seq, at_table, at_cos, at_sin, at_k, at_v, at_ks, at_vs, code, seqs, cols, angles if turns else 0, pages, n,
+        heads, kv_heads, d, page_size, _stream_of(index)), "rope_store_int8")
 
 
 def read_pages_int8(k: torch.Tensor, v: torch.Tensor, k_scales: torch.Tensor, v_scales: torch.Tensor, page_table: torch.Tensor,
@@ -3094,32 +3140,26 @@ def read_pages_int8(k: torch.Tensor, v: torch.Tensor, k_scales: torch.Tensor, v_
     ``page_table`` names in the same place.  k, v int8 [pages, kv_heads, page_size, d], their scales float32 [pages, kv_heads,
     page_size]; k_out, v_out float32 or bfloat16 [out_pages, kv_heads, page_size, d].  A page id outside its store is passed over.
     No two places name the same page of the outputs."""
-    shape, places, table_shape, outs, dtype, index = k.shape, local_table.shape, page_table.shape, k_out.shape, k_out.dtype, k.get_device()
-    if not (len(shape) == len(outs) == 4 and len(places) == len(table_shape) == 2 and outs[1:] == shape[1:] and v.shape == shape
-            and v_out.shape == outs and k_scales.shape == shape[:3] and v_scales.shape == shape[:3] and shape[1] > 0 and shape[2] > 0
-            and 2 <= shape[3] <= 256 and shape[3] % 2 == 0
-            and table_shape[0] >= places[0] and table_shape[1] >= places[1] and dtype in _DTYPE_CODE and v_out.dtype is dtype
-            and k.dtype is v.dtype is torch.int8 and k_scales.dtype is v_scales.dtype is torch.float32
-            and page_table.dtype is local_table.dtype is torch.int32
-            and 0 <= index == v.get_device() == k_scales.get_device() == v_scales.get_device() == k_out.get_device() == v_out.get_device()
-            == page_table.get_device() == local_table.get_device()
-            and k.is_contiguous() and v.is_contiguous() and k_scales.is_contiguous() and v_scales.is_contiguous()
-            and k_out.is_contiguous() and v_out.is_contiguous() and page_table.is_contiguous() and local_table.is_contiguous()):
+    facts = (_host_functions.get("read_pages_int8") or _native("read_pages_int8"))(k, v, k_scales, v_scales, page_table, local_table, k_out, v_out)
+    if facts is not None:
+        (index, code, pages, kv_heads, page_size, d, seqs, cols, places, columns, outs, at_k, at_v, at_ks, at_vs, at_table, at_local, at_ko,
+         at_vo) = facts
+    if facts is None or not (kv_heads > 0 and page_size > 0 and 2 <= d <= 256 and d % 2 == 0 and seqs >= places and cols >= columns):
+        shape, outs, dtype = k.shape, k_out.shape, k_out.dtype
         code_of(dtype)
         _need(len(shape) == 4, f"read_pages_int8: k is int8 [pages, kv_heads, page_size, d]; got {tuple(shape)}")
         _wanted("read_pages_int8", **_store8("read_pages_int8", k, v, k_scales, v_scales, shape[1], shape[3], shape[2]),
                 page_table=(page_table, torch.int32, (None, None)), local_table=(local_table, torch.int32, (None, None)),
                 k_out=(k_out, dtype, (None, *shape[1:])), v_out=(v_out, dtype, (outs[0] if outs else 0, *shape[1:])))
         raise KernelError(f"read_pages_int8: local_table {tuple(local_table.shape)} reaches beyond page_table {tuple(page_table.shape)}")
-    if not local_table.numel() or not outs[0] or not k.numel():
+    if not places or not columns or not outs or not pages:
         return
     if _device_now() != index:
         with torch.cuda.device(index):
             return read_pages_int8(k, v, k_scales, v_scales, page_table, local_table, k_out, v_out)
-    _check(_entry("nnis_read_pages_int8")(
-        k.data_ptr(), v.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), page_table.data_ptr(), local_table.data_ptr(),
-        k_out.data_ptr(), v_out.data_ptr(), table_shape[1], places[0], places[1], _DTYPE_CODE[dtype], shape[0], outs[0], shape[1], shape[2],
-        shape[3], _stream_of(index)), "read_pages_int8")
+    _check((_host_functions.get("nnis_read_pages_int8") or _native("nnis_read_pages_int8"))(
+        at_k, at_v, at_ks, at_vs, at_table, at_local, at_ko, at_vo, cols, places, columns, code, pages, outs, kv_heads, page_size, d,
+        _stream_of(index)), "read_pages_int8")
 
 
 # A prompt step whose sequences bring at most this many tokens each attends over the codes row by row; others read their pages back and
@@ -3183,22 +3223,17 @@ def attention_int8(q: torch.Tensor, q_stride: int, k: torch.Tensor, v: torch.Ten
     heads * d] of its type.  A position whose page the table does not name, or beyond it, holds no key; a row that sees none (a
     padding row at position -1 among them) is zero.  Every row of a call reads its keys by itself: for single tokens and a few
     drafted ones (prompts read their pages back and take the kernels of the 16-bit cache)."""
-    # (checked in one expression: a call of its own for each tensor costs the host 3 us more)
-    d, dtype, index = head_dim, q.dtype, k.get_device()
-    shape, q_shape, out_shape, table_shape, per_head = k.shape, q.shape, out.shape, page_table.shape, k_scales.shape
-    if not (len(shape) == 4 and len(q_shape) == len(out_shape) == len(table_shape) == 2 and shape[1] == kv_heads and shape[3] == d
-            and v.shape == shape and per_head == shape[:3] and v_scales.shape == per_head and out_shape[1] == heads * d
-            and q_shape[0] >= out_shape[0] and q_shape[1] >= heads * d <= q_stride < 1 << 31 and q.stride() == (q_stride, 1)
-            and 2 <= d <= 256 and d % 2 == 0 and 0 < heads <= 65535 and kv_heads > 0 and heads % kv_heads == 0 and shape[2] > 0
-            and 0 <= window < 1 << 31 and 0 < scale < math.inf and dtype in _DTYPE_CODE and out.dtype is dtype
-            and (shape[0] > 0 and table_shape[0] > 0 and table_shape[1] > 0 or not out_shape[0])
-            and k.dtype is v.dtype is torch.int8 and k_scales.dtype is v_scales.dtype is torch.float32
-            and token_pos.dtype is token_seq.dtype is page_table.dtype is torch.int32
-            and token_pos.numel() >= out_shape[0] <= token_seq.numel()
-            and 0 <= index == v.get_device() == k_scales.get_device() == v_scales.get_device() == q.get_device() == out.get_device()
-            == token_pos.get_device() == token_seq.get_device() == page_table.get_device()
-            and k.is_contiguous() and v.is_contiguous() and k_scales.is_contiguous() and v_scales.is_contiguous() and out.is_contiguous()
-            and token_pos.is_contiguous() and token_seq.is_contiguous() and page_table.is_contiguous()):
+    d = head_dim
+    facts = (_host_functions.get("attention_int8") or _native("attention_int8"))(
+        kv_heads, d, k, v, k_scales, v_scales, out, q, token_pos, token_seq, page_table)
+    if facts is not None:
+        (index, code, pages, page_size, n, wide, rows, q_wide, stride, seqs, cols, at_k, at_v, at_ks, at_vs, at_out, at_q, at_pos, at_seq,
+         at_table) = facts
+    if facts is None or not (wide == heads * d <= q_wide and wide <= q_stride < 1 << 31 and rows >= n and (q_stride == stride or rows < 2)
+                             and 2 <= d <= 256 and d % 2 == 0 and 0 < heads <= 65535 and kv_heads > 0 and heads % kv_heads == 0
+                             and page_size > 0 and 0 <= window < 1 << 31 and 0 < scale < math.inf
+                             and (pages > 0 and seqs > 0 and cols > 0 or not n)):
+        dtype, shape, out_shape = q.dtype, k.shape, out.shape
         code_of(dtype)
         n, page_size = out_shape[0] if out_shape else 0, shape[2] if len(shape) == 4 else 1
         _need(not n or (k.numel() > 0 and page_table.numel() > 0), "attention_int8: a store and a page table of at least one page")
@@ -3210,29 +3245,31 @@ def attention_int8(q: torch.Tensor, q_stride: int, k: torch.Tensor, v: torch.Ten
             f"sequence for every row, and q [rows, heads * d] in rows of q_stride on the cache's device; got {heads} heads over "
             f"{kv_heads}, window {window}, scale {scale}, q {tuple(q.shape)} in strides {q.stride()} (q_stride {q_stride}) on "
             f"{q.device}, out {tuple(out.shape)}, {token_pos.numel()} positions, {token_seq.numel()} sequences")
-    n, pages, page_size, (seqs, cols) = out_shape[0], shape[0], shape[2], table_shape
     if n == 0:
         return
     if _device_now() != index:
         with torch.cuda.device(index):
             return attention_int8(q, q_stride, k, v, k_scales, v_scales, token_pos, token_seq, page_table, out, heads, kv_heads, d,
                                   window, scale, workspace)
-    tickets = status = slice_pieces = rows = cluster = eights = 0
-    at = k.data_ptr(), v.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), out.data_ptr()
-    if page_size == 64 and d in (32, 64, 96, 128) and not (at[0] | at[1] | at[2] | at[3] | at[4]) % 16:
-        splits, slice_pieces, rows, cluster, eights = attention_int8_plan(n, seqs, heads, kv_heads, d, cols, window, _sm_count.get(index) or sm_count(k.device))
+    tickets = status = slice_pieces = together = cluster = eights = 0
+    if page_size == 64 and d in (32, 64, 96, 128) and not (at_k | at_v | at_ks | at_vs | at_out) % 16:
+        splits, slice_pieces, together, cluster, eights = attention_int8_plan(n, seqs, heads, kv_heads, d, cols, window,
+                                                                              _sm_count.get(index) or sm_count(k.device))
         partial = workspace.room("attn_int8_records", n * heads * splits * (d + 4), torch.float32).data_ptr() if splits > 1 else 0
-        tickets = workspace.zeros_room("attn_int8_tickets", n * kv_heads * -(-rows * (heads // kv_heads) // 8), torch.int32).data_ptr() \
+        tickets = workspace.zeros_room("attn_int8_tickets", n * kv_heads * -(-together * (heads // kv_heads) // 8), torch.int32).data_ptr() \
             if splits > 1 else 0
-        status = status_word(k.device).data_ptr()
+        status = (_status[index] if index in _status else status_word(k.device)).data_ptr()
     else:
         keys = cols * page_size
         splits = attention_int8_splits(n, heads, min(keys, window) if window else keys, k.device)
         partial = workspace.room("attn_int8_partial", n * heads * splits * (d + 2), torch.float32).data_ptr() if splits > 1 else 0
-    _check(_entry("nnis_attention_int8")(
-        q.data_ptr(), at[0], at[1], at[2], at[3], token_pos.data_ptr(), token_seq.data_ptr(), page_table.data_ptr(), at[4], partial,
-        tickets, status, q_stride, seqs, cols, pages, n, heads, kv_heads, d, page_size, window, scale, splits, slice_pieces, rows, cluster, eights, _DTYPE_CODE[dtype], _stream_of(index)),
+    _check((_host_functions.get("nnis_attention_int8") or _native("nnis_attention_int8"))(
+        at_q, at_k, at_v, at_ks, at_vs, at_pos, at_seq, at_table, at_out, partial, tickets, status, q_stride, seqs, cols, pages, n, heads,
+        kv_heads, d, page_size, window, scale, splits, slice_pieces, together, cluster, eights, code, _stream_of(index)),
         "attention_int8", 2 if splits > 1 and not slice_pieces else 1)
+
+
+INT8_LONGEST = 133136  # places of K: beyond it a sum of products of codes could pass 32 bits
 
 
 def int8_width(k: int) -> int:
@@ -3244,21 +3281,23 @@ def quantize_rows(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor) ->
     """Every row of x [rows, k], float32 or bfloat16, in rows of any stride, as 8-bit codes rint(x * (127 / top)) and the scale top /
     127, top = max |x|: codes int8 [rows, int8_width(k)], scales float32 [rows].  A row of zeros has the scale zero; one that holds
     an infinity or a NaN has the scale NaN and codes of zero."""
-    code = code_of(x.dtype)
-    _need(x.dim() == 2 and (x.shape[1] == 1 or x.stride(1) == 1) and x.shape[1] > 0,
-          f"quantize_rows: x [rows, k >= 1], a row's values beside one another; got {tuple(x.shape)} in strides {x.stride()}")
-    rows, k = x.shape
-    _wanted("quantize_rows", codes=(codes, torch.int8, (rows, int8_width(k))), scales=(scales, torch.float32, (rows,)))
-    _need(codes.device == x.device, "quantize_rows: tensors on several devices")
+    facts = (_host_functions.get("quantize_rows") or _native("quantize_rows"))(x, codes, scales)
+    if facts is not None:
+        index, code, rows, k, stride, width, at_x, at_codes, at_scales = facts
+    if facts is None or not (k > 0 and width == int8_width(k)):
+        code_of(x.dtype)
+        _need(x.dim() == 2 and (x.shape[1] == 1 or x.stride(1) == 1) and x.shape[1] > 0,
+              f"quantize_rows: x [rows, k >= 1], a row's values beside one another; got {tuple(x.shape)} in strides {x.stride()}")
+        rows, k = x.shape
+        _wanted("quantize_rows", codes=(codes, torch.int8, (rows, int8_width(k))), scales=(scales, torch.float32, (rows,)))
+        raise KernelError("quantize_rows: tensors on several devices")
     if rows == 0:
         return
-    index = x.get_device()
     if _device_now() != index:
         with torch.cuda.device(index):
             return quantize_rows(x, codes, scales)
-    stride = x.stride(0) if rows > 1 else k
-    _check(_entry("nnis_quantize_rows")(x.data_ptr(), codes.data_ptr(), scales.data_ptr(), stride, code, rows, k, _stream_of(index)),
-           "quantize_rows")
+    _check((_host_functions.get("nnis_quantize_rows") or _native("nnis_quantize_rows"))(
+        at_x, at_codes, at_scales, stride, code, rows, k, _stream_of(index)), "quantize_rows")
 
 
 def rmsnorm_int8_takes(width: int) -> bool:
@@ -3268,46 +3307,54 @@ def rmsnorm_int8_takes(width: int) -> bool:
 def rmsnorm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float, codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype) -> None:
     """``rmsnorm`` to ``dtype`` and ``quantize_rows`` in one: x float32 [n, width], a width of a multiple of 4 up to 8,192; codes int8 [n,
     int8_width(width)], scales float32 [n]."""
-    _need(x.dim() == 2, f"rmsnorm_int8: x [n, width]; got {tuple(x.shape)}")
-    n, width = x.shape
-    _need(rmsnorm_int8_takes(width) and eps > 0, f"rmsnorm_int8: a width of a multiple of 4 up to 8,192 and a positive eps; got {width}, {eps}")
-    _wanted("rmsnorm_int8", x=(x, torch.float32, (n, width)), weight=(weight, torch.float32, (width,)),
-            codes=(codes, torch.int8, (n, int8_width(width))), scales=(scales, torch.float32, (n,)))
+    facts = (_host_functions.get("rmsnorm_int8") or _native("rmsnorm_int8"))(x, weight, codes, scales)
+    if facts is not None:
+        index, _, n, width, coded, at_x, at_weight, at_codes, at_scales = facts
+    if facts is None or not (rmsnorm_int8_takes(width) and eps > 0 and coded == int8_width(width)):
+        _need(x.dim() == 2, f"rmsnorm_int8: x [n, width]; got {tuple(x.shape)}")
+        n, width = x.shape
+        _need(rmsnorm_int8_takes(width) and eps > 0, f"rmsnorm_int8: a width of a multiple of 4 up to 8,192 and a positive eps; got {width}, {eps}")
+        _wanted("rmsnorm_int8", x=(x, torch.float32, (n, width)), weight=(weight, torch.float32, (width,)),
+                codes=(codes, torch.int8, (n, int8_width(width))), scales=(scales, torch.float32, (n,)))
+        raise KernelError("rmsnorm_int8: bad argument")
     code = code_of(dtype)
     if n == 0:
         return
-    index = x.get_device()
     if _device_now() != index:
         with torch.cuda.device(index):
             return rmsnorm_int8(x, weight, eps, codes, scales, dtype)
-    _check(_entry("nnis_rmsnorm_int8")(x.data_ptr(), weight.data_ptr(), codes.data_ptr(), scales.data_ptr(), n, width, code, eps,
-                                       _stream_of(index)), "rmsnorm_int8")
+    _check((_host_functions.get("nnis_rmsnorm_int8") or _native("nnis_rmsnorm_int8"))(
+        at_x, at_weight, at_codes, at_scales, n, width, code, eps, _stream_of(index)), "rmsnorm_int8")
 
 
 def linear_int8_coded(codes: torch.Tensor, scales: torch.Tensor, k: int, w: torch.Tensor, w_scales: torch.Tensor,
                       bias: Optional[torch.Tensor], out: torch.Tensor, mode: int) -> None:
     """``linear_int8`` of rows that are codes already (``rmsnorm_int8``, ``quantize_rows``): codes int8 [m, int8_width(k)], scales float32
     [m]; in the modes STORE and GEMM_GATED out is float32 or bfloat16."""
-    _need(codes.dim() == 2 == w.dim(), f"linear_int8_coded: codes [m, width] and w [rows, width]; got {tuple(codes.shape)} and {tuple(w.shape)}")
-    m, rows = codes.shape[0], w.shape[0]
-    n = rows // 2 if mode == GEMM_GATED else rows
-    _need(mode in (STORE, STORE_F32, ADD_F32, GEMM_GATED) and 0 < k <= 133136 and (mode != GEMM_GATED or rows % 2 == 0) and n > 0,
-          f"linear_int8_coded: mode {mode}, k {k}, {rows} rows of w")
-    kept = out.dtype if mode in (STORE, GEMM_GATED) else torch.float32
-    code = code_of(out.dtype)
-    _wanted("linear_int8_coded", codes=(codes, torch.int8, (m, int8_width(k))), scales=(scales, torch.float32, (m,)),
-            w=(w, torch.int8, (rows, int8_width(k))), w_scales=(w_scales, torch.float32, (rows,)), bias=(bias, torch.float32, (rows,)),
-            out=(out, kept, (m, n)))
+    name = "linear_int8_coded" if mode == STORE or mode == GEMM_GATED else "linear_int8_coded/float32"
+    facts = (_host_functions.get(name) or _native(name))(codes, scales, w, w_scales, bias, out)
+    if facts is not None:
+        index, code, m, coded, rows, width, n, at_codes, at_scales, at_w, at_ws, at_bias, at_out = facts
+    if facts is None or not (mode in (STORE, STORE_F32, ADD_F32, GEMM_GATED) and 0 < k <= INT8_LONGEST and coded == width == int8_width(k)
+                             and rows == (2 * n if mode == GEMM_GATED else n) and n > 0):
+        _need(codes.dim() == 2 == w.dim(), f"linear_int8_coded: codes [m, width] and w [rows, width]; got {tuple(codes.shape)} and {tuple(w.shape)}")
+        m, rows = codes.shape[0], w.shape[0]
+        n = rows // 2 if mode == GEMM_GATED else rows
+        _need(mode in (STORE, STORE_F32, ADD_F32, GEMM_GATED) and 0 < k <= INT8_LONGEST and (mode != GEMM_GATED or rows % 2 == 0) and n > 0,
+              f"linear_int8_coded: mode {mode}, k {k}, {rows} rows of w")
+        code_of(out.dtype)
+        _wanted("linear_int8_coded", codes=(codes, torch.int8, (m, int8_width(k))), scales=(scales, torch.float32, (m,)),
+                w=(w, torch.int8, (rows, int8_width(k))), w_scales=(w_scales, torch.float32, (rows,)), bias=(bias, torch.float32, (rows,)),
+                out=(out, out.dtype if mode in (STORE, GEMM_GATED) else torch.float32, (m, n)))
+        raise KernelError("linear_int8_coded: bad argument")
     if m == 0:
         return
-    index = w.get_device()
     if _device_now() != index:
         with torch.cuda.device(index):
             return linear_int8_coded(codes, scales, k, w, w_scales, bias, out, mode)
-    _check(_entry("nnis_linear_int8")(
-        0, w.data_ptr(), w_scales.data_ptr(), 0 if bias is None else bias.data_ptr(), out.data_ptr(), codes.data_ptr(), scales.data_ptr(),
-        status_word(w.device).data_ptr(), 0, m, n, k, mode, code, _sm_count.get(index) or sm_count(w.device), 1, _stream_of(index)),
-        "linear_int8_coded")
+    _check((_host_functions.get("nnis_linear_int8") or _native("nnis_linear_int8"))(
+        0, at_w, at_ws, at_bias, at_out, at_codes, at_scales, (_status[index] if index in _status else status_word(w.device)).data_ptr(), 0, m,
+        n, k, mode, max(code, F32), _sm_count.get(index) or sm_count(w.device), 1, _stream_of(index)), "linear_int8_coded")
 
 
 def linear_int8(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, bias: Optional[torch.Tensor], out: torch.Tensor, mode: int,
@@ -3317,36 +3364,33 @@ def linear_int8(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, bias: 
     one float32 product with each scale follows.  x [m, k] float32 or bfloat16, bias float32 [n] or None.  ``mode``: STORE (out of
     x's type [m, n]), STORE_F32 or ADD_F32 (float32 [m, n], written or added to), GEMM_GATED (w = [gate; up] rows, out of x's type [m, n /
     2] = silu(gate) * up).  k at most 133,136: beyond it a sum could pass 32 bits."""
-    dtype = x.dtype
-    if not x.dim() == 2 == w.dim():
-        raise KernelError(f"linear_int8: x [m, k] and w [rows, width]; got {tuple(x.shape)} and {tuple(w.shape)}")
-    (m, k), (rows, width) = x.shape, w.shape
-    n = rows // 2 if mode == GEMM_GATED else rows
-    kept = dtype if mode in (STORE, GEMM_GATED) else torch.float32
-    if not (dtype in _DTYPE_CODE and 0 < k <= 133136 and mode in (STORE, STORE_F32, ADD_F32, GEMM_GATED) and n > 0
-            and (mode != GEMM_GATED or rows % 2 == 0) and (k == 1 or x.stride(1) == 1) and x.get_device() == w.get_device()
-            and _good((w, torch.int8, (rows, int8_width(k))), (w_scales, torch.float32, (rows,)), (out, kept, (m, n)))
-            and (bias is None or _good((w, torch.int8, w.shape), (bias, torch.float32, (rows,))))):
-        code_of(dtype)
+    name = "linear_int8" if mode == STORE or mode == GEMM_GATED else "linear_int8/float32"
+    facts = (_host_functions.get(name) or _native(name))(x, w, w_scales, bias, out)
+    if facts is not None:
+        index, code, m, k, stride, rows, width, n, at_x, at_w, at_ws, at_bias, at_out = facts
+    if facts is None or not (mode in (STORE, STORE_F32, ADD_F32, GEMM_GATED) and 0 < k <= INT8_LONGEST and width == -(-k // 16) * 16
+                             and rows == (2 * n if mode == GEMM_GATED else n) and n > 0):
+        _need(x.dim() == 2 == w.dim(), f"linear_int8: x [m, k] and w [rows, width]; got {tuple(x.shape)} and {tuple(w.shape)}")
+        (m, k), rows = x.shape, w.shape[0]
+        code_of(x.dtype)
         _need(mode in (STORE, STORE_F32, ADD_F32, GEMM_GATED), f"linear_int8: mode {mode}")
         _need(mode != GEMM_GATED or rows % 2 == 0, f"linear_int8: {rows} rows are no gate and up")
         _wanted("linear_int8", w=(w, torch.int8, (rows, int8_width(k))), w_scales=(w_scales, torch.float32, (rows,)),
-                bias=(bias, torch.float32, (rows,)), out=(out, kept, (m, n)))
-        raise KernelError(f"linear_int8: x [m, k] with 0 < k <= 133136 and a row's values beside one another, on w's device; got "
+                bias=(bias, torch.float32, (rows,)), out=(out, x.dtype if mode in (STORE, GEMM_GATED) else torch.float32,
+                                                          (m, rows // 2 if mode == GEMM_GATED else rows)))
+        raise KernelError(f"linear_int8: x [m, k] with 0 < k <= {INT8_LONGEST} and a row's values beside one another, on w's device; got "
                           f"{tuple(x.shape)} in strides {x.stride()} on {x.device}")
     if m == 0:
         return
-    index = w.get_device()
     if _device_now() != index:
         with torch.cuda.device(index):
             return linear_int8(x, w, w_scales, bias, out, mode, workspace)
     sms = _sm_count.get(index) or sm_count(w.device)
     # (what the library does: one or two rows become codes in the product's own kernel)
-    fused = m <= 2 and -(-n // (8 if mode == GEMM_GATED else 16)) <= sms and width <= 16384 and k % 8 == 0 \
-        and (m == 1 or x.stride(0) % 8 == 0) and x.data_ptr() % (16 if dtype == torch.float32 else 8) == 0
-    codes = workspace.room("int8_codes", m * width, torch.int8)
-    scales = workspace.room("int8_scales", m, torch.float32)
-    _check(_entry("nnis_linear_int8")(
-        x.data_ptr(), w.data_ptr(), w_scales.data_ptr(), 0 if bias is None else bias.data_ptr(), out.data_ptr(), codes.data_ptr(),
-        scales.data_ptr(), status_word(w.device).data_ptr(), x.stride(0) if m > 1 else k, m, n, k, mode, _DTYPE_CODE[dtype],
-        sms, 0, _stream_of(index)), "linear_int8", 1 if fused else 2)
+    fused = m <= 2 and -(-n // (8 if mode == GEMM_GATED else 16)) <= sms and width <= 16384 and k % 8 == 0 and stride % 8 == 0 \
+        and at_x % (16 if code == F32 else 8) == 0
+    codes = 0 if fused else workspace.room("int8_codes", m * width, torch.int8).data_ptr()
+    scales = 0 if fused else workspace.room("int8_scales", m, torch.float32).data_ptr()
+    _check((_host_functions.get("nnis_linear_int8") or _native("nnis_linear_int8"))(
+        at_x, at_w, at_ws, at_bias, at_out, codes, scales, (_status[index] if index in _status else status_word(w.device)).data_ptr(), stride,
+        m, n, k, mode, code, sms, 0, _stream_of(index)), "linear_int8", 1 if fused else 2)

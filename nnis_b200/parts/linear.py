@@ -29,6 +29,8 @@ class Int8Matrix:
     @classmethod
     def of(cls, weight: torch.Tensor) -> "Int8Matrix":
         n, k = weight.shape
+        if k > ops.INT8_LONGEST:
+            raise ValueError(f"an 8-bit matrix has up to {ops.INT8_LONGEST} columns; got {k}")
         codes = torch.empty((n, ops.int8_width(k)), dtype=torch.int8, device=weight.device)
         scales = torch.empty(n, dtype=torch.float32, device=weight.device)
         ops.quantize_rows(weight, codes, scales)

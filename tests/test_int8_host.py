@@ -257,3 +257,123 @@ def test_operands_of_other_ranks_are_refused():
         ops.linear_int8_coded(empty(48, dtype=I8), empty(1), 40, empty(12, 48, dtype=I8), empty(12), None, empty(1, 12), ops.STORE)
     with pytest.raises(ops.KernelError, match=r"x \[n, width\]"):
         ops.rmsnorm_int8(empty(64), empty(64), 1e-5, empty(1, 64, dtype=I8), empty(1), BF16)
+
+
+@pytest.fixture
+def reached(monkeypatch):
+    """Entries that were reached, with the operators' native checks taking the CPU's tensors for a GPU's and nothing launched."""
+    import ctypes
+    from nnis_b200.csrc import ops
+    calls, lib = [], None
+    ops._native("quantize_rows")
+    lib = ops._build.load_locked()
+    functions = {name: lib.nnis_host_function(ctypes.c_int(0), ctypes.py_object(ops._described(*lines, device_type=1)))
+                 for name, lines in ops._CALLS8.items()}
+    for name in ops._RECORDS8:
+        functions[name] = lambda *values, name=name: calls.append((name, values)) or 0
+    monkeypatch.setattr(ops, "_host_functions", functions)
+    monkeypatch.setattr(ops, "_device_now", lambda: 0)
+    monkeypatch.setattr(ops, "_stream_of", lambda index: 77)
+    monkeypatch.setitem(ops._sm_count, 0, 148)
+    monkeypatch.setattr(ops, "_status", {0: torch.zeros(1, dtype=I32)})
+    return calls
+
+
+def space():
+    from nnis_b200.engine.workspace import Workspace
+    return Workspace(torch.device("cpu"))
+
+
+def coded_args(**change):
+    a = dict(codes=empty(5, 48, dtype=I8), scales=empty(5), k=40, w=empty(12, 48, dtype=I8), ws=empty(12), bias=None, out=empty(5, 12, dtype=BF16), mode=0)
+    a.update(change)
+    return list(a.values())
+
+
+def test_what_fits_is_passed_on(reached):
+    from nnis_b200.csrc import ops
+    at = lambda *tensors: tuple(t.data_ptr() for t in tensors)
+    qkv, q, pos, seq, table, cos, sin, k, v, ks, vs = a = store_args()[:11]
+    ops.rope_store_int8(*store_args(**dict(zip(("qkv", "q", "pos", "seq", "table", "cos", "sin", "k", "v", "ks", "vs"), a))))
+    assert reached.pop() == ("nnis_rope_store_int8", (*at(*a), 1, 2, 3, 9, 4, 5, 3, 1, 64, 64, 77))
+    ops.rope_store_int8(*store_args(cos=None, sin=None, k=k, qkv=empty(5, 320), q=empty(5, 192)))
+    assert reached.pop()[1][5:8] == (0, 0, k.data_ptr())
+    k, v, ks, vs, table, local, ko, vo = a = read_args(ko=empty(5, 2, 64, 64), vo=empty(5, 2, 64, 64))
+    ops.read_pages_int8(*a)
+    assert reached.pop() == ("nnis_read_pages_int8", (*at(*a), 3, 2, 3, 0, 4, 5, 2, 64, 64, 77))
+    wide = empty(7, 500, dtype=BF16)
+    for queries, stride, page in ((wide[:, 8:392], 500, 64), (wide[:1, 8:392], 999, 64), (empty(5, 384, dtype=BF16), 384, 16)):
+        n = min(5, queries.shape[0])
+        store = dict(k=empty(4, 2, page, 64, dtype=I8), v=empty(4, 2, page, 64, dtype=I8), ks=empty(4, 2, page), vs=empty(4, 2, page))
+        a = attend_args(q=queries, stride=stride, out=empty(n, 384, dtype=BF16), ws=space(), **store)
+        ops.attention_int8(*a)
+        name, got = reached.pop()
+        assert name == "nnis_attention_int8" and got[:5] == at(queries, *a[2:6]) and got[12:22] == (stride, 2, 3, 4, n, 6, 2, 64, page, 0)
+        assert got[5:9] == at(a[6], a[7], a[8], a[9]) and got[22] == 0.125 and got[-2:] == (1, 77) and (got[24] > 0) == (page == 64)
+    x = empty(5, 50, dtype=BF16)[:, :40]
+    for change, want in ((dict(), (50, 5, 12, 40, 0, 1, 148, 0, 77)), (dict(mode=2, out=empty(5, 12)), (50, 5, 12, 40, 2, 1, 148, 0, 77)),
+                         (dict(mode=3, out=empty(5, 6, dtype=BF16), bias=empty(12)), (50, 5, 6, 40, 3, 1, 148, 0, 77)),
+                         (dict(x=empty(1, 40), out=empty(1, 12)), (40, 1, 12, 40, 0, 0, 148, 0, 77))):
+        a = product_args(**{"x": x, "space": space(), **change})
+        ops.linear_int8(*a)
+        name, got = reached.pop()
+        assert name == "nnis_linear_int8" and got[8:] == want and got[:3] == at(a[0], a[1], a[2]) and got[4] == a[4].data_ptr()
+        assert got[3] == (a[3].data_ptr() if a[3] is not None else 0) and (got[5] == 0) == (want[1] == 1)
+    for change, want in ((dict(), (0, 5, 12, 40, 0, 1, 148, 1, 77)), (dict(mode=1, out=empty(5, 12)), (0, 5, 12, 40, 1, 0, 148, 1, 77))):
+        ops.linear_int8_coded(*coded_args(**change))
+        assert reached.pop()[1][8:] == want
+    ops.quantize_rows(x, empty(5, 48, dtype=I8), empty(5))
+    assert reached.pop()[1][3:] == (50, 1, 5, 40, 77)
+    ops.rmsnorm_int8(empty(5, 40), empty(40), 1e-5, empty(5, 48, dtype=I8), empty(5), BF16)
+    assert reached.pop()[1][4:] == (5, 40, 1, 1e-5, 77)
+    ops.linear_int8(*product_args(x=empty(0, 40, dtype=BF16), out=empty(0, 12, dtype=BF16)))
+    ops.attention_int8(*attend_args(q=empty(0, 384, dtype=BF16), out=empty(0, 384, dtype=BF16)))
+    assert not reached
+
+
+REFUSED = [("rope_store_int8", store_args, change) for change, _ in test_writing_refuses.pytestmark[0].args[1] if change] + \
+    [("read_pages_int8", read_args, change) for change, _ in test_reading_refuses.pytestmark[0].args[1] if change] + \
+    [("attention_int8", attend_args, change) for change, _ in test_attention_refuses.pytestmark[0].args[1] if change] + \
+    [("attention_int8", attend_args, change) for change, _ in test_attention_without_a_page_or_a_scale_is_refused.pytestmark[0].args[1]] + \
+    [("rope_store_int8", store_args, change) for change in test_writing_without_a_page_is_refused.pytestmark[0].args[1]] + \
+    [("linear_int8", product_args, change) for change, _ in test_products_refuse.pytestmark[0].args[1] if change] + \
+    [("rope_store_int8", store_args, change) for change in (
+        dict(cos=None), dict(cos=empty(9, 32).double()), dict(v=empty(4, 1, 64, 64, dtype=I8).transpose(2, 3)), dict(k=None), dict(pos=None),
+        dict(heads=2), dict(page=32), dict(table=empty(3, 2, dtype=I32).t()), dict(qkv=[[0.0]]))] + \
+    [("read_pages_int8", read_args, change) for change in (
+        dict(local=empty(3, 3, dtype=I32)), dict(local=empty(2, 4, dtype=I32)), dict(ko=empty(5, 2, 64, 64)), dict(table=empty(2, 6, dtype=I32)[:, ::2]))] + \
+    [("attention_int8", attend_args, change) for change in (
+        dict(stride=383), dict(stride=385), dict(heads=5), dict(heads=7), dict(kv_heads=3), dict(window=-1), dict(scale=0.0), dict(scale=-1.0),
+        dict(d=32), dict(q=empty(4, 384, dtype=BF16)), dict(q=empty(5, 768, dtype=BF16)[:, ::2], stride=768), dict(pos=empty(4, dtype=I32)),
+        dict(out=empty(5, 768, dtype=BF16)[:, :384]), dict(vs=empty(2, 4, 64).transpose(0, 1)))] + \
+    [("linear_int8", product_args, change) for change in (
+        dict(mode=4), dict(mode=1), dict(mode=3), dict(mode=0.5), dict(w=empty(12, 40, dtype=I8)), dict(w=empty(12, 64, dtype=I8)), dict(bias=empty(11)),
+        dict(bias=empty(12, dtype=BF16)), dict(x=empty(40, 5, dtype=BF16).t()), dict(ws=empty(24)[::2]), dict(out=empty(12, 5, dtype=BF16).t()))] + \
+    [("linear_int8_coded", coded_args, change) for change in (
+        dict(k=0), dict(k=50), dict(k=32), dict(k=133137), dict(mode=1), dict(mode=3), dict(mode=7), dict(codes=empty(5, 64, dtype=I8)),
+        dict(scales=empty(6)), dict(out=empty(4, 12, dtype=BF16)), dict(w=empty(12, 48)))]
+
+
+@pytest.mark.parametrize("name,args,change", REFUSED, ids=[f"{name}-{i}" for i, (name, _, _) in enumerate(REFUSED)])
+def test_what_does_not_fit_reaches_no_entry(reached, name, args, change):
+    from nnis_b200.csrc import ops
+    with pytest.raises((ops.KernelError, AttributeError, TypeError)):
+        getattr(ops, name)(*args(**change))
+    assert not reached
+
+
+def test_records_refuse_values_that_are_not_a_field_s():
+    """The native caller of an entry: an entry that is not reached cannot fault, so a refusing one is called with no addresses."""
+    from nnis_b200.csrc import ops
+    call = ops._native("nnis_quantize_rows")
+    assert call(0, 0, 0, 1, 1, 1, 1, 0) == -1 == call(0, 0, 0, 1 << 31, 1, 1, 1, 0) == call(0, 0, 0, 1) == call(0, 0, 0, "1", 1, 1, 1, 0)
+    assert call(0, 0, 0, 1.5, 1, 1, 1, 0) == -1 == call(0, 0, 0, 1, 1, 1, 1, 0, 0)
+    norm = ops._native("nnis_rmsnorm_int8")
+    assert norm(0, 0, 0, 0, 1, 8, 1, "x", 0) == -1 == norm(0, 0, 0, 0, 1, 8, 1, 1e-5, 0)
+
+
+def test_a_matrix_with_too_many_columns_is_refused():
+    from nnis_b200.csrc import ops
+    from nnis_b200.parts.linear import Int8Matrix
+    with pytest.raises(ValueError, match="up to 133136 columns"):
+        Int8Matrix.of(empty(1, ops.INT8_LONGEST + 1, dtype=BF16))
