@@ -76,6 +76,42 @@ __global__ void __launch_bounds__(128) quantize_rows_kernel(const __grid_constan
     release_late(p);
 }
 
+// Rows of odd lengths or at odd addresses: a CTA each, the row's values in registers, CHUNKS runs of four a thread.
+template <typename T, int CHUNKS>
+__global__ void __launch_bounds__(128) quantize_rows_odd_kernel(const __grid_constant__ Quantize8 p) {
+    __shared__ uint32_t tops[4];
+    pdl_wait();
+    release_early(p);
+    const T* x = reinterpret_cast<const T*>(p.x) + (size_t)blockIdx.x * p.x_stride;
+    float v[CHUNKS][4];
+    uint32_t top = 0;
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int i = (c * 128 + threadIdx.x) * 4 + j;
+            v[c][j] = i < p.k ? to_float(x[i]) : 0.f;
+        }
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) top = max(top, magnitude_bits(v[c][j]));
+    top = group_max<32>(top);
+    if (threadIdx.x % 32 == 0) tops[threadIdx.x / 32] = top;
+    __syncthreads();
+    top = max(max(tops[0], tops[1]), max(tops[2], tops[3]));
+    const RowScale r = row_scale(top);
+    const uint32_t good = good_row(r.scale);
+    int8_t* codes = p.codes + (size_t)blockIdx.x * p.kp;
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) {
+        const int i = (c * 128 + threadIdx.x) * 4;
+        if (i < p.kp) *reinterpret_cast<uint32_t*>(codes + i) = code_word(v[c][0], v[c][1], v[c][2], v[c][3], r.inverse, good);
+    }
+    if (threadIdx.x == 0) p.scales[blockIdx.x] = r.scale;
+    release_late(p);
+}
+
 // Any row: a CTA each, read twice.
 template <typename T>
 __global__ void __launch_bounds__(128) quantize_rows_any_kernel(const __grid_constant__ Quantize8 p) {
@@ -164,6 +200,11 @@ static cudaError_t launch_rmsnorm8(const float* x, const float* w, int8_t* codes
 template <typename T>
 static cudaError_t launch_quantize(const Quantize8& p, cudaStream_t stream) {
     const bool eights = p.k % 8 == 0 && p.x_stride % 8 == 0 && (uintptr_t)p.x % (4 * sizeof(T)) == 0;
+    if (!eights && p.kp <= 4096) {
+        auto kernel = p.kp <= 1024 ? quantize_rows_odd_kernel<T, 2> : p.kp <= 2048 ? quantize_rows_odd_kernel<T, 4>
+                      : quantize_rows_odd_kernel<T, 8>;
+        return launch_dependent(kernel, (unsigned)p.rows, 128, 0, stream, p);
+    }
     if (!eights || p.kp > 8192) return launch_dependent(quantize_rows_any_kernel<T>, (unsigned)p.rows, 128, 0, stream, p);
     // (a warp a row up to 1,024 values, and up to 2,048 where rows are many)
     if (p.kp <= 1024 || (p.kp <= 2048 && p.rows >= 1024)) {

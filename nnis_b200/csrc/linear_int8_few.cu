@@ -32,8 +32,11 @@ __device__ __forceinline__ void few_mma(int (&c)[4], uint32_t a0, uint32_t a1, u
 constexpr int kFusedRows = 2;
 // NT: tiles of 8 rows of x; kFewWarps: 8, or 16 where there are fewer CTAs than SMs and a long K.
 // X: the type of x where its rows are still values (fused), int8_t where they are codes.
+// (up to eight rows of codes: registers for three CTAs an SM, which is asked for: 80 where the compiler takes 70 by itself and keeps fewer loads
+// ahead.  8 rows, us without / with: gate and up 16,384 x 2,048 10.2 / 9.8, 576 x 1,536 3.5 / 3.1, 32,768 x 2,048 16.0 / 15.2.  A CTA that walks
+// over tiles with the next one's loads ahead: 10.9, 3.6, 16.8)
 template <typename T, bool ADD, bool GATED, int NT, int kFewWarps, typename X = int8_t>
-__global__ void __launch_bounds__(kFewWarps * 32) linear_int8_few_kernel(const __grid_constant__ Linear8 p) {
+__global__ void __launch_bounds__(kFewWarps * 32, kFewWarps == 8 && NT == 1 && std::is_same<X, int8_t>::value ? 3 : 0) linear_int8_few_kernel(const __grid_constant__ Linear8 p) {
     constexpr int kAhead = 4, kOut = GATED ? 8 : 16;  // runs of K that a lane has asked for; outputs of a CTA and row of x
     constexpr bool kFused = !std::is_same<X, int8_t>::value;
     __shared__ int sums[kFewWarps][NT * 128];
