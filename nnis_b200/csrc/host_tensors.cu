@@ -140,8 +140,8 @@ bool places(const unsigned char* what, int device_type, int tensors, void* const
 }
 
 // self: bytes, the numbers of symbols that are given, of all symbols and of tensors, the type of device, then the tensors' descriptions.  Called with the given
-// symbols' values and the tensors.  None where something does not fit, else (device, float type or -1, the other symbols' values, the
-// tensors' addresses).  One that is None counts for nothing but an address of 0.
+// symbols' values and the tensors.  None where something does not fit, else (device, torch's current stream there or -1 where another device is the
+// current one, float type or -1, the other symbols' values, the tensors' addresses).  One that is None counts for nothing but an address of 0.
 void* check(void* self, void* const* args, long count) {
     const unsigned char* what = reinterpret_cast<const unsigned char*>(py().bytes(self));
     const int given = what[0], all = what[1], tensors = what[2];
@@ -158,7 +158,14 @@ void* check(void* self, void* const* args, long count) {
         if (py().error()) py().clear();
         return none();
     }
-    void* facts = py().new_tuple(2 + all - given + tensors);
+    void* stream = nullptr;
+    int current = (int)device;
+    const bool here = what[3] != 2 || (cudaGetDevice(&current) == cudaSuccess && current == (int)device);
+    if (what[3] == 2 && here && exchange->stream(2, (int32_t)device, &stream) != 0) {
+        py().clear();
+        return none();
+    }
+    void* facts = py().new_tuple(3 + all - given + tensors);
     if (!facts) return nullptr;
     long n = 0;
     auto put = [&](long long v) {
@@ -166,7 +173,7 @@ void* check(void* self, void* const* args, long count) {
         if (number) py().set_item(facts, n++, number);
         return number != nullptr;
     };
-    bool whole = put(device) && put(dtype);
+    bool whole = put(device) && put(here ? reinterpret_cast<long long>(stream) : -1) && put(dtype);
     for (int i = given; whole && i < all; ++i) whole = put(symbols[i] == kUnbound ? -1 : symbols[i]);
     for (int i = 0; whole && i < tensors; ++i) whole = put(at[i]);
     if (whole) return facts;
@@ -226,7 +233,7 @@ void* call(void* self, void* const* args, long count) {
 // Once, before the others, with the interpreter's lock held: the address of the exchange interface and the class of tensors.
 NNIS_API int nnis_tensors_begin(void* interface, void* tensors) {
     const Exchange* e = static_cast<const Exchange*>(interface);
-    if (!py().found || !e || e->major != 1 || e->minor < 3 || !e->describe || !tensors) return NNIS_ERR_UNSUPPORTED;
+    if (!py().found || !e || e->major != 1 || e->minor < 3 || !e->describe || !e->stream || !tensors) return NNIS_ERR_UNSUPPORTED;
     py().hold(tensors);
     exchange = e;
     tensor_class = tensors;

@@ -3074,7 +3074,8 @@ def _described(given: str, *lines: str, device_type: int = 2) -> bytes:
 
 
 def _native(name: str):
-    """The native check of a call of ``_CALLS8`` (its result: None, or the device, the float type's code, the values of all names that
+    """The native check of a call of ``_CALLS8`` (its result: None, or the device, the current stream there, -1 where
+    another device is the current one, the float type's code, the values of all names that
     are not given, in the order of the lines, sizes before distances, and the addresses), or an entry of ``_RECORDS8``."""
     lib = _build.load_locked()
     if not _host_functions:
@@ -3105,7 +3106,7 @@ def rope_store_int8(qkv: torch.Tensor, q: torch.Tensor, token_pos: torch.Tensor,
     facts = (_host_functions.get("rope_store_int8") or _native("rope_store_int8"))(
         kv_heads, page_size, d, k, v, k_scales, v_scales, qkv, q, token_pos, token_seq, page_table, cos, sin)
     if facts is not None:
-        (index, code, pages, n, wide, q_wide, seqs, cols, angles, half, at_k, at_v, at_ks, at_vs, at_qkv, at_q, at_pos, at_seq, at_table,
+        (index, stream, code, pages, n, wide, q_wide, seqs, cols, angles, half, at_k, at_v, at_ks, at_vs, at_qkv, at_q, at_pos, at_seq, at_table,
          at_cos, at_sin) = facts
     if facts is None or not (wide == (heads + 2 * kv_heads) * d and q_wide == heads * d and 2 <= d <= 256 and d % 2 == 0 and heads > 0
                              and kv_heads > 0 and page_size > 0 and turns == (sin is not None) and (not turns or half == d // 2)
@@ -3124,13 +3125,13 @@ def rope_store_int8(qkv: torch.Tensor, q: torch.Tensor, token_pos: torch.Tensor,
         raise KernelError("rope_store_int8: bad argument")
     if n == 0:
         return
-    if _device_now() != index:
+    if stream < 0:  # (another device is the current one)
         with torch.cuda.device(index):
             return rope_store_int8(qkv, q, token_pos, token_seq, page_table, cos, sin, k, v, k_scales, v_scales, heads, kv_heads, d,
                                    page_size)
     _check((_host_functions.get("nnis_rope_store_int8") or _native("nnis_rope_store_int8"))(
         at_qkv, at_q, at_pos, at_seq, at_table, at_cos, at_sin, at_k, at_v, at_ks, at_vs, code, seqs, cols, angles if turns else 0, pages, n,
-        heads, kv_heads, d, page_size, _stream_of(index)), "rope_store_int8")
+        heads, kv_heads, d, page_size, stream), "rope_store_int8")
 
 
 def read_pages_int8(k: torch.Tensor, v: torch.Tensor, k_scales: torch.Tensor, v_scales: torch.Tensor, page_table: torch.Tensor,
@@ -3142,7 +3143,7 @@ def read_pages_int8(k: torch.Tensor, v: torch.Tensor, k_scales: torch.Tensor, v_
     No two places name the same page of the outputs."""
     facts = (_host_functions.get("read_pages_int8") or _native("read_pages_int8"))(k, v, k_scales, v_scales, page_table, local_table, k_out, v_out)
     if facts is not None:
-        (index, code, pages, kv_heads, page_size, d, seqs, cols, places, columns, outs, at_k, at_v, at_ks, at_vs, at_table, at_local, at_ko,
+        (index, stream, code, pages, kv_heads, page_size, d, seqs, cols, places, columns, outs, at_k, at_v, at_ks, at_vs, at_table, at_local, at_ko,
          at_vo) = facts
     if facts is None or not (kv_heads > 0 and page_size > 0 and 2 <= d <= 256 and d % 2 == 0 and seqs >= places and cols >= columns):
         shape, outs, dtype = k.shape, k_out.shape, k_out.dtype
@@ -3154,12 +3155,12 @@ def read_pages_int8(k: torch.Tensor, v: torch.Tensor, k_scales: torch.Tensor, v_
         raise KernelError(f"read_pages_int8: local_table {tuple(local_table.shape)} reaches beyond page_table {tuple(page_table.shape)}")
     if not places or not columns or not outs or not pages:
         return
-    if _device_now() != index:
+    if stream < 0:  # (another device is the current one)
         with torch.cuda.device(index):
             return read_pages_int8(k, v, k_scales, v_scales, page_table, local_table, k_out, v_out)
     _check((_host_functions.get("nnis_read_pages_int8") or _native("nnis_read_pages_int8"))(
         at_k, at_v, at_ks, at_vs, at_table, at_local, at_ko, at_vo, cols, places, columns, code, pages, outs, kv_heads, page_size, d,
-        _stream_of(index)), "read_pages_int8")
+        stream), "read_pages_int8")
 
 
 # A prompt step whose sequences bring at most this many tokens each attends over the codes row by row; others read their pages back and
@@ -3227,7 +3228,7 @@ def attention_int8(q: torch.Tensor, q_stride: int, k: torch.Tensor, v: torch.Ten
     facts = (_host_functions.get("attention_int8") or _native("attention_int8"))(
         kv_heads, d, k, v, k_scales, v_scales, out, q, token_pos, token_seq, page_table)
     if facts is not None:
-        (index, code, pages, page_size, n, wide, rows, q_wide, stride, seqs, cols, at_k, at_v, at_ks, at_vs, at_out, at_q, at_pos, at_seq,
+        (index, stream, code, pages, page_size, n, wide, rows, q_wide, stride, seqs, cols, at_k, at_v, at_ks, at_vs, at_out, at_q, at_pos, at_seq,
          at_table) = facts
     if facts is None or not (wide == heads * d <= q_wide and wide <= q_stride < 1 << 31 and rows >= n and (q_stride == stride or rows < 2)
                              and 2 <= d <= 256 and d % 2 == 0 and 0 < heads <= 65535 and kv_heads > 0 and heads % kv_heads == 0
@@ -3247,7 +3248,7 @@ def attention_int8(q: torch.Tensor, q_stride: int, k: torch.Tensor, v: torch.Ten
             f"{q.device}, out {tuple(out.shape)}, {token_pos.numel()} positions, {token_seq.numel()} sequences")
     if n == 0:
         return
-    if _device_now() != index:
+    if stream < 0:  # (another device is the current one)
         with torch.cuda.device(index):
             return attention_int8(q, q_stride, k, v, k_scales, v_scales, token_pos, token_seq, page_table, out, heads, kv_heads, d,
                                   window, scale, workspace)
@@ -3265,7 +3266,7 @@ def attention_int8(q: torch.Tensor, q_stride: int, k: torch.Tensor, v: torch.Ten
         partial = workspace.room("attn_int8_partial", n * heads * splits * (d + 2), torch.float32).data_ptr() if splits > 1 else 0
     _check((_host_functions.get("nnis_attention_int8") or _native("nnis_attention_int8"))(
         at_q, at_k, at_v, at_ks, at_vs, at_pos, at_seq, at_table, at_out, partial, tickets, status, q_stride, seqs, cols, pages, n, heads,
-        kv_heads, d, page_size, window, scale, splits, slice_pieces, together, cluster, eights, code, _stream_of(index)),
+        kv_heads, d, page_size, window, scale, splits, slice_pieces, together, cluster, eights, code, stream),
         "attention_int8", 2 if splits > 1 and not slice_pieces else 1)
 
 
@@ -3283,7 +3284,7 @@ def quantize_rows(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor) ->
     an infinity or a NaN has the scale NaN and codes of zero."""
     facts = (_host_functions.get("quantize_rows") or _native("quantize_rows"))(x, codes, scales)
     if facts is not None:
-        index, code, rows, k, stride, width, at_x, at_codes, at_scales = facts
+        index, stream, code, rows, k, stride, width, at_x, at_codes, at_scales = facts
     if facts is None or not (k > 0 and width == int8_width(k)):
         code_of(x.dtype)
         _need(x.dim() == 2 and (x.shape[1] == 1 or x.stride(1) == 1) and x.shape[1] > 0,
@@ -3293,11 +3294,11 @@ def quantize_rows(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor) ->
         raise KernelError("quantize_rows: tensors on several devices")
     if rows == 0:
         return
-    if _device_now() != index:
+    if stream < 0:  # (another device is the current one)
         with torch.cuda.device(index):
             return quantize_rows(x, codes, scales)
     _check((_host_functions.get("nnis_quantize_rows") or _native("nnis_quantize_rows"))(
-        at_x, at_codes, at_scales, stride, code, rows, k, _stream_of(index)), "quantize_rows")
+        at_x, at_codes, at_scales, stride, code, rows, k, stream), "quantize_rows")
 
 
 def rmsnorm_int8_takes(width: int) -> bool:
@@ -3309,7 +3310,7 @@ def rmsnorm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float, codes: torch
     int8_width(width)], scales float32 [n]."""
     facts = (_host_functions.get("rmsnorm_int8") or _native("rmsnorm_int8"))(x, weight, codes, scales)
     if facts is not None:
-        index, _, n, width, coded, at_x, at_weight, at_codes, at_scales = facts
+        index, stream, _, n, width, coded, at_x, at_weight, at_codes, at_scales = facts
     if facts is None or not (rmsnorm_int8_takes(width) and eps > 0 and coded == int8_width(width)):
         _need(x.dim() == 2, f"rmsnorm_int8: x [n, width]; got {tuple(x.shape)}")
         n, width = x.shape
@@ -3320,11 +3321,11 @@ def rmsnorm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float, codes: torch
     code = code_of(dtype)
     if n == 0:
         return
-    if _device_now() != index:
+    if stream < 0:  # (another device is the current one)
         with torch.cuda.device(index):
             return rmsnorm_int8(x, weight, eps, codes, scales, dtype)
     _check((_host_functions.get("nnis_rmsnorm_int8") or _native("nnis_rmsnorm_int8"))(
-        at_x, at_weight, at_codes, at_scales, n, width, code, eps, _stream_of(index)), "rmsnorm_int8")
+        at_x, at_weight, at_codes, at_scales, n, width, code, eps, stream), "rmsnorm_int8")
 
 
 def linear_int8_coded(codes: torch.Tensor, scales: torch.Tensor, k: int, w: torch.Tensor, w_scales: torch.Tensor,
@@ -3334,7 +3335,7 @@ def linear_int8_coded(codes: torch.Tensor, scales: torch.Tensor, k: int, w: torc
     name = "linear_int8_coded" if mode == STORE or mode == GEMM_GATED else "linear_int8_coded/float32"
     facts = (_host_functions.get(name) or _native(name))(codes, scales, w, w_scales, bias, out)
     if facts is not None:
-        index, code, m, coded, rows, width, n, at_codes, at_scales, at_w, at_ws, at_bias, at_out = facts
+        index, stream, code, m, coded, rows, width, n, at_codes, at_scales, at_w, at_ws, at_bias, at_out = facts
     if facts is None or not (mode in (STORE, STORE_F32, ADD_F32, GEMM_GATED) and 0 < k <= INT8_LONGEST and coded == width == int8_width(k)
                              and rows == (2 * n if mode == GEMM_GATED else n) and n > 0):
         _need(codes.dim() == 2 == w.dim(), f"linear_int8_coded: codes [m, width] and w [rows, width]; got {tuple(codes.shape)} and {tuple(w.shape)}")
@@ -3349,12 +3350,12 @@ def linear_int8_coded(codes: torch.Tensor, scales: torch.Tensor, k: int, w: torc
         raise KernelError("linear_int8_coded: bad argument")
     if m == 0:
         return
-    if _device_now() != index:
+    if stream < 0:  # (another device is the current one)
         with torch.cuda.device(index):
             return linear_int8_coded(codes, scales, k, w, w_scales, bias, out, mode)
     _check((_host_functions.get("nnis_linear_int8") or _native("nnis_linear_int8"))(
         0, at_w, at_ws, at_bias, at_out, at_codes, at_scales, (_status[index] if index in _status else status_word(w.device)).data_ptr(), 0, m,
-        n, k, mode, max(code, F32), _sm_count.get(index) or sm_count(w.device), 1, _stream_of(index)), "linear_int8_coded")
+        n, k, mode, max(code, F32), _sm_count.get(index) or sm_count(w.device), 1, stream), "linear_int8_coded")
 
 
 def linear_int8(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, bias: Optional[torch.Tensor], out: torch.Tensor, mode: int,
@@ -3367,7 +3368,7 @@ def linear_int8(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, bias: 
     name = "linear_int8" if mode == STORE or mode == GEMM_GATED else "linear_int8/float32"
     facts = (_host_functions.get(name) or _native(name))(x, w, w_scales, bias, out)
     if facts is not None:
-        index, code, m, k, stride, rows, width, n, at_x, at_w, at_ws, at_bias, at_out = facts
+        index, stream, code, m, k, stride, rows, width, n, at_x, at_w, at_ws, at_bias, at_out = facts
     if facts is None or not (mode in (STORE, STORE_F32, ADD_F32, GEMM_GATED) and 0 < k <= INT8_LONGEST and width == -(-k // 16) * 16
                              and rows == (2 * n if mode == GEMM_GATED else n) and n > 0):
         _need(x.dim() == 2 == w.dim(), f"linear_int8: x [m, k] and w [rows, width]; got {tuple(x.shape)} and {tuple(w.shape)}")
@@ -3382,7 +3383,7 @@ def linear_int8(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, bias: 
                           f"{tuple(x.shape)} in strides {x.stride()} on {x.device}")
     if m == 0:
         return
-    if _device_now() != index:
+    if stream < 0:  # (another device is the current one)
         with torch.cuda.device(index):
             return linear_int8(x, w, w_scales, bias, out, mode, workspace)
     sms = _sm_count.get(index) or sm_count(w.device)
@@ -3393,4 +3394,4 @@ def linear_int8(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, bias: 
     scales = 0 if fused else workspace.room("int8_scales", m, torch.float32).data_ptr()
     _check((_host_functions.get("nnis_linear_int8") or _native("nnis_linear_int8"))(
         at_x, at_w, at_ws, at_bias, at_out, codes, scales, (_status[index] if index in _status else status_word(w.device)).data_ptr(), stride,
-        m, n, k, mode, code, sms, 0, _stream_of(index)), "linear_int8", 1 if fused else 2)
+        m, n, k, mode, code, sms, 0, stream), "linear_int8", 1 if fused else 2)

@@ -272,8 +272,6 @@ def reached(monkeypatch):
     for name in ops._RECORDS8:
         functions[name] = lambda *values, name=name: calls.append((name, values)) or 0
     monkeypatch.setattr(ops, "_host_functions", functions)
-    monkeypatch.setattr(ops, "_device_now", lambda: 0)
-    monkeypatch.setattr(ops, "_stream_of", lambda index: 77)
     monkeypatch.setitem(ops._sm_count, 0, 148)
     monkeypatch.setattr(ops, "_status", {0: torch.zeros(1, dtype=I32)})
     return calls
@@ -295,12 +293,12 @@ def test_what_fits_is_passed_on(reached):
     at = lambda *tensors: tuple(t.data_ptr() for t in tensors)
     qkv, q, pos, seq, table, cos, sin, k, v, ks, vs = a = store_args()[:11]
     ops.rope_store_int8(*store_args(**dict(zip(("qkv", "q", "pos", "seq", "table", "cos", "sin", "k", "v", "ks", "vs"), a))))
-    assert reached.pop() == ("nnis_rope_store_int8", (*at(*a), 1, 2, 3, 9, 4, 5, 3, 1, 64, 64, 77))
+    assert reached.pop() == ("nnis_rope_store_int8", (*at(*a), 1, 2, 3, 9, 4, 5, 3, 1, 64, 64, 0))
     ops.rope_store_int8(*store_args(cos=None, sin=None, k=k, qkv=empty(5, 320), q=empty(5, 192)))
     assert reached.pop()[1][5:8] == (0, 0, k.data_ptr())
     k, v, ks, vs, table, local, ko, vo = a = read_args(ko=empty(5, 2, 64, 64), vo=empty(5, 2, 64, 64))
     ops.read_pages_int8(*a)
-    assert reached.pop() == ("nnis_read_pages_int8", (*at(*a), 3, 2, 3, 0, 4, 5, 2, 64, 64, 77))
+    assert reached.pop() == ("nnis_read_pages_int8", (*at(*a), 3, 2, 3, 0, 4, 5, 2, 64, 64, 0))
     wide = empty(7, 500, dtype=BF16)
     for queries, stride, page in ((wide[:, 8:392], 500, 64), (wide[:1, 8:392], 999, 64), (empty(5, 384, dtype=BF16), 384, 16)):
         n = min(5, queries.shape[0])
@@ -309,23 +307,23 @@ def test_what_fits_is_passed_on(reached):
         ops.attention_int8(*a)
         name, got = reached.pop()
         assert name == "nnis_attention_int8" and got[:5] == at(queries, *a[2:6]) and got[12:22] == (stride, 2, 3, 4, n, 6, 2, 64, page, 0)
-        assert got[5:9] == at(a[6], a[7], a[8], a[9]) and got[22] == 0.125 and got[-2:] == (1, 77) and (got[24] > 0) == (page == 64)
+        assert got[5:9] == at(a[6], a[7], a[8], a[9]) and got[22] == 0.125 and got[-2:] == (1, 0) and (got[24] > 0) == (page == 64)
     x = empty(5, 50, dtype=BF16)[:, :40]
-    for change, want in ((dict(), (50, 5, 12, 40, 0, 1, 148, 0, 77)), (dict(mode=2, out=empty(5, 12)), (50, 5, 12, 40, 2, 1, 148, 0, 77)),
-                         (dict(mode=3, out=empty(5, 6, dtype=BF16), bias=empty(12)), (50, 5, 6, 40, 3, 1, 148, 0, 77)),
-                         (dict(x=empty(1, 40), out=empty(1, 12)), (40, 1, 12, 40, 0, 0, 148, 0, 77))):
+    for change, want in ((dict(), (50, 5, 12, 40, 0, 1, 148, 0, 0)), (dict(mode=2, out=empty(5, 12)), (50, 5, 12, 40, 2, 1, 148, 0, 0)),
+                         (dict(mode=3, out=empty(5, 6, dtype=BF16), bias=empty(12)), (50, 5, 6, 40, 3, 1, 148, 0, 0)),
+                         (dict(x=empty(1, 40), out=empty(1, 12)), (40, 1, 12, 40, 0, 0, 148, 0, 0))):
         a = product_args(**{"x": x, "space": space(), **change})
         ops.linear_int8(*a)
         name, got = reached.pop()
         assert name == "nnis_linear_int8" and got[8:] == want and got[:3] == at(a[0], a[1], a[2]) and got[4] == a[4].data_ptr()
         assert got[3] == (a[3].data_ptr() if a[3] is not None else 0) and (got[5] == 0) == (want[1] == 1)
-    for change, want in ((dict(), (0, 5, 12, 40, 0, 1, 148, 1, 77)), (dict(mode=1, out=empty(5, 12)), (0, 5, 12, 40, 1, 0, 148, 1, 77))):
+    for change, want in ((dict(), (0, 5, 12, 40, 0, 1, 148, 1, 0)), (dict(mode=1, out=empty(5, 12)), (0, 5, 12, 40, 1, 0, 148, 1, 0))):
         ops.linear_int8_coded(*coded_args(**change))
         assert reached.pop()[1][8:] == want
     ops.quantize_rows(x, empty(5, 48, dtype=I8), empty(5))
-    assert reached.pop()[1][3:] == (50, 1, 5, 40, 77)
+    assert reached.pop()[1][3:] == (50, 1, 5, 40, 0)
     ops.rmsnorm_int8(empty(5, 40), empty(40), 1e-5, empty(5, 48, dtype=I8), empty(5), BF16)
-    assert reached.pop()[1][4:] == (5, 40, 1, 1e-5, 77)
+    assert reached.pop()[1][4:] == (5, 40, 1, 1e-5, 0)
     ops.linear_int8(*product_args(x=empty(0, 40, dtype=BF16), out=empty(0, 12, dtype=BF16)))
     ops.attention_int8(*attend_args(q=empty(0, 384, dtype=BF16), out=empty(0, 384, dtype=BF16)))
     assert not reached
