@@ -119,8 +119,9 @@ linear_int8_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
     pdl_wait();
     pdl_launch_dependents();
 
+    int issued = warp == 0 ? 0 : ahead;
     if (lane == 0 && (warp == 0 || warp == 2)) {
-        for (int i = warp == 0 ? 0 : ahead; i < slices; ++i) {
+        for (int& i = issued; i < slices; ++i) {
             if (i >= STAGES && !mbar_wait(&empty[i % STAGES], (uint32_t)(i / STAGES - 1) & 1u)) {
                 abort_flag = 1;
                 break;
@@ -310,6 +311,8 @@ linear_int8_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
     }
     tc_fence_before();
     __syncthreads();
+    if (threadIdx.x == 0 && rank == 0 && abort_flag)  // (copies that are on their way, of both CTAs of a pair, do not outlive them)
+        for (int i = issued > STAGES ? issued - STAGES : 0; i < issued; ++i) mbar_wait(&full[i % STAGES], (uint32_t)(i / STAGES) & 1u);
     if constexpr (PAIR || SPLIT) cluster_meet();
     if (warp == 1) {
         tc_fence_after();
