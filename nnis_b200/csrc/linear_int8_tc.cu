@@ -241,30 +241,23 @@ linear_int8_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
                         y[j + 2] = h.x;
                         y[j + 3] = h.y;
                     }
-                    if (p.out_by_tma) {
-                        if constexpr (sizeof(T) == 2) {
-                            const int unit = c0 % 64 / 8;
+                    if constexpr (sizeof(T) == 2) {
+                        const int unit = c0 % 64 / 8;
 #pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                uint32_t w[4];
+                        for (int j = 0; j < 4; ++j) {
+                            uint32_t w[4];
 #pragma unroll
-                                for (int e = 0; e < 4; ++e) {
-                                    __nv_bfloat162 two = __floats2bfloat162_rn(y[8 * j + 2 * e], y[8 * j + 2 * e + 1]);
-                                    w[e] = *reinterpret_cast<uint32_t*>(&two);
-                                }
-                                *reinterpret_cast<uint4*>(box + lane * 128 + (((unit + j) ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                            for (int e = 0; e < 4; ++e) {
+                                __nv_bfloat162 two = __floats2bfloat162_rn(y[8 * j + 2 * e], y[8 * j + 2 * e + 1]);
+                                w[e] = *reinterpret_cast<uint32_t*>(&two);
                             }
-                        } else {
-#pragma unroll
-                            for (int j = 0; j < 8; ++j)
-                                *reinterpret_cast<float4*>(box + lane * 128 + ((j ^ (lane & 7)) << 4)) =
-                                    make_float4(y[4 * j], y[4 * j + 1], y[4 * j + 2], y[4 * j + 3]);
+                            *reinterpret_cast<uint4*>(box + lane * 128 + (((unit + j) ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
                         }
-                    } else if (m < p.m) {
-                        T* out = reinterpret_cast<T*>(p.out) + (size_t)m * p.n + n0 + c0;
+                    } else {
 #pragma unroll
-                        for (int j = 0; j < 32; ++j)
-                            if (n0 + c0 + j < p.n) out[j] = from_float<T>(ADD ? to_float(out[j]) + y[j] : y[j]);
+                        for (int j = 0; j < 8; ++j)
+                            *reinterpret_cast<float4*>(box + lane * 128 + ((j ^ (lane & 7)) << 4)) =
+                                make_float4(y[4 * j], y[4 * j + 1], y[4 * j + 2], y[4 * j + 3]);
                     }
                 }
                 if (p.out_by_tma) {
@@ -275,6 +268,29 @@ linear_int8_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
                         else tma_store_2d(&map_out, n0 + b * kBoxCols, m0 + quarter * 32, box);
                         asm volatile("cp.async.bulk.commit_group;" ::: "memory");
                     }
+                } else {
+                    // (rows that TMA cannot write: eight at a time, lanes side by side.  us by lanes with a row each / so: 4,096 rows 961 x 1,024
+                    // bfloat16 48 / 9.6, 4,001 x 2,048 added into float32 495 / 69)
+                    __syncwarp();
+                    constexpr int kUnit = 16 / (int)sizeof(T), kRowsAtOnce = 8;
+                    const int rows = min(32, p.m - m0 - quarter * 32);
+                    T* out = reinterpret_cast<T*>(p.out) + (size_t)(m0 + quarter * 32) * p.n + n0 + b * kBoxCols;
+                    for (int r0 = 0; r0 < rows; r0 += kRowsAtOnce)
+#pragma unroll
+                        for (int c = lane; c < kBoxCols; c += 32) {
+                            T y[kRowsAtOnce];
+                            const bool in = n0 + b * kBoxCols + c < p.n;
+#pragma unroll
+                            for (int i = 0; i < kRowsAtOnce; ++i) {
+                                const int r = r0 + i;
+                                y[i] = *reinterpret_cast<const T*>(box + r * 128 + ((c / kUnit ^ (r & 7)) << 4) + c % kUnit * (int)sizeof(T));
+                                if (ADD && in && r < rows) y[i] = from_float<T>(to_float(y[i]) + to_float(out[(size_t)r * p.n + c]));
+                            }
+#pragma unroll
+                            for (int i = 0; i < kRowsAtOnce; ++i)
+                                if (in && r0 + i < rows) out[(size_t)(r0 + i) * p.n + c] = y[i];
+                        }
+                    __syncwarp();
                 }
             }
             if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");

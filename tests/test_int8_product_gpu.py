@@ -199,3 +199,11 @@ def test_a_matrix_that_was_just_put_into_codes(m, n, k, is_coded):
         product()
         assert torch.equal(got, out)
     del graph
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,n,k", [(300, 997, 64), (131, 65, 100), (1999, 1537, 64), (2050, 1543, 33)])
+@pytest.mark.parametrize("mode", [0, 1, 2, 3])
+def test_outputs_whose_rows_are_no_multiple_of_16_bytes(dtype, m, n, k, mode):
+    """Tiles of one CTA and of pairs, whole and cut off at both ends, that no bulk copy can write."""
+    check(dtype, m, n, k, mode, bias=n % 2 == 1)
