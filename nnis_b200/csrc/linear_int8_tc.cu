@@ -395,16 +395,18 @@ int linear_int8_tc(Linear8 p, int mode, bool f32, int sms, cudaStream_t stream) 
     p.out_by_tma = (uintptr_t)p.out % 16 == 0 && (long long)p.n * bytes % 16 == 0 && make_map(&mo, p.out, p.m, p.n, 32, 0, bytes);
     if (!p.out_by_tma) mo = mx;
     const bool alone = (pair ? pairs : singles) <= sms;
-    // CTAs that share a tile's K, two runs of 128 places each at least, none of them empty: clusters have to find their SMs side by side,
-    // and where they would fill the device some wait for a second turn.  us with 2, 3, 4, 8: 16 tiles (64 x 2,048 x 2,048) 8.8, 7.8, 6.8,
-    // 11.0; x 8,192 17.3, 13.7, 11.5, 15.9; 8 tiles (64 x 960 x 2,560) 9.4, 8.1, 7.3, 6.8; 32 tiles (256 x 2,048 x 8,192) 20.7, 17.3,
-    // 15.3; 48 tiles (64 x 6,144 x 2,048) 8.9, 14.1.
+    // CTAs that share a tile's K, two runs of 128 places each at least, none of them empty, where that saves a CTA six runs (eight beyond 64
+    // rows, which are more to add up): a run takes 0.33 us, sharing 2 to 2.6.  Clusters have to find their SMs side by side, and where they
+    // would fill the device some wait for a second turn.  us with 1, 2, 3, 4, 8: 16 tiles (64 x 2,048 x 2,048) 8.4, 8.2, 7.0, 5.9, 9.8;
+    // x 8,192 24.6, 16.6, 12.7, 10.4, 14.5; 32 tiles (256 x 2,048 x 8,192) 25.6, 20.6, 16.2, 13.2, 27.7; 44 tiles (1,400 x 512 x 4,096) 14.2,
+    // 12.0, 10.5, 16.3, 21.8; 48 tiles (64 x 6,144 x 2,048) 8.2, 7.5, 12.5; 1 tile (128 x 128 x 2,555) 9.5, 8.8, 7.7, 6.3, 6.0; 10 tiles of 5
+    // runs (239 x 576 x 576) 4.5, 6.5; 64 of 8 (911 x 960 x 960) 6.4, 7.4; 8 of 8 (64 x 960 x 960) 5.2, 5.5, 5.3, 4.4.
     const int slices = (p.kp + kSlice8 - 1) / kSlice8;
-    int parts = pair ? 1 : 16 * singles <= sms ? 8 : 32 * singles <= 7 * sms ? 4 : 16 * singles <= 7 * sms ? 2 : 1;
+    int parts = pair ? 1 : 16 * singles <= sms ? 8 : 32 * singles <= 7 * sms ? 4 : 30 * singles <= 9 * sms ? 3 : 16 * singles <= 7 * sms ? 2 : 1;
     if (parts > slices / 2) parts = slices / 2;
     if (parts > 1) {
         const int each = (slices + parts - 1) / parts;
-        parts = (slices + each - 1) / each;
+        parts = slices - each < (p.m <= 64 ? 6 : 8) ? 1 : (slices + each - 1) / each;
     }
     if (gated)
         return (int)(f32 ? launch_tc8_of<float, false, true>(mx, mw, mo, p, pair, alone, parts, stream)

@@ -207,3 +207,11 @@ def test_a_matrix_that_was_just_put_into_codes(m, n, k, is_coded):
 def test_outputs_whose_rows_are_no_multiple_of_16_bytes(dtype, m, n, k, mode):
     """Tiles of one CTA and of pairs, whole and cut off at both ends, that no bulk copy can write."""
     check(dtype, m, n, k, mode, bias=n % 2 == 1)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,n,k", [(70, 4609, 2050), (129, 2305, 2100), (66, 1000, 1300), (40, 50, 1537), (128, 129, 1200)])
+@pytest.mark.parametrize("mode", [0, 1, 2, 3])
+def test_tiles_whose_k_several_ctas_share(dtype, m, n, k, mode):
+    """In two, three, five and six parts, the last shorter than the others."""
+    check(dtype, m, n, k, mode, bias=m % 2 == 0)
