@@ -202,18 +202,22 @@ __global__ void __launch_bounds__(kWarps8 * 32, D <= 32 ? 4 : D <= 96 ? 3 : 2) a
                 for (int c = 0; c < D / 4; ++c) x[i][c] = to_float(q[c]);
             }
         }
-        // ---- the run, its keys and this slice's part of them (the same for every thread of the CTA)
-        const int seq = p.token_seq[r0];
-        int top_pos = -1, low = INT_MAX, low_pos = INT_MAX, top_low = 0;
-        for (r1 = r0; r1 < row_end && p.token_seq[r1] == seq; ++r1) {
-            const int pos = p.token_pos[r1];
-            if (pos < 0) continue;
-            const int lo = p.window > 0 ? max(0, pos - p.window + 1) : 0;
-            top_pos = max(top_pos, pos);
-            low_pos = min(low_pos, pos);
-            low = min(low, lo);
-            top_low = max(top_low, lo);
+        // ---- the run, its keys and this slice's part of them (the same for every thread of the CTA): a lane a row, for a loop over rows
+        // waits for each
+        int seq = -1, top_pos = -1, low_pos = INT_MAX;
+        for (int first_row = r0;; first_row += 32) {
+            const bool there = first_row + lane < row_end;
+            const int mine_seq = there ? p.token_seq[first_row + lane] : -1, pos = there ? p.token_pos[first_row + lane] : -1;
+            if (first_row == r0) seq = __shfl_sync(0xffffffffu, mine_seq, 0);
+            const uint32_t others = ~__ballot_sync(0xffffffffu, there && mine_seq == seq);
+            const int count = others ? __ffs(others) - 1 : 32;
+            const bool counts = lane < count && pos >= 0;
+            top_pos = max(top_pos, __reduce_max_sync(0xffffffffu, counts ? pos : -1));
+            low_pos = min(low_pos, __reduce_min_sync(0xffffffffu, counts ? pos : INT_MAX));
+            r1 = first_row + count;
+            if (count < 32 || r1 >= row_end) break;
         }
+        const int low = p.window > 0 && low_pos != INT_MAX ? max(0, low_pos - p.window + 1) : 0, top_low = p.window > 0 ? max(0, top_pos - p.window + 1) : 0;
         const int entries = (r1 - r0) * per;
         if (e0 >= entries) continue;
         const bool known = seq >= 0 && seq < p.table_rows && top_pos >= 0;

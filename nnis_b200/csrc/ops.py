@@ -3180,24 +3180,26 @@ def attention_int8_splits(n: int, heads: int, keys: int, device) -> int:
 @functools.lru_cache(maxsize=4096)
 def attention_int8_plan(n: int, seqs: int, heads: int, kv_heads: int, d: int, cols: int, window: int, sms: int):
     """(slices, pieces of a slice, rows taken together, CTAs of a slice's cluster or 0 for a warp a unit, eights of queries in a
-    tile) of the tensor cores' kernel; a piece is 64 positions,
-    32 for heads of 96 and 128.  Rows of a sequence lie together, as many as come on each, up to 64 queries a key/value head."""
+    tile) of the tensor cores' kernel; a piece is 64 positions, 32 for heads of 96 and 128.  Rows of a sequence lie together, as many as
+    come on each, up to 64 (where they were cut at 64 queries a key/value head, runs crossed the ends of sequences, one part after the
+    other: five rows of 20 heads on one, two sequences of 500 12.7 us, now 7.6)."""
     per, half = heads // kv_heads, 1 if d <= 64 else 2
-    rows = max(1, min(-(-n // max(1, seqs)), 64 // per))
+    rows = max(1, min(-(-n // max(1, seqs)), 64))
     length = 64 // half
     seen = min(half * cols, (window + rows + length - 2) // length + 1) if window else half * cols
     resident = sms * (4 if d <= 32 else 3 if d <= 96 else 2)
     # tiles of 8 queries; of 16 where those of 8 would take the device more than one turn, and with heads beyond 64, whose tiles of 8 leave
     # the tensor cores waiting, where four CTAs a unit fill it.  us in tiles of 8 / 16, each with its best number of CTAs: five rows of four
     # heads of 128, 16 sequences of 4,000 94 / 65, 4 of 8,000 54 / 42; 24 heads of 128, 64 sequences of 4,000 52 / 40, 8 of 4,000 14.2 /
-    # 17.4; 20 heads of 64, 64 sequences of 4,096 23 / 29; five rows of three heads of 64, 64 sequences of 2,000 22.8 / 22.1
+    # 17.4; 20 heads of 64, 64 sequences of 4,096 23 / 29; five rows of three heads of 64, 64 sequences of 2,000 22.8 / 22.1; five rows of
+    # eight heads of 128, 15 sequences of 88 7.3 / 8.9
     runs = -(-n // rows) * kv_heads
     turns = resident // (runs * -(-rows * per // 16))
-    eights = 2 if rows * per > 8 and (runs * -(-rows * per // 8) > resident or (d > 64 and turns <= 4)) else 1
+    eights = 2 if rows * per > 8 and (runs * -(-rows * per // 8) > resident or (d > 64 and turns <= 4 and seen >= 8)) else 1
     units = runs * -(-rows * per // (8 * eights))
     # A warp a unit where units are many and short: us by four warps / one: 1,760 units of one piece 18.6 / 6.4, 2,048 of two 25.4 / 14.8,
-    # of eight 39.8 / 37.4, of 16 58.6 / 66.1; 512 (heads of 128) of ten 20.5 / 16.5, of 32 36.7 / 39.7.
-    if units >= resident and seen <= INT8_ALONE_PIECES:
+    # of eight 39.8 / 37.4, of 16 58.6 / 66.1; 512 (heads of 128) of ten 20.5 / 16.5, of 32 36.7 / 39.7, 560 of 24 39.9 / 35.4.
+    if units >= resident and seen <= INT8_ALONE_PIECES[half]:
         return 1, half * cols, rows, 0, eights
     # CTAs a unit (a run of rows, a key/value head, a tile of queries): up to half of what the device holds at once, since a cluster's and a
     # join's meeting cost what two pieces do; all of it where that is two, or where eight pieces are left to each.  us with 1, 2, 4, 8,
@@ -3207,13 +3209,16 @@ def attention_int8_plan(n: int, seqs: int, heads: int, kv_heads: int, d: int, co
     held, most, ctas = resident // units, -(-seen // 2) if seen <= 8 else -(-seen // 3), 1
     while 2 * ctas <= min(held, most) and (ctas == 1 or 4 * ctas <= held or seen >= 16 * ctas):
         ctas *= 2
-    cluster = min(8, ctas)
+    # (clusters have to find their SMs side by side: where those of more than two would fill three quarters of the device, slices.  144 units of
+    # 44 pieces, heads of 32, float32: clusters of four 19.9, four slices 13.7, clusters of two 14.8; 192 of eight pieces: clusters of two
+    # 7.5, two slices 8.5)
+    cluster = min(8, ctas) if ctas <= 2 or 4 * units * ctas <= 3 * resident else 1
     slices = min(64, ctas // cluster)
     pieces = -(-half * cols // slices)
     return -(-half * cols // pieces), pieces, rows, cluster, eights
 
 
-INT8_ALONE_PIECES = 10
+INT8_ALONE_PIECES = {1: 10, 2: 24}  # pieces of 64, of 32 positions
 
 
 def attention_int8(q: torch.Tensor, q_stride: int, k: torch.Tensor, v: torch.Tensor, k_scales: torch.Tensor, v_scales: torch.Tensor,

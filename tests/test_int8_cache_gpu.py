@@ -423,3 +423,22 @@ def test_tickets_and_records_serve_calls_of_all_sizes():
         for c, want in zip(kept, alone):
             assert torch.equal(run(*c, ws), want)
     ops.check_status("cuda:0")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv_heads,d", [(3, 1, 64), (2, 2, 32), (6, 2, 128), (20, 1, 96)])
+@pytest.mark.parametrize("tokens", [[64, 64], [33, 31, 32], [100, 1, 70], [40, 0, 3, 150]])
+def test_runs_of_many_rows(dtype, heads, kv_heads, d, tokens):
+    """More rows of a sequence than a warp has lanes, than are taken together; runs that cross the ends of sequences, padding rows among
+    them, in a sequence of their own and in others'."""
+    gen = torch.Generator().manual_seed(19)
+    lengths = [t + 90 * (i % 2) + 1 for i, t in enumerate(tokens)]
+    table, pages = place(lengths, gen)
+    positions, seqs = [], []
+    for i, (t, n) in enumerate(zip(tokens, lengths)):
+        rows = [n - t + j for j in range(t)]
+        if t > 30:
+            rows[t // 2] = rows[5] = -1
+        positions += rows + [-1, -1]
+        seqs += [i] * t + [i, -1]
+    check(dtype, heads, kv_heads, d, positions, seqs, table, pages, window=37 if heads == 6 else 0, seed=11)

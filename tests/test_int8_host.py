@@ -208,7 +208,7 @@ def test_plans_of_attention_cover_every_key(d):
                     per_page = 1 if d <= 64 else 2
                     assert 1 <= slices <= 64 and slices * pieces >= per_page * cols and (slices - 1) * pieces < per_page * cols
                     assert cluster in (0, 1, 2, 4, 8) and (cluster > 0 or slices == 1) and eights in (1, 2)
-                    assert 1 <= rows <= max(1, 64 // (heads // kv_heads)) and slices * cluster <= 65535
+                    assert 1 <= rows <= 64 and slices * cluster <= 65535
 
 
 def test_norms_and_coded_rows_refuse():
