@@ -3164,11 +3164,11 @@ def read_pages_int8(k: torch.Tensor, v: torch.Tensor, k_scales: torch.Tensor, v_
 
 
 # A prompt step whose sequences bring at most this many tokens each attends over the codes row by row; others read their pages back and
-# take the kernels of the 16-bit or float32 cache.  us by rows / read back, 9 query and 3 key/value heads of 64, bfloat16: eight sequences
-# of 4,000, 8 tokens 15 / 39, 16 tokens 24 / 40, 24 tokens 61 / 40; one of 4,000, 64 tokens 17 / 24; float32: eight of 1,000, 32 tokens
-# 28 / 37, eight of 4,000 76 / 112; 32 and 8 heads of 128, eight of 4,000: bfloat16 16 tokens 66 / 185, 24 tokens 132 / 159, float32
-# 64 tokens 373 / 1,761.
-INT8_ROWS_AT_ONCE = {torch.bfloat16: 16, torch.float32: 64}
+# take the kernels of the 16-bit or float32 cache.  us by rows / read back with 16, 32, 64 tokens, bfloat16: 9 query and 3 key/value heads of
+# 64, eight sequences of 4,000 22 / 40, 36 / 40, 48 / 41; 32 and 32 heads of 64, one of 4,000 15 / 32, 22 / 32, 36 / 34; 32 and 8 heads of 128, eight
+# of 1,000 23 / 48, 43 / 56, 85 / 53, of 4,000 63 / 184, 121 / 162, 223 / 186; float32: 9 and 3 heads of 64, eight of 4,000 26 / 112, 43 / 113,
+# 66 / 10,990; 32 and 8 of 128 106 / 1,752, 190 / 1,759, 361 / 1,768.
+INT8_ROWS_AT_ONCE = {torch.bfloat16: 32, torch.float32: 64}
 
 
 def attention_int8_splits(n: int, heads: int, keys: int, device) -> int:
