@@ -139,7 +139,8 @@ NNIS_API int nnis_attention_int8(const void* call) {
     const auto [q, k, v, k_scales, v_scales, token_pos, token_seq, page_table, out, partial, tickets, status, q_stride, table_rows, table_cols, pages, n,
                 nq, nkv, d, page_size, window, scale, splits, slice_pieces, rows_at_once, cluster, tile_eights, dtype, stream] = c;
     if (n <= 0 || nq <= 0 || nkv <= 0 || nq % nkv || table_rows <= 0 || table_cols <= 0 || pages <= 0 || page_size <= 0 || window < 0 ||
-        splits < 1 || (splits > 1 && !partial) || !q || !k || !v || !k_scales || !v_scales || !out)
+        splits < 1 || (splits > 1 && !partial) || !q || !k || !v || !k_scales || !v_scales || !token_pos || !token_seq ||
+        !page_table || !out)
         return NNIS_ERR_ARGUMENT;
     if (d < 2 || d % 2 || d > 256 || nq > 65535 || splits > 64) return NNIS_ERR_UNSUPPORTED;
     if (((uintptr_t)k | (uintptr_t)v) % 4) return NNIS_ERR_ALIGNMENT;

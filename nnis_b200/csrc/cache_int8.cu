@@ -322,7 +322,7 @@ NNIS_API int nnis_rope_store_int8(const void* call) {
     const auto [qkv, q, token_pos, token_seq, page_table, cos_t, sin_t, k, v, k_scales, v_scales, dtype, table_rows, table_cols,
                 angle_rows, pages, n, nq, nkv, d, page_size, stream] = c;
     if (n <= 0 || nq <= 0 || nkv <= 0 || table_rows <= 0 || table_cols <= 0 || pages <= 0 || page_size <= 0 || !qkv || !q || !k ||
-        !v || !k_scales || !v_scales || !page_table || !cos_t != !sin_t)
+        !v || !k_scales || !v_scales || !token_pos || !token_seq || !page_table || !cos_t != !sin_t)
         return NNIS_ERR_ARGUMENT;
     if (d < 2 || d % 2 || d > 256) return NNIS_ERR_UNSUPPORTED;
     const uintptr_t rows = (uintptr_t)qkv | (uintptr_t)q | (uintptr_t)cos_t | (uintptr_t)sin_t, codes = (uintptr_t)k | (uintptr_t)v;

@@ -375,3 +375,16 @@ def test_a_matrix_with_too_many_columns_is_refused():
     from nnis_b200.parts.linear import Int8Matrix
     with pytest.raises(ValueError, match="up to 133136 columns"):
         Int8Matrix.of(empty(1, ops.INT8_LONGEST + 1, dtype=BF16))
+
+
+def test_entries_refuse_what_has_no_address():
+    """Nothing is launched for a tensor without memory, whichever it is."""
+    from nnis_b200.csrc import ops
+    at = 1 << 20  # (looked at by nobody: an entry that refuses launches nothing)
+    for name, places, sizes in (("nnis_rope_store_int8", 11, (0, 1, 1, 1, 1, 1, 1, 1, 64, 64)), ("nnis_read_pages_int8", 8, (1, 1, 1, 0, 1, 1, 1, 64, 64)),
+                                ("nnis_attention_int8", 9, (0, 0, 0, 64, 1, 1, 1, 1, 1, 64, 64, 0, 0.5, 1, 0, 0, 0, 0, 0)),
+                                ("nnis_quantize_rows", 3, (8, 0, 1, 8)), ("nnis_rmsnorm_int8", 4, (1, 8, 0, 1e-5))):
+        for missing in range(places):
+            assert ops._native(name)(*(0 if i == missing else at for i in range(places)), *sizes, 0) == -1, (name, missing)
+    for missing in (1, 2, 4, 5, 6):
+        assert ops._native("nnis_linear_int8")(*(0 if i in (missing, 3, 7) else at for i in range(8)), 0, 1, 16, 16, 0, 0, 148, 1, 0) == -1
