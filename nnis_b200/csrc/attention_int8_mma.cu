@@ -126,7 +126,7 @@ __device__ __forceinline__ float query_codes(const float (&x)[D / 4], uint32_t (
     for (int i = 0; i < D / 4; ++i) top = max(top, magnitude_bits(x[i]));
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    constexpr float kMost = F32 ? 8323072.f : 32512.f;  // 127 * 65,536, 127 * 256
+    constexpr float kMost = F32 ? 127.f * 65536.f : 127.f * 256.f;
     const bool none = top >= 0x7f800000u, zero = __uint_as_float(top) < 0x1p-100f;
     const float inverse = none || zero ? 0.f : __fdiv_rn(kMost, __uint_as_float(top));
 #pragma unroll
