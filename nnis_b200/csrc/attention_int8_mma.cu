@@ -376,7 +376,8 @@ __global__ void __launch_bounds__(kWarps8 * 32, D <= 32 ? 4 : D <= 96 ? 3 : 2) a
                 t_most = fmaxf(t_most, __shfl_xor_sync(0xffffffffu, t_most, 1));
                 t_most = fmaxf(t_most, __shfl_xor_sync(0xffffffffu, t_most, 2));
                 float grown = 1.f;
-                if (t_most >= unit_t && t_most >= 0x1p-100f) {
+                // (a row that is not put into zeros has a scale of 2^-107 at least; 2^15 / T is a number down to T = 2^-112)
+                if (t_most >= unit_t && t_most >= 0x1p-112f) {
                     const uint32_t bits = min((__float_as_uint(t_most) & 0x7f800000u) + 0x00800000u, 0x7e800000u);  // (at most 2^126)
                     grown = unit_t * __uint_as_float(0x7f000000u - bits);  // T before / T now
                     unit_t = __uint_as_float(bits);
@@ -475,7 +476,7 @@ __global__ void __launch_bounds__(kWarps8 * 32, D <= 32 ? 4 : D <= 96 ? 3 : 2) a
                 const bool sees = pos_of[i] >= 0;
                 l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
                 l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-                const float inv = sees && l[i] != 0.f ? unit_t * (1.f / 32768.f) / l[i] : 0.f;
+                const float inv = sees && l[i] != 0.f ? 1.f / l[i] : 0.f, back = unit_t * (1.f / 32768.f);
                 const int e = e0 + 8 * i + g;
                 if (e >= entries) continue;
                 T* row = reinterpret_cast<T*>(p.out) + ((size_t)(r0 + e / per) * p.nq + hk * per + e % per) * D + t * (D / 4);
@@ -488,7 +489,7 @@ __global__ void __launch_bounds__(kWarps8 * 32, D <= 32 ? 4 : D <= 96 ? 3 : 2) a
                         for (int j = 0; j < 4; ++j) {
                             if constexpr (F32) y[j] = o[i][c + j][half] + o[i][c + j][2 + half];
                             else y[j] = o[i / 2][c + j][2 * (i & 1) + half];
-                            y[j] = sees ? y[j] * inv : 0.f;
+                            y[j] = sees ? y[j] * inv * back : 0.f;
                         }
                         store4(row + half * (D / 8) + c, make_float4(y[0], y[1], y[2], y[3]));
                     }
