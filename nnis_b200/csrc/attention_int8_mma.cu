@@ -7,7 +7,9 @@
 // rows 8 to 15, so that a thread gets both sums of a score, exact, and score = (256 hi + lo) * (top / top') * key scale * scale.
 // The value's codes become float16 (a byte b of 0 to 255 behind the byte 0x64 is 1,024 + b) for products of 16 x 8 x 16 with the weights
 // w_j = 2^15 p_j t_j / T, where t_j is the value's scale and T a power of two above all scales that the warp has met: w_j is below
-// 2^15, and float16 holds what is 2^-29 of the largest weight to its full 11 bits.  bfloat16: eight more queries in rows 8 to 15.
+// 2^15, and float16 holds what is 2^-29 of T to its full 11 bits.  A row whose weighted values all lie far below T, because the large values
+// that its warp has met have next to no weight for it, is looked at again in float32 (attend_alone8).  bfloat16: eight more queries in rows
+// 8 to 15.
 // float32: what float16 has left of the weights there, so that a weight has 22 bits.  Maxima, sums and outputs are float32.
 //
 // Any order of a head's values serves the first product and any order of positions the second, so a thread's part of every fragment lies
@@ -145,6 +147,66 @@ __device__ __forceinline__ float query_codes(const float (&x)[D / 4], uint32_t (
         lo[w] = pack_codes(l[0], l[1], l[2], l[3]);
     }
     return none ? __uint_as_float(0x7fc00000u) : zero ? 0.f : __fdiv_rn(__uint_as_float(top), kMost);
+}
+
+// One row over a warp's pieces, by all lanes of the warp, in float32 throughout: sums of weights times values, [D] to `sums`; its maximum
+// (of scores in units of log 2) and sum of weights.  For rows that float16 has lost: a weight is off by up to 2^-25, half of float16's least
+// step, so a sum over n positions by up to n 127 2^-25, and where a row's sums are all below lost8 that is told from nothing no more
+// (4,096 positions: 2^-6 / lost8; a row of weight one on values as large as any has 2^20).
+__host__ __device__ constexpr float lost8(bool f32) { return f32 ? 4096.f : 256.f; }
+template <int D, typename T>
+__device__ __forceinline__ float2 attend_alone8(const Attend8& p, const int* table, int hk, const T* q, int low, int pos, int first, int last, int step,
+                                             float* query, float* sums) {
+    constexpr int kPiece = piece8(D), kPieces = kPage8 / kPiece, kOwn = D / 32;
+    const int lane = threadIdx.x & 31;
+    for (int i = lane; i < D; i += 32) query[i] = to_float(q[i]);
+    __syncwarp();
+    float m = -INFINITY, l = 0.f, acc[kOwn] = {};
+    for (int piece = first; piece < last; piece += step) {
+        const int page = table[(unsigned)piece / kPieces];
+        if ((unsigned)page >= (unsigned)p.pages) continue;
+        for (int at = 0; at < kPiece; at += 32) {
+            const int key = piece * kPiece + at + lane;
+            const bool seen = key >= low && key <= pos;
+            if (!__any_sync(0xffffffffu, seen)) continue;
+            const size_t row = ((size_t)page * p.nkv + hk) * kPage8 + piece % kPieces * kPiece + at;
+            float score = -INFINITY, t = 0.f;
+            if (seen) {
+                const uint32_t* codes = reinterpret_cast<const uint32_t*>(p.k + (row + lane) * D);
+                float dot = 0.f;
+                for (int i = 0; i < D / 4; ++i)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) dot = fmaf(query[4 * i + c], code_value(codes[i], c), dot);
+                score = dot * p.k_scales[row + lane] * (p.scale * 1.4426950408889634f);
+                t = p.v_scales[row + lane];
+            }
+            const float now = fmaxf(m, warp_max(score)), base = now == -INFINITY ? 0.f : now, shrink = ex2_8(m - base);
+            float w = seen ? ex2_8(score - base) : 0.f;
+            l = fmaf(l, shrink, warp_sum(w));
+            m = now;
+            w = w == 0.f ? 0.f : w * t;
+#pragma unroll
+            for (int r = 0; r < kOwn; ++r) acc[r] *= shrink;
+            for (int j = 0; j < 32; ++j) {
+                const float wj = __shfl_sync(0xffffffffu, w, j);
+                if (wj == 0.f) continue;
+                const int8_t* value = p.v + (row + j) * D + lane;
+#pragma unroll
+                for (int r = 0; r < kOwn; ++r) acc[r] = fmaf(wj, (float)value[32 * r], acc[r]);
+            }
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < kOwn; ++r) sums[lane + 32 * r] = acc[r];
+    __syncwarp();
+    return make_float2(m, l);
+}
+
+// The same as a call, where the row's registers beside a tile's of sixteen queries would spill the tile's
+template <int D, typename T>
+__device__ __noinline__ float2 attend_alone_call8(const Attend8& p, const int* table, int hk, const T* q, int low, int pos, int first, int last, int step,
+                                                  float* query, float* sums) {
+    return attend_alone8<D, T>(p, table, hk, q, low, pos, first, last, step, query, sums);
 }
 
 // SOLO: a warp a unit, its whole range of keys, for many rows with few keys.
@@ -470,6 +532,38 @@ __global__ void __launch_bounds__(kWarps8 * 32, D <= 32 ? 4 : D <= 96 ? 3 : 2) a
             }
         }
 
+        // ---- rows that float16 has lost (below), a bit for each of a row's four lanes
+        uint32_t lost[MT];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            float largest = 0.f;
+#pragma unroll
+            for (int c = 0; c < kCols; ++c)
+#pragma unroll
+                for (int half = 0; half < 2; ++half) largest = fmaxf(largest, fabsf(F32 ? o[i][c][half] : o[i / 2][c][2 * (i & 1) + half]));
+            largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
+            largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
+            lost[i] = __ballot_sync(0xffffffffu, pos_of[i] >= 0 && l[i] > 0.f && unit_t > 0.f && largest < lost8(F32));
+        }
+        // `with`: what becomes of a lost row, given its place in the tile, maximum, sum of weights and sums
+        auto again = [&](float* query, float* sums, auto with) {
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+                while (lost[i]) {
+                    const int row = (__ffs(lost[i]) - 1) / 4, e = e0 + 8 * i + row;
+                    lost[i] &= ~(15u << (4 * row));
+                    const T* q = reinterpret_cast<const T*>(p.q) + (size_t)(r0 + e / per) * p.q_stride + (size_t)(hk * per + e % per) * D;
+                    const int pos = __shfl_sync(0xffffffffu, pos_of[i], 4 * row), from = __shfl_sync(0xffffffffu, low_of[i], 4 * row);
+                    const int mine_first = SOLO ? first : first + rank * kWarps8 + warp;
+                    float* to = sums + (SOLO ? 0 : (8 * i + row) * D);
+                    float2 ml;
+                    if constexpr (MT == 1) ml = attend_alone8<D, T>(p, table, hk, q, from, pos, mine_first, last, step, query, to);
+                    else ml = attend_alone_call8<D, T>(p, table, hk, q, from, pos, mine_first, last, step, query, to);
+                    with(8 * i + row, ml);
+                }
+            __syncwarp();
+        };
         if constexpr (SOLO) {
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
@@ -494,7 +588,14 @@ __global__ void __launch_bounds__(kWarps8 * 32, D <= 32 ? 4 : D <= 96 ? 3 : 2) a
                         store4(row + half * (D / 8) + c, make_float4(y[0], y[1], y[2], y[3]));
                     }
             }
-            __syncwarp();
+            float* kept = reinterpret_cast<float*>(ring);
+            again(kept, kept + D, [&](int row, float2 ml) {
+                const int e = e0 + row;
+                T* out = reinterpret_cast<T*>(p.out) + ((size_t)(r0 + e / per) * p.nq + hk * per + e % per) * D;
+                for (int d = lane; d < D; d += 32) out[d] = from_float<T>(ml.y == 0.f ? 0.f : kept[D + d] / ml.y);
+                fence_async_shared8();
+                __syncwarp();
+            });
             continue;
         }
         // ---- the four warps' parts are joined: [queries][D] sums, then maxima and sums of weights, in the warp's own ring
@@ -523,6 +624,12 @@ __global__ void __launch_bounds__(kWarps8 * 32, D <= 32 ? 4 : D <= 96 ? 3 : 2) a
                 }
             }
         }
+        again(stats + 2 * kTile, sums, [&](int row, float2 ml) {
+            if (lane == 0) {
+                stats[2 * row] = ml.x;
+                stats[2 * row + 1] = ml.y;
+            }
+        });
         __syncthreads();
         const int count = min(kTile, entries - e0);
         auto warp_part = [&](int w) { return reinterpret_cast<const float*>(smem + (size_t)w * kStages * kStage); };
@@ -642,6 +749,7 @@ template <int D, bool F32, int MT, bool SOLO>
 static cudaError_t launch_mma8(const Attend8& p, unsigned units, cudaStream_t stream) {
     constexpr size_t smem = (size_t)kWarps8 * stages8(D) * stage_bytes8(D);
     static_assert(stages8(D) * stage_bytes8(D) >= 2 * 8 * MT * (D + 2) * 4, "a warp's part of the outputs fits its ring, twice in the first");
+    static_assert(stages8(D) * stage_bytes8(D) >= 8 * MT * (D + 2) * 4 + D * 4, "and a query behind it");
     auto kernel = attn_int8_mma_kernel<D, F32, MT, SOLO>;
     static std::atomic<int> held[16];
     const cudaError_t e = allow_shared(kernel, smem, held);

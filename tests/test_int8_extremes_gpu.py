@@ -43,3 +43,65 @@ def test_values_of_the_smallest_scales(dtype, heads, kv_heads, d, lengths, token
                                   d ** -0.5, dtype == torch.float32)
     got = attend(q, k, v, ks, vs * 2.0 ** -low, positions, seqs, table, heads, kv_heads, 0, d ** -0.5)[shown] * 2.0 ** low
     assert ((got - want).abs() <= bound).all(), float(((got - want).abs() / bound).max())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv_heads,d", [(9, 3, 64), (8, 2, 128), (12, 4, 96), (4, 2, 32), (2, 1, 40)])
+@pytest.mark.parametrize("lengths,tokens", SHAPES)
+@pytest.mark.parametrize("at", ["first", "middle", "last"])
+@pytest.mark.parametrize("large", [20, 40, 100])
+def test_a_large_value_that_has_no_weight(dtype, heads, kv_heads, d, lengths, tokens, at, large):
+    """One position of a page has values 2^large times the others' and a key that no query turns to: its scores lie at least 2 (large + 40)
+    below the others' (in natural units), so its share is below 2^-(large + 60) of any other's and the outputs are those without it."""
+    gen = torch.Generator().manual_seed(large + d)
+    table, pages = place(lengths, gen)
+    k, ks = plain.store(pages, kv_heads, d, gen)
+    v, vs = plain.store(pages, kv_heads, d, gen)
+    q = (1.5 * torch.randn((len(lengths) * tokens, heads * d), generator=gen)).to(dtype).view(-1, heads, d)
+    scale = d ** -0.5
+    # value 0 of every query is 4 and every key's is 0, but that of the large positions, which have nothing else
+    q[..., 0] = 4.0
+    k[..., 0] = 0
+    for line, n in zip(table, lengths):
+        for j in {"first": [0], "middle": [(n - tokens) // 2], "last": [n - tokens]}[at]:
+            page, slot = line[j // PAGE], j % PAGE
+            k[page, :, slot] = 0
+            k[page, :, slot, 0] = -127
+            ks[page, :, slot] = 2.0 * (large + 60) / (4 * 127 * scale)
+            vs[page, :, slot] *= 2.0 ** large
+    q = q.reshape(len(lengths) * tokens, heads * d)
+    positions, seqs = [n - tokens + j for n in lengths for j in range(tokens)], [i for i in range(len(lengths)) for _ in range(tokens)]
+    shown = [i for i in range(len(positions)) if i < 6 or i > len(positions) - 4]
+    # (the bound is that of the others: one with this position's key of zeros and its value as large as theirs, whose share of some
+    # hundredths moves theirs by as much)
+    plain_ks, plain_vs = ks.clone(), vs.clone()
+    for line, n in zip(table, lengths):
+        j = {"first": 0, "middle": (n - tokens) // 2, "last": n - tokens}[at]
+        plain_ks[line[j // PAGE], :, j % PAGE] = 0.0
+        plain_vs[line[j // PAGE], :, j % PAGE] *= 2.0 ** -large
+    rows = [positions[i] for i in shown], [seqs[i] for i in shown], table, heads, kv_heads, 0, scale, dtype == torch.float32
+    want, _ = plain.attention(q[shown], k, v, ks, plain_vs, *rows)
+    _, bound = plain.attention(q[shown], k, v, plain_ks, plain_vs, *rows)
+    got = attend(q, k, v, ks, vs, positions, seqs, table, heads, kv_heads, 0, scale)[shown]
+    assert ((got - want).abs() <= 1.05 * bound).all(), float(((got - want).abs() / bound).max())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv_heads,d", [(9, 3, 64), (20, 1, 64), (8, 2, 128), (12, 4, 96), (4, 2, 32), (2, 1, 40)])
+@pytest.mark.parametrize("window,at", [(100, 296), (0, 399)])
+@pytest.mark.parametrize("sequences", [1, 120])
+def test_a_large_value_that_others_see(dtype, heads, kv_heads, d, window, at, sequences):
+    """Five rows of a sequence, of which the first (the last) alone sees a position whose values are 2^60 times the others'."""
+    gen = torch.Generator().manual_seed(at + d)
+    table, pages = place([400] * sequences, gen)
+    k, ks = plain.store(pages, kv_heads, d, gen)
+    v, vs = plain.store(pages, kv_heads, d, gen)
+    for line in table:
+        vs[line[at // PAGE], :, at % PAGE] *= 2.0 ** 60
+    q = (1.5 * torch.randn((5 * sequences, heads * d), generator=gen)).to(dtype)
+    positions, seqs = [395, 396, 397, 398, 399] * sequences, [i for i in range(sequences) for _ in range(5)]
+    shown = list(range(5)) if sequences == 1 else [*range(5), *range(5 * sequences - 10, 5 * sequences)]
+    want, bound = plain.attention(q[shown], k, v, ks, vs, [positions[i] for i in shown], [seqs[i] for i in shown], table, heads, kv_heads, window,
+                                  d ** -0.5, dtype == torch.float32)
+    got = attend(q, k, v, ks, vs, positions, seqs, table, heads, kv_heads, window, d ** -0.5)[shown]
+    assert ((got - want).abs() <= bound).all(), float(((got - want).abs() / bound).max())
