@@ -3123,7 +3123,7 @@ def rope_store_int8(qkv: torch.Tensor, q: torch.Tensor, token_pos: torch.Tensor,
                 page_table=(page_table, torch.int32, (None, None)), cos=(cos, torch.float32, (None, d // 2)),
                 sin=(sin, torch.float32, (half[0] if half else 0, d // 2)))
         raise KernelError("rope_store_int8: bad argument")
-    if n == 0:
+    if n == 0 or (turns and angles == 0):  # (every position lies beyond angles of none; their tables have no address)
         return
     if stream < 0:  # (another device is the current one)
         with torch.cuda.device(index):

@@ -105,3 +105,19 @@ def test_a_large_value_that_others_see(dtype, heads, kv_heads, d, window, at, se
                                   d ** -0.5, dtype == torch.float32)
     got = attend(q, k, v, ks, vs, positions, seqs, table, heads, kv_heads, window, d ** -0.5)[shown]
     assert ((got - want).abs() <= bound).all(), float(((got - want).abs() / bound).max())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [64, 40])
+def test_angles_of_no_position(dtype, d):
+    """Tables of angles without a row: every position lies beyond them, so nothing is written."""
+    from nnis_b200.csrc import ops
+    gen = torch.Generator().manual_seed(3)
+    k, ks = plain.store(2, 1, d, gen)
+    v, vs = plain.store(2, 1, d, gen)
+    stores = cuda(k, v, ks, vs)
+    q = torch.full((3, 2 * d), 7.0, dtype=dtype, device="cuda")
+    i32 = [torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([0, 5, 70], [0, 0, 0], [[1, 0]])]
+    none = torch.empty((0, d // 2), device="cuda")
+    ops.rope_store_int8(torch.randn((3, 4 * d), generator=gen).to(dtype).cuda(), q, *i32, none, none, *stores, 2, 1, d, PAGE)
+    assert (q == 7).all() and all(torch.equal(a.cpu(), b) for a, b in zip(stores, (k, v, ks, vs)))

@@ -388,3 +388,12 @@ def test_entries_refuse_what_has_no_address():
             assert ops._native(name)(*(0 if i == missing else at for i in range(places)), *sizes, 0) == -1, (name, missing)
     for missing in (1, 2, 4, 5, 6):
         assert ops._native("nnis_linear_int8")(*(0 if i in (missing, 3, 7) else at for i in range(8)), 0, 1, 16, 16, 0, 0, 148, 1, 0) == -1
+
+
+def test_angles_of_no_position_write_nothing(reached):
+    """Tables without a row have no address, and without an address nothing would be turned: no entry is reached."""
+    from nnis_b200.csrc import ops
+    ops.rope_store_int8(*store_args(cos=empty(0, 32), sin=empty(0, 32)))
+    assert not reached
+    with pytest.raises(ops.KernelError):
+        ops.rope_store_int8(*store_args(cos=empty(0, 31), sin=empty(0, 31)))
