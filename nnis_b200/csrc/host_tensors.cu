@@ -181,7 +181,8 @@ void* check(void* self, void* const* args, long count) {
     return nullptr;
 }
 
-// self: bytes, the address of an entry that takes a record, then the record's fields (p: an address, i: an int, f: a float), ended by a zero.
+// self: bytes, the address of an entry that takes a record, then the record's fields (p: an address or another whole number of 64 bits, i: an int, f: a
+// float), ended by a zero.
 // Called with their values: the entry's code, NNIS_ERR_ARGUMENT where a value is not one of its field.  The interpreter's lock is not held
 // meanwhile: a launch may have to wait for the launches ahead of it.
 void* call(void* self, void* const* args, long count) {

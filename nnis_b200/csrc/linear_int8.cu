@@ -217,12 +217,14 @@ static cudaError_t launch_quantize(const Quantize8& p, cudaStream_t stream) {
 
 }  // namespace nnis
 
-// codes [rows, kp], kp = k rounded up to a multiple of 16; scales [rows]
+// codes [rows, kp], kp = k rounded up to a multiple of 16; scales [rows].  Rows of x lie `x_stride` elements apart, 0 or less than k where they
+// share memory.
 struct Quantize8Call {
     const void* x;
     void* codes;
     float* scales;
-    int x_stride, dtype, rows, k;
+    long long x_stride;
+    int dtype, rows, k;
     cudaStream_t stream;
 };
 NNIS_API int nnis_quantize_rows(const void* call) {
@@ -230,7 +232,7 @@ NNIS_API int nnis_quantize_rows(const void* call) {
     Quantize8Call c;
     memcpy(&c, call, sizeof c);
     const auto [x, codes, scales, x_stride, dtype, rows, k, stream] = c;
-    if (!x || !codes || !scales || rows <= 0 || k <= 0 || k > 0x7ffffff0 || x_stride < k) return NNIS_ERR_ARGUMENT;
+    if (!x || !codes || !scales || rows <= 0 || k <= 0 || k > 0x7ffffff0 || x_stride < 0) return NNIS_ERR_ARGUMENT;
     if ((uintptr_t)codes % 16) return NNIS_ERR_ALIGNMENT;
     const Quantize8 p{x, x_stride, (int8_t*)codes, scales, rows, k, (k + 15) / 16 * 16, 1};
     if (dtype == NNIS_DTYPE_F32) return (int)launch_quantize<float>(p, stream);
@@ -271,7 +273,8 @@ struct Linear8Call {
     void *out, *codes;
     float* scales;
     int* status;
-    int x_stride, m, n, k, mode, dtype, sms, coded;
+    long long x_stride;
+    int m, n, k, mode, dtype, sms, coded;
     cudaStream_t stream;
 };
 NNIS_API int nnis_linear_int8(const void* call) {
@@ -280,7 +283,7 @@ NNIS_API int nnis_linear_int8(const void* call) {
     memcpy(&c, call, sizeof c);
     const auto [x, w, ws, bias, out, codes, scales, status, x_stride, m, n, k, mode, dtype, sms, coded, stream] = c;
     const int kp = (k + 15) / 16 * 16;
-    if ((!x && !coded) || !w || !ws || !out || (coded && (!codes || !scales)) || m <= 0 || n <= 0 || k <= 0 || (!coded && x_stride < k) || mode < 0 || mode > 3)
+    if ((!x && !coded) || !w || !ws || !out || (coded && (!codes || !scales)) || m <= 0 || n <= 0 || k <= 0 || (!coded && x_stride < 0) || mode < 0 || mode > 3)
         return NNIS_ERR_ARGUMENT;
     if (k > 133136 || (dtype != NNIS_DTYPE_F32 && dtype != NNIS_DTYPE_BF16)) return NNIS_ERR_UNSUPPORTED;
     if (((uintptr_t)codes | (uintptr_t)w) % 16) return NNIS_ERR_ALIGNMENT;

@@ -3046,8 +3046,8 @@ _CALLS8 = {
     "linear_int8": ("", *_VALUES8, "out any m n"), "linear_int8/float32": ("", *_VALUES8, "out float32 m n"),
     "linear_int8_coded": ("", *_CODED8, "out any m n"), "linear_int8_coded/float32": ("", *_CODED8, "out float32 m n")}
 _RECORDS8 = {"nnis_rope_store_int8": "pppppppppppiiiiiiiiiip", "nnis_read_pages_int8": "ppppppppiiiiiiiiip",
-             "nnis_attention_int8": "ppppppppppppiiiiiiiiiifiiiiiip", "nnis_quantize_rows": "pppiiiip", "nnis_rmsnorm_int8": "ppppiiifp",
-             "nnis_linear_int8": "ppppppppiiiiiiiip"}
+             "nnis_attention_int8": "ppppppppppppiiiiiiiiiifiiiiiip", "nnis_quantize_rows": "ppppiiip", "nnis_rmsnorm_int8": "ppppiiifp",
+             "nnis_linear_int8": "pppppppppiiiiiiip"}
 _TYPES8 = {"any": 0, "float32": 1, "int8": 2, "int32": 3}
 _host_functions = {}
 
@@ -3367,7 +3367,7 @@ def linear_int8(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, bias: 
                 workspace) -> None:
     """y = x . W^T (+ bias) with the rows of x put into 8-bit codes with a scale for every token (``quantize_rows``), W held in such
     codes with a scale for every row, w int8 [n, int8_width(k)], and the codes multiplied as whole numbers: the sum is exact, and
-    one float32 product with each scale follows.  x [m, k] float32 or bfloat16, bias float32 [n] or None.  ``mode``: STORE (out of
+    one float32 product with each scale follows.  x [m, k] float32 or bfloat16 in rows of any stride, bias float32 [n] or None.  ``mode``: STORE (out of
     x's type [m, n]), STORE_F32 or ADD_F32 (float32 [m, n], written or added to), GEMM_GATED (w = [gate; up] rows, out of x's type [m, n /
     2] = silu(gate) * up).  k at most 133,136: beyond it a sum could pass 32 bits."""
     name = "linear_int8" if mode == STORE or mode == GEMM_GATED else "linear_int8/float32"

@@ -121,3 +121,41 @@ def test_angles_of_no_position(dtype, d):
     none = torch.empty((0, d // 2), device="cuda")
     ops.rope_store_int8(torch.randn((3, 4 * d), generator=gen).to(dtype).cuda(), q, *i32, none, none, *stores, 2, 1, d, PAGE)
     assert (q == 7).all() and all(torch.equal(a.cpu(), b) for a, b in zip(stores, (k, v, ks, vs)))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,k", [(5, 64), (130, 96), (3, 37), (40, 2048), (2, 9000)])
+def test_rows_that_share_memory(dtype, rows, k):
+    """Rows of any stride: one row many times over, and rows that overlap."""
+    from nnis_b200.csrc import ops
+    from nnis_b200.engine.workspace import Workspace
+    gen = torch.Generator().manual_seed(k)
+    flat = torch.randn(k + 8 * rows, generator=gen).to(dtype).cuda()
+    w, w_scales = plain.codes_of(torch.randn((24, k), generator=gen))
+    w = torch.nn.functional.pad(w, (0, ops.int8_width(k) - k)).cuda()
+    w_scales = w_scales.cuda()
+    for x in (flat[:k].expand(rows, k), flat.as_strided((rows, k), (8, 1)), flat.as_strided((rows, k), (1, 1))):
+        got, want = ([torch.full((rows, ops.int8_width(k)), 9, dtype=torch.int8, device="cuda"), torch.full((rows,), 9.0, device="cuda")]
+                     for _ in range(2))
+        ops.quantize_rows(x, *got)
+        ops.quantize_rows(x.contiguous(), *want)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        outs = [torch.empty((rows, 24), dtype=dtype, device="cuda") for _ in range(2)]
+        for out, values in zip(outs, (x, x.contiguous())):
+            ops.linear_int8(values, w, w_scales, None, out, ops.STORE, Workspace(torch.device("cuda")))
+        assert torch.equal(*outs)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_rows_far_apart(dtype):
+    """Rows whose distance, in elements, passes 31 bits."""
+    from nnis_b200.csrc import ops
+    gen = torch.Generator().manual_seed(4)
+    apart, k = (1 << 31) + 8, 96
+    flat = torch.empty(2 * apart + k, dtype=dtype, device="cuda")
+    x = flat.as_strided((3, k), (apart, 1))
+    x.copy_(torch.randn((3, k), generator=gen).to(dtype))
+    got, want = ([torch.full((3, k), 9, dtype=torch.int8, device="cuda"), torch.full((3,), 9.0, device="cuda")] for _ in range(2))
+    ops.quantize_rows(x, *got)
+    ops.quantize_rows(x.contiguous(), *want)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])

@@ -397,3 +397,19 @@ def test_angles_of_no_position_write_nothing(reached):
     assert not reached
     with pytest.raises(ops.KernelError):
         ops.rope_store_int8(*store_args(cos=empty(0, 31), sin=empty(0, 31)))
+
+
+def test_rows_at_any_distance_are_passed_on(reached):
+    """Rows that are one row, that overlap, that lie further apart than 31 bits say; the entries take what they are passed."""
+    from nnis_b200.csrc import ops
+    for distance in (0, 1, 8, 39):
+        x = empty(400, dtype=BF16).as_strided((5, 40), (distance, 1))
+        ops.quantize_rows(x, empty(5, 48, dtype=I8), empty(5))
+        assert reached.pop()[1][3:] == (distance, 1, 5, 40, 0)
+        ops.linear_int8(*product_args(x=x, space=space()))
+        assert reached.pop()[1][8:] == (distance, 5, 12, 40, 0, 1, 148, 0, 0)
+    # (codes at an address that is refused after all else: nothing is launched)
+    at = 1 << 20
+    for distance in (0, 1, (1 << 31) + 8):
+        assert ops._native("nnis_quantize_rows")(at, at + 1, at, distance, 1, 1, 40, 0) == ops._native("nnis_quantize_rows")(at, at + 1, at, 40, 1, 1, 40, 0) != -1
+    assert ops._native("nnis_quantize_rows")(at, at, at, -1, 1, 1, 40, 0) == -1
