@@ -116,7 +116,7 @@ static cudaError_t launch_warps8(const Attend8& p, cudaStream_t stream) {
 
 // slice_pieces 0: a warp a row, head and slice, `partial` n * nq * splits * (d + 2) floats where splits > 1.  slice_pieces > 0: the tensor
 // cores' kernel (heads of 32, 64, 96, 128, pages of 64): rows_at_once rows of a sequence together, slices of that many runs of 64
-// positions (32 for heads of 96 and 128) that cover the whole table, each shared by a cluster of 1, 2, 4 or 8 CTAs (0: a
+// positions (32 for heads of 96 and 128), the last with what is left, each shared by a cluster of 1, 2, 4 or 8 CTAs (0: a
 // warp takes a unit alone), tiles of 8 or 16 queries; `partial` n * nq *
 // splits * (d + 4) floats and n * nkv * (heads of rows_at_once rows / 8, rounded up) tickets where splits > 1.
 struct Attend8Call {
@@ -152,7 +152,7 @@ NNIS_API int nnis_attention_int8(const void* call) {
         if (page_size != 64 || (d != 32 && d != 64 && d != 96 && d != 128) || (dtype != NNIS_DTYPE_F32 && dtype != NNIS_DTYPE_BF16))
             return NNIS_ERR_UNSUPPORTED;
         if (cluster == 0 ? splits != 1 : cluster != 1 && cluster != 2 && cluster != 4 && cluster != 8) return NNIS_ERR_UNSUPPORTED;
-        if (rows_at_once < 1 || tile_eights < 1 || tile_eights > 2 || !status || (splits > 1 && !tickets) || (long long)splits * slice_pieces < (d <= 64 ? 1LL : 2LL) * table_cols) return NNIS_ERR_ARGUMENT;
+        if (rows_at_once < 1 || tile_eights < 1 || tile_eights > 2 || !status || (splits > 1 && !tickets)) return NNIS_ERR_ARGUMENT;
         if (((uintptr_t)k | (uintptr_t)v | (uintptr_t)k_scales | (uintptr_t)v_scales | (uintptr_t)out | (uintptr_t)partial) % 16)
             return NNIS_ERR_ALIGNMENT;
         return (int)attend_int8_mma(p, dtype == NNIS_DTYPE_F32, stream);

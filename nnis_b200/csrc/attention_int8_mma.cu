@@ -18,7 +18,8 @@
 //
 // A CTA: four warps, (run of rows with one sequence, key/value head, tile of queries, slice of positions); a warp takes every fourth piece
 // of 64 or 32 positions of the slice through a ring of its own, filled by bulk copies, so that nothing meets before the slice's end.  Slices are of a
-// fixed number of pieces, so sequences of all lengths are cut into equal pieces; the slice that ends last joins them.
+// fixed number of pieces, so sequences of all lengths are cut into equal pieces (where a run's rows lie further apart than its window is
+// long, the last slice has what the others leave); the slice that ends last joins them.
 #include <float.h>
 #include <string.h>
 
@@ -287,9 +288,9 @@ __global__ void __launch_bounds__(kWarps8 * 32, D <= 32 ? 4 : D <= 96 ? 3 : 2) a
         constexpr int kHalves = kPage8 / kPiece8;
         const int piece_low = known ? low / kPiece8 : 0, piece_top = known ? (int)min((long long)top_pos / kPiece8 + 1, (long long)kHalves * p.table_cols) : 0;
         // a slice's pieces are dealt out to all warps of its cluster
-        const int slices = max(1, (piece_top - piece_low + p.slice_pieces - 1) / p.slice_pieces);
+        const int slices = max(1, min(p.splits, (piece_top - piece_low + p.slice_pieces - 1) / p.slice_pieces));
         if (!SOLO && slice >= slices) continue;
-        const int first = SOLO ? piece_low : piece_low + slice * p.slice_pieces, last = SOLO ? piece_top : min(piece_top, first + p.slice_pieces);
+        const int first = SOLO ? piece_low : piece_low + slice * p.slice_pieces, last = SOLO || slice == slices - 1 ? piece_top : first + p.slice_pieces;
         const int step = SOLO ? 1 : kWarps8 * p.cluster;
 
         // ---- copies: this warp's pieces are every step-th; those of pages outside the store are passed over.  The next

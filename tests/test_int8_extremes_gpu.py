@@ -108,6 +108,30 @@ def test_a_large_value_that_others_see(dtype, heads, kv_heads, d, window, at, se
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv_heads,d,sequences,window,tokens", [(32, 8, 128, 8, 2100, 1), (9, 3, 64, 32, 2100, 1), (32, 8, 128, 8, 1300, 2),
+                                                                     (9, 3, 64, 32, 2200, 2), (8, 8, 32, 16, 3000, 2), (12, 4, 96, 24, 1999, 2)])
+def test_windows_that_several_slices_share(dtype, heads, kv_heads, d, sequences, window, tokens):
+    """Windows cut into slices, at positions all over a piece; of several rows of a sequence some lie further apart than a window is long,
+    so that what they see together is more than the slices' parts."""
+    from nnis_b200.csrc import ops
+    gen = torch.Generator().manual_seed(window)
+    lengths = [4600 - 37 * i for i in range(sequences)]
+    table, pages = place(lengths, gen)
+    positions = [n - 1 - j * (1 if i % 2 else 1450) for i, n in enumerate(lengths) for j in range(tokens)]
+    seqs = [i for i in range(sequences) for _ in range(tokens)]
+    slices, pieces, rows, cluster, _ = ops.attention_int8_plan(len(positions), sequences, heads, kv_heads, d, len(table[0]), window,
+                                                               ops.sm_count(torch.device("cuda:0")))
+    assert rows == tokens and slices > 1 and ops.attention_int8_slice(slices, pieces, rows, d, window) < pieces
+    k, ks = plain.store(pages, kv_heads, d, gen)
+    v, vs = plain.store(pages, kv_heads, d, gen)
+    q = (1.5 * torch.randn((len(positions), heads * d), generator=gen)).to(dtype)
+    shown = list(range(6))
+    want, bound = plain.attention(q[shown], k, v, ks, vs, positions[:6], seqs[:6], table, heads, kv_heads, window, d ** -0.5, dtype == torch.float32)
+    got = attend(q, k, v, ks, vs, positions, seqs, table, heads, kv_heads, window, d ** -0.5)[shown]
+    assert ((got - want).abs() <= bound).all(), float(((got - want).abs() / bound).max())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("d", [64, 40])
 def test_angles_of_no_position(dtype, d):
     """Tables of angles without a row: every position lies beyond them, so nothing is written."""

@@ -413,3 +413,22 @@ def test_rows_at_any_distance_are_passed_on(reached):
     for distance in (0, 1, (1 << 31) + 8):
         assert ops._native("nnis_quantize_rows")(at, at + 1, at, distance, 1, 1, 40, 0) == ops._native("nnis_quantize_rows")(at, at + 1, at, 40, 1, 1, 40, 0) != -1
     assert ops._native("nnis_quantize_rows")(at, at, at, -1, 1, 1, 40, 0) == -1
+
+
+@pytest.mark.parametrize("d", [32, 64, 96, 128])
+def test_slices_share_what_a_window_shows(d):
+    """The pieces that a run of rows can see, wherever its window begins, fall to all slices alike, and to no more of them than the plan has."""
+    from nnis_b200.csrc import ops
+    length, cut = 64 if d <= 64 else 32, 0
+    for n, seqs in ((1, 1), (4, 4), (8, 8), (32, 32), (5, 1), (64, 16)):
+        for heads, kv_heads in ((9, 3), (32, 8), (32, 32), (16, 2)):
+            for cols in (1, 3, 64, 512, 4096):
+                for window in (1, 63, 64, 1000, 4096, 5000):
+                    slices, pieces, rows, cluster, _ = ops.attention_int8_plan(n, seqs, heads, kv_heads, d, cols, window, 148)
+                    got = ops.attention_int8_slice(slices, pieces, rows, d, window)
+                    # (window + rows - 1 keys in a row lie on so many pieces at most; equal parts of them are what a slice can have at best, and
+                    # one more piece than there can be may be counted)
+                    most = min((window + rows + length - 3) // length + 1, cols * 64 // length)
+                    assert slices * got >= most and (slices == 1 or got <= -(-(most + 1) // slices))
+                    cut += slices > 1
+    assert cut > 20  # (some are cut)
