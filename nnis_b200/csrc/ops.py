@@ -3169,6 +3169,11 @@ def read_pages_int8(k: torch.Tensor, v: torch.Tensor, k_scales: torch.Tensor, v_
 # of 1,000 23 / 48, 43 / 56, 85 / 53, of 4,000 63 / 184, 121 / 162, 223 / 186; float32: 9 and 3 heads of 64, eight of 4,000 26 / 112, 43 / 113,
 # 66 / 10,990; 32 and 8 of 128 106 / 1,752, 190 / 1,759, 361 / 1,768.
 INT8_ROWS_AT_ONCE = {torch.bfloat16: 32, torch.float32: 64}
+# ... unless another sequence of the step brings more and the few tokens' contexts, read back, are at most this many bytes a layer (or no longer
+# than the others'): one kernel for all of a step's rows costs less than two until then.  ms a step of four layers, a prompt of 200 tokens
+# beside n single tokens at contexts of 4,000, all read back / the single tokens on the codes: 32 heads of 64 (63 MB a context), n = 1, 2, 3, 4, 8,
+# 63 1.02 / 1.08, 1.05 / 1.12, 1.10 / 1.14, 1.22 / 1.20, 1.44 / 1.43, 4.94 / 2.00 and 4 GB of scratch; 3 heads of 64, n = 63 1.41 / 0.83.
+INT8_READ_BACK = 5 << 25
 
 
 def attention_int8_splits(n: int, heads: int, keys: int, device) -> int:

@@ -338,7 +338,7 @@ class Engine:
         """Second time a prompt shape is seen: run it into buffers of its own (this
         run's logits are the step's result), then record the same launches as a graph
         for the next time."""
-        workspace = Workspace(self.device)
+        workspace = Workspace(self.device, beside=self.workspace)
         ctx, d_want, slots, new_lengths = self.prepare(batch, workspace)
         dev = workspace.get("step_ints", (self._staged,), torch.int32)
         ints = self._staging[:self._staged].clone().pin_memory()

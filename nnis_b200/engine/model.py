@@ -51,10 +51,12 @@ class DecoderModel:
             if value not in (None, "int8"):
                 raise ValueError(f"{what} must be None or 'int8'; got {value!r}")
         self.weights_in_int8 = weight_dtype == "int8"
+        mixers = [b.mixer for b in self.blocks if b.mixer is not None]
+        widest = max((m.kv_heads * m.head_dim for m in mixers if hasattr(m, "cache_in_int8")), default=0)
         for layer, block in enumerate(self.blocks):
             if cache_dtype == "int8" and block.mixer is not None:
                 if getattr(block.mixer, "cache_in_int8", None) is not None:
-                    block.mixer.cache_in_int8()
+                    block.mixer.cache_in_int8(widest)
                 else:
                     raise ValueError(f"cache_dtype='int8': layer {layer}'s mixer ({type(block.mixer).__name__}) has no 8-bit cache")
             for part in block.parts() if self.weights_in_int8 else ():

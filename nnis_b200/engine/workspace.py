@@ -9,7 +9,7 @@ from __future__ import annotations
 
 import contextlib
 import gc
-from typing import Dict, Tuple
+from typing import Dict, Optional, Tuple
 
 import torch
 
@@ -29,8 +29,10 @@ def recording(graph: torch.cuda.CUDAGraph):
 
 
 class Workspace:
-    def __init__(self, device: torch.device):
+    def __init__(self, device: torch.device, beside: Optional["Workspace"] = None):
+        """``beside``: the workspace of other steps that run before or after this one's, never at the same time (``lent``)."""
         self.device = device
+        self._beside = beside
         self._buffers: Dict[Tuple[str, torch.dtype], torch.Tensor] = {}
         self._frozen = False
         self._children: Dict[str, "Workspace"] = {}
@@ -73,6 +75,23 @@ class Workspace:
                 raise RuntimeError(f"workspace buffer {name!r} would move after graph capture")
             # grow with headroom so a slowly growing batch does not reallocate each step
             buf = torch.empty(max(count, 1), dtype=dtype, device=self.device)
+            self._buffers[key] = buf
+        return buf[:count].view(*shape)
+
+    def lent(self, name: str, shape, dtype: torch.dtype) -> torch.Tensor:
+        """Like ``get``, for large scratch that is written and read within a layer: a captured step's is that of the workspace ``beside`` it
+        where that is large enough (whoever has used a buffer keeps it, so a graph's stays where it is)."""
+        count, key = 1, (name + "#lent", dtype)
+        for s in shape:
+            count *= int(s)
+        buf = self._buffers.get(key)
+        if buf is None or buf.numel() < count:
+            if self.frozen:
+                raise RuntimeError(f"workspace buffer {name!r} would move after graph capture")
+            owner = self if self._beside is None else self._beside
+            buf = owner._buffers.get(key)
+            if buf is None or buf.numel() < count:
+                buf = owner._buffers[key] = torch.empty(max(count, 1), dtype=dtype, device=self.device)
             self._buffers[key] = buf
         return buf[:count].view(*shape)
 

@@ -14,7 +14,7 @@ model hands it (another schedule entry's).
 
 The cache may be held in 8 bits (``cache_in_int8``) and the matrices too (``hold_int8``).  With an 8-bit cache the rows are
 projected, then rotated and put into codes by one kernel; single tokens, and a few of a sequence, read the codes as they are, and a
-prompt step reads its sequences' pages back into scratch, a layer at a time, and takes the kernels of the 16-bit (or float32) cache.
+prompt step reads its prompts' pages back into scratch, a layer at a time, and takes the kernels of the 16-bit (or float32) cache.
 """
 from __future__ import annotations
 
@@ -92,9 +92,10 @@ class Attention(Part):
         return sum(matrix_bytes(t) for t in (self.w_qkv, self.w_o, self.b_qkv, self.b_o))
 
     # -- cache ------------------------------------------------------------
-    def cache_in_int8(self) -> None:
-        """Keys and values are held in 8-bit codes with a scale for every position and head."""
-        self.codes = True
+    def cache_in_int8(self, widest: int = 0) -> None:
+        """Keys and values are held in 8-bit codes with a scale for every position and head.  ``widest``: the most values that a position's keys
+        have in a layer of the model."""
+        self.codes, self.widest = True, max(widest, self.kv_heads * self.head_dim)
 
     def cache_request(self) -> Optional[KVRequest]:
         return KVRequest(self.kv_heads, self.head_dim, self.window, codes=self.codes) if self.own_kv else None
@@ -137,13 +138,24 @@ class Attention(Part):
     def _read_back_name(self) -> str:
         return f"int8_pages/window{self.window}"
 
+    def _reads_codes(self, counts, starts):
+        """For each sequence of a step, whether its rows read the 8-bit cache as it is.  Those that bring few tokens do, unless others bring
+        many and the few ones' contexts are no longer than theirs, or read back take no more than ``ops.INT8_READ_BACK`` bytes: all then go
+        one way, for the launches.  The same in all layers, whose kernels share work lists (so whole contexts count, whatever the window)."""
+        few = [c <= ops.INT8_ROWS_AT_ONCE[self.dtype] for c in counts]
+        pages = [-(-(s + c) // PAGE_SIZE) for c, s in zip(counts, starts)]
+        short = sum(p for p, f in zip(pages, few) if f)
+        apart = short > sum(pages) - short and short * PAGE_SIZE * 2 * self.widest * self.dtype.itemsize > ops.INT8_READ_BACK
+        return few if all(few) or apart else [False] * len(few)
+
     def _read_back_table(self, counts, starts):
         """Which pages of an 8-bit cache a prompt step reads back, and to which places: [sequences, columns], -1 for pages that lie
-        before every window.  None where every sequence brings few tokens: their rows read the codes as they are."""
-        if max(counts) <= ops.INT8_ROWS_AT_ONCE[self.dtype]:
+        before every window and for sequences that read the codes as they are.  None where all do."""
+        codes = self._reads_codes(counts, starts)
+        if all(codes):
             return None
-        spans = [(max(0, s - self.window + 1) // PAGE_SIZE if self.window > 0 else 0, -(-(s + c) // PAGE_SIZE))
-                 for c, s in zip(counts, starts)]
+        spans = [(0, 0) if own else (max(0, s - self.window + 1) // PAGE_SIZE if self.window > 0 else 0, -(-(s + c) // PAGE_SIZE))
+                 for own, c, s in zip(codes, counts, starts)]
         table = np.full((len(spans), max(b for _, b in spans)), -1, dtype=np.int32)
         at = 0
         for row, (a, b) in zip(table, spans):
@@ -160,21 +172,23 @@ class Attention(Part):
         mma.sync kernel (head sizes 64 and 128), the same for every layer.  In float32
         the units of the tensor cores' kernel (head size 64) where it pays; 64-query tiles, the ones
         with the most keys first, for other head sizes and for steps of single pages, where those pay.
-        With an 8-bit cache, before all: the pages to read back."""
-        if self.codes:
-            name = self._read_back_name()
-            if name + "/pages" in have:  # (a layer of this window has asked)
-                places, read = {}, None
-            else:
-                read = self._read_back_table(counts, starts)
-                places = {name + "/pages": np.asarray([read[1] if read else 0], dtype=np.int32)}
-                if read:
-                    places[name] = read[0]
-            if max(counts) <= ops.INT8_ROWS_AT_ONCE[self.dtype]:
-                return places
-            places.update(self._kernel_tables(counts, starts, have))
-            return places
-        return self._kernel_tables(counts, starts, have)
+        With an 8-bit cache, before all: the pages to read back, and the rows that read the codes beside them."""
+        if not self.codes:
+            return self._kernel_tables(counts, starts, have)
+        name, codes, places = self._read_back_name(), self._reads_codes(counts, starts), {}
+        if name + "/pages" not in have:  # (else a layer of this window has asked)
+            read = self._read_back_table(counts, starts)
+            places[name + "/pages"] = np.asarray([read[1] if read else 0], dtype=np.int32)
+            if read:
+                places[name] = read[0]
+                if any(codes):  # the packed rows of neighbours that read the codes: [runs, 2], first and end
+                    ends = np.cumsum(counts)
+                    edges = [int(e) for e, a, b in zip([0, *ends], [False, *codes], [*codes, False]) if a != b]
+                    places[name + "/codes"] = np.asarray(edges, dtype=np.int32).reshape(-1, 2)
+        if not all(codes):
+            places.update(self._kernel_tables([0 if own else c for own, c in zip(codes, counts)],
+                                              [0 if own else s for own, s in zip(codes, starts)], have))
+        return places
 
     def _kernel_tables(self, counts, starts, have):
         if self.dtype != torch.bfloat16:
@@ -344,8 +358,11 @@ class Attention(Part):
                                nq, self.stored_kv, d, cache.page_size)
                 q_buf, q_stride = qkv, qkv.shape[1]
         from_codes = self.codes and (ctx.decode or self._read_back_name() not in ctx.tables)
+        held, held_table, apart = cache, table, ()
         if self.codes and not from_codes:
             cache, table = self._read_back(ctx, cache, table)
+            runs = ctx.host_tables.get(self._read_back_name() + "/codes")
+            apart = runs.tolist() if runs is not None else ()
         if from_codes:
             ops.attention_int8(q_buf, q_stride, cache.k, cache.v, cache.k_scales, cache.v_scales, ctx.token_pos, ctx.token_seq, table,
                                attn, nq, nkv, d, self.window, self.scale, ws)
@@ -420,6 +437,9 @@ class Attention(Part):
                 if splits > 1 else None
             ops.attention_generic(q_buf, q_stride, cache.k, cache.v, ctx.token_pos, ctx.token_seq,
                                   table, attn, nq, nkv, d, self.window, self.scale, splits, partial)
+        for a, b in apart:  # (last: a kernel of rows, not tiles, has written zeros for these, whose pages were not read back)
+            ops.attention_int8(q_buf[a:b], q_stride, held.k, held.v, held.k_scales, held.v_scales, ctx.token_pos[a:b], ctx.token_seq[a:b],
+                               held_table, attn[a:b], nq, nkv, d, self.window, self.scale, ws)
         if self._fused_out(ctx, n):
             ops.gemv_bf16(self.w_o, self.b_o, residual, ops.EPI_ADD_F32, x=attn, emit=begin_norm(ctx, n, self.hidden),
                           split=ops.gemv_split(n, *self.w_o.shape, ws))
@@ -431,7 +451,7 @@ class Attention(Part):
         name, ws = self._read_back_name(), ctx.workspace
         local, pages = ctx.tables[name], int(ctx.host_tables[name + "/pages"][0])
         shape = (pages, self.kv_heads, cache.page_size, self.head_dim)
-        k, v = ws.get("int8_k_read", shape, self.dtype), ws.get("int8_v_read", shape, self.dtype)
+        k, v = ws.lent("int8_k_read", shape, self.dtype), ws.lent("int8_v_read", shape, self.dtype)
         ops.read_pages_int8(cache.k, cache.v, cache.k_scales, cache.v_scales, table, local, k, v)
         return KVView(cache.group, k, v, cache.page_size, cache.window), local
 

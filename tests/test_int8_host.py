@@ -432,3 +432,49 @@ def test_slices_share_what_a_window_shows(d):
                     assert slices * got >= most and (slices == 1 or got <= -(-(most + 1) // slices))
                     cut += slices > 1
     assert cut > 20  # (some are cut)
+
+
+def test_a_step_reads_back_what_long_sequences_have(monkeypatch):
+    """Beside a prompt, sequences with few tokens and long contexts read the codes: their pages are not read back, no kernel of prompts has
+    work for them, and their rows are named.  The bytes read back are bounded by that."""
+    from nnis_b200.config import config_from_dict
+    from nnis_b200.csrc import ops
+    from nnis_b200.engine.model import DecoderModel
+    from helpers import TINY_A
+    spec = config_from_dict(TINY_A).to_spec()
+    for dtype, many in ((BF16, 33), (F32, 65)):
+        mixer = DecoderModel(spec, dtype, torch.device("cpu"), "int8").blocks[0].mixer
+        name = mixer._read_back_name()
+        counts, starts = [1, 5, many, 1, 200, 1], [500, 90, 0, 64, 130, 4000]
+        both = mixer.step_tables(counts, starts)
+        assert name + "/codes" not in both and both[name + "/pages"].tolist() == [8 + 2 + -(-many // 64) + 2 + 6 + 63]
+        monkeypatch.setattr(ops, "INT8_READ_BACK", 0)
+        tables = mixer.step_tables(counts, starts)
+        assert tables[name + "/pages"].tolist() == [-(-many // 64) + 6] and tables[name].shape[1] == 6
+        assert [row for row, line in enumerate(tables[name].tolist()) if max(line) >= 0] == [2, 4]
+        assert tables[name + "/codes"].tolist() == [[0, 6], [6 + many, 7 + many], [207 + many, 208 + many]]
+        for key in tables:
+            if key.endswith("/units") or key == mixer.TILES_64 or key.startswith("prefill_f32"):
+                assert set(tables[key][:, 0].tolist()) == {2, 4}
+        assert set(mixer.step_tables(counts, starts, tuple(tables))) <= set(tables) - {name, name + "/pages", name + "/codes"}
+        # contexts of few tokens that are no longer than the others' go with them
+        assert name + "/codes" not in mixer.step_tables([1, many, 300], [100, 64, 1])
+        monkeypatch.undo()
+        # a server's step: 63 contexts of 4,000 and a prompt of 200 tokens, a layer of 32 heads of 64
+        mixer.widest = 2048
+        tables = mixer.step_tables([1] * 63 + [200], [4000] * 63 + [0])
+        assert tables[name + "/pages"].tolist() == [4] and tables[name + "/codes"].tolist() == [[0, 63]]
+
+
+def test_scratch_that_steps_lend_one_another():
+    from nnis_b200.engine.workspace import Workspace
+    own = Workspace(torch.device("cpu"))
+    first, second, other = (Workspace(torch.device("cpu"), beside=own) for _ in range(3))
+    a = first.lent("k", (3, 4), F32)
+    first.frozen = True
+    assert own.lent("k", (2, 4), F32).data_ptr() == a.data_ptr() == second.lent("k", (12,), F32).data_ptr() != second.get("k", (12,), F32).data_ptr()
+    larger = second.lent("k", (13,), F32)  # (the first keeps what its graph holds)
+    assert larger.data_ptr() != a.data_ptr() == first.lent("k", (12,), F32).data_ptr() and larger.data_ptr() == other.lent("k", (5,), F32).data_ptr()
+    with pytest.raises(RuntimeError, match="would move"):
+        first.lent("k", (13,), F32)
+    assert own.lent("k", (13,), F32).data_ptr() == larger.data_ptr() and own.lent("k", (1,), BF16).dtype == BF16

@@ -229,3 +229,37 @@ def test_drafted_steps_are_captured(dtype, tmp_path, monkeypatch):
     if dtype == "float32":
         assert got == want
     engine.check_status()
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("config", ["A", "D", "E"])
+def test_prompts_beside_single_tokens(dtype, config, tmp_path, monkeypatch):
+    """A step of two prompts among sequences that bring one token or a few, which attend over the codes while the prompts' pages are read back:
+    logits as of the same tokens step by step; run by run and replayed.  No more pages are read back than the prompts have."""
+    from nnis_b200.csrc import ops
+    from nnis_b200.engine import Engine, SequenceStep
+    monkeypatch.setattr(ops, "INT8_READ_BACK", 0)
+    engine = Engine.from_dir(make_model(str(tmp_path), {**MODELS[config], "max_position_embeddings": 2048}, 3), dtype=dtype, max_tokens=1 << 14,
+                             cache_dtype="int8")
+    read, real = [], ops.read_pages_int8
+    monkeypatch.setattr(ops, "read_pages_int8", lambda *a: (read.append(a[6].shape[0]), real(*a))[1])
+    vocab = engine.spec.vocab_size
+    held, new = [700, 1, 0, 300, 90, 650], [1, 3, 150, 1, 130, 5]
+    history = [[t % vocab for t in tokens(60 + i, a + 4 * b)] for i, (a, b) in enumerate(zip(held, new))]
+    slots = [engine.acquire_slot() for _ in held]
+    for s, h, n in zip(slots, history, held):
+        if n:
+            engine.step([SequenceStep(s, h[:n], [])])
+    want = []
+    for h, n, c in zip(history, held, new):
+        alone = engine.acquire_slot()
+        want.append(engine.step([SequenceStep(alone, h[:n + c], list(range(n, n + c)))]).cpu().numpy())
+        engine.release_slot(alone)
+    for turn in range(4):  # (captured in the second, replayed from the third on)
+        read.clear()
+        got = engine.step([SequenceStep(s, h[n:n + c], list(range(c))) for s, h, n, c in zip(slots, history, held, new)]).cpu().numpy()
+        assert set(read) <= {3 + 4}
+        near(got, np.concatenate(want), dtype)
+        for s, n in zip(slots, held):
+            engine.truncate(s, n)
+    engine.check_status()
