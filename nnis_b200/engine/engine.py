@@ -24,7 +24,7 @@ from ..cache import PAGE_SIZE, CacheManager
 from ..config import read_config
 from ..csrc import ops
 from ..config.spec import ModelSpec
-from ..weights import load_weights
+from ..weights import TensorsOnDemand, load_weights, open_weights
 from ..weights.loader import shape_fits
 from .context import StepContext
 from .model import DecoderModel
@@ -94,6 +94,9 @@ class Engine:
         device = require_cuda(device)
         spec = read_config(model_dir).to_spec()
         wanted = DecoderModel.weight_specs_of(spec)
+        if kwargs.get("weight_dtype") is not None:  # (matrices that need not fit in 16 bits, block by block)
+            with open_weights(model_dir, wanted, _DTYPES[dtype], device) as tensors:
+                return cls(spec, tensors, dtype, device, **kwargs)
         tensors = load_weights(model_dir, wanted, _DTYPES[dtype], device)
         return cls(spec, tensors, dtype, device, **kwargs)
 
@@ -112,7 +115,10 @@ class Engine:
             t = tensors[name]
             if not shape_fits(tuple(t.shape), tuple(ws.shape)):
                 raise ValueError(f"{name}: shape {list(t.shape)}, expected {list(ws.shape)}")
-            kept[name] = t.to(torch.float32 if ws.role == "vector" else compute).to(device).contiguous()
+            if kwargs.get("weight_dtype") is None:
+                kept[name] = t.to(torch.float32 if ws.role == "vector" else compute).to(device).contiguous()
+        if kwargs.get("weight_dtype") is not None:  # (block by block)
+            kept = TensorsOnDemand(wanted, lambda name: tensors[name], compute, device)
         return cls(spec, kept, dtype, device, **kwargs)
 
     # -- slots ----------------------------------------------------------------

@@ -81,13 +81,16 @@ class DecoderModel:
         return DecoderModel(spec, torch.float32, torch.device("cpu")).weight_specs()
 
     def load(self, tensors: Mapping[str, torch.Tensor]) -> None:
-        for part in (self.embedding, *self.blocks, self.final_norm, self.head):
+        """``tensors``: by name, on the device, of the kept types.  Blocks in 8 bits are put into codes one after another: of tensors that are
+        read on demand no more are held in 16 or 32 bits than a block's."""
+        self.embedding.load(tensors)
+        for block in self.blocks:
+            block.load(tensors)
+            for part in block.parts() if self.weights_in_int8 else ():
+                if getattr(part, "hold_int8", None) is not None:
+                    part.hold_int8()
+        for part in (self.final_norm, self.head):
             part.load(tensors)
-        if self.weights_in_int8:
-            for block in self.blocks:
-                for part in block.parts():
-                    if getattr(part, "hold_int8", None) is not None:
-                        part.hold_int8()
         self._enter_tensors = {name: tensors[name].to(torch.float32).contiguous() for name, _ in self._enter_names}
 
     def parameter_bytes(self) -> int:

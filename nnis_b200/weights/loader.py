@@ -16,11 +16,14 @@ stored in 32-bit stays 32-bit; integer tensors become int32.
 """
 from __future__ import annotations
 
+import contextlib
 import json
 import os
 import re
+import weakref
+from collections.abc import Mapping
 from dataclasses import dataclass
-from typing import Dict, List, Mapping, Tuple
+from typing import Callable, Dict, List, Tuple
 
 import torch
 
@@ -174,17 +177,41 @@ def check_weights(model_dir: str, wanted: Mapping[str, WeightSpec]) -> Dict[str,
             f.close()
 
 
-def load_weights(model_dir: str, wanted: Mapping[str, WeightSpec], compute_dtype: torch.dtype,
-                 device: torch.device) -> Dict[str, torch.Tensor]:
+class TensorsOnDemand(Mapping):
+    """Tensors by name, each read and brought to the device when it is asked for, so that whoever takes them one after another and
+    lets go of them holds no more than that.  One that is still held (an embedding's table that is the head's too) is given out again."""
+
+    def __init__(self, wanted: Mapping[str, WeightSpec], read: Callable[[str], torch.Tensor], compute_dtype: torch.dtype, device: torch.device):
+        self._roles = {name: spec.role for name, spec in wanted.items() if spec.role != "unused"}
+        self._read, self._compute, self._device = read, compute_dtype, device
+        self._held: "weakref.WeakValueDictionary[str, torch.Tensor]" = weakref.WeakValueDictionary()
+
+    def __getitem__(self, name: str) -> torch.Tensor:
+        role, held = self._roles[name], self._held.get(name)
+        if held is None:
+            t = self._read(name)
+            held = self._held[name] = t.to(_kept_dtype(role, t.dtype, self._compute)).to(self._device).contiguous()
+        return held
+
+    def __iter__(self):
+        return iter(self._roles)
+
+    def __len__(self) -> int:
+        return len(self._roles)
+
+
+@contextlib.contextmanager
+def open_weights(model_dir: str, wanted: Mapping[str, WeightSpec], compute_dtype: torch.dtype, device: torch.device):
+    """What ``load_weights`` gives, checked like it, as ``TensorsOnDemand`` for as long as the files are open."""
     files, where, _ = _open_and_check(model_dir, wanted)
     try:
-        out: Dict[str, torch.Tensor] = {}
-        for name, spec in wanted.items():
-            if spec.role == "unused":
-                continue
-            t = where[name].tensor(name)
-            out[name] = t.to(_kept_dtype(spec.role, t.dtype, compute_dtype)).to(device).contiguous()
-        return out
+        yield TensorsOnDemand(wanted, lambda name: where[name].tensor(name), compute_dtype, device)
     finally:
         for f in files:
             f.close()
+
+
+def load_weights(model_dir: str, wanted: Mapping[str, WeightSpec], compute_dtype: torch.dtype,
+                 device: torch.device) -> Dict[str, torch.Tensor]:
+    with open_weights(model_dir, wanted, compute_dtype, device) as tensors:
+        return dict(tensors)

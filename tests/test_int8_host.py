@@ -478,3 +478,56 @@ def test_scratch_that_steps_lend_one_another():
     with pytest.raises(RuntimeError, match="would move"):
         first.lent("k", (13,), F32)
     assert own.lent("k", (13,), F32).data_ptr() == larger.data_ptr() and own.lent("k", (1,), BF16).dtype == BF16
+
+
+def test_tensors_are_read_when_they_are_asked_for(tmp_path):
+    """By file and role as the loader keeps them; what is still held is given out again, what nobody holds is read anew."""
+    from helpers import TINY_A, make_model
+    from nnis_b200.config import read_config
+    from nnis_b200.engine.model import DecoderModel
+    from nnis_b200.weights import TensorsOnDemand, WeightError, load_weights, open_weights
+    made = make_model(str(tmp_path / "m"), TINY_A, 3)
+    wanted = DecoderModel.weight_specs_of(read_config(made).to_spec())
+    for dtype in (F32, BF16):
+        eager = load_weights(made, wanted, dtype, torch.device("cpu"))
+        with open_weights(made, wanted, dtype, torch.device("cpu")) as tensors:
+            assert isinstance(tensors, TensorsOnDemand) and set(tensors) == set(eager) and len(tensors) == len(eager)
+            for name, t in eager.items():
+                assert tensors[name].dtype == t.dtype and torch.equal(tensors[name], t)
+    reads = []
+    lazy = TensorsOnDemand(wanted, lambda name: (reads.append(name), eager[name].clone())[1], BF16, torch.device("cpu"))
+    name = next(n for n, w in wanted.items() if w.role == "matrix")
+    held = lazy[name]
+    assert lazy[name] is held and reads == [name]
+    del held
+    assert torch.equal(lazy[name], eager[name]) and reads == [name] * 2
+    with pytest.raises(WeightError, match="missing"):
+        with open_weights(made, {**wanted, "more": wanted[name]}, BF16, torch.device("cpu")):
+            pass
+
+
+def test_blocks_are_put_into_codes_one_after_another(monkeypatch):
+    """A model in 8 bits holds the matrices of one block, at most, in 16."""
+    import weakref
+    from helpers import TINY_A
+    from nnis_b200.config import config_from_dict
+    from nnis_b200.csrc import ops
+    from nnis_b200.engine.model import DecoderModel
+    from nnis_b200.weights import TensorsOnDemand
+    spec = config_from_dict({**TINY_A, "num_hidden_layers": 6}).to_spec()
+    model = DecoderModel(spec, BF16, torch.device("cpu"), None, "int8")
+    wanted, given, most, done = model.weight_specs(), [], [0], []
+    monkeypatch.setattr(ops, "quantize_rows", lambda x, codes, scales: done.append(tuple(x.shape)))
+    blocks = {n for n, w in wanted.items() if w.role == "matrix" and ".layers." in n}
+
+    def read(name):
+        t = torch.zeros(wanted[name].shape)
+        if name in blocks:
+            most[0] = max(most[0], 1 + sum(r() is not None for r in given))
+        return t
+
+    lazy = TensorsOnDemand(wanted, read, BF16, torch.device("cpu"))
+    real = TensorsOnDemand.__getitem__
+    monkeypatch.setattr(TensorsOnDemand, "__getitem__", lambda self, name: (lambda t: (given.append(weakref.ref(t)) if name in blocks else None, t)[1])(real(self, name)))
+    model.load(lazy)
+    assert most[0] <= len(blocks) // 6 and len(done) == 6 * 4  # (q, k, v in one; gate and up in one)

@@ -263,3 +263,27 @@ def test_prompts_beside_single_tokens(dtype, config, tmp_path, monkeypatch):
         for s, n in zip(slots, held):
             engine.truncate(s, n)
     engine.check_status()
+
+
+@pytest.mark.parametrize("from_dir", [True, False])
+def test_loading_in_8_bits_takes_less_than_the_16_bit_weights(from_dir, tmp_path):
+    """Matrices that would not fit in 16 bits may be held in 8: at no time are there 16-bit tensors of more than a block beside the codes."""
+    from nnis_b200.config import read_config
+    from nnis_b200.engine import Engine
+    made = make_model(str(tmp_path), {**SHARED, "hidden_size": 768, "intermediate_size": 3000, "num_hidden_layers": 8, "head_dim": 64,
+                                      "num_attention_heads": 12, "num_key_value_heads": 4}, 3)
+    kept = load_plain_weights(made, True)
+    whole = 2 * sum(t.numel() for t in kept.values())
+    block = 2 * sum(t.numel() for name, t in kept.items() if ".layers.0." in name)
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    if from_dir:
+        engine = Engine.from_dir(made, max_tokens=64, weight_dtype="int8")
+    else:
+        engine = Engine.from_spec(read_config(made).to_spec(), {n: t.to(torch.bfloat16) for n, t in kept.items()}, max_tokens=64, weight_dtype="int8")
+    peak = torch.cuda.max_memory_allocated() - before
+    tables = engine.model.embedding.table.numel() * 2 * (1 if engine.model.head.weight is engine.model.embedding.table else 2)
+    # codes and scales, the tables, a block's tensors and what they are joined to; a page of cache and small things
+    assert peak < (whole - tables) // 2 * 1.02 + tables + 2 * block + (4 << 20) < 0.9 * whole
