@@ -266,7 +266,7 @@ NNIS_API int nnis_rmsnorm_int8(const void* call) {
 // x [m, k] (rows `x_stride` apart) is put into `codes` [m, kp] and `scales` [m] (or, one row or two, into shared memory), w [n (gated: 2
 // n), kp] codes, ws their scales, bias float32 like ws or null, out [m, n]: `dtype` (x's) in the modes 0 (store) and 3 (gated: silu(first half of w's rows) * the
 // second), float32 in 1 (store) and 2 (add).  `coded`:
-// `codes` and `scales` are there already.  Both may be null for rows that go into shared memory.
+// `codes` and `scales` are there already.  Both are null where the caller wants rows put into shared memory.
 struct Linear8Call {
     const void *x, *w;
     const float *ws, *bias;
@@ -290,7 +290,7 @@ NNIS_API int nnis_linear_int8(const void* call) {
     const bool f32 = dtype == NNIS_DTYPE_F32;
     const Linear8 p{(const int8_t*)codes, (const int8_t*)w, scales, ws, bias, out, m, n, kp, status, 0, x, x_stride, k};
     const int held = sms > 0 ? sms : 148;
-    if (!coded && linear_int8_fuses(p, mode == INT8_GATED, f32, held)) return (int)linear_int8_few(p, mode, f32, true, stream);
+    if (!codes && !scales && linear_int8_may_fuse(p, f32)) return (int)linear_int8_few(p, mode, f32, true, stream);
     if (!codes || !scales) return NNIS_ERR_ARGUMENT;
     const Quantize8 q{x, x_stride, (int8_t*)codes, scales, m, k, kp, 0};
     const cudaError_t e = coded ? cudaSuccess : f32 ? launch_quantize<float>(q, stream) : launch_quantize<bf16>(q, stream);

@@ -27,9 +27,9 @@ __device__ __forceinline__ float silu_gate(float gate, float up) {
     return gate * r * up;
 }
 
-// The product of few rows (`fused`: rows that are still values), whether they are few enough for that; of many (tcgen05).  `f32`: the
-// operands' type is float32.
-bool linear_int8_fuses(const Linear8& p, bool gated, bool f32, int sms);
+// The product of few rows (`fused`: rows that are still values, where the kernel takes them as such); of many (tcgen05).  `f32`: the operands'
+// type is float32.
+bool linear_int8_may_fuse(const Linear8& p, bool f32);
 cudaError_t linear_int8_few(const Linear8& p, int mode, bool f32, bool fused, cudaStream_t stream);
 int linear_int8_tc(Linear8 p, int mode, bool f32, int sms, cudaStream_t stream);
 

@@ -153,9 +153,8 @@ static cudaError_t launch_fused(const Linear8& p, cudaStream_t stream) {
     return launch_dependent(linear_int8_few_kernel<T, ADD, GATED, 1, 8, X>, ctas, 256, smem, stream, p);
 }
 
-bool linear_int8_fuses(const Linear8& p, bool gated, bool f32, int sms) {
-    const int ctas = gated ? (p.n + 7) / 8 : (p.n + 15) / 16;
-    return p.m <= kFusedRows && ctas <= sms && p.kp <= 16384 && p.k % 8 == 0 && p.x_stride % 8 == 0 && (uintptr_t)p.values % (f32 ? 16 : 8) == 0;
+bool linear_int8_may_fuse(const Linear8& p, bool f32) {
+    return p.m <= kFusedRows && p.kp <= 16384 && p.k % 8 == 0 && p.x_stride % 8 == 0 && (uintptr_t)p.values % (f32 ? 16 : 8) == 0;
 }
 
 cudaError_t linear_int8_few(const Linear8& p, int mode, bool f32, bool fused, cudaStream_t stream) {

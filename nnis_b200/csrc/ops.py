@@ -3408,7 +3408,7 @@ def linear_int8(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, bias: 
         with torch.cuda.device(index):
             return linear_int8(x, w, w_scales, bias, out, mode, workspace)
     sms = _sm_count.get(index) or sm_count(w.device)
-    # (what the library does: one or two rows become codes in the product's own kernel)
+    # one or two rows become codes in the product's own kernel, in every CTA, where each has an SM (linear_int8_few.cu has both sides' times)
     fused = m <= 2 and -(-n // (8 if mode == GEMM_GATED else 16)) <= sms and width <= 16384 and k % 8 == 0 and stride % 8 == 0 \
         and at_x % (16 if code == F32 else 8) == 0
     codes = 0 if fused else workspace.room("int8_codes", m * width, torch.int8).data_ptr()
