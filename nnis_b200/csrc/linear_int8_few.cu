@@ -1,6 +1,6 @@
 // Products of 8-bit codes with few rows (decode steps), bound by the bytes of W: a CTA's eight warps share 16 rows of W (gated: 8 gate
 // and the 8 up rows), each takes every eighth run of 64 places of K straight into registers, and multiplies them (mma.sync, signed
-// bytes, W as the 16-row operand) with up to 64 rows of x; the eight sums, whole numbers, are added in shared memory.
+// bytes, W as the 16-row operand) with up to 32 rows of x; the eight sums, whole numbers, are added in shared memory.
 //
 // Any order of K serves a sum: a lane holds 16 bytes of a row that lie side by side, so that a warp's load of 8 rows takes whole
 // 64-byte runs and no byte is moved afterwards.  The first loads of W go out ahead of the wait for the kernel that makes x's codes.
@@ -29,7 +29,7 @@ __device__ __forceinline__ void few_mma(int (&c)[4], uint32_t a0, uint32_t a1, u
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-constexpr int kFusedRows = 2;
+constexpr int kFusedRows = 2, kFewRows = 32;
 // NT: tiles of 8 rows of x; kFewWarps: 8, or 16 where there are fewer CTAs than SMs and a long K.
 // X: the type of x where its rows are still values (fused), int8_t where they are codes.
 // (up to eight rows of codes: registers for three CTAs an SM, which is asked for: 80 where the compiler takes 70 by itself and keeps fewer loads
@@ -158,6 +158,7 @@ bool linear_int8_may_fuse(const Linear8& p, bool f32) {
 }
 
 cudaError_t linear_int8_few(const Linear8& p, int mode, bool f32, bool fused, cudaStream_t stream) {
+    if (p.m > (fused ? kFusedRows : kFewRows)) return cudaErrorInvalidValue;
     if (fused) {
         if (mode == INT8_GATED) return f32 ? launch_fused<float, false, true, float>(p, stream) : launch_fused<bf16, false, true, bf16>(p, stream);
         if (mode == INT8_ADD_F32) return f32 ? launch_fused<float, true, false, float>(p, stream) : launch_fused<float, true, false, bf16>(p, stream);
