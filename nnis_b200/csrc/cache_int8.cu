@@ -362,7 +362,7 @@ NNIS_API int nnis_read_pages_int8(const void* call) {
     const long long codes = (long long)kv_heads * page_size * d;
     const int run = (dtype == NNIS_DTYPE_F32 ? 4 : 8) * 128;
     long long share = (codes + run * kReadAhead - 1) / (run * kReadAhead);
-    const long long fill = (8 * 148 + 2LL * seqs * local_cols - 1) / (2LL * seqs * local_cols), most = (codes + run - 1) / run;
+    const long long fill = (8LL * device_sms() + 2LL * seqs * local_cols - 1) / (2LL * seqs * local_cols), most = (codes + run - 1) / run;
     if (share < fill) share = fill < most ? fill : most;
     if (share > 65535) share = 65535;
     const dim3 grid((unsigned)(seqs * local_cols), (unsigned)share, 2);

@@ -16,7 +16,7 @@ struct Linear8 {
     int out_by_tma;
     const void* values;  // x before it is put into codes, rows `x_stride` apart, k values each
     long long x_stride;
-    int k;
+    int k, sms;
 };
 
 // silu(gate) * up with the two approximate instructions (2^x and 1 / x, relative error about 1e-7 each)

@@ -131,7 +131,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, kFewWarps == 8 && NT == 1 && s
 }
 
 // Warps of a CTA: 16 where there are fewer CTAs than SMs and a long K.
-static bool few_wide(unsigned ctas, const Linear8& p) { return ctas <= 148 && p.kp >= 2048 && p.m <= 16; }
+static bool few_wide(unsigned ctas, const Linear8& p) { return ctas <= (unsigned)p.sms && p.kp >= 2048 && p.m <= 16; }
 
 template <typename T, bool ADD, bool GATED>
 static cudaError_t launch_few(const Linear8& p, cudaStream_t stream) {
