@@ -183,3 +183,39 @@ def test_rows_far_apart(dtype):
     ops.quantize_rows(x, *got)
     ops.quantize_rows(x.contiguous(), *want)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv_heads,d", [(32, 8, 128), (6, 3, 40)])
+def test_a_store_of_more_than_2_31_codes(dtype, heads, kv_heads, d):
+    """Pages at the far end of a store, and of what they are read back to, hold and give what they do in a small one."""
+    from nnis_b200.csrc import ops
+    gen = torch.Generator().manual_seed(d)
+    pages = (1 << 31) // (kv_heads * PAGE * d) + 9
+    lengths, n = [500, 130], 70
+    table, small = place(lengths, gen)
+    qkv = torch.randn((n, (heads + 2 * kv_heads) * d), generator=gen).to(dtype).cuda()
+    at = [(i, p) for i, length in enumerate(lengths) for p in range(length - n // 2, length)]
+    token_seq, token_pos = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in zip(*at))
+    k, ks = plain.store(small, kv_heads, d, gen)
+    v, vs = plain.store(small, kv_heads, d, gen)
+    cos, sin = cuda(*plain.angles(500, d))
+    results = []
+    for count, first in ((small, 0), (pages, pages - small)):
+        stores = [torch.empty((count, *t.shape[1:]), dtype=t.dtype, device="cuda") for t in (k, v, ks, vs)]
+        for store, t in zip(stores, (k, v, ks, vs)):
+            store[first:] = t.cuda()
+        ids = torch.tensor(table, dtype=torch.int32)
+        ids = torch.where(ids < 0, ids, ids + first).cuda()
+        q = torch.empty((n, heads * d), dtype=dtype, device="cuda")
+        ops.rope_store_int8(qkv, q, token_pos, token_seq, ids, cos, sin, *stores, heads, kv_heads, d, PAGE)
+        outs = [torch.zeros((count, kv_heads, PAGE, d), dtype=dtype, device="cuda") for _ in range(2)]
+        ops.read_pages_int8(*stores, ids, ids, *outs)
+        from nnis_b200.engine.workspace import Workspace
+        attn = torch.empty_like(q)
+        ops.attention_int8(q, heads * d, *stores, token_pos, token_seq, ids, attn, heads, kv_heads, d, 0, d ** -0.5, Workspace(torch.device("cuda")))
+        results.append([q, attn, *(t[first:].clone() for t in (*stores, *outs))])
+        del stores, outs
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+    assert results[0][1].abs().amax() > 0

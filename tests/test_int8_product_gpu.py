@@ -215,3 +215,44 @@ def test_outputs_whose_rows_are_no_multiple_of_16_bytes(dtype, m, n, k, mode):
 def test_tiles_whose_k_several_ctas_share(dtype, m, n, k, mode):
     """In two, three, five and six parts, the last shorter than the others."""
     check(dtype, m, n, k, mode, bias=m % 2 == 0)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,width", [(1, 4), (3, 20), (7, 576), (40, 2048), (2, 8192), (5, 1028), (300, 64)])
+def test_a_norm_s_codes_are_the_nearest(dtype, n, width):
+    """Every code of a norm's row is the nearest whole number to what the row allows, and the product of these codes is theirs.
+
+    A thread adds width / 256 squares, 13 additions join the threads' sums, and the root halves that error; the mean, the epsilon, the root,
+    its inverse, and two products are seven roundings more: less than width / 256 + 24 of 2^-24.  So a value lies between the roundings to
+    `dtype` of two numbers that far apart, its quotient by the largest between two quotients, and its code within half a step of those (the
+    two roundings of the product with 127 / top: 2^-22 of at most 127)."""
+    from nnis_b200.csrc import ops
+    gen = torch.Generator().manual_seed(width + n)
+    x, w = 3.0 * torch.randn((n, width), generator=gen), 1 + 0.1 * torch.randn(width, generator=gen)
+    codes, scales = torch.full((n, ops.int8_width(width)), 77, dtype=torch.int8, device="cuda"), torch.empty(n, device="cuda")
+    ops.rmsnorm_int8(x.cuda(), w.cuda(), 1e-5, codes, scales, dtype)
+    got, got_scales = codes.cpu()[:, :width].double(), scales.cpu().double()[:, None]
+    assert (codes.cpu()[:, width:] == 0).all()
+    y = x.double() / torch.sqrt(x.double().square().mean(1, keepdim=True) + 1e-5) * w.double()
+    off = (width / 256 + 24) * 2.0 ** -24
+    # (rounded from 64 bits at once: through float32 first, a value could fall on the wrong side of a tie)
+    ends = [y.abs() * (1 + side * off) for side in (-1, 1)]
+    low, high = (round_to(e, dtype) for e in ends)
+    top_low, top_high = low.amax(1, keepdim=True), high.amax(1, keepdim=True)
+    assert (got_scales >= top_low / 127 * (1 - 2.0 ** -23)).all() and (got_scales <= top_high / 127 * (1 + 2.0 ** -23)).all()
+    least, most = 127 * low / top_high - 0.5 - 127 * 2.0 ** -22, 127 * high / top_low + 0.5 + 127 * 2.0 ** -22
+    assert (got.abs() >= least).all() and (got.abs() <= most).all() and (torch.sign(got) * torch.sign(y) >= 0).all()
+    assert ((most - least) < 1.01 + 254 * off).double().mean() > 0.9  # (few values may fall either way)
+    m, s = coded(torch.randn((24, width), generator=gen))
+    out = torch.empty((n, 24), device="cuda")
+    ops.linear_int8_coded(codes, scales, width, m, s, None, out, ops.STORE)
+    want = (got @ m.cpu()[:, :width].double().T) * got_scales * s.cpu().double()
+    # (the sum as float32, two products)
+    assert ((out.cpu().double() - want).abs() <= 3.01 * 2.0 ** -24 * want.abs() + 1e-37).all()
+
+
+def round_to(x, dtype):
+    """float64 to the nearest number of `dtype` (24 or 8 bits, ties to even), exactly."""
+    mantissa, exponent = torch.frexp(x)
+    bits = 24 if dtype == torch.float32 else 8
+    return torch.ldexp(torch.round(torch.ldexp(mantissa, torch.tensor(bits))), exponent - bits)
