@@ -288,8 +288,9 @@ NNIS_API int nnis_linear_int8(const void* call) {
     if (k > 133136 || (dtype != NNIS_DTYPE_F32 && dtype != NNIS_DTYPE_BF16)) return NNIS_ERR_UNSUPPORTED;
     if (((uintptr_t)codes | (uintptr_t)w) % 16) return NNIS_ERR_ALIGNMENT;
     const bool f32 = dtype == NNIS_DTYPE_F32;
-    const Linear8 p{(const int8_t*)codes, (const int8_t*)w, scales, ws, bias, out, m, n, kp, status, 0, x, x_stride, k, sms > 0 ? sms : device_sms()};
-    if (!codes && !scales && linear_int8_may_fuse(p, f32)) return (int)linear_int8_few(p, mode, f32, true, stream);
+    const Linear8 p{(const int8_t*)codes, (const int8_t*)w, scales, ws, bias, out, status, x, x_stride, m, n, kp, k, 0};
+    const int held = sms > 0 ? sms : device_sms();
+    if (!codes && !scales && linear_int8_may_fuse(p, f32)) return (int)linear_int8_few(p, mode, f32, true, held, stream);
     if (!codes || !scales) return NNIS_ERR_ARGUMENT;
     const Quantize8 q{x, x_stride, (int8_t*)codes, scales, m, k, kp, 0};
     const cudaError_t e = coded ? cudaSuccess : f32 ? launch_quantize<float>(q, stream) : launch_quantize<bf16>(q, stream);
@@ -297,6 +298,6 @@ NNIS_API int nnis_linear_int8(const void* call) {
     // us by few rows' kernel / by tcgen05: 16 rows 16,384 x 2,048 13.2 / 13.7, 2,048 x 8,192 8.8 / 11; 32 rows 960 x 576 4.5 / 5.9,
     // 2,048 x 2,048 6.1 / 6.4, 6,144 x 2,048 9.1 / 8.2, 2,048 x 8,192 14.4 / 11.1, 16,384 x 2,048 18.0 / 13.5
     const long long bytes = (long long)(mode == INT8_GATED ? 2 : 1) * n * kp;
-    if (m <= 16 || (m <= 32 && bytes < 8 << 20)) return (int)linear_int8_few(p, mode, f32, false, stream);
-    return linear_int8_tc(p, mode, f32, p.sms, stream);
+    if (m <= 16 || (m <= 32 && bytes < 8 << 20)) return (int)linear_int8_few(p, mode, f32, false, held, stream);
+    return linear_int8_tc(p, mode, f32, held, stream);
 }

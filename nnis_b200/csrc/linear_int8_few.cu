@@ -131,12 +131,12 @@ __global__ void __launch_bounds__(kFewWarps * 32, kFewWarps == 8 && NT == 1 && s
 }
 
 // Warps of a CTA: 16 where there are fewer CTAs than SMs and a long K.
-static bool few_wide(unsigned ctas, const Linear8& p) { return ctas <= (unsigned)p.sms && p.kp >= 2048 && p.m <= 16; }
+static bool few_wide(unsigned ctas, const Linear8& p, int sms) { return ctas <= (unsigned)sms && p.kp >= 2048 && p.m <= 16; }
 
 template <typename T, bool ADD, bool GATED>
-static cudaError_t launch_few(const Linear8& p, cudaStream_t stream) {
+static cudaError_t launch_few(const Linear8& p, int sms, cudaStream_t stream) {
     const unsigned ctas = (unsigned)((p.n + (GATED ? 7 : 15)) / (GATED ? 8 : 16));
-    if (few_wide(ctas, p)) {
+    if (few_wide(ctas, p, sms)) {
         auto kernel = p.m <= 8 ? linear_int8_few_kernel<T, ADD, GATED, 1, 16> : linear_int8_few_kernel<T, ADD, GATED, 2, 16>;
         return launch_dependent(kernel, ctas, 512, 0, stream, p);
     }
@@ -146,10 +146,10 @@ static cudaError_t launch_few(const Linear8& p, cudaStream_t stream) {
 }
 
 template <typename T, bool ADD, bool GATED, typename X>
-static cudaError_t launch_fused(const Linear8& p, cudaStream_t stream) {
+static cudaError_t launch_fused(const Linear8& p, int sms, cudaStream_t stream) {
     const unsigned ctas = (unsigned)((p.n + (GATED ? 7 : 15)) / (GATED ? 8 : 16));
     const size_t smem = (size_t)p.m * (((p.kp + 63) / 64) | 1) * 64;
-    if (few_wide(ctas, p)) return launch_dependent(linear_int8_few_kernel<T, ADD, GATED, 1, 16, X>, ctas, 512, smem, stream, p);
+    if (few_wide(ctas, p, sms)) return launch_dependent(linear_int8_few_kernel<T, ADD, GATED, 1, 16, X>, ctas, 512, smem, stream, p);
     return launch_dependent(linear_int8_few_kernel<T, ADD, GATED, 1, 8, X>, ctas, 256, smem, stream, p);
 }
 
@@ -157,18 +157,18 @@ bool linear_int8_may_fuse(const Linear8& p, bool f32) {
     return p.m <= kFusedRows && p.kp <= 16384 && p.k % 8 == 0 && p.x_stride % 8 == 0 && (uintptr_t)p.values % (f32 ? 16 : 8) == 0;
 }
 
-cudaError_t linear_int8_few(const Linear8& p, int mode, bool f32, bool fused, cudaStream_t stream) {
+cudaError_t linear_int8_few(const Linear8& p, int mode, bool f32, bool fused, int sms, cudaStream_t stream) {
     if (p.m > (fused ? kFusedRows : kFewRows)) return cudaErrorInvalidValue;
     if (fused) {
-        if (mode == INT8_GATED) return f32 ? launch_fused<float, false, true, float>(p, stream) : launch_fused<bf16, false, true, bf16>(p, stream);
-        if (mode == INT8_ADD_F32) return f32 ? launch_fused<float, true, false, float>(p, stream) : launch_fused<float, true, false, bf16>(p, stream);
+        if (mode == INT8_GATED) return f32 ? launch_fused<float, false, true, float>(p, sms, stream) : launch_fused<bf16, false, true, bf16>(p, sms, stream);
+        if (mode == INT8_ADD_F32) return f32 ? launch_fused<float, true, false, float>(p, sms, stream) : launch_fused<float, true, false, bf16>(p, sms, stream);
         if (mode == INT8_STORE_F32)
-            return f32 ? launch_fused<float, false, false, float>(p, stream) : launch_fused<float, false, false, bf16>(p, stream);
-        return f32 ? launch_fused<float, false, false, float>(p, stream) : launch_fused<bf16, false, false, bf16>(p, stream);
+            return f32 ? launch_fused<float, false, false, float>(p, sms, stream) : launch_fused<float, false, false, bf16>(p, sms, stream);
+        return f32 ? launch_fused<float, false, false, float>(p, sms, stream) : launch_fused<bf16, false, false, bf16>(p, sms, stream);
     }
-    if (mode == INT8_GATED) return f32 ? launch_few<float, false, true>(p, stream) : launch_few<bf16, false, true>(p, stream);
-    if (mode == INT8_ADD_F32) return launch_few<float, true, false>(p, stream);
-    return f32 || mode == INT8_STORE_F32 ? launch_few<float, false, false>(p, stream) : launch_few<bf16, false, false>(p, stream);
+    if (mode == INT8_GATED) return f32 ? launch_few<float, false, true>(p, sms, stream) : launch_few<bf16, false, true>(p, sms, stream);
+    if (mode == INT8_ADD_F32) return launch_few<float, true, false>(p, sms, stream);
+    return f32 || mode == INT8_STORE_F32 ? launch_few<float, false, false>(p, sms, stream) : launch_few<bf16, false, false>(p, sms, stream);
 }
 
 }  // namespace nnis
