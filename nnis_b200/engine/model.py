@@ -51,17 +51,19 @@ class DecoderModel:
             if value not in (None, "int8"):
                 raise ValueError(f"{what} must be None or 'int8'; got {value!r}")
         self.weights_in_int8 = weight_dtype == "int8"
-        mixers = [b.mixer for b in self.blocks if b.mixer is not None]
-        widest = max((m.kv_heads * m.head_dim for m in mixers if hasattr(m, "cache_in_int8")), default=0)
         for layer, block in enumerate(self.blocks):
             if cache_dtype == "int8" and block.mixer is not None:
                 if getattr(block.mixer, "cache_in_int8", None) is not None:
-                    block.mixer.cache_in_int8(widest)
+                    block.mixer.cache_in_int8()
                 else:
                     raise ValueError(f"cache_dtype='int8': layer {layer}'s mixer ({type(block.mixer).__name__}) has no 8-bit cache")
             for part in block.parts() if self.weights_in_int8 else ():
                 if getattr(part, "hold_int8", None) is None and any(w.role == "matrix" for w in part.weight_specs().values()):
                     raise ValueError(f"weight_dtype='int8': layer {layer}'s {type(part).__name__} has no 8-bit product")
+        # (layers decide alike which sequences of a step read the codes: by the widest)
+        alike = [b.mixer for b in self.blocks if hasattr(b.mixer, "widest_row")]
+        for mixer in alike:
+            mixer.widest_row = max(m.widest_row for m in alike)
 
     # -- weights ------------------------------------------------------------
     def weight_specs(self) -> Dict[str, WeightSpec]:

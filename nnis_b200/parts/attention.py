@@ -44,6 +44,7 @@ class Attention(Part):
         self.window = int(params.get("window", 0))
         self.own_kv = params.get("kv", "own") == "own"
         self.names = params["names"]
+        self.widest_row = self.kv_heads * self.head_dim  # the most values of a position's keys in a layer of the model
         if self.heads % self.kv_heads:
             raise ValueError(f"heads={self.heads} is not a multiple of kv_heads={self.kv_heads}")
         if self.head_dim % 2 or not 2 <= self.head_dim <= 256:
@@ -92,10 +93,9 @@ class Attention(Part):
         return sum(matrix_bytes(t) for t in (self.w_qkv, self.w_o, self.b_qkv, self.b_o))
 
     # -- cache ------------------------------------------------------------
-    def cache_in_int8(self, widest: int = 0) -> None:
-        """Keys and values are held in 8-bit codes with a scale for every position and head.  ``widest``: the most values that a position's keys
-        have in a layer of the model."""
-        self.codes, self.widest = True, max(widest, self.kv_heads * self.head_dim)
+    def cache_in_int8(self) -> None:
+        """Keys and values are held in 8-bit codes with a scale for every position and head."""
+        self.codes = True
 
     def cache_request(self) -> Optional[KVRequest]:
         return KVRequest(self.kv_heads, self.head_dim, self.window, codes=self.codes) if self.own_kv else None
@@ -145,7 +145,7 @@ class Attention(Part):
         few = [c <= ops.INT8_ROWS_AT_ONCE[self.dtype] for c in counts]
         pages = [-(-(s + c) // PAGE_SIZE) for c, s in zip(counts, starts)]
         short = sum(p for p, f in zip(pages, few) if f)
-        apart = short > sum(pages) - short and short * PAGE_SIZE * 2 * self.widest * self.dtype.itemsize > ops.INT8_READ_BACK
+        apart = short > sum(pages) - short and short * PAGE_SIZE * 2 * self.widest_row * self.dtype.itemsize > ops.INT8_READ_BACK
         return few if all(few) or apart else [False] * len(few)
 
     def _read_back_table(self, counts, starts):

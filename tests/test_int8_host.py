@@ -461,7 +461,7 @@ def test_a_step_reads_back_what_long_sequences_have(monkeypatch):
         assert name + "/codes" not in mixer.step_tables([1, many, 300], [100, 64, 1])
         monkeypatch.undo()
         # a server's step: 63 contexts of 4,000 and a prompt of 200 tokens, a layer of 32 heads of 64
-        mixer.widest = 2048
+        mixer.widest_row = 2048
         tables = mixer.step_tables([1] * 63 + [200], [4000] * 63 + [0])
         assert tables[name + "/pages"].tolist() == [4] and tables[name + "/codes"].tolist() == [[0, 63]]
 
