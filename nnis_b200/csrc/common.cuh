@@ -103,12 +103,15 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 // (NNIS_PDL=0 turns it off everywhere); defined in elementwise.cu.
 bool dependent_launches();
 
-// The current device's SMs (a B200's where it cannot be asked).
+// The current device's SMs (a B200's where it cannot be asked).  Asked once a device: the driver takes 0.1 us for it.
 inline int device_sms() {
+    static std::atomic<int> held[16];
     int device = 0, sms = 0;
-    const bool known = cudaGetDevice(&device) == cudaSuccess &&
-                       cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) == cudaSuccess && sms > 0;
-    return known ? sms : 148;
+    if (cudaGetDevice(&device) != cudaSuccess) return 148;
+    if (device < 16 && (sms = held[device].load(std::memory_order_relaxed)) > 0) return sms;
+    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || sms <= 0) return 148;
+    if (device < 16) held[device].store(sms, std::memory_order_relaxed);
+    return sms;
 }
 
 // Lets `kernel` have `bytes` of dynamic shared memory on the current device; `held` (16 zeros of the caller's, one place a device)
